@@ -578,6 +578,62 @@ int64_t odp_calibrate_mfma_flops(int32_t workgroups, int32_t iters);
 int odp_abi_version(void);
 const char* odp_last_error(void);
 
+/* ---- embedding tables ----------------------------------------------------
+ * A table W [vocab][width] (float32, bfloat16 or float16, pitch ldw elements)
+ * read at tokens y [n] (int32 or int64, token_bytes 4 or 8), and its gradient
+ * from the rows g [n][width] (pitch ldg) that come back.  Tokens outside
+ * [0, vocab) are read as rows of NaN and have no gradient; the kernels never
+ * access memory for them.  n < 2^31 - 64, width < 2^24, vocab < 2^31 - 1.
+ * The reference trains embeddings through torch's own lookup, whose
+ * per-example gradient vmap(grad) makes as a dense [examples][vocab][width]
+ * tensor (opaque-engine/.../clipping/_clipped_fun.py:756-762); the norms and
+ * the clipped sum here need no such tensor.                                 */
+
+/* out[i] = scale W[y_i], rounded once (an exact copy at scale 1). */
+int odp_embed_rows(odp_stream_t stream, int dtype, const void* tokens, int token_bytes, int64_t n,
+                   const void* weight, int64_t ldw, int64_t vocab, int64_t width, float scale, void* out);
+
+/* Positions sorted by token, stable: keys[n] ascending and rows[n] the
+ * positions.  Dropped positions (tokens outside the table, the token
+ * `padding` (-1: none), and with segments the rows outside them) get the key
+ * `vocab` and come last.  With segments row_seg[n] receives each row's index
+ * into them.  scratch: odp_token_sort_scratch() bytes.                      */
+int64_t odp_token_sort_scratch(int64_t n, int64_t vocab);
+int odp_token_sort(odp_stream_t stream, const void* tokens, int token_bytes, int64_t n, int64_t vocab,
+                   int64_t padding, const int32_t* seg_row_start, const int32_t* seg_row_len, int32_t n_seg,
+                   void* scratch, uint32_t* keys, uint32_t* rows, int32_t* row_seg);
+
+/* Bytes of the scratch of the sums below (second: with second moments), and
+ * the partial slots per row of a segment that odp_embed_sqnorm writes.      */
+int64_t odp_embed_sum_scratch(int dtype, int64_t n, int64_t width, int second);
+int64_t odp_embed_pieces(int dtype, int64_t width);
+
+/* out [vocab][width] (of g's dtype) = scale times the sum of each token's
+ * rows of g, in float32 and rounded once; zero rows for absent tokens.      */
+int odp_embed_grad(odp_stream_t stream, int dtype, const void* g, int64_t ldg, int64_t n, int64_t width,
+                   const uint32_t* keys, const uint32_t* rows, int64_t vocab, float scale, void* scratch, void* out);
+
+/* Squared-norm partials of every example's gradient of the table, the sum
+ * over tokens of |S|^2 with S = scale times the example's rows of that token
+ * (non-finite entries of S count as 0 and set *nf_flag):
+ * part[seg_example[s]][slot + (row - seg_row_start[s]) pieces + piece] for the
+ * first row of every (segment, token); the other slots are left as they are
+ * (zero them first).  whole: half of odp_embed_sum_scratch(.., 0) bytes, kept
+ * for odp_embed_clipped_sum.                                                */
+int odp_embed_sqnorm(odp_stream_t stream, int dtype, const void* g, int64_t ldg, int64_t n, int64_t width,
+                     const uint32_t* keys, const uint32_t* rows, const int32_t* row_seg, int64_t vocab, float scale,
+                     const int32_t* seg_row_start, const int32_t* seg_example, void* scratch, float* whole,
+                     double* part, int64_t part_stride, int64_t slot, int64_t* nf_flag);
+
+/* out [vocab][width] = sum over examples of scales[example] S, over
+ * normalize_by, in float32 and rounded once to out_dtype; out2 (may be null)
+ * the sum of the squares of the scaled S.  After odp_embed_sqnorm on the same
+ * inputs.                                                                   */
+int odp_embed_clipped_sum(odp_stream_t stream, int dtype, const void* g, int64_t ldg, int64_t n, int64_t width,
+                          const uint32_t* keys, const uint32_t* rows, const int32_t* row_seg, int64_t vocab,
+                          float scale, const int32_t* seg_example, void* scratch, const float* whole,
+                          const double* scales, float normalize_by, int out_dtype, void* out, void* out2);
+
 #ifdef __cplusplus
 }
 #endif

@@ -123,6 +123,24 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "odp_pack_planes_blocks": (_c_i64, [_c_i64]),
     "odp_pack_planes": (_c_int, [_ptr, _ptr, _ptr, _c_i32, _c_i32, _ptr, _ptr]),
+    "odp_embed_rows": (_c_int, [_ptr, _c_int, _ptr, _c_int, _c_i64, _ptr, _c_i64, _c_i64, _c_i64, _c_f32, _ptr]),
+    "odp_token_sort_scratch": (_c_i64, [_c_i64, _c_i64]),
+    "odp_token_sort": (
+        _c_int, [_ptr, _ptr, _c_int, _c_i64, _c_i64, _c_i64, _ptr, _ptr, _c_i32, _ptr, _ptr, _ptr, _ptr]),
+    "odp_embed_sum_scratch": (_c_i64, [_c_int, _c_i64, _c_i64, _c_int]),
+    "odp_embed_pieces": (_c_i64, [_c_int, _c_i64]),
+    "odp_embed_grad": (
+        _c_int, [_ptr, _c_int, _ptr, _c_i64, _c_i64, _c_i64, _ptr, _ptr, _c_i64, _c_f32, _ptr, _ptr]),
+    "odp_embed_sqnorm": (
+        _c_int,
+        [_ptr, _c_int, _ptr, _c_i64, _c_i64, _c_i64, _ptr, _ptr, _ptr, _c_i64, _c_f32, _ptr, _ptr, _ptr, _ptr,
+         _ptr, _c_i64, _c_i64, _ptr],
+    ),
+    "odp_embed_clipped_sum": (
+        _c_int,
+        [_ptr, _c_int, _ptr, _c_i64, _c_i64, _c_i64, _ptr, _ptr, _ptr, _c_i64, _c_f32, _ptr, _ptr, _ptr, _ptr,
+         _c_f32, _c_int, _ptr, _ptr],
+    ),
     "odp_linear_moments_blocks": (_c_i64, [_c_i64, _c_i64, _c_i32]),
     "odp_linear_moments": (
         _c_int, [_ptr, _ptr, _ptr, _c_i32, _c_i32, _ptr, _ptr, _ptr, _ptr, _c_i32, _c_i32, _c_f32, _c_i32]),

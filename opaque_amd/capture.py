@@ -42,9 +42,13 @@ class SiteRecord:
     segments: Any = None  # MoE expert: engine Segments of x's rows (x is then [rows, d_in])
     v: torch.Tensor | None = None  # LoRA: x A, kept from the forward ([B, *, r])
     u: torch.Tensor | None = None  # LoRA: g B^T, kept from the backward ([B, *, r])
+    tokens: torch.Tensor | None = None  # embedding: the tokens [B, *] (w_obj is the table)
+    padding: int = -1  # embedding: the token without a gradient
 
     @property
     def kind(self) -> str:
+        if self.tokens is not None:
+            return "embedding"
         return "linear" if self.w_obj is not None else "lora"
 
 

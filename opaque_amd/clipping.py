@@ -39,6 +39,7 @@ from opaque_amd.capture import CaptureSession, SiteRecord
 from opaque_amd.engine import (
     LORA_PTRS,
     ClipSpec,
+    EmbeddingSite,
     GhostPlan,
     LeafOut,
     LinearSite,
@@ -505,9 +506,9 @@ class _ClipEngine:
     def _finish(self, n: int, paths: list, treedef, shapes: list, dtypes: list, device,
                 sites: list[LoraSite], mats: list[MaterializedLeaf], segments: Segments,
                 normalize_by: float, out_dtype_of, values, loss_aux, all_finite,
-                lins: list[LinearSite] = ()) -> tuple:
+                lins: list[LinearSite] = (), embeds: list[EmbeddingSite] = ()) -> tuple:
         t0 = time.perf_counter()
-        capture = bool(sites) or bool(lins)
+        capture = bool(sites) or bool(lins) or bool(embeds)
         # Clip constants and output leaves depend only on the tree's shapes,
         # dtypes and paths and on the thresholds (which adaptive clipping
         # moves every step): kept from the last call when those match.
@@ -534,24 +535,26 @@ class _ClipEngine:
         if self._lora_ptrs.numel() < LORA_PTRS * len(sites):
             self._lora_ptrs = torch.empty(LORA_PTRS * len(sites), dtype=torch.int64)
         key = plan_key(segments=segments, leaves=outs, clip=spec, lora_sites=sites, materialized=mats,
-                       linear_sites=lins, device=device, leaves_key_=outs_key, lora_ptrs=self._lora_ptrs, **kw)
+                       linear_sites=lins, embedding_sites=embeds, device=device, leaves_key_=outs_key, lora_ptrs=self._lora_ptrs, **kw)
         plan = None
         if self._plan is not None and self._plan.key == key:
             plan = self._plan
-            if not plan.rebind(sites, mats, list(lins), spec, key=key, lora_ptrs=self._lora_ptrs):
+            if not plan.rebind(sites, mats, list(lins), spec, key=key, lora_ptrs=self._lora_ptrs,
+                               embedding_sites=list(embeds)):
                 plan = None
         self.last_rebound = plan is not None
         if plan is None:
             self._plan = None  # release the old plan's buffers before building
             plan = GhostPlan(segments=segments, leaves=outs, clip=spec, lora_sites=sites,
-                             materialized=mats, linear_sites=list(lins), device=device, **kw)
+                             materialized=mats, linear_sites=list(lins), embedding_sites=list(embeds),
+                             device=device, **kw)
             self._plan = plan
         self.last_prep_ms = (time.perf_counter() - t0) * 1e3
         res = plan.run()
         self.last_plan_ms = (time.perf_counter() - t0) * 1e3
         if all_finite is not None and plan.pe_views():
             all_finite = all_finite & _pe_finite(plan)
-        if all_finite is not None and lins:
+        if all_finite is not None and (lins or embeds):
             all_finite = all_finite & plan.linear_finite()
         # ||scaled gradient||: per group, scale * group norm (class 0 scale).
         cn2 = (res.scales[0].float() * res.group_norms).square().sum(0).sqrt()
@@ -685,6 +688,13 @@ class _ClipEngine:
         mats: list[MaterializedLeaf] = []
         rows_per_ex: dict[int, int] = {}
         for r in recs:
+            if r.tokens is not None:
+                w = leaves[obj_leaf[id(r.w_obj)]]
+                if r.g is None:
+                    r.g = torch.zeros(*r.tokens.shape, w.shape[1], dtype=w.dtype, device=w.device)
+                t_rows = r.tokens[0].numel()
+                rows_per_ex[t_rows] = rows_per_ex.get(t_rows, 0) + 1
+                continue
             if r.g is None:
                 d_out = r.w_obj.shape[-2] if r.w_obj is not None else r.B.shape[1]
                 r.g = torch.zeros(*r.x.shape[:-1], d_out, dtype=r.x.dtype, device=r.x.device)
@@ -694,8 +704,19 @@ class _ClipEngine:
             rows_per_ex[t_rows] = rows_per_ex.get(t_rows, 0) + 1
         seq = max(rows_per_ex, key=rows_per_ex.get) if rows_per_ex else 1
         lins: list[LinearSite] = []
+        embeds: list[EmbeddingSite] = []
         stacked: dict[int, torch.Tensor] = {}
         for r in recs:
+            if r.tokens is not None:
+                kw = obj_leaf[id(r.w_obj)]
+                # The site sums in float32: a float64 sum asked for is made from
+                # the per-example gradients.
+                if r.tokens[0].numel() == seq and r.tokens.shape[0] == n and self.compute_dtype != torch.float64:
+                    embeds.append(EmbeddingSite(tokens=r.tokens, g=r.g, w_leaf=kw, scale=r.scaling,
+                                                padding=r.padding))
+                else:
+                    mats.append(MaterializedLeaf(per_example=_table_per_example(r, leaves[kw], n), leaf=kw))
+                continue
             if r.w_obj is not None and r.segments is not None:
                 kw = obj_leaf[id(r.w_obj)]
                 if (r.x.dtype == r.g.dtype == leaves[kw].dtype == torch.bfloat16
@@ -747,7 +768,7 @@ class _ClipEngine:
         dtypes = [t.dtype for t in leaves]
         seg = Segments.padded(n, seq)
         return self._finish(n, paths, treedef, shapes, dtypes, device, sites, mats, seg,
-                            normalize_by, out_dtype_of, values.detach(), loss_aux, all_finite, lins)
+                            normalize_by, out_dtype_of, values.detach(), loss_aux, all_finite, lins, embeds)
 
     # -- the call ----------------------------------------------------------------
     def __call__(self, args: tuple, kwargs: dict) -> Any:
@@ -868,6 +889,14 @@ def _pe_finite(plan: GhostPlan) -> torch.Tensor:
     for view in plan.pe_views():
         ok = ok & torch.isfinite(view).all()
     return ok
+
+
+def _table_per_example(r: SiteRecord, leaf: torch.Tensor, n: int) -> torch.Tensor:
+    """Per-example gradients [n, vocabulary * width] of an embedding table from its captured tokens and g."""
+    from opaque_amd.vocabulary import table_gradient  # the seam's module imports the engine
+
+    return torch.stack([table_gradient(r.tokens[i], r.g[i], leaf.shape[0], r.scaling, r.padding).reshape(-1)
+                        for i in range(n)])
 
 
 def _site_per_example(r: SiteRecord, ka: int | None, kb: int | None,

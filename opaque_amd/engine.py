@@ -268,6 +268,25 @@ class LinearSite:
     index: int | None = None  # slice of a stacked [E, d_out, d_in] leaf (an MoE expert); None: the whole leaf
 
 
+@dataclass
+class EmbeddingSite:
+    """A token table's lookup ``scale * W[tokens]`` over the batch rows.
+
+    ``tokens`` holds one int64 or int32 token per row, ``g`` the output
+    gradients [rows, width] (float32, bfloat16 or float16); ``w_leaf``
+    indexes the plan's leaf list, shaped [vocabulary, width].  ``padding`` is
+    the token whose row gets no gradient (-1: none); tokens outside the table
+    and rows outside the segments get none either.
+    """
+
+    tokens: torch.Tensor
+    g: torch.Tensor
+    w_leaf: int
+    scale: float = 1.0
+    padding: int = -1
+    segments: Segments | None = None  # rows of tokens / g; None: the plan's segments
+
+
 # Time per flop of the Gram-form norm kernel that choose_form assumes,
 # relative to the outer form: the rates on MI355X when the line was drawn were
 # 746 and 1264 TFLOP/s.  The outer kernel without the store has since reached
@@ -504,7 +523,7 @@ _PLAN_OPTIONS = {"second_moment": False, "fuse_g_side": True, "stream_factors": 
 
 
 def plan_key(*, segments: Segments, leaves: list[LeafOut], clip: ClipSpec, lora_sites=(), materialized=(),
-             linear_sites=(), device=None, leaves_key_: tuple | None = None, lora_ptrs: torch.Tensor | None = None,
+             linear_sites=(), embedding_sites=(), device=None, leaves_key_: tuple | None = None, lora_ptrs: torch.Tensor | None = None,
              **options) -> tuple:
     """What fixes a GhostPlan's tables: a plan built from inputs with this key
     can be rebound (GhostPlan.rebind) to other inputs with the same key.
@@ -545,6 +564,8 @@ def plan_key(*, segments: Segments, leaves: list[LeafOut], clip: ClipSpec, lora_
     mats = tuple((_tensor_key(m.per_example), m.leaf, _seg_key(m.segments)) for m in materialized)
     lins = tuple((shared(ls.x), _tensor_key(ls.g), ls.w_leaf, ls.form, ls.index,
                   _seg_key(ls.segments)) for ls in linear_sites)
+    embeds = tuple((tuple(es.tokens.shape), es.tokens.dtype, _tensor_key(es.g), es.w_leaf, float(es.scale),
+                    int(es.padding), _seg_key(es.segments)) for es in embedding_sites)
     outs = leaves_key(leaves) if leaves_key_ is None else leaves_key_
     clip_s = (clip.mode, len(clip.thresholds), tuple(g[2] for g in clip.guards))
     unknown = set(options) - set(_PLAN_OPTIONS)
@@ -554,7 +575,7 @@ def plan_key(*, segments: Segments, leaves: list[LeafOut], clip: ClipSpec, lora_
     dev = torch.device(device) if device is not None else None
     if dev is not None and dev.type == "cuda" and dev.index is None:
         dev = torch.device("cuda", torch.cuda.current_device())
-    return (str(dev), _seg_key(segments), outs, clip_s, tuple(xkeys), lora, mats, lins, opts)
+    return (str(dev), _seg_key(segments), outs, clip_s, tuple(xkeys), lora, mats, lins, embeds, opts)
 
 
 # ---------------------------------------------------------------------------
@@ -578,6 +599,64 @@ STREAM_MIN_ROUNDS = 1
 # moved by more than runs differ (two layers at 4 x 4096: 778-793 us), except
 # one layer at 4 x 300 tokens (47.5 us up to 4 steps, 51 from 10).
 STREAM_MIN_STEPS = 10
+
+class _EmbeddingWork:
+    """Buffers and launches of one embedding site of a plan."""
+
+    def __init__(self, es: EmbeddingSite, view: _SegView, leaf: LeafOut, slot: int, second: bool) -> None:
+        self.view, self.leaf, self.slot, self.site = view, leaf, slot, es
+        self.vocab, self.width = leaf.shape
+        self.n, dev = es.tokens.numel(), es.g.device
+        self.dt = dtype_code(es.g.dtype)
+        self._take(es)
+        lib = N.load()
+        sums = int(lib.odp_embed_sum_scratch(self.dt, self.n, self.width, int(second)))
+        self.scratch = torch.empty(max(sums, int(lib.odp_token_sort_scratch(self.n, self.vocab)), 4) // 4,
+                                   dtype=torch.float32, device=dev)
+        # Sums of the runs that cross windows, kept from the norms for the clipped sum.
+        self.whole = torch.empty(max(int(lib.odp_embed_sum_scratch(self.dt, self.n, self.width, 0)) // 8, 1),
+                                 dtype=torch.float32, device=dev)
+        self.ids = torch.empty((3, max(self.n, 1)), dtype=torch.int32, device=dev)  # sorted tokens, rows; segments
+
+    def _take(self, es: EmbeddingSite) -> None:
+        self.site = es
+        self.tokens = es.tokens.detach().reshape(-1).contiguous()
+        g = es.g.detach().reshape(-1, self.width)
+        if (g.stride(1) != 1 and self.width > 1) or g.stride(0) < self.width:
+            g = g.clone(memory_format=torch.contiguous_format)
+        self.g = g
+
+    def rebind(self, es: EmbeddingSite, trusted: bool) -> bool:
+        old = self.site
+        if not trusted and (es.tokens.shape != old.tokens.shape or es.tokens.dtype != old.tokens.dtype
+                            or es.g.shape != old.g.shape or es.g.dtype != old.g.dtype or es.g.device != old.g.device
+                            or (es.w_leaf, es.scale, es.padding) != (old.w_leaf, old.scale, old.padding)):
+            return False
+        self._take(es)
+        return True
+
+    def _seg(self, t: torch.Tensor) -> int:
+        return t.data_ptr() + 4 * self.view.first
+
+    def norms(self, plan: GhostPlan, stream: int) -> None:
+        keys, rows, row_seg = (self.ids[k].data_ptr() for k in range(3))
+        N.call("odp_token_sort", stream, self.tokens.data_ptr(), self.tokens.element_size(), self.n, self.vocab,
+               int(self.site.padding), self._seg(plan.seg_start), self._seg(plan.seg_len), self.view.n_seg,
+               self.scratch.data_ptr(), keys, rows, row_seg)
+        N.call("odp_embed_sqnorm", stream, self.dt, self.g.data_ptr(), self.g.stride(0), self.n, self.width, keys,
+               rows, row_seg, self.vocab, float(self.site.scale), self._seg(plan.seg_start), self._seg(plan.seg_ex),
+               self.scratch.data_ptr(), self.whole.data_ptr(), plan.part.data_ptr(), plan.n_slots, self.slot,
+               plan._nf_flag_addr)
+
+    def clipped_sum(self, plan: GhostPlan, stream: int) -> None:
+        keys, rows, row_seg = (self.ids[k].data_ptr() for k in range(3))
+        i = self.site.w_leaf
+        out2 = plan.out2[i].data_ptr() if plan.out2 is not None else None
+        N.call("odp_embed_clipped_sum", stream, self.dt, self.g.data_ptr(), self.g.stride(0), self.n, self.width,
+               keys, rows, row_seg, self.vocab, float(self.site.scale), self._seg(plan.seg_ex),
+               self.scratch.data_ptr(), self.whole.data_ptr(), plan.scales[self.leaf.cls][self.leaf.group].data_ptr(),
+               float(plan.clip.normalize_by), dtype_code(self.leaf.out_dtype), plan.out[i].data_ptr(), out2)
+
 
 # Stages launched after the clip factors, in table order.
 _AFTER_CLIP = ("scale_sum", "lin_prescale", "lin_sum", "lin_moments")
@@ -618,6 +697,7 @@ class GhostPlan:
         lora_sites: list[LoraSite] = (),
         materialized: list[MaterializedLeaf] = (),
         linear_sites: list[LinearSite] = (),
+        embedding_sites: list[EmbeddingSite] = (),
         device: torch.device | str = "cuda",
         second_moment: bool = False,
         fuse_g_side: bool = True,
@@ -658,20 +738,23 @@ class GhostPlan:
         # The structure this plan was built for: rebind(key=...) with an equal
         # key skips re-deriving the input layout.
         self.key = plan_key(segments=segments, leaves=leaves, clip=clip, lora_sites=lora_sites,
-                            materialized=materialized, linear_sites=linear_sites, device=dev,
-                            second_moment=second_moment, fuse_g_side=fuse_g_side, stream_factors=stream_factors,
+                            materialized=materialized, linear_sites=linear_sites,
+                            embedding_sites=embedding_sites, device=dev, second_moment=second_moment, fuse_g_side=fuse_g_side, stream_factors=stream_factors,
                             prescale_bytes=prescale_bytes,
                             linear_pe_bytes=linear_pe_bytes, square_f64=square_f64, sum_f64=sum_f64,
                             raw_values=raw_values)
-        self._build(list(lora_sites), list(materialized), list(linear_sites))
+        self._build(list(lora_sites), list(materialized), list(linear_sites), list(embedding_sites))
         self.build_ms = (time.perf_counter() - t_build) * 1e3  # host time of the construction
 
     # -- construction --------------------------------------------------------
-    def _build(self, sites: list[LoraSite], mats: list[MaterializedLeaf], lins: list[LinearSite]) -> None:
+    def _build(self, sites: list[LoraSite], mats: list[MaterializedLeaf], lins: list[LinearSite],
+               embeds: list[EmbeddingSite]) -> None:
         seg = self.segments
         dev = self.device
         reg = _SegRegistry(seg)
         self._segreg = reg
+        for es in embeds:
+            self._check_embedding(es, reg.view(es.segments))
         for ls in lins:
             if ls.x.device != dev or ls.g.device != dev:
                 raise ValueError("linear site tensors must be on the plan device")
@@ -884,6 +967,11 @@ class GhostPlan:
         for k, taken in slices.items():
             if -1 not in taken and taken != set(range(self.leaves[k].shape[0])):
                 raise ValueError(f"stacked leaf {k} needs a linear site for every slice")
+        for es in embeds:
+            if es.w_leaf in leaf_slots:
+                raise ValueError(f"leaf {es.w_leaf} has more than one producer")
+            leaf_slots[es.w_leaf] = max(1, reg.view(es.segments).max_len * int(
+                lib.odp_embed_pieces(dtype_code(es.g.dtype), es.g.shape[-1])))
         if set(leaf_slots) != set(range(len(self.leaves))):
             missing = sorted(set(range(len(self.leaves))) - set(leaf_slots))
             raise ValueError(f"every output leaf needs exactly one producer; missing {missing}")
@@ -923,6 +1011,8 @@ class GhostPlan:
         self._nf_flag_addr = self._part_buf.data_ptr() + seg.n_ex * self.n_slots * 8
 
         ext.update(self._alloc_outputs())
+        self._embeds = [_EmbeddingWork(es, reg.view(es.segments), self.leaves[es.w_leaf], slot_base[es.w_leaf],
+                                       self.second_moment) for es in embeds]
 
         # Q planes (U and V) for every chunk, carved from one allocation per dtype.
         q_need: dict[torch.dtype, int] = {}
@@ -1270,7 +1360,7 @@ class GhostPlan:
                      2 * valid * d_in * d_out,
                      io=(0 if site_chunk[i] is not None else valid * (d_in + d_out) * 2)
                      + d_in * d_out * out.element_size())
-        lin_leaves = {ls.w_leaf for ls in lins}
+        lin_leaves = {ls.w_leaf for ls in lins} | {es.w_leaf for es in embeds}
 
         ss = _Table(N.SS_FIELDS)
         for i, off in lin_pe.items():
@@ -1417,7 +1507,7 @@ class GhostPlan:
 
     def rebind(self, lora_sites: list[LoraSite] = (), materialized: list[MaterializedLeaf] = (),
                linear_sites: list[LinearSite] = (), clip: ClipSpec | None = None, key: tuple | None = None,
-               lora_ptrs: torch.Tensor | None = None) -> bool:
+               lora_ptrs: torch.Tensor | None = None, embedding_sites: list[EmbeddingSite] = ()) -> bool:
         """Points the plan at a new call's inputs with the same structure and
         gives it fresh outputs; scratch buffers and tables are reused.
 
@@ -1440,6 +1530,9 @@ class GhostPlan:
                                  or len(clip.guards) != len(self.clip.guards)):
             return False
         trusted = key is not None and key == self.key
+        if len(embedding_sites) != len(self._embeds) or not all(
+                w.rebind(es, trusted) for w, es in zip(self._embeds, embedding_sites)):
+            return False
         fast = self._fast if trusted and lora_ptrs is not None else None
         chunks = []
         if fast is None:
@@ -1886,10 +1979,23 @@ class GhostPlan:
                 return s.b_transposed
         return False
 
+    def _check_embedding(self, es: EmbeddingSite, view: _SegView) -> None:
+        if es.tokens.device != self.device or es.g.device != self.device:
+            raise ValueError("embedding site tensors must be on the plan device")
+        if es.tokens.dtype not in (torch.int64, torch.int32):
+            raise TypeError("embedding site tokens must be int64 or int32")
+        if es.g.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            raise TypeError("embedding site gradients must be float32, bfloat16 or float16")
+        shape = tuple(self.leaves[es.w_leaf].shape)
+        if len(shape) != 2 or 0 in shape or es.g.shape[-1] != shape[1]:
+            raise ValueError("an embedding site's leaf must be shaped [vocabulary, width]")
+        if es.tokens.numel() != view.n_rows or es.g.numel() != view.n_rows * shape[1]:
+            raise ValueError("embedding site row count does not match the segments")
+
     def linear_finite(self) -> torch.Tensor:
-        """Device bool: no per-example weight gradient of a linear site held a
-        non-finite entry in the last run (outer-form norms flag them; the
-        other sites' column masks record them)."""
+        """Device bool: no per-example weight gradient of a linear or embedding
+        site held a non-finite entry in the last run (outer-form and embedding
+        norms flag them; the other sites' column masks record them)."""
         ok = self._part_buf[-1:].view(torch.int64)[0] == 0
         if self._has_masks:
             ok = ok & (self.nf_mask == 0).all()
@@ -1930,7 +2036,7 @@ class GhostPlan:
         """Launch the step on the current stream.
 
         ``events`` may map a stage name ("pack", "planes", "project", "factor_project", "factor_stream",
-        "factor", "sqnorm", "nonfinite", "lin_norm", "clip", "scale_sum", "lin_sum") to a
+        "factor", "sqnorm", "nonfinite", "lin_norm", "embed_norm", "clip", "scale_sum", "lin_sum", "embed_sum") to a
         (start, end) pair of torch.cuda.Event that are recorded around that
         stage's launches ("lin_sum" spans the clipped sums of full weights:
         their prescale, GEMM and moments launches).  ``launch_log``, when a
@@ -2005,6 +2111,12 @@ class GhostPlan:
                 end_ev.record(main)
             if name in ev and (name == "factor_stream" or name not in names[idx + 1:]):
                 ev[name][1].record(main)
+        if "embed_norm" in ev:
+            ev["embed_norm"][0].record()
+        for work in self._embeds:
+            work.norms(self, stream)
+        if "embed_norm" in ev:
+            ev["embed_norm"][1].record()
         if "clip" in ev:
             ev["clip"][0].record()
         N.check(
@@ -2051,6 +2163,12 @@ class GhostPlan:
                 end_ev.record()
             if st in ev and st not in stage[idx + 1:]:
                 ev[st][1].record()
+        if "embed_sum" in ev:
+            ev["embed_sum"][0].record()
+        for work in self._embeds:
+            work.clipped_sum(self, stream)
+        if "embed_sum" in ev:
+            ev["embed_sum"][1].record()
         return GhostResult(
             leaves=self.out,
             norms=self.norms,
@@ -2066,6 +2184,7 @@ class GhostPlan:
 __all__ = [
     "plan_key",
     "ClipSpec",
+    "EmbeddingSite",
     "GhostPlan",
     "GhostResult",
     "LeafOut",
