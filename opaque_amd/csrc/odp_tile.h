@@ -1,0 +1,300 @@
+// C = A B^T over LDS-staged MFMA tiles, for operands in either order of the
+// contraction: the products of the vocabulary loss.
+//
+// Included inside an anonymous namespace, after odp_internal.h.  A workgroup
+// owns an ET x ET tile of C (256 x 256 in bfloat16, 128 x 128 in float32):
+// rows o from A, columns n from B.  An operand is K-contiguous (KC: element
+// (row, k) at row * ld + k, as the rows of activations or of a weight) or
+// K-major (element (row, k) at k * ld + row: the contraction runs over the
+// rows of memory).  A step covers 64 bytes of k; both orders then stage the
+// same bytes, 64-byte rows of k or 512-byte rows of o or n, by buffer loads
+// straight into a ring of four LDS stages, three steps ahead of the MFMAs.
+#pragma once
+
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef u32x4_t u32x4_alias_t __attribute__((may_alias));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef u32x2_t u32x2_alias_t __attribute__((may_alias));
+typedef short v4i16_t __attribute__((ext_vector_type(4)));
+
+#define ODP_LDS __attribute__((address_space(3)))
+#define ODP_CONST __attribute__((address_space(4)))
+
+constexpr uint32_t T_RSRC = 0x00020000;  // raw buffer resource, 32-bit offsets
+constexpr uint32_t T_OOB = 0x80000000u;  // an offset past every buffer's end: reads as zero
+constexpr int T_RING = 4;
+
+template <int DT>
+struct Tile {
+  static constexpr bool F32 = DT == ODP_DTYPE_F32;
+  static constexpr int ES = F32 ? 4 : 2;          // bytes per element
+  static constexpr int ET = 512 / ES;             // rows (o) and columns (n) of the tile
+  static constexpr int EK = 64 / ES;              // k per step
+  static constexpr int WAVES = F32 ? 4 : 8;       // 2 x (WAVES / 2) over the tile
+  static constexpr int THREADS = 64 * WAVES;
+  static constexpr int WM = ET / 2, WN = 64;      // a wave's block
+  static constexpr int BI = WM / 16, BJ = WN / 16;
+  static constexpr int HALF = 512 * EK;           // bytes of one operand's stage
+  static constexpr int STAGE = 2 * HALF;
+  static constexpr int DMA = HALF / 1024 / WAVES;  // 1 KB loads per wave, operand and step
+  typedef f32x4_t Acc[BI][BJ];
+};
+
+// Stage k of the ring: separate arrays, so that reads of one are not made to
+// wait for the loads into another.
+template <int BYTES, int K>
+__device__ __forceinline__ char* t_array() {
+  __shared__ __attribute__((aligned(16))) char s[BYTES];
+  return s;
+}
+template <int DT>
+__device__ __forceinline__ char* t_stage(int k) {
+  constexpr int B = Tile<DT>::STAGE;
+  return k == 0 ? t_array<B, 0>() : k == 1 ? t_array<B, 1>() : k == 2 ? t_array<B, 2>() : t_array<B, 3>();
+}
+
+// Swizzles.  64-byte rows of k: 16-byte slot s of row r lies at slot
+// s ^ ((r >> 1) & 3) (full rate for operand reads, measured on the Gram
+// kernels).  512-byte rows of 16-bit columns: 8-byte chunks XOR-ed as the
+// transposing reads of the full-weight kernels take them; of 32-bit columns:
+// 64-byte groups XOR-ed with the row's quarter, so that the four rows a lane
+// group reads lie on different banks.
+__device__ __forceinline__ int t_kswz(int row) { return (row >> 1) & 3; }
+template <int DT>
+__device__ __forceinline__ int t_cswz(int row) {  // in 16-byte pieces
+  return DT == ODP_DTYPE_F32 ? ((row >> 2) & 3) << 2 : ((row & 3) | ((row >> 1) & 4)) << 1;
+}
+
+// The MFMA operand of 16 rows from row0 of a staged operand: lane & 15 = row,
+// 16 bytes of k per lane (the slot lane >> 4).
+template <int DT, bool KC>
+__device__ __forceinline__ u32x4_t t_frag(const char* half, int row0) {
+  const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+  if constexpr (KC) {
+    const int row = row0 + c;
+    return *(const u32x4_alias_t*)(half + row * 64 + 16 * (q ^ t_kswz(row)));
+  } else if constexpr (DT == ODP_DTYPE_F32) {
+    u32x4_t v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int k = 4 * q + e;
+      v[e] = *(const uint32_t*)(half + k * 512 + 16 * (((row0 + c) >> 2) ^ t_cswz<DT>(k)) + 4 * (c & 3));
+    }
+    return v;
+  } else {
+    // Rows k and k + 4 share the swizzle; each read transposes a 4 x 16 block.
+    const int k = 8 * q + (c >> 2);
+    const int chunk = ((row0 >> 2) + (c & 3)) ^ (t_cswz<DT>(k) << 1);
+    const char* src = half + k * 512 + 8 * chunk;
+    const v4i16_t t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ODP_LDS v4i16_t*)(ODP_LDS void*)src);
+    const v4i16_t t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ODP_LDS v4i16_t*)(ODP_LDS void*)(src + 4 * 512));
+    const v4i16_t tt[2] = {t0, t1};
+    return __builtin_bit_cast(u32x4_t, tt);
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ f32x4_t t_mfma(u32x4_t b, u32x4_t a, f32x4_t c) {
+  if constexpr (DT == ODP_DTYPE_F32) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(b[e]), __uint_as_float(a[e]), c, 0, 0, 0);
+    return c;
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, b), __builtin_bit_cast(bf16x8_t, a),
+                                                   c, 0, 0, 0);
+  }
+}
+
+__device__ __forceinline__ uint32_t t_uniform(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+}
+__device__ __forceinline__ uint64_t t_uniform64(uint64_t v) {
+  return ((uint64_t)t_uniform((uint32_t)(v >> 32)) << 32) | t_uniform((uint32_t)v);
+}
+
+// One operand of a tile: `base` is element (row 0 of the matrix, k = 0),
+// `row0` the tile's first row, `rows` the matrix's.  ld * element size < 2^22
+// (host checks), rows of a tile stay within 32-bit offsets.
+struct Operand {
+  const void* base;
+  int64_t ld;
+  int64_t row0;
+  int64_t rows;
+};
+
+// What a lane needs to issue its loads of one operand.
+template <int DT, bool KC>
+struct Loader {
+  using T = Tile<DT>;
+  uint64_t at;       // base of the step's loads
+  uint32_t step;     // bytes the base moves per step
+  uint32_t ldb;      // bytes per row of memory
+  uint32_t off[T::DMA];
+  int32_t k8[T::DMA];  // KC: first k of the load's 16 bytes
+
+  __device__ __forceinline__ void init(const Operand& op, int wave) {
+    const int lane = threadIdx.x & 63;
+    ldb = t_uniform((uint32_t)(op.ld * T::ES));
+    if constexpr (KC) {
+      at = t_uniform64((uint64_t)op.base + (uint64_t)op.row0 * ldb);
+      step = 64;
+#pragma unroll
+      for (int i = 0; i < T::DMA; ++i) {
+        const int row = 16 * (T::DMA * wave + i) + (lane >> 2), slot = (lane & 3) ^ t_kswz(row);
+        off[i] = op.row0 + row < op.rows ? (uint32_t)row * ldb + 16u * slot : T_OOB;
+        k8[i] = slot * (16 / T::ES);
+      }
+    } else {
+      at = t_uniform64((uint64_t)op.base + (uint64_t)op.row0 * T::ES);
+      step = t_uniform(ldb * T::EK);
+#pragma unroll
+      for (int i = 0; i < T::DMA; ++i) {
+        const int k = 2 * (T::DMA * wave + i) + (lane >> 5);
+        const int piece = (lane & 31) ^ t_cswz<DT>(k), col = piece * (16 / T::ES);
+        off[i] = op.row0 + col < op.rows ? (uint32_t)k * ldb + 16u * piece : T_OOB;
+        k8[i] = 0;
+      }
+    }
+  }
+
+  // Load i of the step whose first k is k0 of kn (k0 >= kn: zeros).
+  __device__ __forceinline__ void issue(char* half, int wave, int i, int32_t k0, int32_t kn) const {
+    uint32_t o = off[i], bytes;
+    if constexpr (KC) {
+      bytes = 0x7fffffffu;
+      if (k8[i] + k0 >= kn) o = T_OOB;
+    } else {
+      const int32_t left = kn - k0;
+      bytes = left <= 0 ? 0u : (uint32_t)(left < T::EK ? left : T::EK) * ldb;
+    }
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)at, (short)0, (int)bytes, T_RSRC);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (ODP_LDS void*)(half + 1024 * (T::DMA * wave + i)), 16, o, 0, 0, 0);
+  }
+};
+
+// The operands a step starts with, read during the step before it.
+template <int DT>
+struct Head {
+  u32x4_t b[Tile<DT>::BJ], a[2];
+};
+
+template <int DT, bool AKC, bool BKC>
+__device__ __forceinline__ void t_head(const char* st, Head<DT>& h) {
+  using T = Tile<DT>;
+  const int wave = threadIdx.x >> 6, wm = T::WM * (wave & 1), wn = T::WN * (wave >> 1);
+#pragma unroll
+  for (int j = 0; j < T::BJ; ++j) h.b[j] = t_frag<DT, BKC>(st + T::HALF, wn + 16 * j);
+  h.a[0] = t_frag<DT, AKC>(st, wm);
+  h.a[1] = t_frag<DT, AKC>(st, wm + 16);
+}
+
+// One step: its MFMAs from `cur` and the operands in h, the loads of a later
+// step into `nxt` between the first of them, the next step's first operands
+// from `ahead` beside the last.  The stages are restrict parameters so that
+// the reads do not wait for the loads into `nxt`.
+template <int DT, bool AKC, bool BKC, typename Issue>
+__device__ __forceinline__ void t_step(char* __restrict__ nxt, const char* __restrict__ cur,
+                                       const char* __restrict__ ahead, Issue issue, Head<DT>& h, Head<DT>& n,
+                                       typename Tile<DT>::Acc& acc) {
+  using T = Tile<DT>;
+  const int wave = threadIdx.x >> 6, wm = T::WM * (wave & 1), wn = T::WN * (wave >> 1);
+  u32x4_t a[3] = {h.a[0], h.a[1], h.a[1]};
+#pragma unroll
+  for (int i = 0; i < T::BI; ++i) {
+    if (i + 2 < T::BI) a[(i + 2) % 3] = t_frag<DT, AKC>(cur, wm + 16 * (i + 2));
+    // 2 * DMA loads over the first block rows (one a row where there are enough).
+    constexpr int PER = (2 * T::DMA + T::BI - 1) / T::BI;
+#pragma unroll
+    for (int l = PER * i; l < PER * (i + 1) && l < 2 * T::DMA; ++l) issue(nxt, l);
+    constexpr int B0 = T::BI - 1 - T::BJ < 0 ? 0 : T::BI - 1 - T::BJ;  // block row from which b is read ahead
+    if constexpr (B0 + T::BJ < T::BI) {
+      if (i >= B0 && i < B0 + T::BJ) n.b[i - B0] = t_frag<DT, BKC>(ahead + T::HALF, wn + 16 * (i - B0));
+    } else {
+      n.b[i] = t_frag<DT, BKC>(ahead + T::HALF, wn + 16 * i);
+    }
+    if (i >= T::BI - 2) n.a[i - (T::BI - 2)] = t_frag<DT, AKC>(ahead, wm + 16 * (i - (T::BI - 2)));
+#pragma unroll
+    for (int j = 0; j < T::BJ; ++j) acc[i][j] = t_mfma<DT>(h.b[j], a[i % 3], acc[i][j]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// acc += A B^T over k in [0, kn).
+template <int DT, bool AKC, bool BKC>
+__device__ __forceinline__ void t_product(const Operand& A, const Operand& B, int32_t kn,
+                                          typename Tile<DT>::Acc& acc) {
+  using T = Tile<DT>;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  kn = (int32_t)t_uniform((uint32_t)kn);
+  Loader<DT, AKC> la;
+  Loader<DT, BKC> lb;
+  la.init(A, wave);
+  lb.init(B, wave);
+  int32_t kl = 0;  // first k of the next step to load
+  auto issue = [&](char* st, int l) __attribute__((always_inline)) {
+    if (l < T::DMA) la.issue(st, wave, l, kl, kn);
+    else lb.issue(st + T::HALF, wave, l - T::DMA, kl, kn);
+  };
+  auto advance = [&]() __attribute__((always_inline)) {
+    kl += T::EK;
+    la.at += la.step;
+    lb.at += lb.step;
+  };
+#pragma unroll
+  for (int q = 0; q < T_RING - 1; ++q) {
+#pragma unroll
+    for (int l = 0; l < 2 * T::DMA; ++l) issue(t_stage<DT>(q), l);
+    advance();
+  }
+#pragma unroll
+  for (int i = 0; i < T::BI; ++i)
+#pragma unroll
+    for (int j = 0; j < T::BJ; ++j) __asm__ volatile("" : "+v"(acc[i][j]));
+  Head<DT> h[2];
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm((T_RING - 2) * 2 * T::DMA));
+  __asm__ volatile("s_barrier" ::: "memory");
+  t_head<DT, AKC, BKC>(t_stage<DT>(0), h[0]);
+  int32_t k = 0;
+  while (k < kn) {
+#pragma unroll
+    for (int u = 0; u < T_RING; ++u) {
+      if (k >= kn) break;
+      // The next step's loads have landed (this wave's; the barrier says so
+      // for the others); those of the step after may fly.
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm((T_RING - 3) * 2 * T::DMA));
+      __asm__ volatile("s_barrier" ::: "memory");
+      t_step<DT, AKC, BKC>(t_stage<DT>((u + T_RING - 1) % T_RING), t_stage<DT>(u % T_RING),
+                           t_stage<DT>((u + 1) % T_RING), issue, h[u & 1], h[(u + 1) & 1], acc);
+      advance();
+      k += T::EK;
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(0);  // no load into LDS may outlive the workgroup
+  __asm__ volatile("s_barrier" ::: "memory");
+}
+
+// Entry e of block (i, j) of the wave's accumulators is row o = 16 i +
+// (lane & 15) and column n = 16 j + 4 (lane >> 4) + e of the wave's block.
+__device__ __forceinline__ int t_row(int i) { return 16 * i + (int)(threadIdx.x & 15); }
+__device__ __forceinline__ int t_col(int j) { return 16 * j + 4 * (int)((threadIdx.x & 63) >> 4); }
+
+template <int V>
+struct Idx {
+  static constexpr int value = V;
+};
+template <int N, int K = 0, typename F>
+__device__ __forceinline__ void static_for(F&& f) {
+  if constexpr (K < N) {
+    f(Idx<K>{});
+    static_for<N, K + 1>(f);
+  }
+}
+
+template <int I, int J>
+__device__ __forceinline__ void t_zero(f32x4_t (&acc)[I][J]) {
+#pragma unroll
+  for (int i = 0; i < I; ++i)
+#pragma unroll
+    for (int j = 0; j < J; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+}

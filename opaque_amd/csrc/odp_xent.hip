@@ -1,0 +1,655 @@
+// Softmax cross entropy of x W^T over a large vocabulary, without the logits.
+//
+//   u = x W^T,  z = u or c tanh(u / c)
+//   lse_t = log sum_v exp z_tv,  loss_t = lse_t - z_t,y(t)
+//   d_tv = g_t (exp(z_tv - lse_t) - [v = y(t)]) (1 - (z_tv / c)^2)
+//   dx = d W,  dW = d^T x
+//
+// The tokens that bear a loss are first gathered (k_xent_pick, k_xent_pack),
+// so that prompts and padding cost nothing in the products.  The forward's
+// tiles of logits never leave the registers: each leaves its rows' maximum
+// and sum of exponentials (k_xent_stats), which k_xent_losses joins.  The
+// backward forms the logits again, a piece of the vocabulary at a time, as d
+// in the inputs' type (k_xent_dlogits), and multiplies each piece by W
+// (k_xent_dx) and by x (k_xent_dw).  Sums, statistics and losses are
+// float32; d is rounded to the inputs' type because the matrix cores take it
+// so (a relative 2^-8 of an entry at most in bfloat16, of the order of the
+// rounding of the gradients themselves).
+#include "odp_internal.h"
+
+namespace {
+
+#include "odp_tile.h"
+
+constexpr float LOG2E = 1.44269504088896340736f;
+
+// The tile of a workgroup, from `tiles` = tm x tn tiles of which only those
+// of the live tokens are walked: XCD j (blockIdx % 8) takes the j-th eighth,
+// in groups of 8 tile rows walked column by column, so that the tiles one L2
+// serves at a time share operands.  False for the workgroups past the end.
+__device__ __forceinline__ bool tile_of(int bid, int tm, int tn, int& ti, int& tj) {
+  const int tiles = tm * tn, nblk = (tiles + 7) / 8;
+  if (bid >= 8 * nblk) return false;
+  const int p = (bid & 7) * nblk + (bid >> 3);
+  if (p >= tiles) return false;
+  const int per = 8 * tn, g = p / per, gm = min(tm - 8 * g, 8), r = p - g * per;
+  ti = 8 * g + r % gm;
+  tj = r / gm;
+  return true;
+}
+
+__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
+
+// c tanh(u / c) as c (1 - 2 / (1 + exp(2 u / c))): within 2^-22 c.
+__device__ __forceinline__ float softcapped(float u, float cap, float inv_cap2) {
+  const float e = fast_exp(u * inv_cap2);  // inf and 0 give cap and -cap
+  return cap - 2.0f * cap * __builtin_amdgcn_rcpf(1.0f + e);
+}
+
+// ---------------------------------------------------------------------------
+// Rows that bear a loss.
+// ---------------------------------------------------------------------------
+
+// where[i] = the place of row i among the packed rows, -1 for a row without a
+// loss, -2 for one whose target lies outside the vocabulary (loss NaN).
+// keep: every row is packed, with target -1 where it bears no loss.
+__global__ __launch_bounds__(1024) void k_xent_pick(const void* __restrict__ target, int wide, int64_t n,
+                                                    int64_t vocab, int64_t ignore, int keep, int32_t* __restrict__ act,
+                                                    int32_t* __restrict__ tgt, int32_t* __restrict__ where,
+                                                    int32_t* __restrict__ count, float* __restrict__ losses,
+                                                    float* __restrict__ lse) {
+  __shared__ int32_t sums[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int32_t base = 0;
+  for (int64_t i0 = 0; i0 < n; i0 += 1024) {
+    const int64_t i = i0 + threadIdx.x;
+    int64_t t = -1;
+    bool live = false;
+    if (i < n) {
+      t = wide ? ((const int64_t*)target)[i] : (int64_t)((const int32_t*)target)[i];
+      live = t != ignore && t >= 0 && t < vocab;
+      if (!live) {
+        if (losses != nullptr) losses[i] = t == ignore ? 0.f : __uint_as_float(0x7fc00000u);
+        if (lse != nullptr) lse[i] = 0.f;
+      }
+    }
+    const bool taken = keep ? i < n : live;
+    const uint64_t m = __builtin_amdgcn_ballot_w64(taken);
+    __syncthreads();
+    if (lane == 0) sums[wave] = __popcll(m);
+    __syncthreads();
+    int32_t before = base, all = 0;
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) before += sums[w];
+      all += sums[w];
+    }
+    const int32_t k = before + __popcll(m & ((1ull << lane) - 1));
+    if (taken) {
+      act[k] = (int32_t)i;
+      tgt[k] = live ? (int32_t)t : -1;
+    }
+    if (i < n) where[i] = live ? k : t == ignore ? -1 : -2;
+    base += all;
+  }
+  if (threadIdx.x == 0) *count = base;
+}
+
+// Packed rows xc [count][width] from x's rows `act`, columns past `cols` zero.
+template <int DT>
+__global__ __launch_bounds__(256) void k_xent_pack(const char* __restrict__ x, int64_t ldx, int64_t cols,
+                                                   int64_t width, const int32_t* __restrict__ act,
+                                                   const int32_t* __restrict__ count, int vec,
+                                                   char* __restrict__ xc) {
+  constexpr int ES = Tile<DT>::ES, V = 16 / ES;
+  const int64_t pieces = width / V;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t k = i / pieces, c = (i - k * pieces) * V;
+  if (k >= *count) return;
+  const char* src = x + ((int64_t)act[k] * ldx + c) * ES;
+  u32x4_t v = {0, 0, 0, 0};
+  if (vec) {
+    v = *(const u32x4_t*)src;
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      if (c + e >= cols) continue;
+      if constexpr (DT == ODP_DTYPE_F32) v[e] = ((const uint32_t*)src)[e];
+      else v[e / 2] |= (uint32_t)((const uint16_t*)src)[e] << (16 * (e & 1));
+    }
+  }
+  odp_gstore((u32x4_t*)(xc + (k * width + c) * ES), v);
+}
+
+struct Xent {
+  const void* xc;  // [count][width]
+  const void* w;   // [vocab][ldw]
+  int64_t ldw, vocab, width, n;
+  const int32_t* count;
+  const int32_t* act;
+  const int32_t* tgt;
+  float cap, inv_cap2;  // softcap and 2 / softcap (cap 0: none)
+};
+
+// ---------------------------------------------------------------------------
+// Forward: per (row, tile of the vocabulary) the maximum and the sum of
+// exponentials below it, and each row's target logit.
+// ---------------------------------------------------------------------------
+template <int DT>
+__global__ __launch_bounds__(Tile<DT>::THREADS, 2) void k_xent_stats(Xent p, float* __restrict__ pmax,
+                                                                     float* __restrict__ psum,
+                                                                     float* __restrict__ ztgt) {
+  using T = Tile<DT>;
+  const int cnt = *(const ODP_CONST int32_t*)p.count;
+  int ti, tj;
+  if (!tile_of(blockIdx.x, (cnt + T::ET - 1) / T::ET, (int)((p.vocab + T::ET - 1) / T::ET), ti, tj)) return;
+  const int64_t o0 = (int64_t)ti * T::ET, n0 = (int64_t)tj * T::ET;
+  typename T::Acc acc;
+  t_zero(acc);
+  t_product<DT, true, true>(Operand{p.xc, p.width, o0, cnt}, Operand{p.w, p.ldw, n0, p.vocab}, (int32_t)p.width, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = T::WM * (wave & 1), wn = T::WN * (wave >> 1);
+  float* red = (float*)t_stage<DT>(0);  // [waves across n][ET rows][2]
+  static_for<T::BI>([&](auto ii) {
+    constexpr int i = decltype(ii)::value;
+    const int64_t o = o0 + wm + t_row(i);
+    const int32_t tgt = o < cnt ? p.tgt[o] : -1;
+    float z[T::BJ][4], m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < T::BJ; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t n = n0 + wn + t_col(j) + e;
+        float v = acc[i][j][e];
+        if (p.cap != 0.f) v = softcapped(v, p.cap, p.inv_cap2);
+        if (n == tgt) ztgt[o] = v;
+        z[j][e] = n < p.vocab ? v : -INFINITY;
+        m = fmaxf(m, z[j][e]);
+      }
+    const float ms = m == -INFINITY ? 0.f : m;
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < T::BJ; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s += fast_exp(z[j][e] - ms);
+    // The row's other columns of this wave: lanes 16, 32 and 48 further on.
+#pragma unroll
+    for (int off = 16; off <= 32; off <<= 1) {
+      const float m2 = __shfl_xor(m, off), s2 = __shfl_xor(s, off);
+      const float mm = fmaxf(m, m2), ref = mm == -INFINITY ? 0.f : mm;
+      s = s * fast_exp(m - ref) + s2 * fast_exp(m2 - ref);
+      m = mm;
+    }
+    if (lane < 16) {
+      float* r = red + 2 * ((wave >> 1) * T::ET + wm + t_row(i));
+      r[0] = m;
+      r[1] = s;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  });
+  __syncthreads();
+  for (int r = threadIdx.x; r < T::ET; r += T::THREADS) {
+    if (o0 + r >= cnt) break;
+    float m = -INFINITY, s = 0.f;
+#pragma unroll
+    for (int w = 0; w < T::WAVES / 2; ++w) m = fmaxf(m, red[2 * (w * T::ET + r)]);
+    const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int w = 0; w < T::WAVES / 2; ++w)
+      s += red[2 * (w * T::ET + r) + 1] * fast_exp(red[2 * (w * T::ET + r)] - ref);
+    pmax[(int64_t)tj * p.n + o0 + r] = m;
+    psum[(int64_t)tj * p.n + o0 + r] = s;
+  }
+}
+
+// Joins the tiles' statistics: 16 rows a workgroup, 16 lanes each.
+__global__ __launch_bounds__(256) void k_xent_losses(const float* __restrict__ pmax, const float* __restrict__ psum,
+                                                     const float* __restrict__ ztgt, int tiles, int64_t n,
+                                                     const int32_t* __restrict__ count,
+                                                     const int32_t* __restrict__ act, const int32_t* __restrict__ tgt,
+                                                     float* __restrict__ losses, float* __restrict__ lse) {
+  __shared__ float rm[16][17], rs[16][17];
+  const int r = threadIdx.x & 15, q = threadIdx.x >> 4;
+  const int64_t row = (int64_t)blockIdx.x * 16 + r;
+  const bool on = row < *count;
+  float m = -INFINITY, s = 0.f;
+  if (on)
+    for (int t = q; t < tiles; t += 16) {
+      const float m2 = pmax[(int64_t)t * n + row], s2 = psum[(int64_t)t * n + row];
+      const float mm = fmaxf(m, m2), ref = mm == -INFINITY ? 0.f : mm;
+      s = s * fast_exp(m - ref) + s2 * fast_exp(m2 - ref);
+      m = mm;
+    }
+  rm[q][r] = m;
+  rs[q][r] = s;
+  __syncthreads();
+  if (q != 0 || !on) return;
+  for (int t = 1; t < 16; ++t) m = fmaxf(m, rm[t][r]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  s = 0.f;
+  for (int t = 0; t < 16; ++t) s += rs[t][r] * fast_exp(rm[t][r] - ref);
+  const float l = ref + logf(s);
+  lse[act[row]] = l;
+  if (tgt[row] >= 0) losses[act[row]] = l - ztgt[row];
+}
+
+// ---------------------------------------------------------------------------
+// Stores of a tile in the operands' type: rows o (of `rows`) of pitch ld from
+// row o0, columns n0 + .. below `cols`, val(i, j, e) the entries.  16-bit
+// tiles go through the idle ring so that rows leave in 16-byte pieces.
+// ---------------------------------------------------------------------------
+template <int DT, typename Val>
+__device__ __forceinline__ void t_store(void* out, int64_t ld, int64_t o0, int64_t rows, int64_t n0, int64_t cols,
+                                        Val val) {
+  using T = Tile<DT>;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = T::WM * (wave & 1), wn = T::WN * (wave >> 1);
+  if constexpr (DT == ODP_DTYPE_F32) {
+    static_for<T::BI * T::BJ>([&](auto q) {
+      constexpr int i = decltype(q)::value / T::BJ, j = decltype(q)::value % T::BJ;
+      const int64_t o = o0 + wm + t_row(i), n = n0 + wn + t_col(j);
+      const f32x4_t v = val(Idx<i>{}, Idx<j>{});
+      if (o < rows && n < cols) odp_gstore((f32x4_t*)((float*)out + o * ld + n), v);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  } else {
+    uint16_t* stg = (uint16_t*)(t_stage<DT>(wave >> 1) + (wave & 1) * (T::WM * T::WN * 2));
+    static_for<T::BI * T::BJ>([&](auto q) {
+      constexpr int i = decltype(q)::value / T::BJ, j = decltype(q)::value % T::BJ;
+      const f32x4_t v = val(Idx<i>{}, Idx<j>{});
+      const int r = t_row(i), c = t_col(j);
+      *(u32x2_alias_t*)&stg[r * T::WN + 8 * ((c >> 3) ^ (r & 7)) + (c & 7)] =
+          u32x2_t{odp_f2bf2(v[0], v[1]), odp_f2bf2(v[2], v[3])};
+      __builtin_amdgcn_sched_barrier(0);
+    });
+#pragma unroll
+    for (int k = 0; k < T::WM / 8; ++k) {
+      const int r = 8 * k + (lane >> 3), c = lane & 7;
+      const u32x4_t v = *(const u32x4_alias_t*)&stg[r * T::WN + 8 * (c ^ (r & 7))];
+      const int64_t o = o0 + wm + r, n = n0 + wn + 8 * c;
+      if (o < rows && n < cols) odp_gstore((u32x4_t*)((uint16_t*)out + o * ld + n), v);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Backward: d of the vocabulary's columns [v0, v0 + vc), [count][ldd], with
+// zeros up to ldd (a multiple of the tile).
+// ---------------------------------------------------------------------------
+template <int DT>
+__global__ __launch_bounds__(Tile<DT>::THREADS, 2) void k_xent_dlogits(Xent p, int64_t v0, int64_t vc,
+                                                                       const float* __restrict__ lse,
+                                                                       const float* __restrict__ g, void* dl,
+                                                                       int64_t ldd) {
+  using T = Tile<DT>;
+  const int cnt = *(const ODP_CONST int32_t*)p.count;
+  int ti, tj;
+  if (!tile_of(blockIdx.x, (cnt + T::ET - 1) / T::ET, (int)(ldd / T::ET), ti, tj)) return;
+  const int64_t o0 = (int64_t)ti * T::ET, n0 = (int64_t)tj * T::ET;
+  typename T::Acc acc;
+  t_zero(acc);
+  const void* w = (const char*)p.w + v0 * p.ldw * T::ES;
+  t_product<DT, true, true>(Operand{p.xc, p.width, o0, cnt}, Operand{w, p.ldw, n0, vc}, (int32_t)p.width, acc);
+  const int wave = threadIdx.x >> 6;
+  const int wm = T::WM * (wave & 1), wn = T::WN * (wave >> 1);
+  float rl[T::BI], rg[T::BI];
+  constexpr int32_t NONE = INT32_MIN;  // no loss: a target may lie just below the piece
+  int32_t rt[T::BI];
+#pragma unroll
+  for (int i = 0; i < T::BI; ++i) {
+    const int64_t o = o0 + wm + t_row(i);
+    const int32_t t = o < cnt ? p.tgt[o] : -1;
+    const int64_t row = o < cnt ? p.act[o] : 0;
+    rl[i] = t >= 0 ? lse[row] : 0.f;
+    rg[i] = t >= 0 ? g[row] : 0.f;
+    rt[i] = t >= 0 ? t - (int32_t)v0 : NONE;
+  }
+  const float inv_cap = 0.5f * p.inv_cap2;
+  t_store<DT>(dl, ldd, o0, cnt, n0, ldd, [&](auto ii, auto jj) __attribute__((always_inline)) {
+    constexpr int i = decltype(ii)::value, j = decltype(jj)::value;
+    f32x4_t d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int64_t n = n0 + wn + t_col(j) + e;
+      float z = acc[i][j][e], slope = 1.f;
+      if (p.cap != 0.f) {
+        z = softcapped(z, p.cap, p.inv_cap2);
+        const float y = z * inv_cap;
+        slope = 1.f - y * y;
+      }
+      const float q = fast_exp(z - rl[i]) - (n == (int64_t)rt[i] ? 1.f : 0.f);
+      d[e] = rt[i] != NONE && n < vc ? rg[i] * q * slope : 0.f;
+    }
+    return d;
+  });
+}
+
+// How many slices of the contraction each tile of dx is split into: the
+// fewest of 1 .. 8 with which the workgroups fill the 256 CUs' rounds best,
+// as far as the slots (`cap` tiles) and slices of 16 steps go.
+__host__ __device__ inline int dx_split(int tiles, int cap, int64_t steps) {
+  int best = 1, rounds = (tiles + 255) / 256;
+  for (int s = 2; s <= 8 && s * tiles <= cap && steps >= 16 * s; ++s) {
+    const int r = (s * tiles + 255) / 256;
+    if (r * best < rounds * s) best = s, rounds = r;
+  }
+  return best;
+}
+
+// Slot s of dx [slices][count][width] (float32) (+)= d[:, slice s] W[slice s].
+template <int DT>
+__global__ __launch_bounds__(Tile<DT>::THREADS, 2) void k_xent_dx(Xent p, int64_t v0, int64_t vc, int64_t piece,
+                                                                  const void* dl, int64_t ldd, int cap, int first,
+                                                                  float* __restrict__ slots) {
+  using T = Tile<DT>;
+  const int cnt = *(const ODP_CONST int32_t*)p.count;
+  const int tm = (cnt + T::ET - 1) / T::ET, tn = (int)((p.width + T::ET - 1) / T::ET);
+  if (tm == 0) return;
+  const int split = dx_split(tm * tn, cap, piece / T::EK);
+  int ti, tj;
+  if (!tile_of(blockIdx.x, tm, tn * split, ti, tj)) return;
+  const int s = tj / tn;
+  tj -= s * tn;
+  const int64_t o0 = (int64_t)ti * T::ET, n0 = (int64_t)tj * T::ET;
+  // Slices of whole steps, the same for every piece.
+  const int64_t per = (piece / T::EK + split - 1) / split * T::EK, k0 = s * per;
+  const int32_t kn = (int32_t)max((int64_t)0, min(per, vc - k0));
+  if (kn == 0 && !first) return;
+  typename T::Acc acc;
+  t_zero(acc);
+  t_product<DT, true, false>(Operand{(const char*)dl + k0 * T::ES, ldd, o0, cnt},
+                             Operand{(const char*)p.w + (v0 + k0) * p.ldw * T::ES, p.ldw, n0, p.width}, kn, acc);
+  const int wave = threadIdx.x >> 6;
+  const int wm = T::WM * (wave & 1), wn = T::WN * (wave >> 1);
+  float* out = slots + (int64_t)s * cnt * p.width;
+  static_for<T::BI * T::BJ>([&](auto q) {
+    constexpr int i = decltype(q)::value / T::BJ, j = decltype(q)::value % T::BJ;
+    const int64_t o = o0 + wm + t_row(i), n = n0 + wn + t_col(j);
+    if (o < cnt && n < p.width) {
+      f32x4_t* at = (f32x4_t*)(out + o * p.width + n);
+      f32x4_t v = acc[i][j];
+      if (!first) v = v + *(const ODP_GMEM f32x4_t*)(const ODP_GMEM void*)at;
+      odp_gstore(at, v);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  });
+}
+
+// dx [n][cols] in the inputs' type from the slots; rows without a loss are
+// zero, rows with a target outside the vocabulary NaN.
+template <int DT>
+__global__ __launch_bounds__(256) void k_xent_dx_rows(const float* __restrict__ slots, int64_t width, int64_t cols,
+                                                      int64_t n, const int32_t* __restrict__ count,
+                                                      const int32_t* __restrict__ where, int tn, int cap,
+                                                      int64_t steps, void* __restrict__ dx) {
+  const int64_t quads = width / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = i / quads, c = (i - row * quads) * 4;
+  if (row >= n) return;
+  const int cnt = *count, k = where[row];
+  f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+  if (k >= 0) {
+    const int split = dx_split((cnt + Tile<DT>::ET - 1) / Tile<DT>::ET * tn, cap, steps);
+    const float* at = slots + (int64_t)k * width + c;
+    v = *(const f32x4_t*)at;
+    for (int s = 1; s < split; ++s) v = v + *(const f32x4_t*)(at + (int64_t)s * cnt * width);
+  } else if (k == -2) {
+    v[0] = v[1] = v[2] = v[3] = __uint_as_float(0x7fc00000u);
+  }
+  if (cols == width) {
+    if constexpr (DT == ODP_DTYPE_F32) odp_gstore((f32x4_t*)((float*)dx + row * cols + c), v);
+    else odp_gstore((u32x2_t*)((uint16_t*)dx + row * cols + c), u32x2_t{odp_f2bf2(v[0], v[1]), odp_f2bf2(v[2], v[3])});
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (c + e < cols) odp_store_from_float(dx, row * cols + c + e, DT, v[e]);
+}
+
+// dW rows [0, vc) of pitch lddw = d^T x.
+template <int DT>
+__global__ __launch_bounds__(Tile<DT>::THREADS, 2) void k_xent_dw(Xent p, int64_t vc, const void* dl, int64_t ldd,
+                                                                  void* dw, int64_t lddw) {
+  using T = Tile<DT>;
+  const int cnt = *(const ODP_CONST int32_t*)p.count;
+  int ti, tj;
+  if (!tile_of(blockIdx.x, (int)((vc + T::ET - 1) / T::ET), (int)((p.width + T::ET - 1) / T::ET), ti, tj)) return;
+  const int64_t o0 = (int64_t)ti * T::ET, n0 = (int64_t)tj * T::ET;
+  typename T::Acc acc;
+  t_zero(acc);
+  t_product<DT, false, false>(Operand{dl, ldd, o0, ldd}, Operand{p.xc, p.width, n0, p.width}, cnt, acc);
+  t_store<DT>(dw, lddw, o0, vc, n0, p.width, [&](auto ii, auto jj) __attribute__((always_inline)) {
+    return acc[decltype(ii)::value][decltype(jj)::value];
+  });
+}
+
+int check_xent(const char* what, int dtype, int64_t n, int64_t width, int64_t ldw, int64_t vocab) {
+  if (dtype != ODP_DTYPE_F32 && dtype != ODP_DTYPE_BF16) {
+    odp_set_error("%s: rows must be float32 or bfloat16 (dtype %d)", what, dtype);
+    return ODP_ERR_UNSUPPORTED;
+  }
+  const int64_t per = dtype == ODP_DTYPE_F32 ? 4 : 8;
+  if (n < 0 || n >= ((int64_t)1 << 31) - 512 || width <= 0 || width % per != 0 || width >= (int64_t)1 << 20 ||
+      ldw < width || ldw % per != 0 || ldw >= (int64_t)1 << 20 || vocab <= 0 || vocab >= ((int64_t)1 << 31) - 512) {
+    odp_set_error("%s: invalid sizes (n %lld, width %lld, pitch %lld, vocab %lld)", what, (long long)n,
+                  (long long)width, (long long)ldw, (long long)vocab);
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  return ODP_OK;
+}
+
+int tile_edge(int dtype) { return dtype == ODP_DTYPE_F32 ? 128 : 256; }
+
+// Workgroups of a tm x tn grid of tiles (tile_of).
+int grid_of(const char* what, int64_t tm, int64_t tn, unsigned& blocks) {
+  const int64_t b = (tm * tn + 7) / 8 * 8;
+  if (b >= (int64_t)1 << 23) {
+    odp_set_error("%s: the launch needs %lld workgroups", what, (long long)b);
+    return ODP_ERR_UNSUPPORTED;
+  }
+  blocks = (unsigned)b;
+  return ODP_OK;
+}
+
+int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+Xent xent_of(const void* xc, const void* w, int64_t ldw, int64_t vocab, int64_t width, int64_t n,
+             const int32_t* count, const int32_t* act, const int32_t* tgt, float cap) {
+  return Xent{xc, w, ldw, vocab, width, n, count, act, tgt, cap, cap != 0.f ? 2.0f / cap : 0.f};
+}
+
+bool on16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+}  // namespace
+
+#define ODP_XENT_LAUNCH(K, GRID, ...)                                                                          \
+  do {                                                                                                         \
+    if (dtype == ODP_DTYPE_F32)                                                                                \
+      hipLaunchKernelGGL((K<ODP_DTYPE_F32>), dim3(GRID), dim3(Tile<ODP_DTYPE_F32>::THREADS), 0, s, __VA_ARGS__); \
+    else                                                                                                       \
+      hipLaunchKernelGGL((K<ODP_DTYPE_BF16>), dim3(GRID), dim3(Tile<ODP_DTYPE_BF16>::THREADS), 0, s, __VA_ARGS__); \
+  } while (0)
+
+extern "C" int odp_xent_rows(odp_stream_t stream, int dtype, const void* x, int64_t ldx, int64_t n, int64_t cols,
+                             int64_t width, const void* target, int target_bytes, int64_t vocab, int64_t ignore,
+                             int keep, void* xc, int32_t* act, int32_t* tgt, int32_t* where, int32_t* count,
+                             float* losses, float* lse) {
+  if (int rc = check_xent("odp_xent_rows", dtype, n, width, width, vocab)) return rc;
+  if (cols <= 0 || cols > width || ldx < cols || (target_bytes != 4 && target_bytes != 8)) {
+    odp_set_error("odp_xent_rows: %lld columns of pitch %lld, targets of %d bytes", (long long)cols, (long long)ldx,
+                  target_bytes);
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  if (n > 0 && (x == nullptr || target == nullptr || xc == nullptr || act == nullptr || tgt == nullptr ||
+                where == nullptr)) {
+    odp_set_error("odp_xent_rows: null pointer");
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  if (count == nullptr || !on16(xc)) {
+    odp_set_error("odp_xent_rows: null count or packed rows off the 16-byte grid");
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  const hipStream_t s = odp_hip_stream(stream);
+  hipLaunchKernelGGL(k_xent_pick, dim3(1), dim3(1024), 0, s, target, target_bytes == 8 ? 1 : 0, n, vocab, ignore, keep,
+                     act, tgt, where, count, losses, lse);
+  const int64_t es = dtype == ODP_DTYPE_F32 ? 4 : 2;
+  const int64_t blocks = up(n * (width * es / 16), 256);
+  if (blocks >= (int64_t)1 << 24) {
+    odp_set_error("odp_xent_rows: the launch needs %lld workgroups", (long long)blocks);
+    return ODP_ERR_UNSUPPORTED;
+  }
+  if (blocks > 0) {
+    const int vec = cols == width && on16(x) && ldx * es % 16 == 0;
+    if (dtype == ODP_DTYPE_F32)
+      hipLaunchKernelGGL((k_xent_pack<ODP_DTYPE_F32>), dim3((unsigned)blocks), dim3(256), 0, s, (const char*)x, ldx,
+                         cols, width, act, count, vec, (char*)xc);
+    else
+      hipLaunchKernelGGL((k_xent_pack<ODP_DTYPE_BF16>), dim3((unsigned)blocks), dim3(256), 0, s, (const char*)x, ldx,
+                         cols, width, act, count, vec, (char*)xc);
+  }
+  return odp_check_launch("odp_xent_rows");
+}
+
+extern "C" int64_t odp_xent_stats_scratch(int dtype, int64_t n, int64_t vocab) {
+  if (n <= 0 || vocab <= 0) return 0;
+  return 4 * n * (2 * up(vocab, tile_edge(dtype)) + 1);
+}
+
+extern "C" int odp_xent_losses(odp_stream_t stream, int dtype, const void* xc, int64_t n, int64_t width,
+                               const int32_t* act, const int32_t* tgt, const int32_t* count, const void* w,
+                               int64_t ldw, int64_t vocab, float softcap, void* scratch, float* losses, float* lse) {
+  if (int rc = check_xent("odp_xent_losses", dtype, n, width, ldw, vocab)) return rc;
+  if (n == 0) return ODP_OK;
+  if (xc == nullptr || act == nullptr || tgt == nullptr || count == nullptr || w == nullptr || scratch == nullptr ||
+      losses == nullptr || lse == nullptr || !on16(xc) || !on16(w)) {
+    odp_set_error("odp_xent_losses: null pointer, or rows off the 16-byte grid");
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  const hipStream_t s = odp_hip_stream(stream);
+  const int64_t tn = up(vocab, tile_edge(dtype));
+  unsigned blocks;
+  if (int rc = grid_of("odp_xent_losses", up(n, tile_edge(dtype)), tn, blocks)) return rc;
+  const Xent p = xent_of(xc, w, ldw, vocab, width, n, count, act, tgt, softcap);
+  float* pmax = (float*)scratch;
+  float* psum = pmax + n * tn;
+  float* ztgt = psum + n * tn;
+  ODP_XENT_LAUNCH(k_xent_stats, blocks, p, pmax, psum, ztgt);
+  hipLaunchKernelGGL(k_xent_losses, dim3((unsigned)up(n, 16)), dim3(256), 0, s, pmax, psum, ztgt, (int)tn, n, count,
+                     act, tgt, losses, lse);
+  return odp_check_launch("odp_xent_losses");
+}
+
+extern "C" int64_t odp_xent_pitch(int dtype, int64_t columns) {
+  return columns > 0 ? up(columns, tile_edge(dtype)) * tile_edge(dtype) : 0;
+}
+
+extern "C" int odp_xent_dlogits(odp_stream_t stream, int dtype, const void* xc, int64_t n, int64_t width,
+                                const int32_t* act, const int32_t* tgt, const int32_t* count, const void* w,
+                                int64_t ldw, int64_t vocab, float softcap, int64_t v0, int64_t vc, const float* lse,
+                                const float* g, void* dl, int64_t ldd) {
+  if (int rc = check_xent("odp_xent_dlogits", dtype, n, width, ldw, vocab)) return rc;
+  if (v0 < 0 || vc <= 0 || v0 + vc > vocab || ldd != odp_xent_pitch(dtype, vc)) {
+    odp_set_error("odp_xent_dlogits: columns [%lld, %lld) of %lld at pitch %lld", (long long)v0,
+                  (long long)(v0 + vc), (long long)vocab, (long long)ldd);
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  if (n == 0) return ODP_OK;
+  if (xc == nullptr || act == nullptr || tgt == nullptr || count == nullptr || w == nullptr || lse == nullptr ||
+      g == nullptr || dl == nullptr || !on16(xc) || !on16(w) || !on16(dl)) {
+    odp_set_error("odp_xent_dlogits: null pointer, or rows off the 16-byte grid");
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  const hipStream_t s = odp_hip_stream(stream);
+  unsigned blocks;
+  if (int rc = grid_of("odp_xent_dlogits", up(n, tile_edge(dtype)), ldd / tile_edge(dtype), blocks)) return rc;
+  const Xent p = xent_of(xc, w, ldw, vocab, width, n, count, act, tgt, softcap);
+  ODP_XENT_LAUNCH(k_xent_dlogits, blocks, p, v0, vc, lse, g, dl, ldd);
+  return odp_check_launch("odp_xent_dlogits");
+}
+
+// Tiles of the slots: those of n rows, or a few times as many to split.
+static int dx_cap(int dtype, int64_t n, int64_t width) {
+  const int64_t tiles = up(n, tile_edge(dtype)) * up(width, tile_edge(dtype));
+  const int64_t most = tiles * 8 < 512 ? tiles * 8 : 512;
+  return (int)(tiles > most ? tiles : most);
+}
+
+extern "C" int64_t odp_xent_dx_scratch(int dtype, int64_t n, int64_t width) {
+  if (n <= 0 || width <= 0) return 0;
+  return 4 * (int64_t)dx_cap(dtype, n, width) * tile_edge(dtype) * tile_edge(dtype);
+}
+
+extern "C" int odp_xent_dx(odp_stream_t stream, int dtype, int64_t n, int64_t width, const int32_t* count,
+                           const void* w, int64_t ldw, int64_t vocab, int64_t v0, int64_t vc, int64_t piece,
+                           const void* dl, int64_t ldd, void* scratch) {
+  if (int rc = check_xent("odp_xent_dx", dtype, n, width, ldw, vocab)) return rc;
+  if (v0 < 0 || vc <= 0 || vc > piece || v0 + vc > vocab || ldd != odp_xent_pitch(dtype, vc) ||
+      ldd >= (int64_t)1 << 20) {
+    odp_set_error("odp_xent_dx: columns [%lld, %lld) of %lld in pieces of %lld at pitch %lld", (long long)v0,
+                  (long long)(v0 + vc), (long long)vocab, (long long)piece, (long long)ldd);
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  if (n == 0) return ODP_OK;
+  if (count == nullptr || w == nullptr || dl == nullptr || scratch == nullptr || !on16(w) || !on16(dl) ||
+      !on16(scratch)) {
+    odp_set_error("odp_xent_dx: null pointer, or rows off the 16-byte grid");
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  const hipStream_t s = odp_hip_stream(stream);
+  const int cap = dx_cap(dtype, n, width);
+  const int64_t tiles = up(n, tile_edge(dtype)) * up(width, tile_edge(dtype));
+  unsigned blocks;
+  if (int rc = grid_of("odp_xent_dx", tiles > cap ? tiles : cap, 1, blocks)) return rc;
+  const Xent p = xent_of(nullptr, w, ldw, vocab, width, n, count, nullptr, nullptr, 0.f);
+  const int64_t whole = odp_xent_pitch(dtype, piece);
+  ODP_XENT_LAUNCH(k_xent_dx, blocks, p, v0, vc, whole, dl, ldd, cap, v0 == 0 ? 1 : 0, (float*)scratch);
+  return odp_check_launch("odp_xent_dx");
+}
+
+extern "C" int odp_xent_dx_rows(odp_stream_t stream, int dtype, int64_t n, int64_t cols, int64_t width,
+                                const int32_t* count, const int32_t* where, int64_t piece, const void* scratch,
+                                void* dx) {
+  if (int rc = check_xent("odp_xent_dx_rows", dtype, n, width, width, 1)) return rc;
+  if (cols <= 0 || cols > width || piece <= 0) {
+    odp_set_error("odp_xent_dx_rows: %lld columns of %lld, pieces of %lld", (long long)cols, (long long)width,
+                  (long long)piece);
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  if (n == 0) return ODP_OK;
+  if (count == nullptr || where == nullptr || scratch == nullptr || dx == nullptr || !on16(scratch) ||
+      (cols == width && !on16(dx))) {
+    odp_set_error("odp_xent_dx_rows: null pointer, or rows off the 16-byte grid");
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  const int64_t blocks = up(n * (width / 4), 256);
+  if (blocks >= (int64_t)1 << 24) {
+    odp_set_error("odp_xent_dx_rows: the launch needs %lld workgroups", (long long)blocks);
+    return ODP_ERR_UNSUPPORTED;
+  }
+  const hipStream_t s = odp_hip_stream(stream);
+  const int tn = (int)up(width, tile_edge(dtype)), cap = dx_cap(dtype, n, width);
+  const int64_t steps = odp_xent_pitch(dtype, piece) / (dtype == ODP_DTYPE_F32 ? 16 : 32);
+  if (dtype == ODP_DTYPE_F32)
+    hipLaunchKernelGGL((k_xent_dx_rows<ODP_DTYPE_F32>), dim3((unsigned)blocks), dim3(256), 0, s,
+                       (const float*)scratch, width, cols, n, count, where, tn, cap, steps, dx);
+  else
+    hipLaunchKernelGGL((k_xent_dx_rows<ODP_DTYPE_BF16>), dim3((unsigned)blocks), dim3(256), 0, s,
+                       (const float*)scratch, width, cols, n, count, where, tn, cap, steps, dx);
+  return odp_check_launch("odp_xent_dx_rows");
+}
+
+extern "C" int odp_xent_dw(odp_stream_t stream, int dtype, const void* xc, int64_t n, int64_t width,
+                           const int32_t* count, int64_t vc, const void* dl, int64_t ldd, void* dw, int64_t lddw) {
+  if (int rc = check_xent("odp_xent_dw", dtype, n, width, lddw, vc)) return rc;
+  if (ldd != odp_xent_pitch(dtype, vc) || ldd >= (int64_t)1 << 20 || count == nullptr || dw == nullptr || !on16(dw) ||
+      (n > 0 && (xc == nullptr || dl == nullptr || !on16(xc) || !on16(dl)))) {
+    odp_set_error("odp_xent_dw: pitch %lld for %lld columns, null pointer, or rows off the 16-byte grid",
+                  (long long)ldd, (long long)vc);
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  const hipStream_t s = odp_hip_stream(stream);
+  unsigned blocks;
+  if (int rc = grid_of("odp_xent_dw", up(vc, tile_edge(dtype)), up(width, tile_edge(dtype)), blocks)) return rc;
+  const Xent p = xent_of(xc, nullptr, width, vc, width, n, count, nullptr, nullptr, 0.f);
+  ODP_XENT_LAUNCH(k_xent_dw, blocks, p, vc, dl, ldd, dw, lddw);
+  return odp_check_launch("odp_xent_dw");
+}

@@ -208,4 +208,256 @@ class Embedding(torch.nn.Embedding):
         return embedding(tokens, self.weight, scale=self.scale, padding_idx=self.padding_idx)
 
 
-__all__ = ["Embedding", "embedding"]
+# ---------------------------------------------------------------------------
+# Linear cross entropy
+# ---------------------------------------------------------------------------
+
+_HEAD_DTYPES = (torch.float32, torch.bfloat16)
+# Bytes of d (the logits' gradient, in the inputs' type) that the backward
+# holds at a time: a piece of the vocabulary for all tokens.
+PIECE_BYTES = 512 << 20
+
+
+def _lanes(dtype: torch.dtype) -> int:
+    """Elements in 16 bytes."""
+    return 4 if dtype == torch.float32 else 8
+
+
+def _head_rows(weight: torch.Tensor) -> torch.Tensor:
+    """The head with rows on the 16-byte grid: itself, or a copy whose width is padded with zeros."""
+    w, per = pitched_rows(weight.detach()), _lanes(weight.dtype)
+    if w.shape[1] % per == 0 and w.stride(0) % per == 0 and w.data_ptr() % 16 == 0:
+        return w
+    wide = w.new_zeros(w.shape[0], -(-w.shape[1] // per) * per)
+    wide[:, : w.shape[1]] = w
+    return wide
+
+
+class _Packed:
+    """The rows that bear a loss, gathered (every row with ``keep``)."""
+
+    def __init__(self, x: torch.Tensor, w: torch.Tensor, target: torch.Tensor, ignore: int, keep: bool = False,
+                 losses: torch.Tensor | None = None, lse: torch.Tensor | None = None) -> None:
+        rows, flat = pitched_rows(x.detach()), _flat_tokens(target)
+        self.dt, self.n, self.cols = dtype_code(x.dtype), flat.numel(), rows.shape[1]
+        self.w, self.vocab, self.width = w, w.shape[0], w.shape[1]
+        dev = x.device
+        self.xc = torch.empty((max(self.n, 1), self.width), dtype=x.dtype, device=dev)
+        ids = torch.empty((4, max(self.n, 1)), dtype=torch.int32, device=dev)
+        self.act, self.tgt, self.where, self.count = (ids[k].data_ptr() for k in range(4))
+        self._ids = ids
+        N.call("odp_xent_rows", _stream(x), self.dt, rows.data_ptr(), rows.stride(0), self.n, self.cols, self.width,
+               flat.data_ptr(), flat.element_size(), self.vocab, ignore, int(keep), self.xc.data_ptr(), self.act,
+               self.tgt, self.where, self.count, None if losses is None else losses.data_ptr(),
+               None if lse is None else lse.data_ptr())
+
+    def losses(self, softcap: float, losses: torch.Tensor, lse: torch.Tensor) -> None:
+        scratch = torch.empty(max(int(N.load().odp_xent_stats_scratch(self.dt, self.n, self.vocab)) // 4, 1),
+                              dtype=torch.float32, device=self.xc.device)
+        N.call("odp_xent_losses", _stream(self.xc), self.dt, self.xc.data_ptr(), self.n, self.width, self.act,
+               self.tgt, self.count, self.w.data_ptr(), self.w.stride(0), self.vocab, softcap, scratch.data_ptr(),
+               losses.data_ptr(), lse.data_ptr())
+
+    def dlogits(self, softcap: float, lse: torch.Tensor, g: torch.Tensor, v0: int, vc: int, d: torch.Tensor) -> int:
+        """d of the columns [v0, v0 + vc) in ``d``; returns its pitch."""
+        ldd = int(N.load().odp_xent_pitch(self.dt, vc))
+        N.call("odp_xent_dlogits", _stream(self.xc), self.dt, self.xc.data_ptr(), self.n, self.width, self.act,
+               self.tgt, self.count, self.w.data_ptr(), self.w.stride(0), self.vocab, softcap, v0, vc,
+               lse.data_ptr(), g.data_ptr(), d.data_ptr(), ldd)
+        return ldd
+
+    def piece(self, whole: bool = False) -> int:
+        """Columns of the vocabulary a piece of d holds."""
+        edge = int(N.load().odp_xent_pitch(self.dt, 1))
+        fit = PIECE_BYTES // (max(self.n, 1) * self.xc.element_size()) // edge * edge
+        return self.vocab if whole else min(self.vocab, max(fit, edge))
+
+    def gradients(self, softcap: float, lse: torch.Tensor, g: torch.Tensor, x_shape: torch.Size | None,
+                  need_w: bool, keep_d: bool = False):
+        """(dx, dW, d): dx where ``x_shape`` is given; d [n, vocab] where ``keep_d`` (packed with ``keep``)."""
+        dev, dtype, lib = self.xc.device, self.xc.dtype, N.load()
+        piece = self.piece(keep_d)
+        d = torch.empty((max(self.n, 1), int(lib.odp_xent_pitch(self.dt, piece))), dtype=dtype, device=dev)
+        dx = dw = sums = None
+        s = _stream(self.xc)
+        if x_shape is not None:
+            dx = torch.empty(x_shape, dtype=dtype, device=dev)
+            sums = torch.empty(max(int(lib.odp_xent_dx_scratch(self.dt, self.n, self.width)) // 4, 1),
+                               dtype=torch.float32, device=dev)
+        if need_w:
+            dw = torch.empty((self.vocab, self.width), dtype=dtype, device=dev)
+        for v0 in range(0, self.vocab, piece):
+            vc = min(piece, self.vocab - v0)
+            ldd = self.dlogits(softcap, lse, g, v0, vc, d)
+            if dx is not None:
+                N.call("odp_xent_dx", s, self.dt, self.n, self.width, self.count, self.w.data_ptr(),
+                       self.w.stride(0), self.vocab, v0, vc, piece, d.data_ptr(), ldd, sums.data_ptr())
+            if dw is not None:
+                N.call("odp_xent_dw", s, self.dt, self.xc.data_ptr(), self.n, self.width, self.count, vc,
+                       d.data_ptr(), ldd, dw[v0:].data_ptr(), self.width)
+        if dx is not None:
+            N.call("odp_xent_dx_rows", s, self.dt, self.n, self.cols, self.width, self.count, self.where, piece,
+                   sums.data_ptr(), dx.data_ptr())
+        if dw is not None and self.cols != self.width:
+            dw = dw[:, : self.cols].contiguous()
+        return dx, dw, d[: self.n, : self.vocab] if keep_d else None
+
+
+def _xent_losses(x, weight, target, softcap, ignore):
+    losses = torch.empty(target.shape, dtype=torch.float32, device=x.device)
+    lse = torch.empty(target.shape, dtype=torch.float32, device=x.device)
+    with torch.cuda.device(x.device):
+        p = _Packed(x, _head_rows(weight), target, ignore, False, losses, lse)
+        p.losses(softcap, losses, lse)
+    return losses, lse
+
+
+def _xent_gradients(g, x, weight, target, lse, softcap, ignore, need_x, need_w, keep_d=False):
+    g, lse = g.detach().float().contiguous(), lse.contiguous()
+    with torch.cuda.device(x.device):
+        p = _Packed(x, _head_rows(weight), target, ignore, keep_d)
+        return p.gradients(softcap, lse, g, x.shape if need_x else None, need_w, keep_d)
+
+
+class _XentGrad(torch.autograd.Function):
+    """Gradients of the token losses; per example under vmap."""
+
+    generate_vmap_rule = False
+
+    @staticmethod
+    def forward(g, x, weight, target, lse, softcap, ignore, need_x, need_w):
+        dx, dw, _ = _xent_gradients(g, x, weight, target, lse, softcap, ignore, need_x, need_w)
+        return dx, dw
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        pass
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise NotImplementedError("linear_cross_entropy has no second derivative here")
+
+    @staticmethod
+    def vmap(info, in_dims, g, x, weight, target, lse, softcap, ignore, need_x, need_w):
+        n = info.batch_size
+        g, x, target, lse = (_front(t, d, n) for t, d in zip((g, x, target, lse), (*in_dims[:2], *in_dims[3:5])))
+        if in_dims[2] is None and not need_w:  # one head: the batch is one set of rows
+            return _XentGrad.apply(g, x, weight, target, lse, softcap, ignore, need_x, need_w), (0, None)
+        w = _front(weight, in_dims[2], n)
+        out = [_XentGrad.apply(g[i], x[i], w[i], target[i], lse[i], softcap, ignore, need_x, need_w)
+               for i in range(n)]
+        return (torch.stack([o[0] for o in out]) if need_x else None,
+                torch.stack([o[1] for o in out]) if need_w else None), (0 if need_x else None, 0 if need_w else None)
+
+
+class _Xent(torch.autograd.Function):
+    """Token losses [*target.shape] and their log-sum-exp; merges the batch
+    under vmap and, in a capture pass, records x and the logits' gradient of
+    an eligible head."""
+
+    generate_vmap_rule = False
+
+    @staticmethod
+    def forward(x, weight, target, softcap, ignore):
+        return _xent_losses(x, weight, target, softcap, ignore)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        x, weight, target, ctx.softcap, ctx.ignore = inputs
+        ctx.mark_non_differentiable(output[1])
+        ctx.save_for_backward(x, weight, target, output[1])
+
+    @staticmethod
+    def backward(ctx, g, _):
+        x, weight, target, lse = ctx.saved_tensors
+        need_x, need_w = ctx.needs_input_grad[:2]
+        dx, dw = _XentGrad.apply(g, x, weight, target, lse, ctx.softcap, ctx.ignore, need_x, need_w)
+        return dx, dw, None, None, None
+
+    @staticmethod
+    def vmap(info, in_dims, x, weight, target, softcap, ignore):
+        n = info.batch_size
+        x, target = _front(x, in_dims[0], n), _front(target, in_dims[2], n)
+        if in_dims[1] is not None:  # a head per example
+            w = weight.movedim(in_dims[1], 0)
+            out = [_Xent.apply(x[i], w[i], target[i], softcap, ignore) for i in range(n)]
+            return (torch.stack([o[0] for o in out]), torch.stack([o[1] for o in out])), (0, 0)
+        sess = active_session()
+        if sess is None or sess.mode != "capture" or id(weight) not in sess.eligible:
+            return _Xent.apply(x, weight, target, softcap, ignore), (0, 0)
+        rec = SiteRecord(x=x, A=None, B=None, scaling=1.0, a_obj=None, b_obj=None, a_transposed=False,
+                         b_transposed=False, w_obj=weight)
+        sess.sites.append(rec)
+        return _TapXent.apply(x, weight, target, softcap, ignore, sess.anchor, rec), (0, 0)
+
+
+class _TapXent(torch.autograd.Function):
+    """Physical losses of a head that trains under ``clipped_grad``: the
+    backward keeps d (the logits' gradient, [rows, vocabulary] in the
+    inputs' type), from which the plan takes the head's per-example norms and
+    clipped sum as of any full-weight linear."""
+
+    @staticmethod
+    def forward(x, weight, target, softcap, ignore, anchor, record):
+        return _xent_losses(x, weight, target, softcap, ignore)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        x, weight, target, ctx.softcap, ctx.ignore, _, ctx.record = inputs
+        ctx.mark_non_differentiable(output[1])
+        ctx.save_for_backward(x, weight, target, output[1])
+
+    @staticmethod
+    def backward(ctx, g, _):
+        x, weight, target, lse = ctx.saved_tensors
+        dx, _, d = _xent_gradients(g, x, weight, target, lse, ctx.softcap, ctx.ignore, ctx.needs_input_grad[0],
+                                   False, keep_d=True)
+        ctx.record.g = d[: target.numel()].unflatten(0, target.shape) if target.dim() > 1 else d
+        return dx, None, None, None, None, torch.zeros((), dtype=torch.float32, device=g.device), None
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *,
+                         softcap: float | None = None, ignore_index: int = -100,
+                         reduction: str = "mean") -> torch.Tensor:
+    """Cross entropy of ``x weight^T`` against ``target``, without the [tokens, vocabulary] logits.
+
+    ``x`` [..., width] and ``weight`` [vocabulary, width] are both float32 or
+    both bfloat16, ``target`` [...] int64 or int32.  ``softcap`` bounds the
+    logits as ``softcap * tanh(logits / softcap)``.  ``reduction`` "none"
+    gives the float32 loss of every token, "sum" and "mean" their sum and
+    mean over the tokens whose target is not ``ignore_index`` (NaN when there
+    is none, as torch's).  A target outside the vocabulary gives NaN.  Logits
+    and statistics are float32; the gradients are summed in float32 and
+    rounded once, from logit gradients in the inputs' type.
+
+    Replaces the reference's linear cross entropy
+    (opaque-patches/.../kernels/linear_cross_entropy.py:249).  Inside
+    ``clipped_grad`` a trainable head reached only through it is a seam.
+    """
+    if reduction not in ("none", "mean", "sum"):
+        raise ValueError(f"reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise ValueError(f"x [..., width] and weight [vocabulary, width] do not match: {tuple(x.shape)} and "
+                         f"{tuple(weight.shape)}")
+    if target.shape != x.shape[:-1]:
+        raise ValueError(f"target must be shaped {tuple(x.shape[:-1])}, got {tuple(target.shape)}")
+    if target.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"target must be int64 or int32, got {target.dtype}")
+    if x.dtype != weight.dtype or x.dtype not in _HEAD_DTYPES:
+        raise TypeError(f"x and weight must both be float32 or both bfloat16, got {x.dtype} and {weight.dtype}")
+    if weight.device.type != "cuda" or x.device != weight.device or target.device != weight.device:
+        raise RuntimeError("linear_cross_entropy runs on the GPU: its arguments must be CUDA tensors of one device")
+    if softcap is not None and not (math.isfinite(softcap) and softcap > 0):
+        raise ValueError(f"softcap must be positive and finite, got {softcap}")
+    sess = active_session()
+    if sess is not None and sess.mode == "discover":
+        sess.uses[id(weight)] = sess.uses.get(id(weight), 0) + 1
+        weight = weight.detach()
+    losses, _ = _Xent.apply(x, weight, target, float(softcap or 0.0), int(ignore_index))
+    if reduction == "none":
+        return losses
+    total = losses.sum()
+    return total if reduction == "sum" else total / (target != ignore_index).sum()
+
+
+__all__ = ["Embedding", "embedding", "linear_cross_entropy"]
