@@ -52,15 +52,16 @@ __device__ __forceinline__ float softcapped(float u, float cap, float inv_cap2) 
 
 // where[i] = the place of row i among the packed rows, -1 for a row without a
 // loss, -2 for one whose target lies outside the vocabulary (loss NaN).
-// keep: every row is packed, with target -1 where it bears no loss.
+// keep: every row is packed, with target -1 where it bears no loss.  count[0]:
+// the packed rows, count[1] (float32): the targets that are not `ignore`.
 __global__ __launch_bounds__(1024) void k_xent_pick(const void* __restrict__ target, int wide, int64_t n,
                                                     int64_t vocab, int64_t ignore, int keep, int32_t* __restrict__ act,
                                                     int32_t* __restrict__ tgt, int32_t* __restrict__ where,
                                                     int32_t* __restrict__ count, float* __restrict__ losses,
                                                     float* __restrict__ lse) {
-  __shared__ int32_t sums[16];
+  __shared__ int32_t sums[16], other[16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int32_t base = 0;
+  int32_t base = 0, counted = 0;
   for (int64_t i0 = 0; i0 < n; i0 += 1024) {
     const int64_t i = i0 + threadIdx.x;
     int64_t t = -1;
@@ -75,13 +76,18 @@ __global__ __launch_bounds__(1024) void k_xent_pick(const void* __restrict__ tar
     }
     const bool taken = keep ? i < n : live;
     const uint64_t m = __builtin_amdgcn_ballot_w64(taken);
+    const uint64_t some = __builtin_amdgcn_ballot_w64(i < n && t != ignore);
     __syncthreads();
-    if (lane == 0) sums[wave] = __popcll(m);
+    if (lane == 0) {
+      sums[wave] = __popcll(m);
+      other[wave] = __popcll(some);
+    }
     __syncthreads();
     int32_t before = base, all = 0;
     for (int w = 0; w < 16; ++w) {
       if (w < wave) before += sums[w];
       all += sums[w];
+      counted += other[w];
     }
     const int32_t k = before + __popcll(m & ((1ull << lane) - 1));
     if (taken) {
@@ -91,7 +97,10 @@ __global__ __launch_bounds__(1024) void k_xent_pick(const void* __restrict__ tar
     if (i < n) where[i] = live ? k : t == ignore ? -1 : -2;
     base += all;
   }
-  if (threadIdx.x == 0) *count = base;
+  if (threadIdx.x == 0) {
+    count[0] = base;
+    ((float*)count)[1] = (float)counted;
+  }
 }
 
 // Packed rows xc [count][width] from x's rows `act`, columns past `cols` zero.
@@ -232,6 +241,21 @@ __global__ __launch_bounds__(256) void k_xent_losses(const float* __restrict__ p
   if (tgt[row] >= 0) losses[act[row]] = l - ztgt[row];
 }
 
+// The sum of the losses (in fp64, in one order), over *over where it is given.
+__global__ __launch_bounds__(1024) void k_xent_reduce(const float* __restrict__ losses, int64_t n,
+                                                      const float* __restrict__ over, float* __restrict__ out) {
+  __shared__ double red[16];
+  double s = 0.0;
+  for (int64_t i = threadIdx.x; i < n; i += 1024) s += (double)losses[i];
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int w = 1; w < 16; ++w) s += red[w];
+  *out = over != nullptr ? (float)s / *over : (float)s;
+}
+
 // ---------------------------------------------------------------------------
 // Stores of a tile in the operands' type: rows o (of `rows`) of pitch ld from
 // row o0, columns n0 + .. below `cols`, val(i, j, e) the entries.  16-bit
@@ -278,7 +302,8 @@ __device__ __forceinline__ void t_store(void* out, int64_t ld, int64_t o0, int64
 template <int DT>
 __global__ __launch_bounds__(Tile<DT>::THREADS, 2) void k_xent_dlogits(Xent p, int64_t v0, int64_t vc,
                                                                        const float* __restrict__ lse,
-                                                                       const float* __restrict__ g, void* dl,
+                                                                       const float* __restrict__ g, int g_stride,
+                                                                       const float* __restrict__ over, void* dl,
                                                                        int64_t ldd) {
   using T = Tile<DT>;
   const int cnt = *(const ODP_CONST int32_t*)p.count;
@@ -300,7 +325,8 @@ __global__ __launch_bounds__(Tile<DT>::THREADS, 2) void k_xent_dlogits(Xent p, i
     const int32_t t = o < cnt ? p.tgt[o] : -1;
     const int64_t row = o < cnt ? p.act[o] : 0;
     rl[i] = t >= 0 ? lse[row] : 0.f;
-    rg[i] = t >= 0 ? g[row] : 0.f;
+    rg[i] = t >= 0 ? g[row * g_stride] : 0.f;
+    if (over != nullptr) rg[i] = rg[i] / *over;
     rt[i] = t >= 0 ? t - (int32_t)v0 : NONE;
   }
   const float inv_cap = 0.5f * p.inv_cap2;
@@ -538,6 +564,15 @@ extern "C" int odp_xent_losses(odp_stream_t stream, int dtype, const void* xc, i
   return odp_check_launch("odp_xent_losses");
 }
 
+extern "C" int odp_xent_reduce(odp_stream_t stream, const float* losses, int64_t n, const float* over, float* out) {
+  if (n < 0 || out == nullptr || (n > 0 && losses == nullptr)) {
+    odp_set_error("odp_xent_reduce: null pointer or %lld losses", (long long)n);
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  hipLaunchKernelGGL(k_xent_reduce, dim3(1), dim3(1024), 0, odp_hip_stream(stream), losses, n, over, out);
+  return odp_check_launch("odp_xent_reduce");
+}
+
 extern "C" int64_t odp_xent_pitch(int dtype, int64_t columns) {
   return columns > 0 ? up(columns, tile_edge(dtype)) * tile_edge(dtype) : 0;
 }
@@ -545,7 +580,7 @@ extern "C" int64_t odp_xent_pitch(int dtype, int64_t columns) {
 extern "C" int odp_xent_dlogits(odp_stream_t stream, int dtype, const void* xc, int64_t n, int64_t width,
                                 const int32_t* act, const int32_t* tgt, const int32_t* count, const void* w,
                                 int64_t ldw, int64_t vocab, float softcap, int64_t v0, int64_t vc, const float* lse,
-                                const float* g, void* dl, int64_t ldd) {
+                                const float* g, int g_stride, const float* over, void* dl, int64_t ldd) {
   if (int rc = check_xent("odp_xent_dlogits", dtype, n, width, ldw, vocab)) return rc;
   if (v0 < 0 || vc <= 0 || v0 + vc > vocab || ldd != odp_xent_pitch(dtype, vc)) {
     odp_set_error("odp_xent_dlogits: columns [%lld, %lld) of %lld at pitch %lld", (long long)v0,
@@ -562,7 +597,7 @@ extern "C" int odp_xent_dlogits(odp_stream_t stream, int dtype, const void* xc, 
   unsigned blocks;
   if (int rc = grid_of("odp_xent_dlogits", up(n, tile_edge(dtype)), ldd / tile_edge(dtype), blocks)) return rc;
   const Xent p = xent_of(xc, w, ldw, vocab, width, n, count, act, tgt, softcap);
-  ODP_XENT_LAUNCH(k_xent_dlogits, blocks, p, v0, vc, lse, g, dl, ldd);
+  ODP_XENT_LAUNCH(k_xent_dlogits, blocks, p, v0, vc, lse, g, g_stride, over, dl, ldd);
   return odp_check_launch("odp_xent_dlogits");
 }
 

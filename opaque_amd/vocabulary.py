@@ -14,6 +14,7 @@ stream; there is no CPU route.
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -25,21 +26,50 @@ from opaque_amd.engine import dtype_code
 _ROW_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
+_functions: dict[str, object] = {}
+
+
+def _call(name: str, *args) -> None:
+    """A C entry point through a kept handle (these calls are a few microseconds of host time)."""
+    f = _functions.get(name)
+    if f is None:
+        f = _functions[name] = getattr(N.load(), name)
+    rc = f(*args)
+    if rc != N.ODP_OK:
+        N.check(rc, name)
+
+
 def _stream(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+class _OnDevice:
+    """Makes a tensor's device current where it is not."""
+
+    def __init__(self, t: torch.Tensor) -> None:
+        self.ctx = None if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+    def __enter__(self) -> None:
+        if self.ctx is not None:
+            self.ctx.__enter__()
+
+    def __exit__(self, *exc) -> None:
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+
+
+def _transformed() -> bool:
+    """Whether a torch.func transform is active (the Functions with vmap rules then take the call)."""
+    return torch._C._are_functorch_transforms_active()
 
 
 def pitched_rows(t: torch.Tensor) -> torch.Tensor:
     """2-D view [rows, d] with unit column stride and a pitch of at least d;
     rows laid out otherwise (transposed, expanded) are copied."""
-    t2 = t.reshape(-1, t.shape[-1])
+    t2 = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
     if (t2.stride(1) != 1 and t2.shape[1] > 1) or t2.stride(0) < t2.shape[1]:
         t2 = t2.clone(memory_format=torch.contiguous_format)
     return t2
-
-
-def _flat_tokens(tokens: torch.Tensor) -> torch.Tensor:
-    return tokens.reshape(-1).contiguous()
 
 
 # ---------------------------------------------------------------------------
@@ -47,40 +77,65 @@ def _flat_tokens(tokens: torch.Tensor) -> torch.Tensor:
 # ---------------------------------------------------------------------------
 
 
+@functools.lru_cache(maxsize=256)
+def _grad_words(dt: int, n: int, vocab: int, width: int) -> int:
+    """float32 words of scratch of a table gradient: the sort's, then the sums'."""
+    lib = N.load()
+    return max(int(lib.odp_token_sort_scratch(n, vocab)), int(lib.odp_embed_sum_scratch(dt, n, width, 0))) // 4
+
+
 def _embed_rows(tokens: torch.Tensor, weight: torch.Tensor, scale: float) -> torch.Tensor:
     w = pitched_rows(weight.detach())
-    flat = _flat_tokens(tokens)
-    out = torch.empty((*tokens.shape, weight.shape[1]), dtype=weight.dtype, device=weight.device)
-    if out.numel():
-        with torch.cuda.device(weight.device):
-            N.call("odp_embed_rows", _stream(weight), dtype_code(w.dtype), flat.data_ptr(), flat.element_size(),
-                   flat.numel(), w.data_ptr(), w.stride(0), w.shape[0], w.shape[1], scale, out.data_ptr())
+    flat = tokens.contiguous()
+    vocab, width = weight.shape
+    out = torch.empty((*tokens.shape, width), dtype=weight.dtype, device=weight.device)
+    n = flat.numel()
+    if n:
+        with _OnDevice(weight):
+            _call("odp_embed_rows", _stream(weight), dtype_code(w.dtype), flat.data_ptr(), flat.element_size(), n,
+                  w.data_ptr(), w.stride(0), vocab, width, scale, out.data_ptr())
     return out
 
 
 def table_gradient(tokens: torch.Tensor, g: torch.Tensor, vocab: int, scale: float, padding: int) -> torch.Tensor:
     """[vocab, width] = scale times the sum of each token's rows of g (the backward of ``embedding``)."""
     rows = pitched_rows(g.detach())
-    flat = _flat_tokens(tokens)
+    flat = tokens.contiguous()
     n, width, dev = flat.numel(), g.shape[-1], g.device
+    dt = dtype_code(g.dtype)
     out = torch.empty((vocab, width), dtype=g.dtype, device=dev)
-    lib, dt = N.load(), dtype_code(g.dtype)
-    sort = int(lib.odp_token_sort_scratch(n, vocab))
-    words = max(sort, int(lib.odp_embed_sum_scratch(dt, n, width, 0))) // 4
-    ids = torch.empty((2, n), dtype=torch.int32, device=dev)
-    scratch = torch.empty(words, dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
+    words = (_grad_words(dt, n, vocab, width) + 3) // 4 * 4
+    scratch = torch.empty(words + 2 * n, dtype=torch.int32, device=dev)
+    at = scratch.data_ptr()
+    keys = at + 4 * words
+    with _OnDevice(g):
         s = _stream(g)
-        N.call("odp_token_sort", s, flat.data_ptr(), flat.element_size(), n, vocab, padding, None, None, 0,
-               scratch.data_ptr(), ids[0].data_ptr(), ids[1].data_ptr(), None)
-        N.call("odp_embed_grad", s, dt, rows.data_ptr(), rows.stride(0), n, width, ids[0].data_ptr(),
-               ids[1].data_ptr(), vocab, scale, scratch.data_ptr(), out.data_ptr())
+        _call("odp_token_sort", s, flat.data_ptr(), flat.element_size(), n, vocab, padding, None, None, 0, at, keys,
+              keys + 4 * n, None)
+        _call("odp_embed_grad", s, dt, rows.data_ptr(), rows.stride(0), n, width, keys, keys + 4 * n, vocab, scale, at,
+              out.data_ptr())
     return out
 
 
 def _front(t: torch.Tensor, d: int | None, size: int) -> torch.Tensor:
     """The vmapped axis first (a shared tensor is expanded)."""
     return t.unsqueeze(0).expand(size, *t.shape) if d is None else t.movedim(d, 0)
+
+
+class _EagerEmbed(torch.autograd.Function):
+    """scale * weight[tokens] outside torch.func."""
+
+    @staticmethod
+    def forward(ctx, tokens, weight, scale, padding):
+        ctx.save_for_backward(tokens)
+        ctx.args = weight.shape[0], scale, padding
+        return _embed_rows(tokens, weight, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        (tokens,) = ctx.saved_tensors
+        return None, table_gradient(tokens, g, *ctx.args), None, None
 
 
 class _EmbedGrad(torch.autograd.Function):
@@ -192,8 +247,12 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
     sess = active_session()
     if sess is not None and sess.mode == "discover":
         sess.uses[id(weight)] = sess.uses.get(id(weight), 0) + 1
-        return _Embed.apply(tokens, weight.detach(), float(scale), padding)
-    return _Embed.apply(tokens, weight, float(scale), padding)
+        weight = weight.detach()
+    if _transformed():
+        return _Embed.apply(tokens, weight, float(scale), padding)
+    if weight.requires_grad and torch.is_grad_enabled():
+        return _EagerEmbed.apply(tokens, weight, float(scale), padding)
+    return _embed_rows(tokens, weight, float(scale))
 
 
 class Embedding(torch.nn.Embedding):
@@ -233,90 +292,133 @@ def _head_rows(weight: torch.Tensor) -> torch.Tensor:
     return wide
 
 
+@functools.lru_cache(maxsize=256)
+def _xent_words(dt: int, n: int, width: int, vocab: int) -> tuple[int, int]:
+    """float32 words of the statistics' scratch and of dx's sums."""
+    lib = N.load()
+    return (max(int(lib.odp_xent_stats_scratch(dt, n, vocab)) // 4, 1),
+            max(int(lib.odp_xent_dx_scratch(dt, n, width)) // 4, 1))
+
+
+@functools.lru_cache(maxsize=256)
+def _xent_pitch(dt: int, columns: int) -> int:
+    return int(N.load().odp_xent_pitch(dt, columns))
+
+
 class _Packed:
     """The rows that bear a loss, gathered (every row with ``keep``)."""
 
     def __init__(self, x: torch.Tensor, w: torch.Tensor, target: torch.Tensor, ignore: int, keep: bool = False,
                  losses: torch.Tensor | None = None, lse: torch.Tensor | None = None) -> None:
-        rows, flat = pitched_rows(x.detach()), _flat_tokens(target)
+        rows, flat = pitched_rows(x.detach()), target.contiguous()
         self.dt, self.n, self.cols = dtype_code(x.dtype), flat.numel(), rows.shape[1]
         self.w, self.vocab, self.width = w, w.shape[0], w.shape[1]
-        dev = x.device
-        self.xc = torch.empty((max(self.n, 1), self.width), dtype=x.dtype, device=dev)
-        ids = torch.empty((4, max(self.n, 1)), dtype=torch.int32, device=dev)
-        self.act, self.tgt, self.where, self.count = (ids[k].data_ptr() for k in range(4))
-        self._ids = ids
-        N.call("odp_xent_rows", _stream(x), self.dt, rows.data_ptr(), rows.stride(0), self.n, self.cols, self.width,
-               flat.data_ptr(), flat.element_size(), self.vocab, ignore, int(keep), self.xc.data_ptr(), self.act,
-               self.tgt, self.where, self.count, None if losses is None else losses.data_ptr(),
-               None if lse is None else lse.data_ptr())
+        dev, room = x.device, max(self.n, 1)
+        self.xc = torch.empty((room, self.width), dtype=x.dtype, device=dev)
+        self.ids = torch.empty(3 * room + 2, dtype=torch.int32, device=dev)
+        at = self.ids.data_ptr()
+        # How many rows are packed, then (float32) how many targets are not ignored.
+        self.count, self.counted = at, at + 4
+        self.act, self.tgt, self.where = (at + 8 + 4 * k * room for k in range(3))
+        _call("odp_xent_rows", _stream(x), self.dt, rows.data_ptr(), rows.stride(0), self.n, self.cols, self.width,
+              flat.data_ptr(), flat.element_size(), self.vocab, ignore, int(keep), self.xc.data_ptr(), self.act,
+              self.tgt, self.where, self.count, None if losses is None else losses.data_ptr(),
+              None if lse is None else lse.data_ptr())
 
     def losses(self, softcap: float, losses: torch.Tensor, lse: torch.Tensor) -> None:
-        scratch = torch.empty(max(int(N.load().odp_xent_stats_scratch(self.dt, self.n, self.vocab)) // 4, 1),
-                              dtype=torch.float32, device=self.xc.device)
-        N.call("odp_xent_losses", _stream(self.xc), self.dt, self.xc.data_ptr(), self.n, self.width, self.act,
-               self.tgt, self.count, self.w.data_ptr(), self.w.stride(0), self.vocab, softcap, scratch.data_ptr(),
-               losses.data_ptr(), lse.data_ptr())
+        scratch = torch.empty(_xent_words(self.dt, self.n, self.width, self.vocab)[0], dtype=torch.float32,
+                              device=self.xc.device)
+        _call("odp_xent_losses", _stream(self.xc), self.dt, self.xc.data_ptr(), self.n, self.width, self.act,
+              self.tgt, self.count, self.w.data_ptr(), self.w.stride(0), self.vocab, softcap, scratch.data_ptr(),
+              losses.data_ptr(), lse.data_ptr())
 
-    def dlogits(self, softcap: float, lse: torch.Tensor, g: torch.Tensor, v0: int, vc: int, d: torch.Tensor) -> int:
-        """d of the columns [v0, v0 + vc) in ``d``; returns its pitch."""
-        ldd = int(N.load().odp_xent_pitch(self.dt, vc))
-        N.call("odp_xent_dlogits", _stream(self.xc), self.dt, self.xc.data_ptr(), self.n, self.width, self.act,
-               self.tgt, self.count, self.w.data_ptr(), self.w.stride(0), self.vocab, softcap, v0, vc,
-               lse.data_ptr(), g.data_ptr(), d.data_ptr(), ldd)
-        return ldd
+    def reduced(self, losses: torch.Tensor, mean: bool) -> torch.Tensor:
+        out = torch.empty((), dtype=torch.float32, device=losses.device)
+        _call("odp_xent_reduce", _stream(losses), losses.data_ptr(), self.n, self.counted if mean else None,
+              out.data_ptr())
+        return out
 
     def piece(self, whole: bool = False) -> int:
         """Columns of the vocabulary a piece of d holds."""
-        edge = int(N.load().odp_xent_pitch(self.dt, 1))
+        edge = _xent_pitch(self.dt, 1)
         fit = PIECE_BYTES // (max(self.n, 1) * self.xc.element_size()) // edge * edge
         return self.vocab if whole else min(self.vocab, max(fit, edge))
 
     def gradients(self, softcap: float, lse: torch.Tensor, g: torch.Tensor, x_shape: torch.Size | None,
-                  need_w: bool, keep_d: bool = False):
-        """(dx, dW, d): dx where ``x_shape`` is given; d [n, vocab] where ``keep_d`` (packed with ``keep``)."""
-        dev, dtype, lib = self.xc.device, self.xc.dtype, N.load()
+                  need_w: bool, keep_d: bool = False, mean: bool = False):
+        """(dx, dW, d): dx where ``x_shape`` is given; d [n, vocab] where
+        ``keep_d`` (packed with ``keep``).  ``g`` holds one gradient per row,
+        or one for all, over the number of counted targets with ``mean``."""
+        dev, dtype, dt = self.xc.device, self.xc.dtype, self.dt
         piece = self.piece(keep_d)
-        d = torch.empty((max(self.n, 1), int(lib.odp_xent_pitch(self.dt, piece))), dtype=dtype, device=dev)
+        d = torch.empty((max(self.n, 1), _xent_pitch(dt, piece)), dtype=dtype, device=dev)
         dx = dw = sums = None
         s = _stream(self.xc)
         if x_shape is not None:
             dx = torch.empty(x_shape, dtype=dtype, device=dev)
-            sums = torch.empty(max(int(lib.odp_xent_dx_scratch(self.dt, self.n, self.width)) // 4, 1),
-                               dtype=torch.float32, device=dev)
+            sums = torch.empty(_xent_words(dt, self.n, self.width, self.vocab)[1], dtype=torch.float32, device=dev)
         if need_w:
             dw = torch.empty((self.vocab, self.width), dtype=dtype, device=dev)
+        w, ldw, xc = self.w.data_ptr(), self.w.stride(0), self.xc.data_ptr()
         for v0 in range(0, self.vocab, piece):
             vc = min(piece, self.vocab - v0)
-            ldd = self.dlogits(softcap, lse, g, v0, vc, d)
+            ldd = _xent_pitch(dt, vc)
+            _call("odp_xent_dlogits", s, dt, xc, self.n, self.width, self.act, self.tgt, self.count, w, ldw,
+                  self.vocab, softcap, v0, vc, lse.data_ptr(), g.data_ptr(), 1 if g.dim() else 0,
+                  self.counted if mean else None, d.data_ptr(), ldd)
             if dx is not None:
-                N.call("odp_xent_dx", s, self.dt, self.n, self.width, self.count, self.w.data_ptr(),
-                       self.w.stride(0), self.vocab, v0, vc, piece, d.data_ptr(), ldd, sums.data_ptr())
+                _call("odp_xent_dx", s, dt, self.n, self.width, self.count, w, ldw, self.vocab, v0, vc, piece,
+                      d.data_ptr(), ldd, sums.data_ptr())
             if dw is not None:
-                N.call("odp_xent_dw", s, self.dt, self.xc.data_ptr(), self.n, self.width, self.count, vc,
-                       d.data_ptr(), ldd, dw[v0:].data_ptr(), self.width)
+                _call("odp_xent_dw", s, dt, xc, self.n, self.width, self.count, vc, d.data_ptr(), ldd,
+                      dw.data_ptr() + v0 * self.width * dw.element_size(), self.width)
         if dx is not None:
-            N.call("odp_xent_dx_rows", s, self.dt, self.n, self.cols, self.width, self.count, self.where, piece,
-                   sums.data_ptr(), dx.data_ptr())
+            _call("odp_xent_dx_rows", s, dt, self.n, self.cols, self.width, self.count, self.where, piece,
+                  sums.data_ptr(), dx.data_ptr())
         if dw is not None and self.cols != self.width:
             dw = dw[:, : self.cols].contiguous()
         return dx, dw, d[: self.n, : self.vocab] if keep_d else None
 
 
 def _xent_losses(x, weight, target, softcap, ignore):
-    losses = torch.empty(target.shape, dtype=torch.float32, device=x.device)
-    lse = torch.empty(target.shape, dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
+    losses, lse = torch.empty((2, *target.shape), dtype=torch.float32, device=x.device).unbind(0)
+    with _OnDevice(x):
         p = _Packed(x, _head_rows(weight), target, ignore, False, losses, lse)
         p.losses(softcap, losses, lse)
-    return losses, lse
+    return losses, lse, p
 
 
 def _xent_gradients(g, x, weight, target, lse, softcap, ignore, need_x, need_w, keep_d=False):
-    g, lse = g.detach().float().contiguous(), lse.contiguous()
-    with torch.cuda.device(x.device):
+    g, lse = g.detach().float().contiguous().reshape(-1), lse.contiguous()
+    with _OnDevice(x):
         p = _Packed(x, _head_rows(weight), target, ignore, keep_d)
         return p.gradients(softcap, lse, g, x.shape if need_x else None, need_w, keep_d)
+
+
+class _EagerXent(torch.autograd.Function):
+    """The reduced losses outside torch.func; the packed rows are kept for the backward."""
+
+    @staticmethod
+    def forward(ctx, x, weight, target, softcap, ignore, reduction):
+        out, lse, p = _xent_losses(x, weight, target, softcap, ignore)
+        if reduction != "none":
+            with _OnDevice(x):
+                out = p.reduced(out, reduction == "mean")
+        ctx.save_for_backward(weight)  # a later change of the head in place is an error
+        ctx.kept = p, lse, softcap, x.shape, reduction == "mean"
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        (weight,) = ctx.saved_tensors
+        p, lse, softcap, x_shape, mean = ctx.kept
+        need_x, need_w = ctx.needs_input_grad[:2]
+        if g.dim():
+            g = g.contiguous().reshape(-1)
+        with _OnDevice(weight):
+            dx, dw, _ = p.gradients(softcap, lse, g, x_shape if need_x else None, need_w, mean=mean)
+        return dx, dw, None, None, None, None
 
 
 class _XentGrad(torch.autograd.Function):
@@ -359,7 +461,7 @@ class _Xent(torch.autograd.Function):
 
     @staticmethod
     def forward(x, weight, target, softcap, ignore):
-        return _xent_losses(x, weight, target, softcap, ignore)
+        return _xent_losses(x, weight, target, softcap, ignore)[:2]
 
     @staticmethod
     def setup_context(ctx, inputs, output):
@@ -399,7 +501,7 @@ class _TapXent(torch.autograd.Function):
 
     @staticmethod
     def forward(x, weight, target, softcap, ignore, anchor, record):
-        return _xent_losses(x, weight, target, softcap, ignore)
+        return _xent_losses(x, weight, target, softcap, ignore)[:2]
 
     @staticmethod
     def setup_context(ctx, inputs, output):
@@ -453,6 +555,14 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     if sess is not None and sess.mode == "discover":
         sess.uses[id(weight)] = sess.uses.get(id(weight), 0) + 1
         weight = weight.detach()
+    if not _transformed():
+        if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+            return _EagerXent.apply(x, weight, target, float(softcap or 0.0), int(ignore_index), reduction)
+        losses, _, p = _xent_losses(x, weight, target, float(softcap or 0.0), int(ignore_index))
+        if reduction == "none":
+            return losses
+        with _OnDevice(x):
+            return p.reduced(losses, reduction == "mean")
     losses, _ = _Xent.apply(x, weight, target, float(softcap or 0.0), int(ignore_index))
     if reduction == "none":
         return losses
