@@ -596,12 +596,15 @@ int odp_embed_rows(odp_stream_t stream, int dtype, const void* tokens, int token
 /* Positions sorted by token, stable: keys[n] ascending and rows[n] the
  * positions.  Dropped positions (tokens outside the table, the token
  * `padding` (-1: none), and with segments the rows outside them) get the key
- * `vocab` and come last.  With segments row_seg[n] receives each row's index
- * into them.  scratch: odp_token_sort_scratch() bytes.                      */
+ * `vocab` and come last.  With segments seg_of[n] receives the sorted
+ * positions' indices into them.  scratch: odp_token_sort_scratch() bytes on
+ * the 16-byte grid.  zero (may be null): zero_bytes of memory that the
+ * launches zero beside their own work, such as the table gradient that the
+ * sums below write the present tokens' rows of.                             */
 int64_t odp_token_sort_scratch(int64_t n, int64_t vocab);
 int odp_token_sort(odp_stream_t stream, const void* tokens, int token_bytes, int64_t n, int64_t vocab,
                    int64_t padding, const int32_t* seg_row_start, const int32_t* seg_row_len, int32_t n_seg,
-                   void* scratch, uint32_t* keys, uint32_t* rows, int32_t* row_seg);
+                   void* scratch, uint32_t* keys, uint32_t* rows, int32_t* seg_of, void* zero, int64_t zero_bytes);
 
 /* Bytes of the scratch of the sums below (second: with second moments), and
  * the partial slots per row of a segment that odp_embed_sqnorm writes.      */
@@ -609,7 +612,8 @@ int64_t odp_embed_sum_scratch(int dtype, int64_t n, int64_t width, int second);
 int64_t odp_embed_pieces(int dtype, int64_t width);
 
 /* out [vocab][width] (of g's dtype) = scale times the sum of each token's
- * rows of g, in float32 and rounded once; zero rows for absent tokens.      */
+ * rows of g, in float32 and rounded once.  Absent tokens' rows are not
+ * written: zero them first (odp_token_sort's zero).                         */
 int odp_embed_grad(odp_stream_t stream, int dtype, const void* g, int64_t ldg, int64_t n, int64_t width,
                    const uint32_t* keys, const uint32_t* rows, int64_t vocab, float scale, void* scratch, void* out);
 
@@ -621,16 +625,17 @@ int odp_embed_grad(odp_stream_t stream, int dtype, const void* g, int64_t ldg, i
  * (zero them first).  whole: half of odp_embed_sum_scratch(.., 0) bytes, kept
  * for odp_embed_clipped_sum.                                                */
 int odp_embed_sqnorm(odp_stream_t stream, int dtype, const void* g, int64_t ldg, int64_t n, int64_t width,
-                     const uint32_t* keys, const uint32_t* rows, const int32_t* row_seg, int64_t vocab, float scale,
+                     const uint32_t* keys, const uint32_t* rows, const int32_t* seg_of, int64_t vocab, float scale,
                      const int32_t* seg_row_start, const int32_t* seg_example, void* scratch, float* whole,
                      double* part, int64_t part_stride, int64_t slot, int64_t* nf_flag);
 
 /* out [vocab][width] = sum over examples of scales[example] S, over
  * normalize_by, in float32 and rounded once to out_dtype; out2 (may be null)
  * the sum of the squares of the scaled S.  After odp_embed_sqnorm on the same
- * inputs.                                                                   */
+ * inputs.  Absent tokens' rows of out are not written (zero them first); out2
+ * is zeroed here.                                                           */
 int odp_embed_clipped_sum(odp_stream_t stream, int dtype, const void* g, int64_t ldg, int64_t n, int64_t width,
-                          const uint32_t* keys, const uint32_t* rows, const int32_t* row_seg, int64_t vocab,
+                          const uint32_t* keys, const uint32_t* rows, const int32_t* seg_of, int64_t vocab,
                           float scale, const int32_t* seg_example, void* scratch, const float* whole,
                           const double* scales, float normalize_by, int out_dtype, void* out, void* out2);
 

@@ -126,7 +126,7 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "odp_embed_rows": (_c_int, [_ptr, _c_int, _ptr, _c_int, _c_i64, _ptr, _c_i64, _c_i64, _c_i64, _c_f32, _ptr]),
     "odp_token_sort_scratch": (_c_i64, [_c_i64, _c_i64]),
     "odp_token_sort": (
-        _c_int, [_ptr, _ptr, _c_int, _c_i64, _c_i64, _c_i64, _ptr, _ptr, _c_i32, _ptr, _ptr, _ptr, _ptr]),
+        _c_int, [_ptr, _ptr, _c_int, _c_i64, _c_i64, _c_i64, _ptr, _ptr, _c_i32, _ptr, _ptr, _ptr, _ptr, _ptr, _c_i64]),
     "odp_embed_sum_scratch": (_c_i64, [_c_int, _c_i64, _c_i64, _c_int]),
     "odp_embed_pieces": (_c_i64, [_c_int, _c_i64]),
     "odp_embed_grad": (

@@ -21,12 +21,13 @@
 namespace {
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
-constexpr int EM_WIN = 32;   // sorted positions per window
+constexpr int EM_WIN = 32;   // sorted positions per window, at most
 constexpr int EM_LOAD = 8;   // rows in flight per wave
 constexpr int EM_WAVES = 4;  // waves per workgroup
 
-enum { EM_GRAD = 0, EM_NORM = 1, EM_CLIP = 2 };
+enum { EM_GRAD = 0, EM_NORM = 1, EM_CLIP = 2, EM_CLIP2 = 3 };  // CLIP2: with second moments
 
 __device__ __forceinline__ int uniform_int(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
@@ -43,8 +44,12 @@ __device__ __forceinline__ int em_col(int cb, int i) {
   return cb * 64 * V + (AL ? lane * V + i : lane + 64 * i);
 }
 
-// Reads the lane's values of the row at p as 16 raw bytes or as floats.
-template <int DT, bool AL>
+// The lane's 16 bytes of a row piece.  NT: a non-temporal load, for gradient
+// rows, which a pass reads once (32768 x 4096 bfloat16: 85 us, 125 through the
+// caches; the two passes of a clip step over 16384 x 4096: 71 us, 90); table
+// rows, of which frequent tokens' come again, are read through the caches
+// (66 us, 97).
+template <int DT, bool AL, bool NT = false>
 struct EmPiece {
   static constexpr int V = em_vec<DT>();
   u32x4_t w;
@@ -52,9 +57,9 @@ struct EmPiece {
     if constexpr (AL) {
       const int c = em_col<DT, AL>(cb, 0);
       w = u32x4_t{0, 0, 0, 0};
-      if (c < width)
-        w = __builtin_nontemporal_load(
-            (const ODP_GMEM u32x4_t*)(const ODP_GMEM void*)(p + (int64_t)c * (DT == ODP_DTYPE_F32 ? 4 : 2)));
+      const ODP_GMEM u32x4_t* src =
+          (const ODP_GMEM u32x4_t*)(const ODP_GMEM void*)(p + (int64_t)c * (DT == ODP_DTYPE_F32 ? 4 : 2));
+      if (c < width) w = NT ? __builtin_nontemporal_load(src) : *src;
     } else {
       uint32_t h[V];
 #pragma unroll
@@ -119,34 +124,45 @@ __device__ __forceinline__ int64_t token_at(const void* tokens, int wide, int64_
 }
 
 // ---------------------------------------------------------------------------
-// Lookup.  One wave per (row, 64 pieces of 16 bytes); a token outside the
-// table gives a row of NaN.
+// Lookup.  A wave takes EM_ITEMS (row, 64 pieces of 16 bytes) items, their
+// loads in flight together; a token outside the table gives a row of NaN.
 // ---------------------------------------------------------------------------
+constexpr int EM_ITEMS = 4;
 template <int DT, bool AL>
 __global__ __launch_bounds__(64 * EM_WAVES) void k_embed_rows(const void* __restrict__ tokens, int wide, int64_t n,
                                                               const char* __restrict__ weight, int64_t ldw,
                                                               int64_t vocab, int width, int ncb, float scale,
                                                               void* __restrict__ out) {
-  const int64_t item = (int64_t)blockIdx.x * EM_WAVES + uniform_int(threadIdx.x >> 6);
-  const int64_t row = item / ncb;
-  const int cb = (int)(item - row * ncb);
-  if (row >= n) return;
-  const int64_t t = token_at(tokens, wide, row);
   constexpr int V = em_vec<DT>();
-  float v[V];
-  if (t >= 0 && t < vocab) {
-    EmPiece<DT, AL> p;
-    p.load(weight + t * ldw * (DT == ODP_DTYPE_F32 ? 4 : 2), cb, width);
-    p.get(v);
-    if (scale != 1.0f) {
+  const int64_t first = ((int64_t)blockIdx.x * EM_WAVES + uniform_int(threadIdx.x >> 6)) * EM_ITEMS;
+  EmPiece<DT, AL> p[EM_ITEMS];
+  int64_t row[EM_ITEMS];
+  int cb[EM_ITEMS];
+  bool ok[EM_ITEMS];
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = __fmul_rn(v[i], scale);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = __uint_as_float(0x7fc00000u);
+  for (int q = 0; q < EM_ITEMS; ++q) {
+    row[q] = (first + q) / ncb;
+    cb[q] = (int)(first + q - row[q] * ncb);
+    const int64_t t = row[q] < n ? token_at(tokens, wide, row[q]) : -1;
+    ok[q] = t >= 0 && t < vocab;
+    if (ok[q]) p[q].load(weight + t * ldw * (DT == ODP_DTYPE_F32 ? 4 : 2), cb[q], width);
   }
-  em_store<DT, AL>(out, DT, row, width, cb, v);
+#pragma unroll
+  for (int q = 0; q < EM_ITEMS; ++q) {
+    if (row[q] >= n) return;
+    float v[V];
+    if (ok[q]) {
+      p[q].get(v);
+      if (scale != 1.0f) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = __fmul_rn(v[i], scale);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = __uint_as_float(0x7fc00000u);
+    }
+    em_store<DT, AL>(out, DT, row[q], width, cb[q], v);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -158,9 +174,36 @@ __global__ __launch_bounds__(64 * EM_WAVES) void k_embed_rows(const void* __rest
 // outside every segment) get the key `vocab` and end up last.
 // ---------------------------------------------------------------------------
 constexpr int SORT_BITS = 9, SORT_BINS = 1 << SORT_BITS;
-constexpr int SORT_KEYS = 512;                            // positions per wave
+constexpr int SORT_KEYS = 512;                            // positions a wave holds at a time
+constexpr int SORT_NW = 128;                              // waves of the other, at most
 constexpr int SORT_WAVES = 16;                            // waves of the one-workgroup sort
 constexpr int64_t SORT_SMALL = SORT_WAVES * SORT_KEYS;    // positions it takes
+constexpr int SORT_SEGS = 1024;                           // segments it keeps in LDS
+
+// Memory that the sort's launches zero beside their own work, with
+// workgroups the sort leaves idle: pieces [first, first + count) of
+// ZERO_BYTES of 16 bytes a thread, one after the other in address order (a
+// table of 1.05 GB: 152 us, 6.9 TB/s; with 1024 to 16384 workgroups striding
+// over it 195-280 us).
+struct ZeroShare {
+  char* at;
+  int64_t bytes;
+  int64_t first, count;
+  int per;  // pieces a workgroup
+};
+
+__device__ __forceinline__ void zero_pieces(const ZeroShare& z, int64_t wg) {
+  const int64_t size = (int64_t)blockDim.x * 16;
+  for (int q = 0; q < z.per; ++q) {
+    const int64_t p = wg * z.per + q;
+    if (p >= z.count) return;
+    const int64_t b = (z.first + p) * size + 16 * (int64_t)threadIdx.x;
+    if (b + 16 <= z.bytes && ((uintptr_t)z.at & 15) == 0)
+      odp_gstore((u32x4_t*)(z.at + b), u32x4_t{0, 0, 0, 0});
+    else
+      for (int64_t i = b; i < b + 16 && i < z.bytes; ++i) z.at[i] = 0;
+  }
+}
 
 struct SortIn {
   const void* tokens;
@@ -169,43 +212,60 @@ struct SortIn {
   const int32_t* sstart;  // segments (nullptr: every row counts)
   const int32_t* slen;
   int n_seg;
-  int32_t* row_seg;  // [n] each row's segment, written in the first pass (with segments)
+  int32_t* row_seg;  // [n] each row's segment, written when the keys are counted first (with segments)
+  int32_t* seg_of;   // [n] the sorted positions' segments, written in the last (with segments)
+  ZeroShare zero;
 };
 
-__device__ __forceinline__ uint32_t sort_key(const SortIn& a, int64_t i, bool record) {
+// `starts`: the segments' starts, in LDS where they fit.
+__device__ __forceinline__ uint32_t sort_key(const SortIn& a, const int32_t* starts, int64_t i, bool record) {
   const int64_t t = token_at(a.tokens, a.wide, i);
   bool ok = t >= 0 && t < a.vocab && t != a.padding;
   if (a.sstart != nullptr) {
     int lo = 0, hi = a.n_seg - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if ((int64_t)a.sstart[mid] <= i) lo = mid; else hi = mid - 1;
+      if ((int64_t)starts[mid] <= i) lo = mid; else hi = mid - 1;
     }
-    const bool in = a.n_seg > 0 && i >= a.sstart[lo] && i < (int64_t)a.sstart[lo] + a.slen[lo];
+    const bool in = a.n_seg > 0 && i >= starts[lo] && i < (int64_t)starts[lo] + a.slen[lo];
     ok = ok && in;
     if (record) a.row_seg[i] = in ? lo : 0;
   }
   return ok ? (uint32_t)t : (uint32_t)a.vocab;
 }
 
-// Adds the digits of positions [lo, hi) to the wave's counts h.
-template <typename Key>
-__device__ __forceinline__ void sort_count(uint32_t* h, int64_t lo, int64_t hi, int shift, uint32_t mask, Key key) {
-  for (int64_t i = lo + (threadIdx.x & 63); i < hi; i += 64) atomicAdd(&h[(key(i) >> shift) & mask], 1u);
+// Positions [lo, hi), at most 64 R, in the wave's registers: all loads in flight together.
+template <int R, typename Key>
+__device__ __forceinline__ void sort_load(uint32_t (&v)[R], int64_t lo, int64_t hi, Key key) {
+#pragma unroll
+  for (int q = 0; q < R; ++q) {
+    const int64_t i = lo + 64 * q + (threadIdx.x & 63);
+    v[q] = i < hi ? key(i) : 0u;
+  }
 }
 
-// Sends positions [lo, hi) to where the wave's h says, in order.
-template <typename Key, typename Row>
-__device__ __forceinline__ void sort_scatter(uint32_t* h, int64_t lo, int64_t hi, int shift, int bits, Key key,
-                                             Row row, uint32_t* ok, uint32_t* orow) {
+// Adds the digits of the wave's keys to its counts h.
+template <int R>
+__device__ __forceinline__ void sort_count(uint32_t* h, int64_t lo, int64_t hi, int shift, uint32_t mask,
+                                           const uint32_t (&key)[R]) {
+#pragma unroll
+  for (int q = 0; q < R; ++q)
+    if (lo + 64 * q + (threadIdx.x & 63) < hi) atomicAdd(&h[(key[q] >> shift) & mask], 1u);
+}
+
+// Sends them to where h says, in order.
+template <int R>
+__device__ __forceinline__ void sort_scatter(uint32_t* h, int64_t lo, int64_t hi, int shift, int bits,
+                                             const uint32_t (&key)[R], const uint32_t (&row)[R],
+                                             uint32_t* ok, uint32_t* orow, const int32_t* row_seg, int32_t* seg_of) {
   const int lane = threadIdx.x & 63;
   const uint64_t before = (1ull << lane) - 1;
-  for (int64_t i0 = lo; i0 < hi; i0 += 64) {
-    const int64_t i = i0 + lane;
-    const bool on = i < hi;
-    const uint32_t k = on ? key(i) : 0u, r = on ? row(i) : 0u;
-    const uint32_t d = (k >> shift) & ((1u << bits) - 1);
+#pragma unroll
+  for (int q = 0; q < R; ++q) {
+    const bool on = lo + 64 * q + lane < hi;
+    const uint32_t k = key[q], d = (k >> shift) & ((1u << bits) - 1);
     uint64_t peers = __builtin_amdgcn_ballot_w64(on);
+    if (peers == 0) break;
     for (int b = 0; b < bits; ++b) {
       const bool set = (d >> b) & 1u;
       const uint64_t m = __builtin_amdgcn_ballot_w64(on && set);
@@ -221,7 +281,8 @@ __device__ __forceinline__ void sort_scatter(uint32_t* h, int64_t lo, int64_t hi
     if (on) {
       const uint32_t to = base + (uint32_t)__popcll(peers & before);
       ok[to] = k;
-      orow[to] = r;
+      orow[to] = row[q];
+      if (seg_of != nullptr) seg_of[to] = row_seg[row[q]];
     }
   }
 }
@@ -252,10 +313,20 @@ __device__ __forceinline__ uint32_t block_exclusive(uint32_t v, int nw, uint32_t
 
 // The whole sort in one workgroup (n <= SORT_SMALL): one launch instead of
 // three per pass.
+template <int R>
 __global__ __launch_bounds__(64 * SORT_WAVES) void k_sort_small(SortIn a, int passes, int bits, uint32_t* k0,
                                                                 uint32_t* r0, uint32_t* k1, uint32_t* r1) {
   __shared__ uint32_t hist[SORT_WAVES][SORT_BINS];
   __shared__ uint32_t red[SORT_WAVES];
+  if (blockIdx.x > 0) {
+    zero_pieces(a.zero, blockIdx.x - 1);
+    return;
+  }
+  __shared__ int32_t seg_start[SORT_SEGS];
+  const bool kept = a.sstart != nullptr && a.n_seg <= SORT_SEGS;
+  if (kept)
+    for (int i = threadIdx.x; i < a.n_seg; i += blockDim.x) seg_start[i] = a.sstart[i];
+  const int32_t* starts = kept ? seg_start : a.sstart;
   const int wave = threadIdx.x >> 6, bins = 1 << bits;
   const int64_t per = (a.n + SORT_WAVES * 64 - 1) / (SORT_WAVES * 64) * 64;
   const int64_t lo = min(a.n, wave * per), hi = min(a.n, lo + per);
@@ -269,13 +340,12 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void k_sort_small(SortIn a, int pa
     const uint32_t* ir = to0 ? r1 : r0;
     uint32_t* ok = to0 ? k0 : k1;
     uint32_t* orow = to0 ? r0 : r1;
-    auto key = [&](int64_t i) { return p == 0 ? sort_key(a, i, false) : ik[i]; };
-    auto row = [&](int64_t i) {
-      if (p > 0) return ir[i];
-      if (a.sstart != nullptr) sort_key(a, i, true);
-      return (uint32_t)i;
-    };
-    sort_count(hist[wave], lo, hi, shift, (uint32_t)bins - 1, key);
+    // The wave's positions in rounds of 64 R, their loads in flight together.
+    uint32_t key[R], row[R];
+    for (int64_t c = lo; c < hi; c += 64 * R) {
+      sort_load(key, c, hi, [&](int64_t i) { return p == 0 ? sort_key(a, starts, i, a.sstart != nullptr) : ik[i]; });
+      sort_count(hist[wave], c, hi, shift, (uint32_t)bins - 1, key);
+    }
     __syncthreads();
     // Exclusive sums over (digit, wave): thread d takes digit d.
     uint32_t mine = 0;
@@ -290,70 +360,91 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void k_sort_small(SortIn a, int pa
         at += c;
       }
     __syncthreads();
-    sort_scatter(hist[wave], lo, hi, shift, bits, key, row, ok, orow);
+    for (int64_t c = lo; c < hi; c += 64 * R) {
+      sort_load(key, c, hi, [&](int64_t i) { return p == 0 ? sort_key(a, starts, i, false) : ik[i]; });
+      sort_load(row, c, hi, [&](int64_t i) { return p == 0 ? (uint32_t)i : ir[i]; });
+      sort_scatter(hist[wave], c, hi, shift, bits, key, row, ok, orow, a.row_seg,
+                   p == passes - 1 ? a.seg_of : nullptr);
+    }
     __threadfence_block();
     __syncthreads();
   }
 }
 
-// counts[digit][wave of the launch].
+// The sort of more positions: per pass a launch that counts, counts[wave][digit],
+// and one that sums the counts and scatters.
 __global__ __launch_bounds__(64 * EM_WAVES) void k_sort_count(SortIn a, const uint32_t* ik, int first, int shift,
-                                                              int bits, uint32_t* counts, int nw) {
+                                                              int bits, uint32_t* counts, int nw, int64_t per) {
   __shared__ uint32_t hist[EM_WAVES][SORT_BINS];
+  const int own = (nw + EM_WAVES - 1) / EM_WAVES;
+  if ((int)blockIdx.x >= own) {
+    zero_pieces(a.zero, blockIdx.x - own);
+    return;
+  }
   const int wave = threadIdx.x >> 6, bins = 1 << bits;
   for (int i = threadIdx.x; i < EM_WAVES * SORT_BINS; i += blockDim.x) (&hist[0][0])[i] = 0;
   __syncthreads();
-  const int64_t w = (int64_t)blockIdx.x * EM_WAVES + wave;
-  const int64_t lo = min(a.n, w * SORT_KEYS), hi = min(a.n, lo + SORT_KEYS);
-  sort_count(hist[wave], lo, hi, shift, (uint32_t)bins - 1,
-             [&](int64_t i) { return first ? sort_key(a, i, false) : ik[i]; });
-  __syncthreads();
-  if (w < nw)
-    for (int d = threadIdx.x & 63; d < bins; d += 64) counts[(int64_t)d * nw + w] = hist[wave][d];
-}
-
-// Exclusive sums of counts in place, one workgroup.
-__global__ __launch_bounds__(1024) void k_sort_scan(uint32_t* counts, int64_t n) {
-  __shared__ uint32_t red[16];
-  uint32_t carry = 0;
-  for (int64_t i0 = 0; i0 < n; i0 += 4096) {
-    uint32_t v[4], s = 0;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int64_t i = i0 + 4 * threadIdx.x + q;
-      v[q] = i < n ? counts[i] : 0u;
-      s += v[q];
-    }
-    uint32_t total;
-    uint32_t at = carry + block_exclusive(s, 16, red, total);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int64_t i = i0 + 4 * threadIdx.x + q;
-      if (i < n) counts[i] = at;
-      at += v[q];
-    }
-    carry += total;
+  const int w = blockIdx.x * EM_WAVES + wave;
+  const int64_t lo = min(a.n, w * per), hi = min(a.n, lo + per);
+  for (int64_t c = lo; c < hi; c += SORT_KEYS) {
+    uint32_t key[SORT_KEYS / 64];
+    sort_load(key, c, hi, [&](int64_t i) { return first ? sort_key(a, a.sstart, i, a.sstart != nullptr) : ik[i]; });
+    sort_count(hist[wave], c, hi, shift, (uint32_t)bins - 1, key);
   }
+  if (w < nw)
+    for (int d = threadIdx.x & 63; d < bins; d += 64) counts[(int64_t)w * SORT_BINS + d] = hist[wave][d];
 }
 
 __global__ __launch_bounds__(64 * EM_WAVES) void k_sort_scatter(SortIn a, const uint32_t* ik, const uint32_t* ir,
                                                                 int first, int shift, int bits,
-                                                                const uint32_t* counts, int nw, uint32_t* ok,
-                                                                uint32_t* orow) {
+                                                                const uint32_t* counts, int nw, int64_t per,
+                                                                uint32_t* ok, uint32_t* orow, int last) {
   __shared__ uint32_t hist[EM_WAVES][SORT_BINS];
-  const int wave = threadIdx.x >> 6, bins = 1 << bits;
-  const int64_t w = (int64_t)blockIdx.x * EM_WAVES + wave;
-  if (w < nw)
-    for (int d = threadIdx.x & 63; d < bins; d += 64) hist[wave][d] = counts[(int64_t)d * nw + w];
+  __shared__ uint32_t red[EM_WAVES];
+  const int own = (nw + EM_WAVES - 1) / EM_WAVES;
+  if ((int)blockIdx.x >= own) {
+    zero_pieces(a.zero, blockIdx.x - own);
+    return;
+  }
+  const int wave = threadIdx.x >> 6;
+  const int w0 = blockIdx.x * EM_WAVES;
+  static_assert(SORT_BINS == 2 * 64 * EM_WAVES, "two digits a thread");
+  // Where this workgroup's waves' keys of digits 2 t and 2 t + 1 go: after
+  // every smaller digit's and the earlier waves' of the same (digits past
+  // the pass's have no counts: they are not read).
+  const bool on = 2 * (int)threadIdx.x < (1 << bits);
+  u32x2_t all = {0, 0}, before = {0, 0}, mine[EM_WAVES];
+#pragma unroll
+  for (int j = 0; j < EM_WAVES; ++j) mine[j] = u32x2_t{0, 0};
+  if (on) {
+    const u32x2_t* at = (const u32x2_t*)counts + threadIdx.x;
+#pragma unroll 16
+    for (int w = 0; w < nw; ++w) {
+      const u32x2_t c = at[(int64_t)w * (SORT_BINS / 2)];
+      all = all + c;
+      if (w < w0) before = before + c;
+    }
+#pragma unroll
+    for (int j = 0; j < EM_WAVES; ++j)
+      if (w0 + j < nw) mine[j] = at[(int64_t)(w0 + j) * (SORT_BINS / 2)];
+  }
+  uint32_t total;
+  const uint32_t below = block_exclusive(all[0] + all[1], EM_WAVES, red, total);
+  u32x2_t to = {below + before[0], below + all[0] + before[1]};
+#pragma unroll
+  for (int j = 0; j < EM_WAVES; ++j) {
+    hist[j][2 * threadIdx.x] = to[0];
+    hist[j][2 * threadIdx.x + 1] = to[1];
+    to = to + mine[j];
+  }
   __syncthreads();
-  const int64_t lo = min(a.n, w * SORT_KEYS), hi = min(a.n, lo + SORT_KEYS);
-  sort_scatter(hist[wave], lo, hi, shift, bits, [&](int64_t i) { return first ? sort_key(a, i, false) : ik[i]; },
-               [&](int64_t i) {
-                 if (!first) return ir[i];
-                 if (a.sstart != nullptr) sort_key(a, i, true);
-                 return (uint32_t)i;
-               },
-               ok, orow);
+  const int64_t lo = min(a.n, (w0 + wave) * per), hi = min(a.n, lo + per);
+  for (int64_t c = lo; c < hi; c += SORT_KEYS) {
+    uint32_t key[SORT_KEYS / 64], row[SORT_KEYS / 64];
+    sort_load(key, c, hi, [&](int64_t i) { return first ? sort_key(a, a.sstart, i, false) : ik[i]; });
+    sort_load(row, c, hi, [&](int64_t i) { return first ? (uint32_t)i : ir[i]; });
+    sort_scatter(hist[wave], c, hi, shift, bits, key, row, ok, orow, a.row_seg, last ? a.seg_of : nullptr);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -363,10 +454,12 @@ struct EmbedSum {
   const char* g;  // gradient rows
   int64_t ldg;    // elements
   int64_t n;
+  int win;      // sorted positions per window: 8, 16 or 32
+  int grouped;  // whether k_embed_group has run
   int width, ncb;
   const uint32_t* keys;   // sorted tokens, `vocab` for dropped positions
   const uint32_t* rows;   // the positions, sorted
-  const int32_t* row_seg;  // NORM, CLIP: segment of each row
+  const int32_t* seg_of;  // NORM, CLIP: the sorted positions' segments
   uint32_t vocab;
   float scale;
   float* ws;     // [windows][2][width] partials of runs that cross windows
@@ -413,6 +506,45 @@ __device__ __forceinline__ void em_add(const float* p, float (&v)[V]) {
   }
 }
 
+// Adds slot `slot` of windows first, first + step, .. last, JOIN_LOAD rows in flight.
+constexpr int JOIN_LOAD = 8, JOIN_GROUP = 16;
+template <int DT>
+__device__ __forceinline__ void em_gather(const float* ws, int64_t first, int64_t last, int step, int slot,
+                                          const EmbedSum& a, int cb, float (&v)[em_vec<DT>()]) {
+  constexpr int V = em_vec<DT>();
+  for (int64_t w = first; w <= last; w += JOIN_LOAD * step) {
+    f32x4_t x[JOIN_LOAD][V / 4];
+#pragma unroll
+    for (int k = 0; k < JOIN_LOAD; ++k)
+#pragma unroll
+      for (int i = 0; i < V / 4; ++i)
+        if (w + k * step <= last)
+          x[k][i] = *(const ODP_GMEM f32x4_t*)(const ODP_GMEM void*)(em_ws<DT>((float*)ws, 2 * (w + k * step) + slot,
+                                                                               a, cb) +
+                                                                     4 * i);
+#pragma unroll
+    for (int k = 0; k < JOIN_LOAD; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (w + k * step <= last) v[i] += x[k][i / 4][i % 4];
+  }
+}
+
+// Adds the partials of windows first .. last of a run that ends in `last`,
+// whole groups by their sums (a.grouped).
+template <int DT>
+__device__ __forceinline__ void em_join(const float* ws, int64_t first, int64_t last, const EmbedSum& a, int cb,
+                                        float (&v)[em_vec<DT>()]) {
+  const int64_t g0 = (first + JOIN_GROUP - 1) / JOIN_GROUP * JOIN_GROUP, g1 = last / JOIN_GROUP * JOIN_GROUP;
+  if (!a.grouped || g0 >= g1) {
+    em_gather<DT>(ws, first, last, 1, 0, a, cb, v);
+    return;
+  }
+  em_gather<DT>(ws, first, g0 - 1, 1, 0, a, cb, v);
+  em_gather<DT>(ws, g0, g1 - 1, JOIN_GROUP, 1, a, cb, v);  // windows before g1 lie wholly inside the run
+  em_gather<DT>(ws, g1, last, 1, 0, a, cb, v);
+}
+
 // An (example, token) run's S is complete: its squares go to the partial of
 // its first row and this piece.
 template <int DT>
@@ -427,8 +559,8 @@ __device__ __forceinline__ void em_norm(const EmbedSum& a, uint32_t head_row, in
     bad |= !fin;
     if (fin) s += (double)__fmul_rn(x, x);
   }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off);
+  // Across the lanes on the VALU: a window may close a run at every position.
+  s = rows_sum4(row_sum16(s));
   const uint64_t any = __builtin_amdgcn_ballot_w64(bad);
   if ((threadIdx.x & 63) == 0) {
     a.part[(int64_t)a.sex[seg] * a.part_stride + a.slot + ((int64_t)head_row - a.sstart[seg]) * a.ncb + cb] = s;
@@ -449,7 +581,7 @@ __device__ __forceinline__ void em_finish(const EmbedSum& a, int mode, uint32_t 
     for (int i = 0; i < V; ++i) v[i] = __fdiv_rn(v[i], a.normalize_by);
   }
   em_store<DT, AL>(a.out, a.odt, key, a.width, cb, v);
-  if (mode == EM_CLIP && a.out2 != nullptr) {
+  if (mode == EM_CLIP2) {
     if (a.normalize_by != 1.0f) {
 #pragma unroll
       for (int i = 0; i < V; ++i) q[i] = __fdiv_rn(q[i], a.normalize_by);
@@ -464,37 +596,34 @@ __global__ __launch_bounds__(64 * EM_WAVES) void k_embed_sum(EmbedSum a) {
   constexpr int V = em_vec<DT>(), ES = DT == ODP_DTYPE_F32 ? 4 : 2;
   const int lane = threadIdx.x & 63;
   const int64_t item = (int64_t)blockIdx.x * EM_WAVES + uniform_int(threadIdx.x >> 6);
-  const int64_t win = item / a.ncb, p0 = win * EM_WIN;
+  const int64_t win = item / a.ncb, p0 = win * a.win;
   const int cb = (int)(item - win * a.ncb);
   if (p0 >= a.n) return;
   // Lane l holds position p0 - 1 + l: the window, the one before and the one after.
   const int64_t pos = p0 - 1 + lane;
-  const bool in = pos >= 0 && pos < a.n && lane <= EM_WIN + 1;
+  const bool in = pos >= 0 && pos < a.n && lane <= a.win + 1;
   const uint32_t key = in ? a.keys[pos] : a.vocab;
   const uint32_t row = in ? a.rows[pos] : 0u;
-  int seg = 0;
+  const int seg = MODE != EM_GRAD && in ? a.seg_of[pos] : 0;
   float c = 0.f;
-  if (MODE != EM_GRAD && key != a.vocab) {
-    seg = a.row_seg[row];
-    if (MODE == EM_CLIP) c = (float)a.scales[a.sex[seg]];
-  }
+  if (MODE >= EM_CLIP && key != a.vocab) c = (float)a.scales[a.sex[seg]];
   const uint32_t pkey = __shfl_up(key, 1);
   const int pseg = __shfl_up(seg, 1);
   // Bit p: position p0 + p counts / starts a token's run / an (example, token)
-  // run (bit EM_WIN: the position after the window).
+  // run (bit a.win: the position after the window).
   const bool live_l = key != a.vocab && lane >= 1;
   const uint64_t live = __builtin_amdgcn_ballot_w64(live_l) >> 1;
   const uint64_t tok = __builtin_amdgcn_ballot_w64(live_l && key != pkey) >> 1;
   const uint64_t sub = MODE == EM_GRAD ? tok : __builtin_amdgcn_ballot_w64(live_l && (key != pkey || seg != pseg)) >> 1;
-  const int n_live = __popcll(live & ((1ull << EM_WIN) - 1));  // dropped positions come last
+  const int n_live = __popcll(live & ((1ull << a.win) - 1));  // dropped positions come last
   if (n_live == 0) return;
-  const bool more = (live >> EM_WIN) & 1;
-  const bool tok_on = more && !((tok >> EM_WIN) & 1);  // the last run goes on in the next window
-  const bool sub_on = more && !((sub >> EM_WIN) & 1);
+  const bool more = (live >> a.win) & 1;
+  const bool tok_on = more && !((tok >> a.win) & 1);  // the last run goes on in the next window
+  const bool sub_on = more && !((sub >> a.win) & 1);
   // Rows of (example, token) runs that cross windows were added by the NORM
   // pass: CLIP takes their sum from `whole` at the run's first window.
   int from = 0, to = n_live;
-  if (MODE == EM_CLIP) {
+  if (MODE >= EM_CLIP) {
     const uint64_t heads = sub & ((1ull << n_live) - 1);
     from = heads ? __builtin_ctzll(heads) : n_live;
     if (sub_on && heads) to = 63 - __builtin_clzll(heads);
@@ -517,7 +646,7 @@ __global__ __launch_bounds__(64 * EM_WAVES) void k_embed_sum(EmbedSum a) {
     } else {
       const int64_t slot = 2 * win + (began ? 1 : 0);
       em_put(em_ws<DT>(a.ws, slot, a, cb), v);
-      if (MODE == EM_CLIP && a.out2 != nullptr) em_put(em_ws<DT>(a.ws_sq, slot, a, cb), acc2);
+      if (MODE == EM_CLIP2) em_put(em_ws<DT>(a.ws_sq, slot, a, cb), acc2);
     }
     em_clear(v);
     em_clear(acc2);
@@ -539,12 +668,12 @@ __global__ __launch_bounds__(64 * EM_WAVES) void k_embed_sum(EmbedSum a) {
         float x = __fmul_rn(sum[i], a.scale);
         x = isfinite(x) ? __fmul_rn(f, x) : 0.f;
         acc[i] += x;
-        acc2[i] = __builtin_fmaf(x, x, acc2[i]);
+        if (MODE == EM_CLIP2) acc2[i] = __builtin_fmaf(x, x, acc2[i]);
       }
     }
     em_clear(sum);
   };
-  EmPiece<DT, AL> piece[EM_LOAD];
+  EmPiece<DT, AL, true> piece[EM_LOAD];
   for (int b = 0; b < n_live; b += EM_LOAD) {
 #pragma unroll
     for (int q = 0; q < EM_LOAD; ++q) {
@@ -571,27 +700,49 @@ __global__ __launch_bounds__(64 * EM_WAVES) void k_embed_sum(EmbedSum a) {
   }
 }
 
-// Adds the partials of a run that begins in window `win` and crosses into the
-// next ones: one workgroup per (window, 64 pieces), whose waves take the
-// windows in turn.
+// Runs of hundreds of windows (a padding token's) are joined in two steps:
+// first, the partials of every JOIN_GROUP windows that lie wholly inside a
+// run, into the group's first window's second slot (unused there).
+template <int DT, int MODE>
+__global__ __launch_bounds__(64 * EM_WAVES) void k_embed_group(EmbedSum a) {
+  constexpr int V = em_vec<DT>();
+  const int64_t item = (int64_t)blockIdx.x * EM_WAVES + uniform_int(threadIdx.x >> 6);
+  const int64_t group = item / a.ncb, win = group * JOIN_GROUP;
+  const int cb = (int)(item - group * a.ncb);
+  const int64_t first = win * a.win, last = first + JOIN_GROUP * a.win - 1;
+  if (win == 0 || last >= a.n) return;
+  const uint32_t key = a.keys[first];
+  if (key == a.vocab || a.keys[first - 1] != key || a.keys[last] != key) return;
+  if (MODE == EM_NORM && (a.seg_of[first - 1] != a.seg_of[first] || a.seg_of[last] != a.seg_of[first])) return;
+  float v[V];
+  em_clear(v);
+  em_gather<DT>(a.ws, win, win + JOIN_GROUP - 1, 1, 0, a, cb, v);
+  em_put(em_ws<DT>(a.ws, 2 * win + 1, a, cb), v);
+  if (MODE == EM_CLIP2) {
+    em_clear(v);
+    em_gather<DT>(a.ws_sq, win, win + JOIN_GROUP - 1, 1, 0, a, cb, v);
+    em_put(em_ws<DT>(a.ws_sq, 2 * win + 1, a, cb), v);
+  }
+}
+
+// Adds the partials of a run that begins in a window and crosses into the
+// next ones, one wave per (window, 64 pieces).
 template <int DT, bool AL, int MODE>
 __global__ __launch_bounds__(64 * EM_WAVES) void k_embed_join(EmbedSum a) {
   constexpr int V = em_vec<DT>();
-  const int64_t win = blockIdx.x / a.ncb;
-  const int cb = (int)(blockIdx.x - win * a.ncb);
-  const int lane = threadIdx.x & 63, wave = uniform_int(threadIdx.x >> 6);
-  const int64_t p0 = win * EM_WIN, last = p0 + EM_WIN - 1;
+  const int64_t item = (int64_t)blockIdx.x * EM_WAVES + uniform_int(threadIdx.x >> 6);
+  const int64_t win = item / a.ncb;
+  const int cb = (int)(item - win * a.ncb);
+  const int64_t p0 = win * a.win, last = p0 + a.win - 1;
   if (last + 1 >= a.n) return;
   const uint32_t key = a.keys[last];
   if (key == a.vocab || a.keys[last + 1] != key) return;
   int seg = 0;
   if (MODE == EM_NORM) {
-    seg = a.row_seg[a.rows[last]];
-    if (a.row_seg[a.rows[last + 1]] != seg) return;
+    seg = a.seg_of[last];
+    if (a.seg_of[last + 1] != seg) return;
   }
-  auto same = [&](int64_t p) {
-    return a.keys[p] == key && (MODE != EM_NORM || a.row_seg[a.rows[p]] == seg);
-  };
+  auto same = [&](int64_t p) { return a.keys[p] == key && (MODE != EM_NORM || a.seg_of[p] == seg); };
   if (p0 > 0 && same(p0) && same(p0 - 1)) return;  // it began before
   // The run's last position: positions after it compare greater.
   int64_t lo = last + 1, hi = a.n - 1;
@@ -599,34 +750,15 @@ __global__ __launch_bounds__(64 * EM_WAVES) void k_embed_join(EmbedSum a) {
     const int64_t mid = (lo + hi + 1) >> 1;
     if (same(mid)) lo = mid; else hi = mid - 1;
   }
-  const int64_t end = lo / EM_WIN;  // its last window
-  __shared__ float red[2][EM_WAVES][64 * V];
+  const int64_t end = lo / a.win;  // its last window
+  constexpr bool second = MODE == EM_CLIP2;
   float v[V], q[V];
-  em_clear(v);
-  em_clear(q);
-  const bool second = MODE == EM_CLIP && a.out2 != nullptr;
-#pragma unroll 4
-  for (int64_t w = win + 1 + wave; w <= end; w += EM_WAVES) em_add(em_ws<DT>(a.ws, 2 * w, a, cb), v);
-  if (second)
-    for (int64_t w = win + 1 + wave; w <= end; w += EM_WAVES) em_add(em_ws<DT>(a.ws_sq, 2 * w, a, cb), q);
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    red[0][wave][i * 64 + lane] = v[i];
-    red[1][wave][i * 64 + lane] = q[i];
-  }
-  __syncthreads();
-  if (wave != 0) return;
   em_clear(v);
   em_clear(q);
   em_add(em_ws<DT>(a.ws, 2 * win + 1, a, cb), v);
   if (second) em_add(em_ws<DT>(a.ws_sq, 2 * win + 1, a, cb), q);
-#pragma unroll
-  for (int w = 0; w < EM_WAVES; ++w)
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      v[i] += red[0][w][i * 64 + lane];
-      q[i] += red[1][w][i * 64 + lane];
-    }
+  em_join<DT>(a.ws, win + 1, end, a, cb, v);
+  if (second) em_join<DT>(a.ws_sq, win + 1, end, a, cb, q);
   if (MODE != EM_NORM) {
     em_finish<DT, AL>(a, MODE, key, cb, v, q);
     return;
@@ -638,12 +770,17 @@ __global__ __launch_bounds__(64 * EM_WAVES) void k_embed_join(EmbedSum a) {
   em_put(em_ws<DT>(a.whole, win, a, cb), v);
 }
 
-// Zeroes `bytes` bytes.
-__global__ __launch_bounds__(256) void k_embed_zero(char* out, int64_t bytes) {
-  const int64_t n16 = ((uintptr_t)out & 15) == 0 ? bytes / 16 : 0;
-  const int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, nt = (int64_t)gridDim.x * blockDim.x;
-  for (int64_t i = t; i < n16; i += nt) odp_gstore((u32x4_t*)(out + 16 * i), u32x4_t{0, 0, 0, 0});
-  for (int64_t i = 16 * n16 + t; i < bytes; i += nt) out[i] = 0;
+__global__ __launch_bounds__(256) void k_embed_zero(ZeroShare z) { zero_pieces(z, blockIdx.x); }
+
+// Shares [k, l) of n of the pieces, and the workgroups (of `threads`) they take.
+ZeroShare zero_share(void* at, int64_t bytes, int threads, int64_t k, int64_t l, int64_t n, unsigned& blocks) {
+  ZeroShare z{(char*)at, at != nullptr ? bytes : 0, 0, 0, 1};
+  const int64_t size = (int64_t)threads * 16, pieces = (z.bytes + size - 1) / size;
+  z.first = pieces * k / n;
+  z.count = pieces * l / n - z.first;
+  z.per = (int)(1 + z.count / ((int64_t)1 << 22));
+  blocks = (unsigned)((z.count + z.per - 1) / z.per);
+  return z;
 }
 
 int sort_passes(int64_t vocab, int& bits) {
@@ -654,12 +791,26 @@ int sort_passes(int64_t vocab, int& bits) {
   return passes;
 }
 
-int64_t sort_waves(int64_t n) { return (n + SORT_KEYS - 1) / SORT_KEYS; }
+// Waves of the sort of n positions and the positions of each.
+int64_t sort_waves(int64_t n, int64_t& per) {
+  int64_t w = (n + SORT_KEYS - 1) / SORT_KEYS;
+  if (w > SORT_NW) w = SORT_NW;
+  per = ((n + w - 1) / w + 63) / 64 * 64;
+  return (n + per - 1) / per;
+}
 int64_t pieces(int dtype, int64_t width) {
   const int64_t per = 64 * (dtype == ODP_DTYPE_F32 ? 4 : 8);
   return (width + per - 1) / per;
 }
-int64_t windows(int64_t n) { return (n + EM_WIN - 1) / EM_WIN; }
+// Sorted positions per window: 32, or 16 or 8 where that leaves fewer than
+// EM_FILL waves, which then would each wait for their loads in turn.
+constexpr int64_t EM_FILL = 8192;
+int window(int64_t n, int64_t ncb) {
+  int w = EM_WIN;
+  while (w > 8 && (n + w - 1) / w * ncb < EM_FILL) w /= 2;
+  return w;
+}
+int64_t windows(int64_t n, int64_t ncb) { return (n + window(n, ncb) - 1) / window(n, ncb); }
 
 int check_rows(const char* what, int dtype, int64_t n, int64_t width, int64_t vocab, int64_t ld) {
   if (dtype != ODP_DTYPE_F32 && dtype != ODP_DTYPE_BF16 && dtype != ODP_DTYPE_F16) {
@@ -684,14 +835,19 @@ int check_grid(const char* what, int64_t blocks) {
 }
 
 template <int MODE>
-int launch_sum(const char* what, hipStream_t s, int dtype, bool aligned, const EmbedSum& a) {
-  const int64_t items = windows(a.n) * a.ncb;
+int launch_sum(const char* what, hipStream_t s, int dtype, bool aligned, EmbedSum a) {
+  a.win = window(a.n, a.ncb);
+  const int64_t items = windows(a.n, a.ncb) * a.ncb;
   if (int rc = check_grid(what, items)) return rc;
-  const dim3 grid((unsigned)((items + EM_WAVES - 1) / EM_WAVES)), block(64 * EM_WAVES), jgrid((unsigned)items);
-#define ODP_EM(DT, AL)                                                   \
-  do {                                                                   \
+  const dim3 grid((unsigned)((items + EM_WAVES - 1) / EM_WAVES)), block(64 * EM_WAVES);
+  const int64_t groups = windows(a.n, a.ncb) / JOIN_GROUP * a.ncb;
+  a.grouped = windows(a.n, a.ncb) >= 4 * JOIN_GROUP;  // below, no run has groups worth a launch
+  const dim3 ggrid((unsigned)((groups + EM_WAVES - 1) / EM_WAVES));
+#define ODP_EM(DT, AL)                                                     \
+  do {                                                                     \
     hipLaunchKernelGGL((k_embed_sum<DT, AL, MODE>), grid, block, 0, s, a); \
-    hipLaunchKernelGGL((k_embed_join<DT, AL, MODE>), jgrid, block, 0, s, a); \
+    if (a.grouped) hipLaunchKernelGGL((k_embed_group<DT, MODE>), ggrid, block, 0, s, a); \
+    hipLaunchKernelGGL((k_embed_join<DT, AL, MODE>), grid, block, 0, s, a); \
   } while (0)
   if (dtype == ODP_DTYPE_F32) {
     if (aligned) ODP_EM(ODP_DTYPE_F32, true); else ODP_EM(ODP_DTYPE_F32, false);
@@ -710,9 +866,9 @@ bool rows_aligned(int dtype, const void* p, int64_t ld, int64_t width) {
 }
 
 int launch_zero(const char* what, hipStream_t s, void* out, int64_t bytes) {
-  int64_t blocks = (bytes + 16383) / 16384;
-  if (blocks > 4096) blocks = 4096;
-  if (blocks > 0) hipLaunchKernelGGL(k_embed_zero, dim3((unsigned)blocks), dim3(256), 0, s, (char*)out, bytes);
+  unsigned blocks;
+  const ZeroShare z = zero_share(out, bytes, 256, 0, 1, 1, blocks);
+  if (blocks > 0) hipLaunchKernelGGL(k_embed_zero, dim3(blocks), dim3(256), 0, s, z);
   return odp_check_launch(what);
 }
 
@@ -731,7 +887,7 @@ extern "C" int odp_embed_rows(odp_stream_t stream, int dtype, const void* tokens
     return ODP_ERR_INVALID_ARGUMENT;
   }
   const int ncb = (int)pieces(dtype, width);
-  const int64_t blocks = (n * ncb + EM_WAVES - 1) / EM_WAVES;
+  const int64_t blocks = (n * ncb + EM_WAVES * EM_ITEMS - 1) / (EM_WAVES * EM_ITEMS);
   if (int rc = check_grid("odp_embed_rows", blocks)) return rc;
   const bool al = rows_aligned(dtype, weight, ldw, width) && ((uintptr_t)out & 15) == 0;
   const hipStream_t s = odp_hip_stream(stream);
@@ -751,56 +907,73 @@ extern "C" int odp_embed_rows(odp_stream_t stream, int dtype, const void* tokens
 
 extern "C" int64_t odp_token_sort_scratch(int64_t n, int64_t vocab) {
   if (n <= 0 || vocab <= 0) return 0;
-  int bits;
-  sort_passes(vocab, bits);
-  return 4 * (2 * n + (n > SORT_SMALL ? ((int64_t)1 << bits) * sort_waves(n) : 0));
+  int64_t per;
+  return 4 * ((3 * n + 3) / 4 * 4 + (n > SORT_SMALL ? SORT_BINS * sort_waves(n, per) : 0));
 }
 
 extern "C" int odp_token_sort(odp_stream_t stream, const void* tokens, int token_bytes, int64_t n, int64_t vocab,
                               int64_t padding, const int32_t* seg_row_start, const int32_t* seg_row_len,
-                              int32_t n_seg, void* scratch, uint32_t* keys, uint32_t* rows, int32_t* row_seg) {
+                              int32_t n_seg, void* scratch, uint32_t* keys, uint32_t* rows, int32_t* seg_of,
+                              void* zero, int64_t zero_bytes) {
   if (int rc = check_rows("odp_token_sort", ODP_DTYPE_F32, n, 1, vocab, 1)) return rc;
   if (token_bytes != 4 && token_bytes != 8) {
     odp_set_error("odp_token_sort: tokens of %d bytes", token_bytes);
     return ODP_ERR_UNSUPPORTED;
   }
-  if (n == 0) return ODP_OK;
-  if (tokens == nullptr || scratch == nullptr || keys == nullptr || rows == nullptr || n_seg < 0 ||
-      (seg_row_start != nullptr && (seg_row_len == nullptr || row_seg == nullptr))) {
-    odp_set_error("odp_token_sort: null pointer or negative n_seg (%d)", n_seg);
+  if (zero_bytes < 0) {
+    odp_set_error("odp_token_sort: %lld bytes to zero", (long long)zero_bytes);
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  const hipStream_t s = odp_hip_stream(stream);
+  if (n == 0) return zero != nullptr ? launch_zero("odp_token_sort", s, zero, zero_bytes) : ODP_OK;
+  if (tokens == nullptr || scratch == nullptr || ((uintptr_t)scratch & 15) != 0 || keys == nullptr ||
+      rows == nullptr || n_seg < 0 || (seg_row_start != nullptr && (seg_row_len == nullptr || seg_of == nullptr))) {
+    odp_set_error("odp_token_sort: null pointer, scratch off the 16-byte grid or negative n_seg (%d)", n_seg);
     return ODP_ERR_INVALID_ARGUMENT;
   }
   int bits;
   const int passes = sort_passes(vocab, bits);
-  SortIn a{tokens, token_bytes == 8 ? 1 : 0, n, vocab, padding, seg_row_start, seg_row_len, n_seg, row_seg};
   uint32_t* k1 = (uint32_t*)scratch;
   uint32_t* r1 = k1 + n;
-  const hipStream_t s = odp_hip_stream(stream);
+  const bool segs = seg_row_start != nullptr;
+  SortIn a{tokens, token_bytes == 8 ? 1 : 0, n, vocab, padding, seg_row_start, seg_row_len, n_seg,
+           segs ? (int32_t*)(r1 + n) : nullptr, segs ? seg_of : nullptr, ZeroShare{}};
+  unsigned zb;
   if (n <= SORT_SMALL) {
-    hipLaunchKernelGGL(k_sort_small, dim3(1), dim3(64 * SORT_WAVES), 0, s, a, passes, bits, keys, rows, k1, r1);
+    a.zero = zero_share(zero, zero_bytes, 64 * SORT_WAVES, 0, 1, 1, zb);
+#define ODP_SORT(R) \
+  hipLaunchKernelGGL(k_sort_small<R>, dim3(1 + zb), dim3(64 * SORT_WAVES), 0, s, a, passes, bits, keys, rows, k1, r1)
+    if (n <= SORT_WAVES * 64 * 2) ODP_SORT(2);
+    else ODP_SORT(8);
+#undef ODP_SORT
     return odp_check_launch("odp_token_sort");
   }
-  uint32_t* counts = r1 + n;
-  const int nw = (int)sort_waves(n);
-  const dim3 grid((unsigned)((nw + EM_WAVES - 1) / EM_WAVES)), block(64 * EM_WAVES);
+  uint32_t* counts = k1 + (3 * n + 3) / 4 * 4;
+  int64_t per;
+  const int nw = (int)sort_waves(n, per);
+  const unsigned own = (unsigned)((nw + EM_WAVES - 1) / EM_WAVES);
+  const dim3 block(64 * EM_WAVES);
   for (int p = 0; p < passes; ++p) {
     const bool to0 = ((passes - 1 - p) & 1) == 0;
     const uint32_t* ik = to0 ? k1 : keys;
     const uint32_t* ir = to0 ? r1 : rows;
     uint32_t* ok = to0 ? keys : k1;
     uint32_t* orow = to0 ? rows : r1;
-    hipLaunchKernelGGL(k_sort_count, grid, block, 0, s, a, ik, p == 0 ? 1 : 0, p * bits, bits, counts, nw);
-    hipLaunchKernelGGL(k_sort_scan, dim3(1), dim3(1024), 0, s, counts, ((int64_t)1 << bits) * nw);
-    hipLaunchKernelGGL(k_sort_scatter, grid, block, 0, s, a, ik, ir, p == 0 ? 1 : 0, p * bits, bits, counts, nw, ok,
-                       orow);
+    // The zeroing goes out in shares of two to three, as the launches' times do.
+    a.zero = zero_share(zero, zero_bytes, 64 * EM_WAVES, 5 * p, 5 * p + 2, 5 * passes, zb);
+    hipLaunchKernelGGL(k_sort_count, dim3(own + zb), block, 0, s, a, ik, p == 0 ? 1 : 0, p * bits, bits, counts, nw,
+                       per);
+    a.zero = zero_share(zero, zero_bytes, 64 * EM_WAVES, 5 * p + 2, 5 * p + 5, 5 * passes, zb);
+    hipLaunchKernelGGL(k_sort_scatter, dim3(own + zb), block, 0, s, a, ik, ir, p == 0 ? 1 : 0, p * bits, bits, counts,
+                       nw, per, ok, orow, p == passes - 1 ? 1 : 0);
   }
   return odp_check_launch("odp_token_sort");
 }
 
 extern "C" int64_t odp_embed_sum_scratch(int dtype, int64_t n, int64_t width, int second) {
   if (n <= 0 || width <= 0) return 0;
-  const int64_t row = pieces(dtype, width) * 64 * (dtype == ODP_DTYPE_F32 ? 4 : 8);
-  return 4 * row * windows(n) * (second ? 4 : 2);
+  const int64_t ncb = pieces(dtype, width), row = ncb * 64 * (dtype == ODP_DTYPE_F32 ? 4 : 8);
+  return 4 * row * windows(n, ncb) * (second ? 4 : 2);
 }
 
 extern "C" int64_t odp_embed_pieces(int dtype, int64_t width) { return width > 0 ? pieces(dtype, width) : 0; }
@@ -813,9 +986,8 @@ extern "C" int odp_embed_grad(odp_stream_t stream, int dtype, const void* g, int
     odp_set_error("odp_embed_grad: null pointer");
     return ODP_ERR_INVALID_ARGUMENT;
   }
-  const hipStream_t s = odp_hip_stream(stream);
-  if (int rc = launch_zero("odp_embed_grad", s, out, vocab * width * (dtype == ODP_DTYPE_F32 ? 4 : 2))) return rc;
   if (n == 0) return ODP_OK;
+  const hipStream_t s = odp_hip_stream(stream);
   EmbedSum a{};
   a.g = (const char*)g;
   a.ldg = ldg;
@@ -835,12 +1007,12 @@ extern "C" int odp_embed_grad(odp_stream_t stream, int dtype, const void* g, int
 }
 
 extern "C" int odp_embed_sqnorm(odp_stream_t stream, int dtype, const void* g, int64_t ldg, int64_t n, int64_t width,
-                                const uint32_t* keys, const uint32_t* rows, const int32_t* row_seg, int64_t vocab,
+                                const uint32_t* keys, const uint32_t* rows, const int32_t* seg_of, int64_t vocab,
                                 float scale, const int32_t* seg_row_start, const int32_t* seg_example, void* scratch,
                                 float* whole, double* part, int64_t part_stride, int64_t slot, int64_t* nf_flag) {
   if (int rc = check_rows("odp_embed_sqnorm", dtype, n, width, vocab, ldg)) return rc;
   if (n == 0) return ODP_OK;
-  if (g == nullptr || keys == nullptr || rows == nullptr || row_seg == nullptr || seg_row_start == nullptr ||
+  if (g == nullptr || keys == nullptr || rows == nullptr || seg_of == nullptr || seg_row_start == nullptr ||
       seg_example == nullptr || scratch == nullptr || whole == nullptr || part == nullptr || nf_flag == nullptr ||
       slot < 0 || slot >= part_stride) {
     odp_set_error("odp_embed_sqnorm: null pointer or slot %lld outside [0, %lld)", (long long)slot,
@@ -855,7 +1027,7 @@ extern "C" int odp_embed_sqnorm(odp_stream_t stream, int dtype, const void* g, i
   a.ncb = (int)pieces(dtype, width);
   a.keys = keys;
   a.rows = rows;
-  a.row_seg = row_seg;
+  a.seg_of = seg_of;
   a.vocab = (uint32_t)vocab;
   a.scale = scale;
   a.ws = (float*)scratch;
@@ -871,7 +1043,7 @@ extern "C" int odp_embed_sqnorm(odp_stream_t stream, int dtype, const void* g, i
 
 extern "C" int odp_embed_clipped_sum(odp_stream_t stream, int dtype, const void* g, int64_t ldg, int64_t n,
                                      int64_t width, const uint32_t* keys, const uint32_t* rows,
-                                     const int32_t* row_seg, int64_t vocab, float scale, const int32_t* seg_example,
+                                     const int32_t* seg_of, int64_t vocab, float scale, const int32_t* seg_example,
                                      void* scratch, const float* whole, const double* scales, float normalize_by,
                                      int out_dtype, void* out, void* out2) {
   if (int rc = check_rows("odp_embed_clipped_sum", dtype, n, width, vocab, ldg)) return rc;
@@ -879,17 +1051,15 @@ extern "C" int odp_embed_clipped_sum(odp_stream_t stream, int dtype, const void*
     odp_set_error("odp_embed_clipped_sum: out_dtype %d", out_dtype);
     return ODP_ERR_UNSUPPORTED;
   }
-  if (out == nullptr || (n > 0 && (g == nullptr || keys == nullptr || rows == nullptr || row_seg == nullptr ||
+  if (out == nullptr || (n > 0 && (g == nullptr || keys == nullptr || rows == nullptr || seg_of == nullptr ||
                                    seg_example == nullptr || scratch == nullptr || whole == nullptr ||
                                    scales == nullptr))) {
     odp_set_error("odp_embed_clipped_sum: null pointer");
     return ODP_ERR_INVALID_ARGUMENT;
   }
   const hipStream_t s = odp_hip_stream(stream);
-  const int64_t bytes = vocab * width * odp_dtype_size(out_dtype);
-  if (int rc = launch_zero("odp_embed_clipped_sum", s, out, bytes)) return rc;
   if (out2 != nullptr)
-    if (int rc = launch_zero("odp_embed_clipped_sum", s, out2, bytes)) return rc;
+    if (int rc = launch_zero("odp_embed_clipped_sum", s, out2, vocab * width * odp_dtype_size(out_dtype))) return rc;
   if (n == 0) return ODP_OK;
   EmbedSum a{};
   a.g = (const char*)g;
@@ -899,7 +1069,7 @@ extern "C" int odp_embed_clipped_sum(odp_stream_t stream, int dtype, const void*
   a.ncb = (int)pieces(dtype, width);
   a.keys = keys;
   a.rows = rows;
-  a.row_seg = row_seg;
+  a.seg_of = seg_of;
   a.vocab = (uint32_t)vocab;
   a.scale = scale;
   a.ws = (float*)scratch;
@@ -911,8 +1081,7 @@ extern "C" int odp_embed_clipped_sum(odp_stream_t stream, int dtype, const void*
   a.sex = seg_example;
   a.scales = scales;
   a.normalize_by = normalize_by;
-  return launch_sum<EM_CLIP>("odp_embed_clipped_sum", s, dtype,
-                             rows_aligned(dtype, g, ldg, width) && ((uintptr_t)out & 15) == 0 &&
-                                 ((uintptr_t)out2 & 15) == 0,
-                             a);
+  const bool aligned = rows_aligned(dtype, g, ldg, width) && ((uintptr_t)out & 15) == 0 && ((uintptr_t)out2 & 15) == 0;
+  return out2 != nullptr ? launch_sum<EM_CLIP2>("odp_embed_clipped_sum", s, dtype, aligned, a)
+                         : launch_sum<EM_CLIP>("odp_embed_clipped_sum", s, dtype, aligned, a);
 }

@@ -616,7 +616,7 @@ class _EmbeddingWork:
         # Sums of the runs that cross windows, kept from the norms for the clipped sum.
         self.whole = torch.empty(max(int(lib.odp_embed_sum_scratch(self.dt, self.n, self.width, 0)) // 8, 1),
                                  dtype=torch.float32, device=dev)
-        self.ids = torch.empty((3, max(self.n, 1)), dtype=torch.int32, device=dev)  # sorted tokens, rows; segments
+        self.ids = torch.empty((3, max(self.n, 1)), dtype=torch.int32, device=dev)  # sorted tokens, rows and segments
 
     def _take(self, es: EmbeddingSite) -> None:
         self.site = es
@@ -639,21 +639,22 @@ class _EmbeddingWork:
         return t.data_ptr() + 4 * self.view.first
 
     def norms(self, plan: GhostPlan, stream: int) -> None:
-        keys, rows, row_seg = (self.ids[k].data_ptr() for k in range(3))
+        keys, rows, seg_of = (self.ids[k].data_ptr() for k in range(3))
+        out = plan.out[self.site.w_leaf]
         N.call("odp_token_sort", stream, self.tokens.data_ptr(), self.tokens.element_size(), self.n, self.vocab,
                int(self.site.padding), self._seg(plan.seg_start), self._seg(plan.seg_len), self.view.n_seg,
-               self.scratch.data_ptr(), keys, rows, row_seg)
+               self.scratch.data_ptr(), keys, rows, seg_of, out.data_ptr(), out.numel() * out.element_size())
         N.call("odp_embed_sqnorm", stream, self.dt, self.g.data_ptr(), self.g.stride(0), self.n, self.width, keys,
-               rows, row_seg, self.vocab, float(self.site.scale), self._seg(plan.seg_start), self._seg(plan.seg_ex),
+               rows, seg_of, self.vocab, float(self.site.scale), self._seg(plan.seg_start), self._seg(plan.seg_ex),
                self.scratch.data_ptr(), self.whole.data_ptr(), plan.part.data_ptr(), plan.n_slots, self.slot,
                plan._nf_flag_addr)
 
     def clipped_sum(self, plan: GhostPlan, stream: int) -> None:
-        keys, rows, row_seg = (self.ids[k].data_ptr() for k in range(3))
+        keys, rows, seg_of = (self.ids[k].data_ptr() for k in range(3))
         i = self.site.w_leaf
         out2 = plan.out2[i].data_ptr() if plan.out2 is not None else None
         N.call("odp_embed_clipped_sum", stream, self.dt, self.g.data_ptr(), self.g.stride(0), self.n, self.width,
-               keys, rows, row_seg, self.vocab, float(self.site.scale), self._seg(plan.seg_ex),
+               keys, rows, seg_of, self.vocab, float(self.site.scale), self._seg(plan.seg_ex),
                self.scratch.data_ptr(), self.whole.data_ptr(), plan.scales[self.leaf.cls][self.leaf.group].data_ptr(),
                float(plan.clip.normalize_by), dtype_code(self.leaf.out_dtype), plan.out[i].data_ptr(), out2)
 

@@ -111,7 +111,7 @@ def table_gradient(tokens: torch.Tensor, g: torch.Tensor, vocab: int, scale: flo
     with _OnDevice(g):
         s = _stream(g)
         _call("odp_token_sort", s, flat.data_ptr(), flat.element_size(), n, vocab, padding, None, None, 0, at, keys,
-              keys + 4 * n, None)
+              keys + 4 * n, None, out.data_ptr(), out.numel() * out.element_size())
         _call("odp_embed_grad", s, dt, rows.data_ptr(), rows.stride(0), n, width, keys, keys + 4 * n, vocab, scale, at,
               out.data_ptr())
     return out

@@ -356,3 +356,31 @@ def test_clipped_grad_routes_the_table(groups, microbatch, double):
     ref, _ = dp_ref.clipped_grad(twice_plain, params, (y, c), clipping_norm=cpu_norm, normalize_by=float(n))
     for k in ref:
         assert float((got.pytree[k].double().cpu() - ref[k].double()).norm() / ref[k].double().norm()) < 1e-5
+
+
+@pytest.mark.parametrize("n", [2048, 2049, 32768, 32769, 70001])
+def test_sort_sizes(n):
+    """Either side of the sizes at which the sort changes its launches, with a token run of thousands."""
+    g = gen(n)
+    vocab, width = 3000, 8
+    y = tokens_of("text", n, vocab, g)
+    y[n // 4 : n // 2] = 77
+    w = torch.zeros(vocab, width, device=DEV, requires_grad=True)
+    go = torch.randint(-8, 9, (n, width), generator=g).float()  # sums exact in float32
+    (dw,) = torch.autograd.grad(embedding(y.to(DEV), w), w, go.to(DEV))
+    s, _, _ = table_sums(y, go, vocab)
+    assert torch.equal(dw.double().cpu(), s)
+    batch = 3
+    seq = n // batch
+    clip = clip_of((vocab, width), torch.float32)
+    plan = GhostPlan(segments=Segments.padded(batch, seq), leaves=[LeafOut((vocab, width), torch.float32)], clip=clip,
+                     embedding_sites=[EmbeddingSite(tokens=y[: batch * seq].to(DEV), g=go[: batch * seq].to(DEV),
+                                                    w_leaf=0)])
+    res = plan.run()
+    S, _, _ = per_example(y[: batch * seq], go[: batch * seq], [seq] * batch, seq, vocab)
+    norms = S.flatten(1).norm(dim=1)
+    assert ((res.norms.double().cpu() - norms).abs() <= 4 * U32 * norms).all()  # squares, root and store
+    c = res.scales[0, 0].cpu().float().double().view(-1, 1, 1)
+    want = (c * S).sum(0) / clip.normalize_by
+    bound = 8 * U32 * (c * S).abs().sum(0) / clip.normalize_by + LEAST[torch.float32]
+    assert ((res.leaves[0].double().cpu() - want).abs() <= bound).all()
