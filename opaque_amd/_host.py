@@ -1,7 +1,8 @@
-"""The host-side helper extension (``csrc/odp_host.cpp``): structure
+"""The host-side helper extension (``csrc/odp_host*.cpp``): structure
 signatures and addresses of a call's LoRA sites, and output leaf views, for
-GhostPlan.rebind.  Built by ``opaque_amd.build.build_host``; without it the
-same work runs in Python (host bookkeeping only, no arithmetic)."""
+GhostPlan.rebind; and the vocabulary operators' calls outside torch.func.
+Built by ``opaque_amd.build.build_host``; without it the same work runs in
+Python (host bookkeeping only, no arithmetic)."""
 
 from __future__ import annotations
 

@@ -105,13 +105,13 @@ def build_sanitized(verbose: bool = False) -> Path:
     return SAN_LIB
 
 
-HOST_SRC = CSRC / "odp_host.cpp"
+HOST_SRCS = [CSRC / "odp_host.cpp", CSRC / "odp_host_vocab.cpp"]
 HOST_DIR = PKG_DIR / "_host_build"
 HOST_NAME = "_odp_host"
 
 
 def build_host(verbose: bool = False) -> Path:
-    """Compile the host-side helper (a torch C++ extension, no device code)
+    """Compile the host-side helpers (a torch C++ extension, no device code)
     into opaque_amd/_host_build/_odp_host.so.  Always recompiles."""
     import torch.utils.cpp_extension as ext
 
@@ -119,8 +119,11 @@ def build_host(verbose: bool = False) -> Path:
     for stale in HOST_DIR.glob("*"):
         if stale.is_file():
             stale.unlink()
-    ext.load(name=HOST_NAME, sources=[str(HOST_SRC)], build_directory=str(HOST_DIR),
-             extra_cflags=["-O2"], verbose=verbose)
+    rocm = Path(hipcc_path()).resolve().parent.parent
+    ext.load(name=HOST_NAME, sources=[str(s) for s in HOST_SRCS], build_directory=str(HOST_DIR),
+             extra_cflags=["-O2", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1"],
+             extra_include_paths=[str(rocm / "include")], extra_ldflags=["-lc10_hip", "-ltorch_hip"],
+             verbose=verbose)
     return HOST_DIR / f"{HOST_NAME}.so"
 
 

@@ -841,7 +841,7 @@ int launch_sum(const char* what, hipStream_t s, int dtype, bool aligned, EmbedSu
   if (int rc = check_grid(what, items)) return rc;
   const dim3 grid((unsigned)((items + EM_WAVES - 1) / EM_WAVES)), block(64 * EM_WAVES);
   const int64_t groups = windows(a.n, a.ncb) / JOIN_GROUP * a.ncb;
-  a.grouped = windows(a.n, a.ncb) >= 4 * JOIN_GROUP;  // below, no run has groups worth a launch
+  a.grouped = windows(a.n, a.ncb) > 8 * JOIN_GROUP;  // below, no run is long enough to be worth a launch
   const dim3 ggrid((unsigned)((groups + EM_WAVES - 1) / EM_WAVES));
 #define ODP_EM(DT, AL)                                                     \
   do {                                                                     \

@@ -1,0 +1,324 @@
+// The vocabulary operators' calls outside torch.func, on the host: arguments
+// to addresses, workspaces, and the autograd nodes.  No device code; the work
+// is the C entry points of libopaque_dp.so, bound by address.
+//
+// The same calls in Python cost 100 us (a lookup and its gradient) to 180 us
+// (a loss and its gradients) of host time, most of it in the backward pass,
+// whose thread takes the interpreter lock; small batches are bound by that.
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/extension.h>
+
+#include <string>
+#include <unordered_map>
+
+#include "../../include/opaque_dp.h"
+
+namespace py = pybind11;
+
+namespace {
+
+// The bound entry points.
+struct Abi {
+  decltype(&odp_last_error) last_error = nullptr;
+  decltype(&odp_embed_rows) embed_rows = nullptr;
+  decltype(&odp_token_sort_scratch) token_sort_scratch = nullptr;
+  decltype(&odp_token_sort) token_sort = nullptr;
+  decltype(&odp_embed_sum_scratch) embed_sum_scratch = nullptr;
+  decltype(&odp_embed_grad) embed_grad = nullptr;
+  decltype(&odp_xent_rows) xent_rows = nullptr;
+  decltype(&odp_xent_stats_scratch) xent_stats_scratch = nullptr;
+  decltype(&odp_xent_losses) xent_losses = nullptr;
+  decltype(&odp_xent_reduce) xent_reduce = nullptr;
+  decltype(&odp_xent_pitch) xent_pitch = nullptr;
+  decltype(&odp_xent_dlogits) xent_dlogits = nullptr;
+  decltype(&odp_xent_dx_scratch) xent_dx_scratch = nullptr;
+  decltype(&odp_xent_dx) xent_dx = nullptr;
+  decltype(&odp_xent_dx_rows) xent_dx_rows = nullptr;
+  decltype(&odp_xent_dw) xent_dw = nullptr;
+};
+Abi abi;
+
+void bind(const std::unordered_map<std::string, uintptr_t>& at) {
+  Abi b;
+#define ODP_BIND(name) b.name = reinterpret_cast<decltype(b.name)>(at.at("odp_" #name))
+  ODP_BIND(last_error);
+  ODP_BIND(embed_rows);
+  ODP_BIND(token_sort_scratch);
+  ODP_BIND(token_sort);
+  ODP_BIND(embed_sum_scratch);
+  ODP_BIND(embed_grad);
+  ODP_BIND(xent_rows);
+  ODP_BIND(xent_stats_scratch);
+  ODP_BIND(xent_losses);
+  ODP_BIND(xent_reduce);
+  ODP_BIND(xent_pitch);
+  ODP_BIND(xent_dlogits);
+  ODP_BIND(xent_dx_scratch);
+  ODP_BIND(xent_dx);
+  ODP_BIND(xent_dx_rows);
+  ODP_BIND(xent_dw);
+#undef ODP_BIND
+  abi = b;
+}
+
+void check(int rc, const char* what) { TORCH_CHECK(rc == ODP_OK, what, " failed with status ", rc, ": ", abi.last_error()); }
+
+int code_of(const at::Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return ODP_DTYPE_F32;
+    case at::kBFloat16: return ODP_DTYPE_BF16;
+    case at::kHalf: return ODP_DTYPE_F16;
+    default: TORCH_CHECK_TYPE(false, "unsupported dtype ", t.scalar_type());
+  }
+}
+
+odp_stream_t stream_of(const at::Tensor& t) {
+  return reinterpret_cast<odp_stream_t>(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.get_device()).stream());
+}
+
+at::Tensor bytes_on(const at::Tensor& t, int64_t n) { return at::empty({n}, t.options().dtype(at::kByte)); }
+int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
+
+// Rows with unit column stride and a pitch of at least the width, copied if laid out otherwise.
+at::Tensor pitched(const at::Tensor& t) {
+  at::Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+  if ((r.stride(1) != 1 && r.size(1) > 1) || r.stride(0) < r.size(1)) r = r.clone(at::MemoryFormat::Contiguous);
+  return r;
+}
+
+// Ties a first derivative to the gradient it came from, so that asking for a
+// second one is an error instead of zero.
+struct NoSecond : torch::autograd::Function<NoSecond> {
+  static at::Tensor forward(torch::autograd::AutogradContext*, const at::Tensor&, const at::Tensor& d) {
+    return d.detach();
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
+    TORCH_CHECK(false, "the vocabulary operators have no second derivative");
+  }
+};
+at::Tensor first_only(const at::Tensor& g, at::Tensor d) {
+  return d.defined() && at::GradMode::is_enabled() && g.requires_grad() ? NoSecond::apply(g, d) : d;
+}
+
+// ---------------------------------------------------------------------------
+// Embedding
+// ---------------------------------------------------------------------------
+
+at::Tensor embed_rows(const at::Tensor& tokens, const at::Tensor& weight, double scale) {
+  const c10::OptionalDeviceGuard guard(weight.device());
+  const at::Tensor w = pitched(weight), y = tokens.contiguous();
+  std::vector<int64_t> shape(tokens.sizes().vec());
+  shape.push_back(w.size(1));
+  at::Tensor out = at::empty(shape, w.options());
+  check(abi.embed_rows(stream_of(w), code_of(w), y.data_ptr(), (int)y.element_size(), y.numel(), w.data_ptr(),
+                       w.stride(0), w.size(0), w.size(1), (float)scale, out.data_ptr()),
+        "odp_embed_rows");
+  return out;
+}
+
+struct Embed : torch::autograd::Function<Embed> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& tokens, const at::Tensor& weight,
+                            double scale, int64_t padding) {
+    ctx->save_for_backward({tokens});
+    ctx->saved_data["vocab"] = weight.size(0);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    return embed_rows(tokens, weight, scale);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    if (!ctx->needs_input_grad(1) || !grads[0].defined()) return {{}, {}, {}, {}};
+    at::Tensor dw;
+    {
+      at::NoGradGuard no_grad;
+      const c10::OptionalDeviceGuard guard(grads[0].device());
+      const at::Tensor g = pitched(grads[0]), y = ctx->get_saved_variables()[0].contiguous();
+      const int64_t n = y.numel(), width = g.size(1), vocab = ctx->saved_data["vocab"].toInt();
+      const int dt = code_of(g);
+      dw = at::empty({vocab, width}, g.options());
+      const int64_t scratch = up16(std::max(abi.token_sort_scratch(n, vocab), abi.embed_sum_scratch(dt, n, width, 0)));
+      const at::Tensor work = bytes_on(g, scratch + 8 * n);
+      char* at = (char*)work.data_ptr();
+      uint32_t* keys = (uint32_t*)(at + scratch);
+      const odp_stream_t s = stream_of(g);
+      check(abi.token_sort(s, y.data_ptr(), (int)y.element_size(), n, vocab, ctx->saved_data["padding"].toInt(),
+                           nullptr, nullptr, 0, at, keys, keys + n, nullptr, dw.data_ptr(), (int64_t)dw.nbytes()),
+            "odp_token_sort");
+      check(abi.embed_grad(s, dt, g.data_ptr(), g.stride(0), n, width, keys, keys + n, vocab,
+                           (float)ctx->saved_data["scale"].toDouble(), at, dw.data_ptr()),
+            "odp_embed_grad");
+    }
+    return {{}, first_only(grads[0], dw), {}, {}};
+  }
+};
+
+at::Tensor embedding(const at::Tensor& tokens, const at::Tensor& weight, double scale, int64_t padding) {
+  py::gil_scoped_release nogil;
+  if (at::GradMode::is_enabled() && weight.requires_grad()) return Embed::apply(tokens, weight, scale, padding);
+  return embed_rows(tokens, weight, scale);
+}
+
+// ---------------------------------------------------------------------------
+// Linear cross entropy
+// ---------------------------------------------------------------------------
+
+// The head with rows on the 16-byte grid: itself, or a copy padded with zero columns.
+at::Tensor head_rows(const at::Tensor& weight) {
+  at::Tensor w = pitched(weight);
+  const int64_t per = 16 / w.element_size();
+  if (w.size(1) % per == 0 && w.stride(0) % per == 0 && reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0) return w;
+  at::Tensor wide = at::zeros({w.size(0), (w.size(1) + per - 1) / per * per}, w.options());
+  wide.narrow(1, 0, w.size(1)).copy_(w);
+  return wide;
+}
+
+// The packed rows of a call (odp_xent_rows) and what its backward needs.
+struct Packed {
+  at::Tensor w, xc, ids, losses, lse;
+  int64_t n, cols, width, vocab;
+  int dt;
+  int32_t* count() const { return (int32_t*)ids.data_ptr(); }
+  float* counted() const { return (float*)count() + 1; }
+  int32_t* act() const { return count() + 2; }
+  int32_t* tgt() const { return act() + std::max<int64_t>(n, 1); }
+  int32_t* where() const { return tgt() + std::max<int64_t>(n, 1); }
+};
+
+Packed xent_forward(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target, double softcap,
+                    int64_t ignore) {
+  Packed p;
+  p.w = head_rows(weight);
+  const at::Tensor rows = pitched(x), y = target.contiguous();
+  p.n = y.numel();
+  p.cols = rows.size(1);
+  p.width = p.w.size(1);
+  p.vocab = p.w.size(0);
+  p.dt = code_of(rows);
+  const int64_t room = std::max<int64_t>(p.n, 1);
+  p.xc = at::empty({room, p.width}, rows.options());
+  p.ids = at::empty({3 * room + 2}, rows.options().dtype(at::kInt));
+  p.losses = at::empty(target.sizes(), rows.options().dtype(at::kFloat));
+  p.lse = at::empty({p.n}, p.losses.options());
+  float* losses = (float*)p.losses.data_ptr();
+  float* lse = (float*)p.lse.data_ptr();
+  const odp_stream_t s = stream_of(rows);
+  check(abi.xent_rows(s, p.dt, rows.data_ptr(), rows.stride(0), p.n, p.cols, p.width, y.data_ptr(),
+                      (int)y.element_size(), p.vocab, ignore, 0, p.xc.data_ptr(), p.act(), p.tgt(), p.where(),
+                      p.count(), losses, lse),
+        "odp_xent_rows");
+  const at::Tensor work = bytes_on(rows, abi.xent_stats_scratch(p.dt, p.n, p.vocab));
+  check(abi.xent_losses(s, p.dt, p.xc.data_ptr(), p.n, p.width, p.act(), p.tgt(), p.count(), p.w.data_ptr(),
+                        p.w.stride(0), p.vocab, (float)softcap, work.data_ptr(), losses, lse),
+        "odp_xent_losses");
+  return p;
+}
+
+// reduction: 0 none, 1 sum, 2 mean.
+at::Tensor xent_result(const Packed& p, int64_t reduction) {
+  if (reduction == 0) return p.losses;
+  at::Tensor out = at::empty({}, p.losses.options());
+  check(abi.xent_reduce(stream_of(p.xc), (const float*)p.losses.data_ptr(), p.n, reduction == 2 ? p.counted() : nullptr,
+                        (float*)out.data_ptr()),
+        "odp_xent_reduce");
+  return out;
+}
+
+struct Xent : torch::autograd::Function<Xent> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight,
+                            const at::Tensor& target, double softcap, int64_t ignore, int64_t reduction,
+                            int64_t piece_bytes) {
+    const c10::OptionalDeviceGuard guard(x.device());
+    const Packed p = xent_forward(x, weight, target, softcap, ignore);
+    ctx->save_for_backward({weight});  // a later change of the head in place is an error
+    auto& d = ctx->saved_data;
+    d["w"] = p.w;
+    d["xc"] = p.xc;
+    d["ids"] = p.ids;
+    d["lse"] = p.lse;
+    d["n"] = p.n;
+    d["cols"] = p.cols;
+    d["softcap"] = softcap;
+    d["mean"] = reduction == 2;
+    d["piece_bytes"] = piece_bytes;
+    d["x_shape"] = x.sizes().vec();
+    return xent_result(p, reduction);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    at::Tensor dx, dw;
+    if (!grads[0].defined()) return {{}, {}, {}, {}, {}, {}, {}};
+    ctx->get_saved_variables();
+    {
+      at::NoGradGuard no_grad;
+      auto& sd = ctx->saved_data;
+      Packed p;
+      p.w = sd["w"].toTensor();
+      p.xc = sd["xc"].toTensor();
+      p.ids = sd["ids"].toTensor();
+      p.n = sd["n"].toInt();
+      p.cols = sd["cols"].toInt();
+      p.width = p.w.size(1);
+      p.vocab = p.w.size(0);
+      p.dt = code_of(p.xc);
+      const at::Tensor lse = sd["lse"].toTensor();
+      const float softcap = (float)sd["softcap"].toDouble();
+      const c10::OptionalDeviceGuard guard(p.xc.device());
+      const at::Tensor g = grads[0].contiguous();
+      const int stride = g.dim() > 0 ? 1 : 0;
+      const float* over = sd["mean"].toBool() ? p.counted() : nullptr;
+      const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+      const int64_t es = p.xc.element_size(), edge = abi.xent_pitch(p.dt, 1);
+      const int64_t fit = sd["piece_bytes"].toInt() / (std::max<int64_t>(p.n, 1) * es) / edge * edge;
+      const int64_t piece = std::min(p.vocab, std::max(fit, edge));
+      const at::Tensor d = at::empty({std::max<int64_t>(p.n, 1), abi.xent_pitch(p.dt, piece)}, p.xc.options());
+      at::Tensor sums;
+      if (need_x) {
+        dx = at::empty(sd["x_shape"].toIntVector(), p.xc.options());
+        sums = bytes_on(p.xc, abi.xent_dx_scratch(p.dt, p.n, p.width));
+      }
+      if (need_w) dw = at::empty({p.vocab, p.width}, p.xc.options());
+      const odp_stream_t s = stream_of(p.xc);
+      for (int64_t v0 = 0; v0 < p.vocab; v0 += piece) {
+        const int64_t vc = std::min(piece, p.vocab - v0), ldd = abi.xent_pitch(p.dt, vc);
+        check(abi.xent_dlogits(s, p.dt, p.xc.data_ptr(), p.n, p.width, p.act(), p.tgt(), p.count(), p.w.data_ptr(),
+                               p.w.stride(0), p.vocab, softcap, v0, vc, (const float*)lse.data_ptr(),
+                               (const float*)g.data_ptr(), stride, over, d.data_ptr(), ldd),
+              "odp_xent_dlogits");
+        if (need_x)
+          check(abi.xent_dx(s, p.dt, p.n, p.width, p.count(), p.w.data_ptr(), p.w.stride(0), p.vocab, v0, vc, piece,
+                            d.data_ptr(), ldd, sums.data_ptr()),
+                "odp_xent_dx");
+        if (need_w)
+          check(abi.xent_dw(s, p.dt, p.xc.data_ptr(), p.n, p.width, p.count(), vc, d.data_ptr(), ldd,
+                            (char*)dw.data_ptr() + v0 * p.width * es, p.width),
+                "odp_xent_dw");
+      }
+      if (need_x)
+        check(abi.xent_dx_rows(s, p.dt, p.n, p.cols, p.width, p.count(), p.where(), piece, sums.data_ptr(),
+                               dx.data_ptr()),
+              "odp_xent_dx_rows");
+      if (need_w && p.cols != p.width) dw = dw.narrow(1, 0, p.cols).contiguous();
+    }
+    return {first_only(grads[0], dx), first_only(grads[0], dw), {}, {}, {}, {}, {}};
+  }
+};
+
+at::Tensor cross_entropy(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target, double softcap,
+                         int64_t ignore, int64_t reduction, int64_t piece_bytes) {
+  py::gil_scoped_release nogil;
+  if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad()))
+    return Xent::apply(x, weight, target, softcap, ignore, reduction, piece_bytes);
+  const c10::OptionalDeviceGuard guard(x.device());
+  return xent_result(xent_forward(x, weight, target, softcap, ignore), reduction);
+}
+
+}  // namespace
+
+void add_vocabulary(py::module_& m) {
+  m.def("bind", &bind, py::arg("entry_points"));
+  m.def("embedding", &embedding, py::arg("tokens"), py::arg("weight"), py::arg("scale"), py::arg("padding"));
+  m.def("cross_entropy", &cross_entropy, py::arg("x"), py::arg("weight"), py::arg("target"), py::arg("softcap"),
+        py::arg("ignore"), py::arg("reduction"), py::arg("piece_bytes"));
+}

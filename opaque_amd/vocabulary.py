@@ -9,16 +9,20 @@ gradients, where ``vmap(grad)`` would make a dense [examples, vocabulary,
 width] gradient (opaque-engine/.../clipping/_clipped_fun.py:756-762).
 
 The work runs in the HIP kernels of ``libopaque_dp.so`` on the current
-stream; there is no CPU route.
+stream; there is no CPU route.  Outside torch.func the host helper makes the
+calls; inside it (and without the helper) the Functions below do, whose vmap
+rules merge the batch.
 """
 
 from __future__ import annotations
 
+import ctypes
 import functools
 import math
 
 import torch
 
+from opaque_amd import _host
 from opaque_amd import _native as N
 from opaque_amd.capture import SiteRecord, active_session
 from opaque_amd.engine import dtype_code
@@ -56,6 +60,20 @@ class _OnDevice:
     def __exit__(self, *exc) -> None:
         if self.ctx is not None:
             self.ctx.__exit__(*exc)
+
+
+_host_ready: list = []
+
+
+def _bound():
+    """The host helper with the library's entry points bound, or None when it has not been built."""
+    if not _host_ready:
+        host, lib = _host.load(), N.load()
+        if host is not None:
+            host.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
+                       for name in N.exported_symbols()})
+        _host_ready.append(host)
+    return _host_ready[0]
 
 
 def _transformed() -> bool:
@@ -120,22 +138,6 @@ def table_gradient(tokens: torch.Tensor, g: torch.Tensor, vocab: int, scale: flo
 def _front(t: torch.Tensor, d: int | None, size: int) -> torch.Tensor:
     """The vmapped axis first (a shared tensor is expanded)."""
     return t.unsqueeze(0).expand(size, *t.shape) if d is None else t.movedim(d, 0)
-
-
-class _EagerEmbed(torch.autograd.Function):
-    """scale * weight[tokens] outside torch.func."""
-
-    @staticmethod
-    def forward(ctx, tokens, weight, scale, padding):
-        ctx.save_for_backward(tokens)
-        ctx.args = weight.shape[0], scale, padding
-        return _embed_rows(tokens, weight, scale)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        (tokens,) = ctx.saved_tensors
-        return None, table_gradient(tokens, g, *ctx.args), None, None
 
 
 class _EmbedGrad(torch.autograd.Function):
@@ -248,11 +250,10 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
     if sess is not None and sess.mode == "discover":
         sess.uses[id(weight)] = sess.uses.get(id(weight), 0) + 1
         weight = weight.detach()
-    if _transformed():
-        return _Embed.apply(tokens, weight, float(scale), padding)
-    if weight.requires_grad and torch.is_grad_enabled():
-        return _EagerEmbed.apply(tokens, weight, float(scale), padding)
-    return _embed_rows(tokens, weight, float(scale))
+    host = None if _transformed() else _bound()
+    if host is not None:
+        return host.embedding(tokens, weight, scale, padding)
+    return _Embed.apply(tokens, weight, float(scale), padding)
 
 
 class Embedding(torch.nn.Embedding):
@@ -275,6 +276,7 @@ _HEAD_DTYPES = (torch.float32, torch.bfloat16)
 # Bytes of d (the logits' gradient, in the inputs' type) that the backward
 # holds at a time: a piece of the vocabulary for all tokens.
 PIECE_BYTES = 512 << 20
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 
 def _lanes(dtype: torch.dtype) -> int:
@@ -317,8 +319,7 @@ class _Packed:
         self.xc = torch.empty((room, self.width), dtype=x.dtype, device=dev)
         self.ids = torch.empty(3 * room + 2, dtype=torch.int32, device=dev)
         at = self.ids.data_ptr()
-        # How many rows are packed, then (float32) how many targets are not ignored.
-        self.count, self.counted = at, at + 4
+        self.count = at
         self.act, self.tgt, self.where = (at + 8 + 4 * k * room for k in range(3))
         _call("odp_xent_rows", _stream(x), self.dt, rows.data_ptr(), rows.stride(0), self.n, self.cols, self.width,
               flat.data_ptr(), flat.element_size(), self.vocab, ignore, int(keep), self.xc.data_ptr(), self.act,
@@ -332,12 +333,6 @@ class _Packed:
               self.tgt, self.count, self.w.data_ptr(), self.w.stride(0), self.vocab, softcap, scratch.data_ptr(),
               losses.data_ptr(), lse.data_ptr())
 
-    def reduced(self, losses: torch.Tensor, mean: bool) -> torch.Tensor:
-        out = torch.empty((), dtype=torch.float32, device=losses.device)
-        _call("odp_xent_reduce", _stream(losses), losses.data_ptr(), self.n, self.counted if mean else None,
-              out.data_ptr())
-        return out
-
     def piece(self, whole: bool = False) -> int:
         """Columns of the vocabulary a piece of d holds."""
         edge = _xent_pitch(self.dt, 1)
@@ -345,10 +340,9 @@ class _Packed:
         return self.vocab if whole else min(self.vocab, max(fit, edge))
 
     def gradients(self, softcap: float, lse: torch.Tensor, g: torch.Tensor, x_shape: torch.Size | None,
-                  need_w: bool, keep_d: bool = False, mean: bool = False):
+                  need_w: bool, keep_d: bool = False):
         """(dx, dW, d): dx where ``x_shape`` is given; d [n, vocab] where
-        ``keep_d`` (packed with ``keep``).  ``g`` holds one gradient per row,
-        or one for all, over the number of counted targets with ``mean``."""
+        ``keep_d`` (packed with ``keep``).  ``g`` holds one gradient per row."""
         dev, dtype, dt = self.xc.device, self.xc.dtype, self.dt
         piece = self.piece(keep_d)
         d = torch.empty((max(self.n, 1), _xent_pitch(dt, piece)), dtype=dtype, device=dev)
@@ -364,8 +358,7 @@ class _Packed:
             vc = min(piece, self.vocab - v0)
             ldd = _xent_pitch(dt, vc)
             _call("odp_xent_dlogits", s, dt, xc, self.n, self.width, self.act, self.tgt, self.count, w, ldw,
-                  self.vocab, softcap, v0, vc, lse.data_ptr(), g.data_ptr(), 1 if g.dim() else 0,
-                  self.counted if mean else None, d.data_ptr(), ldd)
+                  self.vocab, softcap, v0, vc, lse.data_ptr(), g.data_ptr(), 1, None, d.data_ptr(), ldd)
             if dx is not None:
                 _call("odp_xent_dx", s, dt, self.n, self.width, self.count, w, ldw, self.vocab, v0, vc, piece,
                       d.data_ptr(), ldd, sums.data_ptr())
@@ -381,11 +374,12 @@ class _Packed:
 
 
 def _xent_losses(x, weight, target, softcap, ignore):
-    losses, lse = torch.empty((2, *target.shape), dtype=torch.float32, device=x.device).unbind(0)
+    losses = torch.empty(target.shape, dtype=torch.float32, device=x.device)
+    lse = torch.empty_like(losses)
     with _OnDevice(x):
         p = _Packed(x, _head_rows(weight), target, ignore, False, losses, lse)
         p.losses(softcap, losses, lse)
-    return losses, lse, p
+    return losses, lse
 
 
 def _xent_gradients(g, x, weight, target, lse, softcap, ignore, need_x, need_w, keep_d=False):
@@ -393,32 +387,6 @@ def _xent_gradients(g, x, weight, target, lse, softcap, ignore, need_x, need_w, 
     with _OnDevice(x):
         p = _Packed(x, _head_rows(weight), target, ignore, keep_d)
         return p.gradients(softcap, lse, g, x.shape if need_x else None, need_w, keep_d)
-
-
-class _EagerXent(torch.autograd.Function):
-    """The reduced losses outside torch.func; the packed rows are kept for the backward."""
-
-    @staticmethod
-    def forward(ctx, x, weight, target, softcap, ignore, reduction):
-        out, lse, p = _xent_losses(x, weight, target, softcap, ignore)
-        if reduction != "none":
-            with _OnDevice(x):
-                out = p.reduced(out, reduction == "mean")
-        ctx.save_for_backward(weight)  # a later change of the head in place is an error
-        ctx.kept = p, lse, softcap, x.shape, reduction == "mean"
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        (weight,) = ctx.saved_tensors
-        p, lse, softcap, x_shape, mean = ctx.kept
-        need_x, need_w = ctx.needs_input_grad[:2]
-        if g.dim():
-            g = g.contiguous().reshape(-1)
-        with _OnDevice(weight):
-            dx, dw, _ = p.gradients(softcap, lse, g, x_shape if need_x else None, need_w, mean=mean)
-        return dx, dw, None, None, None, None
 
 
 class _XentGrad(torch.autograd.Function):
@@ -461,7 +429,7 @@ class _Xent(torch.autograd.Function):
 
     @staticmethod
     def forward(x, weight, target, softcap, ignore):
-        return _xent_losses(x, weight, target, softcap, ignore)[:2]
+        return _xent_losses(x, weight, target, softcap, ignore)
 
     @staticmethod
     def setup_context(ctx, inputs, output):
@@ -501,7 +469,7 @@ class _TapXent(torch.autograd.Function):
 
     @staticmethod
     def forward(x, weight, target, softcap, ignore, anchor, record):
-        return _xent_losses(x, weight, target, softcap, ignore)[:2]
+        return _xent_losses(x, weight, target, softcap, ignore)
 
     @staticmethod
     def setup_context(ctx, inputs, output):
@@ -536,7 +504,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     (opaque-patches/.../kernels/linear_cross_entropy.py:249).  Inside
     ``clipped_grad`` a trainable head reached only through it is a seam.
     """
-    if reduction not in ("none", "mean", "sum"):
+    if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
         raise ValueError(f"x [..., width] and weight [vocabulary, width] do not match: {tuple(x.shape)} and "
@@ -555,18 +523,13 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     if sess is not None and sess.mode == "discover":
         sess.uses[id(weight)] = sess.uses.get(id(weight), 0) + 1
         weight = weight.detach()
-    if not _transformed():
-        if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
-            return _EagerXent.apply(x, weight, target, float(softcap or 0.0), int(ignore_index), reduction)
-        losses, _, p = _xent_losses(x, weight, target, float(softcap or 0.0), int(ignore_index))
-        if reduction == "none":
-            return losses
-        with _OnDevice(x):
-            return p.reduced(losses, reduction == "mean")
+    host = None if _transformed() else _bound()
+    if host is not None:
+        return host.cross_entropy(x, weight, target, softcap or 0.0, ignore_index, _REDUCTIONS[reduction], PIECE_BYTES)
     losses, _ = _Xent.apply(x, weight, target, float(softcap or 0.0), int(ignore_index))
     if reduction == "none":
         return losses
-    total = losses.sum()
+    total = losses.double().sum().float()  # added in 64 bits and rounded once
     return total if reduction == "sum" else total / (target != ignore_index).sum()
 
 

@@ -321,3 +321,44 @@ def test_token_model_trains():
         opt.step()
         first = float(loss.detach()) if first is None else first
     assert float(loss.detach()) < 0.5 * first
+
+
+def test_without_the_host_helper(monkeypatch):
+    """The Functions with vmap rules take the calls outside torch.func when the helper is missing, with the same bits."""
+    x, w, y, gl = inputs(60, 72, 310, torch.bfloat16, seed=23)
+    toks = torch.randint(0, 310, (60,), device=DEV)
+
+    def all_of():
+        out = list(run(x, w, y, gl, 9.0))
+        xd, wd = x.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+        for reduction in ("sum", "mean"):
+            loss = linear_cross_entropy(xd, wd, y.to(DEV), reduction=reduction)
+            out += [loss.detach(), *torch.autograd.grad(loss, [xd, wd])]
+        e = embedding(toks, wd, scale=3.0, padding_idx=7)
+        out += [e.detach(), *torch.autograd.grad(e, [wd], torch.ones_like(e))]
+        return out
+
+    base = all_of()
+    monkeypatch.setattr(vocabulary, "_host_ready", [None])
+    for a, b in zip(all_of(), base):
+        assert torch.equal(a, b)
+
+
+def test_no_second_derivative():
+    x, w, y, gl = inputs(8, 16, 30, torch.float32, seed=5, ignored=0.0)
+    xd, wd = x.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+    (dx,) = torch.autograd.grad(linear_cross_entropy(xd, wd, y.to(DEV)).square(), [xd], create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dx.sum(), [xd])
+    (dw,) = torch.autograd.grad(embedding(y.to(DEV), wd).square().sum(), [wd], create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dw.sum(), [wd])
+
+
+def test_head_changed_before_the_backward():
+    x, w, y, gl = inputs(8, 16, 30, torch.float32, seed=5)
+    xd, wd = x.to(DEV).requires_grad_(), w.to(DEV)
+    loss = linear_cross_entropy(xd, wd, y.to(DEV))
+    wd.add_(1.0)
+    with pytest.raises(RuntimeError):
+        loss.backward()
