@@ -220,59 +220,78 @@ __device__ __forceinline__ void t_step(char* __restrict__ nxt, const char* __res
   }
 }
 
-// acc += A B^T over k in [0, kn).
+// The product of a tile in two parts: begin() issues the first steps' loads,
+// run() does the rest.  A workgroup that walks several tiles begins the next
+// one before it stores the last, so that the loads' latency passes beside the
+// epilogue (which must leave the ring alone).
 template <int DT, bool AKC, bool BKC>
-__device__ __forceinline__ void t_product(const Operand& A, const Operand& B, int32_t kn,
-                                          typename Tile<DT>::Acc& acc) {
+struct Product {
   using T = Tile<DT>;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  kn = (int32_t)t_uniform((uint32_t)kn);
   Loader<DT, AKC> la;
   Loader<DT, BKC> lb;
-  la.init(A, wave);
-  lb.init(B, wave);
-  int32_t kl = 0;  // first k of the next step to load
-  auto issue = [&](char* st, int l) __attribute__((always_inline)) {
+  int32_t kl, kn;  // first k of the next step to load, and the end
+  int wave;
+
+  __device__ __forceinline__ void issue(char* st, int l) const {
     if (l < T::DMA) la.issue(st, wave, l, kl, kn);
     else lb.issue(st + T::HALF, wave, l - T::DMA, kl, kn);
-  };
-  auto advance = [&]() __attribute__((always_inline)) {
+  }
+  __device__ __forceinline__ void advance() {
     kl += T::EK;
     la.at += la.step;
     lb.at += lb.step;
-  };
-#pragma unroll
-  for (int q = 0; q < T_RING - 1; ++q) {
-#pragma unroll
-    for (int l = 0; l < 2 * T::DMA; ++l) issue(t_stage<DT>(q), l);
-    advance();
   }
+
+  // The ring is idle (no wave reads it, no load into it is in flight).
+  __device__ __forceinline__ void begin(const Operand& A, const Operand& B, int32_t k) {
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    kn = (int32_t)t_uniform((uint32_t)k);
+    kl = 0;
+    la.init(A, wave);
+    lb.init(B, wave);
 #pragma unroll
-  for (int i = 0; i < T::BI; ++i)
+    for (int q = 0; q < T_RING - 1; ++q) {
 #pragma unroll
-    for (int j = 0; j < T::BJ; ++j) __asm__ volatile("" : "+v"(acc[i][j]));
-  Head<DT> h[2];
-  __builtin_amdgcn_s_waitcnt(vmcnt_imm((T_RING - 2) * 2 * T::DMA));
-  __asm__ volatile("s_barrier" ::: "memory");
-  t_head<DT, AKC, BKC>(t_stage<DT>(0), h[0]);
-  int32_t k = 0;
-  while (k < kn) {
-#pragma unroll
-    for (int u = 0; u < T_RING; ++u) {
-      if (k >= kn) break;
-      // The next step's loads have landed (this wave's; the barrier says so
-      // for the others); those of the step after may fly.
-      __builtin_amdgcn_s_waitcnt(vmcnt_imm((T_RING - 3) * 2 * T::DMA));
-      __asm__ volatile("s_barrier" ::: "memory");
-      t_step<DT, AKC, BKC>(t_stage<DT>((u + T_RING - 1) % T_RING), t_stage<DT>(u % T_RING),
-                           t_stage<DT>((u + 1) % T_RING), issue, h[u & 1], h[(u + 1) & 1], acc);
+      for (int l = 0; l < 2 * T::DMA; ++l) issue(t_stage<DT>(q), l);
       advance();
-      k += T::EK;
     }
   }
-  __builtin_amdgcn_s_waitcnt(0);  // no load into LDS may outlive the workgroup
-  __asm__ volatile("s_barrier" ::: "memory");
-}
+
+  // acc = A B^T over k in [0, kn).
+  __device__ __forceinline__ void run(typename T::Acc& acc) {
+#pragma unroll
+    for (int i = 0; i < T::BI; ++i)
+#pragma unroll
+      for (int j = 0; j < T::BJ; ++j) {
+        acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        __asm__ volatile("" : "+v"(acc[i][j]));
+      }
+    Head<DT> h[2];
+    // Everything so far, an epilogue's stores among it.
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    __asm__ volatile("s_barrier" ::: "memory");
+    t_head<DT, AKC, BKC>(t_stage<DT>(0), h[0]);
+    int32_t k = 0;
+    while (k < kn) {
+#pragma unroll
+      for (int u = 0; u < T_RING; ++u) {
+        if (k >= kn) break;
+        // The next step's loads have landed (this wave's; the barrier says so
+        // for the others); those of the step after may fly.
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm((T_RING - 3) * 2 * T::DMA));
+        __asm__ volatile("s_barrier" ::: "memory");
+        t_step<DT, AKC, BKC>(t_stage<DT>((u + T_RING - 1) % T_RING), t_stage<DT>(u % T_RING),
+                             t_stage<DT>((u + 1) % T_RING),
+                             [&](char* st, int l) __attribute__((always_inline)) { issue(st, l); }, h[u & 1],
+                             h[(u + 1) & 1], acc);
+        advance();
+        k += T::EK;
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(0);  // no load into LDS may outlive the tile
+    __asm__ volatile("s_barrier" ::: "memory");
+  }
+};
 
 // Entry e of block (i, j) of the wave's accumulators is row o = 16 i +
 // (lane & 15) and column n = 16 j + 4 (lane >> 4) + e of the wave's block.
@@ -289,12 +308,4 @@ __device__ __forceinline__ void static_for(F&& f) {
     f(Idx<K>{});
     static_for<N, K + 1>(f);
   }
-}
-
-template <int I, int J>
-__device__ __forceinline__ void t_zero(f32x4_t (&acc)[I][J]) {
-#pragma unroll
-  for (int i = 0; i < I; ++i)
-#pragma unroll
-    for (int j = 0; j < J; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 }

@@ -23,20 +23,28 @@ namespace {
 
 constexpr float LOG2E = 1.44269504088896340736f;
 
-// The tile of a workgroup, from `tiles` = tm x tn tiles of which only those
-// of the live tokens are walked: XCD j (blockIdx % 8) takes the j-th eighth,
-// in groups of 8 tile rows walked column by column, so that the tiles one L2
-// serves at a time share operands.  False for the workgroups past the end.
-__device__ __forceinline__ bool tile_of(int bid, int tm, int tn, int& ti, int& tj) {
-  const int tiles = tm * tn, nblk = (tiles + 7) / 8;
-  if (bid >= 8 * nblk) return false;
-  const int p = (bid & 7) * nblk + (bid >> 3);
-  if (p >= tiles) return false;
-  const int per = 8 * tn, g = p / per, gm = min(tm - 8 * g, 8), r = p - g * per;
-  ti = 8 * g + r % gm;
-  tj = r / gm;
-  return true;
-}
+// The tiles a workgroup walks, of tm x tn: XCD j (blockIdx % 8) takes the j-th
+// eighth, its workgroups one tile each in turn, in groups of 8 tile rows
+// walked column by column, so that the tiles one L2 serves at a time share
+// operands.
+struct Walk {
+  int tm, tn, each, at, step;
+  __device__ __forceinline__ Walk(int tm_, int tn_) : tm(tm_), tn(tn_) {
+    each = (tm * tn + 7) / 8;
+    at = blockIdx.x >> 3;
+    step = gridDim.x >> 3;
+  }
+  // The tile at the walk's place; false past the end.
+  __device__ __forceinline__ bool tile(int& ti, int& tj) const {
+    const int p = (blockIdx.x & 7) * each + at;
+    if (at >= each || p >= tm * tn) return false;
+    const int per = 8 * tn, g = p / per, gm = min(tm - 8 * g, 8), r = p - g * per;
+    ti = 8 * g + r % gm;
+    tj = r / gm;
+    return true;
+  }
+  __device__ __forceinline__ void next() { at += step; }
+};
 
 __device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
 
@@ -143,43 +151,40 @@ struct Xent {
 // Forward: per (row, tile of the vocabulary) the maximum and the sum of
 // exponentials below it, and each row's target logit.
 // ---------------------------------------------------------------------------
-template <int DT>
-__global__ __launch_bounds__(Tile<DT>::THREADS, 2) void k_xent_stats(Xent p, float* __restrict__ pmax,
-                                                                     float* __restrict__ psum,
-                                                                     float* __restrict__ ztgt) {
+template <int DT, bool CAP, bool WHOLE>
+__device__ __forceinline__ void stats_tile(const Xent& p, const typename Tile<DT>::Acc& acc, int cnt, int64_t o0,
+                                           int64_t n0, const int32_t (&tgt)[Tile<DT>::BI], float* red,
+                                           float* __restrict__ ztgt) {
   using T = Tile<DT>;
-  const int cnt = *(const ODP_CONST int32_t*)p.count;
-  int ti, tj;
-  if (!tile_of(blockIdx.x, (cnt + T::ET - 1) / T::ET, (int)((p.vocab + T::ET - 1) / T::ET), ti, tj)) return;
-  const int64_t o0 = (int64_t)ti * T::ET, n0 = (int64_t)tj * T::ET;
-  typename T::Acc acc;
-  t_zero(acc);
-  t_product<DT, true, true>(Operand{p.xc, p.width, o0, cnt}, Operand{p.w, p.ldw, n0, p.vocab}, (int32_t)p.width, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = T::WM * (wave & 1), wn = T::WN * (wave >> 1);
-  float* red = (float*)t_stage<DT>(0);  // [waves across n][ET rows][2]
-  static_for<T::BI>([&](auto ii) {
+  // Columns of this lane are c0 + 16 j + e of the tile; `edge` columns of it exist.
+  const int c0 = wn + t_col(0), edge = (int)min((int64_t)T::ET, p.vocab - n0);
+  static_for<T::BI>([&](auto ii) __attribute__((always_inline)) {
     constexpr int i = decltype(ii)::value;
-    const int64_t o = o0 + wm + t_row(i);
-    const int32_t tgt = o < cnt ? p.tgt[o] : -1;
-    float z[T::BJ][4], m = -INFINITY;
+    // The row's target, counted from c0 (no column of the lane for none here).
+    const int at = tgt[i] - (int)n0 - c0;
+    float z[T::BJ][4], m = -INFINITY, zt = 0.f;
+    bool here = false;
 #pragma unroll
     for (int j = 0; j < T::BJ; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int64_t n = n0 + wn + t_col(j) + e;
         float v = acc[i][j][e];
-        if (p.cap != 0.f) v = softcapped(v, p.cap, p.inv_cap2);
-        if (n == tgt) ztgt[o] = v;
-        z[j][e] = n < p.vocab ? v : -INFINITY;
+        if (CAP) v = softcapped(v, p.cap, p.inv_cap2);
+        const bool hit = at == 16 * j + e;
+        zt = hit ? v : zt;
+        here |= hit;
+        z[j][e] = WHOLE || c0 + 16 * j + e < edge ? v : -INFINITY;
         m = fmaxf(m, z[j][e]);
       }
-    const float ms = m == -INFINITY ? 0.f : m;
+    if (here) ztgt[o0 + wm + t_row(i)] = zt;
+    const float ms = m == -INFINITY ? 0.f : m * LOG2E;
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < T::BJ; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s += fast_exp(z[j][e] - ms);
+      for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(__builtin_fmaf(z[j][e], LOG2E, -ms));
     // The row's other columns of this wave: lanes 16, 32 and 48 further on.
 #pragma unroll
     for (int off = 16; off <= 32; off <<= 1) {
@@ -195,18 +200,51 @@ __global__ __launch_bounds__(Tile<DT>::THREADS, 2) void k_xent_stats(Xent p, flo
     }
     __builtin_amdgcn_sched_barrier(0);
   });
-  __syncthreads();
-  for (int r = threadIdx.x; r < T::ET; r += T::THREADS) {
-    if (o0 + r >= cnt) break;
-    float m = -INFINITY, s = 0.f;
+}
+
+template <int DT, bool CAP>
+__global__ __launch_bounds__(Tile<DT>::THREADS, 2) void k_xent_stats(Xent p, float* __restrict__ pmax,
+                                                                     float* __restrict__ psum,
+                                                                     float* __restrict__ ztgt) {
+  using T = Tile<DT>;
+  __shared__ float red[T::WAVES / 2 * T::ET * 2];  // [waves across n][rows][maximum, sum]
+  const int cnt = *(const ODP_CONST int32_t*)p.count;
+  Walk walk((cnt + T::ET - 1) / T::ET, (int)((p.vocab + T::ET - 1) / T::ET));
+  const int wm = T::WM * ((threadIdx.x >> 6) & 1);
+  Product<DT, true, true> prod;
+  int ti, tj;
+  auto begin = [&]() {
+    prod.begin(Operand{p.xc, p.width, (int64_t)ti * T::ET, cnt}, Operand{p.w, p.ldw, (int64_t)tj * T::ET, p.vocab},
+               (int32_t)p.width);
+  };
+  bool more = walk.tile(ti, tj);
+  if (more) begin();
+  while (more) {
+    const int64_t o0 = (int64_t)ti * T::ET, n0 = (int64_t)tj * T::ET;
+    typename T::Acc acc;
+    prod.run(acc);
+    int32_t tgt[T::BI];
 #pragma unroll
-    for (int w = 0; w < T::WAVES / 2; ++w) m = fmaxf(m, red[2 * (w * T::ET + r)]);
-    const float ref = m == -INFINITY ? 0.f : m;
+    for (int i = 0; i < T::BI; ++i) tgt[i] = o0 + wm + t_row(i) < cnt ? p.tgt[o0 + wm + t_row(i)] : -1;
+    const int column = tj;
+    walk.next();
+    more = walk.tile(ti, tj);
+    if (more) begin();
+    if (n0 + T::ET <= p.vocab) stats_tile<DT, CAP, true>(p, acc, cnt, o0, n0, tgt, red, ztgt);
+    else stats_tile<DT, CAP, false>(p, acc, cnt, o0, n0, tgt, red, ztgt);
+    __syncthreads();
+    for (int r = threadIdx.x; r < T::ET; r += T::THREADS) {
+      if (o0 + r >= cnt) break;
+      float m = -INFINITY, s = 0.f;
 #pragma unroll
-    for (int w = 0; w < T::WAVES / 2; ++w)
-      s += red[2 * (w * T::ET + r) + 1] * fast_exp(red[2 * (w * T::ET + r)] - ref);
-    pmax[(int64_t)tj * p.n + o0 + r] = m;
-    psum[(int64_t)tj * p.n + o0 + r] = s;
+      for (int w = 0; w < T::WAVES / 2; ++w) m = fmaxf(m, red[2 * (w * T::ET + r)]);
+      const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int w = 0; w < T::WAVES / 2; ++w)
+        s += red[2 * (w * T::ET + r) + 1] * fast_exp(red[2 * (w * T::ET + r)] - ref);
+      pmax[(int64_t)column * p.n + o0 + r] = m;
+      psum[(int64_t)column * p.n + o0 + r] = s;
+    }
   }
 }
 
@@ -258,9 +296,15 @@ __global__ __launch_bounds__(1024) void k_xent_reduce(const float* __restrict__ 
 
 // ---------------------------------------------------------------------------
 // Stores of a tile in the operands' type: rows o (of `rows`) of pitch ld from
-// row o0, columns n0 + .. below `cols`, val(i, j, e) the entries.  16-bit
-// tiles go through the idle ring so that rows leave in 16-byte pieces.
+// row o0, columns n0 + .. below `cols`, val(i, j) the blocks' entries.  16-bit
+// tiles go through LDS beside the ring, 32 rows of a wave at a time, so that
+// rows leave in 16-byte pieces.
 // ---------------------------------------------------------------------------
+template <int N>
+__device__ __forceinline__ uint16_t* t_staged() {
+  __shared__ __attribute__((aligned(16))) uint16_t s[N];
+  return s;
+}
 template <int DT, typename Val>
 __device__ __forceinline__ void t_store(void* out, int64_t ld, int64_t o0, int64_t rows, int64_t n0, int64_t cols,
                                         Val val) {
@@ -268,7 +312,7 @@ __device__ __forceinline__ void t_store(void* out, int64_t ld, int64_t o0, int64
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = T::WM * (wave & 1), wn = T::WN * (wave >> 1);
   if constexpr (DT == ODP_DTYPE_F32) {
-    static_for<T::BI * T::BJ>([&](auto q) {
+    static_for<T::BI * T::BJ>([&](auto q) __attribute__((always_inline)) {
       constexpr int i = decltype(q)::value / T::BJ, j = decltype(q)::value % T::BJ;
       const int64_t o = o0 + wm + t_row(i), n = n0 + wn + t_col(j);
       const f32x4_t v = val(Idx<i>{}, Idx<j>{});
@@ -276,22 +320,27 @@ __device__ __forceinline__ void t_store(void* out, int64_t ld, int64_t o0, int64
       __builtin_amdgcn_sched_barrier(0);
     });
   } else {
-    uint16_t* stg = (uint16_t*)(t_stage<DT>(wave >> 1) + (wave & 1) * (T::WM * T::WN * 2));
-    static_for<T::BI * T::BJ>([&](auto q) {
-      constexpr int i = decltype(q)::value / T::BJ, j = decltype(q)::value % T::BJ;
-      const f32x4_t v = val(Idx<i>{}, Idx<j>{});
-      const int r = t_row(i), c = t_col(j);
-      *(u32x2_alias_t*)&stg[r * T::WN + 8 * ((c >> 3) ^ (r & 7)) + (c & 7)] =
-          u32x2_t{odp_f2bf2(v[0], v[1]), odp_f2bf2(v[2], v[3])};
+    constexpr int PART = 32 * T::WN;  // elements of a wave's 32 rows
+    uint16_t* stg = t_staged<T::WAVES * PART>() + wave * PART;
+    static_for<T::BI / 2>([&](auto hh) __attribute__((always_inline)) {
+      constexpr int h = decltype(hh)::value;
+      static_for<2 * T::BJ>([&](auto q) __attribute__((always_inline)) {
+        constexpr int ib = decltype(q)::value / T::BJ, j = decltype(q)::value % T::BJ;
+        const f32x4_t v = val(Idx<2 * h + ib>{}, Idx<j>{});
+        const int r = t_row(ib), c = t_col(j);
+        *(u32x2_alias_t*)&stg[r * T::WN + 8 * ((c >> 3) ^ (r & 7)) + (c & 7)] =
+            u32x2_t{odp_f2bf2(v[0], v[1]), odp_f2bf2(v[2], v[3])};
+        __builtin_amdgcn_sched_barrier(0);
+      });
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int r = 8 * k + (lane >> 3), c = lane & 7;
+        const u32x4_t v = *(const u32x4_alias_t*)&stg[r * T::WN + 8 * (c ^ (r & 7))];
+        const int64_t o = o0 + wm + 32 * h + r, n = n0 + wn + 8 * c;
+        if (o < rows && n < cols) odp_gstore((u32x4_t*)((uint16_t*)out + o * ld + n), v);
+      }
       __builtin_amdgcn_sched_barrier(0);
     });
-#pragma unroll
-    for (int k = 0; k < T::WM / 8; ++k) {
-      const int r = 8 * k + (lane >> 3), c = lane & 7;
-      const u32x4_t v = *(const u32x4_alias_t*)&stg[r * T::WN + 8 * (c ^ (r & 7))];
-      const int64_t o = o0 + wm + r, n = n0 + wn + 8 * c;
-      if (o < rows && n < cols) odp_gstore((u32x4_t*)((uint16_t*)out + o * ld + n), v);
-    }
   }
 }
 
@@ -300,6 +349,42 @@ __device__ __forceinline__ void t_store(void* out, int64_t ld, int64_t o0, int64
 // zeros up to ldd (a multiple of the tile).
 // ---------------------------------------------------------------------------
 template <int DT>
+struct DRows {  // of a lane's rows of a tile
+  float lse[Tile<DT>::BI], g[Tile<DT>::BI];  // log-sum-exp (in powers of 2), gradient
+  int32_t tgt[Tile<DT>::BI];                 // target less the piece's first column
+};
+constexpr int32_t NO_LOSS = INT32_MIN;  // a target may lie anywhere beside the piece
+
+template <int DT, bool CAP, bool WHOLE>
+__device__ __forceinline__ void dlogits_tile(const Xent& p, const typename Tile<DT>::Acc& acc, const DRows<DT>& rows,
+                                             int cnt, int64_t o0, int64_t n0, int64_t vc, void* dl, int64_t ldd) {
+  using T = Tile<DT>;
+  const int wn = T::WN * (threadIdx.x >> 7);
+  // Columns of this lane are c0 + 16 j + e of the tile; `edge` columns of it exist.
+  const int c0 = wn + t_col(0), edge = (int)min((int64_t)T::ET, vc - n0);
+  const float inv_cap = 0.5f * p.inv_cap2;
+  t_store<DT>(dl, ldd, o0, cnt, n0, ldd, [&](auto ii, auto jj) __attribute__((always_inline)) {
+    constexpr int i = decltype(ii)::value, j = decltype(jj)::value;
+    const int at = rows.tgt[i] - (int)n0 - c0;
+    const bool live = rows.tgt[i] != NO_LOSS;
+    f32x4_t d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float z = acc[i][j][e];
+      if (CAP) z = softcapped(z, p.cap, p.inv_cap2);
+      float q = __builtin_amdgcn_exp2f(__builtin_fmaf(z, LOG2E, -rows.lse[i]));
+      q = (at == 16 * j + e ? q - 1.f : q) * rows.g[i];
+      if (CAP) {
+        const float y = z * inv_cap;
+        q *= 1.f - y * y;
+      }
+      d[e] = live && (WHOLE || c0 + 16 * j + e < edge) ? q : 0.f;
+    }
+    return d;
+  });
+}
+
+template <int DT, bool CAP>
 __global__ __launch_bounds__(Tile<DT>::THREADS, 2) void k_xent_dlogits(Xent p, int64_t v0, int64_t vc,
                                                                        const float* __restrict__ lse,
                                                                        const float* __restrict__ g, int g_stride,
@@ -307,46 +392,38 @@ __global__ __launch_bounds__(Tile<DT>::THREADS, 2) void k_xent_dlogits(Xent p, i
                                                                        int64_t ldd) {
   using T = Tile<DT>;
   const int cnt = *(const ODP_CONST int32_t*)p.count;
-  int ti, tj;
-  if (!tile_of(blockIdx.x, (cnt + T::ET - 1) / T::ET, (int)(ldd / T::ET), ti, tj)) return;
-  const int64_t o0 = (int64_t)ti * T::ET, n0 = (int64_t)tj * T::ET;
-  typename T::Acc acc;
-  t_zero(acc);
+  Walk walk((cnt + T::ET - 1) / T::ET, (int)(ldd / T::ET));
+  const int wm = T::WM * ((threadIdx.x >> 6) & 1);
   const void* w = (const char*)p.w + v0 * p.ldw * T::ES;
-  t_product<DT, true, true>(Operand{p.xc, p.width, o0, cnt}, Operand{w, p.ldw, n0, vc}, (int32_t)p.width, acc);
-  const int wave = threadIdx.x >> 6;
-  const int wm = T::WM * (wave & 1), wn = T::WN * (wave >> 1);
-  float rl[T::BI], rg[T::BI];
-  constexpr int32_t NONE = INT32_MIN;  // no loss: a target may lie just below the piece
-  int32_t rt[T::BI];
+  const float part = over != nullptr ? *over : 1.f;
+  Product<DT, true, true> prod;
+  int ti, tj;
+  auto begin = [&]() {
+    prod.begin(Operand{p.xc, p.width, (int64_t)ti * T::ET, cnt}, Operand{w, p.ldw, (int64_t)tj * T::ET, vc},
+               (int32_t)p.width);
+  };
+  bool more = walk.tile(ti, tj);
+  if (more) begin();
+  while (more) {
+    const int64_t o0 = (int64_t)ti * T::ET, n0 = (int64_t)tj * T::ET;
+    typename T::Acc acc;
+    prod.run(acc);
+    DRows<DT> rows;
 #pragma unroll
-  for (int i = 0; i < T::BI; ++i) {
-    const int64_t o = o0 + wm + t_row(i);
-    const int32_t t = o < cnt ? p.tgt[o] : -1;
-    const int64_t row = o < cnt ? p.act[o] : 0;
-    rl[i] = t >= 0 ? lse[row] : 0.f;
-    rg[i] = t >= 0 ? g[row * g_stride] : 0.f;
-    if (over != nullptr) rg[i] = rg[i] / *over;
-    rt[i] = t >= 0 ? t - (int32_t)v0 : NONE;
-  }
-  const float inv_cap = 0.5f * p.inv_cap2;
-  t_store<DT>(dl, ldd, o0, cnt, n0, ldd, [&](auto ii, auto jj) __attribute__((always_inline)) {
-    constexpr int i = decltype(ii)::value, j = decltype(jj)::value;
-    f32x4_t d;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int64_t n = n0 + wn + t_col(j) + e;
-      float z = acc[i][j][e], slope = 1.f;
-      if (p.cap != 0.f) {
-        z = softcapped(z, p.cap, p.inv_cap2);
-        const float y = z * inv_cap;
-        slope = 1.f - y * y;
-      }
-      const float q = fast_exp(z - rl[i]) - (n == (int64_t)rt[i] ? 1.f : 0.f);
-      d[e] = rt[i] != NONE && n < vc ? rg[i] * q * slope : 0.f;
+    for (int i = 0; i < T::BI; ++i) {
+      const int64_t o = o0 + wm + t_row(i);
+      const int32_t t = o < cnt ? p.tgt[o] : -1;
+      const int64_t row = o < cnt ? p.act[o] : 0;
+      rows.lse[i] = t >= 0 ? lse[row] * LOG2E : 0.f;
+      rows.g[i] = t >= 0 ? g[row * g_stride] / part : 0.f;
+      rows.tgt[i] = t >= 0 ? t - (int32_t)v0 : NO_LOSS;
     }
-    return d;
-  });
+    walk.next();
+    more = walk.tile(ti, tj);
+    if (more) begin();
+    if (n0 + T::ET <= vc) dlogits_tile<DT, CAP, true>(p, acc, rows, cnt, o0, n0, vc, dl, ldd);
+    else dlogits_tile<DT, CAP, false>(p, acc, rows, cnt, o0, n0, vc, dl, ldd);
+  }
 }
 
 // How many slices of the contraction each tile of dx is split into: the
@@ -372,7 +449,7 @@ __global__ __launch_bounds__(Tile<DT>::THREADS, 2) void k_xent_dx(Xent p, int64_
   if (tm == 0) return;
   const int split = dx_split(tm * tn, cap, piece / T::EK);
   int ti, tj;
-  if (!tile_of(blockIdx.x, tm, tn * split, ti, tj)) return;
+  if (!Walk(tm, tn * split).tile(ti, tj)) return;  // a workgroup per tile
   const int s = tj / tn;
   tj -= s * tn;
   const int64_t o0 = (int64_t)ti * T::ET, n0 = (int64_t)tj * T::ET;
@@ -381,9 +458,10 @@ __global__ __launch_bounds__(Tile<DT>::THREADS, 2) void k_xent_dx(Xent p, int64_
   const int32_t kn = (int32_t)max((int64_t)0, min(per, vc - k0));
   if (kn == 0 && !first) return;
   typename T::Acc acc;
-  t_zero(acc);
-  t_product<DT, true, false>(Operand{(const char*)dl + k0 * T::ES, ldd, o0, cnt},
-                             Operand{(const char*)p.w + (v0 + k0) * p.ldw * T::ES, p.ldw, n0, p.width}, kn, acc);
+  Product<DT, true, false> prod;
+  prod.begin(Operand{(const char*)dl + k0 * T::ES, ldd, o0, cnt},
+             Operand{(const char*)p.w + (v0 + k0) * p.ldw * T::ES, p.ldw, n0, p.width}, kn);
+  prod.run(acc);
   const int wave = threadIdx.x >> 6;
   const int wm = T::WM * (wave & 1), wn = T::WN * (wave >> 1);
   float* out = slots + (int64_t)s * cnt * p.width;
@@ -437,15 +515,25 @@ __global__ __launch_bounds__(Tile<DT>::THREADS, 2) void k_xent_dw(Xent p, int64_
                                                                   void* dw, int64_t lddw) {
   using T = Tile<DT>;
   const int cnt = *(const ODP_CONST int32_t*)p.count;
+  Walk walk((int)((vc + T::ET - 1) / T::ET), (int)((p.width + T::ET - 1) / T::ET));
+  Product<DT, false, false> prod;
   int ti, tj;
-  if (!tile_of(blockIdx.x, (int)((vc + T::ET - 1) / T::ET), (int)((p.width + T::ET - 1) / T::ET), ti, tj)) return;
-  const int64_t o0 = (int64_t)ti * T::ET, n0 = (int64_t)tj * T::ET;
-  typename T::Acc acc;
-  t_zero(acc);
-  t_product<DT, false, false>(Operand{dl, ldd, o0, ldd}, Operand{p.xc, p.width, n0, p.width}, cnt, acc);
-  t_store<DT>(dw, lddw, o0, vc, n0, p.width, [&](auto ii, auto jj) __attribute__((always_inline)) {
-    return acc[decltype(ii)::value][decltype(jj)::value];
-  });
+  auto begin = [&]() {
+    prod.begin(Operand{dl, ldd, (int64_t)ti * T::ET, ldd}, Operand{p.xc, p.width, (int64_t)tj * T::ET, p.width}, cnt);
+  };
+  bool more = walk.tile(ti, tj);
+  if (more) begin();
+  while (more) {
+    const int64_t o0 = (int64_t)ti * T::ET, n0 = (int64_t)tj * T::ET;
+    typename T::Acc acc;
+    prod.run(acc);
+    walk.next();
+    more = walk.tile(ti, tj);
+    if (more) begin();
+    t_store<DT>(dw, lddw, o0, vc, n0, p.width, [&](auto ii, auto jj) __attribute__((always_inline)) {
+      return acc[decltype(ii)::value][decltype(jj)::value];
+    });
+  }
 }
 
 int check_xent(const char* what, int dtype, int64_t n, int64_t width, int64_t ldw, int64_t vocab) {
@@ -465,14 +553,15 @@ int check_xent(const char* what, int dtype, int64_t n, int64_t width, int64_t ld
 
 int tile_edge(int dtype) { return dtype == ODP_DTYPE_F32 ? 128 : 256; }
 
-// Workgroups of a tm x tn grid of tiles (tile_of).
-int grid_of(const char* what, int64_t tm, int64_t tn, unsigned& blocks) {
-  const int64_t b = (tm * tn + 7) / 8 * 8;
-  if (b >= (int64_t)1 << 23) {
-    odp_set_error("%s: the launch needs %lld workgroups", what, (long long)b);
+// Workgroups that walk a tm x tn grid of tiles: as many as the CUs hold at a
+// time (one of 16-bit tiles a CU, two of float32), or one a tile (`all`).
+int grid_of(const char* what, int dtype, int64_t tm, int64_t tn, bool all, unsigned& blocks) {
+  const int64_t b = (tm * tn + 7) / 8 * 8, held = dtype == ODP_DTYPE_F32 ? 512 : 256;
+  if (b >= (int64_t)1 << 31) {
+    odp_set_error("%s: %lld tiles", what, (long long)b);
     return ODP_ERR_UNSUPPORTED;
   }
-  blocks = (unsigned)b;
+  blocks = (unsigned)(all || b < held ? b : held);
   return ODP_OK;
 }
 
@@ -493,6 +582,19 @@ bool on16(const void* p) { return ((uintptr_t)p & 15) == 0; }
       hipLaunchKernelGGL((K<ODP_DTYPE_F32>), dim3(GRID), dim3(Tile<ODP_DTYPE_F32>::THREADS), 0, s, __VA_ARGS__); \
     else                                                                                                       \
       hipLaunchKernelGGL((K<ODP_DTYPE_BF16>), dim3(GRID), dim3(Tile<ODP_DTYPE_BF16>::THREADS), 0, s, __VA_ARGS__); \
+  } while (0)
+
+#define ODP_XENT_LAUNCH_CAP(K, GRID, ...)                                                                             \
+  do {                                                                                                                \
+    constexpr int F = ODP_DTYPE_F32, B = ODP_DTYPE_BF16;                                                              \
+    if (dtype == F && softcap != 0.f)                                                                                 \
+      hipLaunchKernelGGL((K<F, true>), dim3(GRID), dim3(Tile<F>::THREADS), 0, s, __VA_ARGS__);                        \
+    else if (dtype == F)                                                                                              \
+      hipLaunchKernelGGL((K<F, false>), dim3(GRID), dim3(Tile<F>::THREADS), 0, s, __VA_ARGS__);                       \
+    else if (softcap != 0.f)                                                                                          \
+      hipLaunchKernelGGL((K<B, true>), dim3(GRID), dim3(Tile<B>::THREADS), 0, s, __VA_ARGS__);                        \
+    else                                                                                                              \
+      hipLaunchKernelGGL((K<B, false>), dim3(GRID), dim3(Tile<B>::THREADS), 0, s, __VA_ARGS__);                       \
   } while (0)
 
 extern "C" int odp_xent_rows(odp_stream_t stream, int dtype, const void* x, int64_t ldx, int64_t n, int64_t cols,
@@ -553,12 +655,12 @@ extern "C" int odp_xent_losses(odp_stream_t stream, int dtype, const void* xc, i
   const hipStream_t s = odp_hip_stream(stream);
   const int64_t tn = up(vocab, tile_edge(dtype));
   unsigned blocks;
-  if (int rc = grid_of("odp_xent_losses", up(n, tile_edge(dtype)), tn, blocks)) return rc;
+  if (int rc = grid_of("odp_xent_losses", dtype, up(n, tile_edge(dtype)), tn, false, blocks)) return rc;
   const Xent p = xent_of(xc, w, ldw, vocab, width, n, count, act, tgt, softcap);
   float* pmax = (float*)scratch;
   float* psum = pmax + n * tn;
   float* ztgt = psum + n * tn;
-  ODP_XENT_LAUNCH(k_xent_stats, blocks, p, pmax, psum, ztgt);
+  ODP_XENT_LAUNCH_CAP(k_xent_stats, blocks, p, pmax, psum, ztgt);
   hipLaunchKernelGGL(k_xent_losses, dim3((unsigned)up(n, 16)), dim3(256), 0, s, pmax, psum, ztgt, (int)tn, n, count,
                      act, tgt, losses, lse);
   return odp_check_launch("odp_xent_losses");
@@ -595,9 +697,9 @@ extern "C" int odp_xent_dlogits(odp_stream_t stream, int dtype, const void* xc, 
   }
   const hipStream_t s = odp_hip_stream(stream);
   unsigned blocks;
-  if (int rc = grid_of("odp_xent_dlogits", up(n, tile_edge(dtype)), ldd / tile_edge(dtype), blocks)) return rc;
+  if (int rc = grid_of("odp_xent_dlogits", dtype, up(n, tile_edge(dtype)), ldd / tile_edge(dtype), false, blocks)) return rc;
   const Xent p = xent_of(xc, w, ldw, vocab, width, n, count, act, tgt, softcap);
-  ODP_XENT_LAUNCH(k_xent_dlogits, blocks, p, v0, vc, lse, g, g_stride, over, dl, ldd);
+  ODP_XENT_LAUNCH_CAP(k_xent_dlogits, blocks, p, v0, vc, lse, g, g_stride, over, dl, ldd);
   return odp_check_launch("odp_xent_dlogits");
 }
 
@@ -633,7 +735,7 @@ extern "C" int odp_xent_dx(odp_stream_t stream, int dtype, int64_t n, int64_t wi
   const int cap = dx_cap(dtype, n, width);
   const int64_t tiles = up(n, tile_edge(dtype)) * up(width, tile_edge(dtype));
   unsigned blocks;
-  if (int rc = grid_of("odp_xent_dx", tiles > cap ? tiles : cap, 1, blocks)) return rc;
+  if (int rc = grid_of("odp_xent_dx", dtype, tiles > cap ? tiles : cap, 1, true, blocks)) return rc;
   const Xent p = xent_of(nullptr, w, ldw, vocab, width, n, count, nullptr, nullptr, 0.f);
   const int64_t whole = odp_xent_pitch(dtype, piece);
   ODP_XENT_LAUNCH(k_xent_dx, blocks, p, v0, vc, whole, dl, ldd, cap, v0 == 0 ? 1 : 0, (float*)scratch);
@@ -683,7 +785,7 @@ extern "C" int odp_xent_dw(odp_stream_t stream, int dtype, const void* xc, int64
   }
   const hipStream_t s = odp_hip_stream(stream);
   unsigned blocks;
-  if (int rc = grid_of("odp_xent_dw", up(vc, tile_edge(dtype)), up(width, tile_edge(dtype)), blocks)) return rc;
+  if (int rc = grid_of("odp_xent_dw", dtype, up(vc, tile_edge(dtype)), up(width, tile_edge(dtype)), false, blocks)) return rc;
   const Xent p = xent_of(xc, nullptr, width, vc, width, n, count, nullptr, nullptr, 0.f);
   ODP_XENT_LAUNCH(k_xent_dw, blocks, p, vc, dl, ldd, dw, lddw);
   return odp_check_launch("odp_xent_dw");
