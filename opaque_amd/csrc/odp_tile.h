@@ -2,13 +2,14 @@
 // contraction: the products of the vocabulary loss.
 //
 // Included inside an anonymous namespace, after odp_internal.h.  A workgroup
-// owns an ET x ET tile of C (256 x 256 in bfloat16, 128 x 128 in float32):
-// rows o from A, columns n from B.  An operand is K-contiguous (KC: element
+// owns an OT x NT tile of C: rows o from A, columns n from B.  256 x 256 in
+// bfloat16 and 128 x 128 in float32; with S, for few rows, 64 x 128 and a ring
+// of more, smaller stages, since such a product waits for B's memory.  An operand is K-contiguous (KC: element
 // (row, k) at row * ld + k, as the rows of activations or of a weight) or
 // K-major (element (row, k) at k * ld + row: the contraction runs over the
 // rows of memory).  A step covers 64 bytes of k; both orders then stage the
-// same bytes, 64-byte rows of k or 512-byte rows of o or n, by buffer loads
-// straight into a ring of four LDS stages, three steps ahead of the MFMAs.
+// same bytes, 64-byte rows of k or rows of o or n, by buffer loads straight
+// into a ring of LDS stages, all but one step ahead of the MFMAs.
 #pragma once
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
@@ -22,21 +23,23 @@ typedef short v4i16_t __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t T_RSRC = 0x00020000;  // raw buffer resource, 32-bit offsets
 constexpr uint32_t T_OOB = 0x80000000u;  // an offset past every buffer's end: reads as zero
-constexpr int T_RING = 4;
 
-template <int DT>
+template <int DT, int S>
 struct Tile {
   static constexpr bool F32 = DT == ODP_DTYPE_F32;
   static constexpr int ES = F32 ? 4 : 2;          // bytes per element
-  static constexpr int ET = 512 / ES;             // rows (o) and columns (n) of the tile
+  static constexpr int OT = S ? 64 : 512 / ES;    // rows (o) of the tile
+  static constexpr int NT = S ? 128 : 512 / ES;   // columns (n)
   static constexpr int EK = 64 / ES;              // k per step
-  static constexpr int WAVES = F32 ? 4 : 8;       // 2 x (WAVES / 2) over the tile
+  static constexpr int WAVES = NT / 64 * 2;       // 2 x (WAVES / 2) over the tile
   static constexpr int THREADS = 64 * WAVES;
-  static constexpr int WM = ET / 2, WN = 64;      // a wave's block
+  static constexpr int WM = OT / 2, WN = 64;      // a wave's block
   static constexpr int BI = WM / 16, BJ = WN / 16;
-  static constexpr int HALF = 512 * EK;           // bytes of one operand's stage
-  static constexpr int STAGE = 2 * HALF;
-  static constexpr int DMA = HALF / 1024 / WAVES;  // 1 KB loads per wave, operand and step
+  static constexpr int ABYTES = OT * 64, BBYTES = NT * 64, STAGE = ABYTES + BBYTES;  // of a step
+  static constexpr int ALOADS = ABYTES / 1024 / WAVES, BLOADS = BBYTES / 1024 / WAVES;  // 1 KB loads per wave
+  static constexpr int LOADS = ALOADS + BLOADS;
+  static constexpr int RING = S ? 6 : 4;
+  static_assert(ALOADS * WAVES * 1024 == ABYTES && BLOADS * WAVES * 1024 == BBYTES, "whole loads");
   typedef f32x4_t Acc[BI][BJ];
 };
 
@@ -47,16 +50,24 @@ __device__ __forceinline__ char* t_array() {
   __shared__ __attribute__((aligned(16))) char s[BYTES];
   return s;
 }
-template <int DT>
+template <int DT, int S>
 __device__ __forceinline__ char* t_stage(int k) {
-  constexpr int B = Tile<DT>::STAGE;
-  return k == 0 ? t_array<B, 0>() : k == 1 ? t_array<B, 1>() : k == 2 ? t_array<B, 2>() : t_array<B, 3>();
+  constexpr int B = Tile<DT, S>::STAGE;
+  if constexpr (S == 0)
+    return k == 0 ? t_array<B, 0>() : k == 1 ? t_array<B, 1>() : k == 2 ? t_array<B, 2>() : t_array<B, 3>();
+  else
+    return k == 0   ? t_array<B, 0>()
+           : k == 1 ? t_array<B, 1>()
+           : k == 2 ? t_array<B, 2>()
+           : k == 3 ? t_array<B, 3>()
+           : k == 4 ? t_array<B, 4>()
+                    : t_array<B, 5>();
 }
 
 // Swizzles.  64-byte rows of k: 16-byte slot s of row r lies at slot
 // s ^ ((r >> 1) & 3) (full rate for operand reads, measured on the Gram
-// kernels).  512-byte rows of 16-bit columns: 8-byte chunks XOR-ed as the
-// transposing reads of the full-weight kernels take them; of 32-bit columns:
+// kernels).  Rows of 16-bit columns: 8-byte chunks XOR-ed as the transposing
+// reads of the full-weight kernels take them; of 32-bit columns:
 // 64-byte groups XOR-ed with the row's quarter, so that the four rows a lane
 // group reads lie on different banks.
 __device__ __forceinline__ int t_kswz(int row) { return (row >> 1) & 3; }
@@ -67,8 +78,9 @@ __device__ __forceinline__ int t_cswz(int row) {  // in 16-byte pieces
 
 // The MFMA operand of 16 rows from row0 of a staged operand: lane & 15 = row,
 // 16 bytes of k per lane (the slot lane >> 4).
-template <int DT, bool KC>
+template <int DT, bool KC, int EXT>
 __device__ __forceinline__ u32x4_t t_frag(const char* half, int row0) {
+  constexpr int PITCH = EXT * (DT == ODP_DTYPE_F32 ? 4 : 2);  // bytes of a K-major row of EXT columns
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
   if constexpr (KC) {
     const int row = row0 + c;
@@ -78,16 +90,16 @@ __device__ __forceinline__ u32x4_t t_frag(const char* half, int row0) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int k = 4 * q + e;
-      v[e] = *(const uint32_t*)(half + k * 512 + 16 * (((row0 + c) >> 2) ^ t_cswz<DT>(k)) + 4 * (c & 3));
+      v[e] = *(const uint32_t*)(half + k * PITCH + 16 * (((row0 + c) >> 2) ^ t_cswz<DT>(k)) + 4 * (c & 3));
     }
     return v;
   } else {
     // Rows k and k + 4 share the swizzle; each read transposes a 4 x 16 block.
     const int k = 8 * q + (c >> 2);
     const int chunk = ((row0 >> 2) + (c & 3)) ^ (t_cswz<DT>(k) << 1);
-    const char* src = half + k * 512 + 8 * chunk;
+    const char* src = half + k * PITCH + 8 * chunk;
     const v4i16_t t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ODP_LDS v4i16_t*)(ODP_LDS void*)src);
-    const v4i16_t t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ODP_LDS v4i16_t*)(ODP_LDS void*)(src + 4 * 512));
+    const v4i16_t t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ODP_LDS v4i16_t*)(ODP_LDS void*)(src + 4 * PITCH));
     const v4i16_t tt[2] = {t0, t1};
     return __builtin_bit_cast(u32x4_t, tt);
   }
@@ -123,35 +135,36 @@ struct Operand {
   int64_t rows;
 };
 
-// What a lane needs to issue its loads of one operand.
-template <int DT, bool KC>
+// What a lane needs to issue its N loads of one operand, of EXT rows (o or n) a step.
+template <int DT, bool KC, int EXT, int N>
 struct Loader {
-  using T = Tile<DT>;
-  uint64_t at;       // base of the step's loads
-  uint32_t step;     // bytes the base moves per step
-  uint32_t ldb;      // bytes per row of memory
-  uint32_t off[T::DMA];
-  int32_t k8[T::DMA];  // KC: first k of the load's 16 bytes
+  static constexpr int ES = DT == ODP_DTYPE_F32 ? 4 : 2, EK = 64 / ES;
+  static constexpr int LPR = EXT * ES / 16, RPL = 64 / LPR;  // K-major: lanes per row, rows per load
+  uint64_t at;    // base of the step's loads
+  uint32_t step;  // bytes the base moves per step
+  uint32_t ldb;   // bytes per row of memory
+  uint32_t off[N];
+  int32_t k8[N];  // KC: first k of the load's 16 bytes
 
   __device__ __forceinline__ void init(const Operand& op, int wave) {
     const int lane = threadIdx.x & 63;
-    ldb = t_uniform((uint32_t)(op.ld * T::ES));
+    ldb = t_uniform((uint32_t)(op.ld * ES));
     if constexpr (KC) {
       at = t_uniform64((uint64_t)op.base + (uint64_t)op.row0 * ldb);
       step = 64;
 #pragma unroll
-      for (int i = 0; i < T::DMA; ++i) {
-        const int row = 16 * (T::DMA * wave + i) + (lane >> 2), slot = (lane & 3) ^ t_kswz(row);
+      for (int i = 0; i < N; ++i) {
+        const int row = 16 * (N * wave + i) + (lane >> 2), slot = (lane & 3) ^ t_kswz(row);
         off[i] = op.row0 + row < op.rows ? (uint32_t)row * ldb + 16u * slot : T_OOB;
-        k8[i] = slot * (16 / T::ES);
+        k8[i] = slot * (16 / ES);
       }
     } else {
-      at = t_uniform64((uint64_t)op.base + (uint64_t)op.row0 * T::ES);
-      step = t_uniform(ldb * T::EK);
+      at = t_uniform64((uint64_t)op.base + (uint64_t)op.row0 * ES);
+      step = t_uniform(ldb * EK);
 #pragma unroll
-      for (int i = 0; i < T::DMA; ++i) {
-        const int k = 2 * (T::DMA * wave + i) + (lane >> 5);
-        const int piece = (lane & 31) ^ t_cswz<DT>(k), col = piece * (16 / T::ES);
+      for (int i = 0; i < N; ++i) {
+        const int k = RPL * (N * wave + i) + lane / LPR;
+        const int piece = (lane % LPR) ^ t_cswz<DT>(k), col = piece * (16 / ES);
         off[i] = op.row0 + col < op.rows ? (uint32_t)k * ldb + 16u * piece : T_OOB;
         k8[i] = 0;
       }
@@ -166,54 +179,55 @@ struct Loader {
       if (k8[i] + k0 >= kn) o = T_OOB;
     } else {
       const int32_t left = kn - k0;
-      bytes = left <= 0 ? 0u : (uint32_t)(left < T::EK ? left : T::EK) * ldb;
+      bytes = left <= 0 ? 0u : (uint32_t)(left < EK ? left : EK) * ldb;
     }
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)at, (short)0, (int)bytes, T_RSRC);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (ODP_LDS void*)(half + 1024 * (T::DMA * wave + i)), 16, o, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (ODP_LDS void*)(half + 1024 * (N * wave + i)), 16, o, 0, 0, 0);
   }
 };
 
 // The operands a step starts with, read during the step before it.
-template <int DT>
+template <int DT, int S>
 struct Head {
-  u32x4_t b[Tile<DT>::BJ], a[2];
+  u32x4_t b[Tile<DT, S>::BJ], a[2];
 };
 
-template <int DT, bool AKC, bool BKC>
-__device__ __forceinline__ void t_head(const char* st, Head<DT>& h) {
-  using T = Tile<DT>;
+template <int DT, int S, bool AKC, bool BKC>
+__device__ __forceinline__ void t_head(const char* st, Head<DT, S>& h) {
+  using T = Tile<DT, S>;
   const int wave = threadIdx.x >> 6, wm = T::WM * (wave & 1), wn = T::WN * (wave >> 1);
 #pragma unroll
-  for (int j = 0; j < T::BJ; ++j) h.b[j] = t_frag<DT, BKC>(st + T::HALF, wn + 16 * j);
-  h.a[0] = t_frag<DT, AKC>(st, wm);
-  h.a[1] = t_frag<DT, AKC>(st, wm + 16);
+  for (int j = 0; j < T::BJ; ++j) h.b[j] = t_frag<DT, BKC, T::NT>(st + T::ABYTES, wn + 16 * j);
+  h.a[0] = t_frag<DT, AKC, T::OT>(st, wm);
+  h.a[1] = t_frag<DT, AKC, T::OT>(st, wm + 16);
 }
 
 // One step: its MFMAs from `cur` and the operands in h, the loads of a later
 // step into `nxt` between the first of them, the next step's first operands
 // from `ahead` beside the last.  The stages are restrict parameters so that
 // the reads do not wait for the loads into `nxt`.
-template <int DT, bool AKC, bool BKC, typename Issue>
+template <int DT, int S, bool AKC, bool BKC, typename Issue>
 __device__ __forceinline__ void t_step(char* __restrict__ nxt, const char* __restrict__ cur,
-                                       const char* __restrict__ ahead, Issue issue, Head<DT>& h, Head<DT>& n,
-                                       typename Tile<DT>::Acc& acc) {
-  using T = Tile<DT>;
+                                       const char* __restrict__ ahead, Issue issue, Head<DT, S>& h, Head<DT, S>& n,
+                                       typename Tile<DT, S>::Acc& acc) {
+  using T = Tile<DT, S>;
   const int wave = threadIdx.x >> 6, wm = T::WM * (wave & 1), wn = T::WN * (wave >> 1);
+  // Block rows beside which the next step's b is read: the last but one of as
+  // many as it takes, or all.
+  constexpr int ROWS = T::BJ < T::BI ? T::BJ : T::BI, R0 = T::BJ < T::BI ? T::BI - 1 - T::BJ : 0;
+  constexpr int PER = (T::LOADS + T::BI - 1) / T::BI;  // loads a block row, over the first of them
   u32x4_t a[3] = {h.a[0], h.a[1], h.a[1]};
 #pragma unroll
   for (int i = 0; i < T::BI; ++i) {
-    if (i + 2 < T::BI) a[(i + 2) % 3] = t_frag<DT, AKC>(cur, wm + 16 * (i + 2));
-    // 2 * DMA loads over the first block rows (one a row where there are enough).
-    constexpr int PER = (2 * T::DMA + T::BI - 1) / T::BI;
+    if (i + 2 < T::BI) a[(i + 2) % 3] = t_frag<DT, AKC, T::OT>(cur, wm + 16 * (i + 2));
 #pragma unroll
-    for (int l = PER * i; l < PER * (i + 1) && l < 2 * T::DMA; ++l) issue(nxt, l);
-    constexpr int B0 = T::BI - 1 - T::BJ < 0 ? 0 : T::BI - 1 - T::BJ;  // block row from which b is read ahead
-    if constexpr (B0 + T::BJ < T::BI) {
-      if (i >= B0 && i < B0 + T::BJ) n.b[i - B0] = t_frag<DT, BKC>(ahead + T::HALF, wn + 16 * (i - B0));
-    } else {
-      n.b[i] = t_frag<DT, BKC>(ahead + T::HALF, wn + 16 * i);
+    for (int l = PER * i; l < PER * (i + 1) && l < T::LOADS; ++l) issue(nxt, l);
+    if (i >= R0 && i < R0 + ROWS) {
+#pragma unroll
+      for (int j = T::BJ * (i - R0) / ROWS; j < T::BJ * (i - R0 + 1) / ROWS; ++j)
+        n.b[j] = t_frag<DT, BKC, T::NT>(ahead + T::ABYTES, wn + 16 * j);
     }
-    if (i >= T::BI - 2) n.a[i - (T::BI - 2)] = t_frag<DT, AKC>(ahead, wm + 16 * (i - (T::BI - 2)));
+    if (i >= T::BI - 2) n.a[i - (T::BI - 2)] = t_frag<DT, AKC, T::OT>(ahead, wm + 16 * (i - (T::BI - 2)));
 #pragma unroll
     for (int j = 0; j < T::BJ; ++j) acc[i][j] = t_mfma<DT>(h.b[j], a[i % 3], acc[i][j]);
     __builtin_amdgcn_sched_barrier(0);
@@ -224,17 +238,17 @@ __device__ __forceinline__ void t_step(char* __restrict__ nxt, const char* __res
 // run() does the rest.  A workgroup that walks several tiles begins the next
 // one before it stores the last, so that the loads' latency passes beside the
 // epilogue (which must leave the ring alone).
-template <int DT, bool AKC, bool BKC>
+template <int DT, int S, bool AKC, bool BKC>
 struct Product {
-  using T = Tile<DT>;
-  Loader<DT, AKC> la;
-  Loader<DT, BKC> lb;
+  using T = Tile<DT, S>;
+  Loader<DT, AKC, T::OT, T::ALOADS> la;
+  Loader<DT, BKC, T::NT, T::BLOADS> lb;
   int32_t kl, kn;  // first k of the next step to load, and the end
   int wave;
 
   __device__ __forceinline__ void issue(char* st, int l) const {
-    if (l < T::DMA) la.issue(st, wave, l, kl, kn);
-    else lb.issue(st + T::HALF, wave, l - T::DMA, kl, kn);
+    if (l < T::ALOADS) la.issue(st, wave, l, kl, kn);
+    else lb.issue(st + T::ABYTES, wave, l - T::ALOADS, kl, kn);
   }
   __device__ __forceinline__ void advance() {
     kl += T::EK;
@@ -250,9 +264,9 @@ struct Product {
     la.init(A, wave);
     lb.init(B, wave);
 #pragma unroll
-    for (int q = 0; q < T_RING - 1; ++q) {
+    for (int q = 0; q < T::RING - 1; ++q) {
 #pragma unroll
-      for (int l = 0; l < 2 * T::DMA; ++l) issue(t_stage<DT>(q), l);
+      for (int l = 0; l < T::LOADS; ++l) issue(t_stage<DT, S>(q), l);
       advance();
     }
   }
@@ -266,22 +280,22 @@ struct Product {
         acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         __asm__ volatile("" : "+v"(acc[i][j]));
       }
-    Head<DT> h[2];
+    Head<DT, S> h[2];
     // Everything so far, an epilogue's stores among it.
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
     __asm__ volatile("s_barrier" ::: "memory");
-    t_head<DT, AKC, BKC>(t_stage<DT>(0), h[0]);
+    t_head<DT, S, AKC, BKC>(t_stage<DT, S>(0), h[0]);
     int32_t k = 0;
     while (k < kn) {
 #pragma unroll
-      for (int u = 0; u < T_RING; ++u) {
+      for (int u = 0; u < T::RING; ++u) {
         if (k >= kn) break;
         // The next step's loads have landed (this wave's; the barrier says so
-        // for the others); those of the step after may fly.
-        __builtin_amdgcn_s_waitcnt(vmcnt_imm((T_RING - 3) * 2 * T::DMA));
+        // for the others); those of the steps after it may fly.
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm((T::RING - 3) * T::LOADS));
         __asm__ volatile("s_barrier" ::: "memory");
-        t_step<DT, AKC, BKC>(t_stage<DT>((u + T_RING - 1) % T_RING), t_stage<DT>(u % T_RING),
-                             t_stage<DT>((u + 1) % T_RING),
+        t_step<DT, S, AKC, BKC>(t_stage<DT, S>((u + T::RING - 1) % T::RING), t_stage<DT, S>(u % T::RING),
+                             t_stage<DT, S>((u + 1) % T::RING),
                              [&](char* st, int l) __attribute__((always_inline)) { issue(st, l); }, h[u & 1],
                              h[(u + 1) & 1], acc);
         advance();

@@ -117,7 +117,7 @@ __global__ __launch_bounds__(256) void k_xent_pack(const char* __restrict__ x, i
                                                    int64_t width, const int32_t* __restrict__ act,
                                                    const int32_t* __restrict__ count, int vec,
                                                    char* __restrict__ xc) {
-  constexpr int ES = Tile<DT>::ES, V = 16 / ES;
+  constexpr int ES = Tile<DT, 0>::ES, V = 16 / ES;
   const int64_t pieces = width / V;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t k = i / pieces, c = (i - k * pieces) * V;
@@ -151,15 +151,15 @@ struct Xent {
 // Forward: per (row, tile of the vocabulary) the maximum and the sum of
 // exponentials below it, and each row's target logit.
 // ---------------------------------------------------------------------------
-template <int DT, bool CAP, bool WHOLE>
-__device__ __forceinline__ void stats_tile(const Xent& p, const typename Tile<DT>::Acc& acc, int cnt, int64_t o0,
-                                           int64_t n0, const int32_t (&tgt)[Tile<DT>::BI], float* red,
+template <int DT, int S, bool CAP, bool WHOLE>
+__device__ __forceinline__ void stats_tile(const Xent& p, const typename Tile<DT, S>::Acc& acc, int cnt, int64_t o0,
+                                           int64_t n0, const int32_t (&tgt)[Tile<DT, S>::BI], float* red,
                                            float* __restrict__ ztgt) {
-  using T = Tile<DT>;
+  using T = Tile<DT, S>;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = T::WM * (wave & 1), wn = T::WN * (wave >> 1);
   // Columns of this lane are c0 + 16 j + e of the tile; `edge` columns of it exist.
-  const int c0 = wn + t_col(0), edge = (int)min((int64_t)T::ET, p.vocab - n0);
+  const int c0 = wn + t_col(0), edge = (int)min((int64_t)T::NT, p.vocab - n0);
   static_for<T::BI>([&](auto ii) __attribute__((always_inline)) {
     constexpr int i = decltype(ii)::value;
     // The row's target, counted from c0 (no column of the lane for none here).
@@ -194,7 +194,7 @@ __device__ __forceinline__ void stats_tile(const Xent& p, const typename Tile<DT
       m = mm;
     }
     if (lane < 16) {
-      float* r = red + 2 * ((wave >> 1) * T::ET + wm + t_row(i));
+      float* r = red + 2 * ((wave >> 1) * T::OT + wm + t_row(i));
       r[0] = m;
       r[1] = s;
     }
@@ -202,25 +202,25 @@ __device__ __forceinline__ void stats_tile(const Xent& p, const typename Tile<DT
   });
 }
 
-template <int DT, bool CAP>
-__global__ __launch_bounds__(Tile<DT>::THREADS, 2) void k_xent_stats(Xent p, float* __restrict__ pmax,
+template <int DT, int S, bool CAP>
+__global__ __launch_bounds__((Tile<DT, S>::THREADS), 2) void k_xent_stats(Xent p, float* __restrict__ pmax,
                                                                      float* __restrict__ psum,
                                                                      float* __restrict__ ztgt) {
-  using T = Tile<DT>;
-  __shared__ float red[T::WAVES / 2 * T::ET * 2];  // [waves across n][rows][maximum, sum]
+  using T = Tile<DT, S>;
+  __shared__ float red[T::WAVES / 2 * T::OT * 2];  // [waves across n][rows][maximum, sum]
   const int cnt = *(const ODP_CONST int32_t*)p.count;
-  Walk walk((cnt + T::ET - 1) / T::ET, (int)((p.vocab + T::ET - 1) / T::ET));
+  Walk walk((cnt + T::OT - 1) / T::OT, (int)((p.vocab + T::NT - 1) / T::NT));
   const int wm = T::WM * ((threadIdx.x >> 6) & 1);
-  Product<DT, true, true> prod;
+  Product<DT, S, true, true> prod;
   int ti, tj;
   auto begin = [&]() {
-    prod.begin(Operand{p.xc, p.width, (int64_t)ti * T::ET, cnt}, Operand{p.w, p.ldw, (int64_t)tj * T::ET, p.vocab},
+    prod.begin(Operand{p.xc, p.width, (int64_t)ti * T::OT, cnt}, Operand{p.w, p.ldw, (int64_t)tj * T::NT, p.vocab},
                (int32_t)p.width);
   };
   bool more = walk.tile(ti, tj);
   if (more) begin();
   while (more) {
-    const int64_t o0 = (int64_t)ti * T::ET, n0 = (int64_t)tj * T::ET;
+    const int64_t o0 = (int64_t)ti * T::OT, n0 = (int64_t)tj * T::NT;
     typename T::Acc acc;
     prod.run(acc);
     int32_t tgt[T::BI];
@@ -230,18 +230,18 @@ __global__ __launch_bounds__(Tile<DT>::THREADS, 2) void k_xent_stats(Xent p, flo
     walk.next();
     more = walk.tile(ti, tj);
     if (more) begin();
-    if (n0 + T::ET <= p.vocab) stats_tile<DT, CAP, true>(p, acc, cnt, o0, n0, tgt, red, ztgt);
-    else stats_tile<DT, CAP, false>(p, acc, cnt, o0, n0, tgt, red, ztgt);
+    if (n0 + T::NT <= p.vocab) stats_tile<DT, S, CAP, true>(p, acc, cnt, o0, n0, tgt, red, ztgt);
+    else stats_tile<DT, S, CAP, false>(p, acc, cnt, o0, n0, tgt, red, ztgt);
     __syncthreads();
-    for (int r = threadIdx.x; r < T::ET; r += T::THREADS) {
+    for (int r = threadIdx.x; r < T::OT; r += T::THREADS) {
       if (o0 + r >= cnt) break;
       float m = -INFINITY, s = 0.f;
 #pragma unroll
-      for (int w = 0; w < T::WAVES / 2; ++w) m = fmaxf(m, red[2 * (w * T::ET + r)]);
+      for (int w = 0; w < T::WAVES / 2; ++w) m = fmaxf(m, red[2 * (w * T::OT + r)]);
       const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int w = 0; w < T::WAVES / 2; ++w)
-        s += red[2 * (w * T::ET + r) + 1] * fast_exp(red[2 * (w * T::ET + r)] - ref);
+        s += red[2 * (w * T::OT + r) + 1] * fast_exp(red[2 * (w * T::OT + r)] - ref);
       pmax[(int64_t)column * p.n + o0 + r] = m;
       psum[(int64_t)column * p.n + o0 + r] = s;
     }
@@ -305,10 +305,10 @@ __device__ __forceinline__ uint16_t* t_staged() {
   __shared__ __attribute__((aligned(16))) uint16_t s[N];
   return s;
 }
-template <int DT, typename Val>
+template <int DT, int S, typename Val>
 __device__ __forceinline__ void t_store(void* out, int64_t ld, int64_t o0, int64_t rows, int64_t n0, int64_t cols,
                                         Val val) {
-  using T = Tile<DT>;
+  using T = Tile<DT, S>;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = T::WM * (wave & 1), wn = T::WN * (wave >> 1);
   if constexpr (DT == ODP_DTYPE_F32) {
@@ -348,22 +348,22 @@ __device__ __forceinline__ void t_store(void* out, int64_t ld, int64_t o0, int64
 // Backward: d of the vocabulary's columns [v0, v0 + vc), [count][ldd], with
 // zeros up to ldd (a multiple of the tile).
 // ---------------------------------------------------------------------------
-template <int DT>
+template <int DT, int S>
 struct DRows {  // of a lane's rows of a tile
-  float lse[Tile<DT>::BI], g[Tile<DT>::BI];  // log-sum-exp (in powers of 2), gradient
-  int32_t tgt[Tile<DT>::BI];                 // target less the piece's first column
+  float lse[Tile<DT, S>::BI], g[Tile<DT, S>::BI];  // log-sum-exp (in powers of 2), gradient
+  int32_t tgt[Tile<DT, S>::BI];                 // target less the piece's first column
 };
 constexpr int32_t NO_LOSS = INT32_MIN;  // a target may lie anywhere beside the piece
 
-template <int DT, bool CAP, bool WHOLE>
-__device__ __forceinline__ void dlogits_tile(const Xent& p, const typename Tile<DT>::Acc& acc, const DRows<DT>& rows,
+template <int DT, int S, bool CAP, bool WHOLE>
+__device__ __forceinline__ void dlogits_tile(const Xent& p, const typename Tile<DT, S>::Acc& acc, const DRows<DT, S>& rows,
                                              int cnt, int64_t o0, int64_t n0, int64_t vc, void* dl, int64_t ldd) {
-  using T = Tile<DT>;
+  using T = Tile<DT, S>;
   const int wn = T::WN * (threadIdx.x >> 7);
   // Columns of this lane are c0 + 16 j + e of the tile; `edge` columns of it exist.
-  const int c0 = wn + t_col(0), edge = (int)min((int64_t)T::ET, vc - n0);
+  const int c0 = wn + t_col(0), edge = (int)min((int64_t)T::NT, vc - n0);
   const float inv_cap = 0.5f * p.inv_cap2;
-  t_store<DT>(dl, ldd, o0, cnt, n0, ldd, [&](auto ii, auto jj) __attribute__((always_inline)) {
+  t_store<DT, S>(dl, ldd, o0, cnt, n0, ldd, [&](auto ii, auto jj) __attribute__((always_inline)) {
     constexpr int i = decltype(ii)::value, j = decltype(jj)::value;
     const int at = rows.tgt[i] - (int)n0 - c0;
     const bool live = rows.tgt[i] != NO_LOSS;
@@ -384,31 +384,31 @@ __device__ __forceinline__ void dlogits_tile(const Xent& p, const typename Tile<
   });
 }
 
-template <int DT, bool CAP>
-__global__ __launch_bounds__(Tile<DT>::THREADS, 2) void k_xent_dlogits(Xent p, int64_t v0, int64_t vc,
+template <int DT, int S, bool CAP>
+__global__ __launch_bounds__((Tile<DT, S>::THREADS), (DT == ODP_DTYPE_BF16 && S ? 1 : 2)) void k_xent_dlogits(Xent p, int64_t v0, int64_t vc,
                                                                        const float* __restrict__ lse,
                                                                        const float* __restrict__ g, int g_stride,
                                                                        const float* __restrict__ over, void* dl,
                                                                        int64_t ldd) {
-  using T = Tile<DT>;
+  using T = Tile<DT, S>;
   const int cnt = *(const ODP_CONST int32_t*)p.count;
-  Walk walk((cnt + T::ET - 1) / T::ET, (int)(ldd / T::ET));
+  Walk walk((cnt + T::OT - 1) / T::OT, (int)(ldd / T::NT));
   const int wm = T::WM * ((threadIdx.x >> 6) & 1);
   const void* w = (const char*)p.w + v0 * p.ldw * T::ES;
   const float part = over != nullptr ? *over : 1.f;
-  Product<DT, true, true> prod;
+  Product<DT, S, true, true> prod;
   int ti, tj;
   auto begin = [&]() {
-    prod.begin(Operand{p.xc, p.width, (int64_t)ti * T::ET, cnt}, Operand{w, p.ldw, (int64_t)tj * T::ET, vc},
+    prod.begin(Operand{p.xc, p.width, (int64_t)ti * T::OT, cnt}, Operand{w, p.ldw, (int64_t)tj * T::NT, vc},
                (int32_t)p.width);
   };
   bool more = walk.tile(ti, tj);
   if (more) begin();
   while (more) {
-    const int64_t o0 = (int64_t)ti * T::ET, n0 = (int64_t)tj * T::ET;
+    const int64_t o0 = (int64_t)ti * T::OT, n0 = (int64_t)tj * T::NT;
     typename T::Acc acc;
     prod.run(acc);
-    DRows<DT> rows;
+    DRows<DT, S> rows;
 #pragma unroll
     for (int i = 0; i < T::BI; ++i) {
       const int64_t o = o0 + wm + t_row(i);
@@ -421,17 +421,17 @@ __global__ __launch_bounds__(Tile<DT>::THREADS, 2) void k_xent_dlogits(Xent p, i
     walk.next();
     more = walk.tile(ti, tj);
     if (more) begin();
-    if (n0 + T::ET <= vc) dlogits_tile<DT, CAP, true>(p, acc, rows, cnt, o0, n0, vc, dl, ldd);
-    else dlogits_tile<DT, CAP, false>(p, acc, rows, cnt, o0, n0, vc, dl, ldd);
+    if (n0 + T::NT <= vc) dlogits_tile<DT, S, CAP, true>(p, acc, rows, cnt, o0, n0, vc, dl, ldd);
+    else dlogits_tile<DT, S, CAP, false>(p, acc, rows, cnt, o0, n0, vc, dl, ldd);
   }
 }
 
 // How many slices of the contraction each tile of dx is split into: the
-// fewest of 1 .. 8 with which the workgroups fill the 256 CUs' rounds best,
+// fewest of 1 .. 16 with which the workgroups fill the 256 CUs' rounds best,
 // as far as the slots (`cap` tiles) and slices of 16 steps go.
 __host__ __device__ inline int dx_split(int tiles, int cap, int64_t steps) {
   int best = 1, rounds = (tiles + 255) / 256;
-  for (int s = 2; s <= 8 && s * tiles <= cap && steps >= 16 * s; ++s) {
+  for (int s = 2; s <= 16 && s * tiles <= cap && steps >= 16 * s; ++s) {
     const int r = (s * tiles + 255) / 256;
     if (r * best < rounds * s) best = s, rounds = r;
   }
@@ -439,33 +439,33 @@ __host__ __device__ inline int dx_split(int tiles, int cap, int64_t steps) {
 }
 
 // Slot s of dx [slices][count][width] (float32) (+)= d[:, slice s] W[slice s].
-template <int DT>
-__global__ __launch_bounds__(Tile<DT>::THREADS, 2) void k_xent_dx(Xent p, int64_t v0, int64_t vc, int64_t piece,
-                                                                  const void* dl, int64_t ldd, int cap, int first,
-                                                                  float* __restrict__ slots) {
-  using T = Tile<DT>;
+template <int DT, int S>
+__global__ __launch_bounds__((Tile<DT, S>::THREADS), 2) void k_xent_dx(Xent p, int64_t v0, int64_t vc, int64_t piece,
+                                                                     const void* dl, int64_t ldd, int cap, int first,
+                                                                     float* __restrict__ slots) {
+  using T = Tile<DT, S>;
   const int cnt = *(const ODP_CONST int32_t*)p.count;
-  const int tm = (cnt + T::ET - 1) / T::ET, tn = (int)((p.width + T::ET - 1) / T::ET);
+  const int tm = (cnt + T::OT - 1) / T::OT, tn = (int)((p.width + T::NT - 1) / T::NT);
   if (tm == 0) return;
   const int split = dx_split(tm * tn, cap, piece / T::EK);
   int ti, tj;
   if (!Walk(tm, tn * split).tile(ti, tj)) return;  // a workgroup per tile
   const int s = tj / tn;
   tj -= s * tn;
-  const int64_t o0 = (int64_t)ti * T::ET, n0 = (int64_t)tj * T::ET;
+  const int64_t o0 = (int64_t)ti * T::OT, n0 = (int64_t)tj * T::NT;
   // Slices of whole steps, the same for every piece.
   const int64_t per = (piece / T::EK + split - 1) / split * T::EK, k0 = s * per;
   const int32_t kn = (int32_t)max((int64_t)0, min(per, vc - k0));
   if (kn == 0 && !first) return;
   typename T::Acc acc;
-  Product<DT, true, false> prod;
+  Product<DT, S, true, false> prod;
   prod.begin(Operand{(const char*)dl + k0 * T::ES, ldd, o0, cnt},
              Operand{(const char*)p.w + (v0 + k0) * p.ldw * T::ES, p.ldw, n0, p.width}, kn);
   prod.run(acc);
   const int wave = threadIdx.x >> 6;
   const int wm = T::WM * (wave & 1), wn = T::WN * (wave >> 1);
   float* out = slots + (int64_t)s * cnt * p.width;
-  static_for<T::BI * T::BJ>([&](auto q) {
+  static_for<T::BI * T::BJ>([&](auto q) __attribute__((always_inline)) {
     constexpr int i = decltype(q)::value / T::BJ, j = decltype(q)::value % T::BJ;
     const int64_t o = o0 + wm + t_row(i), n = n0 + wn + t_col(j);
     if (o < cnt && n < p.width) {
@@ -483,7 +483,7 @@ __global__ __launch_bounds__(Tile<DT>::THREADS, 2) void k_xent_dx(Xent p, int64_
 template <int DT>
 __global__ __launch_bounds__(256) void k_xent_dx_rows(const float* __restrict__ slots, int64_t width, int64_t cols,
                                                       int64_t n, const int32_t* __restrict__ count,
-                                                      const int32_t* __restrict__ where, int tn, int cap,
+                                                      const int32_t* __restrict__ where, int ot, int tn, int cap,
                                                       int64_t steps, void* __restrict__ dx) {
   const int64_t quads = width / 4;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -492,7 +492,7 @@ __global__ __launch_bounds__(256) void k_xent_dx_rows(const float* __restrict__ 
   const int cnt = *count, k = where[row];
   f32x4_t v = {0.f, 0.f, 0.f, 0.f};
   if (k >= 0) {
-    const int split = dx_split((cnt + Tile<DT>::ET - 1) / Tile<DT>::ET * tn, cap, steps);
+    const int split = dx_split((cnt + ot - 1) / ot * tn, cap, steps);
     const float* at = slots + (int64_t)k * width + c;
     v = *(const f32x4_t*)at;
     for (int s = 1; s < split; ++s) v = v + *(const f32x4_t*)(at + (int64_t)s * cnt * width);
@@ -511,26 +511,26 @@ __global__ __launch_bounds__(256) void k_xent_dx_rows(const float* __restrict__ 
 
 // dW rows [0, vc) of pitch lddw = d^T x.
 template <int DT>
-__global__ __launch_bounds__(Tile<DT>::THREADS, 2) void k_xent_dw(Xent p, int64_t vc, const void* dl, int64_t ldd,
+__global__ __launch_bounds__((Tile<DT, 0>::THREADS), 2) void k_xent_dw(Xent p, int64_t vc, const void* dl, int64_t ldd,
                                                                   void* dw, int64_t lddw) {
-  using T = Tile<DT>;
+  using T = Tile<DT, 0>;
   const int cnt = *(const ODP_CONST int32_t*)p.count;
-  Walk walk((int)((vc + T::ET - 1) / T::ET), (int)((p.width + T::ET - 1) / T::ET));
-  Product<DT, false, false> prod;
+  Walk walk((int)((vc + T::OT - 1) / T::OT), (int)((p.width + T::NT - 1) / T::NT));
+  Product<DT, 0, false, false> prod;
   int ti, tj;
   auto begin = [&]() {
-    prod.begin(Operand{dl, ldd, (int64_t)ti * T::ET, ldd}, Operand{p.xc, p.width, (int64_t)tj * T::ET, p.width}, cnt);
+    prod.begin(Operand{dl, ldd, (int64_t)ti * T::OT, ldd}, Operand{p.xc, p.width, (int64_t)tj * T::NT, p.width}, cnt);
   };
   bool more = walk.tile(ti, tj);
   if (more) begin();
   while (more) {
-    const int64_t o0 = (int64_t)ti * T::ET, n0 = (int64_t)tj * T::ET;
+    const int64_t o0 = (int64_t)ti * T::OT, n0 = (int64_t)tj * T::NT;
     typename T::Acc acc;
     prod.run(acc);
     walk.next();
     more = walk.tile(ti, tj);
     if (more) begin();
-    t_store<DT>(dw, lddw, o0, vc, n0, p.width, [&](auto ii, auto jj) __attribute__((always_inline)) {
+    t_store<DT, 0>(dw, lddw, o0, vc, n0, p.width, [&](auto ii, auto jj) __attribute__((always_inline)) {
       return acc[decltype(ii)::value][decltype(jj)::value];
     });
   }
@@ -551,12 +551,24 @@ int check_xent(const char* what, int dtype, int64_t n, int64_t width, int64_t ld
   return ODP_OK;
 }
 
+// Columns a piece of d is padded to, and the edges of the tiles (few: those of few rows).
 int tile_edge(int dtype) { return dtype == ODP_DTYPE_F32 ? 128 : 256; }
+int tile_rows(int dtype, bool few) { return few ? 64 : tile_edge(dtype); }
+int tile_cols(int dtype, bool few) { return few ? 128 : tile_edge(dtype); }
+
+int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Whether a product of n rows takes the tiles of few rows.  Loss and dx, us,
+// with the small tiles and the large ones: bfloat16, 32000 x 2048, 47 tokens
+// 94 and 157, 64 95 and 156, 128 119 and 161, 192 153 and 164, 256 185 and
+// 167; 128256 x 4096, 64 tokens 623 and 639, 65 1022 and 729; float32, 50257
+// x 768, 64 tokens 242 and 420, 256 598 and 643, 384 791 and 738.
+bool few_rows(int dtype, int64_t n) { return n <= (dtype == ODP_DTYPE_F32 ? 256 : 64); }
 
 // Workgroups that walk a tm x tn grid of tiles: as many as the CUs hold at a
-// time (one of 16-bit tiles a CU, two of float32), or one a tile (`all`).
-int grid_of(const char* what, int dtype, int64_t tm, int64_t tn, bool all, unsigned& blocks) {
-  const int64_t b = (tm * tn + 7) / 8 * 8, held = dtype == ODP_DTYPE_F32 ? 512 : 256;
+// time (one of the large bfloat16 tiles, two of the others), or one a tile (`all`).
+int grid_of(const char* what, int dtype, bool few, int64_t tm, int64_t tn, bool all, unsigned& blocks) {
+  const int64_t b = (tm * tn + 7) / 8 * 8, held = dtype == ODP_DTYPE_F32 || few ? 512 : 256;
   if (b >= (int64_t)1 << 31) {
     odp_set_error("%s: %lld tiles", what, (long long)b);
     return ODP_ERR_UNSUPPORTED;
@@ -564,8 +576,6 @@ int grid_of(const char* what, int dtype, int64_t tm, int64_t tn, bool all, unsig
   blocks = (unsigned)(all || b < held ? b : held);
   return ODP_OK;
 }
-
-int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 Xent xent_of(const void* xc, const void* w, int64_t ldw, int64_t vocab, int64_t width, int64_t n,
              const int32_t* count, const int32_t* act, const int32_t* tgt, float cap) {
@@ -576,25 +586,30 @@ bool on16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace
 
-#define ODP_XENT_LAUNCH(K, GRID, ...)                                                                          \
-  do {                                                                                                         \
-    if (dtype == ODP_DTYPE_F32)                                                                                \
-      hipLaunchKernelGGL((K<ODP_DTYPE_F32>), dim3(GRID), dim3(Tile<ODP_DTYPE_F32>::THREADS), 0, s, __VA_ARGS__); \
-    else                                                                                                       \
-      hipLaunchKernelGGL((K<ODP_DTYPE_BF16>), dim3(GRID), dim3(Tile<ODP_DTYPE_BF16>::THREADS), 0, s, __VA_ARGS__); \
+#define ODP_XENT_GO(KERNEL, THREADS, GRID, ...) \
+  hipLaunchKernelGGL(KERNEL, dim3(GRID), dim3(THREADS), 0, s, __VA_ARGS__)
+// K<dtype, few rows>
+#define ODP_XENT_LAUNCH(K, GRID, ...)                                                              \
+  do {                                                                                             \
+    constexpr int F = ODP_DTYPE_F32, B = ODP_DTYPE_BF16;                                           \
+    if (dtype == F && few) ODP_XENT_GO((K<F, 1>), (Tile<F, 1>::THREADS), GRID, __VA_ARGS__);       \
+    else if (dtype == F) ODP_XENT_GO((K<F, 0>), (Tile<F, 0>::THREADS), GRID, __VA_ARGS__);         \
+    else if (few) ODP_XENT_GO((K<B, 1>), (Tile<B, 1>::THREADS), GRID, __VA_ARGS__);                \
+    else ODP_XENT_GO((K<B, 0>), (Tile<B, 0>::THREADS), GRID, __VA_ARGS__);                         \
   } while (0)
-
-#define ODP_XENT_LAUNCH_CAP(K, GRID, ...)                                                                             \
-  do {                                                                                                                \
-    constexpr int F = ODP_DTYPE_F32, B = ODP_DTYPE_BF16;                                                              \
-    if (dtype == F && softcap != 0.f)                                                                                 \
-      hipLaunchKernelGGL((K<F, true>), dim3(GRID), dim3(Tile<F>::THREADS), 0, s, __VA_ARGS__);                        \
-    else if (dtype == F)                                                                                              \
-      hipLaunchKernelGGL((K<F, false>), dim3(GRID), dim3(Tile<F>::THREADS), 0, s, __VA_ARGS__);                       \
-    else if (softcap != 0.f)                                                                                          \
-      hipLaunchKernelGGL((K<B, true>), dim3(GRID), dim3(Tile<B>::THREADS), 0, s, __VA_ARGS__);                        \
-    else                                                                                                              \
-      hipLaunchKernelGGL((K<B, false>), dim3(GRID), dim3(Tile<B>::THREADS), 0, s, __VA_ARGS__);                       \
+// K<dtype, few rows, softcap>
+#define ODP_XENT_CAP(K, D, S, GRID, ...)                                                           \
+  do {                                                                                             \
+    if (softcap != 0.f) ODP_XENT_GO((K<D, S, true>), (Tile<D, S>::THREADS), GRID, __VA_ARGS__);    \
+    else ODP_XENT_GO((K<D, S, false>), (Tile<D, S>::THREADS), GRID, __VA_ARGS__);                  \
+  } while (0)
+#define ODP_XENT_LAUNCH_CAP(K, GRID, ...)                                                          \
+  do {                                                                                             \
+    constexpr int F = ODP_DTYPE_F32, B = ODP_DTYPE_BF16;                                           \
+    if (dtype == F && few) ODP_XENT_CAP(K, F, 1, GRID, __VA_ARGS__);                               \
+    else if (dtype == F) ODP_XENT_CAP(K, F, 0, GRID, __VA_ARGS__);                                 \
+    else if (few) ODP_XENT_CAP(K, B, 1, GRID, __VA_ARGS__);                                        \
+    else ODP_XENT_CAP(K, B, 0, GRID, __VA_ARGS__);                                                 \
   } while (0)
 
 extern "C" int odp_xent_rows(odp_stream_t stream, int dtype, const void* x, int64_t ldx, int64_t n, int64_t cols,
@@ -639,7 +654,7 @@ extern "C" int odp_xent_rows(odp_stream_t stream, int dtype, const void* x, int6
 
 extern "C" int64_t odp_xent_stats_scratch(int dtype, int64_t n, int64_t vocab) {
   if (n <= 0 || vocab <= 0) return 0;
-  return 4 * n * (2 * up(vocab, tile_edge(dtype)) + 1);
+  return 4 * n * (2 * up(vocab, tile_cols(dtype, few_rows(dtype, n))) + 1);
 }
 
 extern "C" int odp_xent_losses(odp_stream_t stream, int dtype, const void* xc, int64_t n, int64_t width,
@@ -653,9 +668,10 @@ extern "C" int odp_xent_losses(odp_stream_t stream, int dtype, const void* xc, i
     return ODP_ERR_INVALID_ARGUMENT;
   }
   const hipStream_t s = odp_hip_stream(stream);
-  const int64_t tn = up(vocab, tile_edge(dtype));
+  const bool few = few_rows(dtype, n);
+  const int64_t tn = up(vocab, tile_cols(dtype, few));
   unsigned blocks;
-  if (int rc = grid_of("odp_xent_losses", dtype, up(n, tile_edge(dtype)), tn, false, blocks)) return rc;
+  if (int rc = grid_of("odp_xent_losses", dtype, few, up(n, tile_rows(dtype, few)), tn, false, blocks)) return rc;
   const Xent p = xent_of(xc, w, ldw, vocab, width, n, count, act, tgt, softcap);
   float* pmax = (float*)scratch;
   float* psum = pmax + n * tn;
@@ -696,23 +712,30 @@ extern "C" int odp_xent_dlogits(odp_stream_t stream, int dtype, const void* xc, 
     return ODP_ERR_INVALID_ARGUMENT;
   }
   const hipStream_t s = odp_hip_stream(stream);
+  const bool few = few_rows(dtype, n);
   unsigned blocks;
-  if (int rc = grid_of("odp_xent_dlogits", dtype, up(n, tile_edge(dtype)), ldd / tile_edge(dtype), false, blocks)) return rc;
+  if (int rc = grid_of("odp_xent_dlogits", dtype, few, up(n, tile_rows(dtype, few)), ldd / tile_cols(dtype, few), false,
+                       blocks))
+    return rc;
   const Xent p = xent_of(xc, w, ldw, vocab, width, n, count, act, tgt, softcap);
   ODP_XENT_LAUNCH_CAP(k_xent_dlogits, blocks, p, v0, vc, lse, g, g_stride, over, dl, ldd);
   return odp_check_launch("odp_xent_dlogits");
 }
 
-// Tiles of the slots: those of n rows, or a few times as many to split.
+// Tiles of n rows of dx, and those that the slots hold: as many, or a few times that to split.
+static int64_t dx_tiles(int dtype, int64_t n, int64_t width, bool few) {
+  return up(n, tile_rows(dtype, few)) * up(width, tile_cols(dtype, few));
+}
 static int dx_cap(int dtype, int64_t n, int64_t width) {
-  const int64_t tiles = up(n, tile_edge(dtype)) * up(width, tile_edge(dtype));
-  const int64_t most = tiles * 8 < 512 ? tiles * 8 : 512;
+  const int64_t tiles = dx_tiles(dtype, n, width, few_rows(dtype, n));
+  const int64_t most = tiles * 16 < 512 ? tiles * 16 : 512;
   return (int)(tiles > most ? tiles : most);
 }
 
 extern "C" int64_t odp_xent_dx_scratch(int dtype, int64_t n, int64_t width) {
   if (n <= 0 || width <= 0) return 0;
-  return 4 * (int64_t)dx_cap(dtype, n, width) * tile_edge(dtype) * tile_edge(dtype);
+  const bool few = few_rows(dtype, n);
+  return 4 * (int64_t)dx_cap(dtype, n, width) * tile_rows(dtype, few) * tile_cols(dtype, few);
 }
 
 extern "C" int odp_xent_dx(odp_stream_t stream, int dtype, int64_t n, int64_t width, const int32_t* count,
@@ -733,9 +756,9 @@ extern "C" int odp_xent_dx(odp_stream_t stream, int dtype, int64_t n, int64_t wi
   }
   const hipStream_t s = odp_hip_stream(stream);
   const int cap = dx_cap(dtype, n, width);
-  const int64_t tiles = up(n, tile_edge(dtype)) * up(width, tile_edge(dtype));
+  const bool few = few_rows(dtype, n);
   unsigned blocks;
-  if (int rc = grid_of("odp_xent_dx", dtype, tiles > cap ? tiles : cap, 1, true, blocks)) return rc;
+  if (int rc = grid_of("odp_xent_dx", dtype, few, cap, 1, true, blocks)) return rc;
   const Xent p = xent_of(nullptr, w, ldw, vocab, width, n, count, nullptr, nullptr, 0.f);
   const int64_t whole = odp_xent_pitch(dtype, piece);
   ODP_XENT_LAUNCH(k_xent_dx, blocks, p, v0, vc, whole, dl, ldd, cap, v0 == 0 ? 1 : 0, (float*)scratch);
@@ -763,14 +786,15 @@ extern "C" int odp_xent_dx_rows(odp_stream_t stream, int dtype, int64_t n, int64
     return ODP_ERR_UNSUPPORTED;
   }
   const hipStream_t s = odp_hip_stream(stream);
-  const int tn = (int)up(width, tile_edge(dtype)), cap = dx_cap(dtype, n, width);
+  const bool few = few_rows(dtype, n);
+  const int ot = tile_rows(dtype, few), tn = (int)up(width, tile_cols(dtype, few)), cap = dx_cap(dtype, n, width);
   const int64_t steps = odp_xent_pitch(dtype, piece) / (dtype == ODP_DTYPE_F32 ? 16 : 32);
   if (dtype == ODP_DTYPE_F32)
     hipLaunchKernelGGL((k_xent_dx_rows<ODP_DTYPE_F32>), dim3((unsigned)blocks), dim3(256), 0, s,
-                       (const float*)scratch, width, cols, n, count, where, tn, cap, steps, dx);
+                       (const float*)scratch, width, cols, n, count, where, ot, tn, cap, steps, dx);
   else
     hipLaunchKernelGGL((k_xent_dx_rows<ODP_DTYPE_BF16>), dim3((unsigned)blocks), dim3(256), 0, s,
-                       (const float*)scratch, width, cols, n, count, where, tn, cap, steps, dx);
+                       (const float*)scratch, width, cols, n, count, where, ot, tn, cap, steps, dx);
   return odp_check_launch("odp_xent_dx_rows");
 }
 
@@ -785,8 +809,11 @@ extern "C" int odp_xent_dw(odp_stream_t stream, int dtype, const void* xc, int64
   }
   const hipStream_t s = odp_hip_stream(stream);
   unsigned blocks;
-  if (int rc = grid_of("odp_xent_dw", dtype, up(vc, tile_edge(dtype)), up(width, tile_edge(dtype)), false, blocks)) return rc;
+  if (int rc = grid_of("odp_xent_dw", dtype, false, up(vc, tile_edge(dtype)), up(width, tile_edge(dtype)), false, blocks)) return rc;
   const Xent p = xent_of(xc, nullptr, width, vc, width, n, count, nullptr, nullptr, 0.f);
-  ODP_XENT_LAUNCH(k_xent_dw, blocks, p, vc, dl, ldd, dw, lddw);
+  if (dtype == ODP_DTYPE_F32)
+    ODP_XENT_GO((k_xent_dw<ODP_DTYPE_F32>), (Tile<ODP_DTYPE_F32, 0>::THREADS), blocks, p, vc, dl, ldd, dw, lddw);
+  else
+    ODP_XENT_GO((k_xent_dw<ODP_DTYPE_BF16>), (Tile<ODP_DTYPE_BF16, 0>::THREADS), blocks, p, vc, dl, ldd, dw, lddw);
   return odp_check_launch("odp_xent_dw");
 }
