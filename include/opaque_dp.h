@@ -665,24 +665,26 @@ int odp_xent_losses(odp_stream_t stream, int dtype, const void* xc, int64_t n, i
 /* d [count][ldd] of the columns [v0, v0 + vc): g_t (exp(z - lse_t) - [target])
  * times the softcap's slope, in the inputs' type, zero past vc; ldd =
  * odp_xent_pitch(dtype, vc).  lse is per row of [n], g too (g_stride 1) or one
- * for all (0), divided by *over where that is not null.                      */
+ * for all (0), divided by *over where that is not null.  rest [n]: what
+ * rounding takes off each packed row's target entry (bfloat16).              */
 /* *out = the sum of the losses, over *over where that is not null. */
 int odp_xent_reduce(odp_stream_t stream, const float* losses, int64_t n, const float* over, float* out);
 int64_t odp_xent_pitch(int dtype, int64_t columns);
 int odp_xent_dlogits(odp_stream_t stream, int dtype, const void* xc, int64_t n, int64_t width, const int32_t* act,
                      const int32_t* tgt, const int32_t* count, const void* w, int64_t ldw, int64_t vocab,
                      float softcap, int64_t v0, int64_t vc, const float* lse, const float* g, int g_stride,
-                     const float* over, void* dl, int64_t ldd);
+                     const float* over, void* dl, int64_t ldd, float* rest);
 
 /* Adds d W of a piece of the vocabulary to the float32 sums of dx in scratch
  * (v0 == 0 starts them; pieces of `piece` columns, in order); then
- * odp_xent_dx_rows writes dx [n][cols].                                     */
+ * odp_xent_dx_rows writes dx [n][cols], with the targets' `rest`.           */
 int64_t odp_xent_dx_scratch(int dtype, int64_t n, int64_t width);
 int odp_xent_dx(odp_stream_t stream, int dtype, int64_t n, int64_t width, const int32_t* count, const void* w,
                 int64_t ldw, int64_t vocab, int64_t v0, int64_t vc, int64_t piece, const void* dl, int64_t ldd,
                 void* scratch);
 int odp_xent_dx_rows(odp_stream_t stream, int dtype, int64_t n, int64_t cols, int64_t width, const int32_t* count,
-                     const int32_t* where, int64_t piece, const void* scratch, void* dx);
+                     const int32_t* where, const int32_t* tgt, const void* w, int64_t ldw, int64_t piece,
+                     const void* scratch, const float* rest, void* dx);
 
 /* dW rows of a piece, [vc] of pitch lddw, = d^T x.                          */
 int odp_xent_dw(odp_stream_t stream, int dtype, const void* xc, int64_t n, int64_t width, const int32_t* count,

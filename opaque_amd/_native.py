@@ -154,14 +154,16 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "odp_xent_dlogits": (
         _c_int,
         [_ptr, _c_int, _ptr, _c_i64, _c_i64, _ptr, _ptr, _ptr, _ptr, _c_i64, _c_i64, _c_f32, _c_i64, _c_i64, _ptr,
-         _ptr, _c_int, _ptr, _ptr, _c_i64],
+         _ptr, _c_int, _ptr, _ptr, _c_i64, _ptr],
     ),
     "odp_xent_reduce": (_c_int, [_ptr, _ptr, _c_i64, _ptr, _ptr]),
     "odp_xent_dx_scratch": (_c_i64, [_c_int, _c_i64, _c_i64]),
     "odp_xent_dx": (
         _c_int,
         [_ptr, _c_int, _c_i64, _c_i64, _ptr, _ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _ptr, _c_i64, _ptr]),
-    "odp_xent_dx_rows": (_c_int, [_ptr, _c_int, _c_i64, _c_i64, _c_i64, _ptr, _ptr, _c_i64, _ptr, _ptr]),
+    "odp_xent_dx_rows": (
+        _c_int,
+        [_ptr, _c_int, _c_i64, _c_i64, _c_i64, _ptr, _ptr, _ptr, _ptr, _c_i64, _c_i64, _ptr, _ptr, _ptr]),
     "odp_xent_dw": (
         _c_int, [_ptr, _c_int, _ptr, _c_i64, _c_i64, _ptr, _c_i64, _ptr, _c_i64, _ptr, _c_i64]),
     "odp_linear_moments_blocks": (_c_i64, [_c_i64, _c_i64, _c_i32]),

@@ -279,12 +279,14 @@ struct Xent : torch::autograd::Function<Xent> {
         sums = bytes_on(p.xc, abi.xent_dx_scratch(p.dt, p.n, p.width));
       }
       if (need_w) dw = at::empty({p.vocab, p.width}, p.xc.options());
+      const at::Tensor rest = at::empty({std::max<int64_t>(p.n, 1)}, lse.options());
       const odp_stream_t s = stream_of(p.xc);
       for (int64_t v0 = 0; v0 < p.vocab; v0 += piece) {
         const int64_t vc = std::min(piece, p.vocab - v0), ldd = abi.xent_pitch(p.dt, vc);
         check(abi.xent_dlogits(s, p.dt, p.xc.data_ptr(), p.n, p.width, p.act(), p.tgt(), p.count(), p.w.data_ptr(),
                                p.w.stride(0), p.vocab, softcap, v0, vc, (const float*)lse.data_ptr(),
-                               (const float*)g.data_ptr(), stride, over, d.data_ptr(), ldd),
+                               (const float*)g.data_ptr(), stride, over, d.data_ptr(), ldd,
+                               (float*)rest.data_ptr()),
               "odp_xent_dlogits");
         if (need_x)
           check(abi.xent_dx(s, p.dt, p.n, p.width, p.count(), p.w.data_ptr(), p.w.stride(0), p.vocab, v0, vc, piece,
@@ -296,8 +298,8 @@ struct Xent : torch::autograd::Function<Xent> {
                 "odp_xent_dw");
       }
       if (need_x)
-        check(abi.xent_dx_rows(s, p.dt, p.n, p.cols, p.width, p.count(), p.where(), piece, sums.data_ptr(),
-                               dx.data_ptr()),
+        check(abi.xent_dx_rows(s, p.dt, p.n, p.cols, p.width, p.count(), p.where(), p.tgt(), p.w.data_ptr(),
+                               p.w.stride(0), piece, sums.data_ptr(), (const float*)rest.data_ptr(), dx.data_ptr()),
               "odp_xent_dx_rows");
       if (need_w && p.cols != p.width) dw = dw.narrow(1, 0, p.cols).contiguous();
     }

@@ -14,7 +14,10 @@
 // (k_xent_dx) and by x (k_xent_dw).  Sums, statistics and losses are
 // float32; d is rounded to the inputs' type because the matrix cores take it
 // so (a relative 2^-8 of an entry at most in bfloat16, of the order of the
-// rounding of the gradients themselves).
+// rounding of the gradients themselves).  What rounding takes off the target's
+// entry, often the row's only large one, is added to dx in float32
+// (k_xent_dx_rows): alone it would leave a row of dx as far off as that entry.
+// A row of dW adds many tokens' entries, whose roundings average out.
 #include "odp_internal.h"
 
 namespace {
@@ -46,6 +49,8 @@ struct Walk {
   __device__ __forceinline__ void next() { at += step; }
 };
 
+// Of a difference: x log2(e) formed before the subtraction would be off by the
+// last place of the larger operand.
 __device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
 
 // c tanh(u / c) as c (1 - 2 / (1 + exp(2 u / c))): within 2^-22 c.
@@ -179,12 +184,12 @@ __device__ __forceinline__ void stats_tile(const Xent& p, const typename Tile<DT
         m = fmaxf(m, z[j][e]);
       }
     if (here) ztgt[o0 + wm + t_row(i)] = zt;
-    const float ms = m == -INFINITY ? 0.f : m * LOG2E;
+    const float ms = m == -INFINITY ? 0.f : m;
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < T::BJ; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(__builtin_fmaf(z[j][e], LOG2E, -ms));
+      for (int e = 0; e < 4; ++e) s += fast_exp(z[j][e] - ms);
     // The row's other columns of this wave: lanes 16, 32 and 48 further on.
 #pragma unroll
     for (int off = 16; off <= 32; off <<= 1) {
@@ -274,9 +279,10 @@ __global__ __launch_bounds__(256) void k_xent_losses(const float* __restrict__ p
   const float ref = m == -INFINITY ? 0.f : m;
   s = 0.f;
   for (int t = 0; t < 16; ++t) s += rs[t][r] * fast_exp(rm[t][r] - ref);
-  const float l = ref + logf(s);
-  lse[act[row]] = l;
-  if (tgt[row] >= 0) losses[act[row]] = l - ztgt[row];
+  const float l = logf(s);
+  lse[act[row]] = ref + l;
+  // Not lse less the target's logit: a small loss would keep little of lse's bits.
+  if (tgt[row] >= 0) losses[act[row]] = (ref - ztgt[row]) + l;
 }
 
 // The sum of the losses (in fp64, in one order), over *over where it is given.
@@ -350,16 +356,17 @@ __device__ __forceinline__ void t_store(void* out, int64_t ld, int64_t o0, int64
 // ---------------------------------------------------------------------------
 template <int DT, int S>
 struct DRows {  // of a lane's rows of a tile
-  float lse[Tile<DT, S>::BI], g[Tile<DT, S>::BI];  // log-sum-exp (in powers of 2), gradient
+  float lse[Tile<DT, S>::BI], g[Tile<DT, S>::BI];  // log-sum-exp, gradient
   int32_t tgt[Tile<DT, S>::BI];                 // target less the piece's first column
 };
 constexpr int32_t NO_LOSS = INT32_MIN;  // a target may lie anywhere beside the piece
 
 template <int DT, int S, bool CAP, bool WHOLE>
 __device__ __forceinline__ void dlogits_tile(const Xent& p, const typename Tile<DT, S>::Acc& acc, const DRows<DT, S>& rows,
-                                             int cnt, int64_t o0, int64_t n0, int64_t vc, void* dl, int64_t ldd) {
+                                             int cnt, int64_t o0, int64_t n0, int64_t vc, void* dl, int64_t ldd,
+                                             float* __restrict__ rest) {
   using T = Tile<DT, S>;
-  const int wn = T::WN * (threadIdx.x >> 7);
+  const int wm = T::WM * ((threadIdx.x >> 6) & 1), wn = T::WN * (threadIdx.x >> 7);
   // Columns of this lane are c0 + 16 j + e of the tile; `edge` columns of it exist.
   const int c0 = wn + t_col(0), edge = (int)min((int64_t)T::NT, vc - n0);
   const float inv_cap = 0.5f * p.inv_cap2;
@@ -368,18 +375,24 @@ __device__ __forceinline__ void dlogits_tile(const Xent& p, const typename Tile<
     const int at = rows.tgt[i] - (int)n0 - c0;
     const bool live = rows.tgt[i] != NO_LOSS;
     f32x4_t d;
+    float over = 0.f;
+    bool here = false;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       float z = acc[i][j][e];
       if (CAP) z = softcapped(z, p.cap, p.inv_cap2);
-      float q = __builtin_amdgcn_exp2f(__builtin_fmaf(z, LOG2E, -rows.lse[i]));
-      q = (at == 16 * j + e ? q - 1.f : q) * rows.g[i];
+      float q = fast_exp(z - rows.lse[i]);
+      const bool hit = at == 16 * j + e;
+      here |= hit;
+      q = (hit ? q - 1.f : q) * rows.g[i];
       if (CAP) {
         const float y = z * inv_cap;
         q *= 1.f - y * y;
       }
       d[e] = live && (WHOLE || c0 + 16 * j + e < edge) ? q : 0.f;
+      if (DT == ODP_DTYPE_BF16) over = hit ? q - odp_round_bf16(q) : over;
     }
+    if (DT == ODP_DTYPE_BF16 && here && live) rest[o0 + wm + t_row(i)] = over;
     return d;
   });
 }
@@ -389,7 +402,7 @@ __global__ __launch_bounds__((Tile<DT, S>::THREADS), (DT == ODP_DTYPE_BF16 && S 
                                                                        const float* __restrict__ lse,
                                                                        const float* __restrict__ g, int g_stride,
                                                                        const float* __restrict__ over, void* dl,
-                                                                       int64_t ldd) {
+                                                                       int64_t ldd, float* __restrict__ rest) {
   using T = Tile<DT, S>;
   const int cnt = *(const ODP_CONST int32_t*)p.count;
   Walk walk((cnt + T::OT - 1) / T::OT, (int)(ldd / T::NT));
@@ -414,15 +427,15 @@ __global__ __launch_bounds__((Tile<DT, S>::THREADS), (DT == ODP_DTYPE_BF16 && S 
       const int64_t o = o0 + wm + t_row(i);
       const int32_t t = o < cnt ? p.tgt[o] : -1;
       const int64_t row = o < cnt ? p.act[o] : 0;
-      rows.lse[i] = t >= 0 ? lse[row] * LOG2E : 0.f;
+      rows.lse[i] = t >= 0 ? lse[row] : 0.f;
       rows.g[i] = t >= 0 ? g[row * g_stride] / part : 0.f;
       rows.tgt[i] = t >= 0 ? t - (int32_t)v0 : NO_LOSS;
     }
     walk.next();
     more = walk.tile(ti, tj);
     if (more) begin();
-    if (n0 + T::NT <= vc) dlogits_tile<DT, S, CAP, true>(p, acc, rows, cnt, o0, n0, vc, dl, ldd);
-    else dlogits_tile<DT, S, CAP, false>(p, acc, rows, cnt, o0, n0, vc, dl, ldd);
+    if (n0 + T::NT <= vc) dlogits_tile<DT, S, CAP, true>(p, acc, rows, cnt, o0, n0, vc, dl, ldd, rest);
+    else dlogits_tile<DT, S, CAP, false>(p, acc, rows, cnt, o0, n0, vc, dl, ldd, rest);
   }
 }
 
@@ -484,7 +497,9 @@ template <int DT>
 __global__ __launch_bounds__(256) void k_xent_dx_rows(const float* __restrict__ slots, int64_t width, int64_t cols,
                                                       int64_t n, const int32_t* __restrict__ count,
                                                       const int32_t* __restrict__ where, int ot, int tn, int cap,
-                                                      int64_t steps, void* __restrict__ dx) {
+                                                      int64_t steps, const float* __restrict__ rest,
+                                                      const int32_t* __restrict__ tgt, const char* __restrict__ w,
+                                                      int64_t ldw, void* __restrict__ dx) {
   const int64_t quads = width / 4;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t row = i / quads, c = (i - row * quads) * 4;
@@ -496,6 +511,12 @@ __global__ __launch_bounds__(256) void k_xent_dx_rows(const float* __restrict__ 
     const float* at = slots + (int64_t)k * width + c;
     v = *(const f32x4_t*)at;
     for (int s = 1; s < split; ++s) v = v + *(const f32x4_t*)(at + (int64_t)s * cnt * width);
+    if (DT == ODP_DTYPE_BF16 && tgt[k] >= 0) {
+      const u32x2_t h = *(const u32x2_t*)(w + 2 * (tgt[k] * ldw + c));
+      const float r = rest[k];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(r, odp_bf2f((uint16_t)(h[e / 2] >> (16 * (e & 1)))), v[e]);
+    }
   } else if (k == -2) {
     v[0] = v[1] = v[2] = v[3] = __uint_as_float(0x7fc00000u);
   }
@@ -698,7 +719,8 @@ extern "C" int64_t odp_xent_pitch(int dtype, int64_t columns) {
 extern "C" int odp_xent_dlogits(odp_stream_t stream, int dtype, const void* xc, int64_t n, int64_t width,
                                 const int32_t* act, const int32_t* tgt, const int32_t* count, const void* w,
                                 int64_t ldw, int64_t vocab, float softcap, int64_t v0, int64_t vc, const float* lse,
-                                const float* g, int g_stride, const float* over, void* dl, int64_t ldd) {
+                                const float* g, int g_stride, const float* over, void* dl, int64_t ldd,
+                                float* rest) {
   if (int rc = check_xent("odp_xent_dlogits", dtype, n, width, ldw, vocab)) return rc;
   if (v0 < 0 || vc <= 0 || v0 + vc > vocab || ldd != odp_xent_pitch(dtype, vc)) {
     odp_set_error("odp_xent_dlogits: columns [%lld, %lld) of %lld at pitch %lld", (long long)v0,
@@ -707,7 +729,7 @@ extern "C" int odp_xent_dlogits(odp_stream_t stream, int dtype, const void* xc, 
   }
   if (n == 0) return ODP_OK;
   if (xc == nullptr || act == nullptr || tgt == nullptr || count == nullptr || w == nullptr || lse == nullptr ||
-      g == nullptr || dl == nullptr || !on16(xc) || !on16(w) || !on16(dl)) {
+      g == nullptr || dl == nullptr || rest == nullptr || !on16(xc) || !on16(w) || !on16(dl)) {
     odp_set_error("odp_xent_dlogits: null pointer, or rows off the 16-byte grid");
     return ODP_ERR_INVALID_ARGUMENT;
   }
@@ -718,7 +740,7 @@ extern "C" int odp_xent_dlogits(odp_stream_t stream, int dtype, const void* xc, 
                        blocks))
     return rc;
   const Xent p = xent_of(xc, w, ldw, vocab, width, n, count, act, tgt, softcap);
-  ODP_XENT_LAUNCH_CAP(k_xent_dlogits, blocks, p, v0, vc, lse, g, g_stride, over, dl, ldd);
+  ODP_XENT_LAUNCH_CAP(k_xent_dlogits, blocks, p, v0, vc, lse, g, g_stride, over, dl, ldd, rest);
   return odp_check_launch("odp_xent_dlogits");
 }
 
@@ -766,16 +788,17 @@ extern "C" int odp_xent_dx(odp_stream_t stream, int dtype, int64_t n, int64_t wi
 }
 
 extern "C" int odp_xent_dx_rows(odp_stream_t stream, int dtype, int64_t n, int64_t cols, int64_t width,
-                                const int32_t* count, const int32_t* where, int64_t piece, const void* scratch,
-                                void* dx) {
-  if (int rc = check_xent("odp_xent_dx_rows", dtype, n, width, width, 1)) return rc;
+                                const int32_t* count, const int32_t* where, const int32_t* tgt, const void* w,
+                                int64_t ldw, int64_t piece, const void* scratch, const float* rest, void* dx) {
+  if (int rc = check_xent("odp_xent_dx_rows", dtype, n, width, ldw, 1)) return rc;
   if (cols <= 0 || cols > width || piece <= 0) {
     odp_set_error("odp_xent_dx_rows: %lld columns of %lld, pieces of %lld", (long long)cols, (long long)width,
                   (long long)piece);
     return ODP_ERR_INVALID_ARGUMENT;
   }
   if (n == 0) return ODP_OK;
-  if (count == nullptr || where == nullptr || scratch == nullptr || dx == nullptr || !on16(scratch) ||
+  if (count == nullptr || where == nullptr || tgt == nullptr || w == nullptr || scratch == nullptr ||
+      rest == nullptr || dx == nullptr || !on16(scratch) || !on16(w) ||
       (cols == width && !on16(dx))) {
     odp_set_error("odp_xent_dx_rows: null pointer, or rows off the 16-byte grid");
     return ODP_ERR_INVALID_ARGUMENT;
@@ -791,10 +814,12 @@ extern "C" int odp_xent_dx_rows(odp_stream_t stream, int dtype, int64_t n, int64
   const int64_t steps = odp_xent_pitch(dtype, piece) / (dtype == ODP_DTYPE_F32 ? 16 : 32);
   if (dtype == ODP_DTYPE_F32)
     hipLaunchKernelGGL((k_xent_dx_rows<ODP_DTYPE_F32>), dim3((unsigned)blocks), dim3(256), 0, s,
-                       (const float*)scratch, width, cols, n, count, where, ot, tn, cap, steps, dx);
+                       (const float*)scratch, width, cols, n, count, where, ot, tn, cap, steps, rest, tgt,
+                       (const char*)w, ldw, dx);
   else
     hipLaunchKernelGGL((k_xent_dx_rows<ODP_DTYPE_BF16>), dim3((unsigned)blocks), dim3(256), 0, s,
-                       (const float*)scratch, width, cols, n, count, where, ot, tn, cap, steps, dx);
+                       (const float*)scratch, width, cols, n, count, where, ot, tn, cap, steps, rest, tgt,
+                       (const char*)w, ldw, dx);
   return odp_check_launch("odp_xent_dx_rows");
 }
 

@@ -353,12 +353,14 @@ class _Packed:
             sums = torch.empty(_xent_words(dt, self.n, self.width, self.vocab)[1], dtype=torch.float32, device=dev)
         if need_w:
             dw = torch.empty((self.vocab, self.width), dtype=dtype, device=dev)
+        rest = torch.empty(max(self.n, 1), dtype=torch.float32, device=dev)
         w, ldw, xc = self.w.data_ptr(), self.w.stride(0), self.xc.data_ptr()
         for v0 in range(0, self.vocab, piece):
             vc = min(piece, self.vocab - v0)
             ldd = _xent_pitch(dt, vc)
             _call("odp_xent_dlogits", s, dt, xc, self.n, self.width, self.act, self.tgt, self.count, w, ldw,
-                  self.vocab, softcap, v0, vc, lse.data_ptr(), g.data_ptr(), 1, None, d.data_ptr(), ldd)
+                  self.vocab, softcap, v0, vc, lse.data_ptr(), g.data_ptr(), 1, None, d.data_ptr(), ldd,
+                  rest.data_ptr())
             if dx is not None:
                 _call("odp_xent_dx", s, dt, self.n, self.width, self.count, w, ldw, self.vocab, v0, vc, piece,
                       d.data_ptr(), ldd, sums.data_ptr())
@@ -366,8 +368,8 @@ class _Packed:
                 _call("odp_xent_dw", s, dt, xc, self.n, self.width, self.count, vc, d.data_ptr(), ldd,
                       dw.data_ptr() + v0 * self.width * dw.element_size(), self.width)
         if dx is not None:
-            _call("odp_xent_dx_rows", s, dt, self.n, self.cols, self.width, self.count, self.where, piece,
-                  sums.data_ptr(), dx.data_ptr())
+            _call("odp_xent_dx_rows", s, dt, self.n, self.cols, self.width, self.count, self.where, self.tgt, w,
+                  ldw, piece, sums.data_ptr(), rest.data_ptr(), dx.data_ptr())
         if dw is not None and self.cols != self.width:
             dw = dw[:, : self.cols].contiguous()
         return dx, dw, d[: self.n, : self.vocab] if keep_d else None

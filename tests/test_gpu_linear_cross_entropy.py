@@ -362,3 +362,48 @@ def test_head_changed_before_the_backward():
     wd.add_(1.0)
     with pytest.raises(RuntimeError):
         loss.backward()
+
+
+@pytest.mark.parametrize("n", [1, 5, 300])
+@pytest.mark.parametrize("softcap", [None, 20.0])
+def test_the_targets_entry_keeps_its_bits_in_dx(n, softcap):
+    """dx in bfloat16 takes the target's d in float32: only the other entries' rounding is in its bound."""
+    x, w, y, gl = inputs(n, 128, 900, torch.bfloat16, seed=40 + n, ignored=0.0)
+    _, dx, _ = run(x, w, y, gl, softcap)
+    (_, want, _), _ = reference(x, w, y, gl, softcap, torch.bfloat16)
+    # As in reference(), with d's own rounding left out at the targets.
+    xd, wd, g = x.double().to(DEV), w.double().to(DEV), gl.double().to(DEV).unsqueeze(1)
+    u = xd @ wd.t()
+    Z = 2 * 128 * U32 * (xd.abs() @ wd.abs().t()) + (softcap * 2.0**-21 if softcap else 0.0)
+    z = softcap * torch.tanh(u / softcap) if softcap else u
+    p = torch.softmax(z, 1)
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    r = Z + Z.max(1, keepdim=True).values + (8 + (z - lse).abs()) * 2.0**-22
+    q = p.clone()
+    at = (torch.arange(n, device=DEV), y.to(DEV))
+    q[at] -= 1.0
+    slope = 1 - (z / softcap) ** 2 if softcap else torch.ones_like(z)
+    d = g * q * slope
+    rounding = 2.0**-8 * d.abs()
+    rounding[at] = 2 * U32 * d[at].abs()
+    dd = g.abs() * ((p * r + 4 * U32) * slope.abs() + (q.abs() * 2 * (Z / softcap + 2.0**-22) if softcap else 0.0))
+    dd = dd * 1.01 + rounding + 4 * U32 * d.abs()
+    bound = dd @ wd.abs() + 2 * 908 * U32 * (d.abs() @ wd.abs()) + 2.0**-8 * want.abs() * 1.02 + LEAST
+    assert within(dx, want, bound)
+
+
+def test_small_losses_keep_their_bits():
+    """A loss far below its log-sum-exp: off by the logits' error times 1 - p, not by the log-sum-exp's last place."""
+    width, vocab = 64, 500
+    g = torch.Generator().manual_seed(3)
+    w = torch.randn(vocab, width, generator=g) / 8
+    y = torch.arange(0, vocab, 50)
+    x = w[y] * 60.0  # p(target) near 1
+    loss = linear_cross_entropy(x.to(DEV), w.to(DEV), y.to(DEV), reduction="none").double()
+    xd, wd = x.double().to(DEV), w.double().to(DEV)
+    z = xd @ wd.t()
+    want = torch.logsumexp(z, 1) - z.gather(1, y.to(DEV).unsqueeze(1)).squeeze(1)
+    Z = (2 * width * U32 * (xd.abs() @ wd.abs().t())).max(1).values
+    share = 1 - torch.exp(-want)
+    bound = share * (2 * Z + 2.0**-18) + 4 * U32  # 4 U32: the sum's rounding at 1, and the logarithm's
+    assert float(want.min()) < 0.1 and ((loss - want).abs() <= bound).all()
