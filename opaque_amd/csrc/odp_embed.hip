@@ -730,6 +730,7 @@ __global__ __launch_bounds__(64 * EM_WAVES) void k_embed_group(EmbedSum a) {
 template <int DT, bool AL, int MODE>
 __global__ __launch_bounds__(64 * EM_WAVES) void k_embed_join(EmbedSum a) {
   constexpr int V = em_vec<DT>();
+  const int lane = threadIdx.x & 63;
   const int64_t item = (int64_t)blockIdx.x * EM_WAVES + uniform_int(threadIdx.x >> 6);
   const int64_t win = item / a.ncb;
   const int cb = (int)(item - win * a.ncb);
@@ -744,13 +745,20 @@ __global__ __launch_bounds__(64 * EM_WAVES) void k_embed_join(EmbedSum a) {
   }
   auto same = [&](int64_t p) { return a.keys[p] == key && (MODE != EM_NORM || a.seg_of[p] == seg); };
   if (p0 > 0 && same(p0) && same(p0 - 1)) return;  // it began before
-  // The run's last position: positions after it compare greater.
-  int64_t lo = last + 1, hi = a.n - 1;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi + 1) >> 1;
-    if (same(mid)) lo = mid; else hi = mid - 1;
+  // The run's last window: most often the next one, else that of its last
+  // position (positions after it compare greater).
+  int64_t end = win + 1;
+  const int64_t next = min(last + a.win, a.n - 1);
+  if (same(next)) {
+    int64_t lo = next, hi = a.n - 1;
+    while (lo < hi) {  // 64 places at a time
+      const int64_t step = (hi - lo + 63) / 64, at = lo + (lane + 1) * step;
+      const uint64_t in = __builtin_amdgcn_ballot_w64(at <= hi && same(min(at, hi)));
+      lo += __popcll(in) * step;
+      hi = min(hi, lo + step - 1);
+    }
+    end = lo / a.win;
   }
-  const int64_t end = lo / a.win;  // its last window
   constexpr bool second = MODE == EM_CLIP2;
   float v[V], q[V];
   em_clear(v);
@@ -764,9 +772,8 @@ __global__ __launch_bounds__(64 * EM_WAVES) void k_embed_join(EmbedSum a) {
     return;
   }
   // The first row of the run: the first of this window's positions in it.
-  int64_t h = p0;
-  while (!same(h)) ++h;
-  em_norm<DT>(a, a.rows[h], seg, cb, v);
+  const uint64_t in = __builtin_amdgcn_ballot_w64(lane < a.win && same(p0 + min(lane, a.win - 1)));
+  em_norm<DT>(a, a.rows[p0 + __builtin_ctzll(in)], seg, cb, v);
   em_put(em_ws<DT>(a.whole, win, a, cb), v);
 }
 

@@ -372,7 +372,7 @@ __device__ __forceinline__ void dlogits_tile(const Xent& p, const typename Tile<
   const float inv_cap = 0.5f * p.inv_cap2;
   t_store<DT, S>(dl, ldd, o0, cnt, n0, ldd, [&](auto ii, auto jj) __attribute__((always_inline)) {
     constexpr int i = decltype(ii)::value, j = decltype(jj)::value;
-    const int at = rows.tgt[i] - (int)n0 - c0;
+    const int at = (int)((uint32_t)rows.tgt[i] - (uint32_t)n0 - (uint32_t)c0);
     const bool live = rows.tgt[i] != NO_LOSS;
     f32x4_t d;
     float over = 0.f;

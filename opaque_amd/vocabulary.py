@@ -334,10 +334,11 @@ class _Packed:
               losses.data_ptr(), lse.data_ptr())
 
     def piece(self, whole: bool = False) -> int:
-        """Columns of the vocabulary a piece of d holds."""
+        """Columns of the vocabulary a piece of d holds: as many pieces as PIECE_BYTES makes, of one size."""
         edge = _xent_pitch(self.dt, 1)
-        fit = PIECE_BYTES // (max(self.n, 1) * self.xc.element_size()) // edge * edge
-        return self.vocab if whole else min(self.vocab, max(fit, edge))
+        fit = max(PIECE_BYTES // (max(self.n, 1) * self.xc.element_size()) // edge * edge, edge)
+        pieces = -(-self.vocab // fit)
+        return self.vocab if whole else min(self.vocab, -(-(-(-self.vocab // pieces)) // edge) * edge)
 
     def gradients(self, softcap: float, lse: torch.Tensor, g: torch.Tensor, x_shape: torch.Size | None,
                   need_w: bool, keep_d: bool = False):

@@ -384,3 +384,86 @@ def test_sort_sizes(n):
     want = (c * S).sum(0) / clip.normalize_by
     bound = 8 * U32 * (c * S).abs().sum(0) / clip.normalize_by + LEAST[torch.float32]
     assert ((res.leaves[0].double().cpu() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_dropped_rows_may_hold_anything(dtype):
+    """Rows of the padding token, of tokens outside the table and outside the segments are not read into any result."""
+    g = gen(61)
+    batch, seq, width, vocab = 3, 40, 72, 30
+    y = torch.randint(0, vocab, (batch * seq,), generator=g)
+    go = torch.randn(batch * seq, width, generator=g).to(dtype)
+    lengths = [40, 25, 0]
+    y[[3, 44]] = 5
+    y[[7, 50]] = torch.tensor([vocab, -4])
+    drop = (y == 5) | (y < 0) | (y >= vocab)
+    inside = torch.cat([torch.arange(seq) < ln for ln in lengths])
+    bad = go.clone()
+    bad[drop | ~inside] = math.nan
+    clip = clip_of((vocab, width), dtype)
+
+    def result(t):
+        plan = GhostPlan(segments=Segments.padded(batch, seq, lengths), leaves=[LeafOut((vocab, width), dtype)],
+                         clip=clip, embedding_sites=[EmbeddingSite(tokens=y.to(DEV), g=t.to(DEV), w_leaf=0, padding=5)])
+        res = plan.run()
+        return res.leaves[0], res.norms
+
+    for a, b in zip(result(bad), result(go)):
+        assert torch.equal(a, b)
+    w = torch.zeros(vocab, width, dtype=dtype, device=DEV, requires_grad=True)
+    bad = go.clone()
+    bad[drop] = math.inf
+    both = [torch.autograd.grad(embedding(y.to(DEV), w, padding_idx=5), w, t.to(DEV))[0] for t in (bad, go)]
+    assert torch.equal(*both)
+
+
+@pytest.mark.parametrize("microbatch", [None, 3])
+def test_bfloat16_table_under_clipped_grad(microbatch):
+    """A bfloat16 table, whole and in microbatches (whose sums are kept in float32), within the framework's tolerance."""
+    g = gen(71)
+    n, T, vocab, width = 7, 29, 50, 40
+    params = {"table": torch.randn(vocab, width, generator=g).bfloat16()}
+    y = tokens_of("text", n * T, vocab, g).view(n, T)
+    c = torch.randn(n, T, width, generator=g).bfloat16()
+
+    def loss(embed):
+        return lambda p, yi, ci: (embed(yi, p["table"]).float() * ci.float()).sum()
+
+    grad_fn, st = clipped_grad(loss(seam), clipping_norm=30.0, normalize_by=float(n), batch_argnums=(1, 2),
+                               return_aux=True, microbatch_size=microbatch)
+    (got, aux), st = grad_fn({"table": params["table"].to(DEV)}, y.to(DEV), c.to(DEV), state=st)
+    assert got.pytree["table"].dtype == torch.bfloat16
+    ref, raux = dp_ref.clipped_grad(loss(plain), params, (y, c), clipping_norm=30.0, normalize_by=float(n))
+    assert float(((aux.grad_norms.double().cpu() - raux["norms"].double()) / raux["norms"].double()).abs().max()) < 2e-2
+    a, b = got.pytree["table"].double().cpu(), ref["table"].double()
+    assert float((a - b).norm() / b.norm()) < 2e-2
+
+
+def test_in_a_graph():
+    """Lookup and table gradient replayed from a captured graph, with eager work and new contents between the replays."""
+    vocab, width, n = 700, 48, 300
+    w = torch.randn(vocab, width, device=DEV, requires_grad=True)
+    y = torch.randint(0, vocab, (n,), device=DEV)
+    go = torch.randn(n, width, device=DEV)
+
+    def step():
+        out = embedding(y, w, scale=1.5)
+        return out, torch.autograd.grad(out, w, go)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for k in range(4):
+        y.copy_(torch.randint(0, vocab, (n,), device=DEV))
+        go.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in held]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b.detach())

@@ -407,3 +407,34 @@ def test_small_losses_keep_their_bits():
     share = 1 - torch.exp(-want)
     bound = share * (2 * Z + 2.0**-18) + 4 * U32  # 4 U32: the sum's rounding at 1, and the logarithm's
     assert float(want.min()) < 0.1 and ((loss - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_in_a_graph(dtype):
+    """Loss and gradients replayed from a captured graph, with eager work and new contents between the replays."""
+    x, w, y, _ = inputs(90, 64, 700, dtype, seed=77)
+    x, w, y = x.to(DEV).requires_grad_(), w.to(DEV).requires_grad_(), y.to(DEV)
+
+    def step():
+        loss = linear_cross_entropy(x, w, y)
+        return loss, *torch.autograd.grad(loss, [x, w])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for k in range(4):
+        y.copy_(torch.randint(0, 700, (90,), device=DEV))
+        y[: 20 * k] = -100  # another number of tokens bears a loss
+        with torch.no_grad():
+            x.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.detach().clone() for t in held]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b.detach())
