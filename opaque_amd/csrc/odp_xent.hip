@@ -117,17 +117,71 @@ __global__ __launch_bounds__(1024) void k_xent_pick(const void* __restrict__ tar
 }
 
 // Packed rows xc [count][width] from x's rows `act`, columns past `cols` zero.
-template <int DT>
+// FEW: of up to XENT_FEW tokens, which every workgroup picks from by itself
+// (the first one writes k_xent_pick's results), one launch instead of two.
+struct Pick {
+  const void* target;
+  int wide, keep;
+  int64_t n, vocab, ignore;
+  int32_t *act, *tgt, *where, *count;
+  float *losses, *lse;
+};
+constexpr int XENT_FEW = 1024;
+template <int DT, bool FEW>
 __global__ __launch_bounds__(256) void k_xent_pack(const char* __restrict__ x, int64_t ldx, int64_t cols,
-                                                   int64_t width, const int32_t* __restrict__ act,
-                                                   const int32_t* __restrict__ count, int vec,
-                                                   char* __restrict__ xc) {
+                                                   int64_t width, Pick p, int vec, char* __restrict__ xc) {
   constexpr int ES = Tile<DT, 0>::ES, V = 16 / ES;
+  __shared__ int32_t picked[FEW ? XENT_FEW : 1], sums[4], other[4];
+  int total = 0;
+  if (FEW) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int counted = 0;
+    for (int i0 = 0; i0 < (int)p.n; i0 += 256) {
+      const int i = i0 + threadIdx.x;
+      const bool in = i < (int)p.n;
+      const int64_t t = !in ? -1 : p.wide ? ((const int64_t*)p.target)[i] : (int64_t)((const int32_t*)p.target)[i];
+      const bool live = in && t != p.ignore && t >= 0 && t < p.vocab, taken = p.keep ? in : live;
+      const uint64_t m = __builtin_amdgcn_ballot_w64(taken);
+      const uint64_t some = __builtin_amdgcn_ballot_w64(in && t != p.ignore);
+      __syncthreads();
+      if (lane == 0) {
+        sums[wave] = __popcll(m);
+        other[wave] = __popcll(some);
+      }
+      __syncthreads();
+      int k = total + __popcll(m & ((1ull << lane) - 1));
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        if (w < wave) k += sums[w];
+        total += sums[w];
+        counted += other[w];
+      }
+      if (taken) picked[k] = i;
+      if (blockIdx.x == 0 && in) {
+        if (!live) {
+          if (p.losses != nullptr) p.losses[i] = t == p.ignore ? 0.f : __uint_as_float(0x7fc00000u);
+          if (p.lse != nullptr) p.lse[i] = 0.f;
+        }
+        if (taken) {
+          p.act[k] = i;
+          p.tgt[k] = live ? (int32_t)t : -1;
+        }
+        p.where[i] = live ? k : t == p.ignore ? -1 : -2;
+      }
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      p.count[0] = total;
+      ((float*)p.count)[1] = (float)counted;
+    }
+    __syncthreads();
+  } else {
+    total = *p.count;
+  }
   const int64_t pieces = width / V;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t k = i / pieces, c = (i - k * pieces) * V;
-  if (k >= *count) return;
-  const char* src = x + ((int64_t)act[k] * ldx + c) * ES;
+  if (k >= total) return;
+  const char* src = x + ((int64_t)(FEW ? picked[k] : p.act[k]) * ldx + c) * ES;
   u32x4_t v = {0, 0, 0, 0};
   if (vec) {
     v = *(const u32x4_t*)src;
@@ -253,32 +307,43 @@ __global__ __launch_bounds__((Tile<DT, S>::THREADS), 2) void k_xent_stats(Xent p
   }
 }
 
-// Joins the tiles' statistics: 16 rows a workgroup, 16 lanes each.
+// Joins the tiles' statistics: R rows a workgroup, 256 / R threads each.
+template <int R>
 __global__ __launch_bounds__(256) void k_xent_losses(const float* __restrict__ pmax, const float* __restrict__ psum,
                                                      const float* __restrict__ ztgt, int tiles, int64_t n,
                                                      const int32_t* __restrict__ count,
                                                      const int32_t* __restrict__ act, const int32_t* __restrict__ tgt,
                                                      float* __restrict__ losses, float* __restrict__ lse) {
-  __shared__ float rm[16][17], rs[16][17];
-  const int r = threadIdx.x & 15, q = threadIdx.x >> 4;
-  const int64_t row = (int64_t)blockIdx.x * 16 + r;
+  constexpr int Q = 256 / R;
+  __shared__ float rm[Q][R + 1], rs[Q][R + 1];
+  const int r = threadIdx.x % R, q = threadIdx.x / R;
+  const int64_t row = (int64_t)blockIdx.x * R + r;
   const bool on = row < *count;
   float m = -INFINITY, s = 0.f;
-  if (on)
-    for (int t = q; t < tiles; t += 16) {
+  if (on) {
+#pragma unroll 4
+    for (int t = q; t < tiles; t += Q) {
       const float m2 = pmax[(int64_t)t * n + row], s2 = psum[(int64_t)t * n + row];
       const float mm = fmaxf(m, m2), ref = mm == -INFINITY ? 0.f : mm;
       s = s * fast_exp(m - ref) + s2 * fast_exp(m2 - ref);
       m = mm;
     }
+  }
   rm[q][r] = m;
   rs[q][r] = s;
   __syncthreads();
+  // Halves joined in one order.
+  for (int h = Q / 2; h > 0; h /= 2) {
+    if (q < h) {
+      const float m2 = rm[q + h][r], s2 = rs[q + h][r];
+      const float mm = fmaxf(m, m2), ref = mm == -INFINITY ? 0.f : mm;
+      rs[q][r] = s = s * fast_exp(m - ref) + s2 * fast_exp(m2 - ref);
+      rm[q][r] = m = mm;
+    }
+    __syncthreads();
+  }
   if (q != 0 || !on) return;
-  for (int t = 1; t < 16; ++t) m = fmaxf(m, rm[t][r]);
   const float ref = m == -INFINITY ? 0.f : m;
-  s = 0.f;
-  for (int t = 0; t < 16; ++t) s += rs[t][r] * fast_exp(rm[t][r] - ref);
   const float l = logf(s);
   lse[act[row]] = ref + l;
   // Not lse less the target's logit: a small loss would keep little of lse's bits.
@@ -653,22 +718,28 @@ extern "C" int odp_xent_rows(odp_stream_t stream, int dtype, const void* x, int6
     return ODP_ERR_INVALID_ARGUMENT;
   }
   const hipStream_t s = odp_hip_stream(stream);
-  hipLaunchKernelGGL(k_xent_pick, dim3(1), dim3(1024), 0, s, target, target_bytes == 8 ? 1 : 0, n, vocab, ignore, keep,
-                     act, tgt, where, count, losses, lse);
   const int64_t es = dtype == ODP_DTYPE_F32 ? 4 : 2;
   const int64_t blocks = up(n * (width * es / 16), 256);
   if (blocks >= (int64_t)1 << 24) {
     odp_set_error("odp_xent_rows: the launch needs %lld workgroups", (long long)blocks);
     return ODP_ERR_UNSUPPORTED;
   }
+  const bool few = n > 0 && n <= XENT_FEW;
+  const Pick p{target, target_bytes == 8 ? 1 : 0, keep, n, vocab, ignore, act, tgt, where, count, losses, lse};
+  if (!few)
+    hipLaunchKernelGGL(k_xent_pick, dim3(1), dim3(1024), 0, s, target, p.wide, n, vocab, ignore, keep, act, tgt, where,
+                       count, losses, lse);
   if (blocks > 0) {
     const int vec = cols == width && on16(x) && ldx * es % 16 == 0;
-    if (dtype == ODP_DTYPE_F32)
-      hipLaunchKernelGGL((k_xent_pack<ODP_DTYPE_F32>), dim3((unsigned)blocks), dim3(256), 0, s, (const char*)x, ldx,
-                         cols, width, act, count, vec, (char*)xc);
-    else
-      hipLaunchKernelGGL((k_xent_pack<ODP_DTYPE_BF16>), dim3((unsigned)blocks), dim3(256), 0, s, (const char*)x, ldx,
-                         cols, width, act, count, vec, (char*)xc);
+#define ODP_PACK(D, F) \
+  hipLaunchKernelGGL((k_xent_pack<D, F>), dim3((unsigned)blocks), dim3(256), 0, s, (const char*)x, ldx, cols, width, p, \
+                     vec, (char*)xc)
+    if (dtype == ODP_DTYPE_F32) {
+      if (few) ODP_PACK(ODP_DTYPE_F32, true); else ODP_PACK(ODP_DTYPE_F32, false);
+    } else {
+      if (few) ODP_PACK(ODP_DTYPE_BF16, true); else ODP_PACK(ODP_DTYPE_BF16, false);
+    }
+#undef ODP_PACK
   }
   return odp_check_launch("odp_xent_rows");
 }
@@ -698,8 +769,12 @@ extern "C" int odp_xent_losses(odp_stream_t stream, int dtype, const void* xc, i
   float* psum = pmax + n * tn;
   float* ztgt = psum + n * tn;
   ODP_XENT_LAUNCH_CAP(k_xent_stats, blocks, p, pmax, psum, ztgt);
-  hipLaunchKernelGGL(k_xent_losses, dim3((unsigned)up(n, 16)), dim3(256), 0, s, pmax, psum, ztgt, (int)tn, n, count,
-                     act, tgt, losses, lse);
+  if (few)
+    hipLaunchKernelGGL(k_xent_losses<1>, dim3((unsigned)n), dim3(256), 0, s, pmax, psum, ztgt, (int)tn, n, count, act,
+                       tgt, losses, lse);
+  else
+    hipLaunchKernelGGL(k_xent_losses<16>, dim3((unsigned)up(n, 16)), dim3(256), 0, s, pmax, psum, ztgt, (int)tn, n,
+                       count, act, tgt, losses, lse);
   return odp_check_launch("odp_xent_losses");
 }
 
