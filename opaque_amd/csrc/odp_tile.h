@@ -3,8 +3,9 @@
 //
 // Included inside an anonymous namespace, after odp_internal.h.  A workgroup
 // owns an OT x NT tile of C: rows o from A, columns n from B.  256 x 256 in
-// bfloat16 and 128 x 128 in float32; with S, for few rows, 64 x 128 and a ring
-// of more, smaller stages, since such a product waits for B's memory.  An operand is K-contiguous (KC: element
+// bfloat16 and 128 x 128 in float32; with S == 1, for few rows, 64 x 128 and a ring
+// of more, smaller stages, since such a product waits for B's memory; with S
+// == 2 (bfloat16) 128 x 256.  An operand is K-contiguous (KC: element
 // (row, k) at row * ld + k, as the rows of activations or of a weight) or
 // K-major (element (row, k) at k * ld + row: the contraction runs over the
 // rows of memory).  A step covers 64 bytes of k; both orders then stage the
@@ -28,8 +29,8 @@ template <int DT, int S>
 struct Tile {
   static constexpr bool F32 = DT == ODP_DTYPE_F32;
   static constexpr int ES = F32 ? 4 : 2;          // bytes per element
-  static constexpr int OT = S ? 64 : 512 / ES;    // rows (o) of the tile
-  static constexpr int NT = S ? 128 : 512 / ES;   // columns (n)
+  static constexpr int OT = S == 1 ? 64 : S == 2 ? 128 : 512 / ES;  // rows (o) of the tile
+  static constexpr int NT = S == 1 ? 128 : 512 / ES;                // columns (n)
   static constexpr int EK = 64 / ES;              // k per step
   static constexpr int WAVES = NT / 64 * 2;       // 2 x (WAVES / 2) over the tile
   static constexpr int THREADS = 64 * WAVES;
@@ -38,7 +39,7 @@ struct Tile {
   static constexpr int ABYTES = OT * 64, BBYTES = NT * 64, STAGE = ABYTES + BBYTES;  // of a step
   static constexpr int ALOADS = ABYTES / 1024 / WAVES, BLOADS = BBYTES / 1024 / WAVES;  // 1 KB loads per wave
   static constexpr int LOADS = ALOADS + BLOADS;
-  static constexpr int RING = S ? 6 : 4;
+  static constexpr int RING = S == 1 ? 6 : 4;
   static_assert(ALOADS * WAVES * 1024 == ABYTES && BLOADS * WAVES * 1024 == BBYTES, "whole loads");
   typedef f32x4_t Acc[BI][BJ];
 };
@@ -53,7 +54,7 @@ __device__ __forceinline__ char* t_array() {
 template <int DT, int S>
 __device__ __forceinline__ char* t_stage(int k) {
   constexpr int B = Tile<DT, S>::STAGE;
-  if constexpr (S == 0)
+  if constexpr (S != 1)
     return k == 0 ? t_array<B, 0>() : k == 1 ? t_array<B, 1>() : k == 2 ? t_array<B, 2>() : t_array<B, 3>();
   else
     return k == 0   ? t_array<B, 0>()

@@ -463,7 +463,7 @@ __device__ __forceinline__ void dlogits_tile(const Xent& p, const typename Tile<
 }
 
 template <int DT, int S, bool CAP>
-__global__ __launch_bounds__((Tile<DT, S>::THREADS), (DT == ODP_DTYPE_BF16 && S ? 1 : 2)) void k_xent_dlogits(Xent p, int64_t v0, int64_t vc,
+__global__ __launch_bounds__((Tile<DT, S>::THREADS), (DT == ODP_DTYPE_BF16 && S == 1 ? 1 : 2)) void k_xent_dlogits(Xent p, int64_t v0, int64_t vc,
                                                                        const float* __restrict__ lse,
                                                                        const float* __restrict__ g, int g_stride,
                                                                        const float* __restrict__ over, void* dl,
@@ -637,10 +637,10 @@ int check_xent(const char* what, int dtype, int64_t n, int64_t width, int64_t ld
   return ODP_OK;
 }
 
-// Columns a piece of d is padded to, and the edges of the tiles (few: those of few rows).
+// Columns a piece of d is padded to, and the edges of the tiles of a kind (Tile's S).
 int tile_edge(int dtype) { return dtype == ODP_DTYPE_F32 ? 128 : 256; }
-int tile_rows(int dtype, bool few) { return few ? 64 : tile_edge(dtype); }
-int tile_cols(int dtype, bool few) { return few ? 128 : tile_edge(dtype); }
+int tile_rows(int dtype, int kind) { return kind == 1 ? 64 : kind == 2 ? 128 : tile_edge(dtype); }
+int tile_cols(int dtype, int kind) { return kind == 1 ? 128 : tile_edge(dtype); }
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -651,10 +651,23 @@ int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // x 768, 64 tokens 242 and 420, 256 598 and 643, 384 791 and 738.
 bool few_rows(int dtype, int64_t n) { return n <= (dtype == ODP_DTYPE_F32 ? 256 : 64); }
 
+// The tiles (Tile's S) of a product of n rows and `cols` columns.  A tile of
+// 128 rows takes about 0.7 of the time of one of 256: bfloat16 takes those
+// where that leaves fewer of the larger ones' times, counting whole rounds of
+// the CUs.  Loss and dx, us, with 128 and with 256 rows: 32000 x 2048, 128
+// tokens 134 and 163, 256 151 and 172, 512 233 and 210; 128256 x 4096, 128
+// tokens 648 and 707, 160 820 and 732; 50257 x 768, 600 tokens 231 and 248.
+int tile_kind(int dtype, int64_t n, int64_t cols) {
+  if (few_rows(dtype, n)) return 1;
+  if (dtype == ODP_DTYPE_F32) return 0;
+  const int64_t tn = up(cols, 256);
+  return up(up(n, 128) * tn, 256) * 7 < up(up(n, 256) * tn, 256) * 10 ? 2 : 0;
+}
+
 // Workgroups that walk a tm x tn grid of tiles: as many as the CUs hold at a
 // time (one of the large bfloat16 tiles, two of the others), or one a tile (`all`).
-int grid_of(const char* what, int dtype, bool few, int64_t tm, int64_t tn, bool all, unsigned& blocks) {
-  const int64_t b = (tm * tn + 7) / 8 * 8, held = dtype == ODP_DTYPE_F32 || few ? 512 : 256;
+int grid_of(const char* what, int dtype, int kind, int64_t tm, int64_t tn, bool all, unsigned& blocks) {
+  const int64_t b = (tm * tn + 7) / 8 * 8, held = dtype == ODP_DTYPE_F32 || kind == 1 ? 512 : 256;
   if (b >= (int64_t)1 << 31) {
     odp_set_error("%s: %lld tiles", what, (long long)b);
     return ODP_ERR_UNSUPPORTED;
@@ -692,9 +705,10 @@ bool on16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 #define ODP_XENT_LAUNCH_CAP(K, GRID, ...)                                                          \
   do {                                                                                             \
     constexpr int F = ODP_DTYPE_F32, B = ODP_DTYPE_BF16;                                           \
-    if (dtype == F && few) ODP_XENT_CAP(K, F, 1, GRID, __VA_ARGS__);                               \
+    if (dtype == F && kind == 1) ODP_XENT_CAP(K, F, 1, GRID, __VA_ARGS__);                         \
     else if (dtype == F) ODP_XENT_CAP(K, F, 0, GRID, __VA_ARGS__);                                 \
-    else if (few) ODP_XENT_CAP(K, B, 1, GRID, __VA_ARGS__);                                        \
+    else if (kind == 1) ODP_XENT_CAP(K, B, 1, GRID, __VA_ARGS__);                                  \
+    else if (kind == 2) ODP_XENT_CAP(K, B, 2, GRID, __VA_ARGS__);                                  \
     else ODP_XENT_CAP(K, B, 0, GRID, __VA_ARGS__);                                                 \
   } while (0)
 
@@ -760,16 +774,16 @@ extern "C" int odp_xent_losses(odp_stream_t stream, int dtype, const void* xc, i
     return ODP_ERR_INVALID_ARGUMENT;
   }
   const hipStream_t s = odp_hip_stream(stream);
-  const bool few = few_rows(dtype, n);
-  const int64_t tn = up(vocab, tile_cols(dtype, few));
+  const int kind = tile_kind(dtype, n, vocab);
+  const int64_t tn = up(vocab, tile_cols(dtype, kind));
   unsigned blocks;
-  if (int rc = grid_of("odp_xent_losses", dtype, few, up(n, tile_rows(dtype, few)), tn, false, blocks)) return rc;
+  if (int rc = grid_of("odp_xent_losses", dtype, kind, up(n, tile_rows(dtype, kind)), tn, false, blocks)) return rc;
   const Xent p = xent_of(xc, w, ldw, vocab, width, n, count, act, tgt, softcap);
   float* pmax = (float*)scratch;
   float* psum = pmax + n * tn;
   float* ztgt = psum + n * tn;
   ODP_XENT_LAUNCH_CAP(k_xent_stats, blocks, p, pmax, psum, ztgt);
-  if (few)
+  if (kind == 1)
     hipLaunchKernelGGL(k_xent_losses<1>, dim3((unsigned)n), dim3(256), 0, s, pmax, psum, ztgt, (int)tn, n, count, act,
                        tgt, losses, lse);
   else
@@ -809,10 +823,10 @@ extern "C" int odp_xent_dlogits(odp_stream_t stream, int dtype, const void* xc, 
     return ODP_ERR_INVALID_ARGUMENT;
   }
   const hipStream_t s = odp_hip_stream(stream);
-  const bool few = few_rows(dtype, n);
+  const int kind = tile_kind(dtype, n, ldd);
   unsigned blocks;
-  if (int rc = grid_of("odp_xent_dlogits", dtype, few, up(n, tile_rows(dtype, few)), ldd / tile_cols(dtype, few), false,
-                       blocks))
+  if (int rc = grid_of("odp_xent_dlogits", dtype, kind, up(n, tile_rows(dtype, kind)), ldd / tile_cols(dtype, kind),
+                       false, blocks))
     return rc;
   const Xent p = xent_of(xc, w, ldw, vocab, width, n, count, act, tgt, softcap);
   ODP_XENT_LAUNCH_CAP(k_xent_dlogits, blocks, p, v0, vc, lse, g, g_stride, over, dl, ldd, rest);
