@@ -644,36 +644,40 @@ int odp_embed_clipped_sum(odp_stream_t stream, int dtype, const void* g, int64_t
  * softcap tanh(u / softcap) (softcap 0: none), u = x W^T, for rows x [n][cols]
  * (pitch ldx) and a head W [vocab][ldw], both float32 or both bfloat16, without
  * the [n][vocab] logits.  `width` is cols rounded up to 16 bytes; packed rows,
- * W and d lie on the 16-byte grid.  The reference's counterpart is its linear
+ * W, d and kept logits lie on the 16-byte grid.  The reference's counterpart is its linear
  * cross entropy (opaque-patches/.../kernels/linear_cross_entropy.py:249).
  *
  * odp_xent_rows gathers the rows that bear a loss: packed rows xc [n][width],
  * act[k] the row, tgt[k] its target, count[0] how many and count[1] (float32)
- * how many targets are not `ignore`, where[row] the place (-1: target == ignore, -2: target outside the vocabulary); losses (0, or NaN
- * outside the vocabulary) and lse (0) of the rows that bear none, where those
- * are not null.  keep != 0 packs every row, with tgt -1 where it bears no loss. */
+ * how many targets are not `ignore`, where[row] the place (-1: target ==
+ * ignore, -2: target outside the vocabulary); losses (0, or NaN outside the
+ * vocabulary) and lse (0) of the rows that bear none, where those are not null.  keep != 0 packs every row, with tgt -1 where it bears no loss. */
 int odp_xent_rows(odp_stream_t stream, int dtype, const void* x, int64_t ldx, int64_t n, int64_t cols, int64_t width,
                   const void* target, int target_bytes, int64_t vocab, int64_t ignore, int keep, void* xc,
                   int32_t* act, int32_t* tgt, int32_t* where, int32_t* count, float* losses, float* lse);
 
-/* losses and lse of the packed rows, at their places in [n].               */
+/* losses and lse of the packed rows, at their places in [n]; logits (null: not
+ * kept) [n][ldl] receives the packed rows' z, ldl = odp_xent_pitch(dtype, vocab). */
 int64_t odp_xent_stats_scratch(int dtype, int64_t n, int64_t vocab);
 int odp_xent_losses(odp_stream_t stream, int dtype, const void* xc, int64_t n, int64_t width, const int32_t* act,
                     const int32_t* tgt, const int32_t* count, const void* w, int64_t ldw, int64_t vocab,
-                    float softcap, void* scratch, float* losses, float* lse);
+                    float softcap, void* scratch, float* losses, float* lse, float* logits, int64_t ldl);
+
+/* *out = the sum of the losses, over *over where that is not null.          */
+int odp_xent_reduce(odp_stream_t stream, const float* losses, int64_t n, const float* over, float* out);
 
 /* d [count][ldd] of the columns [v0, v0 + vc): g_t (exp(z - lse_t) - [target])
  * times the softcap's slope, in the inputs' type, zero past vc; ldd =
  * odp_xent_pitch(dtype, vc).  lse is per row of [n], g too (g_stride 1) or one
  * for all (0), divided by *over where that is not null.  rest [n]: what
- * rounding takes off each packed row's target entry (bfloat16).              */
-/* *out = the sum of the losses, over *over where that is not null. */
-int odp_xent_reduce(odp_stream_t stream, const float* losses, int64_t n, const float* over, float* out);
+ * rounding takes off each packed row's target entry (bfloat16).  From the kept
+ * logits where those are given (v0 then a multiple of odp_xent_pitch(dtype, 1)),
+ * else from xc and W.                                                        */
 int64_t odp_xent_pitch(int dtype, int64_t columns);
 int odp_xent_dlogits(odp_stream_t stream, int dtype, const void* xc, int64_t n, int64_t width, const int32_t* act,
                      const int32_t* tgt, const int32_t* count, const void* w, int64_t ldw, int64_t vocab,
                      float softcap, int64_t v0, int64_t vc, const float* lse, const float* g, int g_stride,
-                     const float* over, void* dl, int64_t ldd, float* rest);
+                     const float* over, const float* logits, int64_t ldl, void* dl, int64_t ldd, float* rest);
 
 /* Adds d W of a piece of the vocabulary to the float32 sums of dx in scratch
  * (v0 == 0 starts them; pieces of `piece` columns, in order); then

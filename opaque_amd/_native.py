@@ -149,12 +149,13 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "odp_xent_stats_scratch": (_c_i64, [_c_int, _c_i64, _c_i64]),
     "odp_xent_losses": (
         _c_int,
-        [_ptr, _c_int, _ptr, _c_i64, _c_i64, _ptr, _ptr, _ptr, _ptr, _c_i64, _c_i64, _c_f32, _ptr, _ptr, _ptr]),
+        [_ptr, _c_int, _ptr, _c_i64, _c_i64, _ptr, _ptr, _ptr, _ptr, _c_i64, _c_i64, _c_f32, _ptr, _ptr, _ptr,
+         _ptr, _c_i64]),
     "odp_xent_pitch": (_c_i64, [_c_int, _c_i64]),
     "odp_xent_dlogits": (
         _c_int,
         [_ptr, _c_int, _ptr, _c_i64, _c_i64, _ptr, _ptr, _ptr, _ptr, _c_i64, _c_i64, _c_f32, _c_i64, _c_i64, _ptr,
-         _ptr, _c_int, _ptr, _ptr, _c_i64, _ptr],
+         _ptr, _c_int, _ptr, _ptr, _c_i64, _ptr, _c_i64, _ptr],
     ),
     "odp_xent_reduce": (_c_int, [_ptr, _ptr, _c_i64, _ptr, _ptr]),
     "odp_xent_dx_scratch": (_c_i64, [_c_int, _c_i64, _c_i64]),

@@ -176,7 +176,7 @@ at::Tensor head_rows(const at::Tensor& weight) {
 
 // The packed rows of a call (odp_xent_rows) and what its backward needs.
 struct Packed {
-  at::Tensor w, xc, ids, losses, lse;
+  at::Tensor w, xc, ids, losses, lse, logits;  // logits: where they are kept
   int64_t n, cols, width, vocab;
   int dt;
   int32_t* count() const { return (int32_t*)ids.data_ptr(); }
@@ -184,10 +184,13 @@ struct Packed {
   int32_t* act() const { return count() + 2; }
   int32_t* tgt() const { return act() + std::max<int64_t>(n, 1); }
   int32_t* where() const { return tgt() + std::max<int64_t>(n, 1); }
+  float* kept() const { return logits.defined() ? (float*)logits.data_ptr() : nullptr; }
+  int64_t kept_pitch() const { return abi.xent_pitch(dt, vocab); }
 };
 
+// keep_bytes: up to which the logits are kept for a backward pass.
 Packed xent_forward(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target, double softcap,
-                    int64_t ignore) {
+                    int64_t ignore, int64_t keep_bytes) {
   Packed p;
   p.w = head_rows(weight);
   const at::Tensor rows = pitched(x), y = target.contiguous();
@@ -208,9 +211,11 @@ Packed xent_forward(const at::Tensor& x, const at::Tensor& weight, const at::Ten
                       (int)y.element_size(), p.vocab, ignore, 0, p.xc.data_ptr(), p.act(), p.tgt(), p.where(),
                       p.count(), losses, lse),
         "odp_xent_rows");
+  if (p.n > 0 && p.kept_pitch() <= keep_bytes / 4 / p.n)
+    p.logits = at::empty({p.n, p.kept_pitch()}, p.losses.options());
   const at::Tensor work = bytes_on(rows, abi.xent_stats_scratch(p.dt, p.n, p.vocab));
   check(abi.xent_losses(s, p.dt, p.xc.data_ptr(), p.n, p.width, p.act(), p.tgt(), p.count(), p.w.data_ptr(),
-                        p.w.stride(0), p.vocab, (float)softcap, work.data_ptr(), losses, lse),
+                        p.w.stride(0), p.vocab, (float)softcap, work.data_ptr(), losses, lse, p.kept(), p.kept_pitch()),
         "odp_xent_losses");
   return p;
 }
@@ -228,10 +233,11 @@ at::Tensor xent_result(const Packed& p, int64_t reduction) {
 struct Xent : torch::autograd::Function<Xent> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight,
                             const at::Tensor& target, double softcap, int64_t ignore, int64_t reduction,
-                            int64_t piece_bytes) {
+                            int64_t piece_bytes, int64_t keep_bytes) {
     const c10::OptionalDeviceGuard guard(x.device());
-    const Packed p = xent_forward(x, weight, target, softcap, ignore);
-    ctx->save_for_backward({weight});  // a later change of the head in place is an error
+    const Packed p = xent_forward(x, weight, target, softcap, ignore, keep_bytes);
+    // A later change of the head in place is an error; the kept logits go when the backward pass is through.
+    ctx->save_for_backward({weight, p.logits});
     auto& d = ctx->saved_data;
     d["w"] = p.w;
     d["xc"] = p.xc;
@@ -248,8 +254,8 @@ struct Xent : torch::autograd::Function<Xent> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
     at::Tensor dx, dw;
-    if (!grads[0].defined()) return {{}, {}, {}, {}, {}, {}, {}};
-    ctx->get_saved_variables();
+    if (!grads[0].defined()) return {{}, {}, {}, {}, {}, {}, {}, {}};
+    const torch::autograd::variable_list saved = ctx->get_saved_variables();
     {
       at::NoGradGuard no_grad;
       auto& sd = ctx->saved_data;
@@ -257,6 +263,7 @@ struct Xent : torch::autograd::Function<Xent> {
       p.w = sd["w"].toTensor();
       p.xc = sd["xc"].toTensor();
       p.ids = sd["ids"].toTensor();
+      p.logits = saved[1];
       p.n = sd["n"].toInt();
       p.cols = sd["cols"].toInt();
       p.width = p.w.size(1);
@@ -286,7 +293,7 @@ struct Xent : torch::autograd::Function<Xent> {
         const int64_t vc = std::min(piece, p.vocab - v0), ldd = abi.xent_pitch(p.dt, vc);
         check(abi.xent_dlogits(s, p.dt, p.xc.data_ptr(), p.n, p.width, p.act(), p.tgt(), p.count(), p.w.data_ptr(),
                                p.w.stride(0), p.vocab, softcap, v0, vc, (const float*)lse.data_ptr(),
-                               (const float*)g.data_ptr(), stride, over, d.data_ptr(), ldd,
+                               (const float*)g.data_ptr(), stride, over, p.kept(), p.kept_pitch(), d.data_ptr(), ldd,
                                (float*)rest.data_ptr()),
               "odp_xent_dlogits");
         if (need_x)
@@ -304,17 +311,17 @@ struct Xent : torch::autograd::Function<Xent> {
               "odp_xent_dx_rows");
       if (need_w && p.cols != p.width) dw = dw.narrow(1, 0, p.cols).contiguous();
     }
-    return {first_only(grads[0], dx), first_only(grads[0], dw), {}, {}, {}, {}, {}};
+    return {first_only(grads[0], dx), first_only(grads[0], dw), {}, {}, {}, {}, {}, {}};
   }
 };
 
 at::Tensor cross_entropy(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target, double softcap,
-                         int64_t ignore, int64_t reduction, int64_t piece_bytes) {
+                         int64_t ignore, int64_t reduction, int64_t piece_bytes, int64_t keep_bytes) {
   py::gil_scoped_release nogil;
   if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad()))
-    return Xent::apply(x, weight, target, softcap, ignore, reduction, piece_bytes);
+    return Xent::apply(x, weight, target, softcap, ignore, reduction, piece_bytes, keep_bytes);
   const c10::OptionalDeviceGuard guard(x.device());
-  return xent_result(xent_forward(x, weight, target, softcap, ignore), reduction);
+  return xent_result(xent_forward(x, weight, target, softcap, ignore, 0), reduction);
 }
 
 }  // namespace
@@ -323,5 +330,5 @@ void add_vocabulary(py::module_& m) {
   m.def("bind", &bind, py::arg("entry_points"));
   m.def("embedding", &embedding, py::arg("tokens"), py::arg("weight"), py::arg("scale"), py::arg("padding"));
   m.def("cross_entropy", &cross_entropy, py::arg("x"), py::arg("weight"), py::arg("target"), py::arg("softcap"),
-        py::arg("ignore"), py::arg("reduction"), py::arg("piece_bytes"));
+        py::arg("ignore"), py::arg("reduction"), py::arg("piece_bytes"), py::arg("keep_bytes"));
 }

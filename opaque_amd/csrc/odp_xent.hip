@@ -213,7 +213,7 @@ struct Xent {
 template <int DT, int S, bool CAP, bool WHOLE>
 __device__ __forceinline__ void stats_tile(const Xent& p, const typename Tile<DT, S>::Acc& acc, int cnt, int64_t o0,
                                            int64_t n0, const int32_t (&tgt)[Tile<DT, S>::BI], float* red,
-                                           float* __restrict__ ztgt) {
+                                           float* __restrict__ ztgt, float* __restrict__ logits, int64_t ldl) {
   using T = Tile<DT, S>;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = T::WM * (wave & 1), wn = T::WN * (wave >> 1);
@@ -238,6 +238,11 @@ __device__ __forceinline__ void stats_tile(const Xent& p, const typename Tile<DT
         m = fmaxf(m, z[j][e]);
       }
     if (here) ztgt[o0 + wm + t_row(i)] = zt;
+    if (logits != nullptr && o0 + wm + t_row(i) < cnt) {
+      float* to = logits + (o0 + wm + t_row(i)) * ldl + n0 + c0;
+#pragma unroll
+      for (int j = 0; j < T::BJ; ++j) odp_gstore((f32x4_t*)(to + 16 * j), f32x4_t{z[j][0], z[j][1], z[j][2], z[j][3]});
+    }
     const float ms = m == -INFINITY ? 0.f : m;
     float s = 0.f;
 #pragma unroll
@@ -264,7 +269,8 @@ __device__ __forceinline__ void stats_tile(const Xent& p, const typename Tile<DT
 template <int DT, int S, bool CAP>
 __global__ __launch_bounds__((Tile<DT, S>::THREADS), 2) void k_xent_stats(Xent p, float* __restrict__ pmax,
                                                                      float* __restrict__ psum,
-                                                                     float* __restrict__ ztgt) {
+                                                                     float* __restrict__ ztgt,
+                                                                     float* __restrict__ logits, int64_t ldl) {
   using T = Tile<DT, S>;
   __shared__ float red[T::WAVES / 2 * T::OT * 2];  // [waves across n][rows][maximum, sum]
   const int cnt = *(const ODP_CONST int32_t*)p.count;
@@ -289,8 +295,8 @@ __global__ __launch_bounds__((Tile<DT, S>::THREADS), 2) void k_xent_stats(Xent p
     walk.next();
     more = walk.tile(ti, tj);
     if (more) begin();
-    if (n0 + T::NT <= p.vocab) stats_tile<DT, S, CAP, true>(p, acc, cnt, o0, n0, tgt, red, ztgt);
-    else stats_tile<DT, S, CAP, false>(p, acc, cnt, o0, n0, tgt, red, ztgt);
+    if (n0 + T::NT <= p.vocab) stats_tile<DT, S, CAP, true>(p, acc, cnt, o0, n0, tgt, red, ztgt, logits, ldl);
+    else stats_tile<DT, S, CAP, false>(p, acc, cnt, o0, n0, tgt, red, ztgt, logits, ldl);
     __syncthreads();
     for (int r = threadIdx.x; r < T::OT; r += T::THREADS) {
       if (o0 + r >= cnt) break;
@@ -501,6 +507,58 @@ __global__ __launch_bounds__((Tile<DT, S>::THREADS), (DT == ODP_DTYPE_BF16 && S 
     if (more) begin();
     if (n0 + T::NT <= vc) dlogits_tile<DT, S, CAP, true>(p, acc, rows, cnt, o0, n0, vc, dl, ldd, rest);
     else dlogits_tile<DT, S, CAP, false>(p, acc, rows, cnt, o0, n0, vc, dl, ldd, rest);
+  }
+}
+
+// The same from kept logits (pitch ldl): a workgroup takes KEPT_COLS columns of
+// a row, a thread 16 bytes of d at a time.
+constexpr int KEPT_COLS = 4096;
+template <int DT, bool CAP>
+__global__ __launch_bounds__(256) void k_xent_dkept(Xent p, const float* __restrict__ logits, int64_t ldl, int64_t v0,
+                                                    int64_t vc, int parts, const float* __restrict__ lse,
+                                                    const float* __restrict__ g, int g_stride,
+                                                    const float* __restrict__ over, char* __restrict__ dl, int64_t ldd,
+                                                    float* __restrict__ rest) {
+  constexpr int ES = Tile<DT, 0>::ES, V = 16 / ES, ROUNDS = KEPT_COLS / 256 / V;
+  const int64_t k = blockIdx.x / (uint32_t)parts;
+  const int c0 = (int)(blockIdx.x - (uint32_t)k * (uint32_t)parts) * KEPT_COLS;
+  if (k >= *(const ODP_CONST int32_t*)p.count) return;
+  const float* from = logits + k * ldl + v0;
+  f32x4_t z[ROUNDS][V / 4];
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const int c = c0 + (r * 256 + (int)threadIdx.x) * V;
+#pragma unroll
+    for (int h = 0; h < V / 4; ++h)
+      if (c < ldd) z[r][h] = __builtin_nontemporal_load((const ODP_GMEM f32x4_t*)(const ODP_GMEM void*)(from + c + 4 * h));
+  }
+  const int32_t t = p.tgt[k];
+  const int64_t row = p.act[k];
+  const int at = t - (int)v0;
+  const float l = t >= 0 ? lse[row] : 0.f, part = over != nullptr ? *over : 1.f;
+  const float gr = t >= 0 ? g[row * g_stride] / part : 0.f, inv_cap = 0.5f * p.inv_cap2;
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const int c = c0 + (r * 256 + (int)threadIdx.x) * V;
+    if (c >= ldd) return;
+    float d[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float y = z[r][e / 4][e % 4];
+      float q = fast_exp(y - l);
+      const bool hit = at == c + e;
+      q = (hit ? q - 1.f : q) * gr;
+      if (CAP) q *= 1.f - y * inv_cap * (y * inv_cap);
+      d[e] = t >= 0 && c + e < vc ? q : 0.f;
+      if (DT == ODP_DTYPE_BF16 && hit && t >= 0) rest[k] = q - odp_round_bf16(q);
+    }
+    char* to = dl + (k * ldd + c) * ES;
+    if constexpr (DT == ODP_DTYPE_F32) {
+      odp_gstore((f32x4_t*)to, f32x4_t{d[0], d[1], d[2], d[3]});
+    } else {
+      odp_gstore((u32x4_t*)to, u32x4_t{odp_f2bf2(d[0], d[1]), odp_f2bf2(d[2], d[3]), odp_f2bf2(d[4], d[5]),
+                                       odp_f2bf2(d[6], d[7])});
+    }
   }
 }
 
@@ -765,12 +823,18 @@ extern "C" int64_t odp_xent_stats_scratch(int dtype, int64_t n, int64_t vocab) {
 
 extern "C" int odp_xent_losses(odp_stream_t stream, int dtype, const void* xc, int64_t n, int64_t width,
                                const int32_t* act, const int32_t* tgt, const int32_t* count, const void* w,
-                               int64_t ldw, int64_t vocab, float softcap, void* scratch, float* losses, float* lse) {
+                               int64_t ldw, int64_t vocab, float softcap, void* scratch, float* losses, float* lse,
+                               float* logits, int64_t ldl) {
   if (int rc = check_xent("odp_xent_losses", dtype, n, width, ldw, vocab)) return rc;
   if (n == 0) return ODP_OK;
   if (xc == nullptr || act == nullptr || tgt == nullptr || count == nullptr || w == nullptr || scratch == nullptr ||
       losses == nullptr || lse == nullptr || !on16(xc) || !on16(w)) {
     odp_set_error("odp_xent_losses: null pointer, or rows off the 16-byte grid");
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  if (logits != nullptr && (ldl != odp_xent_pitch(dtype, vocab) || !on16(logits))) {
+    odp_set_error("odp_xent_losses: logits of pitch %lld for a vocabulary of %lld, or off the 16-byte grid",
+                  (long long)ldl, (long long)vocab);
     return ODP_ERR_INVALID_ARGUMENT;
   }
   const hipStream_t s = odp_hip_stream(stream);
@@ -782,7 +846,7 @@ extern "C" int odp_xent_losses(odp_stream_t stream, int dtype, const void* xc, i
   float* pmax = (float*)scratch;
   float* psum = pmax + n * tn;
   float* ztgt = psum + n * tn;
-  ODP_XENT_LAUNCH_CAP(k_xent_stats, blocks, p, pmax, psum, ztgt);
+  ODP_XENT_LAUNCH_CAP(k_xent_stats, blocks, p, pmax, psum, ztgt, logits, ldl);
   if (kind == 1)
     hipLaunchKernelGGL(k_xent_losses<1>, dim3((unsigned)n), dim3(256), 0, s, pmax, psum, ztgt, (int)tn, n, count, act,
                        tgt, losses, lse);
@@ -808,8 +872,8 @@ extern "C" int64_t odp_xent_pitch(int dtype, int64_t columns) {
 extern "C" int odp_xent_dlogits(odp_stream_t stream, int dtype, const void* xc, int64_t n, int64_t width,
                                 const int32_t* act, const int32_t* tgt, const int32_t* count, const void* w,
                                 int64_t ldw, int64_t vocab, float softcap, int64_t v0, int64_t vc, const float* lse,
-                                const float* g, int g_stride, const float* over, void* dl, int64_t ldd,
-                                float* rest) {
+                                const float* g, int g_stride, const float* over, const float* logits, int64_t ldl,
+                                void* dl, int64_t ldd, float* rest) {
   if (int rc = check_xent("odp_xent_dlogits", dtype, n, width, ldw, vocab)) return rc;
   if (v0 < 0 || vc <= 0 || v0 + vc > vocab || ldd != odp_xent_pitch(dtype, vc)) {
     odp_set_error("odp_xent_dlogits: columns [%lld, %lld) of %lld at pitch %lld", (long long)v0,
@@ -823,6 +887,27 @@ extern "C" int odp_xent_dlogits(odp_stream_t stream, int dtype, const void* xc, 
     return ODP_ERR_INVALID_ARGUMENT;
   }
   const hipStream_t s = odp_hip_stream(stream);
+  if (logits != nullptr) {
+    // Pieces start on a tile's edge, so that a piece's padded columns lie inside the logits' row.
+    const int64_t parts = up(ldd, KEPT_COLS);
+    if (ldl != odp_xent_pitch(dtype, vocab) || !on16(logits) || v0 % tile_edge(dtype) != 0 ||
+        n * parts >= (int64_t)1 << 24) {
+      odp_set_error("odp_xent_dlogits: logits of pitch %lld from column %lld, %lld workgroups", (long long)ldl,
+                    (long long)v0, (long long)(n * parts));
+      return ODP_ERR_INVALID_ARGUMENT;
+    }
+    const Xent p = xent_of(nullptr, nullptr, 0, vocab, width, n, count, act, tgt, softcap);
+#define ODP_KEPT(D, C)                                                                                                 \
+  ODP_XENT_GO((k_xent_dkept<D, C>), 256, (unsigned)(n * parts), p, logits, ldl, v0, vc, (int)parts, lse, g, g_stride,  \
+              over, (char*)dl, ldd, rest)
+    if (dtype == ODP_DTYPE_F32) {
+      if (softcap != 0.f) ODP_KEPT(ODP_DTYPE_F32, true); else ODP_KEPT(ODP_DTYPE_F32, false);
+    } else {
+      if (softcap != 0.f) ODP_KEPT(ODP_DTYPE_BF16, true); else ODP_KEPT(ODP_DTYPE_BF16, false);
+    }
+#undef ODP_KEPT
+    return odp_check_launch("odp_xent_dlogits");
+  }
   const int kind = tile_kind(dtype, n, ldd);
   unsigned blocks;
   if (int rc = grid_of("odp_xent_dlogits", dtype, kind, up(n, tile_rows(dtype, kind)), ldd / tile_cols(dtype, kind),

@@ -276,6 +276,8 @@ _HEAD_DTYPES = (torch.float32, torch.bfloat16)
 # Bytes of d (the logits' gradient, in the inputs' type) that the backward
 # holds at a time: a piece of the vocabulary for all tokens.
 PIECE_BYTES = 512 << 20
+# Bytes up to which the forward keeps the float32 logits for the backward.
+KEEP_BYTES = 4 << 30
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 
@@ -331,7 +333,7 @@ class _Packed:
                               device=self.xc.device)
         _call("odp_xent_losses", _stream(self.xc), self.dt, self.xc.data_ptr(), self.n, self.width, self.act,
               self.tgt, self.count, self.w.data_ptr(), self.w.stride(0), self.vocab, softcap, scratch.data_ptr(),
-              losses.data_ptr(), lse.data_ptr())
+              losses.data_ptr(), lse.data_ptr(), None, 0)
 
     def piece(self, whole: bool = False) -> int:
         """Columns of the vocabulary a piece of d holds: as many pieces as PIECE_BYTES makes, of one size."""
@@ -360,8 +362,8 @@ class _Packed:
             vc = min(piece, self.vocab - v0)
             ldd = _xent_pitch(dt, vc)
             _call("odp_xent_dlogits", s, dt, xc, self.n, self.width, self.act, self.tgt, self.count, w, ldw,
-                  self.vocab, softcap, v0, vc, lse.data_ptr(), g.data_ptr(), 1, None, d.data_ptr(), ldd,
-                  rest.data_ptr())
+                  self.vocab, softcap, v0, vc, lse.data_ptr(), g.data_ptr(), 1, None, None, 0, d.data_ptr(),
+                  ldd, rest.data_ptr())
             if dx is not None:
                 _call("odp_xent_dx", s, dt, self.n, self.width, self.count, w, ldw, self.vocab, v0, vc, piece,
                       d.data_ptr(), ldd, sums.data_ptr())
@@ -528,7 +530,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
         weight = weight.detach()
     host = None if _transformed() else _bound()
     if host is not None:
-        return host.cross_entropy(x, weight, target, softcap or 0.0, ignore_index, _REDUCTIONS[reduction], PIECE_BYTES)
+        return host.cross_entropy(x, weight, target, softcap or 0.0, ignore_index, _REDUCTIONS[reduction], PIECE_BYTES,
+                                  KEEP_BYTES)
     losses, _ = _Xent.apply(x, weight, target, float(softcap or 0.0), int(ignore_index))
     if reduction == "none":
         return losses

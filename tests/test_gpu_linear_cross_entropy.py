@@ -438,3 +438,58 @@ def test_in_a_graph(dtype):
         got = [t.detach().clone() for t in held]
         for a, b in zip(got, step()):
             assert torch.equal(a, b.detach())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("n,width,vocab", [(1, 64, 1000), (5, 40, 3), (70, 96, 2050), (130, 72, 4097), (300, 40, 9000),
+                                           (600, 64, 257)])
+@pytest.mark.parametrize("softcap", [None, 5.0])
+def test_kept_logits(n, width, vocab, softcap, dtype, monkeypatch):
+    """The forward's logits, kept, give the bits that forming them again gives, in pieces too."""
+    x, w, y, gl = inputs(n, width, vocab, dtype, seed=n + 3 * vocab)
+    y[0] = vocab - 1
+    kept = run(x, w, y, gl, softcap)
+    monkeypatch.setattr(vocabulary, "PIECE_BYTES", max(n, 1) * 4 * 512)
+    for a, b in zip(kept[:1] + kept[2:], (run(x, w, y, gl, softcap))[:1] + run(x, w, y, gl, softcap)[2:]):
+        assert torch.equal(a, b)  # dx: pieces change the order of its sums
+    monkeypatch.undo()
+    monkeypatch.setattr(vocabulary, "KEEP_BYTES", 0)
+    for a, b in zip(kept, run(x, w, y, gl, softcap)):
+        assert torch.equal(a, b)
+
+
+def test_logits_are_kept_up_to_a_size_and_until_the_backward(monkeypatch):
+    """KEEP_BYTES bounds what a call holds; without a gradient nothing is held, after the backward neither."""
+    n, width, vocab = 512, 64, 16384
+    x, w, y, _ = inputs(n, width, vocab, torch.bfloat16, seed=2)
+    x, w, y = x.to(DEV).requires_grad_(), w.to(DEV), y.to(DEV)
+    logits = 4 * n * vocab
+
+    def held(**kw):
+        before = torch.cuda.memory_allocated()
+        loss = linear_cross_entropy(x, w, y, **kw)
+        mid = torch.cuda.memory_allocated() - before
+        if loss.requires_grad:
+            loss.backward()
+            x.grad = None
+        return mid, torch.cuda.memory_allocated() - before
+
+    held()
+    mid, after = held()
+    assert mid >= logits and after < logits / 4
+    monkeypatch.setattr(vocabulary, "KEEP_BYTES", logits - 1)
+    assert held()[0] < logits / 4
+    monkeypatch.undo()
+    with torch.no_grad():
+        assert held()[0] < logits / 4
+
+
+def test_two_backward_passes_of_one_loss():
+    x, w, y, gl = inputs(40, 64, 700, torch.bfloat16, seed=12)
+    x, w = x.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+    loss = linear_cross_entropy(x, w, y.to(DEV))
+    first = torch.autograd.grad(loss, [x, w], retain_graph=True)
+    for a, b in zip(first, torch.autograd.grad(loss, [x, w])):
+        assert torch.equal(a, b)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(loss, [x, w])
