@@ -657,7 +657,9 @@ int odp_xent_rows(odp_stream_t stream, int dtype, const void* x, int64_t ldx, in
                   int32_t* act, int32_t* tgt, int32_t* where, int32_t* count, float* losses, float* lse);
 
 /* losses and lse of the packed rows, at their places in [n]; logits (null: not
- * kept) [n][ldl] receives the packed rows' z, ldl = odp_xent_pitch(dtype, vocab). */
+ * kept) [n][ldl] receives the packed rows' z, ldl = odp_xent_pitch(dtype, vocab).
+ * odp_xent_kept: their bytes, 0 where forming them again is faster.          */
+int64_t odp_xent_kept(int dtype, int64_t n, int64_t width, int64_t vocab);
 int64_t odp_xent_stats_scratch(int dtype, int64_t n, int64_t vocab);
 int odp_xent_losses(odp_stream_t stream, int dtype, const void* xc, int64_t n, int64_t width, const int32_t* act,
                     const int32_t* tgt, const int32_t* count, const void* w, int64_t ldw, int64_t vocab,
@@ -690,9 +692,11 @@ int odp_xent_dx_rows(odp_stream_t stream, int dtype, int64_t n, int64_t cols, in
                      const int32_t* where, const int32_t* tgt, const void* w, int64_t ldw, int64_t piece,
                      const void* scratch, const float* rest, void* dx);
 
-/* dW rows of a piece, [vc] of pitch lddw, = d^T x.                          */
+/* dW rows of a piece, [vc] of pitch lddw, = d^T x; scratch may be null where
+ * odp_xent_dw_scratch is 0.                                                 */
+int64_t odp_xent_dw_scratch(int dtype, int64_t n, int64_t vc, int64_t width);
 int odp_xent_dw(odp_stream_t stream, int dtype, const void* xc, int64_t n, int64_t width, const int32_t* count,
-                int64_t vc, const void* dl, int64_t ldd, void* dw, int64_t lddw);
+                int64_t vc, const void* dl, int64_t ldd, void* scratch, void* dw, int64_t lddw);
 
 #ifdef __cplusplus
 }

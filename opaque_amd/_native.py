@@ -147,6 +147,7 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
          _ptr, _ptr, _ptr, _ptr],
     ),
     "odp_xent_stats_scratch": (_c_i64, [_c_int, _c_i64, _c_i64]),
+    "odp_xent_kept": (_c_i64, [_c_int, _c_i64, _c_i64, _c_i64]),
     "odp_xent_losses": (
         _c_int,
         [_ptr, _c_int, _ptr, _c_i64, _c_i64, _ptr, _ptr, _ptr, _ptr, _c_i64, _c_i64, _c_f32, _ptr, _ptr, _ptr,
@@ -166,7 +167,8 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _c_int,
         [_ptr, _c_int, _c_i64, _c_i64, _c_i64, _ptr, _ptr, _ptr, _ptr, _c_i64, _c_i64, _ptr, _ptr, _ptr]),
     "odp_xent_dw": (
-        _c_int, [_ptr, _c_int, _ptr, _c_i64, _c_i64, _ptr, _c_i64, _ptr, _c_i64, _ptr, _c_i64]),
+        _c_int, [_ptr, _c_int, _ptr, _c_i64, _c_i64, _ptr, _c_i64, _ptr, _c_i64, _ptr, _ptr, _c_i64]),
+    "odp_xent_dw_scratch": (_c_i64, [_c_int, _c_i64, _c_i64, _c_i64]),
     "odp_linear_moments_blocks": (_c_i64, [_c_i64, _c_i64, _c_i32]),
     "odp_linear_moments": (
         _c_int, [_ptr, _ptr, _ptr, _c_i32, _c_i32, _ptr, _ptr, _ptr, _ptr, _c_i32, _c_i32, _c_f32, _c_i32]),

@@ -29,6 +29,7 @@ struct Abi {
   decltype(&odp_embed_grad) embed_grad = nullptr;
   decltype(&odp_xent_rows) xent_rows = nullptr;
   decltype(&odp_xent_stats_scratch) xent_stats_scratch = nullptr;
+  decltype(&odp_xent_kept) xent_kept = nullptr;
   decltype(&odp_xent_losses) xent_losses = nullptr;
   decltype(&odp_xent_reduce) xent_reduce = nullptr;
   decltype(&odp_xent_pitch) xent_pitch = nullptr;
@@ -36,6 +37,7 @@ struct Abi {
   decltype(&odp_xent_dx_scratch) xent_dx_scratch = nullptr;
   decltype(&odp_xent_dx) xent_dx = nullptr;
   decltype(&odp_xent_dx_rows) xent_dx_rows = nullptr;
+  decltype(&odp_xent_dw_scratch) xent_dw_scratch = nullptr;
   decltype(&odp_xent_dw) xent_dw = nullptr;
 };
 Abi abi;
@@ -51,6 +53,7 @@ void bind(const std::unordered_map<std::string, uintptr_t>& at) {
   ODP_BIND(embed_grad);
   ODP_BIND(xent_rows);
   ODP_BIND(xent_stats_scratch);
+  ODP_BIND(xent_kept);
   ODP_BIND(xent_losses);
   ODP_BIND(xent_reduce);
   ODP_BIND(xent_pitch);
@@ -58,6 +61,7 @@ void bind(const std::unordered_map<std::string, uintptr_t>& at) {
   ODP_BIND(xent_dx_scratch);
   ODP_BIND(xent_dx);
   ODP_BIND(xent_dx_rows);
+  ODP_BIND(xent_dw_scratch);
   ODP_BIND(xent_dw);
 #undef ODP_BIND
   abi = b;
@@ -211,8 +215,8 @@ Packed xent_forward(const at::Tensor& x, const at::Tensor& weight, const at::Ten
                       (int)y.element_size(), p.vocab, ignore, 0, p.xc.data_ptr(), p.act(), p.tgt(), p.where(),
                       p.count(), losses, lse),
         "odp_xent_rows");
-  if (p.n > 0 && p.kept_pitch() <= keep_bytes / 4 / p.n)
-    p.logits = at::empty({p.n, p.kept_pitch()}, p.losses.options());
+  const int64_t kept = abi.xent_kept(p.dt, p.n, p.width, p.vocab);
+  if (kept > 0 && kept <= keep_bytes) p.logits = at::empty({p.n, p.kept_pitch()}, p.losses.options());
   const at::Tensor work = bytes_on(rows, abi.xent_stats_scratch(p.dt, p.n, p.vocab));
   check(abi.xent_losses(s, p.dt, p.xc.data_ptr(), p.n, p.width, p.act(), p.tgt(), p.count(), p.w.data_ptr(),
                         p.w.stride(0), p.vocab, (float)softcap, work.data_ptr(), losses, lse, p.kept(), p.kept_pitch()),
@@ -300,10 +304,13 @@ struct Xent : torch::autograd::Function<Xent> {
           check(abi.xent_dx(s, p.dt, p.n, p.width, p.count(), p.w.data_ptr(), p.w.stride(0), p.vocab, v0, vc, piece,
                             d.data_ptr(), ldd, sums.data_ptr()),
                 "odp_xent_dx");
-        if (need_w)
+        if (need_w) {
+          const int64_t split = abi.xent_dw_scratch(p.dt, p.n, vc, p.width);
+          const at::Tensor slots = split > 0 ? bytes_on(p.xc, split) : at::Tensor();
           check(abi.xent_dw(s, p.dt, p.xc.data_ptr(), p.n, p.width, p.count(), vc, d.data_ptr(), ldd,
-                            (char*)dw.data_ptr() + v0 * p.width * es, p.width),
+                            split > 0 ? slots.data_ptr() : nullptr, (char*)dw.data_ptr() + v0 * p.width * es, p.width),
                 "odp_xent_dw");
+        }
       }
       if (need_x)
         check(abi.xent_dx_rows(s, p.dt, p.n, p.cols, p.width, p.count(), p.where(), p.tgt(), p.w.data_ptr(),

@@ -680,6 +680,62 @@ __global__ __launch_bounds__((Tile<DT, 0>::THREADS), 2) void k_xent_dw(Xent p, i
   }
 }
 
+// A slice of the tokens of each tile of dW into its slot [vc][width] (float32):
+// few tiles of many tokens leave most of the CUs idle otherwise.
+template <int DT>
+__global__ __launch_bounds__((Tile<DT, 0>::THREADS), 2) void k_xent_dw_part(Xent p, int64_t vc, const void* dl,
+                                                                            int64_t ldd, int split,
+                                                                            float* __restrict__ slots) {
+  using T = Tile<DT, 0>;
+  const int cnt = *(const ODP_CONST int32_t*)p.count;
+  const int tm = (int)((vc + T::OT - 1) / T::OT), tn = (int)((p.width + T::NT - 1) / T::NT);
+  int ti, tj;
+  if (!Walk(tm, tn * split).tile(ti, tj)) return;  // a workgroup per tile and slice
+  const int s = tj / tn;
+  tj -= s * tn;
+  const int64_t o0 = (int64_t)ti * T::OT, n0 = (int64_t)tj * T::NT;
+  const int64_t per = ((int64_t)cnt + (int64_t)T::EK * split - 1) / ((int64_t)T::EK * split) * T::EK;
+  const int64_t k0 = min((int64_t)cnt, s * per);
+  typename T::Acc acc;
+  Product<DT, 0, false, false> prod;
+  prod.begin(Operand{(const char*)dl + k0 * ldd * T::ES, ldd, o0, ldd},
+             Operand{(const char*)p.xc + k0 * p.width * T::ES, p.width, n0, p.width}, (int32_t)min(per, cnt - k0));
+  prod.run(acc);
+  const int wave = threadIdx.x >> 6;
+  const int wm = T::WM * (wave & 1), wn = T::WN * (wave >> 1);
+  float* out = slots + s * vc * p.width;
+  static_for<T::BI * T::BJ>([&](auto q) __attribute__((always_inline)) {
+    constexpr int i = decltype(q)::value / T::BJ, j = decltype(q)::value % T::BJ;
+    const int64_t o = o0 + wm + t_row(i), n = n0 + wn + t_col(j);
+    if (o < vc && n < p.width) odp_gstore((f32x4_t*)(out + o * p.width + n), acc[i][j]);
+    __builtin_amdgcn_sched_barrier(0);
+  });
+}
+
+// dW from the slots, added in one order: Q threads each take every Q-th slot.
+template <int DT, int Q>
+__global__ __launch_bounds__(256) void k_xent_dw_rows(const float* __restrict__ slots, int split, int64_t quads,
+                                                      void* __restrict__ dw) {
+  constexpr int R = 256 / Q;
+  __shared__ f32x4_t part[Q][R];
+  const int r = threadIdx.x % R, q = threadIdx.x / R;
+  const int64_t i = (int64_t)blockIdx.x * R + r;
+  f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+  if (i < quads) {
+#pragma unroll 8
+    for (int s = q; s < split; s += Q) v = v + *((const f32x4_t*)slots + s * quads + i);
+  }
+  if constexpr (Q > 1) {
+    part[q][r] = v;
+    __syncthreads();
+    if (q != 0) return;
+    for (int k = 1; k < Q; ++k) v = v + part[k][r];
+  }
+  if (i >= quads) return;
+  if constexpr (DT == ODP_DTYPE_F32) odp_gstore((f32x4_t*)dw + i, v);
+  else odp_gstore((u32x2_t*)dw + i, u32x2_t{odp_f2bf2(v[0], v[1]), odp_f2bf2(v[2], v[3])});
+}
+
 int check_xent(const char* what, int dtype, int64_t n, int64_t width, int64_t ldw, int64_t vocab) {
   if (dtype != ODP_DTYPE_F32 && dtype != ODP_DTYPE_BF16) {
     odp_set_error("%s: rows must be float32 or bfloat16 (dtype %d)", what, dtype);
@@ -720,6 +776,16 @@ int tile_kind(int dtype, int64_t n, int64_t cols) {
   if (dtype == ODP_DTYPE_F32) return 0;
   const int64_t tn = up(cols, 256);
   return up(up(n, 128) * tn, 256) * 7 < up(up(n, 256) * tn, 256) * 10 ? 2 : 0;
+}
+
+// Whether logits are worth keeping for the backward: 8 bytes of traffic each
+// against 2 width operations, or W's share of reading it again where the rows
+// are few.  Loss and gradients, us, formed again and kept: bfloat16, 4096 x
+// 32000, width 256 439 and 519, 640 749 and 768, 768 815 and 802, 1024 971 and
+// 902; 64 x 128256, width 256 106 and 98; float32, 4096 x 32000, width 64 973 and
+// 977, 128 1213 and 1092.
+bool keeps(int dtype, int64_t n, int64_t width) {
+  return width >= (dtype == ODP_DTYPE_F32 ? 128 : 768) || width >= 4 * n;
 }
 
 // Workgroups that walk a tm x tn grid of tiles: as many as the CUs hold at a
@@ -819,6 +885,11 @@ extern "C" int odp_xent_rows(odp_stream_t stream, int dtype, const void* x, int6
 extern "C" int64_t odp_xent_stats_scratch(int dtype, int64_t n, int64_t vocab) {
   if (n <= 0 || vocab <= 0) return 0;
   return 4 * n * (2 * up(vocab, tile_cols(dtype, few_rows(dtype, n))) + 1);
+}
+
+extern "C" int64_t odp_xent_kept(int dtype, int64_t n, int64_t width, int64_t vocab) {
+  if (n <= 0 || width <= 0 || vocab <= 0 || !keeps(dtype, n, width)) return 0;
+  return 4 * n * odp_xent_pitch(dtype, vocab);
 }
 
 extern "C" int odp_xent_losses(odp_stream_t stream, int dtype, const void* xc, int64_t n, int64_t width,
@@ -997,8 +1068,23 @@ extern "C" int odp_xent_dx_rows(odp_stream_t stream, int dtype, int64_t n, int64
   return odp_check_launch("odp_xent_dx_rows");
 }
 
+// Slices of the tokens that the tiles of dW are split into: as many as the CUs
+// hold, of at least 32 steps.
+static int dw_split(int dtype, int64_t n, int64_t vc, int64_t width) {
+  const int64_t tiles = up(vc, tile_edge(dtype)) * up(width, tile_edge(dtype)), held = dtype == ODP_DTYPE_F32 ? 512 : 256;
+  const int64_t most = n / (32 * (dtype == ODP_DTYPE_F32 ? 16 : 32)), s = held / tiles < most ? held / tiles : most;
+  return (int)(s < 2 ? 1 : s);
+}
+
+extern "C" int64_t odp_xent_dw_scratch(int dtype, int64_t n, int64_t vc, int64_t width) {
+  if (n <= 0 || vc <= 0 || width <= 0) return 0;
+  const int split = dw_split(dtype, n, vc, width);
+  return split > 1 ? 4 * split * vc * width : 0;
+}
+
 extern "C" int odp_xent_dw(odp_stream_t stream, int dtype, const void* xc, int64_t n, int64_t width,
-                           const int32_t* count, int64_t vc, const void* dl, int64_t ldd, void* dw, int64_t lddw) {
+                           const int32_t* count, int64_t vc, const void* dl, int64_t ldd, void* scratch, void* dw,
+                           int64_t lddw) {
   if (int rc = check_xent("odp_xent_dw", dtype, n, width, lddw, vc)) return rc;
   if (ldd != odp_xent_pitch(dtype, vc) || ldd >= (int64_t)1 << 20 || count == nullptr || dw == nullptr || !on16(dw) ||
       (n > 0 && (xc == nullptr || dl == nullptr || !on16(xc) || !on16(dl)))) {
@@ -1007,7 +1093,27 @@ extern "C" int odp_xent_dw(odp_stream_t stream, int dtype, const void* xc, int64
     return ODP_ERR_INVALID_ARGUMENT;
   }
   const hipStream_t s = odp_hip_stream(stream);
+  const int split = lddw == width ? dw_split(dtype, n, vc, width) : 1;
   unsigned blocks;
+  if (split > 1) {
+    if (scratch == nullptr || !on16(scratch)) {
+      odp_set_error("odp_xent_dw: scratch is null or off the 16-byte grid");
+      return ODP_ERR_INVALID_ARGUMENT;
+    }
+    const int64_t tiles = up(vc, tile_edge(dtype)) * up(width, tile_edge(dtype)), quads = vc * width / 4;
+    const bool wide = split > 8;
+    blocks = (unsigned)up(tiles * split, 8) * 8;
+    const Xent p = xent_of(xc, nullptr, width, vc, width, n, count, nullptr, nullptr, 0.f);
+#define ODP_DW(D)                                                                                                    \
+  do {                                                                                                               \
+    ODP_XENT_GO((k_xent_dw_part<D>), (Tile<D, 0>::THREADS), blocks, p, vc, dl, ldd, split, (float*)scratch);          \
+    if (wide) ODP_XENT_GO((k_xent_dw_rows<D, 16>), 256, (unsigned)up(quads, 16), (const float*)scratch, split, quads, dw); \
+    else ODP_XENT_GO((k_xent_dw_rows<D, 1>), 256, (unsigned)up(quads, 256), (const float*)scratch, split, quads, dw); \
+  } while (0)
+    if (dtype == ODP_DTYPE_F32) ODP_DW(ODP_DTYPE_F32); else ODP_DW(ODP_DTYPE_BF16);
+#undef ODP_DW
+    return odp_check_launch("odp_xent_dw");
+  }
   if (int rc = grid_of("odp_xent_dw", dtype, false, up(vc, tile_edge(dtype)), up(width, tile_edge(dtype)), false, blocks)) return rc;
   const Xent p = xent_of(xc, nullptr, width, vc, width, n, count, nullptr, nullptr, 0.f);
   if (dtype == ODP_DTYPE_F32)

@@ -305,6 +305,12 @@ def _xent_words(dt: int, n: int, width: int, vocab: int) -> tuple[int, int]:
 
 
 @functools.lru_cache(maxsize=256)
+def _dw_words(dt: int, n: int, vc: int, width: int) -> int:
+    """float32 words that the slices of the tokens of a piece of dW take (0: not split)."""
+    return int(N.load().odp_xent_dw_scratch(dt, n, vc, width)) // 4
+
+
+@functools.lru_cache(maxsize=256)
 def _xent_pitch(dt: int, columns: int) -> int:
     return int(N.load().odp_xent_pitch(dt, columns))
 
@@ -368,8 +374,9 @@ class _Packed:
                 _call("odp_xent_dx", s, dt, self.n, self.width, self.count, w, ldw, self.vocab, v0, vc, piece,
                       d.data_ptr(), ldd, sums.data_ptr())
             if dw is not None:
+                slots = torch.empty(_dw_words(dt, self.n, vc, self.width), dtype=torch.float32, device=dev)
                 _call("odp_xent_dw", s, dt, xc, self.n, self.width, self.count, vc, d.data_ptr(), ldd,
-                      dw.data_ptr() + v0 * self.width * dw.element_size(), self.width)
+                      slots.data_ptr(), dw.data_ptr() + v0 * self.width * dw.element_size(), self.width)
         if dx is not None:
             _call("odp_xent_dx_rows", s, dt, self.n, self.cols, self.width, self.count, self.where, self.tgt, w,
                   ldw, piece, sums.data_ptr(), rest.data_ptr(), dx.data_ptr())

@@ -442,7 +442,8 @@ def test_in_a_graph(dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("n,width,vocab", [(1, 64, 1000), (5, 40, 3), (70, 96, 2050), (130, 72, 4097), (300, 40, 9000),
-                                           (600, 64, 257)])
+                                           (600, 64, 257), (70, 768, 2050), (130, 800, 4097), (300, 1000, 700),
+                                           (600, 776, 257)])
 @pytest.mark.parametrize("softcap", [None, 5.0])
 def test_kept_logits(n, width, vocab, softcap, dtype, monkeypatch):
     """The forward's logits, kept, give the bits that forming them again gives, in pieces too."""
@@ -460,7 +461,7 @@ def test_kept_logits(n, width, vocab, softcap, dtype, monkeypatch):
 
 def test_logits_are_kept_up_to_a_size_and_until_the_backward(monkeypatch):
     """KEEP_BYTES bounds what a call holds; without a gradient nothing is held, after the backward neither."""
-    n, width, vocab = 512, 64, 16384
+    n, width, vocab = 512, 1024, 16384
     x, w, y, _ = inputs(n, width, vocab, torch.bfloat16, seed=2)
     x, w, y = x.to(DEV).requires_grad_(), w.to(DEV), y.to(DEV)
     logits = 4 * n * vocab
@@ -493,3 +494,28 @@ def test_two_backward_passes_of_one_loss():
         assert torch.equal(a, b)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(loss, [x, w])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("n,width,vocab", [(2048, 40, 100), (4100, 264, 300), (20000, 24, 70)])
+def test_many_tokens_of_a_small_vocabulary(n, width, vocab, dtype, monkeypatch):
+    """dW's contraction over the tokens in slices."""
+    assert vocabulary._dw_words(vocabulary.dtype_code(dtype), n, vocab, width) > 0
+    x, w, y, gl = inputs(n, width, vocab, dtype, seed=n)
+    want, bound = reference(x, w, y, gl, None, dtype)
+    got = run(x, w, y, gl)
+    for a, b, c in zip(got, want, bound):
+        assert within(a, b, c)
+    for a, b in zip(got, run(x, w, y, gl)):
+        assert torch.equal(a, b)
+    monkeypatch.setattr(vocabulary, "PIECE_BYTES", 1)
+    for a, b, c in zip(run(x, w, y, gl), want, bound):
+        assert within(a, b, c)
+    monkeypatch.undo()
+    few = torch.full_like(y, -100)
+    few[n // 2] = vocab - 1
+    want, bound = reference(x, w, few, gl, None, dtype)
+    for a, b, c in zip(run(x, w, few, gl), want, bound):
+        assert within(a, b, c)
+    few[n // 2] = -100
+    assert not run(x, w, few, gl)[2].any()
