@@ -61,7 +61,7 @@ typedef enum odp_status {
 typedef enum odp_dtype {
   ODP_DTYPE_F32 = 0,
   ODP_DTYPE_BF16 = 1,
-  ODP_DTYPE_F16 = 2, /* noise, sqnorm, clip factors and scale-sum only */
+  ODP_DTYPE_F16 = 2, /* noise, sqnorm, clip factors, scale-sum and embeddings only */
   ODP_DTYPE_F64 = 3  /* noise, sqnorm, clip factors and scale-sum only */
 } odp_dtype;
 

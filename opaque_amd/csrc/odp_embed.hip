@@ -16,6 +16,10 @@
 // frequencies (half of a batch may be one padding token), every gradient row
 // is read once per pass, nothing is added atomically, and results do not
 // depend on the order of execution.
+//
+// 32768 tokens of a 128256 x 4096 bfloat16 table, lookup and gradient: 340 us
+// for 1.86 GB (5.5 TB/s; a copy runs at 5.2).  A clip step's norms and sum over
+// 16384 of them: 285 us for 1.19 GB, 1.05 GB of it the table's zeros.
 #include "odp_internal.h"
 
 namespace {
@@ -126,6 +130,8 @@ __device__ __forceinline__ int64_t token_at(const void* tokens, int wide, int64_
 // ---------------------------------------------------------------------------
 // Lookup.  A wave takes EM_ITEMS (row, 64 pieces of 16 bytes) items, their
 // loads in flight together; a token outside the table gives a row of NaN.
+// 32768 rows of 8 KB in 83 us (6.5 TB/s, a fifth of them one token's); 16
+// rows in 3.6 us, which is the launch.
 // ---------------------------------------------------------------------------
 constexpr int EM_ITEMS = 4;
 template <int DT, bool AL>
@@ -171,7 +177,10 @@ __global__ __launch_bounds__(64 * EM_WAVES) void k_embed_rows(const void* __rest
 // digit counts, summed exclusively over (digit, wave), are where its keys go,
 // and equal digits within 64 keys are ranked by ballots, so order among equal
 // tokens is kept.  Dropped positions (outside the table, padding, rows
-// outside every segment) get the key `vocab` and end up last.
+// outside every segment) get the key `vocab` and end up last.  Bound by latency,
+// not bytes: 16384 positions take two passes of 8 and 14 us, 1023 in one
+// workgroup 8 us.  The launches therefore zero the output table on the side:
+// with a table of 1.05 GB the two passes take 2 x (48 + 31) us, 6.6 TB/s of it.
 // ---------------------------------------------------------------------------
 constexpr int SORT_BITS = 9, SORT_BINS = 1 << SORT_BITS;
 constexpr int SORT_KEYS = 512;                            // positions a wave holds at a time
@@ -590,7 +599,9 @@ __device__ __forceinline__ void em_finish(const EmbedSum& a, int mode, uint32_t 
   }
 }
 
-// One wave per (window, 64 pieces of 16 bytes of the rows).
+// One wave per (window, 64 pieces of 16 bytes of the rows).  0.27 GB of gradient
+// rows (32768 of 8 KB) read and their tokens' sums written in 86 us; the two
+// passes of a clip step over 16384 rows 36 and 37 us.
 template <int DT, bool AL, int MODE>
 __global__ __launch_bounds__(64 * EM_WAVES) void k_embed_sum(EmbedSum a) {
   constexpr int V = em_vec<DT>(), ES = DT == ODP_DTYPE_F32 ? 4 : 2;
@@ -726,7 +737,8 @@ __global__ __launch_bounds__(64 * EM_WAVES) void k_embed_group(EmbedSum a) {
 }
 
 // Adds the partials of a run that begins in a window and crosses into the
-// next ones, one wave per (window, 64 pieces).
+// next ones, one wave per (window, 64 pieces).  4 us where none is long, 7-12
+// for runs of thousands.
 template <int DT, bool AL, int MODE>
 __global__ __launch_bounds__(64 * EM_WAVES) void k_embed_join(EmbedSum a) {
   constexpr int V = em_vec<DT>();
@@ -785,7 +797,7 @@ ZeroShare zero_share(void* at, int64_t bytes, int threads, int64_t k, int64_t l,
   const int64_t size = (int64_t)threads * 16, pieces = (z.bytes + size - 1) / size;
   z.first = pieces * k / n;
   z.count = pieces * l / n - z.first;
-  z.per = (int)(1 + z.count / ((int64_t)1 << 22));
+  z.per = (int)(1 + z.count / ((int64_t)1 << 21));  // a grid of fewer than 2^32 threads
   blocks = (unsigned)((z.count + z.per - 1) / z.per);
   return z;
 }

@@ -192,9 +192,9 @@ struct Packed {
   int64_t kept_pitch() const { return abi.xent_pitch(dt, vocab); }
 };
 
-// keep_bytes: up to which the logits are kept for a backward pass.
-Packed xent_forward(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target, double softcap,
-                    int64_t ignore, int64_t keep_bytes) {
+// The log-sum-exp goes to lse_out.  keep_bytes: up to which the logits are kept for a backward pass.
+Packed xent_forward(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target,
+                    const at::Tensor& lse_out, double softcap, int64_t ignore, int64_t keep_bytes) {
   Packed p;
   p.w = head_rows(weight);
   const at::Tensor rows = pitched(x), y = target.contiguous();
@@ -207,7 +207,7 @@ Packed xent_forward(const at::Tensor& x, const at::Tensor& weight, const at::Ten
   p.xc = at::empty({room, p.width}, rows.options());
   p.ids = at::empty({3 * room + 2}, rows.options().dtype(at::kInt));
   p.losses = at::empty(target.sizes(), rows.options().dtype(at::kFloat));
-  p.lse = at::empty({p.n}, p.losses.options());
+  p.lse = lse_out;
   float* losses = (float*)p.losses.data_ptr();
   float* lse = (float*)p.lse.data_ptr();
   const odp_stream_t s = stream_of(rows);
@@ -236,10 +236,10 @@ at::Tensor xent_result(const Packed& p, int64_t reduction) {
 
 struct Xent : torch::autograd::Function<Xent> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight,
-                            const at::Tensor& target, double softcap, int64_t ignore, int64_t reduction,
-                            int64_t piece_bytes, int64_t keep_bytes) {
+                            const at::Tensor& target, const at::Tensor& lse, double softcap, int64_t ignore,
+                            int64_t reduction, int64_t piece_bytes, int64_t keep_bytes) {
     const c10::OptionalDeviceGuard guard(x.device());
-    const Packed p = xent_forward(x, weight, target, softcap, ignore, keep_bytes);
+    const Packed p = xent_forward(x, weight, target, lse, softcap, ignore, keep_bytes);
     // A later change of the head in place is an error; the kept logits go when the backward pass is through.
     ctx->save_for_backward({weight, p.logits});
     auto& d = ctx->saved_data;
@@ -258,7 +258,7 @@ struct Xent : torch::autograd::Function<Xent> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
     at::Tensor dx, dw;
-    if (!grads[0].defined()) return {{}, {}, {}, {}, {}, {}, {}, {}};
+    if (!grads[0].defined()) return {{}, {}, {}, {}, {}, {}, {}, {}, {}};
     const torch::autograd::variable_list saved = ctx->get_saved_variables();
     {
       at::NoGradGuard no_grad;
@@ -318,17 +318,35 @@ struct Xent : torch::autograd::Function<Xent> {
               "odp_xent_dx_rows");
       if (need_w && p.cols != p.width) dw = dw.narrow(1, 0, p.cols).contiguous();
     }
-    return {first_only(grads[0], dx), first_only(grads[0], dw), {}, {}, {}, {}, {}, {}};
+    return {first_only(grads[0], dx), first_only(grads[0], dw), {}, {}, {}, {}, {}, {}, {}};
   }
 };
+
+at::Tensor xent(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target, const at::Tensor& lse,
+                double softcap, int64_t ignore, int64_t reduction, int64_t piece_bytes, int64_t keep_bytes) {
+  if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad()))
+    return Xent::apply(x, weight, target, lse, softcap, ignore, reduction, piece_bytes, keep_bytes);
+  const c10::OptionalDeviceGuard guard(x.device());
+  return xent_result(xent_forward(x, weight, target, lse, softcap, ignore, 0), reduction);
+}
+
+at::Tensor lse_of(const at::Tensor& x, const at::Tensor& target) {
+  return at::empty(target.sizes(), x.options().dtype(at::kFloat).requires_grad(false));
+}
 
 at::Tensor cross_entropy(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target, double softcap,
                          int64_t ignore, int64_t reduction, int64_t piece_bytes, int64_t keep_bytes) {
   py::gil_scoped_release nogil;
-  if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad()))
-    return Xent::apply(x, weight, target, softcap, ignore, reduction, piece_bytes, keep_bytes);
-  const c10::OptionalDeviceGuard guard(x.device());
-  return xent_result(xent_forward(x, weight, target, softcap, ignore, 0), reduction);
+  return xent(x, weight, target, lse_of(x, target), softcap, ignore, reduction, piece_bytes, keep_bytes);
+}
+
+// The token losses and their log-sum-exp, which has no gradient.
+std::pair<at::Tensor, at::Tensor> token_losses(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target,
+                                               double softcap, int64_t ignore, int64_t piece_bytes,
+                                               int64_t keep_bytes) {
+  py::gil_scoped_release nogil;
+  const at::Tensor lse = lse_of(x, target);
+  return {xent(x, weight, target, lse, softcap, ignore, 0, piece_bytes, keep_bytes), lse};
 }
 
 }  // namespace
@@ -338,4 +356,6 @@ void add_vocabulary(py::module_& m) {
   m.def("embedding", &embedding, py::arg("tokens"), py::arg("weight"), py::arg("scale"), py::arg("padding"));
   m.def("cross_entropy", &cross_entropy, py::arg("x"), py::arg("weight"), py::arg("target"), py::arg("softcap"),
         py::arg("ignore"), py::arg("reduction"), py::arg("piece_bytes"), py::arg("keep_bytes"));
+  m.def("token_losses", &token_losses, py::arg("x"), py::arg("weight"), py::arg("target"), py::arg("softcap"),
+        py::arg("ignore"), py::arg("piece_bytes"), py::arg("keep_bytes"));
 }

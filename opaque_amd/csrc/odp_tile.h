@@ -11,6 +11,13 @@
 // rows of memory).  A step covers 64 bytes of k; both orders then stage the
 // same bytes, 64-byte rows of k or rows of o or n, by buffer loads straight
 // into a ring of LDS stages, all but one step ahead of the MFMAs.
+//
+// 256 x 256 of bfloat16 keeps 128 registers of sums a lane and reads each
+// staged byte for 8 MFMAs a wave; a CU then holds one workgroup of 8 waves, and
+// what hides latency is the ring (4 stages of 32 KB).  Measured on the loss's
+// products: 1240 TFLOP/s with rows of k for both operands, 1360 with one and
+// 1300 with both K-major (the vendor library 1421, 1373 and 1102 on the same
+// shapes).  float32 has no wider MFMA than 16 x 16 x 4: 119, 114 (library 114, 72).
 #pragma once
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));

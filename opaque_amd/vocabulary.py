@@ -276,7 +276,10 @@ _HEAD_DTYPES = (torch.float32, torch.bfloat16)
 # Bytes of d (the logits' gradient, in the inputs' type) that the backward
 # holds at a time: a piece of the vocabulary for all tokens.
 PIECE_BYTES = 512 << 20
-# Bytes up to which the forward keeps the float32 logits for the backward.
+# Bytes of float32 logits up to which a call that wants gradients keeps them
+# for its backward (1.5 % of the memory of one GPU) where that is faster than
+# forming them again; 0 keeps none.  Neither do the gradients of torch.func
+# (``vmap(grad)``) and of a head that trains under ``clipped_grad``.
 KEEP_BYTES = 4 << 30
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
@@ -466,6 +469,9 @@ class _Xent(torch.autograd.Function):
             return (torch.stack([o[0] for o in out]), torch.stack([o[1] for o in out])), (0, 0)
         sess = active_session()
         if sess is None or sess.mode != "capture" or id(weight) not in sess.eligible:
+            host = None if _transformed() else _bound()
+            if host is not None:
+                return host.token_losses(x, weight, target, softcap, ignore, PIECE_BYTES, KEEP_BYTES), (0, 0)
             return _Xent.apply(x, weight, target, softcap, ignore), (0, 0)
         rec = SiteRecord(x=x, A=None, B=None, scaling=1.0, a_obj=None, b_obj=None, a_transposed=False,
                          b_transposed=False, w_obj=weight)
@@ -501,7 +507,7 @@ class _TapXent(torch.autograd.Function):
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *,
                          softcap: float | None = None, ignore_index: int = -100,
                          reduction: str = "mean") -> torch.Tensor:
-    """Cross entropy of ``x weight^T`` against ``target``, without the [tokens, vocabulary] logits.
+    """Cross entropy of ``x weight^T`` against ``target``, a piece of the vocabulary at a time.
 
     ``x`` [..., width] and ``weight`` [vocabulary, width] are both float32 or
     both bfloat16, ``target`` [...] int64 or int32.  ``softcap`` bounds the
@@ -510,7 +516,9 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     mean over the tokens whose target is not ``ignore_index`` (NaN when there
     is none, as torch's).  A target outside the vocabulary gives NaN.  Logits
     and statistics are float32; the gradients are summed in float32 and
-    rounded once, from logit gradients in the inputs' type.
+    rounded once, from logit gradients in the inputs' type.  No [tokens,
+    vocabulary] tensor is made beyond a piece of PIECE_BYTES in the backward
+    and, where they take at most KEEP_BYTES, the logits between the passes.
 
     Replaces the reference's linear cross entropy
     (opaque-patches/.../kernels/linear_cross_entropy.py:249).  Inside

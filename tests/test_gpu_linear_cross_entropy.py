@@ -519,3 +519,38 @@ def test_many_tokens_of_a_small_vocabulary(n, width, vocab, dtype, monkeypatch):
         assert within(a, b, c)
     few[n // 2] = -100
     assert not run(x, w, few, gl)[2].any()
+
+
+def test_frozen_head_under_clipped_grad_with_and_without_kept_logits(monkeypatch):
+    g = torch.Generator().manual_seed(7)
+    width, vocab, n, T = 136, 700, 4, 8
+    w = (torch.randn(vocab, width, generator=g) / 4).to(DEV)
+    mid = {"mid": (torch.randn(width, width, generator=g) / 8).to(DEV)}
+    x, t = torch.randn(n, T, width, generator=g).to(DEV), torch.randint(0, vocab, (n, T), generator=g).to(DEV)
+
+    def step():
+        f, st = clipped_grad(lambda p, xi, ti: linear_cross_entropy(torch.tanh(xi @ p["mid"].t()), w, ti),
+                             clipping_norm=0.1, normalize_by=float(n), batch_argnums=(1, 2), return_aux=True)
+        (got, aux), _ = f(mid, x, t, state=st)
+        return got.pytree["mid"], aux.grad_norms
+
+    kept = step()
+    monkeypatch.setattr(vocabulary, "KEEP_BYTES", 0)
+    for a, b in zip(kept, step()):
+        assert torch.equal(a, b)
+    ref, raux = dp_ref.clipped_grad(lambda p, xi, ti: plain_loss(torch.tanh(xi @ p["mid"].t()), w.cpu(), ti),
+                                    {"mid": mid["mid"].cpu()}, (x.cpu(), t.cpu()), clipping_norm=0.1,
+                                    normalize_by=float(n))
+    assert float((kept[0].double().cpu() - ref["mid"].double()).norm() / ref["mid"].double().norm()) < 1e-5
+    assert float(((kept[1].double().cpu() - raux["norms"].double()) / raux["norms"].double()).abs().max()) < 1e-5
+
+
+@pytest.mark.parametrize("outside", [False, True])
+def test_gradients_under_vmap(outside):
+    """vmap(grad), of inputs that want a gradient outside it too."""
+    x, w, y, _ = inputs(12, 136, 300, torch.float32, seed=3, ignored=0.0)
+    x, y = x.reshape(3, 4, 136), y.reshape(3, 4)
+    xd, wd, yd = x.to(DEV).requires_grad_(outside), w.to(DEV), y.to(DEV)
+    got = torch.func.vmap(torch.func.grad(lambda a, b: linear_cross_entropy(a, wd, b, reduction="sum")))(xd, yd)
+    want, bound = reference(x.reshape(12, 136), w, y.reshape(12), torch.ones(12), None, torch.float32)
+    assert within(got.detach().reshape(12, 136), want[1], bound[1])
