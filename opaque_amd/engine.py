@@ -8,8 +8,12 @@ on the current HIP stream:
     odp_seg_factor_stream_tables / odp_seg_factor
                     per-example dA, dB and their squared-norm partials
     odp_sqnorm      squared norms of materialised per-example leaves
+    odp_token_sort, odp_embed_sqnorm
+                    an embedding table's per-example norms, from its tokens
     odp_clip_factors  per-example norms -> clip / AUTO-S scales
     odp_scale_sum   clipped sum, cast and normalize_by, into one flat buffer
+    odp_embed_clipped_sum
+                    the embedding tables' clipped sums
 
 LoRA adapters that read the same activation tensor (q/k/v, gate/up) share
 one pass over it: their ranks are laid side by side (up to 4 leaves and 64
