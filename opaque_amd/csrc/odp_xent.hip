@@ -918,7 +918,8 @@ extern "C" int64_t odp_xent_stats_scratch(int dtype, int64_t n, int64_t vocab) {
 
 extern "C" int64_t odp_xent_kept(int dtype, int64_t n, int64_t width, int64_t vocab) {
   if (n <= 0 || width <= 0 || vocab <= 0 || !keeps(dtype, n, width)) return 0;
-  return 4 * n * odp_xent_pitch(dtype, vocab);
+  const int64_t row = 4 * odp_xent_pitch(dtype, vocab);
+  return n <= ((int64_t)1 << 60) / row ? n * row : 0;
 }
 
 extern "C" int odp_xent_losses(odp_stream_t stream, int dtype, const void* xc, int64_t n, int64_t width,
