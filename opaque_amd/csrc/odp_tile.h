@@ -5,7 +5,8 @@
 // owns an OT x NT tile of C: rows o from A, columns n from B.  256 x 256 in
 // bfloat16 and 128 x 128 in float32; with S == 1, for few rows, 64 x 128 and a ring
 // of more, smaller stages, since such a product waits for B's memory; with S
-// == 2 (bfloat16) 128 x 256.  An operand is K-contiguous (KC: element
+// == 2 (bfloat16) 128 x 256; with S == 3 (float32, whose MFMAs would take longer
+// than that memory for 64 rows) 32 x 128.  An operand is K-contiguous (KC: element
 // (row, k) at row * ld + k, as the rows of activations or of a weight) or
 // K-major (element (row, k) at k * ld + row: the contraction runs over the
 // rows of memory).  A step covers 64 bytes of k; both orders then stage the
@@ -36,19 +37,23 @@ template <int DT, int S>
 struct Tile {
   static constexpr bool F32 = DT == ODP_DTYPE_F32;
   static constexpr int ES = F32 ? 4 : 2;          // bytes per element
-  static constexpr int OT = S == 1 ? 64 : S == 2 ? 128 : 512 / ES;  // rows (o) of the tile
-  static constexpr int NT = S == 1 ? 128 : 512 / ES;                // columns (n)
+  static constexpr bool FEW = S == 1 || S == 3;
+  static constexpr int OT = S == 1 ? 64 : S == 2 ? 128 : S == 3 ? 32 : 512 / ES;  // rows (o) of the tile
+  static constexpr int NT = FEW ? 128 : 512 / ES;                                 // columns (n)
   static constexpr int EK = 64 / ES;              // k per step
-  static constexpr int WAVES = NT / 64 * 2;       // 2 x (WAVES / 2) over the tile
-  static constexpr int THREADS = 64 * WAVES;
-  static constexpr int WM = OT / 2, WN = 64;      // a wave's block
+  static constexpr int WR = S == 3 ? 1 : 2;       // waves over the rows
+  static constexpr int WM = OT / WR, WN = 64;     // a wave's block
+  static constexpr int WC = NT / WN, WAVES = WC * WR, THREADS = 64 * WAVES;
   static constexpr int BI = WM / 16, BJ = WN / 16;
   static constexpr int ABYTES = OT * 64, BBYTES = NT * 64, STAGE = ABYTES + BBYTES;  // of a step
   static constexpr int ALOADS = ABYTES / 1024 / WAVES, BLOADS = BBYTES / 1024 / WAVES;  // 1 KB loads per wave
   static constexpr int LOADS = ALOADS + BLOADS;
-  static constexpr int RING = S == 1 ? 6 : 4;
+  static constexpr int RING = FEW ? 6 : 4;
   static_assert(ALOADS * WAVES * 1024 == ABYTES && BLOADS * WAVES * 1024 == BBYTES, "whole loads");
   typedef f32x4_t Acc[BI][BJ];
+  // First row and column of a wave's block.
+  static __device__ __forceinline__ int wm(int wave) { return WM * (wave % WR); }
+  static __device__ __forceinline__ int wn(int wave) { return WN * (wave / WR); }
 };
 
 // Stage k of the ring: separate arrays, so that reads of one are not made to
@@ -61,7 +66,7 @@ __device__ __forceinline__ char* t_array() {
 template <int DT, int S>
 __device__ __forceinline__ char* t_stage(int k) {
   constexpr int B = Tile<DT, S>::STAGE;
-  if constexpr (S != 1)
+  if constexpr (Tile<DT, S>::RING == 4)
     return k == 0 ? t_array<B, 0>() : k == 1 ? t_array<B, 1>() : k == 2 ? t_array<B, 2>() : t_array<B, 3>();
   else
     return k == 0   ? t_array<B, 0>()
@@ -203,7 +208,7 @@ struct Head {
 template <int DT, int S, bool AKC, bool BKC>
 __device__ __forceinline__ void t_head(const char* st, Head<DT, S>& h) {
   using T = Tile<DT, S>;
-  const int wave = threadIdx.x >> 6, wm = T::WM * (wave & 1), wn = T::WN * (wave >> 1);
+  const int wave = threadIdx.x >> 6, wm = T::wm(wave), wn = T::wn(wave);
 #pragma unroll
   for (int j = 0; j < T::BJ; ++j) h.b[j] = t_frag<DT, BKC, T::NT>(st + T::ABYTES, wn + 16 * j);
   h.a[0] = t_frag<DT, AKC, T::OT>(st, wm);
@@ -219,7 +224,7 @@ __device__ __forceinline__ void t_step(char* __restrict__ nxt, const char* __res
                                        const char* __restrict__ ahead, Issue issue, Head<DT, S>& h, Head<DT, S>& n,
                                        typename Tile<DT, S>::Acc& acc) {
   using T = Tile<DT, S>;
-  const int wave = threadIdx.x >> 6, wm = T::WM * (wave & 1), wn = T::WN * (wave >> 1);
+  const int wave = threadIdx.x >> 6, wm = T::wm(wave), wn = T::wn(wave);
   // Block rows beside which the next step's b is read: the last but one of as
   // many as it takes, or all.
   constexpr int ROWS = T::BJ < T::BI ? T::BJ : T::BI, R0 = T::BJ < T::BI ? T::BI - 1 - T::BJ : 0;

@@ -235,7 +235,7 @@ __device__ __forceinline__ void stats_tile(const Xent& p, const typename Tile<DT
                                            float* __restrict__ ztgt, float* __restrict__ logits, int64_t ldl) {
   using T = Tile<DT, S>;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wm = T::WM * (wave & 1), wn = T::WN * (wave >> 1);
+  const int wm = T::wm(wave), wn = T::wn(wave);
   // Columns of this lane are c0 + 16 j + e of the tile; `edge` columns of it exist.
   const int c0 = wn + t_col(0), edge = (int)min((int64_t)T::NT, p.vocab - n0);
   static_for<T::BI>([&](auto ii) __attribute__((always_inline)) {
@@ -277,7 +277,7 @@ __device__ __forceinline__ void stats_tile(const Xent& p, const typename Tile<DT
       m = mm;
     }
     if (lane < 16) {
-      float* r = red + 2 * ((wave >> 1) * T::OT + wm + t_row(i));
+      float* r = red + 2 * (wave / T::WR * T::OT + wm + t_row(i));
       r[0] = m;
       r[1] = s;
     }
@@ -291,10 +291,10 @@ __global__ __launch_bounds__((Tile<DT, S>::THREADS), 2) void k_xent_stats(Xent p
                                                                      float* __restrict__ ztgt,
                                                                      float* __restrict__ logits, int64_t ldl) {
   using T = Tile<DT, S>;
-  __shared__ float red[T::WAVES / 2 * T::OT * 2];  // [waves across n][rows][maximum, sum]
+  __shared__ float red[T::WC * T::OT * 2];  // [waves across n][rows][maximum, sum]
   const int cnt = *(const ODP_CONST int32_t*)p.count;
   Walk walk((cnt + T::OT - 1) / T::OT, (int)((p.vocab + T::NT - 1) / T::NT));
-  const int wm = T::WM * ((threadIdx.x >> 6) & 1);
+  const int wm = T::wm(threadIdx.x >> 6);
   Product<DT, S, true, true> prod;
   int ti, tj;
   auto begin = [&]() {
@@ -321,10 +321,10 @@ __global__ __launch_bounds__((Tile<DT, S>::THREADS), 2) void k_xent_stats(Xent p
       if (o0 + r >= cnt) break;
       float m = -INFINITY, s = 0.f;
 #pragma unroll
-      for (int w = 0; w < T::WAVES / 2; ++w) m = fmaxf(m, red[2 * (w * T::OT + r)]);
+      for (int w = 0; w < T::WC; ++w) m = fmaxf(m, red[2 * (w * T::OT + r)]);
       const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-      for (int w = 0; w < T::WAVES / 2; ++w)
+      for (int w = 0; w < T::WC; ++w)
         s += red[2 * (w * T::OT + r) + 1] * fast_exp(red[2 * (w * T::OT + r)] - ref);
       pmax[(int64_t)column * p.n + o0 + r] = m;
       psum[(int64_t)column * p.n + o0 + r] = s;
@@ -407,7 +407,7 @@ __device__ __forceinline__ void t_store(void* out, int64_t ld, int64_t o0, int64
                                         Val val) {
   using T = Tile<DT, S>;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wm = T::WM * (wave & 1), wn = T::WN * (wave >> 1);
+  const int wm = T::wm(wave), wn = T::wn(wave);
   if constexpr (DT == ODP_DTYPE_F32) {
     static_for<T::BI * T::BJ>([&](auto q) __attribute__((always_inline)) {
       constexpr int i = decltype(q)::value / T::BJ, j = decltype(q)::value % T::BJ;
@@ -458,7 +458,7 @@ __device__ __forceinline__ void dlogits_tile(const Xent& p, const typename Tile<
                                              int cnt, int64_t o0, int64_t n0, int64_t vc, void* dl, int64_t ldd,
                                              float* __restrict__ rest) {
   using T = Tile<DT, S>;
-  const int wm = T::WM * ((threadIdx.x >> 6) & 1), wn = T::WN * (threadIdx.x >> 7);
+  const int wm = T::wm(threadIdx.x >> 6), wn = T::wn(threadIdx.x >> 6);
   // Columns of this lane are c0 + 16 j + e of the tile; `edge` columns of it exist.
   const int c0 = wn + t_col(0), edge = (int)min((int64_t)T::NT, vc - n0);
   const float inv_cap = 0.5f * p.inv_cap2;
@@ -498,7 +498,7 @@ __global__ __launch_bounds__((Tile<DT, S>::THREADS), (DT == ODP_DTYPE_BF16 && S 
   using T = Tile<DT, S>;
   const int cnt = *(const ODP_CONST int32_t*)p.count;
   Walk walk((cnt + T::OT - 1) / T::OT, (int)(ldd / T::NT));
-  const int wm = T::WM * ((threadIdx.x >> 6) & 1);
+  const int wm = T::wm(threadIdx.x >> 6);
   const void* w = (const char*)p.w + v0 * p.ldw * T::ES;
   const float part = over != nullptr ? *over : 1.f;
   Product<DT, S, true, true> prod;
@@ -586,11 +586,15 @@ __global__ __launch_bounds__(256) void k_xent_dkept(Xent p, const float* __restr
 }
 
 // How many slices of the contraction each tile of dx is split into: the
-// fewest of 1 .. 16 with which the workgroups fill the 256 CUs' rounds best,
-// as far as the slots (`cap` tiles) and slices of 16 steps go.
+// fewest of 1 .. DX_SPLIT with which the workgroups fill the 256 CUs' rounds
+// best, as far as the slots (`cap` tiles) and slices of 16 steps go.  dx, us, in
+// up to 16, 32 and 64 slices: bfloat16, 128 tokens, 128256 x 512 139, 78 and 48,
+// 32000 x 2048 44, 31 and 43; 777 tokens, 32000 x 2048 103, 102 and 101; float32,
+// one token, 50257 x 768 103, 56 and 48 (64 slices cost dx_rows 4 us more).
+constexpr int DX_SPLIT = 32;
 __host__ __device__ inline int dx_split(int tiles, int cap, int64_t steps) {
   int best = 1, rounds = (tiles + 255) / 256;
-  for (int s = 2; s <= 16 && s * tiles <= cap && steps >= 16 * s; ++s) {
+  for (int s = 2; s <= DX_SPLIT && s * tiles <= cap && steps >= 16 * s; ++s) {
     const int r = (s * tiles + 255) / 256;
     if (r * best < rounds * s) best = s, rounds = r;
   }
@@ -625,7 +629,7 @@ __global__ __launch_bounds__((Tile<DT, S>::THREADS), 2) void k_xent_dx(Xent p, i
              Operand{(const char*)p.w + (v0 + k0) * p.ldw * T::ES, p.ldw, n0, p.width}, kn);
   prod.run(acc);
   const int wave = threadIdx.x >> 6;
-  const int wm = T::WM * (wave & 1), wn = T::WN * (wave >> 1);
+  const int wm = T::wm(wave), wn = T::wn(wave);
   float* out = slots + (int64_t)s * cnt * p.width;
   static_for<T::BI * T::BJ>([&](auto q) __attribute__((always_inline)) {
     constexpr int i = decltype(q)::value / T::BJ, j = decltype(q)::value % T::BJ;
@@ -659,6 +663,7 @@ __global__ __launch_bounds__(256) void k_xent_dx_rows(const float* __restrict__ 
     const int split = dx_split((cnt + ot - 1) / ot * tn, cap, steps);
     const float* at = slots + (int64_t)k * width + c;
     v = *(const f32x4_t*)at;
+#pragma unroll 4
     for (int s = 1; s < split; ++s) v = v + *(const f32x4_t*)(at + (int64_t)s * cnt * width);
     if (DT == ODP_DTYPE_BF16 && tgt[k] >= 0) {
       const u32x2_t h = *(const u32x2_t*)(w + 2 * (tgt[k] * ldw + c));
@@ -731,7 +736,7 @@ __global__ __launch_bounds__((Tile<DT, 0>::THREADS), 2) void k_xent_dw_part(Xent
              Operand{(const char*)p.xc + k0 * p.width * T::ES, p.width, n0, p.width}, (int32_t)min(per, cnt - k0));
   prod.run(acc);
   const int wave = threadIdx.x >> 6;
-  const int wm = T::WM * (wave & 1), wn = T::WN * (wave >> 1);
+  const int wm = T::wm(wave), wn = T::wn(wave);
   float* out = slots + s * vc * p.width;
   static_for<T::BI * T::BJ>([&](auto q) __attribute__((always_inline)) {
     constexpr int i = decltype(q)::value / T::BJ, j = decltype(q)::value % T::BJ;
@@ -782,8 +787,8 @@ int check_xent(const char* what, int dtype, int64_t n, int64_t width, int64_t ld
 
 // Columns a piece of d is padded to, and the edges of the tiles of a kind (Tile's S).
 int tile_edge(int dtype) { return dtype == ODP_DTYPE_F32 ? 128 : 256; }
-int tile_rows(int dtype, int kind) { return kind == 1 ? 64 : kind == 2 ? 128 : tile_edge(dtype); }
-int tile_cols(int dtype, int kind) { return kind == 1 ? 128 : tile_edge(dtype); }
+int tile_rows(int dtype, int kind) { return kind == 1 ? 64 : kind == 2 ? 128 : kind == 3 ? 32 : tile_edge(dtype); }
+int tile_cols(int dtype, int kind) { return kind == 1 || kind == 3 ? 128 : tile_edge(dtype); }
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -794,6 +799,10 @@ int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // x 768, 64 tokens 242 and 420, 256 598 and 643, 384 791 and 738.
 bool few_rows(int dtype, int64_t n) { return n <= (dtype == ODP_DTYPE_F32 ? 256 : 64); }
 
+// The tiles of few rows of n, else the large ones.  float32, 50257 x 768,
+// 16 tokens: 42 us with tiles of 32 rows, 61 with 64.
+int few_kind(int dtype, int64_t n) { return !few_rows(dtype, n) ? 0 : dtype == ODP_DTYPE_F32 && n <= 32 ? 3 : 1; }
+
 // The tiles (Tile's S) of a product of n rows and `cols` columns.  A tile of
 // 128 rows takes about 0.7 of the time of one of 256: bfloat16 takes those
 // where that leaves fewer of the larger ones' times, counting whole rounds of
@@ -801,7 +810,7 @@ bool few_rows(int dtype, int64_t n) { return n <= (dtype == ODP_DTYPE_F32 ? 256 
 // tokens 134 and 163, 256 151 and 172, 512 233 and 210; 128256 x 4096, 128
 // tokens 648 and 707, 160 820 and 732; 50257 x 768, 600 tokens 231 and 248.
 int tile_kind(int dtype, int64_t n, int64_t cols) {
-  if (few_rows(dtype, n)) return 1;
+  if (few_rows(dtype, n)) return few_kind(dtype, n);
   if (dtype == ODP_DTYPE_F32) return 0;
   const int64_t tn = up(cols, 256);
   return up(up(n, 128) * tn, 256) * 7 < up(up(n, 256) * tn, 256) * 10 ? 2 : 0;
@@ -840,16 +849,17 @@ bool on16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 #define ODP_XENT_GO(KERNEL, THREADS, GRID, ...) \
   hipLaunchKernelGGL(KERNEL, dim3(GRID), dim3(THREADS), 0, s, __VA_ARGS__)
-// K<dtype, few rows>
-#define ODP_XENT_LAUNCH(K, GRID, ...)                                                              \
-  do {                                                                                             \
-    constexpr int F = ODP_DTYPE_F32, B = ODP_DTYPE_BF16;                                           \
-    if (dtype == F && few) ODP_XENT_GO((K<F, 1>), (Tile<F, 1>::THREADS), GRID, __VA_ARGS__);       \
-    else if (dtype == F) ODP_XENT_GO((K<F, 0>), (Tile<F, 0>::THREADS), GRID, __VA_ARGS__);         \
-    else if (few) ODP_XENT_GO((K<B, 1>), (Tile<B, 1>::THREADS), GRID, __VA_ARGS__);                \
-    else ODP_XENT_GO((K<B, 0>), (Tile<B, 0>::THREADS), GRID, __VA_ARGS__);                         \
+// K<dtype, tiles>
+#define ODP_XENT_LAUNCH(K, GRID, ...)                                                                \
+  do {                                                                                               \
+    constexpr int F = ODP_DTYPE_F32, B = ODP_DTYPE_BF16;                                             \
+    if (dtype == F && kind == 3) ODP_XENT_GO((K<F, 3>), (Tile<F, 3>::THREADS), GRID, __VA_ARGS__);   \
+    else if (dtype == F && kind == 1) ODP_XENT_GO((K<F, 1>), (Tile<F, 1>::THREADS), GRID, __VA_ARGS__); \
+    else if (dtype == F) ODP_XENT_GO((K<F, 0>), (Tile<F, 0>::THREADS), GRID, __VA_ARGS__);           \
+    else if (kind == 1) ODP_XENT_GO((K<B, 1>), (Tile<B, 1>::THREADS), GRID, __VA_ARGS__);            \
+    else ODP_XENT_GO((K<B, 0>), (Tile<B, 0>::THREADS), GRID, __VA_ARGS__);                           \
   } while (0)
-// K<dtype, few rows, softcap>
+// K<dtype, tiles, softcap>
 #define ODP_XENT_CAP(K, D, S, GRID, ...)                                                           \
   do {                                                                                             \
     if (softcap != 0.f) ODP_XENT_GO((K<D, S, true>), (Tile<D, S>::THREADS), GRID, __VA_ARGS__);    \
@@ -858,7 +868,8 @@ bool on16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 #define ODP_XENT_LAUNCH_CAP(K, GRID, ...)                                                          \
   do {                                                                                             \
     constexpr int F = ODP_DTYPE_F32, B = ODP_DTYPE_BF16;                                           \
-    if (dtype == F && kind == 1) ODP_XENT_CAP(K, F, 1, GRID, __VA_ARGS__);                         \
+    if (dtype == F && kind == 3) ODP_XENT_CAP(K, F, 3, GRID, __VA_ARGS__);                         \
+    else if (dtype == F && kind == 1) ODP_XENT_CAP(K, F, 1, GRID, __VA_ARGS__);                    \
     else if (dtype == F) ODP_XENT_CAP(K, F, 0, GRID, __VA_ARGS__);                                 \
     else if (kind == 1) ODP_XENT_CAP(K, B, 1, GRID, __VA_ARGS__);                                  \
     else if (kind == 2) ODP_XENT_CAP(K, B, 2, GRID, __VA_ARGS__);                                  \
@@ -948,7 +959,7 @@ extern "C" int odp_xent_losses(odp_stream_t stream, int dtype, const void* xc, i
   float* psum = pmax + n * tn;
   float* ztgt = psum + n * tn;
   ODP_XENT_LAUNCH_CAP(k_xent_stats, blocks, p, pmax, psum, ztgt, logits, ldl);
-  if (kind == 1)
+  if (kind == 1 || kind == 3)
     hipLaunchKernelGGL(k_xent_losses<1>, dim3((unsigned)n), dim3(256), 0, s, pmax, psum, ztgt, (int)tn, n, count, act,
                        tgt, losses, lse);
   else
@@ -1020,19 +1031,20 @@ extern "C" int odp_xent_dlogits(odp_stream_t stream, int dtype, const void* xc, 
 }
 
 // Tiles of n rows of dx, and those that the slots hold: as many, or a few times that to split.
-static int64_t dx_tiles(int dtype, int64_t n, int64_t width, bool few) {
-  return up(n, tile_rows(dtype, few)) * up(width, tile_cols(dtype, few));
+static int64_t dx_tiles(int dtype, int64_t n, int64_t width) {
+  const int kind = few_kind(dtype, n);
+  return up(n, tile_rows(dtype, kind)) * up(width, tile_cols(dtype, kind));
 }
 static int dx_cap(int dtype, int64_t n, int64_t width) {
-  const int64_t tiles = dx_tiles(dtype, n, width, few_rows(dtype, n));
-  const int64_t most = tiles * 16 < 512 ? tiles * 16 : 512;
+  const int64_t tiles = dx_tiles(dtype, n, width);
+  const int64_t most = tiles * DX_SPLIT < 512 ? tiles * DX_SPLIT : 512;
   return (int)(tiles > most ? tiles : most);
 }
 
 extern "C" int64_t odp_xent_dx_scratch(int dtype, int64_t n, int64_t width) {
   if (n <= 0 || width <= 0) return 0;
-  const bool few = few_rows(dtype, n);
-  return 4 * (int64_t)dx_cap(dtype, n, width) * tile_rows(dtype, few) * tile_cols(dtype, few);
+  const int kind = few_kind(dtype, n);
+  return 4 * (int64_t)dx_cap(dtype, n, width) * tile_rows(dtype, kind) * tile_cols(dtype, kind);
 }
 
 extern "C" int odp_xent_dx(odp_stream_t stream, int dtype, int64_t n, int64_t width, const int32_t* count,
@@ -1053,9 +1065,9 @@ extern "C" int odp_xent_dx(odp_stream_t stream, int dtype, int64_t n, int64_t wi
   }
   const hipStream_t s = odp_hip_stream(stream);
   const int cap = dx_cap(dtype, n, width);
-  const bool few = few_rows(dtype, n);
+  const int kind = few_kind(dtype, n);
   unsigned blocks;
-  if (int rc = grid_of("odp_xent_dx", dtype, few, cap, 1, true, blocks)) return rc;
+  if (int rc = grid_of("odp_xent_dx", dtype, kind, cap, 1, true, blocks)) return rc;
   const Xent p = xent_of(nullptr, w, ldw, vocab, width, n, count, nullptr, nullptr, 0.f);
   const int64_t whole = odp_xent_pitch(dtype, piece);
   ODP_XENT_LAUNCH(k_xent_dx, blocks, p, v0, vc, whole, dl, ldd, cap, v0 == 0 ? 1 : 0, (float*)scratch);
@@ -1084,8 +1096,8 @@ extern "C" int odp_xent_dx_rows(odp_stream_t stream, int dtype, int64_t n, int64
     return ODP_ERR_UNSUPPORTED;
   }
   const hipStream_t s = odp_hip_stream(stream);
-  const bool few = few_rows(dtype, n);
-  const int ot = tile_rows(dtype, few), tn = (int)up(width, tile_cols(dtype, few)), cap = dx_cap(dtype, n, width);
+  const int kind = few_kind(dtype, n);
+  const int ot = tile_rows(dtype, kind), tn = (int)up(width, tile_cols(dtype, kind)), cap = dx_cap(dtype, n, width);
   const int64_t steps = odp_xent_pitch(dtype, piece) / (dtype == ODP_DTYPE_F32 ? 16 : 32);
   if (dtype == ODP_DTYPE_F32)
     hipLaunchKernelGGL((k_xent_dx_rows<ODP_DTYPE_F32>), dim3((unsigned)blocks), dim3(256), 0, s,
@@ -1144,7 +1156,7 @@ extern "C" int odp_xent_dw(odp_stream_t stream, int dtype, const void* xc, int64
 #undef ODP_DW
     return odp_check_launch("odp_xent_dw");
   }
-  if (int rc = grid_of("odp_xent_dw", dtype, false, up(vc, tile_edge(dtype)), up(width, tile_edge(dtype)), false, blocks)) return rc;
+  if (int rc = grid_of("odp_xent_dw", dtype, 0, up(vc, tile_edge(dtype)), up(width, tile_edge(dtype)), false, blocks)) return rc;
   const Xent p = xent_of(xc, nullptr, width, vc, width, n, count, nullptr, nullptr, 0.f);
   if (dtype == ODP_DTYPE_F32)
     ODP_XENT_GO((k_xent_dw<ODP_DTYPE_F32>), (Tile<ODP_DTYPE_F32, 0>::THREADS), blocks, p, vc, dl, ldd, dw, lddw);
