@@ -668,6 +668,8 @@ int odp_xent_losses(odp_stream_t stream, int dtype, const void* xc, int64_t n, i
 /* *out = the sum of the losses, over *over where that is not null.          */
 int odp_xent_reduce(odp_stream_t stream, const float* losses, int64_t n, const float* over, float* out);
 
+#define ODP_XENT_PIECE ((int64_t)1 << 22) /* the pitch of d in odp_xent_dx and odp_xent_dw stays below it */
+
 /* d [count][ldd] of the columns [v0, v0 + vc): g_t (exp(z - lse_t) - [target])
  * times the softcap's slope, in the inputs' type, zero past vc; ldd =
  * odp_xent_pitch(dtype, vc).  lse is per row of [n], g too (g_stride 1) or one

@@ -281,7 +281,8 @@ struct Xent : torch::autograd::Function<Xent> {
       const float* over = sd["mean"].toBool() ? p.counted() : nullptr;
       const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
       const int64_t es = p.xc.element_size(), edge = abi.xent_pitch(p.dt, 1);
-      const int64_t fit = sd["piece_bytes"].toInt() / (std::max<int64_t>(p.n, 1) * es) / edge * edge;
+      const int64_t fit = std::min(sd["piece_bytes"].toInt() / (std::max<int64_t>(p.n, 1) * es) / edge * edge,
+                                   ODP_XENT_PIECE - edge);
       const int64_t pieces = (p.vocab + std::max(fit, edge) - 1) / std::max(fit, edge);
       const int64_t piece = std::min(p.vocab, ((p.vocab + pieces - 1) / pieces + edge - 1) / edge * edge);
       const at::Tensor d = at::empty({std::max<int64_t>(p.n, 1), abi.xent_pitch(p.dt, piece)}, p.xc.options());

@@ -139,8 +139,8 @@ __device__ __forceinline__ uint64_t t_uniform64(uint64_t v) {
 }
 
 // One operand of a tile: `base` is element (row 0 of the matrix, k = 0),
-// `row0` the tile's first row, `rows` the matrix's.  ld * element size < 2^22
-// (host checks), rows of a tile stay within 32-bit offsets.
+// `row0` the tile's first row, `rows` the matrix's.  The host's checks of ld (at
+// most 2^23 bytes a row) keep the rows of a tile within 31-bit offsets.
 struct Operand {
   const void* base;
   int64_t ld;

@@ -790,6 +790,8 @@ int tile_edge(int dtype) { return dtype == ODP_DTYPE_F32 ? 128 : 256; }
 int tile_rows(int dtype, int kind) { return kind == 1 ? 64 : kind == 2 ? 128 : kind == 3 ? 32 : tile_edge(dtype); }
 int tile_cols(int dtype, int kind) { return kind == 1 || kind == 3 ? 128 : tile_edge(dtype); }
 
+static_assert(2 * 255 * ODP_XENT_PIECE < T_OOB && 4 * 127 * ODP_XENT_PIECE < T_OOB, "offsets of a tile's rows of d");
+
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Whether a product of n rows takes the tiles of few rows.  Loss and dx, us,
@@ -1052,7 +1054,7 @@ extern "C" int odp_xent_dx(odp_stream_t stream, int dtype, int64_t n, int64_t wi
                            const void* dl, int64_t ldd, void* scratch) {
   if (int rc = check_xent("odp_xent_dx", dtype, n, width, ldw, vocab)) return rc;
   if (v0 < 0 || vc <= 0 || vc > piece || v0 + vc > vocab || ldd != odp_xent_pitch(dtype, vc) ||
-      ldd >= (int64_t)1 << 20) {
+      ldd >= ODP_XENT_PIECE) {
     odp_set_error("odp_xent_dx: columns [%lld, %lld) of %lld in pieces of %lld at pitch %lld", (long long)v0,
                   (long long)(v0 + vc), (long long)vocab, (long long)piece, (long long)ldd);
     return ODP_ERR_INVALID_ARGUMENT;
@@ -1128,7 +1130,7 @@ extern "C" int odp_xent_dw(odp_stream_t stream, int dtype, const void* xc, int64
                            const int32_t* count, int64_t vc, const void* dl, int64_t ldd, void* scratch, void* dw,
                            int64_t lddw) {
   if (int rc = check_xent("odp_xent_dw", dtype, n, width, lddw, vc)) return rc;
-  if (ldd != odp_xent_pitch(dtype, vc) || ldd >= (int64_t)1 << 20 || count == nullptr || dw == nullptr || !on16(dw) ||
+  if (ldd != odp_xent_pitch(dtype, vc) || ldd >= ODP_XENT_PIECE || count == nullptr || dw == nullptr || !on16(dw) ||
       (n > 0 && (xc == nullptr || dl == nullptr || !on16(xc) || !on16(dl)))) {
     odp_set_error("odp_xent_dw: pitch %lld for %lld columns, null pointer, or rows off the 16-byte grid",
                   (long long)ldd, (long long)vc);

@@ -276,6 +276,7 @@ _HEAD_DTYPES = (torch.float32, torch.bfloat16)
 # Bytes of d (the logits' gradient, in the inputs' type) that the backward
 # holds at a time: a piece of the vocabulary for all tokens.
 PIECE_BYTES = 512 << 20
+_PIECE_COLUMNS = 1 << 22  # a piece's columns stay below it (ODP_XENT_PIECE)
 # Bytes of float32 logits up to which a call that wants gradients keeps them
 # for its backward (1.5 % of the memory of one GPU) where that is faster than
 # forming them again; 0 keeps none.  Neither do the gradients of torch.func
@@ -347,7 +348,8 @@ class _Packed:
     def piece(self, whole: bool = False) -> int:
         """Columns of the vocabulary a piece of d holds: as many pieces as PIECE_BYTES makes, of one size."""
         edge = _xent_pitch(self.dt, 1)
-        fit = max(PIECE_BYTES // (max(self.n, 1) * self.xc.element_size()) // edge * edge, edge)
+        fit = max(min(PIECE_BYTES // (max(self.n, 1) * self.xc.element_size()) // edge * edge, _PIECE_COLUMNS - edge),
+                  edge)
         pieces = -(-self.vocab // fit)
         return self.vocab if whole else min(self.vocab, -(-(-(-self.vocab // pieces)) // edge) * edge)
 

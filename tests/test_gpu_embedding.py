@@ -467,3 +467,22 @@ def test_in_a_graph():
         got = [t.clone() for t in held]
         for a, b in zip(got, step()):
             assert torch.equal(a, b.detach())
+
+
+def test_offsets_past_32_bits():
+    """A table of 4.9 GB: its last rows are read, and their gradients written, where they lie."""
+    vocab, width = 2400000, 1024
+    w = torch.zeros(vocab, width, device="cuda", dtype=torch.bfloat16)
+    rows = torch.tensor([vocab - 1, 0, vocab - 2, vocab // 2, vocab - 1], device="cuda")
+    w[rows] = torch.randn(5, width, device="cuda").to(w.dtype)
+    w.requires_grad_()
+    out = embedding(rows, w)
+    assert torch.equal(out, w.detach()[rows])
+    go = torch.randn(5, width, device="cuda").to(w.dtype)
+    (dw,) = torch.autograd.grad(out, [w], go)
+    assert torch.equal(dw[vocab - 1], (go[0].float() + go[4].float()).to(w.dtype))
+    for k in (1, 2, 3):
+        assert torch.equal(dw[rows[k]], go[k])
+        dw[rows[k]] = 0
+    dw[vocab - 1] = 0
+    assert not dw.any()

@@ -554,3 +554,60 @@ def test_gradients_under_vmap(outside):
     got = torch.func.vmap(torch.func.grad(lambda a, b: linear_cross_entropy(a, wd, b, reduction="sum")))(xd, yd)
     want, bound = reference(x.reshape(12, 136), w, y.reshape(12), torch.ones(12), None, torch.float32)
     assert within(got.detach().reshape(12, 136), want[1], bound[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("n,width,vocab", [(300, 768, 700), (2100, 136, 300), (20, 136, 2000)])
+def test_in_a_graph_with_kept_logits_and_slices(n, width, vocab, dtype):
+    x, w, y, _ = inputs(n, width, vocab, dtype, seed=78)
+    x, w, y = x.to(DEV).requires_grad_(), w.to(DEV).requires_grad_(), y.to(DEV)
+
+    def step():
+        loss = linear_cross_entropy(x, w, y)
+        return loss, *torch.autograd.grad(loss, [x, w])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for k in range(4):
+        y.copy_(torch.randint(0, vocab, (n,), device=DEV))
+        y[: 4 * k] = -100
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.detach().clone() for t in held]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b.detach())
+
+
+def test_offsets_past_32_bits():
+    """A head of 4.9 GB: its last rows are read, and their gradients written, where they lie."""
+    n, width, vocab = 24, 1024, 2400000
+    g = torch.Generator(device=DEV).manual_seed(5)
+    w = torch.randn(vocab, width, generator=g, device=DEV, dtype=torch.bfloat16) / 32
+    x = torch.randn(n, width, generator=g, device=DEV, dtype=torch.bfloat16)
+    y = torch.tensor([vocab - 1, 0, vocab // 2, vocab - 257] * 6, device=DEV)
+    x.requires_grad_(), w.requires_grad_()
+    loss = linear_cross_entropy(x, w, y, reduction="none")
+    dx, dw = torch.autograd.grad(loss.sum(), [x, w])
+    with torch.no_grad():
+        z = torch.cat([x.double() @ p.double().t() for p in w.split(200000)], 1)
+        lse = torch.logsumexp(z, 1)
+        want = lse - z.gather(1, y.unsqueeze(1)).squeeze(1)
+        # float32 sums of `width` products and of the exponentials.
+        slack = 4 * width * U32 * (x.double().abs() @ w[y].double().abs().t()).max() + 64 * U32 * lse.abs().max()
+        assert float((loss.double() - want).abs().max()) <= float(slack)
+        d = torch.softmax(z, 1)
+        d[torch.arange(n, device=DEV), y] -= 1.0
+        for row in (0, vocab // 2, vocab - 257, vocab - 1):
+            exact = d[:, row] @ x.double()
+            scale = d[:, row].abs() @ x.double().abs()
+            assert bool(((dw[row].double() - exact).abs() <= 2.0**-7 * scale).all())
+        near = sum(d[:, k : k + 200000] @ w[k : k + 200000].double() for k in range(0, vocab, 200000))
+        size = sum(d[:, k : k + 200000].abs() @ w[k : k + 200000].double().abs() for k in range(0, vocab, 200000))
+        assert bool(((dx.double() - near).abs() <= 2.0**-7 * size).all())
