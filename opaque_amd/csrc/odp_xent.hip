@@ -795,10 +795,11 @@ static_assert(2 * 255 * ODP_XENT_PIECE < T_OOB && 4 * 127 * ODP_XENT_PIECE < T_O
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Whether a product of n rows takes the tiles of few rows.  Loss and dx, us,
-// with the small tiles and the large ones: bfloat16, 32000 x 2048, 47 tokens
-// 94 and 157, 64 95 and 156, 128 119 and 161, 192 153 and 164, 256 185 and
-// 167; 128256 x 4096, 64 tokens 623 and 639, 65 1022 and 729; float32, 50257
-// x 768, 64 tokens 242 and 420, 256 598 and 643, 384 791 and 738.
+// with the small tiles and the large ones: bfloat16, 32000 x 2048, 64 tokens 69
+// and 87, 128 84 and 96, 192 109 and 104, 256 130 and 118; 128256 x 4096, 64
+// tokens 440 and 421, 65 605 and 409 (W past the cache is read once a row of
+// tiles); float32, 50257 x 768, 64 tokens 143 and 231, 256 364 and 394, 384 542
+// and 524.
 bool few_rows(int dtype, int64_t n) { return n <= (dtype == ODP_DTYPE_F32 ? 256 : 64); }
 
 // The tiles of few rows of n, else the large ones.  float32, 50257 x 768,
@@ -809,8 +810,8 @@ int few_kind(int dtype, int64_t n) { return !few_rows(dtype, n) ? 0 : dtype == O
 // 128 rows takes about 0.7 of the time of one of 256: bfloat16 takes those
 // where that leaves fewer of the larger ones' times, counting whole rounds of
 // the CUs.  Loss and dx, us, with 128 and with 256 rows: 32000 x 2048, 128
-// tokens 134 and 163, 256 151 and 172, 512 233 and 210; 128256 x 4096, 128
-// tokens 648 and 707, 160 820 and 732; 50257 x 768, 600 tokens 231 and 248.
+// tokens 96 and 106, 256 118 and 136, 512 189 and 181; 128256 x 4096, 128
+// tokens 469 and 491, 160 568 and 510; 50257 x 768, 600 tokens 187 and 196.
 int tile_kind(int dtype, int64_t n, int64_t cols) {
   if (few_rows(dtype, n)) return few_kind(dtype, n);
   if (dtype == ODP_DTYPE_F32) return 0;
