@@ -67,6 +67,31 @@ class CaptureSession:
     pairs: list[tuple[int, int, int, int]] = field(default_factory=list)  # ids of (A, B, W, bias) per call
     linear_ws: list[int] = field(default_factory=list)  # ids of weights of full-weight linear seams
     eligible: set[int] = field(default_factory=set)  # ids allowed to be captured
+    params: set[int] = field(default_factory=set)  # discover: ids of the differentiated leaves
+
+    def hide(self, t: torch.Tensor) -> torch.Tensor:
+        """Books a seam use of ``t`` and keeps it out of autograd where it is a
+        differentiated leaf itself.  A tensor made from one (a cast, a slice, a
+        scaled copy) stays attached: the gradient it brings to the leaf is a
+        use outside the seams, which no record would hold."""
+        if id(t) not in self.params:
+            return t
+        self.uses[id(t)] = self.uses.get(id(t), 0) + 1
+        return t.detach()
+
+    def derived(self, *ts: torch.Tensor | None) -> bool:
+        """Whether any of the tensors was made from a differentiated leaf."""
+        nodes = [t.grad_fn for t in ts if t is not None and id(t) not in self.params]
+        seen = set()
+        while nodes:
+            fn = nodes.pop()
+            if fn is None or fn in seen:
+                continue
+            seen.add(fn)
+            if id(getattr(fn, "variable", None)) in self.params:
+                return True
+            nodes += [up for up, _ in fn.next_functions]
+        return False
 
     def __enter__(self) -> CaptureSession:
         if getattr(_STATE, "session", None) is not None:
@@ -188,13 +213,14 @@ def _lora(x, W, A, B, scaling, bias, a_obj, b_obj, a_t, b_t):
     if sess is None:
         return _plain(x, W, A, B, scaling, bias)
     if sess.mode == "discover":
-        for t in (a_obj, b_obj):
-            if t is not None:
-                sess.uses[id(t)] = sess.uses.get(id(t), 0) + 1
+        if sess.derived(W, a_obj, b_obj):
+            # Not recorded in a capture pass: its leaves, attached here, go materialised.
+            return _plain(x, W, A, B, scaling, bias)
         sess.pairs.append((id(a_obj), id(b_obj), id(W), id(bias) if bias is not None else 0))
         # Seam parameters are hidden from autograd here, so a gradient that still
         # reaches them afterwards reveals a use outside a seam.
-        return _plain(x, W, A.detach(), B.detach(), scaling, bias)
+        A, B = (t if sess.hide(o) is o else t.detach() for t, o in ((A, a_obj), (B, b_obj)))
+        return _plain(x, W, A, B, scaling, bias)
     if id(a_obj) not in sess.eligible and id(b_obj) not in sess.eligible:
         return _plain(x, W, A, B, scaling, bias)
     return _SeamLoRA.apply(x, W, A, B, scaling, bias, a_obj, b_obj, a_t, b_t)
@@ -416,10 +442,10 @@ def moe(x: torch.Tensor, gate_up_proj: torch.Tensor, down_proj: torch.Tensor,
     if sess is None:
         return _moe_dense(x, gate_up_proj, down_proj, top_k_index, top_k_weights)
     if sess.mode == "discover":
-        for t in (gate_up_proj, down_proj):
-            sess.uses[id(t)] = sess.uses.get(id(t), 0) + 1
-            sess.linear_ws.append(id(t))
-        return _moe_dense(x, gate_up_proj.detach(), down_proj.detach(), top_k_index, top_k_weights)
+        if not sess.derived(gate_up_proj, down_proj):
+            sess.linear_ws += [id(gate_up_proj), id(down_proj)]
+            gate_up_proj, down_proj = sess.hide(gate_up_proj), sess.hide(down_proj)
+        return _moe_dense(x, gate_up_proj, down_proj, top_k_index, top_k_weights)
     if id(gate_up_proj) not in sess.eligible and id(down_proj) not in sess.eligible:
         return _moe_dense(x, gate_up_proj, down_proj, top_k_index, top_k_weights)
     return _SeamMoE.apply(x, gate_up_proj, down_proj, top_k_index, top_k_weights)
@@ -434,9 +460,8 @@ def linear(x: torch.Tensor, W: torch.Tensor, bias: torch.Tensor | None = None) -
     if sess is None:
         return F.linear(x, W, bias)
     if sess.mode == "discover":
-        sess.uses[id(W)] = sess.uses.get(id(W), 0) + 1
         sess.linear_ws.append(id(W))
-        return F.linear(x, W.detach(), bias)
+        return F.linear(x, sess.hide(W), bias)
     if id(W) not in sess.eligible:
         return F.linear(x, W, bias)
     return _SeamLinear.apply(x, W, bias)

@@ -454,7 +454,7 @@ class _ClipEngine:
         single = list(self._with_grad_tree(args, tree_unflatten(treedef, proxies)))
         for i in self.batch_argnums:
             single[i] = tree_map(lambda t: t[0] if isinstance(t, torch.Tensor) else t, single[i])
-        sess = CaptureSession(mode="discover")
+        sess = CaptureSession(mode="discover", params=set(pid))
         with torch.enable_grad(), sess:
             value, _ = self._loss(*single, **kwargs)
         outside = [False] * len(leaves)

@@ -248,8 +248,7 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
         padding = padding_idx % weight.shape[0]
     sess = active_session()
     if sess is not None and sess.mode == "discover":
-        sess.uses[id(weight)] = sess.uses.get(id(weight), 0) + 1
-        weight = weight.detach()
+        weight = sess.hide(weight)
     host = None if _transformed() else _bound()
     if host is not None:
         return host.embedding(tokens, weight, scale, padding)
@@ -543,8 +542,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
         raise ValueError(f"softcap must be positive and finite, got {softcap}")
     sess = active_session()
     if sess is not None and sess.mode == "discover":
-        sess.uses[id(weight)] = sess.uses.get(id(weight), 0) + 1
-        weight = weight.detach()
+        weight = sess.hide(weight)
     host = None if _transformed() else _bound()
     if host is not None:
         return host.cross_entropy(x, weight, target, softcap or 0.0, ignore_index, _REDUCTIONS[reduction], PIECE_BYTES,
