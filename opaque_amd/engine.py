@@ -568,8 +568,8 @@ def plan_key(*, segments: Segments, leaves: list[LeafOut], clip: ClipSpec, lora_
     mats = tuple((_tensor_key(m.per_example), m.leaf, _seg_key(m.segments)) for m in materialized)
     lins = tuple((shared(ls.x), _tensor_key(ls.g), ls.w_leaf, ls.form, ls.index,
                   _seg_key(ls.segments)) for ls in linear_sites)
-    embeds = tuple((tuple(es.tokens.shape), es.tokens.dtype, _tensor_key(es.g), es.w_leaf, float(es.scale),
-                    int(es.padding), _seg_key(es.segments)) for es in embedding_sites)
+    embeds = tuple((tuple(es.tokens.shape), es.tokens.dtype, es.tokens.get_device(), _tensor_key(es.g), es.w_leaf,
+                    float(es.scale), int(es.padding), _seg_key(es.segments)) for es in embedding_sites)
     outs = leaves_key(leaves) if leaves_key_ is None else leaves_key_
     clip_s = (clip.mode, len(clip.thresholds), tuple(g[2] for g in clip.guards))
     unknown = set(options) - set(_PLAN_OPTIONS)
@@ -633,7 +633,8 @@ class _EmbeddingWork:
     def rebind(self, es: EmbeddingSite, trusted: bool) -> bool:
         old = self.site
         if not trusted and (es.tokens.shape != old.tokens.shape or es.tokens.dtype != old.tokens.dtype
-                            or es.g.shape != old.g.shape or es.g.dtype != old.g.dtype or es.g.device != old.g.device
+                            or es.tokens.device != old.tokens.device or es.g.shape != old.g.shape
+                            or es.g.dtype != old.g.dtype or es.g.device != old.g.device
                             or (es.w_leaf, es.scale, es.padding) != (old.w_leaf, old.scale, old.padding)):
             return False
         self._take(es)
