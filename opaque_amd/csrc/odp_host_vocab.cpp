@@ -8,6 +8,8 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
 #include <string>
@@ -92,18 +94,23 @@ at::Tensor pitched(const at::Tensor& t) {
   return r;
 }
 
-// Ties a first derivative to the gradient it came from, so that asking for a
-// second one is an error instead of zero.
-struct NoSecond : torch::autograd::Function<NoSecond> {
-  static at::Tensor forward(torch::autograd::AutogradContext*, const at::Tensor&, const at::Tensor& d) {
-    return d.detach();
-  }
-  static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
-    TORCH_CHECK(false, "the vocabulary operators have no second derivative");
-  }
-};
-at::Tensor first_only(const at::Tensor& g, at::Tensor d) {
-  return d.defined() && at::GradMode::is_enabled() && g.requires_grad() ? NoSecond::apply(g, d) : d;
+// Ties a first derivative to what it depends on, so that asking for a second
+// one is an error instead of zero: to the gradient g it came from and, with
+// `inputs`, to the inputs of the node whose backward pass calls this (by
+// their edges: their values need not be kept).
+at::Tensor first_only(const at::Tensor& g, at::Tensor d, bool inputs) {
+  if (!d.defined() || !at::GradMode::is_enabled()) return d;
+  torch::autograd::edge_list on;
+  if (inputs)
+    for (const auto& e : torch::autograd::get_current_node()->next_edges())
+      if (e.is_valid()) on.push_back(e);
+  if (g.requires_grad()) on.push_back(torch::autograd::impl::gradient_edge(g));
+  if (on.empty()) return d;
+  const auto error = std::make_shared<torch::autograd::Error>(
+      "the vocabulary operators have no second derivative", std::move(on));
+  d = d.detach();
+  torch::autograd::set_history(d, error);
+  return d;
 }
 
 // ---------------------------------------------------------------------------
@@ -154,7 +161,7 @@ struct Embed : torch::autograd::Function<Embed> {
                            (float)ctx->saved_data["scale"].toDouble(), at, dw.data_ptr()),
             "odp_embed_grad");
     }
-    return {{}, first_only(grads[0], dw), {}, {}};
+    return {{}, first_only(grads[0], dw, false), {}, {}};
   }
 };
 
@@ -319,7 +326,7 @@ struct Xent : torch::autograd::Function<Xent> {
               "odp_xent_dx_rows");
       if (need_w && p.cols != p.width) dw = dw.narrow(1, 0, p.cols).contiguous();
     }
-    return {first_only(grads[0], dx), first_only(grads[0], dw), {}, {}, {}, {}, {}, {}, {}};
+    return {first_only(grads[0], dx, true), first_only(grads[0], dw, true), {}, {}, {}, {}, {}, {}, {}};
   }
 };
 

@@ -1,0 +1,72 @@
+"""The vocabulary operators as autograd nodes: what they refuse, what they hold, which gradients they give."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from opaque_amd import vocabulary
+from opaque_amd.vocabulary import embedding, linear_cross_entropy
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+
+
+def inputs(n=8, width=16, vocab=30, dtype=torch.float32, seed=5):
+    g = torch.Generator().manual_seed(seed)
+    x, w = torch.randn(n, width, generator=g), torch.randn(vocab, width, generator=g) / math.sqrt(width)
+    return x.to(dtype).to(DEV), w.to(dtype).to(DEV), torch.randint(0, vocab, (n,), generator=g).to(DEV)
+
+
+@pytest.fixture(params=[True, False], ids=["helper", "functions"])
+def route(request, monkeypatch):
+    if not request.param:
+        monkeypatch.setattr(vocabulary, "_host_ready", [None])
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("trained", ["x", "w", "xw"])
+def test_a_second_derivative_of_the_loss_is_an_error(route, reduction, trained):
+    """Also where the gradient that comes in is a constant: the first derivative depends on x and the head."""
+    x, w, y = inputs()
+    x.requires_grad_("x" in trained), w.requires_grad_("w" in trained)
+    wanted = [t for t in (x, w) if t.requires_grad]
+    loss = linear_cross_entropy(x, w, y, reduction=reduction)
+    gl = torch.ones_like(loss)
+    first = torch.autograd.grad(loss, wanted, gl, create_graph=True)
+    plain = torch.autograd.grad(linear_cross_entropy(x, w, y, reduction=reduction), wanted, gl)
+    for d, p in zip(first, plain):
+        assert d.requires_grad and torch.equal(d.detach(), p) and not p.requires_grad
+        for t in wanted:
+            with pytest.raises(RuntimeError):
+                torch.autograd.grad(d.square().sum(), t, retain_graph=True)
+    loss = linear_cross_entropy(x, w, y, reduction=reduction).sum()
+    first = torch.autograd.grad(loss, wanted, create_graph=True)
+    with pytest.raises(RuntimeError):
+        (loss + sum(d.square().sum() for d in first)).backward()
+
+
+def test_first_derivatives_under_create_graph_are_usable(route):
+    """backward(create_graph=True) itself is no second derivative; a penalty on other tensors differentiates."""
+    x, w, y = inputs()
+    x.requires_grad_(), w.requires_grad_()
+    linear_cross_entropy(x, w, y).backward(create_graph=True)
+    assert x.grad.shape == x.shape and w.grad.shape == w.shape
+    scale = torch.tensor(2.0, device=DEV, requires_grad=True)
+    (dx,) = torch.autograd.grad(linear_cross_entropy(x, w, y), [x], create_graph=True)
+    (ds,) = torch.autograd.grad((scale * dx).square().sum(), [scale])
+    assert torch.allclose(ds, 2 * scale.detach() * dx.detach().square().sum())
+
+
+def test_a_second_derivative_of_the_lookup(route):
+    """The table's gradient is linear in the gradient that comes in, which the kernels do not differentiate; it does
+    not depend on the table."""
+    _, w, y = inputs()
+    w.requires_grad_()
+    go = torch.ones(y.numel(), w.shape[1], device=DEV, requires_grad=True)
+    (dw,) = torch.autograd.grad(embedding(y, w), [w], go, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dw.sum(), [go])
