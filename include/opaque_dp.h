@@ -639,6 +639,9 @@ int odp_embed_clipped_sum(odp_stream_t stream, int dtype, const void* g, int64_t
                           float scale, const int32_t* seg_example, void* scratch, const float* whole,
                           const double* scales, float normalize_by, int out_dtype, void* out, void* out2);
 
+#define ODP_XENT_STAT 3 /* floats that the forward leaves of a row: the maximum of its logits, the sum of \
+                           exponentials below it and p(target) - 1 */
+
 /* ---- linear cross entropy -------------------------------------------------
  * loss_t = lse_t - z_t,y(t), lse_t = log sum_v exp z_tv, z = u or
  * softcap tanh(u / softcap) (softcap 0: none), u = x W^T, for rows x [n][cols]
@@ -651,28 +654,29 @@ int odp_embed_clipped_sum(odp_stream_t stream, int dtype, const void* g, int64_t
  * act[k] the row, tgt[k] its target, count[0] how many and count[1] (float32)
  * how many targets are not `ignore`, where[row] the place (-1: target ==
  * ignore, -2: target outside the vocabulary); losses (0, or NaN outside the
- * vocabulary) and lse (0) of the rows that bear none, where those are not null.  keep != 0 packs every row, with tgt -1 where it bears no loss. */
+ * vocabulary) and stat (0) of the rows that bear none, where those are not
+ * null.  keep != 0 packs every row, with tgt -1 where it bears no loss.     */
 int odp_xent_rows(odp_stream_t stream, int dtype, const void* x, int64_t ldx, int64_t n, int64_t cols, int64_t width,
                   const void* target, int target_bytes, int64_t vocab, int64_t ignore, int keep, void* xc,
-                  int32_t* act, int32_t* tgt, int32_t* where, int32_t* count, float* losses, float* lse);
+                  int32_t* act, int32_t* tgt, int32_t* where, int32_t* count, float* losses, float* stat);
 
-/* losses and lse of the packed rows, at their places in [n]; logits (null: not
+/* losses and stat ([ODP_XENT_STAT]) of the packed rows, at their places in [n]; logits (null: not
  * kept) [n][ldl] receives the packed rows' z, ldl = odp_xent_pitch(dtype, vocab).
  * odp_xent_kept: their bytes, 0 where forming them again is faster.          */
 int64_t odp_xent_kept(int dtype, int64_t n, int64_t width, int64_t vocab);
 int64_t odp_xent_stats_scratch(int dtype, int64_t n, int64_t vocab);
 int odp_xent_losses(odp_stream_t stream, int dtype, const void* xc, int64_t n, int64_t width, const int32_t* act,
                     const int32_t* tgt, const int32_t* count, const void* w, int64_t ldw, int64_t vocab,
-                    float softcap, void* scratch, float* losses, float* lse, float* logits, int64_t ldl);
+                    float softcap, void* scratch, float* losses, float* stat, float* logits, int64_t ldl);
 
 /* *out = the sum of the losses, over *over where that is not null.          */
 int odp_xent_reduce(odp_stream_t stream, const float* losses, int64_t n, const float* over, float* out);
 
 #define ODP_XENT_PIECE ((int64_t)1 << 22) /* the pitch of d in odp_xent_dx and odp_xent_dw stays below it */
 
-/* d [count][ldd] of the columns [v0, v0 + vc): g_t (exp(z - lse_t) - [target])
+/* d [count][ldd] of the columns [v0, v0 + vc): g_t (p_tv - [target])
  * times the softcap's slope, in the inputs' type, zero past vc; ldd =
- * odp_xent_pitch(dtype, vc).  lse is per row of [n], g too (g_stride 1) or one
+ * odp_xent_pitch(dtype, vc).  stat is per row of [n], g too (g_stride 1) or one
  * for all (0), divided by *over where that is not null.  rest [n]: what
  * rounding takes off each packed row's target entry (bfloat16).  From the kept
  * logits where those are given (v0 then a multiple of odp_xent_pitch(dtype, 1)),
@@ -680,7 +684,7 @@ int odp_xent_reduce(odp_stream_t stream, const float* losses, int64_t n, const f
 int64_t odp_xent_pitch(int dtype, int64_t columns);
 int odp_xent_dlogits(odp_stream_t stream, int dtype, const void* xc, int64_t n, int64_t width, const int32_t* act,
                      const int32_t* tgt, const int32_t* count, const void* w, int64_t ldw, int64_t vocab,
-                     float softcap, int64_t v0, int64_t vc, const float* lse, const float* g, int g_stride,
+                     float softcap, int64_t v0, int64_t vc, const float* stat, const float* g, int g_stride,
                      const float* over, const float* logits, int64_t ldl, void* dl, int64_t ldd, float* rest);
 
 /* Adds d W of a piece of the vocabulary to the float32 sums of dx in scratch

@@ -187,7 +187,7 @@ at::Tensor head_rows(const at::Tensor& weight) {
 
 // The packed rows of a call (odp_xent_rows) and what its backward needs.
 struct Packed {
-  at::Tensor w, xc, ids, losses, lse, logits;  // logits: where they are kept
+  at::Tensor w, xc, ids, losses, stat, logits;  // logits: where they are kept
   int64_t n, cols, width, vocab;
   int dt;
   int32_t* count() const { return (int32_t*)ids.data_ptr(); }
@@ -199,9 +199,9 @@ struct Packed {
   int64_t kept_pitch() const { return abi.xent_pitch(dt, vocab); }
 };
 
-// The log-sum-exp goes to lse_out.  keep_bytes: up to which the logits are kept for a backward pass.
+// The rows' statistics go to stat_out.  keep_bytes: up to which the logits are kept for a backward pass.
 Packed xent_forward(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target,
-                    const at::Tensor& lse_out, double softcap, int64_t ignore, int64_t keep_bytes) {
+                    const at::Tensor& stat_out, double softcap, int64_t ignore, int64_t keep_bytes) {
   Packed p;
   p.w = head_rows(weight);
   const at::Tensor rows = pitched(x), y = target.contiguous();
@@ -214,19 +214,19 @@ Packed xent_forward(const at::Tensor& x, const at::Tensor& weight, const at::Ten
   p.xc = at::empty({room, p.width}, rows.options());
   p.ids = at::empty({3 * room + 2}, rows.options().dtype(at::kInt));
   p.losses = at::empty(target.sizes(), rows.options().dtype(at::kFloat));
-  p.lse = lse_out;
+  p.stat = stat_out;
   float* losses = (float*)p.losses.data_ptr();
-  float* lse = (float*)p.lse.data_ptr();
+  float* stat = (float*)p.stat.data_ptr();
   const odp_stream_t s = stream_of(rows);
   check(abi.xent_rows(s, p.dt, rows.data_ptr(), rows.stride(0), p.n, p.cols, p.width, y.data_ptr(),
                       (int)y.element_size(), p.vocab, ignore, 0, p.xc.data_ptr(), p.act(), p.tgt(), p.where(),
-                      p.count(), losses, lse),
+                      p.count(), losses, stat),
         "odp_xent_rows");
   const int64_t kept = abi.xent_kept(p.dt, p.n, p.width, p.vocab);
   if (kept > 0 && kept <= keep_bytes) p.logits = at::empty({p.n, p.kept_pitch()}, p.losses.options());
   const at::Tensor work = bytes_on(rows, abi.xent_stats_scratch(p.dt, p.n, p.vocab));
   check(abi.xent_losses(s, p.dt, p.xc.data_ptr(), p.n, p.width, p.act(), p.tgt(), p.count(), p.w.data_ptr(),
-                        p.w.stride(0), p.vocab, (float)softcap, work.data_ptr(), losses, lse, p.kept(), p.kept_pitch()),
+                        p.w.stride(0), p.vocab, (float)softcap, work.data_ptr(), losses, stat, p.kept(), p.kept_pitch()),
         "odp_xent_losses");
   return p;
 }
@@ -243,17 +243,17 @@ at::Tensor xent_result(const Packed& p, int64_t reduction) {
 
 struct Xent : torch::autograd::Function<Xent> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight,
-                            const at::Tensor& target, const at::Tensor& lse, double softcap, int64_t ignore,
+                            const at::Tensor& target, const at::Tensor& stat, double softcap, int64_t ignore,
                             int64_t reduction, int64_t piece_bytes, int64_t keep_bytes) {
     const c10::OptionalDeviceGuard guard(x.device());
-    const Packed p = xent_forward(x, weight, target, lse, softcap, ignore, keep_bytes);
+    const Packed p = xent_forward(x, weight, target, stat, softcap, ignore, keep_bytes);
     // A later change of the head in place is an error; the kept logits go when the backward pass is through.
     ctx->save_for_backward({weight, p.logits});
     auto& d = ctx->saved_data;
     d["w"] = p.w;
     d["xc"] = p.xc;
     d["ids"] = p.ids;
-    d["lse"] = p.lse;
+    d["stat"] = p.stat;
     d["n"] = p.n;
     d["cols"] = p.cols;
     d["softcap"] = softcap;
@@ -280,7 +280,7 @@ struct Xent : torch::autograd::Function<Xent> {
       p.width = p.w.size(1);
       p.vocab = p.w.size(0);
       p.dt = code_of(p.xc);
-      const at::Tensor lse = sd["lse"].toTensor();
+      const at::Tensor stat = sd["stat"].toTensor();
       const float softcap = (float)sd["softcap"].toDouble();
       const c10::OptionalDeviceGuard guard(p.xc.device());
       const at::Tensor g = grads[0].contiguous();
@@ -299,12 +299,12 @@ struct Xent : torch::autograd::Function<Xent> {
         sums = bytes_on(p.xc, abi.xent_dx_scratch(p.dt, p.n, p.width));
       }
       if (need_w) dw = at::empty({p.vocab, p.width}, p.xc.options());
-      const at::Tensor rest = at::empty({std::max<int64_t>(p.n, 1)}, lse.options());
+      const at::Tensor rest = at::empty({std::max<int64_t>(p.n, 1)}, stat.options());
       const odp_stream_t s = stream_of(p.xc);
       for (int64_t v0 = 0; v0 < p.vocab; v0 += piece) {
         const int64_t vc = std::min(piece, p.vocab - v0), ldd = abi.xent_pitch(p.dt, vc);
         check(abi.xent_dlogits(s, p.dt, p.xc.data_ptr(), p.n, p.width, p.act(), p.tgt(), p.count(), p.w.data_ptr(),
-                               p.w.stride(0), p.vocab, softcap, v0, vc, (const float*)lse.data_ptr(),
+                               p.w.stride(0), p.vocab, softcap, v0, vc, (const float*)stat.data_ptr(),
                                (const float*)g.data_ptr(), stride, over, p.kept(), p.kept_pitch(), d.data_ptr(), ldd,
                                (float*)rest.data_ptr()),
               "odp_xent_dlogits");
@@ -330,31 +330,33 @@ struct Xent : torch::autograd::Function<Xent> {
   }
 };
 
-at::Tensor xent(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target, const at::Tensor& lse,
+at::Tensor xent(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target, const at::Tensor& stat,
                 double softcap, int64_t ignore, int64_t reduction, int64_t piece_bytes, int64_t keep_bytes) {
   if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad()))
-    return Xent::apply(x, weight, target, lse, softcap, ignore, reduction, piece_bytes, keep_bytes);
+    return Xent::apply(x, weight, target, stat, softcap, ignore, reduction, piece_bytes, keep_bytes);
   const c10::OptionalDeviceGuard guard(x.device());
-  return xent_result(xent_forward(x, weight, target, lse, softcap, ignore, 0), reduction);
+  return xent_result(xent_forward(x, weight, target, stat, softcap, ignore, 0), reduction);
 }
 
-at::Tensor lse_of(const at::Tensor& x, const at::Tensor& target) {
-  return at::empty(target.sizes(), x.options().dtype(at::kFloat).requires_grad(false));
+at::Tensor stat_of(const at::Tensor& x, const at::Tensor& target) {
+  std::vector<int64_t> shape(target.sizes().vec());
+  shape.push_back(ODP_XENT_STAT);
+  return at::empty(shape, x.options().dtype(at::kFloat).requires_grad(false));
 }
 
 at::Tensor cross_entropy(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target, double softcap,
                          int64_t ignore, int64_t reduction, int64_t piece_bytes, int64_t keep_bytes) {
   py::gil_scoped_release nogil;
-  return xent(x, weight, target, lse_of(x, target), softcap, ignore, reduction, piece_bytes, keep_bytes);
+  return xent(x, weight, target, stat_of(x, target), softcap, ignore, reduction, piece_bytes, keep_bytes);
 }
 
-// The token losses and their log-sum-exp, which has no gradient.
+// The token losses and their rows' statistics, which have no gradient.
 std::pair<at::Tensor, at::Tensor> token_losses(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target,
                                                double softcap, int64_t ignore, int64_t piece_bytes,
                                                int64_t keep_bytes) {
   py::gil_scoped_release nogil;
-  const at::Tensor lse = lse_of(x, target);
-  return {xent(x, weight, target, lse, softcap, ignore, 0, piece_bytes, keep_bytes), lse};
+  const at::Tensor stat = stat_of(x, target);
+  return {xent(x, weight, target, stat, softcap, ignore, 0, piece_bytes, keep_bytes), stat};
 }
 
 }  // namespace

@@ -105,6 +105,17 @@ __device__ __forceinline__ void softcap_all(float (&v)[N], float cap, float inv_
 // Rows that bear a loss.
 // ---------------------------------------------------------------------------
 
+// What the forward leaves of a row for the backward (ODP_XENT_STAT floats): the
+// maximum of its logits, the sum of exponentials below it and p(target) - 1.
+// One rounded log-sum-exp would take its last place off every d, more than all
+// of a nearly certain target's.
+constexpr int STAT = ODP_XENT_STAT;
+__device__ __forceinline__ void no_stat(float* stat, int64_t i) {
+  if (stat == nullptr) return;
+#pragma unroll
+  for (int k = 0; k < STAT; ++k) stat[STAT * i + k] = 0.f;
+}
+
 // where[i] = the place of row i among the packed rows, -1 for a row without a
 // loss, -2 for one whose target lies outside the vocabulary (loss NaN).
 // keep: every row is packed, with target -1 where it bears no loss.  count[0]:
@@ -113,7 +124,7 @@ __global__ __launch_bounds__(1024) void k_xent_pick(const void* __restrict__ tar
                                                     int64_t vocab, int64_t ignore, int keep, int32_t* __restrict__ act,
                                                     int32_t* __restrict__ tgt, int32_t* __restrict__ where,
                                                     int32_t* __restrict__ count, float* __restrict__ losses,
-                                                    float* __restrict__ lse) {
+                                                    float* __restrict__ stat) {
   __shared__ int32_t sums[16], other[16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int32_t base = 0, counted = 0;
@@ -126,7 +137,7 @@ __global__ __launch_bounds__(1024) void k_xent_pick(const void* __restrict__ tar
       live = t != ignore && t >= 0 && t < vocab;
       if (!live) {
         if (losses != nullptr) losses[i] = t == ignore ? 0.f : __uint_as_float(0x7fc00000u);
-        if (lse != nullptr) lse[i] = 0.f;
+        no_stat(stat, i);
       }
     }
     const bool taken = keep ? i < n : live;
@@ -166,7 +177,7 @@ struct Pick {
   int wide, keep;
   int64_t n, vocab, ignore;
   int32_t *act, *tgt, *where, *count;
-  float *losses, *lse;
+  float *losses, *stat;
 };
 constexpr int XENT_FEW = 1024;
 template <int DT, bool FEW>
@@ -202,7 +213,7 @@ __global__ __launch_bounds__(256) void k_xent_pack(const char* __restrict__ x, i
       if (blockIdx.x == 0 && in) {
         if (!live) {
           if (p.losses != nullptr) p.losses[i] = t == p.ignore ? 0.f : __uint_as_float(0x7fc00000u);
-          if (p.lse != nullptr) p.lse[i] = 0.f;
+          no_stat(p.stat, i);
         }
         if (taken) {
           p.act[k] = i;
@@ -376,7 +387,7 @@ __global__ __launch_bounds__(256) void k_xent_losses(const float* __restrict__ p
                                                      const float* __restrict__ ztgt, int tiles, int64_t n,
                                                      const int32_t* __restrict__ count,
                                                      const int32_t* __restrict__ act, const int32_t* __restrict__ tgt,
-                                                     float* __restrict__ losses, float* __restrict__ lse) {
+                                                     float* __restrict__ losses, float* __restrict__ stat) {
   constexpr int Q = 256 / R;
   __shared__ float rm[Q][R + 1], rs[Q][R + 1];
   const int r = threadIdx.x % R, q = threadIdx.x / R;
@@ -407,10 +418,14 @@ __global__ __launch_bounds__(256) void k_xent_losses(const float* __restrict__ p
   }
   if (q != 0 || !on) return;
   const float ref = m == -INFINITY ? 0.f : m;
-  const float l = logf(s);
-  lse[act[row]] = ref + l;
-  // Not lse less the target's logit: a small loss would keep little of lse's bits.
-  if (tgt[row] >= 0) losses[act[row]] = (ref - ztgt[row]) + l;
+  // Not the log-sum-exp less the target's logit: a small loss would keep little of its bits.
+  const float loss = tgt[row] >= 0 ? (ref - ztgt[row]) + logf(s) : 0.f;
+  const int64_t at = act[row];
+  float* to = stat + STAT * at;
+  to[0] = ref;
+  to[1] = s;
+  to[2] = expm1f(-loss);
+  if (tgt[row] >= 0) losses[at] = loss;
 }
 
 // The sum of the losses (in fp64, in one order), over *over where it is given.
@@ -485,8 +500,10 @@ __device__ __forceinline__ void t_store(void* out, int64_t ld, int64_t o0, int64
 // ---------------------------------------------------------------------------
 template <int DT, int S>
 struct DRows {  // of a lane's rows of a tile
-  float lse[Tile<DT, S>::BI], g[Tile<DT, S>::BI];  // log-sum-exp, gradient
-  int32_t tgt[Tile<DT, S>::BI];                 // target less the piece's first column
+  float m[Tile<DT, S>::BI];   // maximum of the logits
+  float gs[Tile<DT, S>::BI];  // gradient over the sum of exponentials below it: g p = gs exp(z - m)
+  float gt[Tile<DT, S>::BI];  // gradient times p(target) - 1
+  int32_t tgt[Tile<DT, S>::BI];  // target less the piece's first column
 };
 constexpr int32_t NO_LOSS = INT32_MIN;  // a target may lie anywhere beside the piece
 
@@ -511,10 +528,9 @@ __device__ __forceinline__ void dlogits_tile(const Xent& p, const typename Tile<
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float z = zs[e];
-      float q = fast_exp(z - rows.lse[i]);
       const bool hit = at == 16 * j + e;
       here |= hit;
-      q = (hit ? q - 1.f : q) * rows.g[i];
+      float q = hit ? rows.gt[i] : fast_exp(z - rows.m[i]) * rows.gs[i];
       if (CAP) {
         const float y = z * p.inv_cap;
         q *= 1.f - y * y;
@@ -529,7 +545,7 @@ __device__ __forceinline__ void dlogits_tile(const Xent& p, const typename Tile<
 
 template <int DT, int S, bool CAP>
 __global__ __launch_bounds__((Tile<DT, S>::THREADS), (DT == ODP_DTYPE_BF16 && S == 1 ? 1 : 2)) void k_xent_dlogits(Xent p, int64_t v0, int64_t vc,
-                                                                       const float* __restrict__ lse,
+                                                                       const float* __restrict__ stat,
                                                                        const float* __restrict__ g, int g_stride,
                                                                        const float* __restrict__ over, void* dl,
                                                                        int64_t ldd, float* __restrict__ rest) {
@@ -557,8 +573,10 @@ __global__ __launch_bounds__((Tile<DT, S>::THREADS), (DT == ODP_DTYPE_BF16 && S 
       const int64_t o = o0 + wm + t_row(i);
       const int32_t t = o < cnt ? p.tgt[o] : -1;
       const int64_t row = o < cnt ? p.act[o] : 0;
-      rows.lse[i] = t >= 0 ? lse[row] : 0.f;
-      rows.g[i] = t >= 0 ? g[row * g_stride] / part : 0.f;
+      const float gr = t >= 0 ? g[row * g_stride] / part : 0.f;
+      rows.m[i] = t >= 0 ? stat[STAT * row] : 0.f;
+      rows.gs[i] = t >= 0 ? gr / stat[STAT * row + 1] : 0.f;
+      rows.gt[i] = t >= 0 ? gr * stat[STAT * row + 2] : 0.f;
       rows.tgt[i] = t >= 0 ? t - (int32_t)v0 : NO_LOSS;
     }
     walk.next();
@@ -576,7 +594,7 @@ __global__ __launch_bounds__((Tile<DT, S>::THREADS), (DT == ODP_DTYPE_BF16 && S 
 constexpr int KEPT_COLS = 4096;
 template <int DT, bool CAP>
 __global__ __launch_bounds__(256) void k_xent_dkept(Xent p, const float* __restrict__ logits, int64_t ldl, int64_t v0,
-                                                    int64_t vc, int parts, const float* __restrict__ lse,
+                                                    int64_t vc, int parts, const float* __restrict__ stat,
                                                     const float* __restrict__ g, int g_stride,
                                                     const float* __restrict__ over, char* __restrict__ dl, int64_t ldd,
                                                     float* __restrict__ rest) {
@@ -596,8 +614,9 @@ __global__ __launch_bounds__(256) void k_xent_dkept(Xent p, const float* __restr
   const int32_t t = p.tgt[k];
   const int64_t row = p.act[k];
   const int at = t - (int)v0;
-  const float l = t >= 0 ? lse[row] : 0.f, part = over != nullptr ? *over : 1.f;
-  const float gr = t >= 0 ? g[row * g_stride] / part : 0.f;
+  const float part = over != nullptr ? *over : 1.f, gr = t >= 0 ? g[row * g_stride] / part : 0.f;
+  const float m = t >= 0 ? stat[STAT * row] : 0.f, gs = t >= 0 ? gr / stat[STAT * row + 1] : 0.f;
+  const float gt = t >= 0 ? gr * stat[STAT * row + 2] : 0.f;
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
     const int c = c0 + (r * 256 + (int)threadIdx.x) * V;
@@ -606,9 +625,8 @@ __global__ __launch_bounds__(256) void k_xent_dkept(Xent p, const float* __restr
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       const float y = z[r][e / 4][e % 4];
-      float q = fast_exp(y - l);
       const bool hit = at == c + e;
-      q = (hit ? q - 1.f : q) * gr;
+      float q = hit ? gt : fast_exp(y - m) * gs;
       if (CAP) q *= 1.f - y * p.inv_cap * (y * p.inv_cap);
       d[e] = t >= 0 && c + e < vc ? q : 0.f;
       if (DT == ODP_DTYPE_BF16 && hit && t >= 0) rest[k] = q - odp_round_bf16(q);
@@ -920,7 +938,7 @@ bool on16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 extern "C" int odp_xent_rows(odp_stream_t stream, int dtype, const void* x, int64_t ldx, int64_t n, int64_t cols,
                              int64_t width, const void* target, int target_bytes, int64_t vocab, int64_t ignore,
                              int keep, void* xc, int32_t* act, int32_t* tgt, int32_t* where, int32_t* count,
-                             float* losses, float* lse) {
+                             float* losses, float* stat) {
   if (int rc = check_xent("odp_xent_rows", dtype, n, width, width, vocab)) return rc;
   if (cols <= 0 || cols > width || ldx < cols || (target_bytes != 4 && target_bytes != 8)) {
     odp_set_error("odp_xent_rows: %lld columns of pitch %lld, targets of %d bytes", (long long)cols, (long long)ldx,
@@ -944,10 +962,10 @@ extern "C" int odp_xent_rows(odp_stream_t stream, int dtype, const void* x, int6
     return ODP_ERR_UNSUPPORTED;
   }
   const bool few = n > 0 && n <= XENT_FEW;
-  const Pick p{target, target_bytes == 8 ? 1 : 0, keep, n, vocab, ignore, act, tgt, where, count, losses, lse};
+  const Pick p{target, target_bytes == 8 ? 1 : 0, keep, n, vocab, ignore, act, tgt, where, count, losses, stat};
   if (!few)
     hipLaunchKernelGGL(k_xent_pick, dim3(1), dim3(1024), 0, s, target, p.wide, n, vocab, ignore, keep, act, tgt, where,
-                       count, losses, lse);
+                       count, losses, stat);
   if (blocks > 0) {
     const int vec = cols == width && on16(x) && ldx * es % 16 == 0;
 #define ODP_PACK(D, F) \
@@ -976,12 +994,12 @@ extern "C" int64_t odp_xent_kept(int dtype, int64_t n, int64_t width, int64_t vo
 
 extern "C" int odp_xent_losses(odp_stream_t stream, int dtype, const void* xc, int64_t n, int64_t width,
                                const int32_t* act, const int32_t* tgt, const int32_t* count, const void* w,
-                               int64_t ldw, int64_t vocab, float softcap, void* scratch, float* losses, float* lse,
+                               int64_t ldw, int64_t vocab, float softcap, void* scratch, float* losses, float* stat,
                                float* logits, int64_t ldl) {
   if (int rc = check_xent("odp_xent_losses", dtype, n, width, ldw, vocab)) return rc;
   if (n == 0) return ODP_OK;
   if (xc == nullptr || act == nullptr || tgt == nullptr || count == nullptr || w == nullptr || scratch == nullptr ||
-      losses == nullptr || lse == nullptr || !on16(xc) || !on16(w)) {
+      losses == nullptr || stat == nullptr || !on16(xc) || !on16(w)) {
     odp_set_error("odp_xent_losses: null pointer, or rows off the 16-byte grid");
     return ODP_ERR_INVALID_ARGUMENT;
   }
@@ -1002,10 +1020,10 @@ extern "C" int odp_xent_losses(odp_stream_t stream, int dtype, const void* xc, i
   ODP_XENT_LAUNCH_CAP(k_xent_stats, blocks, p, pmax, psum, ztgt, logits, ldl);
   if (kind == 1 || kind == 3)
     hipLaunchKernelGGL(k_xent_losses<1>, dim3((unsigned)n), dim3(256), 0, s, pmax, psum, ztgt, (int)tn, n, count, act,
-                       tgt, losses, lse);
+                       tgt, losses, stat);
   else
     hipLaunchKernelGGL(k_xent_losses<16>, dim3((unsigned)up(n, 16)), dim3(256), 0, s, pmax, psum, ztgt, (int)tn, n,
-                       count, act, tgt, losses, lse);
+                       count, act, tgt, losses, stat);
   return odp_check_launch("odp_xent_losses");
 }
 
@@ -1024,7 +1042,7 @@ extern "C" int64_t odp_xent_pitch(int dtype, int64_t columns) {
 
 extern "C" int odp_xent_dlogits(odp_stream_t stream, int dtype, const void* xc, int64_t n, int64_t width,
                                 const int32_t* act, const int32_t* tgt, const int32_t* count, const void* w,
-                                int64_t ldw, int64_t vocab, float softcap, int64_t v0, int64_t vc, const float* lse,
+                                int64_t ldw, int64_t vocab, float softcap, int64_t v0, int64_t vc, const float* stat,
                                 const float* g, int g_stride, const float* over, const float* logits, int64_t ldl,
                                 void* dl, int64_t ldd, float* rest) {
   if (int rc = check_xent("odp_xent_dlogits", dtype, n, width, ldw, vocab)) return rc;
@@ -1034,7 +1052,7 @@ extern "C" int odp_xent_dlogits(odp_stream_t stream, int dtype, const void* xc, 
     return ODP_ERR_INVALID_ARGUMENT;
   }
   if (n == 0) return ODP_OK;
-  if (xc == nullptr || act == nullptr || tgt == nullptr || count == nullptr || w == nullptr || lse == nullptr ||
+  if (xc == nullptr || act == nullptr || tgt == nullptr || count == nullptr || w == nullptr || stat == nullptr ||
       g == nullptr || dl == nullptr || rest == nullptr || !on16(xc) || !on16(w) || !on16(dl)) {
     odp_set_error("odp_xent_dlogits: null pointer, or rows off the 16-byte grid");
     return ODP_ERR_INVALID_ARGUMENT;
@@ -1051,7 +1069,7 @@ extern "C" int odp_xent_dlogits(odp_stream_t stream, int dtype, const void* xc, 
     }
     const Xent p = xent_of(nullptr, nullptr, 0, vocab, width, n, count, act, tgt, softcap);
 #define ODP_KEPT(D, C)                                                                                                 \
-  ODP_XENT_GO((k_xent_dkept<D, C>), 256, (unsigned)(n * parts), p, logits, ldl, v0, vc, (int)parts, lse, g, g_stride,  \
+  ODP_XENT_GO((k_xent_dkept<D, C>), 256, (unsigned)(n * parts), p, logits, ldl, v0, vc, (int)parts, stat, g, g_stride,  \
               over, (char*)dl, ldd, rest)
     if (dtype == ODP_DTYPE_F32) {
       if (softcap != 0.f) ODP_KEPT(ODP_DTYPE_F32, true); else ODP_KEPT(ODP_DTYPE_F32, false);
@@ -1067,7 +1085,7 @@ extern "C" int odp_xent_dlogits(odp_stream_t stream, int dtype, const void* xc, 
                        false, blocks))
     return rc;
   const Xent p = xent_of(xc, w, ldw, vocab, width, n, count, act, tgt, softcap);
-  ODP_XENT_LAUNCH_CAP(k_xent_dlogits, blocks, p, v0, vc, lse, g, g_stride, over, dl, ldd, rest);
+  ODP_XENT_LAUNCH_CAP(k_xent_dlogits, blocks, p, v0, vc, stat, g, g_stride, over, dl, ldd, rest);
   return odp_check_launch("odp_xent_dlogits");
 }
 

@@ -276,6 +276,7 @@ _HEAD_DTYPES = (torch.float32, torch.bfloat16)
 # holds at a time: a piece of the vocabulary for all tokens.
 PIECE_BYTES = 512 << 20
 _PIECE_COLUMNS = 1 << 22  # a piece's columns stay below it (ODP_XENT_PIECE)
+_STAT = 3  # float32 words that the forward leaves of a row for the backward (ODP_XENT_STAT)
 # Bytes of float32 logits up to which a call that wants gradients keeps them
 # for its backward (1.5 % of the memory of one GPU) where that is faster than
 # forming them again; 0 keeps none.  Neither do the gradients of torch.func
@@ -322,7 +323,7 @@ class _Packed:
     """The rows that bear a loss, gathered (every row with ``keep``)."""
 
     def __init__(self, x: torch.Tensor, w: torch.Tensor, target: torch.Tensor, ignore: int, keep: bool = False,
-                 losses: torch.Tensor | None = None, lse: torch.Tensor | None = None) -> None:
+                 losses: torch.Tensor | None = None, stat: torch.Tensor | None = None) -> None:
         rows, flat = pitched_rows(x.detach()), target.contiguous()
         self.dt, self.n, self.cols = dtype_code(x.dtype), flat.numel(), rows.shape[1]
         self.w, self.vocab, self.width = w, w.shape[0], w.shape[1]
@@ -335,14 +336,14 @@ class _Packed:
         _call("odp_xent_rows", _stream(x), self.dt, rows.data_ptr(), rows.stride(0), self.n, self.cols, self.width,
               flat.data_ptr(), flat.element_size(), self.vocab, ignore, int(keep), self.xc.data_ptr(), self.act,
               self.tgt, self.where, self.count, None if losses is None else losses.data_ptr(),
-              None if lse is None else lse.data_ptr())
+              None if stat is None else stat.data_ptr())
 
-    def losses(self, softcap: float, losses: torch.Tensor, lse: torch.Tensor) -> None:
+    def losses(self, softcap: float, losses: torch.Tensor, stat: torch.Tensor) -> None:
         scratch = torch.empty(_xent_words(self.dt, self.n, self.width, self.vocab)[0], dtype=torch.float32,
                               device=self.xc.device)
         _call("odp_xent_losses", _stream(self.xc), self.dt, self.xc.data_ptr(), self.n, self.width, self.act,
               self.tgt, self.count, self.w.data_ptr(), self.w.stride(0), self.vocab, softcap, scratch.data_ptr(),
-              losses.data_ptr(), lse.data_ptr(), None, 0)
+              losses.data_ptr(), stat.data_ptr(), None, 0)
 
     def piece(self, whole: bool = False) -> int:
         """Columns of the vocabulary a piece of d holds: as many pieces as PIECE_BYTES makes, of one size."""
@@ -352,7 +353,7 @@ class _Packed:
         pieces = -(-self.vocab // fit)
         return self.vocab if whole else min(self.vocab, -(-(-(-self.vocab // pieces)) // edge) * edge)
 
-    def gradients(self, softcap: float, lse: torch.Tensor, g: torch.Tensor, x_shape: torch.Size | None,
+    def gradients(self, softcap: float, stat: torch.Tensor, g: torch.Tensor, x_shape: torch.Size | None,
                   need_w: bool, keep_d: bool = False):
         """(dx, dW, d): dx where ``x_shape`` is given; d [n, vocab] where
         ``keep_d`` (packed with ``keep``).  ``g`` holds one gradient per row."""
@@ -372,7 +373,7 @@ class _Packed:
             vc = min(piece, self.vocab - v0)
             ldd = _xent_pitch(dt, vc)
             _call("odp_xent_dlogits", s, dt, xc, self.n, self.width, self.act, self.tgt, self.count, w, ldw,
-                  self.vocab, softcap, v0, vc, lse.data_ptr(), g.data_ptr(), 1, None, None, 0, d.data_ptr(),
+                  self.vocab, softcap, v0, vc, stat.data_ptr(), g.data_ptr(), 1, None, None, 0, d.data_ptr(),
                   ldd, rest.data_ptr())
             if dx is not None:
                 _call("odp_xent_dx", s, dt, self.n, self.width, self.count, w, ldw, self.vocab, v0, vc, piece,
@@ -391,18 +392,18 @@ class _Packed:
 
 def _xent_losses(x, weight, target, softcap, ignore):
     losses = torch.empty(target.shape, dtype=torch.float32, device=x.device)
-    lse = torch.empty_like(losses)
+    stat = torch.empty((*target.shape, _STAT), dtype=torch.float32, device=x.device)
     with _OnDevice(x):
-        p = _Packed(x, _head_rows(weight), target, ignore, False, losses, lse)
-        p.losses(softcap, losses, lse)
-    return losses, lse
+        p = _Packed(x, _head_rows(weight), target, ignore, False, losses, stat)
+        p.losses(softcap, losses, stat)
+    return losses, stat
 
 
-def _xent_gradients(g, x, weight, target, lse, softcap, ignore, need_x, need_w, keep_d=False):
-    g, lse = g.detach().float().contiguous().reshape(-1), lse.contiguous()
+def _xent_gradients(g, x, weight, target, stat, softcap, ignore, need_x, need_w, keep_d=False):
+    g, stat = g.detach().float().contiguous().reshape(-1), stat.contiguous()
     with _OnDevice(x):
         p = _Packed(x, _head_rows(weight), target, ignore, keep_d)
-        return p.gradients(softcap, lse, g, x.shape if need_x else None, need_w, keep_d)
+        return p.gradients(softcap, stat, g, x.shape if need_x else None, need_w, keep_d)
 
 
 class _XentGrad(torch.autograd.Function):
@@ -411,8 +412,8 @@ class _XentGrad(torch.autograd.Function):
     generate_vmap_rule = False
 
     @staticmethod
-    def forward(g, x, weight, target, lse, softcap, ignore, need_x, need_w):
-        dx, dw, _ = _xent_gradients(g, x, weight, target, lse, softcap, ignore, need_x, need_w)
+    def forward(g, x, weight, target, stat, softcap, ignore, need_x, need_w):
+        dx, dw, _ = _xent_gradients(g, x, weight, target, stat, softcap, ignore, need_x, need_w)
         return dx, dw
 
     @staticmethod
@@ -424,20 +425,20 @@ class _XentGrad(torch.autograd.Function):
         raise NotImplementedError("linear_cross_entropy has no second derivative here")
 
     @staticmethod
-    def vmap(info, in_dims, g, x, weight, target, lse, softcap, ignore, need_x, need_w):
+    def vmap(info, in_dims, g, x, weight, target, stat, softcap, ignore, need_x, need_w):
         n = info.batch_size
-        g, x, target, lse = (_front(t, d, n) for t, d in zip((g, x, target, lse), (*in_dims[:2], *in_dims[3:5])))
+        g, x, target, stat = (_front(t, d, n) for t, d in zip((g, x, target, stat), (*in_dims[:2], *in_dims[3:5])))
         if in_dims[2] is None and not need_w:  # one head: the batch is one set of rows
-            return _XentGrad.apply(g, x, weight, target, lse, softcap, ignore, need_x, need_w), (0, None)
+            return _XentGrad.apply(g, x, weight, target, stat, softcap, ignore, need_x, need_w), (0, None)
         w = _front(weight, in_dims[2], n)
-        out = [_XentGrad.apply(g[i], x[i], w[i], target[i], lse[i], softcap, ignore, need_x, need_w)
+        out = [_XentGrad.apply(g[i], x[i], w[i], target[i], stat[i], softcap, ignore, need_x, need_w)
                for i in range(n)]
         return (torch.stack([o[0] for o in out]) if need_x else None,
                 torch.stack([o[1] for o in out]) if need_w else None), (0 if need_x else None, 0 if need_w else None)
 
 
 class _Xent(torch.autograd.Function):
-    """Token losses [*target.shape] and their log-sum-exp; merges the batch
+    """Token losses [*target.shape] and their rows' statistics; merges the batch
     under vmap and, in a capture pass, records x and the logits' gradient of
     an eligible head."""
 
@@ -455,9 +456,9 @@ class _Xent(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g, _):
-        x, weight, target, lse = ctx.saved_tensors
+        x, weight, target, stat = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[:2]
-        dx, dw = _XentGrad.apply(g, x, weight, target, lse, ctx.softcap, ctx.ignore, need_x, need_w)
+        dx, dw = _XentGrad.apply(g, x, weight, target, stat, ctx.softcap, ctx.ignore, need_x, need_w)
         return dx, dw, None, None, None
 
     @staticmethod
@@ -498,8 +499,8 @@ class _TapXent(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g, _):
-        x, weight, target, lse = ctx.saved_tensors
-        dx, _, d = _xent_gradients(g, x, weight, target, lse, ctx.softcap, ctx.ignore, ctx.needs_input_grad[0],
+        x, weight, target, stat = ctx.saved_tensors
+        dx, _, d = _xent_gradients(g, x, weight, target, stat, ctx.softcap, ctx.ignore, ctx.needs_input_grad[0],
                                    False, keep_d=True)
         ctx.record.g = d[: target.numel()].unflatten(0, target.shape) if target.dim() > 1 else d
         return dx, None, None, None, None, torch.zeros((), dtype=torch.float32, device=g.device), None

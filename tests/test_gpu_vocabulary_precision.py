@@ -89,3 +89,47 @@ def test_softcaps_at_the_ends(cap):
     want, bound = capped(x8, w8, y, torch.ones(4), cap, torch.float32)
     for a, b, c in zip(run(x8, w8, y, torch.ones(4), cap), want, bound):
         assert torch.isfinite(a).all() and ((a.double() - b).abs() <= c).all()
+
+
+@pytest.mark.parametrize("kept", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("helper", [True, False])
+def test_nearly_certain_tokens_keep_their_gradients_bits(dtype, kept, helper, monkeypatch):
+    """Tokens of 1 - p(target) from 1e-6 to 1e-1 whose logits are around 500: the target's d = -(1 - p) is off by the
+    logits' error times 1 - p and by the roundings of a sum of exponentials near 1 (30 of them), not by the last place
+    of the log-sum-exp (1.5e-5)."""
+    width, vocab, n = 136, 500, 40
+    g = torch.Generator().manual_seed(3)
+    w = torch.randn(vocab, width, generator=g) / math.sqrt(width)
+    w[:, 0] = 1.0
+    y = torch.arange(0, vocab, 13)[:n]
+    n = y.numel()
+    x = w[y] * torch.linspace(10.0, 22.0, n).unsqueeze(1)
+    x[:, 0] = 500.0
+    x, w, gl = x.to(dtype), w.to(dtype), torch.linspace(0.5, 2.0, n)
+    if not kept:
+        monkeypatch.setattr(vocabulary, "KEEP_BYTES", 0)
+    if not helper:
+        monkeypatch.setattr(vocabulary, "_host_ready", [None])
+    loss, dx, dw = run(x, w, y, gl)
+    xd, wd, gd, at = x.double().to(DEV), w.double().to(DEV), gl.double().to(DEV).unsqueeze(1), (torch.arange(n), y)
+    z = xd @ wd.t()
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    Z = (2 * width * U32 * (xd.abs() @ wd.abs().t())).max(1, keepdim=True).values
+    p = torch.exp(z - lse)
+    rest = p.clone()
+    rest[at] = 0.0
+    share = rest.sum(1)  # 1 - p(target), to float64's relative precision
+    assert 1e-7 < float(share.min()) < 1e-5 and float(share.max()) > 1e-2
+    q = p.clone()
+    q[at] = -share
+    dq = p * (2 * Z + (8 + (z - lse).abs()) * 2.0**-22 + 30 * U32)
+    dq[at] = share * (2 * Z.squeeze(1) + 48 * 2.0**-22) + 34 * U32
+    assert ((loss.double() + torch.log1p(-share)).abs() <= dq[at] / (1 - share)).all()
+    d, dd = gd * q, gd * dq * 1.01
+    rounding = HALF_ULP[dtype] * d.abs()
+    bw = (dd + rounding).t() @ xd.abs() + 2 * n * U32 * (d.abs().t() @ xd.abs()) + HALF_ULP[dtype] * 1.02 * (d.t() @ xd).abs() + LEAST
+    rounding[at] = 2 * U32 * d[at].abs()  # dx takes the target's entry in float32
+    bx = (dd + rounding) @ wd.abs() + 2 * (vocab + 8) * U32 * (d.abs() @ wd.abs()) + HALF_ULP[dtype] * 1.02 * (d @ wd).abs() + LEAST
+    assert ((dx.double() - d @ wd).abs() <= bx).all()
+    assert ((dw.double() - d.t() @ xd).abs() <= bw).all()
