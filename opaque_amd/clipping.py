@@ -692,8 +692,6 @@ class _ClipEngine:
                 w = leaves[obj_leaf[id(r.w_obj)]]
                 if r.g is None:
                     r.g = torch.zeros(*r.tokens.shape, w.shape[1], dtype=w.dtype, device=w.device)
-                t_rows = r.tokens[0].numel()
-                rows_per_ex[t_rows] = rows_per_ex.get(t_rows, 0) + 1
                 continue
             if r.g is None:
                 d_out = r.w_obj.shape[-2] if r.w_obj is not None else r.B.shape[1]
@@ -702,7 +700,17 @@ class _ClipEngine:
                 continue  # MoE experts bring their own rows
             t_rows = r.x[0].numel() // r.x.shape[-1] if r.x.dim() > 1 else 1
             rows_per_ex[t_rows] = rows_per_ex.get(t_rows, 0) + 1
-        seq = max(rows_per_ex, key=rows_per_ex.get) if rows_per_ex else 1
+        # The plan's segments hold the commonest row count of the linear seams;
+        # full-weight and table seams of another bring their own.
+        seq = max(rows_per_ex, key=rows_per_ex.get) if rows_per_ex else \
+            next((r.tokens[0].numel() for r in recs if r.tokens is not None), 1)
+        own: dict[int, Segments | None] = {seq: None}
+
+        def segments_of(rows: int) -> Segments | None:
+            if rows not in own:
+                own[rows] = Segments.padded(n, rows)
+            return own[rows]
+
         lins: list[LinearSite] = []
         embeds: list[EmbeddingSite] = []
         stacked: dict[int, torch.Tensor] = {}
@@ -711,9 +719,9 @@ class _ClipEngine:
                 kw = obj_leaf[id(r.w_obj)]
                 # The site sums in float32: a float64 sum asked for is made from
                 # the per-example gradients.
-                if r.tokens[0].numel() == seq and r.tokens.shape[0] == n and self.compute_dtype != torch.float64:
+                if r.tokens.shape[0] == n and self.compute_dtype != torch.float64:
                     embeds.append(EmbeddingSite(tokens=r.tokens, g=r.g, w_leaf=kw, scale=r.scaling,
-                                                padding=r.padding))
+                                                padding=r.padding, segments=segments_of(r.tokens[0].numel())))
                 else:
                     mats.append(MaterializedLeaf(per_example=_table_per_example(r, leaves[kw], n), leaf=kw))
                 continue
@@ -728,11 +736,11 @@ class _ClipEngine:
                 continue
             if r.w_obj is not None:
                 kw = obj_leaf[id(r.w_obj)]
-                t_rows = r.x[0].numel() // r.x.shape[-1]
-                if (t_rows == seq and r.x.shape[0] == n
+                if (r.x.shape[0] == n and r.x.numel()
                         and r.x.dtype == r.g.dtype == leaves[kw].dtype == torch.bfloat16
                         and supports_rows(r.x) and supports_rows(r.g)):
-                    lins.append(LinearSite(x=r.x, g=r.g, w_leaf=kw))
+                    lins.append(LinearSite(x=r.x, g=r.g, w_leaf=kw,
+                                           segments=segments_of(r.x[0].numel() // r.x.shape[-1])))
                 else:
                     for k, pe in _site_per_example(r, None, None, leaves, kw):
                         mats.append(MaterializedLeaf(per_example=pe.reshape(n, -1), leaf=k))

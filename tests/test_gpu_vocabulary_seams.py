@@ -10,6 +10,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from opaque_amd import capture
 from opaque_amd.clipping import clipped_grad
 from opaque_amd.vocabulary import embedding, linear_cross_entropy
 from oracle import dp_ref
@@ -46,11 +47,13 @@ def compare(make, params, batch, *, tol, steps=2, clipping_norm=0.7, **kw):
 
 
 class OPS:
+    linear = staticmethod(capture.linear)
     embedding = staticmethod(embedding)
     loss = staticmethod(lambda h, w, t: linear_cross_entropy(h, w, t))
 
 
 class PLAIN:
+    linear = staticmethod(torch.nn.functional.linear)
     embedding = staticmethod(plain_embedding)
     loss = staticmethod(plain_loss)
 
@@ -82,3 +85,54 @@ def test_a_table_tied_to_a_head_made_from_it(made, which):
         return loss
 
     compare(make, params, (y, t), tol=1e-5)
+
+
+def seams_of(engine):
+    """(embedding sites, full-weight sites, whether a leaf is materialised) of the engine's last plan."""
+    plan = engine._plan
+    return (len(plan._embeds), sum(1 for k in plan._ext_keys if k[0] == "linx"),
+            "sqnorm" in {i[0] for i in plan.launch_info})
+
+
+@pytest.mark.parametrize("microbatch", [None, 2])
+def test_seams_of_different_row_counts(microbatch):
+    """More hidden rows than tokens (a prefix before them), the loss over the tokens' rows: each seam brings its rows."""
+    g = torch.Generator().manual_seed(21)
+    n, T, pre, vocab, width = 5, 13, 4, 72, 32
+    params = {"table": torch.randn(vocab, width, generator=g), "mid": torch.randn(width, width, generator=g) / 5,
+              "head": torch.randn(vocab, width, generator=g) / 5}
+    params = {k: v.bfloat16() for k, v in params.items()}
+    prefix = torch.randn(pre, width, generator=g).bfloat16()
+    y, t = torch.randint(0, vocab, (n, T), generator=g), torch.randint(0, vocab, (n, T), generator=g)
+
+    def make(ops):
+        def loss(p, yi, ti):
+            h = ops.embedding(yi, p["table"])
+            h = torch.cat([prefix.to(h.device, h.dtype), h])
+            h = h + torch.tanh(ops.linear(h, p["mid"]))
+            h = torch.cat([h[pre:], h[:pre].sum(0, keepdim=True)])[:T]
+            return ops.loss(h, p["head"], ti)
+
+        return loss
+
+    engine = compare(make, params, (y, t), tol=2e-2, microbatch_size=microbatch)
+    assert seams_of(engine) == (1, 2, False)
+
+
+def test_a_pooled_head_beside_a_lookup():
+    """One lookup of T rows and one linear of one row an example: both are seams, whichever comes first."""
+    g = torch.Generator().manual_seed(22)
+    n, T, vocab, width, classes = 6, 11, 60, 24, 16
+    params = {"table": torch.randn(vocab, width, generator=g).bfloat16(),
+              "head": (torch.randn(classes, width, generator=g) / 5).bfloat16()}
+    y, c = torch.randint(0, vocab, (n, T), generator=g), torch.randint(0, classes, (n,), generator=g)
+
+    def make(ops):
+        def loss(p, yi, ci):
+            z = ops.linear(torch.tanh(ops.embedding(yi, p["table"])).mean(0), p["head"])
+            z = z.to(torch.promote_types(z.dtype, torch.float32))
+            return torch.logsumexp(z, -1) - z.gather(-1, ci.unsqueeze(-1)).squeeze(-1)
+
+        return loss
+
+    assert seams_of(compare(make, params, (y, c), tol=2e-2)) == (1, 1, False)
