@@ -68,6 +68,7 @@ class CaptureSession:
     linear_ws: list[int] = field(default_factory=list)  # ids of weights of full-weight linear seams
     eligible: set[int] = field(default_factory=set)  # ids allowed to be captured
     params: set[int] = field(default_factory=set)  # discover: ids of the differentiated leaves
+    zero: torch.Tensor | None = None  # capture: an int64 zero that carries the batch (one per example)
 
     def hide(self, t: torch.Tensor) -> torch.Tensor:
         """Books a seam use of ``t`` and keeps it out of autograd where it is a
@@ -78,6 +79,13 @@ class CaptureSession:
             return t
         self.uses[id(t)] = self.uses.get(id(t), 0) + 1
         return t.detach()
+
+    def batched(self, tokens: torch.Tensor) -> torch.Tensor:
+        """``tokens`` with the batch on them: torch calls no vmap rule for an
+        op none of whose inputs is batched (a lookup of learned positions)."""
+        if self.zero is None or torch._C._functorch.is_batchedtensor(tokens):
+            return tokens
+        return tokens + self.zero.to(tokens.dtype)
 
     def derived(self, *ts: torch.Tensor | None) -> bool:
         """Whether any of the tensors was made from a differentiated leaf."""

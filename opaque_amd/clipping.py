@@ -659,11 +659,14 @@ class _ClipEngine:
         obj_leaf = {id(leaves[k]): k for k in disc.eligible}
         sess = CaptureSession(mode="capture", anchor=anchor, eligible=set(obj_leaf))
 
-        def per_example(*a):
+        def per_example(zero, *a):
+            sess.zero = zero
             return self._loss(*a, **kwargs)
 
+        zeros = torch.zeros(n, dtype=torch.int64, device=device)
         with torch.enable_grad(), sess:
-            values, loss_aux = torch.func.vmap(per_example, in_dims=in_dims, randomness="same")(*cargs)
+            values, loss_aux = torch.func.vmap(per_example, in_dims=(0, *in_dims), randomness="same")(zeros, *cargs)
+        sess.zero = None
         recs = sess.sites
         seen: dict[int, int] = {}
         want = dict.fromkeys(disc.eligible, 1)

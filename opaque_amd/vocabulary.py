@@ -249,6 +249,8 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
     sess = active_session()
     if sess is not None and sess.mode == "discover":
         weight = sess.hide(weight)
+    elif sess is not None and id(weight) in sess.eligible:
+        tokens = sess.batched(tokens)
     host = None if _transformed() else _bound()
     if host is not None:
         return host.embedding(tokens, weight, scale, padding)

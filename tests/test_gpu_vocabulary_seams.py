@@ -136,3 +136,39 @@ def test_a_pooled_head_beside_a_lookup():
         return loss
 
     assert seams_of(compare(make, params, (y, c), tol=2e-2)) == (1, 1, False)
+
+
+@pytest.mark.parametrize("kind", [torch.int64, torch.int32], ids=str)
+def test_learned_positions_stay_seams(kind):
+    """A table read at positions that are the same for every example (not batched under vmap) is a seam, as are the
+    model's others, on every step."""
+    g = torch.Generator().manual_seed(23)
+    n, T, vocab, width = 4, 10, 48, 24
+    params = {"wte": torch.randn(vocab, width, generator=g), "wpe": torch.randn(16, width, generator=g),
+              "mid": torch.randn(width, width, generator=g) / 4, "head": torch.randn(vocab, width, generator=g) / 4}
+    params = {k: v.bfloat16() for k, v in params.items()}
+    y, t = torch.randint(0, vocab, (n, T), generator=g), torch.randint(0, vocab, (n, T), generator=g)
+
+    def make(ops):
+        def loss(p, yi, ti):
+            at = torch.arange(T, device=p["wpe"].device).to(kind)
+            h = ops.embedding(yi, p["wte"]) + ops.embedding(at, p["wpe"])
+            return ops.loss(torch.tanh(ops.linear(h, p["mid"])), p["head"], ti)
+
+        return loss
+
+    engine = compare(make, params, (y, t), tol=2e-2, steps=3)
+    assert seams_of(engine) == (2, 2, False)
+    assert engine._discovery is not None and engine.last_rebound
+
+
+def test_positions_alone():
+    """The only table is read at positions: a vector per example, of one row."""
+    g = torch.Generator().manual_seed(24)
+    params = {"wpe": torch.randn(5, 8, generator=g)}
+    x = torch.randn(3, 8, generator=g)
+
+    def make(ops):
+        return lambda p, xi: (ops.embedding(torch.tensor(2, device=xi.device), p["wpe"]) * xi).sum().sin()
+
+    assert seams_of(compare(make, params, (x,), tol=1e-5, clipping_norm=10.0)) == (1, 0, False)
