@@ -247,13 +247,10 @@ struct Xent : torch::autograd::Function<Xent> {
                             int64_t reduction, int64_t piece_bytes, int64_t keep_bytes) {
     const c10::OptionalDeviceGuard guard(x.device());
     const Packed p = xent_forward(x, weight, target, stat, softcap, ignore, keep_bytes);
-    // A later change of the head in place is an error; the kept logits go when the backward pass is through.
-    ctx->save_for_backward({weight, p.logits});
+    // Saved as autograd's own are: a later change of the head in place is an error (where it was not copied), hooks
+    // see every tensor, and all go when the backward pass is through.
+    ctx->save_for_backward({p.w, p.xc, p.ids, p.stat, p.logits});
     auto& d = ctx->saved_data;
-    d["w"] = p.w;
-    d["xc"] = p.xc;
-    d["ids"] = p.ids;
-    d["stat"] = p.stat;
     d["n"] = p.n;
     d["cols"] = p.cols;
     d["softcap"] = softcap;
@@ -271,16 +268,16 @@ struct Xent : torch::autograd::Function<Xent> {
       at::NoGradGuard no_grad;
       auto& sd = ctx->saved_data;
       Packed p;
-      p.w = sd["w"].toTensor();
-      p.xc = sd["xc"].toTensor();
-      p.ids = sd["ids"].toTensor();
-      p.logits = saved[1];
+      p.w = saved[0];
+      p.xc = saved[1];
+      p.ids = saved[2];
+      p.logits = saved[4];
       p.n = sd["n"].toInt();
       p.cols = sd["cols"].toInt();
       p.width = p.w.size(1);
       p.vocab = p.w.size(0);
       p.dt = code_of(p.xc);
-      const at::Tensor stat = sd["stat"].toTensor();
+      const at::Tensor stat = saved[3];
       const float softcap = (float)sd["softcap"].toDouble();
       const c10::OptionalDeviceGuard guard(p.xc.device());
       const at::Tensor g = grads[0].contiguous();

@@ -6,6 +6,7 @@ import math
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from opaque_amd import vocabulary
 from opaque_amd.vocabulary import embedding, linear_cross_entropy
@@ -70,3 +71,85 @@ def test_a_second_derivative_of_the_lookup(route):
     (dw,) = torch.autograd.grad(embedding(y, w), [w], go, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(dw.sum(), [go])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("kept", [True, False])
+def test_a_head_that_trains_where_x_does_not(route, dtype, kept, monkeypatch):
+    """Each gradient alone has the bits that both together have."""
+    if not kept:
+        monkeypatch.setattr(vocabulary, "KEEP_BYTES", 0)
+    x, w, y = inputs(60, 136, 700, dtype)
+    both = torch.autograd.grad(linear_cross_entropy(x.requires_grad_(), w.requires_grad_(), y), [x, w])
+    (dw,) = torch.autograd.grad(linear_cross_entropy(x.detach(), w, y), [w])
+    (dx,) = torch.autograd.grad(linear_cross_entropy(x, w.detach(), y), [x])
+    assert torch.equal(dx, both[0]) and torch.equal(dw, both[1])
+
+
+@pytest.mark.parametrize("trained", ["x", "xw"])
+def test_saved_tensors_go_through_autograds_hooks(trained):
+    """What the backward needs is offered to saved-tensor hooks (offloading), rows and head among it, and comes back
+    from them."""
+    x, w, y = inputs(60, 136, 700)
+    x.requires_grad_(), w.requires_grad_("w" in trained)
+    wanted = [t for t in (x, w) if t.requires_grad]
+    want = torch.autograd.grad(linear_cross_entropy(x, w, y), wanted)
+    packed = []
+
+    def pack(t):
+        packed.append(tuple(t.shape))
+        return t.cpu()
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t.to(DEV)):
+        loss = linear_cross_entropy(x, w, y)
+    assert packed.count((60, 136)) == packed.count((700, 136)) == 1
+    for a, b in zip(torch.autograd.grad(loss, wanted), want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("use_reentrant", [True, False])
+def test_under_checkpointing(use_reentrant):
+    x, w, y = inputs(60, 136, 700)
+    x.requires_grad_(), w.requires_grad_()
+    want = torch.autograd.grad(linear_cross_entropy(torch.tanh(x), w, y), [x, w])
+    loss = torch.utils.checkpoint.checkpoint(lambda a, b: linear_cross_entropy(torch.tanh(a), b, y), x, w,
+                                             use_reentrant=use_reentrant)
+    loss.backward()
+    assert torch.equal(x.grad, want[0]) and torch.equal(w.grad, want[1])
+
+
+def test_nothing_is_held_after_the_backward():
+    """The packed rows go with the kept logits when the backward is through, while the loss itself is still held."""
+    n, width, vocab = 2048, 1024, 4096
+    x, w, y = inputs(n, width, vocab, torch.bfloat16)
+    x.requires_grad_()
+
+    def held():
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        loss = linear_cross_entropy(x, w, y)
+        mid = torch.cuda.memory_allocated() - before
+        loss.backward()
+        x.grad = None
+        return mid, torch.cuda.memory_allocated() - before, loss
+
+    held()
+    mid, after, loss = held()
+    assert mid >= 4 * n * vocab + 2 * n * width and after < 2 * n * width // 4
+
+
+def test_a_checkpointed_loss_holds_nothing():
+    """Non-reentrant checkpointing drops what the forward saved, the packed rows too."""
+    n, width, vocab = 2048, 1024, 4096
+    x, w, y = inputs(n, width, vocab, torch.bfloat16)
+    x.requires_grad_()
+
+    def held():
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        loss = torch.utils.checkpoint.checkpoint(lambda a: linear_cross_entropy(a, w, y), x, use_reentrant=False)
+        return torch.cuda.memory_allocated() - before, loss
+
+    held()
+    mid, loss = held()
+    assert mid < 2 * n * width // 4
