@@ -265,6 +265,16 @@ class Embedding(torch.nn.Embedding):
         super().__init__(num_embeddings, embedding_dim, padding_idx, device=device, dtype=dtype)
         self.scale = scale
 
+    @classmethod
+    def from_pretrained(cls, embeddings: torch.Tensor, freeze: bool = True, padding_idx: int | None = None, *,
+                        scale: float = 1.0) -> Embedding:
+        """A module on a given table (shared, not copied), frozen unless told otherwise."""
+        if embeddings.dim() != 2:
+            raise ValueError(f"embeddings must be [vocabulary, width], got {tuple(embeddings.shape)}")
+        m = cls(*embeddings.shape, padding_idx, scale=scale, device="meta", dtype=embeddings.dtype)
+        m.weight = torch.nn.Parameter(embeddings, requires_grad=not freeze)
+        return m
+
     def forward(self, tokens: torch.Tensor) -> torch.Tensor:
         return embedding(tokens, self.weight, scale=self.scale, padding_idx=self.padding_idx)
 
