@@ -20,6 +20,8 @@
 // 32768 tokens of a 128256 x 4096 bfloat16 table, lookup and gradient: 340 us
 // for 1.86 GB (5.5 TB/s; a copy runs at 5.2).  A clip step's norms and sum over
 // 16384 of them: 285 us for 1.19 GB, 1.05 GB of it the table's zeros.
+#include <cmath>
+
 #include "odp_internal.h"
 
 namespace {
@@ -845,6 +847,12 @@ int check_rows(const char* what, int dtype, int64_t n, int64_t width, int64_t vo
   return ODP_OK;
 }
 
+int check_scale(const char* what, float scale) {
+  if (std::isfinite(scale)) return ODP_OK;
+  odp_set_error("%s: scale %g", what, (double)scale);
+  return ODP_ERR_INVALID_ARGUMENT;
+}
+
 int check_grid(const char* what, int64_t blocks) {
   if (blocks >= (int64_t)1 << 24) {
     odp_set_error("%s: the launch needs %lld workgroups", what, (long long)blocks);
@@ -896,6 +904,7 @@ int launch_zero(const char* what, hipStream_t s, void* out, int64_t bytes) {
 extern "C" int odp_embed_rows(odp_stream_t stream, int dtype, const void* tokens, int token_bytes, int64_t n,
                               const void* weight, int64_t ldw, int64_t vocab, int64_t width, float scale, void* out) {
   if (int rc = check_rows("odp_embed_rows", dtype, n, width, vocab, ldw)) return rc;
+  if (int rc = check_scale("odp_embed_rows", scale)) return rc;
   if (token_bytes != 4 && token_bytes != 8) {
     odp_set_error("odp_embed_rows: tokens of %d bytes", token_bytes);
     return ODP_ERR_UNSUPPORTED;
@@ -1001,6 +1010,7 @@ extern "C" int odp_embed_grad(odp_stream_t stream, int dtype, const void* g, int
                               const uint32_t* keys, const uint32_t* rows, int64_t vocab, float scale, void* scratch,
                               void* out) {
   if (int rc = check_rows("odp_embed_grad", dtype, n, width, vocab, ldg)) return rc;
+  if (int rc = check_scale("odp_embed_grad", scale)) return rc;
   if (out == nullptr || (n > 0 && (g == nullptr || keys == nullptr || rows == nullptr || scratch == nullptr))) {
     odp_set_error("odp_embed_grad: null pointer");
     return ODP_ERR_INVALID_ARGUMENT;
@@ -1030,6 +1040,7 @@ extern "C" int odp_embed_sqnorm(odp_stream_t stream, int dtype, const void* g, i
                                 float scale, const int32_t* seg_row_start, const int32_t* seg_example, void* scratch,
                                 float* whole, double* part, int64_t part_stride, int64_t slot, int64_t* nf_flag) {
   if (int rc = check_rows("odp_embed_sqnorm", dtype, n, width, vocab, ldg)) return rc;
+  if (int rc = check_scale("odp_embed_sqnorm", scale)) return rc;
   if (n == 0) return ODP_OK;
   if (g == nullptr || keys == nullptr || rows == nullptr || seg_of == nullptr || seg_row_start == nullptr ||
       seg_example == nullptr || scratch == nullptr || whole == nullptr || part == nullptr || nf_flag == nullptr ||
@@ -1066,6 +1077,7 @@ extern "C" int odp_embed_clipped_sum(odp_stream_t stream, int dtype, const void*
                                      void* scratch, const float* whole, const double* scales, float normalize_by,
                                      int out_dtype, void* out, void* out2) {
   if (int rc = check_rows("odp_embed_clipped_sum", dtype, n, width, vocab, ldg)) return rc;
+  if (int rc = check_scale("odp_embed_clipped_sum", scale)) return rc;
   if (out_dtype < ODP_DTYPE_F32 || out_dtype > ODP_DTYPE_F64) {
     odp_set_error("odp_embed_clipped_sum: out_dtype %d", out_dtype);
     return ODP_ERR_UNSUPPORTED;

@@ -28,6 +28,8 @@
 // entry, often the row's only large one, is added to dx in float32
 // (k_xent_dx_rows): alone it would leave a row of dx as far off as that entry.
 // A row of dW adds many tokens' entries, whose roundings average out.
+#include <cfloat>
+
 #include "odp_internal.h"
 
 namespace {
@@ -841,6 +843,12 @@ int check_xent(const char* what, int dtype, int64_t n, int64_t width, int64_t ld
   return ODP_OK;
 }
 
+int check_cap(const char* what, float softcap) {
+  if (softcap == 0.f || (softcap >= FLT_MIN && softcap <= FLT_MAX)) return ODP_OK;
+  odp_set_error("%s: softcap %g is neither 0 nor a positive normal number", what, (double)softcap);
+  return ODP_ERR_INVALID_ARGUMENT;
+}
+
 // Columns a piece of d is padded to, and the edges of the tiles of a kind (Tile's S).
 int tile_edge(int dtype) { return dtype == ODP_DTYPE_F32 ? 128 : 256; }
 int tile_rows(int dtype, int kind) { return kind == 1 ? 64 : kind == 2 ? 128 : kind == 3 ? 32 : tile_edge(dtype); }
@@ -997,6 +1005,7 @@ extern "C" int odp_xent_losses(odp_stream_t stream, int dtype, const void* xc, i
                                int64_t ldw, int64_t vocab, float softcap, void* scratch, float* losses, float* stat,
                                float* logits, int64_t ldl) {
   if (int rc = check_xent("odp_xent_losses", dtype, n, width, ldw, vocab)) return rc;
+  if (int rc = check_cap("odp_xent_losses", softcap)) return rc;
   if (n == 0) return ODP_OK;
   if (xc == nullptr || act == nullptr || tgt == nullptr || count == nullptr || w == nullptr || scratch == nullptr ||
       losses == nullptr || stat == nullptr || !on16(xc) || !on16(w)) {
@@ -1046,6 +1055,7 @@ extern "C" int odp_xent_dlogits(odp_stream_t stream, int dtype, const void* xc, 
                                 const float* g, int g_stride, const float* over, const float* logits, int64_t ldl,
                                 void* dl, int64_t ldd, float* rest) {
   if (int rc = check_xent("odp_xent_dlogits", dtype, n, width, ldw, vocab)) return rc;
+  if (int rc = check_cap("odp_xent_dlogits", softcap)) return rc;
   if (v0 < 0 || vc <= 0 || v0 + vc > vocab || ldd != odp_xent_pitch(dtype, vc)) {
     odp_set_error("odp_xent_dlogits: columns [%lld, %lld) of %lld at pitch %lld", (long long)v0,
                   (long long)(v0 + vc), (long long)vocab, (long long)ldd);

@@ -18,7 +18,6 @@ from __future__ import annotations
 
 import ctypes
 import functools
-import math
 
 import torch
 
@@ -28,6 +27,7 @@ from opaque_amd.capture import SiteRecord, active_session
 from opaque_amd.engine import dtype_code
 
 _ROW_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+_F32 = torch.finfo(torch.float32)
 
 
 _functions: dict[str, object] = {}
@@ -239,8 +239,8 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
         raise ValueError("embedding weight must not be empty")
     if weight.device.type != "cuda" or tokens.device != weight.device:
         raise RuntimeError("embedding runs on the GPU: tokens and weight must be CUDA tensors of one device")
-    if not math.isfinite(scale):
-        raise ValueError(f"scale must be finite, got {scale}")
+    if not abs(scale) <= _F32.max:  # the kernels take it in float32
+        raise ValueError(f"scale must be finite in float32, got {scale}")
     padding = -1
     if padding_idx is not None:
         if not -weight.shape[0] <= padding_idx < weight.shape[0]:
@@ -551,8 +551,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
         raise TypeError(f"x and weight must both be float32 or both bfloat16, got {x.dtype} and {weight.dtype}")
     if weight.device.type != "cuda" or x.device != weight.device or target.device != weight.device:
         raise RuntimeError("linear_cross_entropy runs on the GPU: its arguments must be CUDA tensors of one device")
-    if softcap is not None and not (math.isfinite(softcap) and softcap > 0):
-        raise ValueError(f"softcap must be positive and finite, got {softcap}")
+    if softcap is not None and not _F32.tiny <= softcap <= _F32.max:
+        raise ValueError(f"softcap must be positive and finite (and normal in float32), got {softcap}")
     sess = active_session()
     if sess is not None and sess.mode == "discover":
         weight = sess.hide(weight)
