@@ -639,6 +639,7 @@ int odp_embed_clipped_sum(odp_stream_t stream, int dtype, const void* g, int64_t
                           float scale, const int32_t* seg_example, void* scratch, const float* whole,
                           const double* scales, float normalize_by, int out_dtype, void* out, void* out2);
 
+#define ODP_XENT_WIDE ((int64_t)1 << 20) /* width and W's pitch, elements, stay below it */
 #define ODP_XENT_STAT 3 /* floats that the forward leaves of a row: the maximum of its logits, the sum of \
                            exponentials below it and p(target) - 1 */
 

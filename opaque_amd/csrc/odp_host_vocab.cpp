@@ -175,11 +175,13 @@ at::Tensor embedding(const at::Tensor& tokens, const at::Tensor& weight, double 
 // Linear cross entropy
 // ---------------------------------------------------------------------------
 
-// The head with rows on the 16-byte grid: itself, or a copy padded with zero columns.
+// The head with rows on the 16-byte grid, less than ODP_XENT_WIDE apart: itself, or a copy padded with zero columns.
 at::Tensor head_rows(const at::Tensor& weight) {
   at::Tensor w = pitched(weight);
   const int64_t per = 16 / w.element_size();
-  if (w.size(1) % per == 0 && w.stride(0) % per == 0 && reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0) return w;
+  if (w.size(1) % per == 0 && w.stride(0) % per == 0 && w.stride(0) < ODP_XENT_WIDE &&
+      reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0)
+    return w;
   at::Tensor wide = at::zeros({w.size(0), (w.size(1) + per - 1) / per * per}, w.options());
   wide.narrow(1, 0, w.size(1)).copy_(w);
   return wide;

@@ -834,8 +834,8 @@ int check_xent(const char* what, int dtype, int64_t n, int64_t width, int64_t ld
     return ODP_ERR_UNSUPPORTED;
   }
   const int64_t per = dtype == ODP_DTYPE_F32 ? 4 : 8;
-  if (n < 0 || n >= ((int64_t)1 << 31) - 512 || width <= 0 || width % per != 0 || width >= (int64_t)1 << 20 ||
-      ldw < width || ldw % per != 0 || ldw >= (int64_t)1 << 20 || vocab <= 0 || vocab >= ((int64_t)1 << 31) - 512) {
+  if (n < 0 || n >= ((int64_t)1 << 31) - 512 || width <= 0 || width % per != 0 || width >= ODP_XENT_WIDE ||
+      ldw < width || ldw % per != 0 || ldw >= ODP_XENT_WIDE || vocab <= 0 || vocab >= ((int64_t)1 << 31) - 512) {
     odp_set_error("%s: invalid sizes (n %lld, width %lld, pitch %lld, vocab %lld)", what, (long long)n,
                   (long long)width, (long long)ldw, (long long)vocab);
     return ODP_ERR_INVALID_ARGUMENT;

@@ -288,6 +288,7 @@ _HEAD_DTYPES = (torch.float32, torch.bfloat16)
 # holds at a time: a piece of the vocabulary for all tokens.
 PIECE_BYTES = 512 << 20
 _PIECE_COLUMNS = 1 << 22  # a piece's columns stay below it (ODP_XENT_PIECE)
+_WIDE = 1 << 20  # rows of the head are narrower and less far apart (ODP_XENT_WIDE)
 _STAT = 3  # float32 words that the forward leaves of a row for the backward (ODP_XENT_STAT)
 # Bytes of float32 logits up to which a call that wants gradients keeps them
 # for its backward (1.5 % of the memory of one GPU) where that is faster than
@@ -303,9 +304,10 @@ def _lanes(dtype: torch.dtype) -> int:
 
 
 def _head_rows(weight: torch.Tensor) -> torch.Tensor:
-    """The head with rows on the 16-byte grid: itself, or a copy whose width is padded with zeros."""
+    """The head with rows on the 16-byte grid, less than ODP_XENT_WIDE apart: itself, or a copy whose width is padded
+    with zeros."""
     w, per = pitched_rows(weight.detach()), _lanes(weight.dtype)
-    if w.shape[1] % per == 0 and w.stride(0) % per == 0 and w.data_ptr() % 16 == 0:
+    if w.shape[1] % per == 0 and w.stride(0) % per == 0 and w.stride(0) < _WIDE and w.data_ptr() % 16 == 0:
         return w
     wide = w.new_zeros(w.shape[0], -(-w.shape[1] // per) * per)
     wide[:, : w.shape[1]] = w

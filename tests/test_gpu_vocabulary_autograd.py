@@ -153,3 +153,15 @@ def test_a_checkpointed_loss_holds_nothing():
     held()
     mid, loss = held()
     assert mid < 2 * n * width // 4
+
+
+@pytest.mark.parametrize("pitch", [(1 << 20) - 8, 1 << 20, (1 << 20) + 3])
+def test_heads_of_far_apart_rows(route, pitch):
+    """Rows of the head farther apart than the kernels' offsets reach are copied, not refused."""
+    x, w, y = inputs(20, 64, 3)
+    far = torch.zeros(3, pitch, device=DEV)
+    far[:, :64] = w
+    v = far[:, :64].requires_grad_()
+    want = torch.autograd.grad(linear_cross_entropy(x.requires_grad_(), w.requires_grad_(), y), [x, w])
+    for a, b in zip(torch.autograd.grad(linear_cross_entropy(x, v, y), [x, v]), want):
+        assert torch.equal(a, b)
