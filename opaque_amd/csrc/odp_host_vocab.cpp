@@ -12,6 +12,8 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
+#include <atomic>
+#include <memory>
 #include <string>
 #include <unordered_map>
 
@@ -201,7 +203,23 @@ struct Packed {
   int64_t kept_pitch() const { return abi.xent_pitch(dt, vocab); }
 };
 
-// The rows' statistics go to stat_out.  keep_bytes: up to which the logits are kept for a backward pass.
+// Kept logits of `bytes` bytes, or an undefined tensor where those of all
+// losses that live would pass `most` together.
+std::atomic<int64_t> kept_bytes{0};
+at::Tensor keep_logits(at::IntArrayRef shape, const at::TensorOptions& options, int64_t bytes, int64_t most) {
+  const int64_t before = kept_bytes.fetch_add(bytes);
+  const auto share = std::shared_ptr<void>(nullptr, [bytes](void*) { kept_bytes.fetch_sub(bytes); });
+  if (before > most - bytes) return {};
+  const at::Tensor own = at::empty(shape, options);
+  return at::for_blob(own.data_ptr(), shape)
+      .deleter([own, share](void*) {})
+      .options(options)
+      .target_device(own.device())
+      .make_tensor();
+}
+
+// The rows' statistics go to stat_out.  keep_bytes: up to which the logits of
+// all live losses are kept for their backward passes.
 Packed xent_forward(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target,
                     const at::Tensor& stat_out, double softcap, int64_t ignore, int64_t keep_bytes) {
   Packed p;
@@ -225,7 +243,8 @@ Packed xent_forward(const at::Tensor& x, const at::Tensor& weight, const at::Ten
                       p.count(), losses, stat),
         "odp_xent_rows");
   const int64_t kept = abi.xent_kept(p.dt, p.n, p.width, p.vocab);
-  if (kept > 0 && kept <= keep_bytes) p.logits = at::empty({p.n, p.kept_pitch()}, p.losses.options());
+  if (kept > 0 && kept <= keep_bytes)
+    p.logits = keep_logits({p.n, p.kept_pitch()}, p.losses.options(), kept, keep_bytes);
   const at::Tensor work = bytes_on(rows, abi.xent_stats_scratch(p.dt, p.n, p.vocab));
   check(abi.xent_losses(s, p.dt, p.xc.data_ptr(), p.n, p.width, p.act(), p.tgt(), p.count(), p.w.data_ptr(),
                         p.w.stride(0), p.vocab, (float)softcap, work.data_ptr(), losses, stat, p.kept(), p.kept_pitch()),

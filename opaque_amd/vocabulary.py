@@ -290,9 +290,9 @@ PIECE_BYTES = 512 << 20
 _PIECE_COLUMNS = 1 << 22  # a piece's columns stay below it (ODP_XENT_PIECE)
 _WIDE = 1 << 20  # rows of the head are narrower and less far apart (ODP_XENT_WIDE)
 _STAT = 3  # float32 words that the forward leaves of a row for the backward (ODP_XENT_STAT)
-# Bytes of float32 logits up to which a call that wants gradients keeps them
-# for its backward (1.5 % of the memory of one GPU) where that is faster than
-# forming them again; 0 keeps none.  Neither do the gradients of torch.func
+# Bytes of float32 logits up to which the process's live losses together (1.5 %
+# of the memory of one GPU) keep them for their backward passes, where that is
+# faster than forming them again; 0 keeps none.  Neither do the gradients of torch.func
 # (``vmap(grad)``) and of a head that trains under ``clipped_grad``.
 KEEP_BYTES = 4 << 30
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
@@ -534,7 +534,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     and statistics are float32; the gradients are summed in float32 and
     rounded once, from logit gradients in the inputs' type.  No [tokens,
     vocabulary] tensor is made beyond a piece of PIECE_BYTES in the backward
-    and, where they take at most KEEP_BYTES, the logits between the passes.
+    and, where all live losses' take at most KEEP_BYTES, the logits between
+    the passes.
 
     Replaces the reference's linear cross entropy
     (opaque-patches/.../kernels/linear_cross_entropy.py:249).  Inside

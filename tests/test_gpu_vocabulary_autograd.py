@@ -165,3 +165,28 @@ def test_heads_of_far_apart_rows(route, pitch):
     want = torch.autograd.grad(linear_cross_entropy(x.requires_grad_(), w.requires_grad_(), y), [x, w])
     for a, b in zip(torch.autograd.grad(linear_cross_entropy(x, v, y), [x, v]), want):
         assert torch.equal(a, b)
+
+
+def test_kept_logits_of_all_live_losses_are_bounded(monkeypatch):
+    """Losses that wait for their backward passes share KEEP_BYTES; what one gives back the next may keep."""
+    n, width, vocab = 512, 1024, 4096
+    logits = 4 * n * vocab
+    x, w, y = inputs(n, width, vocab, torch.bfloat16)
+    x.requires_grad_()
+    monkeypatch.setattr(vocabulary, "KEEP_BYTES", 2 * logits + 1)
+
+    def growth():
+        before = torch.cuda.memory_allocated()
+        loss = linear_cross_entropy(x, w, y)
+        return loss, torch.cuda.memory_allocated() - before >= logits
+
+    torch.autograd.grad(growth()[0], [x])
+    live = [growth() for _ in range(3)]
+    assert [kept for _, kept in live] == [True, True, False]
+    grads = [torch.autograd.grad(live[0][0], [x])[0]]
+    again = growth()
+    assert again[1]
+    grads += [torch.autograd.grad(loss, [x])[0] for loss, _ in (live[1], live[2], again)]
+    for g in grads[1:]:
+        assert torch.equal(g, grads[0])
+    del live, again, growth
