@@ -868,7 +868,12 @@ int launch_sum(const char* what, hipStream_t s, int dtype, bool aligned, EmbedSu
   if (int rc = check_grid(what, items)) return rc;
   const dim3 grid((unsigned)((items + EM_WAVES - 1) / EM_WAVES)), block(64 * EM_WAVES);
   const int64_t groups = windows(a.n, a.ncb) / JOIN_GROUP * a.ncb;
-  a.grouped = windows(a.n, a.ncb) > 8 * JOIN_GROUP;  // below, no run is long enough to be worth a launch
+  // Whether long runs are joined in two steps.  A table gradient in one step and
+  // in two, us, with no run, one over half of the rows and one over all: 64
+  // windows (512 x 768 bfloat16) 18 / 19 / 22 and 21 / 22 / 23; 128 (1024 x 768) 19 /
+  // 24 / 28 and 22 / 23 / 24; 256 (2048 x 768) 19 / 32 / 45 and 22 / 26 / 28; 1024
+  // (8192 x 4096) 56 / 111 / 167 and 58 / 67 / 74.
+  a.grouped = windows(a.n, a.ncb) > 8 * JOIN_GROUP;
   const dim3 ggrid((unsigned)((groups + EM_WAVES - 1) / EM_WAVES));
 #define ODP_EM(DT, AL)                                                     \
   do {                                                                     \

@@ -139,8 +139,9 @@ __device__ __forceinline__ uint64_t t_uniform64(uint64_t v) {
 }
 
 // One operand of a tile: `base` is element (row 0 of the matrix, k = 0),
-// `row0` the tile's first row, `rows` the matrix's.  The host's checks of ld (at
-// most 2^23 bytes a row) keep the rows of a tile within 31-bit offsets.
+// `row0` the tile's first row, `rows` the matrix's.  The host's checks of ld keep
+// the rows of a tile within 31-bit offsets: rows of x and W lie less than 2^22
+// bytes apart, rows of d less than 2^23 (256 of bfloat16) or 2^24 (128 of float32).
 struct Operand {
   const void* base;
   int64_t ld;

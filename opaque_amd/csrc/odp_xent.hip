@@ -1,8 +1,8 @@
 // Softmax cross entropy of x W^T over a large vocabulary, a piece of it at a time.
 //
 //   u = x W^T,  z = u or c tanh(u / c)
-//   lse_t = log sum_v exp z_tv,  loss_t = lse_t - z_t,y(t)
-//   d_tv = g_t (exp(z_tv - lse_t) - [v = y(t)]) (1 - (z_tv / c)^2)
+//   m_t = max_v z_tv,  s_t = sum_v exp(z_tv - m_t),  loss_t = (m_t - z_t,y(t)) + log s_t
+//   p_tv = exp(z_tv - m_t) / s_t,  d_tv = g_t (p_tv - [v = y(t)]) (1 - (z_tv / c)^2)
 //   dx = d W,  dW = d^T x
 //
 // The tokens that bear a loss are first gathered (k_xent_pick, k_xent_pack),
@@ -21,13 +21,18 @@
 // TFLOP/s (a library product of 8192^3 runs at 1216).  One token's loss: 180 us,
 // W at 5.8 TB/s.
 //
-// Sums, statistics and losses are
-// float32; d is rounded to the inputs' type because the matrix cores take it
-// so (a relative 2^-8 of an entry at most in bfloat16, of the order of the
-// rounding of the gradients themselves).  What rounding takes off the target's
-// entry, often the row's only large one, is added to dx in float32
-// (k_xent_dx_rows): alone it would leave a row of dx as far off as that entry.
-// A row of dW adds many tokens' entries, whose roundings average out.
+// Sums, statistics and losses are float32; d is rounded to the inputs' type
+// because the matrix cores take it so (a relative 2^-8 of an entry at most in
+// bfloat16, of the order of the rounding of the gradients themselves).  What
+// rounding takes off the target's entry, often the row's only large one, is added
+// to dx in float32 (k_xent_dx_rows): alone it would leave a row of dx as far off as
+// that entry.  dW takes d as it is rounded: a row of dW that is the target of one
+// token is that entry times x, off by the entry's rounding beside its own, and
+// rows of many tokens by about as much of their size (against 64 bits 0.0021 of
+// the values for 700 tokens, 0.0017 with nothing rounded but the results).  Giving
+// it back there would take an embedding's gradient: the tokens sorted by target
+// and a float32 row for each distinct one (19 us for 1024 x 768, where such a call
+// takes 260).
 #include <cfloat>
 
 #include "odp_internal.h"
@@ -645,8 +650,9 @@ __global__ __launch_bounds__(256) void k_xent_dkept(Xent p, const float* __restr
 
 // How many slices of the contraction each tile of dx is split into: the
 // fewest of 1 .. DX_SPLIT with which the workgroups fill the 256 CUs' rounds
-// best, as far as the slots (`cap` tiles) and slices of 16 steps go.  dx, us, in
-// up to 16, 32 and 64 slices: bfloat16, 128 tokens, 128256 x 512 139, 78 and 48,
+// best, as far as the slots (`cap` tiles) and slices of 16 steps go.  32 is where
+// no measured head loses; 64 would gain on heads of few columns and cost on
+// 32000 x 2048.  dx, us, in up to 16, 32 and 64 slices: bfloat16, 128 tokens, 128256 x 512 139, 78 and 48,
 // 32000 x 2048 44, 31 and 43; 777 tokens, 32000 x 2048 103, 102 and 101; float32,
 // one token, 50257 x 768 103, 56 and 48 (64 slices cost dx_rows 4 us more).
 constexpr int DX_SPLIT = 32;
@@ -858,8 +864,10 @@ static_assert(2 * 255 * ODP_XENT_PIECE < T_OOB && 4 * 127 * ODP_XENT_PIECE < T_O
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Whether a product of n rows takes the tiles of few rows.  Loss and dx, us,
-// with the small tiles and the large ones: bfloat16, 32000 x 2048, 64 tokens 69
+// Whether a product of n rows takes the tiles of few rows.  64 in bfloat16: past
+// it the large heads lose a third, while heads that fit the cache would gain an
+// eighth up to 128.  Rules go by all n tokens, since the host does not know how
+// many bear a loss.  Loss and dx, us, with the small tiles and the large ones: bfloat16, 32000 x 2048, 64 tokens 69
 // and 87, 128 84 and 96, 192 109 and 104, 256 130 and 118; 128256 x 4096, 64
 // tokens 440 and 421, 65 605 and 409 (W past the cache is read once a row of
 // tiles); float32, 50257 x 768, 64 tokens 143 and 231, 256 364 and 394, 384 542

@@ -530,7 +530,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     logits as ``softcap * tanh(logits / softcap)``.  ``reduction`` "none"
     gives the float32 loss of every token, "sum" and "mean" their sum and
     mean over the tokens whose target is not ``ignore_index`` (NaN when there
-    is none, as torch's).  A target outside the vocabulary gives NaN.  Logits
+    is none, as torch's).  A target outside the vocabulary makes its loss and
+    its row of x's gradient NaN, and is left out of the head's.  Logits
     and statistics are float32; the gradients are summed in float32 and
     rounded once, from logit gradients in the inputs' type.  No [tokens,
     vocabulary] tensor is made beyond a piece of PIECE_BYTES in the backward
