@@ -115,6 +115,13 @@ def active_session() -> CaptureSession | None:
     return getattr(_STATE, "session", None)
 
 
+def transformed() -> bool:
+    """Whether a torch.func transform is active.  In the vmap rule of a capture
+    pass: whether the batch at hand is one of the loss's own vmaps, inside the
+    engine's; the seam then merges it and is recorded by the next rule."""
+    return torch._C._are_functorch_transforms_active()
+
+
 def _plain(x, W, A, B, scaling, bias):
     out = F.linear(x, W) + scaling * ((x @ A) @ B)
     return out if bias is None else out + bias
@@ -207,6 +214,8 @@ class _SeamLoRA(torch.autograd.Function):
                 out = out + (bias.view(bias.shape[0], *([1] * (out.dim() - 2)), bias.shape[-1])
                              if bias_d is not None else bias)
             return out, 0
+        if transformed() and bias_d is None:
+            return _SeamLoRA.apply(x, W, A, B, scaling, bias, a_obj, b_obj, a_t, b_t), 0
         rec = SiteRecord(x=x, A=A, B=B, scaling=float(scaling), a_obj=a_obj, b_obj=b_obj,
                          a_transposed=a_t, b_transposed=b_t)
         sess.sites.append(rec)
@@ -299,6 +308,8 @@ class _SeamLinear(torch.autograd.Function):
             else:
                 out = F.linear(x, W)
             return (out if bias is None else out + bias), 0
+        if transformed() and bias_d is None:
+            return _SeamLinear.apply(x, W, bias), 0
         rec = SiteRecord(x=x, A=None, B=None, scaling=1.0, a_obj=None, b_obj=None,
                          a_transposed=False, b_transposed=False, w_obj=W)
         sess.sites.append(rec)
@@ -427,6 +438,8 @@ class _SeamMoE(torch.autograd.Function):
         if (sess is None or sess.mode != "capture" or id(gate_up_proj) not in sess.eligible
                 or id(down_proj) not in sess.eligible):
             return _moe_dense(x, gate_up_proj, down_proj, top_k_index, top_k_weights), 0
+        if transformed():
+            return _SeamMoE.apply(x, gate_up_proj, down_proj, top_k_index, top_k_weights), 0
         return _moe_tapped(sess, x, gate_up_proj, down_proj, top_k_index, top_k_weights), 0
 
 

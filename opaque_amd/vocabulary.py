@@ -23,7 +23,7 @@ import torch
 
 from opaque_amd import _host
 from opaque_amd import _native as N
-from opaque_amd.capture import SiteRecord, active_session
+from opaque_amd.capture import SiteRecord, active_session, transformed
 from opaque_amd.engine import dtype_code
 
 _ROW_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
@@ -74,11 +74,6 @@ def _bound():
                        for name in N.exported_symbols()})
         _host_ready.append(host)
     return _host_ready[0]
-
-
-def _transformed() -> bool:
-    """Whether a torch.func transform is active (the Functions with vmap rules then take the call)."""
-    return torch._C._are_functorch_transforms_active()
 
 
 def pitched_rows(t: torch.Tensor) -> torch.Tensor:
@@ -194,7 +189,7 @@ class _Embed(torch.autograd.Function):
             weight = weight.movedim(in_dims[1], 0)
             return torch.stack([_Embed.apply(tokens[i], weight[i], scale, padding) for i in range(n)]), 0
         sess = active_session()
-        if sess is None or sess.mode != "capture" or id(weight) not in sess.eligible:
+        if sess is None or sess.mode != "capture" or id(weight) not in sess.eligible or transformed():
             return _Embed.apply(tokens, weight, scale, padding), 0
         rec = SiteRecord(x=None, A=None, B=None, scaling=scale, a_obj=None, b_obj=None, a_transposed=False,
                          b_transposed=False, w_obj=weight, tokens=tokens, padding=padding)
@@ -251,7 +246,7 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
         weight = sess.hide(weight)
     elif sess is not None and id(weight) in sess.eligible:
         tokens = sess.batched(tokens)
-    host = None if _transformed() else _bound()
+    host = None if transformed() else _bound()
     if host is not None:
         return host.embedding(tokens, weight, scale, padding)
     return _Embed.apply(tokens, weight, float(scale), padding)
@@ -484,8 +479,8 @@ class _Xent(torch.autograd.Function):
             out = [_Xent.apply(x[i], w[i], target[i], softcap, ignore) for i in range(n)]
             return (torch.stack([o[0] for o in out]), torch.stack([o[1] for o in out])), (0, 0)
         sess = active_session()
-        if sess is None or sess.mode != "capture" or id(weight) not in sess.eligible:
-            host = None if _transformed() else _bound()
+        if sess is None or sess.mode != "capture" or id(weight) not in sess.eligible or transformed():
+            host = None if transformed() else _bound()
             if host is not None:
                 return host.token_losses(x, weight, target, softcap, ignore, PIECE_BYTES, KEEP_BYTES), (0, 0)
             return _Xent.apply(x, weight, target, softcap, ignore), (0, 0)
@@ -560,7 +555,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     sess = active_session()
     if sess is not None and sess.mode == "discover":
         weight = sess.hide(weight)
-    host = None if _transformed() else _bound()
+    host = None if transformed() else _bound()
     if host is not None:
         return host.cross_entropy(x, weight, target, softcap or 0.0, ignore_index, _REDUCTIONS[reduction], PIECE_BYTES,
                                   KEEP_BYTES)

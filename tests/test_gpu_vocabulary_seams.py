@@ -172,3 +172,25 @@ def test_positions_alone():
         return lambda p, xi: (ops.embedding(torch.tensor(2, device=xi.device), p["wpe"]) * xi).sum().sin()
 
     assert seams_of(compare(make, params, (x,), tol=1e-5, clipping_norm=10.0)) == (1, 0, False)
+
+
+@pytest.mark.parametrize("tokens", ["batch", "positions"])
+def test_inner_vmaps_of_the_loss(tokens):
+    """A loss that vmaps over its own tokens: lookups and losses of the batch are recorded by the engine's vmap, a lookup
+    that only the inner one batches is not (the model then goes materialised)."""
+    g = torch.Generator().manual_seed(25)
+    n, T, vocab, width = 4, 6, 40, 16
+    params = {"table": torch.randn(vocab, width, generator=g), "head": torch.randn(vocab, width, generator=g) / 4}
+    y, t = torch.randint(0, vocab, (n, T), generator=g), torch.randint(0, vocab, (n, T), generator=g)
+
+    def make(ops):
+        def loss(p, yi, ti):
+            at = yi if tokens == "batch" else torch.arange(T, device=yi.device)
+            h = torch.func.vmap(lambda k: torch.tanh(ops.embedding(k, p["table"])))(at.unsqueeze(1)).squeeze(1)
+            h = h * (1 + yi.unsqueeze(1) % 3)
+            return torch.func.vmap(lambda r, k: ops.loss(r, p["head"], k))(h, ti).mean()
+
+        return loss
+
+    engine = compare(make, params, (y, t), tol=1e-5)
+    assert seams_of(engine)[0] == (1 if tokens == "batch" else 0)
