@@ -96,6 +96,11 @@ at::Tensor pitched(const at::Tensor& t) {
   return r;
 }
 
+// A tangent on an input would be dropped without a word: the kernels read values.
+void no_tangent(const at::Tensor& t) {
+  TORCH_CHECK(!t._fw_grad(0).defined(), "the vocabulary operators have no forward-mode derivative");
+}
+
 // Ties a first derivative to what it depends on, so that asking for a second
 // one is an error instead of zero: to the gradient g it came from and, with
 // `inputs`, to the inputs of the node whose backward pass calls this (by
@@ -169,6 +174,7 @@ struct Embed : torch::autograd::Function<Embed> {
 
 at::Tensor embedding(const at::Tensor& tokens, const at::Tensor& weight, double scale, int64_t padding) {
   py::gil_scoped_release nogil;
+  no_tangent(weight);
   if (at::GradMode::is_enabled() && weight.requires_grad()) return Embed::apply(tokens, weight, scale, padding);
   return embed_rows(tokens, weight, scale);
 }
@@ -350,6 +356,8 @@ struct Xent : torch::autograd::Function<Xent> {
 
 at::Tensor xent(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target, const at::Tensor& stat,
                 double softcap, int64_t ignore, int64_t reduction, int64_t piece_bytes, int64_t keep_bytes) {
+  no_tangent(x);
+  no_tangent(weight);
   if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad()))
     return Xent::apply(x, weight, target, stat, softcap, ignore, reduction, piece_bytes, keep_bytes);
   const c10::OptionalDeviceGuard guard(x.device());

@@ -190,3 +190,28 @@ def test_kept_logits_of_all_live_losses_are_bounded(monkeypatch):
     for g in grads[1:]:
         assert torch.equal(g, grads[0])
     del live, again, growth
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_forward_mode_is_an_error(route, requires_grad):
+    """A tangent on x, the head or the table is refused, not dropped."""
+    x, w, y = inputs()
+    with torch.autograd.forward_ad.dual_level():
+        dual = [torch.autograd.forward_ad.make_dual(t.clone().requires_grad_(requires_grad), torch.ones_like(t))
+                for t in (x, w)]
+        for call in (lambda: linear_cross_entropy(dual[0], w, y), lambda: linear_cross_entropy(x, dual[1], y),
+                     lambda: embedding(y, dual[1])):
+            with pytest.raises(RuntimeError):
+                call()
+    for f, t in ((lambda a: linear_cross_entropy(a, w, y), x), (lambda a: embedding(y, a), w)):
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(f, (t,), (torch.ones_like(t),))
+
+
+def test_in_inference_mode(route):
+    x, w, y = inputs()
+    want = linear_cross_entropy(x, w, y), embedding(y, w)
+    with torch.inference_mode():
+        got = linear_cross_entropy(x.clone(), w.clone(), y.clone()), embedding(y.clone(), w.clone())
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
