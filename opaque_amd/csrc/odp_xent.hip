@@ -30,9 +30,10 @@
 // token is that entry times x, off by the entry's rounding beside its own, and
 // rows of many tokens by about as much of their size (against 64 bits 0.0021 of
 // the values for 700 tokens, 0.0017 with nothing rounded but the results).  Giving
-// it back there would take an embedding's gradient: the tokens sorted by target
-// and a float32 row for each distinct one (19 us for 1024 x 768, where such a call
-// takes 260).
+// it back in dW's tiles, tokens found by their targets and added sixteen a step
+// of the matrix cores, was right and cost more than it gives: loss and gradients
+// of 777 x 32003 x 1000 297 us against 257, one token of 128256 x 4096 696 against
+// 595, 4096 of them 12.2 ms against 10.8 (targets as frequent as in text).
 #include <cfloat>
 
 #include "odp_internal.h"
