@@ -120,6 +120,18 @@ at::Tensor first_only(const at::Tensor& g, at::Tensor d, bool inputs) {
   return d;
 }
 
+// What comes back from autograd is what was saved, wherever its hooks had it
+// meanwhile: the kernels take addresses.
+void as_saved(const at::Tensor& t, const at::Tensor& like, at::ScalarType type, at::IntArrayRef shape) {
+  TORCH_CHECK(t.device() == like.device() && t.scalar_type() == type && t.sizes() == shape,
+              "vocabulary operators: a saved tensor came back as ", t.scalar_type(), " ", t.sizes(), " on ", t.device(),
+              ", not as ", type, " ", shape, " on ", like.device());
+}
+at::Tensor whole(const at::Tensor& t, const at::Tensor& like, at::ScalarType type, at::IntArrayRef shape) {
+  as_saved(t, like, type, shape);
+  return t.contiguous();
+}
+
 // ---------------------------------------------------------------------------
 // Embedding
 // ---------------------------------------------------------------------------
@@ -143,6 +155,8 @@ struct Embed : torch::autograd::Function<Embed> {
     ctx->saved_data["vocab"] = weight.size(0);
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["padding"] = padding;
+    ctx->saved_data["tokens"] = tokens.sizes().vec();
+    ctx->saved_data["wide"] = tokens.scalar_type() == at::kLong;
     return embed_rows(tokens, weight, scale);
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
@@ -152,7 +166,9 @@ struct Embed : torch::autograd::Function<Embed> {
     {
       at::NoGradGuard no_grad;
       const c10::OptionalDeviceGuard guard(grads[0].device());
-      const at::Tensor g = pitched(grads[0]), y = ctx->get_saved_variables()[0].contiguous();
+      const at::Tensor g = pitched(grads[0]);
+      const at::Tensor y = whole(ctx->get_saved_variables()[0], g, ctx->saved_data["wide"].toBool() ? at::kLong : at::kInt,
+                                 ctx->saved_data["tokens"].toIntVector());
       const int64_t n = y.numel(), width = g.size(1), vocab = ctx->saved_data["vocab"].toInt();
       const int dt = code_of(g);
       dw = at::empty({vocab, width}, g.options());
@@ -279,6 +295,9 @@ struct Xent : torch::autograd::Function<Xent> {
     ctx->save_for_backward({p.w, p.xc, p.ids, p.stat, p.logits});
     auto& d = ctx->saved_data;
     d["n"] = p.n;
+    d["dt"] = (int64_t)p.dt;
+    d["vocab"] = p.vocab;
+    d["width"] = p.width;
     d["cols"] = p.cols;
     d["softcap"] = softcap;
     d["mean"] = reduction == 2;
@@ -293,42 +312,45 @@ struct Xent : torch::autograd::Function<Xent> {
     const torch::autograd::variable_list saved = ctx->get_saved_variables();
     {
       at::NoGradGuard no_grad;
+      const c10::OptionalDeviceGuard guard(grads[0].device());
       auto& sd = ctx->saved_data;
       Packed p;
-      p.w = saved[0];
-      p.xc = saved[1];
-      p.ids = saved[2];
-      p.logits = saved[4];
       p.n = sd["n"].toInt();
       p.cols = sd["cols"].toInt();
-      p.width = p.w.size(1);
-      p.vocab = p.w.size(0);
-      p.dt = code_of(p.xc);
-      const at::Tensor stat = saved[3];
+      p.width = sd["width"].toInt();
+      p.vocab = sd["vocab"].toInt();
+      p.dt = (int)sd["dt"].toInt();
+      const at::ScalarType type = p.dt == ODP_DTYPE_F32 ? at::kFloat : at::kBFloat16;
+      const int64_t room = std::max<int64_t>(p.n, 1);
+      as_saved(saved[0], grads[0], type, {p.vocab, p.width});
+      p.w = head_rows(saved[0]);
+      p.xc = whole(saved[1], grads[0], type, {room, p.width});
+      p.ids = whole(saved[2], grads[0], at::kInt, {3 * room + 2});
+      p.stat = whole(saved[3].reshape({-1}), grads[0], at::kFloat, {p.n * ODP_XENT_STAT});
+      if (saved[4].defined()) p.logits = whole(saved[4], grads[0], at::kFloat, {p.n, p.kept_pitch()});
       const float softcap = (float)sd["softcap"].toDouble();
-      const c10::OptionalDeviceGuard guard(p.xc.device());
       const at::Tensor g = grads[0].contiguous();
       const int stride = g.dim() > 0 ? 1 : 0;
       const float* over = sd["mean"].toBool() ? p.counted() : nullptr;
       const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
       const int64_t es = p.xc.element_size(), edge = abi.xent_pitch(p.dt, 1);
-      const int64_t fit = std::min(sd["piece_bytes"].toInt() / (std::max<int64_t>(p.n, 1) * es) / edge * edge,
+      const int64_t fit = std::min(sd["piece_bytes"].toInt() / (room * es) / edge * edge,
                                    ODP_XENT_PIECE - edge);
       const int64_t pieces = (p.vocab + std::max(fit, edge) - 1) / std::max(fit, edge);
       const int64_t piece = std::min(p.vocab, ((p.vocab + pieces - 1) / pieces + edge - 1) / edge * edge);
-      const at::Tensor d = at::empty({std::max<int64_t>(p.n, 1), abi.xent_pitch(p.dt, piece)}, p.xc.options());
+      const at::Tensor d = at::empty({room, abi.xent_pitch(p.dt, piece)}, p.xc.options());
       at::Tensor sums;
       if (need_x) {
         dx = at::empty(sd["x_shape"].toIntVector(), p.xc.options());
         sums = bytes_on(p.xc, abi.xent_dx_scratch(p.dt, p.n, p.width));
       }
       if (need_w) dw = at::empty({p.vocab, p.width}, p.xc.options());
-      const at::Tensor rest = at::empty({std::max<int64_t>(p.n, 1)}, stat.options());
+      const at::Tensor rest = at::empty({room}, p.stat.options());
       const odp_stream_t s = stream_of(p.xc);
       for (int64_t v0 = 0; v0 < p.vocab; v0 += piece) {
         const int64_t vc = std::min(piece, p.vocab - v0), ldd = abi.xent_pitch(p.dt, vc);
         check(abi.xent_dlogits(s, p.dt, p.xc.data_ptr(), p.n, p.width, p.act(), p.tgt(), p.count(), p.w.data_ptr(),
-                               p.w.stride(0), p.vocab, softcap, v0, vc, (const float*)stat.data_ptr(),
+                               p.w.stride(0), p.vocab, softcap, v0, vc, (const float*)p.stat.data_ptr(),
                                (const float*)g.data_ptr(), stride, over, p.kept(), p.kept_pitch(), d.data_ptr(), ldd,
                                (float*)rest.data_ptr()),
               "odp_xent_dlogits");

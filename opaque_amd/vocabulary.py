@@ -76,6 +76,13 @@ def _bound():
     return _host_ready[0]
 
 
+def _on_one_device(t: torch.Tensor, *saved: torch.Tensor) -> None:
+    """What comes back from autograd lies where the gradient does, wherever its hooks had it meanwhile."""
+    for s in saved:
+        if s.device != t.device:
+            raise RuntimeError(f"vocabulary operators: a saved tensor came back on {s.device}, not {t.device}")
+
+
 def pitched_rows(t: torch.Tensor) -> torch.Tensor:
     """2-D view [rows, d] with unit column stride and a pitch of at least d;
     rows laid out otherwise (transposed, expanded) are copied."""
@@ -114,6 +121,9 @@ def table_gradient(tokens: torch.Tensor, g: torch.Tensor, vocab: int, scale: flo
     """[vocab, width] = scale times the sum of each token's rows of g (the backward of ``embedding``)."""
     rows = pitched_rows(g.detach())
     flat = tokens.contiguous()
+    _on_one_device(g, tokens)
+    if tokens.dtype not in (torch.int64, torch.int32) or tokens.numel() != rows.shape[0]:
+        raise RuntimeError("vocabulary operators: the saved tokens came back otherwise than they were saved")
     n, width, dev = flat.numel(), g.shape[-1], g.device
     dt = dtype_code(g.dtype)
     out = torch.empty((vocab, width), dtype=g.dtype, device=dev)
@@ -410,6 +420,11 @@ def _xent_losses(x, weight, target, softcap, ignore):
 
 def _xent_gradients(g, x, weight, target, stat, softcap, ignore, need_x, need_w, keep_d=False):
     g, stat = g.detach().float().contiguous().reshape(-1), stat.contiguous()
+    _on_one_device(g, x, weight, target, stat)
+    n = g.numel()
+    if (x.dtype != weight.dtype or x.shape[-1] != weight.shape[1] or stat.dtype != torch.float32
+            or (target.numel(), stat.numel(), x.numel()) != (n, n * _STAT, n * x.shape[-1])):
+        raise RuntimeError("vocabulary operators: a saved tensor came back otherwise than it was saved")
     with _OnDevice(x):
         p = _Packed(x, _head_rows(weight), target, ignore, keep_d)
         return p.gradients(softcap, stat, g, x.shape if need_x else None, need_w, keep_d)

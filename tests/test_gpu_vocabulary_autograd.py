@@ -215,3 +215,30 @@ def test_in_inference_mode(route):
         got = linear_cross_entropy(x.clone(), w.clone(), y.clone()), embedding(y.clone(), w.clone())
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("back", ["cpu", "half"])
+def test_saved_tensors_that_come_back_otherwise_are_refused(route, back):
+    """Hooks that leave a saved tensor on the host, or in another type, give an error: the kernels take addresses."""
+    x, w, y = inputs(60, 136, 700)
+    x.requires_grad_(), w.requires_grad_()
+    change = {"cpu": lambda t: t.cpu(), "half": lambda t: t.to(torch.float64) if t.is_floating_point() else t}[back]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+        loss, rows = linear_cross_entropy(x, w, y), embedding(y, w)
+    with pytest.raises((RuntimeError, TypeError)):
+        torch.autograd.grad(loss, [x, w])
+    if back == "cpu":
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(rows, [w], torch.ones_like(rows))
+
+
+def test_saved_heads_come_back_in_another_layout(route):
+    """A hook may change strides: transposed heads and rows give the same bits."""
+    x, w, y = inputs(60, 136, 700)
+    x.requires_grad_(), w.requires_grad_()
+    want = torch.autograd.grad(linear_cross_entropy(x, w, y), [x, w])
+    turned = lambda t: t.t().contiguous().t() if t.dim() == 2 else t
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, turned):
+        loss = linear_cross_entropy(x, w, y)
+    for a, b in zip(torch.autograd.grad(loss, [x, w]), want):
+        assert torch.equal(a, b)
