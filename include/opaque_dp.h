@@ -705,6 +705,71 @@ int64_t odp_xent_dw_scratch(int dtype, int64_t n, int64_t vc, int64_t width);
 int odp_xent_dw(odp_stream_t stream, int dtype, const void* xc, int64_t n, int64_t width, const int32_t* count,
                 int64_t vc, const void* dl, int64_t ldd, void* scratch, void* dw, int64_t lddw);
 
+/* ---- root-mean-square norm -------------------------------------------------
+ * h = x + residual, as the residual stream's type holds it (h = x where residual
+ * is null), y = h / sqrt(mean(h^2) + eps) (gain + offset), for rows x [n][width]
+ * (pitch ldx) of `dtype` (float32, bfloat16 or float16), the stream (pitch ldr) of
+ * stream_dtype, gains [gains][width] (pitch ldg, 0: one for all; null: 1) of
+ * gain_dtype, both `dtype` or float32.  Gain i covers rows [i n / gains, ..): n is
+ * a multiple of gains.  Sums of squares are float32, and y is rounded once.
+ * sum [n][width] receives h where there is a residual, rstd [n] (may be null)
+ * 1 / sqrt(..).  quant 1 or 2: y [n][width] in e4m3 instead, with scales [n] or
+ * [n][ceil(width / 128)] float32, the largest |y| of the row or of its 128 columns
+ * over 448 (at least the least normal float32); a row with a NaN gives NaN.
+ * n < 2^31, width <= ODP_NORM_WIDE.  The reference runs its models' norms through
+ * torch; under vmap(grad) their gains' gradients are per example
+ * (opaque-engine/.../clipping/_clipped_fun.py:756-762).                        */
+#define ODP_NORM_WIDE ((int64_t)32768)
+int odp_rms_norm(odp_stream_t stream, int dtype, int stream_dtype, int gain_dtype, const void* x, int64_t ldx,
+                 const void* residual, int64_t ldr, int64_t n, int64_t width, const void* gain, int64_t ldg,
+                 int64_t gains, float eps, float offset, int quant, void* y, void* sum, float* rstd, float* scales);
+
+/* Gradients from gy (of y; pitch ldy) and gh (of h; may be null): dx [n][width]
+ * of `dtype` (null: not wanted) and dres of stream_dtype (null: not wanted, or the
+ * same as dx where the types are), dgain [gains][width] of gain_dtype (null: not
+ * wanted), summed over each gain's rows in float32.  h has stream_dtype (x's
+ * where there was no residual).  scratch: odp_rms_norm_grad_scratch() bytes.   */
+int64_t odp_rms_norm_grad_scratch(int64_t n, int64_t width, int64_t gains);
+int odp_rms_norm_grad(odp_stream_t stream, int dtype, int stream_dtype, int gain_dtype, const void* h, int64_t ldh,
+                      const float* rstd, const void* gy, int64_t ldy, const void* gh, int64_t ldgh, int64_t n,
+                      int64_t width, const void* gain, int64_t ldg, int64_t gains, float offset, void* scratch,
+                      void* dx, void* dres, void* dgain);
+
+/* ---- routing to experts ----------------------------------------------------
+ * For logits z [n][experts] (pitch ldz; float32, bfloat16 or float16): scores p =
+ * softmax(z), or sigmoid(z) where sigmoid != 0; keys p + bias [biases][experts]
+ * (null: none; bias i for the tokens [i n / biases, ..)); with `groups` > 1 the
+ * best top_groups of the equal consecutive groups stay, by the sum of their two
+ * best keys (best 0) or by their best (1); index [n][top_k] the best keys left,
+ * best first, and weights [n][top_k] = scale p, over the sum of the chosen p with
+ * renormalize.  Equal keys (in 64 bits) give the lower expert.  An expert whose
+ * logit is -inf comes after all others and weighs 0; a NaN (in a softmax also
+ * +inf) makes the row's weights (sigmoid: those it touches) NaN.  index always
+ * holds top_k different experts.  n < 2^31; the reference's models bring their
+ * routing (opaque-patches/.../kernels/moe.py:179 takes top_k_index and weights). */
+#define ODP_ROUTE_EXPERTS 1024
+#define ODP_ROUTE_CHOICES 64
+int odp_route(odp_stream_t stream, int dtype, const void* logits, int64_t ldz, int64_t n, int64_t experts, int sigmoid,
+              const float* bias, int64_t biases, int64_t groups, int64_t top_groups, int best, int64_t top_k,
+              int renormalize, float scale, int64_t* index, float* weights);
+/* dlogits [n][experts] from gw (of the weights; pitch ldw) and the index.     */
+int odp_route_grad(odp_stream_t stream, int dtype, const void* logits, int64_t ldz, int64_t n, int64_t experts,
+                   int sigmoid, int64_t top_k, int renormalize, float scale, const int64_t* index, const float* gw,
+                   int64_t ldw, void* dlogits);
+
+/* ---- norm of a tree of gradients --------------------------------------------
+ * leaves: a table in HOST memory, read during the call, ODP_TN_FIELDS words a
+ * row.  norm = sqrt of the sum of all squares (float64 sums; stored as float64
+ * where wide != 0, else float32); with clip != 0 every leaf's dst = src factor,
+ * factor = max_norm / norm where norm > max_norm, else 1 (an exact copy), NaN for
+ * a NaN norm; dst may be src.  The factor and product are float32 (float64 for
+ * float64 leaves).  scratch: odp_tree_norm_scratch() bytes on the 8-byte grid.
+ * The reference's counterpart is torch's (opaque-engine/.../pytree.py:336-430). */
+enum { ODP_TN_SRC = 0, ODP_TN_DST, ODP_TN_N, ODP_TN_DTYPE, ODP_TN_FIELDS = 4 };
+int64_t odp_tree_norm_scratch(int64_t n_leaves);
+int odp_tree_norm(odp_stream_t stream, const int64_t* leaves, int64_t n_leaves, int clip, double max_norm, int wide,
+                  void* scratch, void* norm);
+
 #ifdef __cplusplus
 }
 #endif

@@ -45,6 +45,8 @@ SQ_X, SQ_N, SQ_NSEG, SQ_SEG_FIRST, SQ_SLOT, SQ_DTYPE = range(6)
 LN_FIELDS = 24
 LN_X, LN_LDX, LN_G, LN_LDG, LN_DIN, LN_DOUT, LN_SEG_FIRST, LN_NSEG, LN_SLOT, LN_OUT, LN_FLAGS, LN_NB, LN_NROWS, LN_PE = range(14)
 LN_XMASK, LN_GMASK, LN_NFFLAG, LN_SCRATCH, LN_OUT2, LN_XAMAX, LN_GAMAX = 14, 15, 16, 17, 18, 19, 20
+TN_FIELDS = 4
+TN_SRC, TN_DST, TN_N, TN_DTYPE = range(4)
 NF_FIELDS = 8
 NF_P, NF_LDP, NF_D, NF_SEG_FIRST, NF_NSEG, NF_MASK, NF_AMAX = range(7)
 FORM_OUTER = 0
@@ -169,6 +171,28 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "odp_xent_dw": (
         _c_int, [_ptr, _c_int, _ptr, _c_i64, _c_i64, _ptr, _c_i64, _ptr, _c_i64, _ptr, _ptr, _c_i64]),
     "odp_xent_dw_scratch": (_c_i64, [_c_int, _c_i64, _c_i64, _c_i64]),
+    "odp_rms_norm": (
+        _c_int,
+        [_ptr, _c_int, _c_int, _c_int, _ptr, _c_i64, _ptr, _c_i64, _c_i64, _c_i64, _ptr, _c_i64, _c_i64, _c_f32, _c_f32,
+         _c_int, _ptr, _ptr, _ptr, _ptr],
+    ),
+    "odp_rms_norm_grad_scratch": (_c_i64, [_c_i64, _c_i64, _c_i64]),
+    "odp_rms_norm_grad": (
+        _c_int,
+        [_ptr, _c_int, _c_int, _c_int, _ptr, _c_i64, _ptr, _ptr, _c_i64, _ptr, _c_i64, _c_i64, _c_i64, _ptr, _c_i64,
+         _c_i64, _c_f32, _ptr, _ptr, _ptr, _ptr],
+    ),
+    "odp_route": (
+        _c_int,
+        [_ptr, _c_int, _ptr, _c_i64, _c_i64, _c_i64, _c_int, _ptr, _c_i64, _c_i64, _c_i64, _c_int, _c_i64, _c_int,
+         _c_f32, _ptr, _ptr],
+    ),
+    "odp_route_grad": (
+        _c_int,
+        [_ptr, _c_int, _ptr, _c_i64, _c_i64, _c_i64, _c_int, _c_i64, _c_int, _c_f32, _ptr, _ptr, _c_i64, _ptr],
+    ),
+    "odp_tree_norm_scratch": (_c_i64, [_c_i64]),
+    "odp_tree_norm": (_c_int, [_ptr, _ptr, _c_i64, _c_int, _c_f64, _c_int, _ptr, _ptr]),
     "odp_linear_moments_blocks": (_c_i64, [_c_i64, _c_i64, _c_i32]),
     "odp_linear_moments": (
         _c_int, [_ptr, _ptr, _ptr, _c_i32, _c_i32, _ptr, _ptr, _ptr, _ptr, _c_i32, _c_i32, _c_f32, _c_i32]),

@@ -18,7 +18,7 @@ INCLUDE = PKG_DIR.parent / "include"
 LIB_NAME = "libopaque_dp.so"
 LIB_PATH = PKG_DIR / LIB_NAME
 SOURCES = ["odp_abi.hip", "odp_lora.hip", "odp_clip.hip", "odp_noise.hip", "odp_linear.hip", "odp_moments.hip",
-           "odp_embed.hip", "odp_xent.hip", "odp_calib.hip"]
+           "odp_embed.hip", "odp_xent.hip", "odp_norm.hip", "odp_route.hip", "odp_tree.hip", "odp_calib.hip"]
 ARCH = "gfx950"
 
 HIPCC_FLAGS = [
@@ -105,7 +105,7 @@ def build_sanitized(verbose: bool = False) -> Path:
     return SAN_LIB
 
 
-HOST_SRCS = [CSRC / "odp_host.cpp", CSRC / "odp_host_vocab.cpp"]
+HOST_SRCS = [CSRC / "odp_host.cpp", CSRC / "odp_host_vocab.cpp", CSRC / "odp_host_block.cpp"]
 HOST_DIR = PKG_DIR / "_host_build"
 HOST_NAME = "_odp_host"
 

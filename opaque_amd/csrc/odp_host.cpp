@@ -213,10 +213,12 @@ class ViewMaker {
 }  // namespace
 
 void add_vocabulary(py::module_& m);  // odp_host_vocab.cpp
+void add_block(py::module_& m);       // odp_host_block.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-  m.doc() = "Host-side helpers of opaque_amd: plan reuse, and the vocabulary operators' calls (no device code).";
+  m.doc() = "Host-side helpers of opaque_amd: plan reuse, and the vocabulary's and the block's operators' calls (no device code).";
   add_vocabulary(m);
+  add_block(m);
   m.def("lora_signature", &lora_signature, py::arg("sites"), py::arg("ptrs"));
   py::class_<ViewMaker>(m, "ViewMaker")
       .def(py::init<std::vector<int64_t>, std::vector<std::vector<int64_t>>, std::vector<std::vector<int64_t>>,

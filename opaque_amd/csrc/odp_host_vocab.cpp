@@ -5,19 +5,12 @@
 // The same calls in Python cost 100 us (a lookup and its gradient) to 180 us
 // (a loss and its gradients) of host time, most of it in the backward pass,
 // whose thread takes the interpreter lock; small batches are bound by that.
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-#include <c10/core/DeviceGuard.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/functions/utils.h>
-#include <torch/extension.h>
-
 #include <atomic>
 #include <memory>
 #include <string>
 #include <unordered_map>
 
-#include "../../include/opaque_dp.h"
+#include "odp_host_tensors.h"
 
 namespace py = pybind11;
 
@@ -73,63 +66,21 @@ void bind(const std::unordered_map<std::string, uintptr_t>& at) {
 
 void check(int rc, const char* what) { TORCH_CHECK(rc == ODP_OK, what, " failed with status ", rc, ": ", abi.last_error()); }
 
-int code_of(const at::Tensor& t) {
-  switch (t.scalar_type()) {
-    case at::kFloat: return ODP_DTYPE_F32;
-    case at::kBFloat16: return ODP_DTYPE_BF16;
-    case at::kHalf: return ODP_DTYPE_F16;
-    default: TORCH_CHECK_TYPE(false, "unsupported dtype ", t.scalar_type());
-  }
-}
+using odp_host::bytes_on;
+using odp_host::code_of;
+using odp_host::pitched;
+using odp_host::stream_of;
+using odp_host::up16;
 
-odp_stream_t stream_of(const at::Tensor& t) {
-  return reinterpret_cast<odp_stream_t>(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.get_device()).stream());
-}
-
-at::Tensor bytes_on(const at::Tensor& t, int64_t n) { return at::empty({n}, t.options().dtype(at::kByte)); }
-int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
-
-// Rows with unit column stride and a pitch of at least the width, copied if laid out otherwise.
-at::Tensor pitched(const at::Tensor& t) {
-  at::Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
-  if ((r.stride(1) != 1 && r.size(1) > 1) || r.stride(0) < r.size(1)) r = r.clone(at::MemoryFormat::Contiguous);
-  return r;
-}
-
-// A tangent on an input would be dropped without a word: the kernels read values.
-void no_tangent(const at::Tensor& t) {
-  TORCH_CHECK(!t._fw_grad(0).defined(), "the vocabulary operators have no forward-mode derivative");
-}
-
-// Ties a first derivative to what it depends on, so that asking for a second
-// one is an error instead of zero: to the gradient g it came from and, with
-// `inputs`, to the inputs of the node whose backward pass calls this (by
-// their edges: their values need not be kept).
+void no_tangent(const at::Tensor& t) { odp_host::no_tangent(t, "the vocabulary operators"); }
 at::Tensor first_only(const at::Tensor& g, at::Tensor d, bool inputs) {
-  if (!d.defined() || !at::GradMode::is_enabled()) return d;
-  torch::autograd::edge_list on;
-  if (inputs)
-    for (const auto& e : torch::autograd::get_current_node()->next_edges())
-      if (e.is_valid()) on.push_back(e);
-  if (g.requires_grad()) on.push_back(torch::autograd::impl::gradient_edge(g));
-  if (on.empty()) return d;
-  const auto error = std::make_shared<torch::autograd::Error>(
-      "the vocabulary operators have no second derivative", std::move(on));
-  d = d.detach();
-  torch::autograd::set_history(d, error);
-  return d;
+  return odp_host::first_only({g}, std::move(d), inputs, "the vocabulary operators");
 }
-
-// What comes back from autograd is what was saved, wherever its hooks had it
-// meanwhile: the kernels take addresses.
 void as_saved(const at::Tensor& t, const at::Tensor& like, at::ScalarType type, at::IntArrayRef shape) {
-  TORCH_CHECK(t.device() == like.device() && t.scalar_type() == type && t.sizes() == shape,
-              "vocabulary operators: a saved tensor came back as ", t.scalar_type(), " ", t.sizes(), " on ", t.device(),
-              ", not as ", type, " ", shape, " on ", like.device());
+  odp_host::as_saved(t, like, type, shape, "vocabulary operators");
 }
 at::Tensor whole(const at::Tensor& t, const at::Tensor& like, at::ScalarType type, at::IntArrayRef shape) {
-  as_saved(t, like, type, shape);
-  return t.contiguous();
+  return odp_host::whole(t, like, type, shape, "vocabulary operators");
 }
 
 // ---------------------------------------------------------------------------

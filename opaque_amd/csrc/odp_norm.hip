@@ -1,0 +1,656 @@
+// The root-mean-square norm behind the residual stream's addition, its
+// gradients and its output in 8 bits.
+//
+//   h = x + r, as the stream's type holds it (h = x without a residual)
+//   u = h / sqrt(mean(h^2) + eps),  y = u w                        k_rms_norm
+//   a = gy w,  dh = (a - u mean(a u)) / sqrt(..) + gh,
+//   dw_i = sum of gy u over the rows of gain i      k_rms_norm_grad, k_gain_sum
+//   scale = max(max |y| / 448, the least normal float32) of a row or of 128
+//   columns of it, q = y / scale in e4m3
+//
+// Every pass reads and writes its tensors once: bound by HBM.  A row is held in
+// registers between the sum of its squares and its output, 8 values a vector:
+// T threads of NV vectors, T from 8 (rows of up to 64 values, 32 rows a
+// workgroup) through one wave to a workgroup of 1024 (32768 values).  A gain of
+// its own for every group of rows (an example's) costs no launch more.  The
+// gains' gradient is summed in registers along a strip of rows, then over the
+// strips: no atomics, so results do not depend on the order of execution.
+//
+// Vectors of 16 bytes are loaded at any address (this target's global loads
+// need no more than the type's own alignment), so odd widths run as even ones
+// do, but for the last vector of a row.
+#include <cmath>
+
+#include "odp_internal.h"
+
+namespace {
+
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+// The same at any 2- or 4-byte address.
+typedef u32x4_t u32x4_h __attribute__((aligned(2)));
+typedef u32x4_t u32x4_w __attribute__((aligned(4)));
+typedef u32x2_t u32x2_b __attribute__((aligned(1)));
+
+// What a thread holds of a row: 8 values of float32 (F32) or of a 16-bit type,
+// as they lie in memory.
+template <bool F32>
+struct Eight {
+  u32x4_t w[F32 ? 2 : 1];
+
+  // Values c to c + 8 of a row of `width` (0 past it).
+  __device__ __forceinline__ void load(const char* row, int c, int width) {
+    if (c + 8 <= width) {
+      if constexpr (F32) {
+        const ODP_GMEM u32x4_w* p = (const ODP_GMEM u32x4_w*)(const ODP_GMEM void*)(row + 4 * c);
+        w[0] = p[0];
+        w[1] = p[1];
+      } else {
+        w[0] = *(const ODP_GMEM u32x4_h*)(const ODP_GMEM void*)(row + 2 * c);
+      }
+      return;
+    }
+    w[0] = u32x4_t{0, 0, 0, 0};
+    if constexpr (F32) w[1] = w[0];
+    if (c >= width) return;
+#pragma unroll
+    for (int i = 0; i < 7; ++i) {
+      if (c + i >= width) break;
+      if constexpr (F32) w[i / 4][i % 4] = ((const uint32_t*)row)[c + i];
+      else w[0][i / 2] |= (uint32_t)((const uint16_t*)row)[c + i] << 16 * (i % 2);
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[8], int dt) const {
+    if constexpr (F32) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i / 4][i % 4]);
+    } else if (dt == ODP_DTYPE_BF16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[0][i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[0][i] & 0xffff0000u);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)w[0][i]);
+        v[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[0][i] >> 16));
+      }
+    }
+  }
+  // Rounded to nearest-even.
+  __device__ __forceinline__ void set(const float (&v)[8], int dt) {
+    if constexpr (F32) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i / 4][i % 4] = __float_as_uint(v[i]);
+    } else if (dt == ODP_DTYPE_BF16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[0][i] = odp_f2bf2(v[2 * i], v[2 * i + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[0][i] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2 * i]) |
+                  (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2 * i + 1]) << 16;
+    }
+  }
+  __device__ __forceinline__ void store(char* row, int c, int width) const {
+    if (c + 8 <= width) {
+      if constexpr (F32) {
+        ODP_GMEM u32x4_w* p = (ODP_GMEM u32x4_w*)(ODP_GMEM void*)(row + 4 * c);
+        p[0] = w[0];
+        p[1] = w[1];
+      } else {
+        *(ODP_GMEM u32x4_h*)(ODP_GMEM void*)(row + 2 * c) = w[0];
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 7; ++i) {
+      if (c + i >= width) break;
+      if constexpr (F32) odp_gstore((uint32_t*)row + c + i, w[i / 4][i % 4]);
+      else odp_gstore((uint16_t*)row + c + i, (uint16_t)(w[0][i / 2] >> 16 * (i % 2)));
+    }
+  }
+};
+
+// 8 gains of the run-time type dt, 1 where there are none.
+__device__ __forceinline__ void load_gain(float (&g)[8], const char* row, int dt, float offset, int c, int width) {
+  if (row == nullptr) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) g[i] = 1.0f;
+    return;
+  }
+  if (dt == ODP_DTYPE_F32) {
+    Eight<true> e;
+    e.load(row, c, width);
+    e.get(g, dt);
+  } else {
+    Eight<false> e;
+    e.load(row, c, width);
+    e.get(g, dt);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) g[i] += offset;
+}
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
+}
+__device__ __forceinline__ float dpp_add(float v, uint32_t o) { return v + __uint_as_float(o); }
+
+// Sum over T threads side by side (T <= 64), the same bits in each.
+template <int T>
+__device__ __forceinline__ float sum_lanes(float v) {
+  v = dpp_add(v, dpp_u32<0xB1>(__float_as_uint(v)));                    // quad_perm 1,0,3,2
+  v = dpp_add(v, dpp_u32<0x4E>(__float_as_uint(v)));                    // quad_perm 2,3,0,1
+  v = dpp_add(v, dpp_u32<0x141>(__float_as_uint(v)));                   // row_half_mirror
+  if constexpr (T >= 16) v = dpp_add(v, dpp_u32<0x140>(__float_as_uint(v)));  // row_mirror
+  if constexpr (T >= 32) v += __shfl_xor(v, 16);
+  if constexpr (T >= 64) v += __shfl_xor(v, 32);
+  return v;
+}
+template <int T>
+__device__ __forceinline__ uint32_t max_lanes(uint32_t v) {
+  v = max(v, dpp_u32<0xB1>(v));
+  v = max(v, dpp_u32<0x4E>(v));
+  v = max(v, dpp_u32<0x141>(v));
+  if constexpr (T >= 16) v = max(v, dpp_u32<0x140>(v));
+  if constexpr (T >= 32) v = max(v, (uint32_t)__shfl_xor((int)v, 16));
+  if constexpr (T >= 64) v = max(v, (uint32_t)__shfl_xor((int)v, 32));
+  return v;
+}
+
+// Over the T threads of a row; for T > 64 through `red` [2][T / 64], the half
+// of it that `turn` names, so that one barrier a row is enough.
+template <int T>
+__device__ __forceinline__ float sum_row(float v, float* red, int turn) {
+  if constexpr (T <= 64) return sum_lanes<T>(v);
+  constexpr int W = T / 64;
+  float* r = red + W * (turn & 1);
+  v = sum_lanes<64>(v);
+  if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < W; ++i) s += r[i];
+  return s;
+}
+template <int T>
+__device__ __forceinline__ uint32_t max_row(uint32_t v, float* red, int turn) {
+  if constexpr (T <= 64) return max_lanes<T>(v);
+  constexpr int W = T / 64;
+  float* r = red + W * (turn & 1);
+  v = max_lanes<64>(v);
+  if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = __uint_as_float(v);
+  __syncthreads();
+  uint32_t s = 0;
+#pragma unroll
+  for (int i = 0; i < W; ++i) s = max(s, __float_as_uint(r[i]));
+  return s;
+}
+
+struct NormArgs {
+  const char *x, *r, *gain;
+  char *y, *h;
+  float *rstd, *scales;
+  int64_t ldx, ldr, ldg, n;  // pitches in bytes
+  int64_t rows_per_gain;
+  int width, dt, ht, gt;
+  float eps, offset;
+};
+
+enum { NQ_NONE = 0, NQ_ROW = 1, NQ_BLOCK = 2 };
+constexpr int NQ_COLS = 128;          // columns of a block
+constexpr float NQ_MOST = 448.0f;     // the largest e4m3 value
+constexpr float NQ_LEAST = 1.17549435e-38f;
+
+template <int T>
+constexpr int norm_threads() { return T < 256 ? 256 : T; }
+
+template <bool XF, bool HF, int T, int NV, int Q>
+__global__ __launch_bounds__(norm_threads<T>()) void k_rms_norm(const NormArgs a) {
+  constexpr int ROWS = norm_threads<T>() / T;
+  __shared__ float red[2][T > 64 ? T / 64 : 1];
+  const int t = T < 256 ? (int)(threadIdx.x % T) : (int)threadIdx.x;
+  int64_t row = (int64_t)blockIdx.x * ROWS + (T < 256 ? (int)(threadIdx.x / T) : 0);
+  const bool live = row < a.n;
+  row = live ? row : a.n - 1;
+  const int width = a.width;
+  Eight<XF> x[NV];
+  Eight<HF> r[NV];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) x[v].load(a.x + row * a.ldx, 8 * (v * T + t), width);
+  if (a.r != nullptr) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) r[v].load(a.r + row * a.ldr, 8 * (v * T + t), width);
+  }
+  float f[NV][8], sum = 0.0f;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    x[v].get(f[v], a.dt);
+    if (a.r != nullptr) {
+      const int c = 8 * (v * T + t);
+      float o[8];
+      r[v].get(o, a.ht);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[v][i] += o[i];
+      r[v].set(f[v], a.ht);
+      if (live) r[v].store(a.h + row * width * (HF ? 4 : 2), c, width);
+      r[v].get(f[v], a.ht);  // the norm is of what is stored
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum = fmaf(f[v][i], f[v][i], sum);
+  }
+  sum = sum_row<T>(sum, red[0], 0);
+  const float inv = 1.0f / sqrtf(sum / (float)width + a.eps);
+  if (a.rstd != nullptr && t == 0 && live) odp_gstore(a.rstd + row, inv);
+  const char* gain = a.gain == nullptr ? nullptr : a.gain + (a.ldg ? row / a.rows_per_gain * a.ldg : 0);
+  uint32_t most = 0;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int c = 8 * (v * T + t);
+    float g[8];
+    load_gain(g, gain, a.gt, a.offset, c, width);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[v][i] = f[v][i] * inv * g[i];
+    if constexpr (Q == NQ_NONE) {
+      Eight<XF> y;
+      y.set(f[v], a.dt);
+      if (live) y.store(a.y + row * width * (XF ? 4 : 2), c, width);
+    } else {
+      uint32_t m = 0;  // by the bits of |y|, above which those of infinities and NaN lie
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = max(m, c + i < width ? __float_as_uint(f[v][i]) & 0x7fffffffu : 0u);
+      if constexpr (Q == NQ_ROW) {
+        most = max(most, m);
+      } else {
+        m = max_lanes<(T < 16 ? T : 16)>(m);  // 16 threads of 8 values
+        const float scale = fmaxf(__uint_as_float(m) / NQ_MOST, NQ_LEAST);
+        const float s = m > 0x7f800000u ? __uint_as_float(m) : scale;
+        if (live && (t & 15) == 0 && c < width)
+          odp_gstore(a.scales + row * ((width + NQ_COLS - 1) / NQ_COLS) + c / NQ_COLS, s);
+        const float by = 1.0f / s;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[v][i] *= by;
+      }
+    }
+  }
+  if constexpr (Q == NQ_NONE) return;
+  float by = 1.0f;
+  if constexpr (Q == NQ_ROW) {
+    most = max_row<T>(most, red[0], 1);
+    const float scale = fmaxf(__uint_as_float(most) / NQ_MOST, NQ_LEAST);
+    const float s = most > 0x7f800000u ? __uint_as_float(most) : scale;
+    if (live && t == 0) odp_gstore(a.scales + row, s);
+    by = 1.0f / s;
+  }
+  if (!live) return;
+  char* q = a.y + row * width;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int c = 8 * (v * T + t);
+    if (c >= width) continue;
+    u32x2_t w;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      int p = __builtin_amdgcn_cvt_pk_fp8_f32(f[v][4 * i] * by, f[v][4 * i + 1] * by, 0, false);
+      p = __builtin_amdgcn_cvt_pk_fp8_f32(f[v][4 * i + 2] * by, f[v][4 * i + 3] * by, p, true);
+      w[i] = (uint32_t)p;
+    }
+    if (c + 8 <= width) {
+      *(ODP_GMEM u32x2_b*)(ODP_GMEM void*)(q + c) = w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 7; ++i)
+        if (c + i < width) odp_gstore((uint8_t*)q + c + i, (uint8_t)(w[i / 4] >> 8 * (i % 4)));
+    }
+  }
+}
+
+struct NormGradArgs {
+  const char *h, *gy, *gh, *gain;
+  const float* rstd;
+  char *dx, *dr, *dw;
+  float* part;
+  int64_t ldh, ldy, ldgh, ldg;  // pitches in bytes
+  int64_t rows_per_gain, len, strips;
+  int width, dt, ht, gt;
+  float offset;
+};
+
+// Workgroup (gain, strip): rows [strip len, ..) of that gain's rows.
+template <bool XF, bool HF, int T, int NV>
+__global__ __launch_bounds__(norm_threads<T>()) void k_rms_norm_grad(const NormGradArgs a) {
+  constexpr int ROWS = norm_threads<T>() / T;
+  __shared__ float red[2][T > 64 ? T / 64 : 1];
+  __shared__ float joined[ROWS > 1 ? ROWS * T * NV * 8 : 1];
+  const int t = T < 256 ? (int)(threadIdx.x % T) : (int)threadIdx.x;
+  const int slot = T < 256 ? (int)(threadIdx.x / T) : 0;
+  const int64_t group = blockIdx.x / a.strips, strip = blockIdx.x - group * a.strips;
+  const int64_t first = group * a.rows_per_gain + strip * a.len;
+  const int64_t last = group * a.rows_per_gain + min((strip + 1) * a.len, a.rows_per_gain);
+  const int width = a.width;
+  const char* gain = a.gain == nullptr ? nullptr : a.gain + group * a.ldg;
+  float g[NV][8], acc[NV][8];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    load_gain(g[v], gain, a.gt, a.offset, 8 * (v * T + t), width);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[v][i] = 0.0f;
+  }
+  int turn = 0;
+  for (int64_t base = first; base < last; base += ROWS, ++turn) {
+    int64_t row = base + slot;
+    const bool live = row < last;
+    row = live ? row : last - 1;
+    Eight<HF> h[NV], gh[NV];
+    Eight<XF> gy[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      h[v].load(a.h + row * a.ldh, 8 * (v * T + t), width);
+      gy[v].load(a.gy + row * a.ldy, 8 * (v * T + t), width);
+    }
+    if (a.gh != nullptr && a.dx != nullptr) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) gh[v].load(a.gh + row * a.ldgh, 8 * (v * T + t), width);
+    }
+    const float inv = a.rstd[row];
+    float u[NV][8], dot = 0.0f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      float d[8];
+      h[v].get(u[v], a.ht);
+      gy[v].get(d, a.dt);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        u[v][i] *= inv;
+        const float p = d[i] * u[v][i];
+        acc[v][i] += live ? p : 0.0f;
+        dot = fmaf(p, g[v][i], dot);
+      }
+    }
+    if (a.dx == nullptr) continue;
+    const float mean = sum_row<T>(dot, red[0], turn) / (float)width;
+    if (!live) continue;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = 8 * (v * T + t);
+      float d[8];
+      gy[v].get(d, a.dt);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) d[i] = inv * (d[i] * g[v][i] - u[v][i] * mean);
+      if (a.gh != nullptr) {
+        float o[8];
+        gh[v].get(o, a.ht);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[i] += o[i];
+      }
+      if (a.dr != nullptr) {
+        Eight<HF> out;
+        out.set(d, a.ht);
+        out.store(a.dr + row * width * (HF ? 4 : 2), c, width);
+      }
+      Eight<XF> out;
+      out.set(d, a.dt);
+      out.store(a.dx + row * width * (XF ? 4 : 2), c, width);
+    }
+  }
+  if (a.part == nullptr && a.dw == nullptr) return;
+  if constexpr (ROWS > 1) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) joined[(slot * NV + v) * T * 8 + t * 8 + i] = acc[v][i];
+    __syncthreads();
+    if (slot != 0) return;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        for (int s = 1; s < ROWS; ++s) acc[v][i] += joined[(s * NV + v) * T * 8 + t * 8 + i];
+  }
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int c = 8 * (v * T + t);
+    if (a.part != nullptr) {
+      Eight<true> out;
+      out.set(acc[v], ODP_DTYPE_F32);
+      out.store((char*)(a.part + (int64_t)blockIdx.x * width), c, width);
+    } else if (a.gt == ODP_DTYPE_F32) {
+      Eight<true> out;
+      out.set(acc[v], a.gt);
+      out.store(a.dw + group * width * 4, c, width);
+    } else {
+      Eight<false> out;
+      out.set(acc[v], a.gt);
+      out.store(a.dw + group * width * 2, c, width);
+    }
+  }
+}
+
+// dw of 64 columns of one gain: 16 waves sum every 16th strip, then each other.
+__global__ __launch_bounds__(1024) void k_gain_sum(const float* __restrict__ part, int64_t strips, int width, int tiles,
+                                                   int gt, void* dw) {
+  __shared__ float red[16][64];
+  const int64_t group = blockIdx.x / tiles;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = (int)(blockIdx.x - group * tiles) * 64 + lane;
+  const float* p = part + group * strips * width + c;
+  float s = 0.0f;
+  if (c < width) {
+    int64_t i = wave;
+    for (; i + 16 * 3 < strips; i += 16 * 4) {
+      float v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = p[(i + 16 * k) * width];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s += v[k];
+    }
+    for (; i < strips; i += 16) s += p[i * width];
+  }
+  red[wave][lane] = s;
+  __syncthreads();
+  if (wave != 0 || c >= width) return;
+#pragma unroll
+  for (int i = 1; i < 16; ++i) s += red[i][lane];
+  odp_store_from_float(dw, group * width + c, gt, s);
+}
+
+// Strips of a gain's rows: about four workgroups a compute unit in all.
+struct Strips {
+  int64_t len, count;
+};
+constexpr int64_t NORM_GROUPS = 1024;
+
+int norm_tile(int64_t width) {  // threads of a row
+  const int64_t v = (width + 7) / 8;
+  return v <= 8 ? 8 : v <= 16 ? 16 : v <= 32 ? 32 : v <= 256 ? 64 : v <= 1024 ? 256 : 1024;
+}
+
+Strips strips_of(int64_t n, int64_t width, int64_t gains) {
+  const int64_t rows = n / gains;
+  const int t = norm_tile(width), at = t < 256 ? 256 / t : 1;
+  int64_t count = (NORM_GROUPS + gains - 1) / gains;
+  int64_t len = (rows + count - 1) / count;
+  len = (len + at - 1) / at * at;
+  if (len < 1) len = 1;
+  return {len, rows > 0 ? (rows + len - 1) / len : 1};
+}
+
+bool norm_type(int dt) { return dt == ODP_DTYPE_F32 || dt == ODP_DTYPE_BF16 || dt == ODP_DTYPE_F16; }
+
+template <bool XF, bool HF, int T, int NV>
+void launch_norm(hipStream_t s, const NormArgs& a, int q) {
+  constexpr int TH = norm_threads<T>();
+  const uint32_t blocks = (uint32_t)((a.n + TH / T - 1) / (TH / T));
+  if (q == NQ_NONE) k_rms_norm<XF, HF, T, NV, NQ_NONE><<<blocks, TH, 0, s>>>(a);
+  else if (q == NQ_ROW) k_rms_norm<XF, HF, T, NV, NQ_ROW><<<blocks, TH, 0, s>>>(a);
+  else k_rms_norm<XF, HF, T, NV, NQ_BLOCK><<<blocks, TH, 0, s>>>(a);
+}
+template <bool XF, bool HF, int T, int NV>
+void launch_grad(hipStream_t s, const NormGradArgs& a, int64_t blocks) {
+  k_rms_norm_grad<XF, HF, T, NV><<<(uint32_t)blocks, norm_threads<T>(), 0, s>>>(a);
+}
+
+// The narrowest form whose registers hold a row.
+#define ODP_NORM_FORM(CALL)                                 \
+  do {                                                      \
+    const int64_t v = (a.width + 7) / 8;                    \
+    if (v <= 8) CALL(8, 1);                                 \
+    else if (v <= 16) CALL(16, 1);                          \
+    else if (v <= 32) CALL(32, 1);                          \
+    else if (v <= 64) CALL(64, 1);                          \
+    else if (v <= 128) CALL(64, 2);                         \
+    else if (v <= 256) CALL(64, 4);                         \
+    else if (v <= 512) CALL(256, 2);                        \
+    else if (v <= 1024) CALL(256, 4);                       \
+    else if (v <= 2048) CALL(1024, 2);                      \
+    else CALL(1024, 4);                                     \
+  } while (0)
+
+template <bool XF, bool HF>
+void norm_form(hipStream_t s, const NormArgs& a, int q) {
+#define ODP_CALL(T, NV) launch_norm<XF, HF, T, NV>(s, a, q)
+  ODP_NORM_FORM(ODP_CALL);
+#undef ODP_CALL
+}
+template <bool XF, bool HF>
+void grad_form(hipStream_t s, const NormGradArgs& a, int64_t blocks) {
+#define ODP_CALL(T, NV) launch_grad<XF, HF, T, NV>(s, a, blocks)
+  ODP_NORM_FORM(ODP_CALL);
+#undef ODP_CALL
+}
+
+int norm_check(const char* what, int dt, int ht, int gt, int64_t n, int64_t width, int64_t gains) {
+  if (!norm_type(dt) || !(ht == dt || ht == ODP_DTYPE_F32) || !(gt == dt || gt == ODP_DTYPE_F32)) {
+    odp_set_error("%s: types %d (rows), %d (stream), %d (gain): a 16-bit type or float32, the others the same or float32",
+                  what, dt, ht, gt);
+    return ODP_ERR_UNSUPPORTED;
+  }
+  if (n < 0 || n >= (int64_t)1 << 31 || width < 1 || width > ODP_NORM_WIDE) {
+    odp_set_error("%s: %lld rows of %lld: fewer than 2^31 rows of 1 to %lld", what, (long long)n, (long long)width,
+                  (long long)ODP_NORM_WIDE);
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  if (gains < 1 || n % gains != 0) {
+    odp_set_error("%s: %lld rows do not divide into %lld gains", what, (long long)n, (long long)gains);
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  return ODP_OK;
+}
+
+}  // namespace
+
+extern "C" int odp_rms_norm(odp_stream_t stream, int dtype, int stream_dtype, int gain_dtype, const void* x,
+                            int64_t ldx, const void* residual, int64_t ldr, int64_t n, int64_t width, const void* gain,
+                            int64_t ldg, int64_t gains, float eps, float offset, int quant, void* y, void* sum,
+                            float* rstd, float* scales) {
+  const char* what = "odp_rms_norm";
+  const int rc = norm_check(what, dtype, stream_dtype, gain_dtype, n, width, gains);
+  if (rc != ODP_OK) return rc;
+  if (quant < NQ_NONE || quant > NQ_BLOCK) {
+    odp_set_error("%s: quant %d: 0 (none), 1 (a scale per row) or 2 (per 128 columns)", what, quant);
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  if (n == 0) return ODP_OK;
+  if (x == nullptr || y == nullptr || (residual == nullptr) != (sum == nullptr) ||
+      (quant != NQ_NONE) != (scales != nullptr)) {
+    odp_set_error("%s: null x or y, a residual without its sum, or scales without quant (or the other way round)", what);
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  if (ldx < width || (residual != nullptr && ldr < width) || (gain != nullptr && ldg != 0 && ldg < width)) {
+    odp_set_error("%s: a pitch is less than the width %lld", what, (long long)width);
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  NormArgs a;
+  a.x = (const char*)x;
+  a.r = (const char*)residual;
+  a.gain = (const char*)gain;
+  a.y = (char*)y;
+  a.h = (char*)sum;
+  a.rstd = rstd;
+  a.scales = scales;
+  a.ldx = ldx * odp_dtype_size(dtype);
+  a.ldr = ldr * odp_dtype_size(stream_dtype);
+  a.ldg = ldg * odp_dtype_size(gain_dtype);
+  a.n = n;
+  a.rows_per_gain = n / gains;
+  a.width = (int)width;
+  a.dt = dtype;
+  a.ht = stream_dtype;
+  a.gt = gain_dtype;
+  a.eps = eps;
+  a.offset = offset;
+  hipStream_t s = odp_hip_stream(stream);
+  if (dtype == ODP_DTYPE_F32) norm_form<true, true>(s, a, quant);
+  else if (stream_dtype == ODP_DTYPE_F32 && residual != nullptr) norm_form<false, true>(s, a, quant);
+  else norm_form<false, false>(s, a, quant);
+  return odp_check_launch(what);
+}
+
+extern "C" int64_t odp_rms_norm_grad_scratch(int64_t n, int64_t width, int64_t gains) {
+  if (n <= 0 || width < 1 || width > ODP_NORM_WIDE || gains < 1 || n % gains != 0) return 0;
+  const Strips s = strips_of(n, width, gains);
+  return s.count > 1 ? 4 * gains * s.count * width : 0;
+}
+
+extern "C" int odp_rms_norm_grad(odp_stream_t stream, int dtype, int stream_dtype, int gain_dtype, const void* h,
+                                 int64_t ldh, const float* rstd, const void* gy, int64_t ldy, const void* gh,
+                                 int64_t ldgh, int64_t n, int64_t width, const void* gain, int64_t ldg, int64_t gains,
+                                 float offset, void* scratch, void* dx, void* dres, void* dgain) {
+  const char* what = "odp_rms_norm_grad";
+  const int rc = norm_check(what, dtype, stream_dtype, gain_dtype, n, width, gains);
+  if (rc != ODP_OK) return rc;
+  if (n == 0) return ODP_OK;
+  if (h == nullptr || rstd == nullptr || gy == nullptr || (dres != nullptr && dx == nullptr)) {
+    odp_set_error("%s: null h, rstd or gy, or the residual's gradient without x's", what);
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  if (ldh < width || ldy < width || (gh != nullptr && ldgh < width) || (gain != nullptr && ldg != 0 && ldg < width)) {
+    odp_set_error("%s: a pitch is less than the width %lld", what, (long long)width);
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  if (dx == nullptr && dgain == nullptr) return ODP_OK;
+  const Strips st = strips_of(n, width, gains);
+  if (dgain != nullptr && st.count > 1 && scratch == nullptr) {
+    odp_set_error("%s: null scratch where odp_rms_norm_grad_scratch is not 0", what);
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  NormGradArgs a;
+  a.h = (const char*)h;
+  a.gy = (const char*)gy;
+  a.gh = (const char*)gh;
+  a.gain = (const char*)gain;
+  a.rstd = rstd;
+  a.dx = (char*)dx;
+  a.dr = (char*)dres;
+  a.dw = dgain != nullptr && st.count == 1 ? (char*)dgain : nullptr;
+  a.part = dgain != nullptr && st.count > 1 ? (float*)scratch : nullptr;
+  a.ldh = ldh * odp_dtype_size(stream_dtype);
+  a.ldy = ldy * odp_dtype_size(dtype);
+  a.ldgh = ldgh * odp_dtype_size(stream_dtype);
+  a.ldg = ldg * odp_dtype_size(gain_dtype);
+  a.rows_per_gain = n / gains;
+  a.len = st.len;
+  a.strips = st.count;
+  a.width = (int)width;
+  a.dt = dtype;
+  a.ht = stream_dtype;
+  a.gt = gain_dtype;
+  a.offset = offset;
+  hipStream_t s = odp_hip_stream(stream);
+  const int64_t blocks = gains * st.count;  // at most n
+  if (dtype == ODP_DTYPE_F32) grad_form<true, true>(s, a, blocks);
+  else if (stream_dtype == ODP_DTYPE_F32) grad_form<false, true>(s, a, blocks);
+  else grad_form<false, false>(s, a, blocks);
+  if (a.part != nullptr) {
+    const int tiles = (int)((width + 63) / 64);
+    if (gains * tiles >= (int64_t)1 << 31) {
+      odp_set_error("%s: too many gains", what);
+      return ODP_ERR_UNSUPPORTED;
+    }
+    k_gain_sum<<<(uint32_t)(gains * tiles), 1024, 0, s>>>(a.part, st.count, (int)width, tiles, gain_dtype, dgain);
+  }
+  return odp_check_launch(what);
+}

@@ -1,0 +1,306 @@
+// The norm of a whole tree of gradients, and the tree scaled to keep below a
+// bound.
+//
+//   norm = sqrt(sum over all leaves of x^2)                k_tree_squares
+//   out = x min(1, bound / norm)                           k_tree_scale
+//
+// Two passes, since no element can be scaled before the last has been read:
+// bound by HBM.  Leaves travel in the kernels' arguments (TN_LEAVES a launch),
+// so a call copies no table and may be captured.  Squares are exact in float64
+// and added there: no overflow, and sums that do not depend on how a tree is cut
+// into leaves by more than 2^-53 of their size a step.  The second pass walks the
+// chunks backwards, the last read first, which the 256 MB cache still holds.
+// Every workgroup adds the first pass's partials for itself, in one order, so
+// neither a third launch nor an atomic is needed.
+#include <cmath>
+
+#include "odp_internal.h"
+
+namespace {
+
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef u32x4_t u32x4_h __attribute__((aligned(2)));  // at any address that a 16-bit type may have
+
+constexpr int TN_LEAVES = 128;   // of a launch: the arguments stay below 4 KB
+constexpr int TN_BLOCKS = 512;   // workgroups of a launch, two a compute unit
+constexpr int TN_THREADS = 1024;
+
+struct Leaves {
+  const char* src[TN_LEAVES];
+  char* dst[TN_LEAVES];
+  int64_t n[TN_LEAVES];
+  int32_t start[TN_LEAVES];  // first chunk
+  uint8_t dt[TN_LEAVES];
+  int32_t count, chunks, chunk;  // leaves, chunks in all, elements of a chunk
+};
+static_assert(sizeof(Leaves) + 64 <= 4096, "a launch's arguments");
+
+// Elements of 16 bytes.
+__device__ __forceinline__ int lanes_of(int dt) { return dt == ODP_DTYPE_F64 ? 2 : dt == ODP_DTYPE_F32 ? 4 : 8; }
+
+// The leaf of a chunk.
+__device__ __forceinline__ int leaf_of(const Leaves& l, int chunk) {
+  int lo = 0, hi = l.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (l.start[mid] <= chunk) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ u32x4_t piece(const char* p) { return *(const ODP_GMEM u32x4_h*)(const ODP_GMEM void*)p; }
+
+template <int DT>
+__device__ __forceinline__ double squares(u32x4_t w, double s) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == ODP_DTYPE_F32) {
+      const double v = __uint_as_float(w[i]);
+      s = fma(v, v, s);
+    } else if constexpr (DT == ODP_DTYPE_F64) {
+      if (i & 1) continue;
+      const double v = __longlong_as_double((long long)((uint64_t)w[i + 1] << 32 | w[i]));
+      s = fma(v, v, s);
+    } else {
+      double a, b;
+      if constexpr (DT == ODP_DTYPE_BF16) {
+        a = __uint_as_float(w[i] << 16);
+        b = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        a = (float)__builtin_bit_cast(_Float16, (uint16_t)w[i]);
+        b = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[i] >> 16));
+      }
+      s = fma(a, a, s);
+      s = fma(b, b, s);
+    }
+  }
+  return s;
+}
+
+template <int DT>
+__device__ __forceinline__ u32x4_t scaled(u32x4_t w, float f, double d) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == ODP_DTYPE_F32) {
+      w[i] = __float_as_uint(__uint_as_float(w[i]) * f);
+    } else if constexpr (DT == ODP_DTYPE_F64) {
+      if (i & 1) continue;
+      const double v = __longlong_as_double((long long)((uint64_t)w[i + 1] << 32 | w[i])) * d;
+      const uint64_t u = (uint64_t)__double_as_longlong(v);
+      w[i] = (uint32_t)u;
+      w[i + 1] = (uint32_t)(u >> 32);
+    } else if constexpr (DT == ODP_DTYPE_BF16) {
+      w[i] = odp_f2bf2(__uint_as_float(w[i] << 16) * f, __uint_as_float(w[i] & 0xffff0000u) * f);
+    } else {
+      const float a = (float)__builtin_bit_cast(_Float16, (uint16_t)w[i]) * f;
+      const float b = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[i] >> 16)) * f;
+      w[i] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)a) |
+             (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)b) << 16;
+    }
+  }
+  return w;
+}
+
+constexpr int TN_FLIGHT = 4;  // 16-byte pieces of a thread in flight
+
+// One chunk's squares, or its scaled copy.
+template <int DT, bool SCALE>
+__device__ __forceinline__ double chunk_pass(const char* src, char* dst, int64_t n, float f, double d, double s) {
+  constexpr int E = DT == ODP_DTYPE_F64 ? 8 : DT == ODP_DTYPE_F32 ? 4 : 2, V = 16 / E;
+  const int pieces = (int)(n / V);
+  int i = threadIdx.x;
+  for (; i + (TN_FLIGHT - 1) * TN_THREADS < pieces; i += TN_FLIGHT * TN_THREADS) {
+    u32x4_t w[TN_FLIGHT];
+#pragma unroll
+    for (int k = 0; k < TN_FLIGHT; ++k) w[k] = piece(src + 16 * (int64_t)(i + k * TN_THREADS));
+#pragma unroll
+    for (int k = 0; k < TN_FLIGHT; ++k) {
+      if constexpr (SCALE)
+        *(ODP_GMEM u32x4_h*)(ODP_GMEM void*)(dst + 16 * (int64_t)(i + k * TN_THREADS)) = scaled<DT>(w[k], f, d);
+      else
+        s = squares<DT>(w[k], s);
+    }
+  }
+  for (; i < pieces; i += TN_THREADS) {
+    const u32x4_t w = piece(src + 16 * (int64_t)i);
+    if constexpr (SCALE) *(ODP_GMEM u32x4_h*)(ODP_GMEM void*)(dst + 16 * (int64_t)i) = scaled<DT>(w, f, d);
+    else s = squares<DT>(w, s);
+  }
+  const int64_t at = (int64_t)pieces * V + threadIdx.x;
+  if (at < n) {
+    const double v = odp_load_as_double(src, at, DT);
+    if constexpr (SCALE) {
+      if constexpr (DT == ODP_DTYPE_F64) odp_gstore((double*)dst + at, v * d);
+      else odp_store_from_float(dst, at, DT, (float)v * f);
+    } else {
+      s = fma(v, v, s);
+    }
+  }
+  return s;
+}
+
+template <bool SCALE>
+__device__ __forceinline__ double one_chunk(const Leaves& l, int c, float f, double d, double s) {
+  const int leaf = leaf_of(l, c), dt = l.dt[leaf];
+  const int64_t first = (int64_t)(c - l.start[leaf]) * l.chunk, n = min((int64_t)l.chunk, l.n[leaf] - first);
+  const int64_t at = first * odp_dtype_size(dt);
+  const char* src = l.src[leaf] + at;
+  char* dst = SCALE ? l.dst[leaf] + at : nullptr;
+  if (dt == ODP_DTYPE_BF16) return chunk_pass<ODP_DTYPE_BF16, SCALE>(src, dst, n, f, d, s);
+  if (dt == ODP_DTYPE_F32) return chunk_pass<ODP_DTYPE_F32, SCALE>(src, dst, n, f, d, s);
+  if (dt == ODP_DTYPE_F16) return chunk_pass<ODP_DTYPE_F16, SCALE>(src, dst, n, f, d, s);
+  return chunk_pass<ODP_DTYPE_F64, SCALE>(src, dst, n, f, d, s);
+}
+
+// Sum over the workgroup, the same bits in every thread.
+__device__ __forceinline__ double sum_block(double s, double* red) {
+  s = rows_sum4(row_sum16(s));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  double t = 0.0;
+#pragma unroll
+  for (int i = 0; i < TN_THREADS / 64; ++i) t += red[i];
+  return t;
+}
+
+__global__ __launch_bounds__(TN_THREADS) void k_tree_squares(const Leaves l, double* part) {
+  __shared__ double red[TN_THREADS / 64];
+  double s = 0.0;
+  for (int c = blockIdx.x; c < l.chunks; c += gridDim.x) s = one_chunk<false>(l, c, 0.0f, 0.0, s);
+  s = sum_block(s, red);
+  if (threadIdx.x == 0) odp_gstore(part + blockIdx.x, s);
+}
+
+__device__ __forceinline__ double factor_of(double norm, double most) {
+  return norm != norm ? norm : norm > most ? most / norm : 1.0;
+}
+
+__device__ __forceinline__ void store_norm(void* out, int wide, double norm) {
+  if (threadIdx.x != 0) return;
+  if (wide) odp_gstore((double*)out, norm);
+  else odp_gstore((float*)out, (float)norm);
+}
+
+// out: where the norm goes (null but in the first launch).
+__global__ __launch_bounds__(TN_THREADS) void k_tree_scale(const Leaves l, const double* __restrict__ part, int parts,
+                                                           double most, int wide, void* out) {
+  __shared__ double red[TN_THREADS / 64];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < parts; i += TN_THREADS) s += part[i];
+  const double norm = sqrt(sum_block(s, red));
+  if (out != nullptr && blockIdx.x == 0) store_norm(out, wide, norm);
+  const double d = factor_of(norm, most);
+  const float f = (float)d;
+  for (int c = l.chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) one_chunk<true>(l, c, f, d, 0.0);
+}
+
+// A small tree in one launch of one workgroup.
+__global__ __launch_bounds__(TN_THREADS) void k_tree_small(const Leaves l, int clip, double most, int wide, void* out) {
+  __shared__ double red[TN_THREADS / 64];
+  double s = 0.0;
+  for (int c = 0; c < l.chunks; ++c) s = one_chunk<false>(l, c, 0.0f, 0.0, s);
+  const double norm = sqrt(sum_block(s, red));
+  store_norm(out, wide, norm);
+  if (!clip) return;
+  const double d = factor_of(norm, most);
+  const float f = (float)d;
+  for (int c = l.chunks - 1; c >= 0; --c) one_chunk<true>(l, c, f, d, 0.0);
+}
+
+// A tree of few and small leaves is one workgroup's.
+constexpr int64_t TN_SMALL = 16384, TN_FEW = 8;
+
+// The next launch's leaves from row `i` on; how many rows it took.
+int64_t fill(Leaves& l, const int64_t* rows, int64_t n_leaves, int64_t i, int64_t chunk) {
+  int64_t took = 0, chunks = 0;
+  l.count = 0;
+  l.chunk = (int)chunk;
+  for (; i + took < n_leaves && l.count < TN_LEAVES; ++took) {
+    const int64_t* r = rows + (i + took) * ODP_TN_FIELDS;
+    if (r[ODP_TN_N] == 0) continue;
+    const int64_t more = (r[ODP_TN_N] + chunk - 1) / chunk;
+    if (chunks + more > INT32_MAX) break;
+    const int k = l.count++;
+    l.src[k] = (const char*)r[ODP_TN_SRC];
+    l.dst[k] = (char*)r[ODP_TN_DST];
+    l.n[k] = r[ODP_TN_N];
+    l.dt[k] = (uint8_t)r[ODP_TN_DTYPE];
+    l.start[k] = (int32_t)chunks;
+    chunks += more;
+  }
+  l.chunks = (int32_t)chunks;
+  return took;
+}
+
+}  // namespace
+
+extern "C" int64_t odp_tree_norm_scratch(int64_t n_leaves) {
+  return n_leaves <= 0 ? 8 : 8 * TN_BLOCKS * ((n_leaves + TN_LEAVES - 1) / TN_LEAVES);
+}
+
+extern "C" int odp_tree_norm(odp_stream_t stream, const int64_t* leaves, int64_t n_leaves, int clip, double max_norm,
+                             int wide, void* scratch, void* norm) {
+  const char* what = "odp_tree_norm";
+  if (n_leaves < 0 || (n_leaves > 0 && leaves == nullptr) || scratch == nullptr || norm == nullptr) {
+    odp_set_error("%s: null pointer or %lld leaves", what, (long long)n_leaves);
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  if (clip && !(max_norm >= 0.0)) {
+    odp_set_error("%s: max_norm %g must be 0 or more", what, max_norm);
+    return ODP_ERR_INVALID_ARGUMENT;
+  }
+  int64_t total = 0, used = 0;
+  for (int64_t i = 0; i < n_leaves; ++i) {
+    const int64_t* r = leaves + i * ODP_TN_FIELDS;
+    const int64_t n = r[ODP_TN_N], dt = r[ODP_TN_DTYPE];
+    if (n < 0 || n > (int64_t)1 << 44 || total > (int64_t)1 << 45) {
+      odp_set_error("%s: leaf %lld has %lld elements", what, (long long)i, (long long)n);
+      return ODP_ERR_INVALID_ARGUMENT;
+    }
+    if (dt < ODP_DTYPE_F32 || dt > ODP_DTYPE_F64) {
+      odp_set_error("%s: leaf %lld has dtype %lld", what, (long long)i, (long long)dt);
+      return ODP_ERR_UNSUPPORTED;
+    }
+    if (n > 0 && (r[ODP_TN_SRC] == 0 || (clip && r[ODP_TN_DST] == 0))) {
+      odp_set_error("%s: leaf %lld has a null pointer", what, (long long)i);
+      return ODP_ERR_INVALID_ARGUMENT;
+    }
+    total += n;
+    used += n > 0;
+  }
+  hipStream_t s = odp_hip_stream(stream);
+  Leaves l;
+  if (total <= TN_SMALL && used <= TN_FEW) {
+    fill(l, leaves, n_leaves, 0, TN_SMALL);
+    k_tree_small<<<1, TN_THREADS, 0, s>>>(l, clip, max_norm, wide, norm);
+    return odp_check_launch(what);
+  }
+  // Chunks of what all threads have in flight at once, or four of it where that
+  // leaves each workgroup several.
+  int64_t chunk = 8 * TN_THREADS * TN_FLIGHT;
+  while (chunk > 2048 && total / chunk < 2 * TN_BLOCKS) chunk >>= 1;
+  while (total / chunk > (int64_t)1 << 28) chunk <<= 1;
+  double* part = (double*)scratch;
+  int64_t parts = 0;
+  for (int64_t i = 0; i < n_leaves;) {
+    i += fill(l, leaves, n_leaves, i, chunk);
+    if (l.chunks == 0) continue;
+    const int blocks = l.chunks < TN_BLOCKS ? l.chunks : TN_BLOCKS;
+    k_tree_squares<<<blocks, TN_THREADS, 0, s>>>(l, part + parts);
+    parts += blocks;
+  }
+  if (!clip) {
+    l.chunks = l.count = 0;
+    k_tree_scale<<<1, TN_THREADS, 0, s>>>(l, part, (int)parts, 0.0, wide, norm);
+    return odp_check_launch(what);
+  }
+  bool told = false;
+  for (int64_t i = 0; i < n_leaves;) {
+    i += fill(l, leaves, n_leaves, i, chunk);
+    if (l.chunks == 0) continue;
+    const int blocks = l.chunks < TN_BLOCKS ? l.chunks : TN_BLOCKS;
+    k_tree_scale<<<blocks, TN_THREADS, 0, s>>>(l, part, (int)parts, max_norm, wide, told ? nullptr : norm);
+    told = true;
+  }
+  return odp_check_launch(what);
+}

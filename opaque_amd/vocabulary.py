@@ -70,8 +70,9 @@ def _bound():
     if not _host_ready:
         host, lib = _host.load(), N.load()
         if host is not None:
-            host.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
-                       for name in N.exported_symbols()})
+            at = {name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in N.exported_symbols()}
+            host.bind(at)
+            host.bind_block(at)
         _host_ready.append(host)
     return _host_ready[0]
 

@@ -1,0 +1,219 @@
+"""clip_by_global_norm and global_norm against the formula in 64 bits.
+
+Squares are exact in float64 and their sums are off by at most n 2^-53 (below 2^-26 for the sizes here), so the norm is
+the exact one rounded to float32 (one step of 2^-24 where the rounding lies on the border).  Scaled values are off by
+the factor's rounding and the product's, 2 steps of 2^-24, and half a step of the leaf's type.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from opaque_amd import vocabulary
+from opaque_amd.global_norm import clip_by_global_norm, global_norm
+from opaque_amd.types import clipped, noised
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+F32, BF16, F16, F64 = torch.float32, torch.bfloat16, torch.float16, torch.float64
+U = 2.0**-24
+
+
+@pytest.fixture(params=[True, False], ids=["helper", "python"])
+def path(request, monkeypatch):
+    if not request.param:
+        monkeypatch.setattr(vocabulary, "_host_ready", [None])
+
+
+def tree(sizes, dtypes, seed=0, scale=1.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    out = {}
+    for i, n in enumerate(sizes):
+        dt = dtypes[i % len(dtypes)]
+        out[f"k{i:03d}"] = (scale * torch.randn(n, generator=g, device=DEV, dtype=torch.float64)).to(dt)
+    return out
+
+
+def check(grads, bound):
+    leaves = list(grads.values())
+    want = math.sqrt(sum(float(t.double().square().sum()) for t in leaves))
+    got, norm = clip_by_global_norm(grads, bound)
+    wide = any(t.dtype == F64 for t in leaves)
+    assert norm.dtype == (F64 if wide else F32) and norm.shape == () and norm.device.type == "cuda"
+    assert abs(float(norm) - want) <= (1e-14 if wide else 1.01 * U) * want + (0 if wide else 1e-45)
+    other = global_norm(grads)
+    assert other.dtype == norm.dtype and torch.equal(other, norm)
+    factor = min(1.0, bound / want) if want else 1.0
+    assert list(got) == list(grads)
+    for k, t in grads.items():
+        o = got[k]
+        assert o.dtype == t.dtype and o.shape == t.shape and o.stride() == t.stride()
+        if factor == 1.0:
+            assert torch.equal(o, t)
+            continue
+        exact = t.double() * factor
+        step = 2.0**-52 if t.dtype == F64 else 2.01 * U + torch.finfo(t.dtype).eps / 2
+        slack = exact.abs() * (step + (1e-14 if t.dtype == F64 else 0))
+        tiny = torch.finfo(t.dtype).smallest_normal * torch.finfo(t.dtype).eps
+        assert ((o.double() - exact).abs() <= slack + tiny).all()
+    return got, norm
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16, F64], ids=str)
+@pytest.mark.parametrize("n", [1, 2, 7, 8, 63, 1000, 2047, 2049, 16384, 16385, 100003, 1 << 20, 5000001])
+def test_one_leaf(dtype, n):
+    t = tree([n], [dtype], seed=n, scale=0.1)
+    norm = float(t["k000"].double().norm())
+    for over in (0.5, 1.0 - 1e-9, 3.0):
+        check(t, norm / over)
+
+
+@pytest.mark.parametrize("count", [2, 8, 9, 60, 127, 128, 129, 300, 513])
+def test_many_leaves(path, count):
+    """Trees of one launch and of several, types mixed, empty leaves among them."""
+    sizes = [(37 * i * i) % 5000 if i % 7 else 0 for i in range(count)]
+    for dtypes in ([F32, BF16], [F16], [BF16, F64, F32]):
+        check(tree(sizes, dtypes, seed=count), 1.0)
+
+
+def test_sizes_that_differ(path):
+    check(tree([1, 3000001, 5, 70000, 1 << 22, 2], [BF16, F32]), 10.0)
+
+
+def test_every_place_of_every_leaf_counts():
+    """One large entry anywhere is found, and every entry is scaled."""
+    sizes = [5, 4097, 70001, 33]
+    for k, n in enumerate(sizes):
+        for place in {0, 1, n // 2, n - 2, n - 1}:
+            t = {f"k{i}": torch.full((m,), 1e-3, device=DEV) for i, m in enumerate(sizes)}
+            t[f"k{k}"][place] = 1e6
+            got, norm = clip_by_global_norm(t, 1.0)
+            assert abs(float(norm) - 1e6) < 1
+            for i in range(len(sizes)):
+                want = t[f"k{i}"].double() / float(norm)
+                assert torch.allclose(got[f"k{i}"].double(), want, rtol=1e-6, atol=0)
+
+
+def test_structure_and_layout(path):
+    """Pytrees of any form; leaves that are views, transposed, unaligned, expanded; others passed over."""
+    base = torch.randn(1001, device=DEV)
+    wide = torch.randn(40, 50, device=DEV)
+    leaves = {"a": [base[1:], (base[3:500:2], None)], "b": {"t": wide.t(), "p": wide[:, :20].permute(1, 0)}, "c": 3,
+              "e": torch.ones(1, device=DEV).expand(70), "s": torch.tensor(2.0, device=DEV),
+              "h": base.to(BF16)[1:334], "z": torch.empty(0, 4, device=DEV)}
+    tensors = [base[1:], base[3:500:2], wide.t(), wide[:, :20].permute(1, 0), leaves["e"], leaves["s"], leaves["h"]]
+    want = math.sqrt(sum(float(t.double().square().sum()) for t in tensors))
+    keep = [t.clone() for t in tensors]
+    got, norm = clip_by_global_norm(leaves, 1.0)
+    assert abs(float(norm) - want) < 2 * U * want
+    new = [got["a"][0], got["a"][1][0], got["b"]["t"], got["b"]["p"], got["e"], got["s"], got["h"]]
+    assert got["a"][1][1] is None and got["c"] == 3 and got["z"].shape == (0, 4)
+    for t, o, k in zip(tensors, new, keep):
+        assert torch.equal(t, k) and o.shape == t.shape and not o.requires_grad
+        assert torch.allclose(o.double(), t.double() / want, rtol=2.0**-8 if t.dtype == BF16 else 1e-6)
+    assert got["b"]["t"].stride() == wide.t().stride()
+    new[0].zero_()  # leaves of one buffer do not overlap
+    assert torch.equal(new[2].double(), clip_by_global_norm(leaves, 1.0)[0]["b"]["t"].double())
+
+
+def test_scales_that_leave_float32(path):
+    """Squares beyond float32's range on both sides."""
+    for scale in (1e25, 1e-30):
+        check({"a": scale * torch.randn(5000, device=DEV), "b": scale * torch.randn(70000, device=DEV).to(BF16)}, scale)
+    check({"a": torch.full((1000,), 1e200, dtype=F64, device=DEV) / 1e60, "b": torch.ones(9, device=DEV)}, 1e3)
+
+
+def test_values_that_are_none(path):
+    for n in (100, 100000):
+        zero = {"a": torch.zeros(n, device=DEV)}
+        got, norm = clip_by_global_norm(zero, 1.0)
+        assert float(norm) == 0 and not got["a"].any()
+        t = tree([n, n], [F32, BF16])
+        got, _ = clip_by_global_norm(t, 0.0)
+        assert not got["k000"].any() and not got["k001"].any()
+        got, norm = clip_by_global_norm(t, math.inf)
+        assert torch.equal(got["k000"], t["k000"]) and norm.isfinite()
+        t["k001"][5] = float("inf")
+        got, norm = clip_by_global_norm(t, 1.0)
+        assert norm.isinf() and not got["k000"].any() and got["k001"][5].isnan() and not got["k001"][:5].any()
+        t["k000"][7] = float("nan")
+        got, norm = clip_by_global_norm(t, 1.0)
+        assert norm.isnan() and got["k000"].isnan().all() and got["k001"].isnan().all()
+
+
+def test_empty_trees(path):
+    assert clip_by_global_norm({}, 1.0)[0] == {} and float(global_norm([None, 3])) == 0
+    got, norm = clip_by_global_norm({"a": torch.empty(0, device=DEV)}, 1.0)
+    assert got["a"].shape == (0,) and float(norm) == 0 and norm.device.type == "cuda"
+
+
+def test_noised_trees(path):
+    t = tree([500, 70], [F32])
+    got, norm = clip_by_global_norm(noised(t, max_norm=1.0, noise_stddev=0.5), 2.0)
+    want = clip_by_global_norm(t, 2.0)
+    assert isinstance(got, dict) and torch.equal(got["k000"], want[0]["k000"]) and torch.equal(norm, want[1])
+    assert torch.equal(global_norm(clipped(t, max_norm=1.0)), norm)
+    with pytest.raises(TypeError, match="add the noise"):
+        clip_by_global_norm(clipped(t, max_norm=1.0), 2.0)
+
+
+def test_leaves_that_require_gradients(path):
+    t = {"a": torch.nn.Parameter(torch.randn(100, device=DEV)), "b": torch.randn(50, device=DEV)}
+    got, norm = clip_by_global_norm(t, 0.5)
+    assert not got["a"].requires_grad and not norm.requires_grad
+    with torch.inference_mode():
+        again, _ = clip_by_global_norm({k: v.detach().clone() for k, v in t.items()}, 0.5)
+    assert torch.equal(again["a"], got["a"])
+    with pytest.raises(NotImplementedError):
+        torch.func.vmap(lambda a: global_norm({"a": a}))(torch.randn(3, 4, device=DEV))
+
+
+def test_repeated_calls_agree():
+    t = tree([300001, 17, 1 << 19, 90000] * 40, [BF16, F32], seed=3)
+    first, norm = clip_by_global_norm(t, 1.0)
+    for _ in range(3):
+        again, other = clip_by_global_norm(t, 1.0)
+        assert torch.equal(norm, other) and all(torch.equal(first[k], again[k]) for k in t)
+
+
+def test_in_a_graph_and_on_another_stream():
+    t = tree([5000, 70001, 12], [F32, BF16])
+    want = clip_by_global_norm(t, 1.0)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = clip_by_global_norm(t, 1.0)
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(want[0][k], got[0][k]) for k in t) and torch.equal(want[1], got[1])
+    small = tree([50, 3], [F32])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = [clip_by_global_norm(t, 1.0), clip_by_global_norm(small, 0.1)]
+        alone = global_norm(t)
+    for k in range(4):
+        for src in (t, small):
+            for v in src.values():
+                v.mul_(1.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        for (a, n), src, bound in zip(out, (t, small), (1.0, 0.1)):
+            b, m = clip_by_global_norm(src, bound)
+            assert torch.equal(n, m) and all(torch.equal(a[key], b[key]) for key in src)
+        assert torch.equal(alone, global_norm(t))
+
+
+def test_offsets_past_32_bits():
+    """A leaf of more than 2^32 bytes and 2^31 elements: its last entries count and are scaled."""
+    n = (1 << 31) + 12345
+    t = {"a": torch.zeros(n, dtype=BF16, device=DEV), "b": torch.full((10,), 2.0, device=DEV)}
+    t["a"][-1], t["a"][1 << 31], t["a"][0] = 3.0, 4.0, 12.0
+    got, norm = clip_by_global_norm(t, 1.0)
+    want = math.sqrt(9 + 16 + 144 + 40)
+    assert abs(float(norm) - want) < 1e-5
+    for i, v in ((-1, 3.0), (1 << 31, 4.0), (0, 12.0)):
+        assert abs(float(got["a"][i]) - v / want) < 2.0**-8
+    assert int(torch.count_nonzero(got["a"])) == 3

@@ -1,0 +1,390 @@
+"""route and Router against the definition in 64 bits.
+
+Choices have to be those of the float64 keys exactly.  Weights are off by a few float32 roundings: an exponential (2
+units), a sum of up to 64 chosen or 1024 scores (10 levels), a division and a product, within 40 steps of 2^-24 of
+their value; the logits' gradient by the same share of its terms' sizes, and half a step of its type.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from opaque_amd import vocabulary
+from opaque_amd.experts import Router, route
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+U = 2.0**-24
+
+
+@pytest.fixture(params=[True, False], ids=["helper", "functions"])
+def path(request, monkeypatch):
+    if not request.param:
+        monkeypatch.setattr(vocabulary, "_host_ready", [None])
+
+
+def choice(z, top_k, scores, bias, groups, top_groups, group_best):
+    """The index by the float64 keys; stable sorts take the lower expert of equal ones."""
+    z = z.double()
+    t, e = z.shape
+    masked = z == -torch.inf
+    if scores == "softmax":
+        p = torch.softmax(torch.where(masked.all(1, keepdim=True), 0.0, z), 1)
+    else:
+        p = torch.sigmoid(z)
+    # Without a sum the logits order as the scores do, where those run together too.
+    key = z if bias is None and (groups == 1 or group_best == "max") else p + (0.0 if bias is None else bias.double())
+    key = torch.where(masked, -torch.inf, key)
+    if groups > 1:
+        each = torch.sort(key.view(t, groups, -1), dim=2, descending=True).values
+        best = each[..., 0]
+        if group_best == "top2" and each.shape[2] > 1:
+            best = torch.where(each[..., 1] == -torch.inf, best, best + each[..., 1])
+        kept = torch.sort(best, dim=1, descending=True, stable=True).indices[:, :top_groups]
+        open_ = torch.zeros(t, groups, dtype=torch.bool, device=z.device).scatter_(1, kept, True)
+        open_ = open_.repeat_interleave(e // groups, 1)
+        # Open experts first, masked ones among them last.
+        order = torch.sort(key, dim=1, descending=True, stable=True).indices
+        rank = torch.sort((~open_).gather(1, order).to(torch.int8), dim=1, stable=True).indices
+        return order.gather(1, rank)[:, :top_k]
+    return torch.sort(key, dim=1, descending=True, stable=True).indices[:, :top_k]
+
+
+def weigh(z, index, scores, renormalize, scale):
+    """The weights of the chosen, differentiable in the float64 logits z."""
+    if scores == "softmax" and renormalize:
+        logp = z  # over the chosen alone: the others have no part, not even a rounding
+    elif scores == "softmax":
+        logp = torch.log_softmax(z, 1)
+    else:
+        logp = torch.nn.functional.logsigmoid(z)
+    chosen = logp.gather(1, index)
+    return scale * (torch.softmax(chosen, 1) if renormalize else chosen.exp())
+
+
+def check(z, top_k, *, scores="softmax", bias=None, groups=1, top_groups=1, group_best="top2", renormalize=True,
+          scale=1.0, seed=1):
+    kw = dict(scores=scores, bias=bias, groups=groups, top_groups=top_groups, group_best=group_best,
+              renormalize=renormalize, scale=scale)
+    leaf = z.detach().requires_grad_()
+    index, weights = route(leaf, top_k, **kw)
+    t, e = z.shape
+    assert index.dtype == torch.int64 and weights.dtype == F32 and index.shape == weights.shape == (t, top_k)
+    want = choice(z, top_k, scores, bias, groups, top_groups, group_best)
+    assert torch.equal(index, want), (index != want).any(1).nonzero().flatten()[:5]
+    far = z.double().requires_grad_()
+    exact = weigh(far, index, scores, renormalize, scale)
+    worst = ((weights.double() - exact).abs() - 40 * U * exact.abs()).max().item()
+    assert worst <= 1e-37, worst
+    gw = torch.randn(t, top_k, generator=torch.Generator().manual_seed(seed)).to(DEV)
+    (dz,) = torch.autograd.grad(weights, [leaf], gw)
+    (dw,) = torch.autograd.grad(exact, [far], gw.double())
+    assert dz.dtype == z.dtype and dz.shape == z.shape
+    terms = exact.detach().abs() * gw.double().abs()
+    if scores == "sigmoid" and not renormalize:
+        size = torch.zeros_like(dw).scatter_(1, index, terms)
+    elif renormalize:
+        size = torch.zeros_like(dw).scatter_(1, index, terms + exact.detach() / abs(scale) * terms.sum(1, keepdim=True))
+    else:
+        size = torch.zeros_like(dw).scatter_(1, index, terms)
+        size = size + torch.softmax(far.detach(), 1) * terms.sum(1, keepdim=True)
+    bound = 100 * U * size + dw.abs() * torch.finfo(z.dtype).eps / 2 + torch.finfo(z.dtype).smallest_normal
+    worst = ((dz.double() - dw).abs() - bound).max().item()
+    assert worst <= 0, worst
+    return index, weights.detach(), dz
+
+
+def logits(t, e, dtype=F32, seed=0, spread=2.0):
+    g = torch.Generator().manual_seed(seed + 1000 * e + t)
+    return (spread * torch.randn(t, e, generator=g)).to(dtype).to(DEV)
+
+
+@pytest.mark.parametrize("e", [1, 2, 5, 8, 9, 16, 17, 32, 33, 60, 64, 65, 100, 128, 129, 160, 256, 257, 384, 512, 513,
+                               1000, 1024])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
+def test_experts(e, dtype):
+    for scores, renorm in (("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)):
+        check(logits(67, e, dtype), min(e, 6), scores=scores, renormalize=renorm, scale=1.5)
+
+
+@pytest.mark.parametrize("e,k", [(1, 1), (4, 4), (8, 8), (16, 16), (40, 33), (64, 64), (256, 64), (1024, 64), (512, 1)])
+def test_choices(e, k):
+    check(logits(33, e), k)
+    check(logits(33, e, BF16), k, scores="sigmoid", bias=0.1 * logits(1, e, seed=5)[0])
+
+
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize("e", [8, 60, 128, 256, 300, 1024])
+def test_bias(scores, dtype, e):
+    b = logits(1, e, seed=3)[0]
+    for size in (0.0, 0.02, 1.0, 1e4):
+        check(logits(1500, e, dtype, spread=1.0), min(e, 8), scores=scores, bias=size * b)
+
+
+@pytest.mark.parametrize("e,groups,top_groups,k", [(8, 4, 2, 3), (8, 8, 3, 3), (64, 8, 3, 6), (256, 8, 4, 8),
+                                                   (60, 5, 2, 7), (21, 3, 1, 7), (128, 64, 5, 8), (1024, 16, 4, 8),
+                                                   (256, 8, 8, 8), (96, 2, 1, 48)])
+@pytest.mark.parametrize("best", ["top2", "max"])
+def test_groups(e, groups, top_groups, k, best):
+    kw = dict(groups=groups, top_groups=top_groups, group_best=best)
+    check(logits(700, e), k, **kw)
+    check(logits(700, e, BF16), k, scores="sigmoid", **kw)
+    check(logits(700, e), k, scores="sigmoid", bias=0.1 * logits(1, e, seed=4)[0], scale=2.5, **kw)
+    check(logits(700, e, F16), k, bias=-0.1 * logits(1, e, seed=4)[0].abs(), renormalize=False, **kw)
+
+
+def test_equal_keys_go_to_the_lower_expert():
+    for dtype in (F32, BF16):
+        for e in (8, 100, 256, 1000):
+            z = torch.zeros(5, e, dtype=dtype, device=DEV)
+            z[1] = torch.arange(e, device=DEV).flip(0) % 3
+            z[2, ::2] = -0.0
+            z[3, e // 2:] = 1.0
+            for kw in ({}, {"scores": "sigmoid"}, {"bias": torch.zeros(e, device=DEV)},
+                       {"scores": "sigmoid", "bias": torch.ones(e, device=DEV)},
+                       {"groups": 4, "top_groups": 2}, {"groups": 4, "top_groups": 2, "group_best": "max"}):
+                index, _, _ = check(z, min(e // 2, 9), **kw)
+                assert index[0].tolist() == list(range(min(e // 2, 9)))
+
+
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("e", [16, 256, 1024])
+def test_keys_closer_than_float32(scores, e):
+    """Biases that undo the scores' order up to float32's last places: the float64 keys decide."""
+    z = logits(400, e)
+    for r in range(0, 400, 50):
+        p = torch.softmax(z[r].double(), 0) if scores == "softmax" else torch.sigmoid(z[r].double())
+        bias = (0.5 - p).to(F32)  # key = 0.5 but for the rounding of the bias
+        check(z[r: r + 1], 8, scores=scores, bias=bias)
+        check(z[r: r + 1], 8, scores=scores, bias=bias, groups=8, top_groups=4)
+        check(z[r: r + 1], 8, scores=scores, bias=bias, groups=8, top_groups=4, group_best="max")
+    # Logits a step apart.
+    z = torch.full((3, e), 1.0, device=DEV)
+    z[0, 3], z[1, 5], z[2, 7:] = 1 + 2**-23, 1 - 2**-24, 1 + 2**-22
+    check(z, 8, scores=scores)
+    check(z, 8, scores=scores, groups=4, top_groups=2, group_best="max")
+
+
+def test_large_and_small_logits():
+    z = logits(200, 64, spread=30.0)
+    z[:50] -= 200.0
+    z[50:100] += 200.0
+    z[100:150] *= 1e30
+    for scores in ("softmax", "sigmoid"):
+        for kw in ({}, {"groups": 8, "top_groups": 3}, {"bias": torch.zeros(64, device=DEV)}):
+            index, w = route(z, 6, scores=scores, **kw)
+            assert w.isfinite().all() and ((w.sum(1) - 1).abs() < 1e-5).all()
+            if not kw:
+                assert torch.equal(index, choice(z, 6, scores, None, 1, 1, "max"))
+        far = z[:50].double()
+        index, w = route(z[:50], 6, scores=scores)
+        exact = weigh(far, index, scores, True, 1.0)
+        assert ((w.double() - exact).abs() <= 40 * U * exact + 1e-37).all()
+
+
+@pytest.mark.parametrize("e", [8, 100, 300])
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_masked_experts(path, e, scores):
+    """-inf comes last and weighs 0; rows with fewer experts than choices, or none; their gradients are 0 and finite."""
+    z = logits(40, e)
+    z[:, e // 2:] = -torch.inf
+    z[5, 1:] = -torch.inf
+    z[6] = -torch.inf
+    z[7, ::2] = -torch.inf
+    low = torch.finfo(F32).min  # a mask of the type's lowest value weighs 0 as well
+    z[8, 1:] = low
+    b = 0.1 * logits(1, e, seed=2)[0]
+    for bias in (None, b):
+        for groups in (1, 4):
+            for renorm in (True, False):
+                kw = dict(scores=scores, bias=bias, groups=groups, top_groups=max(groups // 2, 1))
+                k = min(4, e // groups * max(groups // 2, 1))
+                leaf = z.clone().requires_grad_()
+                index, w = route(leaf, k, renormalize=renorm, **kw)
+                assert torch.equal(index, choice(z, k, scores, bias, groups, kw["top_groups"], "top2"))
+                picked = z.gather(1, index)
+                assert w.isfinite().all() and (w[picked == -torch.inf] == 0).all() and (w[picked > low] > 0).all()
+                assert not w[6].any()
+                if renorm:
+                    assert ((w.sum(1) - 1).abs() < 1e-5)[[i for i in range(40) if i != 6]].all()
+                (dz,) = torch.autograd.grad(w, [leaf], torch.randn_like(w))
+                assert dz.isfinite().all() and not dz[z == -torch.inf].any()
+
+
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_nan_and_infinity(path, scores):
+    """The index stays a set of experts, the other rows keep their bits."""
+    for e, k in ((8, 3), (64, 6), (256, 8)):
+        for kw in ({}, {"bias": 0.1 * logits(1, e, seed=2)[0]}, {"groups": 4, "top_groups": 2}):
+            z = logits(20, e)
+            clean = route(z, k, scores=scores, **kw)
+            z[3, 1], z[5, 2], z[7] = float("nan"), float("inf"), float("nan")
+            leaf = z.clone().requires_grad_()
+            index, w = route(leaf, k, scores=scores, **kw)
+            assert ((index >= 0) & (index < e)).all()
+            assert all(row.unique().numel() == k for row in index)
+            rest = [i for i in range(20) if i not in (3, 5, 7)]
+            assert torch.equal(index[rest], clean[0][rest]) and torch.equal(w[rest], clean[1][rest])
+            assert w[7].isnan().all()
+            if scores == "softmax":
+                assert w[3].isnan().all() and w[5].isnan().all()
+            else:
+                want = choice(z[5:6], k, scores, kw.get("bias"), kw.get("groups", 1), kw.get("top_groups", 1), "top2")
+                assert w[5].isfinite().all() and torch.equal(index[5:6], want)
+            (dz,) = torch.autograd.grad(w, [leaf], torch.randn_like(w))
+            assert dz[rest].isfinite().all()
+    b = torch.zeros(64, device=DEV)
+    b[5], b[9], b[11] = float("inf"), -float("inf"), float("nan")
+    index, w = route(logits(30, 64), 6, scores=scores, bias=b)
+    assert (index[:, 0] == 5).all() and not ((index == 9) | (index == 11)).any() and w.isfinite().all()
+
+
+def test_shapes_and_strides(path):
+    z = logits(24, 40, BF16)
+    b = 0.1 * logits(1, 40, seed=2)[0]
+    want = route(z, 5, bias=b)
+    wide = torch.zeros(24, 55, dtype=BF16, device=DEV)
+    wide[:, 3:43] = z
+    for v in (wide[:, 3:43], z.t().contiguous().t()):
+        assert all(torch.equal(p, q) for p, q in zip(route(v, 5, bias=b), want))
+    strided = torch.zeros(80, device=DEV)
+    strided[::2] = b
+    assert all(torch.equal(p, q) for p, q in zip(route(z, 5, bias=strided[::2]), want))
+    index, w = route(z.view(2, 3, 4, 40), 5, bias=b)
+    assert index.shape == w.shape == (2, 3, 4, 5) and torch.equal(index.view(24, 5), want[0])
+    one = route(z[3], 5, bias=b)
+    assert one[0].shape == (5,) and torch.equal(one[0], want[0][3]) and torch.equal(one[1], want[1][3])
+    none = z[:0].clone().requires_grad_()
+    index, w = route(none, 5)
+    assert index.shape == w.shape == (0, 5) and torch.autograd.grad(w, [none], w.detach())[0].shape == (0, 40)
+    leaf = z.clone().requires_grad_()
+    (dz,) = torch.autograd.grad(route(leaf, 5, renormalize=False)[1].sum(), [leaf])
+    (dw,) = torch.autograd.grad(route(leaf, 5, renormalize=False)[1], [leaf], torch.ones(24, 5, device=DEV))
+    assert torch.equal(dz, dw)
+
+
+@pytest.mark.parametrize("t", [1, 3, 255, 257, 4099])
+def test_tokens(t):
+    """A token's result does not depend on its batch."""
+    z = logits(5000, 72)
+    b = 0.1 * logits(1, 72, seed=2)[0]
+    whole = route(z, 6, scores="sigmoid", bias=b, groups=8, top_groups=3)
+    part = route(z[:t], 6, scores="sigmoid", bias=b, groups=8, top_groups=3)
+    assert all(torch.equal(p, q[:t]) for p, q in zip(part, whole))
+
+
+def test_under_vmap(path):
+    z = logits(6 * 10, 24).view(6, 10, 24)
+    b = 0.1 * logits(6, 24, seed=2)
+    gw = torch.randn(6, 10, 4, generator=torch.Generator().manual_seed(1)).to(DEV)
+
+    def one(z, b, gw=None):
+        index, w = route(z, 4, scores="sigmoid", bias=b)
+        return (index, w) if gw is None else (w * gw).sum()
+
+    got = torch.func.vmap(one)(z, b)
+    shared = torch.func.vmap(one, in_dims=(0, None))(z, b[0])
+    moved = torch.func.vmap(one, in_dims=(1, 0))(z.transpose(0, 1).contiguous(), b)
+    nested = torch.func.vmap(torch.func.vmap(one, in_dims=(0, None)))(z, b)
+    grads = torch.func.vmap(torch.func.grad(one))(z, b, gw)
+    for i in range(6):
+        leaf = z[i].clone().requires_grad_()
+        want = one(leaf, b[i])
+        for out in (got, moved, nested):
+            assert torch.equal(out[0][i], want[0]) and torch.equal(out[1][i], want[1])
+        assert torch.equal(shared[0][i], one(z[i], b[0])[0])
+        assert torch.equal(grads[i], torch.autograd.grad(want[1], [leaf], gw[i])[0])
+    leaf = z.clone().requires_grad_()
+    outer = torch.autograd.grad(torch.func.vmap(one)(leaf, b)[1], [leaf], gw)
+    assert torch.equal(outer[0], grads)
+
+
+def test_autograd_manners(path):
+    z = logits(12, 20).requires_grad_()
+    bias = (0.1 * logits(1, 20, seed=2)[0]).requires_grad_()
+    gw = torch.randn(12, 4, device=DEV, requires_grad=True)
+    index, w = route(z, 4, bias=bias)
+    assert not index.requires_grad and w.requires_grad
+    (dz,) = torch.autograd.grad(w, [z], gw, create_graph=True)
+    for t in (z, gw):
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(dz.sum(), t, retain_graph=True)
+    (plain,) = torch.autograd.grad(route(z, 4, bias=bias)[1], [z], gw.detach())
+    assert torch.equal(plain, dz.detach()) and not plain.requires_grad
+    assert not route(z.detach(), 4, bias=bias)[1].requires_grad
+    w2 = route(z, 4, bias=bias)[1]
+    w2.backward(gw.detach())
+    assert bias.grad is None and torch.equal(z.grad, plain)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.cpu()):
+        w = route(z, 4, bias=bias)[1]
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(w, [z], gw.detach())
+    w = torch.utils.checkpoint.checkpoint(lambda a: route(a, 4, bias=bias)[1], z, use_reentrant=False)
+    assert torch.equal(torch.autograd.grad(w, [z], gw.detach())[0], plain)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(z.detach(), torch.ones_like(z))
+        with pytest.raises(RuntimeError):
+            route(dual, 4)
+    with torch.inference_mode():
+        assert torch.equal(route(z.clone(), 4)[0], route(z, 4)[0])
+
+
+def test_differences():
+    """The logits' gradient against central differences of the definition, the choice held."""
+    for scores, renorm in (("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)):
+        z = logits(3, 10)
+        leaf = z.clone().requires_grad_()
+        index, w = route(leaf, 4, scores=scores, renormalize=renorm, scale=2.0)
+        gw = torch.randn(3, 4, generator=torch.Generator().manual_seed(2)).to(DEV)
+        (dz,) = torch.autograd.grad(w, [leaf], gw)
+        value = lambda z: (weigh(z, index, scores, renorm, 2.0) * gw.double()).sum()
+        for i in range(30):
+            step = torch.zeros(30, dtype=torch.float64, device=DEV)
+            step[i] = 1e-5
+            diff = (value(z.double() + step.view(3, 10)) - value(z.double() - step.view(3, 10))) / 2e-5
+            assert abs(diff - dz.flatten()[i].double()) < 1e-6
+
+
+def test_router_module():
+    torch.manual_seed(0)
+    r = Router(48, 16, 3, scores="sigmoid", balance=True, groups=4, top_groups=2, scale=2.0, device=DEV, dtype=BF16)
+    x = torch.randn(2, 5, 48, device=DEV, dtype=BF16)
+    index, w = r(x)
+    z = torch.nn.functional.linear(x, r.weight)
+    want = route(z, 3, scores="sigmoid", bias=r.balance, groups=4, top_groups=2, scale=2.0)
+    assert torch.equal(index, want[0]) and torch.equal(w, want[1]) and r.balance.dtype == F32
+    w.sum().backward()
+    assert r.weight.grad.isfinite().all() and "balance" in r.state_dict()
+    plain = Router(48, 16, 3, device=DEV)
+    assert plain.balance is None and plain(x.float())[0].shape == (2, 5, 3)
+
+
+def test_in_a_graph_and_on_another_stream():
+    z = logits(300, 64).requires_grad_()
+    b = 0.1 * logits(1, 64, seed=2)[0]
+    gw = torch.randn(300, 6, device=DEV)
+
+    def step():
+        index, w = route(z, 6, scores="sigmoid", bias=b, groups=8, top_groups=4)
+        return [index, w.detach(), *torch.autograd.grad(w, [z], gw)]
+
+    want = step()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = step()
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(a, c) for a, c in zip(want, got))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for k in range(4):
+        with torch.no_grad():
+            z.copy_(logits(300, 64, seed=k))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(out, step()))
