@@ -45,7 +45,7 @@ void bind(const std::unordered_map<std::string, uintptr_t>& at) {
 
 void check(int rc, const char* what) { TORCH_CHECK(rc == ODP_OK, what, " failed with status ", rc, ": ", abi.last_error()); }
 
-using torch::autograd::AutogradContext;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 using Maybe = std::optional<at::Tensor>;
 
@@ -108,69 +108,58 @@ Normed norm_forward(const at::Tensor& x, const Maybe& residual, const Maybe& wei
   return out;
 }
 
-struct Norm : torch::autograd::Function<Norm> {
-  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const Maybe& residual, const Maybe& weight,
-                               double eps, double offset) {
-    Normed o = norm_forward(x, residual, weight, eps, offset, true, 0);
-    const at::Tensor& h = residual.has_value() ? o.h : x;
-    ctx->save_for_backward({h, o.rstd, weight.has_value() ? *weight : at::Tensor()});
-    ctx->set_materialize_grads(false);
-    auto& d = ctx->saved_data;
-    d["residual"] = residual.has_value();
-    d["weight"] = weight.has_value();
-    d["offset"] = offset;
-    d["shape"] = x.sizes().vec();
-    d["x"] = (int64_t)x.scalar_type();
-    d["h"] = (int64_t)h.scalar_type();
-    if (weight.has_value()) {
-      d["w"] = (int64_t)weight->scalar_type();
-      d["w_shape"] = weight->sizes().vec();
-    }
-    ctx->mark_non_differentiable({o.rstd});
-    return residual.has_value() ? variable_list{o.y, o.rstd, o.h} : variable_list{o.y, o.rstd};
+// Nodes of their own, with their fields as they are: torch's wrapper for
+// custom functions keeps them in a map by name, which takes 8 us of a call.
+struct NormNode final : torch::autograd::Node {
+  SavedVariable h, rstd, w;
+  bool has_r = false, has_w = false;
+  double offset = 0.0;
+  at::ScalarType xt, ht, wt;
+  std::vector<int64_t> shape, w_shape;
+
+  std::string name() const override { return "RmsNormBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    h.reset_data();
+    rstd.reset_data();
+    w.reset_data();
   }
 
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    auto& sd = ctx->saved_data;
-    const bool has_r = sd["residual"].toBool(), has_w = sd["weight"].toBool();
-    const at::Tensor gh0 = has_r ? grads[2] : at::Tensor();
-    if (!grads[0].defined() && !gh0.defined()) return {{}, {}, {}, {}, {}};
-    const variable_list saved = ctx->get_saved_variables();
-    const bool need_x = ctx->needs_input_grad(0), need_r = has_r && ctx->needs_input_grad(1);
-    const bool need_w = has_w && ctx->needs_input_grad(has_r ? 2 : 1);
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    const at::Tensor& gy0 = grads[0];
+    const at::Tensor gh0 = has_r ? grads[1] : at::Tensor();
+    if (!gy0.defined() && !gh0.defined()) return variable_list(3);
+    const at::Tensor h_ = h.unpack(has_r ? shared_from_this() : nullptr), rstd_ = rstd.unpack();
+    const at::Tensor w_ = has_w ? w.unpack() : at::Tensor();
+    const bool need_x = task_should_compute_output(0), need_r = task_should_compute_output(1);
+    const bool need_w = task_should_compute_output(2);
     at::Tensor dx, dr, dw;
     {
       at::NoGradGuard no_grad;
-      const at::Tensor& like = grads[0].defined() ? grads[0] : gh0;
+      const at::Tensor& like = gy0.defined() ? gy0 : gh0;
       const c10::OptionalDeviceGuard guard(like.device());
-      const auto shape = sd["shape"].toIntVector();
-      const auto xt = (at::ScalarType)sd["x"].toInt(), ht = (at::ScalarType)sd["h"].toInt();
-      odp_host::as_saved(saved[0], like, ht, shape, kNorms);
-      const at::Tensor h = pitched(saved[0]);
-      const int64_t n = h.size(0), width = h.size(1);
-      const at::Tensor rstd = odp_host::whole(saved[1].reshape({-1}), like, at::kFloat, {n}, kNorms);
-      Maybe w;
-      if (has_w) {
-        odp_host::as_saved(saved[2], like, (at::ScalarType)sd["w"].toInt(), sd["w_shape"].toIntVector(), kNorms);
-        w = saved[2];
-      }
-      const Gain g(w, code_of(at::empty({0}, h.options().dtype(xt))));
-      const at::Tensor gy = grads[0].defined() ? pitched(grads[0]) : at::zeros({n, width}, h.options().dtype(xt));
+      odp_host::as_saved(h_, like, ht, shape, kNorms);
+      const at::Tensor rows = pitched(h_);
+      const int64_t n = rows.size(0), width = rows.size(1);
+      const at::Tensor stat = odp_host::whole(rstd_.reshape({-1}), like, at::kFloat, {n}, kNorms);
+      if (has_w) odp_host::as_saved(w_, like, wt, w_shape, kNorms);
+      const auto options = rows.options().dtype(xt);
+      const at::Tensor gy = gy0.defined() ? pitched(gy0) : at::zeros({n, width}, options);
       const at::Tensor gh = gh0.defined() ? pitched(gh0) : at::Tensor();
+      const Gain g(has_w ? Maybe(w_) : Maybe(), code_of(gy));
       const bool same = xt == ht;
-      if (need_x || need_r) dx = at::empty(shape, gy.options());
-      if (need_r && !same) dr = at::empty(shape, h.options());
-      if (need_w) {
-        dw = n > 0 ? at::empty(w->sizes(), w->options()) : at::zeros(w->sizes(), w->options());
-      }
+      if (need_x || need_r) dx = at::empty(shape, options);
+      if (need_r && !same) dr = at::empty(shape, rows.options());
+      if (need_w) dw = n > 0 ? at::empty(w_shape, rows.options().dtype(wt)) : at::zeros(w_shape, rows.options().dtype(wt));
       const int64_t words = need_w ? abi.rms_norm_grad_scratch(n, width, g.count) : 0;
-      const at::Tensor work = words > 0 ? bytes_on(h, words) : at::Tensor();
-      check(abi.rms_norm_grad(stream_of(h), code_of(gy), code_of(h), g.dt, h.data_ptr(), h.stride(0),
-                              (const float*)rstd.data_ptr(), gy.data_ptr(), gy.stride(0),
+      const at::Tensor work = words > 0 ? bytes_on(rows, words) : at::Tensor();
+      check(abi.rms_norm_grad(stream_of(rows), code_of(gy), code_of(rows), g.dt, rows.data_ptr(), rows.stride(0),
+                              (const float*)stat.data_ptr(), gy.data_ptr(), gy.stride(0),
                               gh.defined() ? gh.data_ptr() : nullptr, gh.defined() ? gh.stride(0) : 0, n, width, g.at,
-                              g.pitch, g.count, (float)sd["offset"].toDouble(),
-                              work.defined() ? work.data_ptr() : nullptr, dx.defined() ? dx.data_ptr() : nullptr,
-                              dr.defined() ? dr.data_ptr() : nullptr, dw.defined() ? dw.data_ptr() : nullptr),
+                              g.pitch, g.count, (float)offset, work.defined() ? work.data_ptr() : nullptr,
+                              dx.defined() ? dx.data_ptr() : nullptr, dr.defined() ? dr.data_ptr() : nullptr,
+                              dw.defined() ? dw.data_ptr() : nullptr),
             "odp_rms_norm_grad");
       if (need_r && same) dr = dx;
       if (!need_x) dx = at::Tensor();
@@ -179,7 +168,7 @@ struct Norm : torch::autograd::Function<Norm> {
     const bool shared = dx.defined() && dr.defined() && dx.is_same(dr);
     dx = odp_host::first_only(grads, dx, true, kNorms);
     dr = shared ? dx : odp_host::first_only(grads, dr, true, kNorms);
-    return {dx, dr, dw, {}, {}};
+    return {dx, dr, dw};
   }
 };
 
@@ -189,9 +178,34 @@ variable_list normed(const at::Tensor& x, const Maybe& residual, const Maybe& we
   odp_host::no_tangent(x, kNorms);
   if (residual.has_value()) odp_host::no_tangent(*residual, kNorms);
   if (weight.has_value()) odp_host::no_tangent(*weight, kNorms);
+  bool grad = true;
   if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(residual) || wants_grad(weight)))
-    return Norm::apply(x, residual, weight, eps, offset);
-  const Normed o = norm_forward(x, residual, weight, eps, offset, keep, 0);
+    keep = true;
+  else
+    grad = false;
+  Normed o;
+  {
+    at::NoGradGuard no_grad;
+    o = norm_forward(x, residual, weight, eps, offset, keep, 0);
+  }
+  if (grad) {
+    const bool has_r = residual.has_value(), has_w = weight.has_value();
+    const at::Tensor none, &r = has_r ? *residual : none, &w = has_w ? *weight : none;
+    auto node = std::shared_ptr<NormNode>(new NormNode(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x, r, w));
+    torch::autograd::set_history(o.y, node);
+    if (has_r) torch::autograd::set_history(o.h, node);
+    node->h = SavedVariable(has_r ? o.h : x, has_r);
+    node->rstd = SavedVariable(o.rstd, false);
+    if (has_w) node->w = SavedVariable(w, false);
+    node->has_r = has_r;
+    node->has_w = has_w;
+    node->offset = offset;
+    node->xt = x.scalar_type();
+    node->ht = has_r ? r.scalar_type() : node->xt;
+    node->shape = x.sizes().vec();
+    if (has_w) node->wt = w.scalar_type(), node->w_shape = w.sizes().vec();
+  }
   return residual.has_value() ? variable_list{o.y, o.rstd, o.h} : variable_list{o.y, o.rstd};
 }
 
@@ -247,44 +261,40 @@ std::pair<at::Tensor, at::Tensor> route_forward(const at::Tensor& z, const Maybe
   return {index, weights};
 }
 
-struct Route : torch::autograd::Function<Route> {
-  static variable_list forward(AutogradContext* ctx, const at::Tensor& z, const Maybe& bias, const Options& o) {
-    const auto out = route_forward(z, bias, o);
-    ctx->mark_non_differentiable({out.first});
-    ctx->set_materialize_grads(false);
-    ctx->save_for_backward({z, out.first});
-    auto& d = ctx->saved_data;
-    d["sigmoid"] = o.sigmoid;
-    d["renorm"] = o.renorm;
-    d["scale"] = o.scale;
-    d["top_k"] = o.top_k;
-    d["type"] = (int64_t)z.scalar_type();
-    d["shape"] = z.sizes().vec();
-    return {out.first, out.second};
+struct RouteNode final : torch::autograd::Node {
+  SavedVariable z, index;
+  Options o;
+  at::ScalarType type;
+  std::vector<int64_t> shape;
+
+  std::string name() const override { return "RouteBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    z.reset_data();
+    index.reset_data();
   }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    if (!grads[1].defined() || !ctx->needs_input_grad(0)) return {{}, {}, {}};
+
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    const at::Tensor& gw = grads[0];
+    if (!gw.defined() || !task_should_compute_output(0)) return variable_list(1);
+    const at::Tensor z_ = z.unpack(), index_ = index.unpack();
     at::Tensor dz;
     {
       at::NoGradGuard no_grad;
-      const at::Tensor& gw = grads[1];
       const c10::OptionalDeviceGuard guard(gw.device());
-      auto& sd = ctx->saved_data;
-      auto shape = sd["shape"].toIntVector();
-      const variable_list saved = ctx->get_saved_variables();
-      odp_host::as_saved(saved[0], gw, (at::ScalarType)sd["type"].toInt(), shape, kRoutes);
-      const at::Tensor rows = pitched(saved[0]);
-      const int64_t top_k = sd["top_k"].toInt();
+      odp_host::as_saved(z_, gw, type, shape, kRoutes);
+      const at::Tensor rows = pitched(z_);
+      std::vector<int64_t> chosen(shape);
+      chosen.back() = o.top_k;
+      const at::Tensor at_ = odp_host::whole(index_, gw, at::kLong, chosen, kRoutes), g = gw.contiguous();
       dz = at::empty(shape, rows.options());
-      shape.back() = top_k;
-      const at::Tensor index = odp_host::whole(saved[1], gw, at::kLong, shape, kRoutes);
-      const at::Tensor g = gw.contiguous();
       check(abi.route_grad(stream_of(rows), code_of(rows), rows.data_ptr(), rows.stride(0), rows.size(0), rows.size(1),
-                           (int)sd["sigmoid"].toBool(), top_k, (int)sd["renorm"].toBool(), (float)sd["scale"].toDouble(),
-                           (const int64_t*)index.data_ptr(), (const float*)g.data_ptr(), top_k, dz.data_ptr()),
+                           (int)o.sigmoid, o.top_k, (int)o.renorm, (float)o.scale, (const int64_t*)at_.data_ptr(),
+                           (const float*)g.data_ptr(), o.top_k, dz.data_ptr()),
             "odp_route_grad");
     }
-    return {odp_host::first_only(grads, dz, true, kRoutes), {}, {}};
+    return {odp_host::first_only(grads, dz, true, kRoutes)};
   }
 };
 
@@ -293,11 +303,22 @@ std::pair<at::Tensor, at::Tensor> route(const at::Tensor& z, const Maybe& bias, 
   py::gil_scoped_release nogil;
   odp_host::no_tangent(z, kRoutes);
   const Options o{sigmoid, groups, top_groups, best, top_k, renorm, scale};
-  if (at::GradMode::is_enabled() && z.requires_grad()) {
-    const variable_list out = Route::apply(z, bias, o);
-    return {out[0], out[1]};
+  std::pair<at::Tensor, at::Tensor> out;
+  {
+    at::NoGradGuard no_grad;
+    out = route_forward(z, bias, o);
   }
-  return route_forward(z, bias, o);
+  if (at::GradMode::is_enabled() && z.requires_grad()) {
+    auto node = std::shared_ptr<RouteNode>(new RouteNode(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(z));
+    torch::autograd::set_history(out.second, node);
+    node->z = SavedVariable(z, false);
+    node->index = SavedVariable(out.first, false);
+    node->o = o;
+    node->type = z.scalar_type();
+    node->shape = z.sizes().vec();
+  }
+  return out;
 }
 
 // ---------------------------------------------------------------------------
@@ -310,9 +331,18 @@ int tree_code(const at::Tensor& t) { return t.scalar_type() == at::kDouble ? ODP
 // lie in one buffer per type, with the leaves' own strides where those leave no
 // gaps.
 std::pair<std::vector<at::Tensor>, at::Tensor> tree_norm(const std::vector<at::Tensor>& leaves, bool clip,
-                                                         double max_norm, bool wide) {
+                                                         double max_norm, const std::string& who) {
   py::gil_scoped_release nogil;
   at::NoGradGuard no_grad;
+  bool wide = false;
+  for (const at::Tensor& t : leaves) {
+    const auto type = t.scalar_type();
+    TORCH_CHECK_TYPE(type == at::kFloat || type == at::kBFloat16 || type == at::kHalf || type == at::kDouble, who,
+                     " supports float32, bfloat16, float16 and float64 leaves, got ", type);
+    TORCH_CHECK(t.is_cuda() && t.device() == leaves[0].device(), who,
+                " runs on the GPU: its leaves must be CUDA tensors of one device");
+    wide = wide || type == at::kDouble;
+  }
   const c10::OptionalDeviceGuard guard(leaves.at(0).device());
   constexpr int64_t kAlign = 64;
   std::vector<at::Tensor> src(leaves.size()), out;
@@ -361,5 +391,5 @@ void add_block(py::module_& m) {
         py::arg("eps"), py::arg("offset"), py::arg("quant"));
   m.def("route", &route, py::arg("z"), py::arg("bias"), py::arg("sigmoid"), py::arg("groups"), py::arg("top_groups"),
         py::arg("best"), py::arg("top_k"), py::arg("renorm"), py::arg("scale"));
-  m.def("tree_norm", &tree_norm, py::arg("leaves"), py::arg("clip"), py::arg("max_norm"), py::arg("wide"));
+  m.def("tree_norm", &tree_norm, py::arg("leaves"), py::arg("clip"), py::arg("max_norm"), py::arg("name"));
 }

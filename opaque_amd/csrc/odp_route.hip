@@ -18,10 +18,10 @@
 // choice is the largest word below the last: the largest of (word - last) in
 // wrapping arithmetic, with nothing to mark.  The leading bits decide as the
 // keys in 64 bits would unless two that the choice hangs on lie within the
-// error of their float32 computation (BIAS_TOL); such a token is done again from
-// float64 keys (`route_exactly`; 0.3 % of the tokens of 256 experts with a bias).
-// Keys are the logits themselves where those order as the scores do (no bias,
-// and no sums over groups); those of 16-bit types always decide.
+// error of their float32 computation (`units_apart`); of such a token the
+// candidates' float64 keys are formed and ranked (`rank_exactly`), which a wave
+// takes in 2-3 us.  Keys are the logits themselves where those order as the scores
+// do (no bias, and no sums over groups); those of 16-bit types always decide.
 #include <cmath>
 
 #include "odp_internal.h"
@@ -132,6 +132,7 @@ struct RouteArgs {
   int64_t ldw;            // pitch of gw
   int experts, top_k, groups, top_groups, size;  // size: of a group
   int dt, sigmoid, best, renorm, bits;           // bits: of an expert's number
+  int span;                                      // threads of a group (0: none of their own)
   float scale, per_size;                         // 1 / size
 };
 
@@ -183,68 +184,116 @@ __device__ __forceinline__ float sigmoid(float z) {
   return (z >= 0.0f ? 1.0f : e) / (1.0f + e);
 }
 
-// The choice from float64 keys, by the L threads of a token; key: [experts] of
-// LDS.  Masked experts (a logit of -inf) come after all others, a NaN key last.
-template <int L>
-__device__ void route_exactly(const RouteArgs& a, const char* row, const float* bias, int t, uint64_t* key,
-                                           int* picked) {
-  const int n = a.experts;
-  double top = -INFINITY, total = 0.0;
-  if (!a.sigmoid) {
-    for (int e = t; e < n; e += L) top = fmax(top, (double)logit(row, a.dt, e));
+// A chosen logit's share of the chosen ones' sum (with renormalize) or its
+// score times what the softmax divides by: over the largest of the chosen, so
+// that the sum is never 0; for sigmoids where all are small.
+struct Shares {
+  bool sigmoid;
+  float shift;
+  __device__ __forceinline__ Shares(const RouteArgs& a, float most, float top)
+      : sigmoid(a.sigmoid), shift(a.sigmoid ? (a.renorm ? fminf(most, 0.0f) : 0.0f) : a.renorm ? most : top) {}
+  __device__ __forceinline__ float operator()(float x) const {
+    if (x == -INFINITY) return 0.0f;
+    if (!sigmoid) return exp_near(x - shift);
+    return x >= 0.0f ? 1.0f / (1.0f + exp_near(-x)) : exp_near(x - shift) / (1.0f + exp_near(x));
+  }
+};
+
+// A row's float64 keys, as ordered words: a masked expert (a logit of -inf)
+// below all others, a NaN key below those.
+struct Keys64 {
+  const RouteArgs& a;
+  const char* row;
+  const float* bias;
+  bool sums;  // the keys are more than the logits
+  double top = 0.0, total = 1.0;
+  template <int L>
+  __device__ __forceinline__ void normalise(int t) {
+    if (!sums || a.sigmoid) return;
+    top = -INFINITY;
+    total = 0.0;
+#pragma unroll 4
+    for (int e = t; e < a.experts; e += L) top = fmax(top, (double)logit(row, a.dt, e));
     top = fmax_of<L>(top);
-    for (int e = t; e < n; e += L) {
+#pragma unroll 4
+    for (int e = t; e < a.experts; e += L) {
       const double z = logit(row, a.dt, e);
       total += z == -INFINITY ? 0.0 : exp(z - top);
     }
     total = sum_of<L>(total);
   }
-  for (int e = t; e < n; e += L) {
+  __device__ __forceinline__ uint64_t operator()(int e) const {
     const double z = logit(row, a.dt, e);
     double k = z + 0.0;  // the logits order as the scores do (-0 as 0)
-    if (bias != nullptr || (a.groups > 1 && a.best == 0)) {
+    if (sums) {
       k = a.sigmoid ? 1.0 / (1.0 + exp(-z)) : exp(z - top) / total;
       k += bias != nullptr ? (double)bias[e] : 0.0;
     }
-    key[e] = ordered(z == -INFINITY ? -INFINITY : k);
+    return ordered(z == -INFINITY ? -INFINITY : k);
   }
+};
+
+// All of them, in a token's words of LDS, and a mask of the open groups from
+// them.  Group g is thread g % L's; masked experts add nothing to its score.
+template <int L, int V>
+__device__ __forceinline__ uint64_t open_exactly(const RouteArgs& a, Keys64& of, int t, uint64_t* key) {
+  of.normalise<L>(t);
+#pragma unroll 2
+  for (int e = t; e < a.experts; e += L) key[e] = of(e);
+  wave_sync();
+  if (a.groups == 1) return ~0ull;
+  constexpr int PER = ((L * V < RT_GROUPS ? L * V : RT_GROUPS) + L - 1) / L;
+  const uint64_t least = ordered(-(double)INFINITY);
+  const auto value = [](uint64_t w) {
+    return __longlong_as_double((long long)((int64_t)w < 0 ? w & 0x7fffffffffffffffull : ~w));
+  };
+  uint64_t mine[PER], open = 0;
+  int above[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int g = t + i * L;
+    mine[i] = 0;
+    above[i] = 0;
+    if (g >= a.groups) continue;
+    uint64_t one = 0, two = 0;
+#pragma unroll 4
+    for (int k = 0; k < a.size; ++k) {
+      const uint64_t w = key[g * a.size + k];
+      two = max(two, min(one, w));
+      one = max(one, w);
+    }
+    mine[i] = a.best == 0 && one > 1 && two > least ? ordered(value(one) + value(two)) : one;
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    for (int l = 0; l < L && i * L + l < a.groups; ++l) {
+      const uint64_t w = (uint64_t)__shfl((long long)mine[i], l, L);
+#pragma unroll
+      for (int k = 0; k < PER; ++k) above[k] += w > mine[k] || (w == mine[k] && i * L + l < t + k * L);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (t + i * L < a.groups && above[i] < a.top_groups) open |= 1ull << (t + i * L);
+  const uint32_t lo = or_of<L>((uint32_t)open), hi = or_of<L>((uint32_t)(open >> 32));
+  return (uint64_t)hi << 32 | lo;
+}
+
+// The choice from float64 keys, by the L threads of a token.
+template <int L, int V>
+__device__ __forceinline__ void route_exactly(const RouteArgs& a, Keys64& of, int t, uint64_t* key, int* picked) {
+  const uint64_t open = open_exactly<L, V>(a, of, t, key);
   wave_sync();
   if (a.groups > 1) {
-    // A group's score as an ordered word too; those that do not come into it (masked) add nothing.
-    uint64_t open = 0;
-    for (int g = t; g < a.groups; g += L) {
-      uint64_t mine = 0;
-      int above = 0;
-      for (int o = -1; o < a.groups; ++o) {  // -1: this group itself, first
-        const uint64_t* k = key + (o < 0 ? g : o) * a.size;
-        uint64_t one = 0, two = 0;
-        for (int i = 0; i < a.size; ++i) {
-          const uint64_t w = k[i];
-          two = max(two, min(one, w));
-          one = max(one, w);
-        }
-        if (a.best == 0 && one > 1 && two > ordered(-(double)INFINITY)) {
-          const auto value = [](uint64_t w) {
-            return __longlong_as_double((long long)((int64_t)w < 0 ? w & 0x7fffffffffffffffull : ~w));
-          };
-          one = ordered(value(one) + value(two));
-        }
-        if (o < 0) mine = one;
-        else above += one > mine || (one == mine && o < g);
-      }
-      if (above < a.top_groups) open |= 1ull << g;
-    }
-    const uint32_t lo = or_of<L>((uint32_t)open), hi = or_of<L>((uint32_t)(open >> 32));
-    open = (uint64_t)hi << 32 | lo;
-    wave_sync();
-    for (int e = t; e < n; e += L)
+    for (int e = t; e < a.experts; e += L)
       if (!(open >> (e / a.size) & 1)) key[e] = 0;
     wave_sync();
   }
   for (int j = 0; j < a.top_k; ++j) {
     uint64_t most = 0;
     int at = t;
-    for (int e = t; e < n; e += L) {
+#pragma unroll 4
+    for (int e = t; e < a.experts; e += L) {
       const uint64_t w = key[e];
       if (w > most) most = w, at = e;
     }
@@ -259,19 +308,53 @@ __device__ void route_exactly(const RouteArgs& a, const char* row, const float* 
   }
 }
 
-// Two words' leading parts within this of each other: the float32 computation
-// may have them the wrong way round.  In units of 2^-24 of the keys' range R
-// (scores' 1 and the bias's): a score is off by up to 16 (an exponential, a sum
-// of up to 1024 of them, a reciprocal), the bias above its least, the sum and
-// the product by one each.
-constexpr uint32_t BIAS_TOL = 64;
+// The best top_k of `count` candidates, in the order of their float64 keys.
+template <int L, int PER>
+__device__ __forceinline__ void rank_exactly(const RouteArgs& a, Keys64& of, int t, int count, uint64_t* key,
+                                             int* picked) {
+  of.normalise<L>(t);
+  int e[PER], above[PER];
+  uint64_t mine[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int j = t + i * L;
+    if (j >= count) break;
+    e[i] = picked[j];
+    mine[i] = of(e[i]);
+    key[j] = mine[i];
+  }
+  wave_sync();
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (t + i * L >= count) break;
+    above[i] = 0;
+#pragma unroll 4
+    for (int j = 0; j < count; ++j) above[i] += key[j] > mine[i] || (key[j] == mine[i] && picked[j] < e[i]);
+  }
+  wave_sync();
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (t + i * L < count && above[i] < a.top_k) picked[above[i]] = e[i];
+  wave_sync();
+}
+
+// How far apart the leading parts of two words may lie with their keys the
+// wrong way round, in units of 2^-24 of the keys' range R (a score's 1 and the
+// bias's; a sigmoid's share is within 4 steps of 2^-24: its exponential 4 s (1 -
+// s), its sum 1, its reciprocal 2; a softmax's score s within 33 s: its
+// exponential 4, the sum of up to 1024 of them 22 + 4, the reciprocal 2, the
+// product 1).  The bias over its least, the sum, the product by 2^24 / R and its
+// whole part are a unit each.  Twice all that, for two words.
+__device__ __forceinline__ uint32_t units_apart(bool sigmoid, float largest) {
+  return sigmoid ? 16 : 9 + (uint32_t)(66.0f * fminf(largest, 1.0f));
+}
 
 template <int L, int V>
 __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
   constexpr int TOKENS = RT_THREADS / L;
   // A token's words: keys of the groups' search (32 bits), or of route_exactly.
   __shared__ uint64_t lds[TOKENS * L * V];
-  constexpr int PICKS = L * V < 64 ? L * V : 64;
+  constexpr int PICKS = L * V < ODP_ROUTE_CHOICES ? L * V : ODP_ROUTE_CHOICES;
   __shared__ int picks[TOKENS * PICKS];
   const int slot = threadIdx.x / L, t = threadIdx.x % L;
   int64_t token = (int64_t)blockIdx.x * TOKENS + slot;
@@ -286,15 +369,22 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
   float z[V];
   load_row<V>(z, row, a.dt, first, a.experts);
   const uint32_t mask = (1u << a.bits) - 1;
-  float top = -INFINITY, total = 0.0f;
-  bool odd = false;  // a NaN or +inf
+  // Keys that are sums (of a score and its bias, or of a group's two) are held
+  // as their share of their range, logits of float32 as theirs of the row's
+  // range, the 128 below the largest of it; 16-bit logits fit as they are.
+  const bool sums = bias != nullptr || (a.groups > 1 && a.best == 0);
+  const bool fits = !sums && a.dt != ODP_DTYPE_F32;
+  const uint32_t steps = 1u << min(24, 32 - a.bits);
+  float top = -INFINITY, low = INFINITY, total = 0.0f;
+  bool odd = false, weird = false;  // odd: a NaN or +inf; weird: a row for route_exactly
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     top = fmaxf(top, z[i]);
+    low = fminf(low, z[i]);
     odd |= !(z[i] < INFINITY);
   }
-  const bool whole = !a.sigmoid && (bias != nullptr || !a.renorm || (a.groups > 1 && a.best == 0));
-  if (!a.sigmoid) top = fmax_of<L>(top);
+  top = fmax_of<L>(top);
+  const bool whole = !a.sigmoid && (sums || !a.renorm);
   float p[V];
   if (whole) {
 #pragma unroll
@@ -304,10 +394,9 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
     }
     total = sum_of<L>(total);
   }
-  uint32_t key[V];
+  uint32_t key[V];  // 0: no expert, or closed; leading parts: 1 masked, 2 and more the others
   uint32_t tol = 0;
-  bool again = false;  // to be done from float64 keys
-  if (bias != nullptr || (a.groups > 1 && a.best == 0)) {
+  if (sums) {
     float lo = INFINITY, hi = -INFINITY, b[V];
     if (bias != nullptr) {
       load_row<V>(b, (const char*)bias, ODP_DTYPE_F32, first, a.experts);
@@ -316,7 +405,7 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
         if (first + i < a.experts) {
           lo = fminf(lo, b[i]);
           hi = fmaxf(hi, b[i]);
-          again |= b[i] != b[i];
+          weird |= b[i] != b[i];
         }
       }
       lo = -fmax_of<L>(-lo);
@@ -327,46 +416,84 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
       for (int i = 0; i < V; ++i) b[i] = 0.0f;
     }
     const float range = 1.0f + (hi - lo);
-    again |= !(range < 1e30f);  // infinities among them, too
-    const uint32_t steps = 1u << min(24, 32 - a.bits);
+    weird |= !(range < 1e30f);  // infinities among them, too
     const float by = (float)(steps - 16) / range;
-    tol = BIAS_TOL >> (24 - min(24, 32 - a.bits));
-    tol += tol < BIAS_TOL ? 1 : 0;
     const float over = a.sigmoid ? 0.0f : __builtin_amdgcn_rcpf(total);
+    tol = (units_apart(a.sigmoid, over) >> (24 - min(24, 32 - a.bits))) + 1;  // the largest score is e^0 over the sum
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int e = first + i;
       const float s = a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + exp_near(-z[i])) : p[i] * over;
-      again |= e < a.experts && z[i] == -INFINITY;
-      const uint32_t q = 1 + (uint32_t)fminf(((b[i] - lo) + s) * by, (float)(steps - 8));
-      key[i] = e < a.experts ? q << a.bits | (mask - (uint32_t)e) : 0;
+      const uint32_t q = 2 + (uint32_t)fminf(((b[i] - lo) + s) * by, (float)(steps - 8));
+      key[i] = e < a.experts ? (z[i] == -INFINITY ? 1u : q) << a.bits | (mask - (uint32_t)e) : 0;
+      weird |= a.groups > 1 && e < a.experts && z[i] == -INFINITY;
     }
-  } else {
+  } else if (fits) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int e = first + i;
       key[i] = e < a.experts ? (ordered(z[i] + 0.0f) & ~mask) | (mask - (uint32_t)e) : 0;
     }
+  } else {
+    low = fmaxf(-fmax_of<L>(-low), top - 128.0f);
+    const float by = (float)(steps - 16) * __builtin_amdgcn_rcpf(fmaxf(top - low, 1e-30f));
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int e = first + i;
+      const uint32_t q = 2 + (uint32_t)fminf(fmaxf(z[i] - low, 0.0f) * by, (float)(steps - 8));
+      key[i] = e < a.experts ? (z[i] == -INFINITY ? 1u : q) << a.bits | (mask - (uint32_t)e) : 0;
+    }
   }
-  again |= odd;
+  const uint32_t both = or_of<L>((odd ? 1u : 0u) | (weird ? 2u : 0u));
+  odd = (both & 1) != 0;
+  weird = both != 0;
+  uint64_t* words = lds + slot * L * V;
+  Keys64 exact{a, row, bias, sums};
 
   if (a.groups > 1) {
-    uint32_t* words = (uint32_t*)(lds + slot * L * V);
     uint32_t* scores = (uint32_t*)picked;  // [groups], before the choices
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (first + i < a.experts) words[first + i] = key[i];
-    wave_sync();
-    for (int g = t; g < a.groups; g += L) {
+    const auto second = [](uint32_t& one, uint32_t& two, uint32_t o1, uint32_t o2) {  // the two largest of four
+      two = max(min(one, o1), max(two, o2));
+      one = max(one, o1);
+    };
+    // The sum of two leading parts takes up to 25 bits, a group's number 6; a
+    // best key stands as it is (its low bits order equal ones by the group).
+    const auto score = [&](uint32_t one, uint32_t two, int g) {
+      return a.best == 0 ? ((one >> a.bits) + (two >> a.bits)) << 6 | (uint32_t)(63 - g) : one;
+    };
+    const int span = a.span;  // threads of a group; 0: its bounds lie between them
+    if (span > 0) {
       uint32_t one = 0, two = 0;
-      for (int i = 0; i < a.size; ++i) {
-        const uint32_t w = words[g * a.size + i];
-        two = max(two, min(one, w));
-        one = max(one, w);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        two = max(two, min(one, key[i]));
+        one = max(one, key[i]);
       }
-      // The sum of two leading parts takes up to 25 bits, a group's number 6; a
-      // best key stands as it is (its low bits order equal ones by the group).
-      scores[g] = a.best == 0 ? ((one >> a.bits) + (two >> a.bits)) << 6 | (uint32_t)(63 - g) : one;
+      if (L > 1 && span > 1) second(one, two, across<1>(one), across<1>(two));
+      if (L > 2 && span > 2) second(one, two, across<2>(one), across<2>(two));
+      if (L > 4 && span > 4) second(one, two, across<4>(one), across<4>(two));
+      if (L > 8 && span > 8) second(one, two, across<8>(one), across<8>(two));
+      if (L > 16 && span > 16) second(one, two, across<16>(one), across<16>(two));
+      const int g = t / span;
+      if (t == g * span && g < a.groups) scores[g] = score(one, two, g);
+    } else {
+      uint32_t* all = (uint32_t*)words;
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (first + i < a.experts) all[first + i] = key[i];
+      wave_sync();
+      for (int g = t; g < a.groups; g += L) {
+        uint32_t one = 0, two = 0;
+        int i = g % a.size;  // each thread from another bank on
+#pragma unroll 4
+        for (int k = 0; k < a.size; ++k) {
+          const uint32_t w = all[g * a.size + i];
+          two = max(two, min(one, w));
+          one = max(one, w);
+          i = i + 1 == a.size ? 0 : i + 1;
+        }
+        scores[g] = score(one, two, g);
+      }
     }
     wave_sync();
     uint64_t open = 0;
@@ -374,6 +501,7 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
     for (int g = t; g < a.groups; g += L) {
       const uint32_t mine = scores[g];
       int above = 0;
+#pragma unroll 4
       for (int o = 0; o < a.groups; ++o) above += scores[o] > mine;
       if (above < a.top_groups) open |= 1ull << g;
       if (above == a.top_groups - 1) last = mine;
@@ -381,73 +509,93 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
     }
     last = max_of<L>(last);
     next = max_of<L>(next);
-    const uint32_t lo = or_of<L>((uint32_t)open), hi = or_of<L>((uint32_t)(open >> 32));
+    const uint32_t lo = or_of<L>((uint32_t)open), hi = a.groups > 32 ? or_of<L>((uint32_t)(open >> 32)) : 0;
     open = (uint64_t)hi << 32 | lo;
-    if (a.top_groups < a.groups) {
-      const int shift = a.best == 0 ? 6 : a.bits;
-      const uint32_t apart = (last >> shift) - (next >> shift);
-      again |= a.best == 0 ? apart <= 2 * tol : tol ? apart <= tol : apart == 0 && a.dt == ODP_DTYPE_F32;
-    }
+    const int shift = a.best == 0 ? 6 : a.bits;
+    const uint32_t apart = (last >> shift) - (next >> shift);
     wave_sync();
+    if (!fits && !weird && apart <= (a.best == 0 ? 2 * tol : tol)) open = open_exactly<L, V>(a, exact, t, words);
+    wave_sync();
+    if (span > 0) {
+      if (!(open >> ((t / span) & 63) & 1)) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int g = (int)(((float)(first + i) + 0.5f) * a.per_size);
-      if (!(open >> (g & 63) & 1)) key[i] = 0;
+        for (int i = 0; i < V; ++i) key[i] = 0;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int g = (int)(((float)(first + i) + 0.5f) * a.per_size);
+        if (!(open >> (g & 63) & 1)) key[i] = 0;
+      }
     }
   }
 
+  // The choices, best first, and beyond them all that lie within `tol` of each
+  // other from the last one on: the exact choice is among these candidates.
   uint32_t last = 0;
-  // One choice more than wanted, for how near the next one lies.
-  for (int j = 0; j <= a.top_k; ++j) {
+  int count = 0;
+  bool unsure = false, more = true, full = false;
+  for (int j = 0;; ++j) {
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < V; ++i) m = max(m, key[i] - last);
     m = max_of<L>(m) + last;
     // Nothing below the last one: the largest difference belongs to one above it (or to it).
-    const bool none = j > 0 && m >= last;
-    if (!none && j > 0) {
-      if ((last >> a.bits) - (m >> a.bits) <= tol && m != 0) {
-        // Equal logits and biases are equal keys, which the words order already.
-        const int e0 = (int)(mask - (last & mask)), e1 = (int)(mask - (m & mask));
-        again |= logit(row, a.dt, e0) != logit(row, a.dt, e1) || (bias != nullptr && bias[e0] != bias[e1]);
-      }
+    const bool none = m == 0 || (j > 0 && m >= last);
+    bool near = false;
+    if (!fits && !none && j > 0 && (last >> a.bits) - (m >> a.bits) <= tol) {
+      near = true;
+      // Equal logits and biases are equal keys, which the words order already, and so are two masked ones.
+      const int e0 = (int)(mask - (last & mask)), e1 = (int)(mask - (m & mask));
+      const float z0 = logit(row, a.dt, e0), z1 = logit(row, a.dt, e1);
+      if (more) unsure |= z0 != z1 || (z0 != -INFINITY && bias != nullptr && bias[e0] != bias[e1]);
     }
-    if (j == a.top_k) break;
-    if (t == 0) picked[j] = (int)(mask - (m & mask));
+    if (j >= a.top_k) {
+      more &= near;
+      full |= more && j >= PICKS;
+      more &= j < PICKS;
+      if (__builtin_amdgcn_ballot_w64(more) == 0) break;
+    }
+    if (more) {
+      if (t == 0) picked[j] = (int)(mask - (m & mask));
+      count = j + 1;
+    }
     last = m;
   }
-  again = or_of<L>(again ? 1u : 0u) != 0;
-  odd = or_of<L>(odd ? 1u : 0u) != 0;
-  if (again) route_exactly<L>(a, row, bias, t, lds + slot * L * V, picked);
+  wave_sync();
+  constexpr int PER = (PICKS + L - 1) / L;
+  if (weird || full) route_exactly<L, V>(a, exact, t, words, picked);
+  else if (unsure) rank_exactly<L, PER>(a, exact, t, count, words, picked);
   wave_sync();
 
-  // The weights of the chosen, a few a thread.
+  // The weights of the chosen, PER a thread.
   const bool off = odd && !a.sigmoid;
-  float most = -INFINITY, sum = 0.0f;
-  if (a.renorm) {
-    for (int j = t; j < a.top_k; j += L) most = fmaxf(most, logit(row, a.dt, picked[j]));
-    most = fmax_of<L>(most);
+  int e[PER];
+  float x[PER], most = -INFINITY, sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int j = t + i * L;
+    if (j >= a.top_k) break;
+    e[i] = picked[j];
+    x[i] = logit(row, a.dt, e[i]);
+    most = fmaxf(most, x[i]);
   }
-  // Over the largest of the chosen, so that the sum is never 0; for sigmoids
-  // where all are small.
-  const float shift = a.sigmoid ? (a.renorm ? fminf(most, 0.0f) : 0.0f) : a.renorm ? most : top;
-  const auto share = [&](float x) {
-    if (x == -INFINITY) return 0.0f;
-    if (!a.sigmoid) return exp_near(x - shift);
-    return x >= 0.0f ? 1.0f / (1.0f + exp_near(-x)) : exp_near(x - shift) / (1.0f + exp_near(x));
-  };
-  if (a.renorm) {
-    for (int j = t; j < a.top_k; j += L) sum += share(logit(row, a.dt, picked[j]));
-    sum = sum_of<L>(sum);
-  } else {
-    sum = a.sigmoid ? 1.0f : total;
+  if (a.renorm) most = fmax_of<L>(most);
+  const Shares share(a, most, top);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (t + i * L >= a.top_k) break;
+    x[i] = share(x[i]);
+    sum += x[i];
   }
+  sum = a.renorm ? sum_of<L>(sum) : a.sigmoid ? 1.0f : total;
   if (!live) return;
-  for (int j = t; j < a.top_k; j += L) {
-    const int e = picked[j];
-    const float s = share(logit(row, a.dt, e));
-    const float w = off ? NAN : s == 0.0f ? 0.0f : a.scale * (s / sum);
-    odp_gstore(a.index + token * a.top_k + j, (int64_t)e);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int j = t + i * L;
+    if (j >= a.top_k) break;
+    const float w = off ? NAN : x[i] == 0.0f ? 0.0f : a.scale * (x[i] / sum);
+    odp_gstore(a.index + token * a.top_k + j, (int64_t)e[i]);
     odp_gstore(a.weights + token * a.top_k + j, w);
   }
 }
@@ -489,43 +637,54 @@ __global__ __launch_bounds__(RT_THREADS) void k_route_grad(const RouteArgs a) {
     }
     total = sum_of<L>(total);
   }
-  const auto place = [&](int j) { return (int)min(max(chosen[j], (int64_t)0), (int64_t)(a.experts - 1)); };
-  float most = -INFINITY, sum = 0.0f, dot = 0.0f;
-  if (a.renorm) {
-    for (int j = t; j < a.top_k; j += L) most = fmaxf(most, logit(row, a.dt, place(j)));
-    most = fmax_of<L>(most);
+  constexpr int PICKS = L * V < ODP_ROUTE_CHOICES ? L * V : ODP_ROUTE_CHOICES, PER = (PICKS + L - 1) / L;
+  int e[PER];
+  float x[PER], g[PER], most = -INFINITY, sum = 0.0f, dot = 0.0f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int j = t + i * L;
+    if (j >= a.top_k) break;
+    e[i] = (int)min(max(chosen[j], (int64_t)0), (int64_t)(a.experts - 1));
+    g[i] = gw[j];
   }
-  const float shift = a.sigmoid ? fminf(most, 0.0f) : most;
-  const auto share = [&](float x) {
-    if (x == -INFINITY) return 0.0f;
-    if (!a.sigmoid) return exp_near(x - shift);
-    return x >= 0.0f ? 1.0f / (1.0f + exp_near(-x)) : exp_near(x - shift) / (1.0f + exp_near(x));
-  };
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (t + i * L >= a.top_k) break;
+    x[i] = logit(row, a.dt, e[i]);
+    most = fmaxf(most, x[i]);
+  }
   if (a.renorm) {
-    for (int j = t; j < a.top_k; j += L) {
-      const float s = share(logit(row, a.dt, place(j)));
-      sum += s;
-      dot += s == 0.0f ? 0.0f : s * gw[j];
+    most = fmax_of<L>(most);
+    const Shares share(a, most, 0.0f);
+    float s[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (t + i * L >= a.top_k) break;
+      s[i] = share(x[i]);
+      sum += s[i];
+      dot += s[i] == 0.0f ? 0.0f : s[i] * g[i];
     }
     sum = sum_of<L>(sum);
     dot = sum_of<L>(dot);
     dot = sum > 0.0f ? dot / sum : 0.0f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (t + i * L >= a.top_k) break;
+      g[i] = s[i] == 0.0f ? 0.0f : s[i] / sum * (g[i] - dot);
+      if (a.sigmoid) g[i] *= sigmoid(-x[i]);
+    }
+  } else if (a.sigmoid) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (t + i * L >= a.top_k) break;
+      g[i] = x[i] == -INFINITY ? 0.0f : sigmoid(x[i]) * sigmoid(-x[i]) * g[i];
+    }
   }
   wave_sync();
-  for (int j = t; j < a.top_k; j += L) {
-    const int e = place(j);
-    const float x = logit(row, a.dt, e);
-    float v;
-    if (a.renorm) {
-      const float s = share(x);
-      v = s == 0.0f ? 0.0f : s / sum * (gw[j] - dot);
-      if (a.sigmoid) v *= sigmoid(-x);
-    } else if (a.sigmoid) {
-      v = x == -INFINITY ? 0.0f : sigmoid(x) * sigmoid(-x) * gw[j];
-    } else {
-      v = gw[j];
-    }
-    d[e] = odd ? NAN : v * a.scale;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (t + i * L >= a.top_k) break;
+    d[e[i]] = odd ? NAN : g[i] * a.scale;
   }
   wave_sync();
   float out[V];
@@ -572,8 +731,10 @@ __global__ __launch_bounds__(RT_THREADS) void k_route_grad(const RouteArgs a) {
 }
 
 template <int L, int V>
-void launch_route(hipStream_t s, const RouteArgs& a, bool grad) {
+void launch_route(hipStream_t s, RouteArgs a, bool grad) {
   constexpr int TOKENS = RT_THREADS / L;
+  const int span = a.size / V;
+  a.span = a.size % V == 0 && (span & (span - 1)) == 0 ? span : 0;
   const uint32_t blocks = (uint32_t)((a.n + TOKENS - 1) / TOKENS);
   if (grad) k_route_grad<L, V><<<blocks, RT_THREADS, 0, s>>>(a);
   else k_route<L, V><<<blocks, RT_THREADS, 0, s>>>(a);

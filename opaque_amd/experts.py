@@ -14,9 +14,10 @@ import math
 
 import torch
 
+from opaque_amd._vmap import front, merged
 from opaque_amd.capture import Linear, transformed
 from opaque_amd.engine import dtype_code
-from opaque_amd.vocabulary import _F32, _bound, _call, _front, _OnDevice, _stream, pitched_rows
+from opaque_amd.vocabulary import _F32, _bound, _call, _OnDevice, _stream, pitched_rows
 
 _LOGIT_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _EXPERTS, _CHOICES, _GROUPS = 1024, 64, 64  # ODP_ROUTE_EXPERTS, ODP_ROUTE_CHOICES
@@ -72,8 +73,18 @@ class _RouteGrad(torch.autograd.Function):
 
     @staticmethod
     def vmap(info, in_dims, gw, z, index, *rest):
-        gw, z, index = (_front(t, d, info.batch_size) for t, d in zip((gw, z, index), in_dims))
+        gw, z, index = (front(t, d, info.batch_size) for t, d in zip((gw, z, index), in_dims))
         return _RouteGrad.apply(gw, z, index, *rest), 0
+
+
+def _merge(n, dims, z, bias):
+    """The operands of a batch of n as those of one call."""
+    z = front(z, dims[0], n)
+    if bias is not None and (dims[1] is not None or bias.dim() == 2):
+        # A bias per example; below another vmap the batch comes before its groups.
+        bias = front(bias, dims[1], n)
+        bias = bias.flatten(0, 1) if bias.dim() == 3 else bias
+    return z, bias
 
 
 class _Route(torch.autograd.Function):
@@ -101,12 +112,7 @@ class _Route(torch.autograd.Function):
 
     @staticmethod
     def vmap(info, in_dims, z, bias, *rest):
-        n = info.batch_size
-        z = _front(z, in_dims[0], n)
-        if bias is not None and (in_dims[1] is not None or bias.dim() == 2):
-            # A bias per example; below another vmap the batch comes before its groups.
-            bias = _front(bias, in_dims[1], n)
-            bias = bias.flatten(0, 1) if bias.dim() == 3 else bias
+        z, bias = _merge(info.batch_size, in_dims, z, bias)
         host = None if transformed() else _bound()
         if host is not None:
             sigmoid, groups, top_groups, best, top_k, renorm, scale = rest
@@ -159,9 +165,13 @@ def route(logits: torch.Tensor, top_k: int, *, scores: str = "softmax", bias: to
         raise ValueError(f"scale must be finite in float32, got {scale}")
     bias = None if bias is None else bias.detach()
     args = (scores == "sigmoid", groups, top_groups, _BEST.index(group_best), top_k, bool(renormalize), float(scale))
-    host = None if transformed() else _bound()
+    host = _bound()
     if host is not None:
-        return host.route(logits, bias, *args)
+        if not transformed():
+            return host.route(logits, bias, *args)
+        out = merged(lambda n, dims, z, b: host.route(*_merge(n, dims, z, b), *args), logits, bias)
+        if out is not None:
+            return out
     return _Route.apply(logits, bias, *args)
 
 

@@ -48,27 +48,45 @@ def _tree_norm(leaves: list[torch.Tensor], clip: bool, max_norm: float, wide: bo
     return out, norm
 
 
-def _run(name: str, grads, max_norm: float | None):
-    """The tree's leaves, its structure, the scaled leaves in their places and the norm."""
-    if transformed():
-        raise NotImplementedError(f"{name} does not run inside torch.func transforms")
-    leaves, td = tree_flatten(grads)
-    places = [i for i, t in enumerate(leaves) if isinstance(t, torch.Tensor)]
-    tensors = [leaves[i].detach() for i in places]
+def _checked(name: str, tensors: list[torch.Tensor]) -> bool:
+    """Whether a leaf is float64; every one has to be of a type and on the device that the kernels take."""
+    first, wide = tensors[0].device, False
     for t in tensors:
         if t.dtype not in _LEAF_DTYPES:
             raise TypeError(f"{name} supports float32, bfloat16, float16 and float64 leaves, got {t.dtype}")
-        if t.device.type != "cuda" or t.device != tensors[0].device:
+        if t.device != first or first.type != "cuda":
             raise RuntimeError(f"{name} runs on the GPU: its leaves must be CUDA tensors of one device")
-    if not tensors:
-        return leaves, td, torch.zeros(())
-    wide = any(t.dtype == torch.float64 for t in tensors)
+        wide |= t.dtype == torch.float64
+    return wide
+
+
+def _run(name: str, grads, max_norm: float | None):
+    """(the scaled tree or None, the norm)."""
+    if transformed():
+        raise NotImplementedError(f"{name} does not run inside torch.func transforms")
     clip, host = max_norm is not None, _bound()
-    with torch.no_grad():
-        out, norm = (host.tree_norm if host is not None else _tree_norm)(tensors, clip, max_norm or 0.0, wide)
+    if type(grads) is dict and all(type(t) is torch.Tensor for t in grads.values()):
+        # The usual tree of a step: no structure to walk (20 us for 50 leaves).
+        tensors, td = list(grads.values()), None
+    else:
+        leaves, td = tree_flatten(grads)
+        places = [i for i, t in enumerate(leaves) if isinstance(t, torch.Tensor)]
+        tensors = [leaves[i] for i in places]
+    if not tensors:
+        return grads if td is None else tree_unflatten(td, leaves), torch.zeros(())
+    if host is not None:
+        out, norm = host.tree_norm(tensors, clip, max_norm or 0.0, name)
+    else:
+        wide = _checked(name, tensors)
+        with torch.no_grad():
+            out, norm = _tree_norm([t.detach() for t in tensors], clip, max_norm or 0.0, wide)
+    if not clip:
+        return None, norm
+    if td is None:
+        return dict(zip(grads, out)), norm
     for i, t in zip(places, out):
         leaves[i] = t
-    return leaves, td, norm
+    return tree_unflatten(td, leaves), norm
 
 
 def global_norm(tree) -> torch.Tensor:
@@ -79,7 +97,7 @@ def global_norm(tree) -> torch.Tensor:
     with a float64 leaf float64.  Nothing is copied to the host, and the result
     has no gradient.  An empty tree's norm is 0, on the CPU.
     """
-    return _run("global_norm", tree.pytree if isinstance(tree, ClippedPytree) else tree, None)[2]
+    return _run("global_norm", tree.pytree if isinstance(tree, ClippedPytree) else tree, None)[1]
 
 
 def clip_by_global_norm(grads, max_norm: float):
@@ -102,8 +120,7 @@ def clip_by_global_norm(grads, max_norm: float):
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must be 0 or more, got {max_norm}")
-    leaves, td, norm = _run("clip_by_global_norm", grads, max_norm)
-    return tree_unflatten(td, leaves), norm
+    return _run("clip_by_global_norm", grads, max_norm)
 
 
 __all__ = ["clip_by_global_norm", "global_norm"]

@@ -17,9 +17,10 @@ from __future__ import annotations
 import torch
 
 from opaque_amd import _native as N
+from opaque_amd._vmap import front, merged
 from opaque_amd.capture import transformed
 from opaque_amd.engine import dtype_code
-from opaque_amd.vocabulary import _F32, _bound, _call, _front, _OnDevice, _stream, pitched_rows
+from opaque_amd.vocabulary import _F32, _bound, _call, _OnDevice, _stream, pitched_rows
 
 _ROW_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _WIDE = 32768  # the widest row (ODP_NORM_WIDE)
@@ -114,7 +115,7 @@ class _NormGrad(torch.autograd.Function):
     @staticmethod
     def vmap(info, in_dims, gy, gh, h, rstd, weight, dtype, offset, groups, need_x, need_r, need_w):
         n = info.batch_size
-        gy, gh, h, rstd = (None if t is None else _front(t, d, n) for t, d in zip((gy, gh, h, rstd), in_dims))
+        gy, gh, h, rstd = (None if t is None else front(t, d, n) for t, d in zip((gy, gh, h, rstd), in_dims))
         each = max(groups, 1)
         if weight is not None:
             weight = _batched_gain(weight, in_dims[4], n, groups)
@@ -133,6 +134,15 @@ def _batched_gain(weight, d, n, groups):
         return weight.unsqueeze(0).expand(n, -1)
     return (weight.unsqueeze(0).expand(n, *weight.shape).flatten(0, 1) if weight.dim() == 2
             else weight.unsqueeze(0).expand(n * groups, -1))
+
+
+def _merge(n, dims, x, residual, weight):
+    """The operands of a batch of n as those of one call."""
+    x = front(x, dims[0], n)
+    residual = None if residual is None else front(residual, dims[1], n)
+    if weight is not None and (dims[2] is not None or weight.dim() == 2):
+        weight = _batched_gain(weight, dims[2], n, weight.shape[0] if dims[2] is None else 0)
+    return x, residual, weight
 
 
 class _Norm(torch.autograd.Function):
@@ -164,11 +174,7 @@ class _Norm(torch.autograd.Function):
 
     @staticmethod
     def vmap(info, in_dims, x, residual, weight, eps, offset):
-        n = info.batch_size
-        x = _front(x, in_dims[0], n)
-        residual = None if residual is None else _front(residual, in_dims[1], n)
-        if weight is not None and (in_dims[2] is not None or weight.dim() == 2):
-            weight = _batched_gain(weight, in_dims[2], n, weight.shape[0] if in_dims[2] is None else 0)
+        x, residual, weight = _merge(info.batch_size, in_dims, x, residual, weight)
         host = None if transformed() else _bound()
         if host is not None:
             y, rstd, *h = host.rms_norm_kept(x, residual, weight, eps, offset)
@@ -215,10 +221,14 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, *, residual: t
     """
     _check("rms_norm", x, weight, residual, eps)
     offset = 1.0 if unit_offset and weight is not None else 0.0
-    host = None if transformed() else _bound()
+    host = _bound()
     if host is not None:
-        out = host.rms_norm(x, residual, weight, eps, offset)
-        return tuple(out) if residual is not None else out[0]
+        if not transformed():
+            out = host.rms_norm(x, residual, weight, eps, offset)
+        else:
+            out = merged(lambda n, dims, *ts: host.rms_norm(*_merge(n, dims, *ts), eps, offset), x, residual, weight)
+        if out is not None:
+            return tuple(out) if residual is not None else out[0]
     y, h, _ = _Norm.apply(x, residual, weight, float(eps), offset)
     return y if residual is None else (y, h)
 
