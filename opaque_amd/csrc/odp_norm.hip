@@ -30,7 +30,9 @@ typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 // The same at any 2- or 4-byte address.
 typedef u32x4_t u32x4_h __attribute__((aligned(2)));
 typedef u32x4_t u32x4_w __attribute__((aligned(4)));
+typedef u32x2_t u32x2_h __attribute__((aligned(2)));
 typedef u32x2_t u32x2_b __attribute__((aligned(1)));
+typedef uint32_t uint32_h __attribute__((aligned(2)));
 
 // What a thread holds of a row: 8 values of float32 (F32) or of a 16-bit type,
 // as they lie in memory.
@@ -38,26 +40,63 @@ template <bool F32>
 struct Eight {
   u32x4_t w[F32 ? 2 : 1];
 
+  // Values c to c + 8 of a row, whatever its width.
+  template <bool NT>
+  __device__ __forceinline__ void load_whole(const char* row, int c) {
+    if constexpr (F32) {
+      const ODP_GMEM u32x4_w* p = (const ODP_GMEM u32x4_w*)(const ODP_GMEM void*)(row + 4 * c);
+      w[0] = NT ? __builtin_nontemporal_load(p) : p[0];
+      w[1] = NT ? __builtin_nontemporal_load(p + 1) : p[1];
+    } else {
+      const ODP_GMEM u32x4_h* p = (const ODP_GMEM u32x4_h*)(const ODP_GMEM void*)(row + 2 * c);
+      w[0] = NT ? __builtin_nontemporal_load(p) : p[0];
+    }
+  }
   // Values c to c + 8 of a row of `width` (0 past it).
+  template <bool NT = false>
   __device__ __forceinline__ void load(const char* row, int c, int width) {
     if (c + 8 <= width) {
-      if constexpr (F32) {
-        const ODP_GMEM u32x4_w* p = (const ODP_GMEM u32x4_w*)(const ODP_GMEM void*)(row + 4 * c);
-        w[0] = p[0];
-        w[1] = p[1];
-      } else {
-        w[0] = *(const ODP_GMEM u32x4_h*)(const ODP_GMEM void*)(row + 2 * c);
-      }
+      load_whole<NT>(row, c);
       return;
     }
-    w[0] = u32x4_t{0, 0, 0, 0};
-    if constexpr (F32) w[1] = w[0];
-    if (c >= width) return;
+    if (c >= width) {
+      w[0] = u32x4_t{0, 0, 0, 0};
+      if constexpr (F32) w[1] = w[0];
+    } else if (width >= 8) {
+      load_whole<NT>(row, width - 8);  // the row's last 8, moved down to c
+      down(c + 8 - width);
+    } else {
+      w[0] = u32x4_t{0, 0, 0, 0};
+      if constexpr (F32) w[1] = w[0];
 #pragma unroll
-    for (int i = 0; i < 7; ++i) {
-      if (c + i >= width) break;
-      if constexpr (F32) w[i / 4][i % 4] = ((const uint32_t*)row)[c + i];
-      else w[0][i / 2] |= (uint32_t)((const uint16_t*)row)[c + i] << 16 * (i % 2);
+      for (int i = 0; i < 7; ++i) {
+        if (i >= width) break;
+        if constexpr (F32) w[i / 4][i % 4] = ((const uint32_t*)row)[i];
+        else w[0][i / 2] |= (uint32_t)((const uint16_t*)row)[i] << 16 * (i % 2);
+      }
+    }
+  }
+  // Value i becomes value i + n's, 0 past the last (n below 8).
+  __device__ __forceinline__ void down(int n) {
+    if constexpr (F32) {
+      uint32_t v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = w[i / 4][i % 4];
+#pragma unroll
+      for (int by = 4; by > 0; by >>= 1)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = n & by ? (i + by < 8 ? v[i + by] : 0) : v[i];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i / 4][i % 4] = v[i];
+    } else {
+      uint32_t v[4] = {w[0][0], w[0][1], w[0][2], w[0][3]};
+#pragma unroll
+      for (int by = 2; by > 0; by >>= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = n & 2 * by ? (i + by < 4 ? v[i + by] : 0) : v[i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = n & 1 ? v[i] >> 16 | (i < 3 ? v[i + 1] << 16 : 0) : v[i];
+      w[0] = u32x4_t{v[0], v[1], v[2], v[3]};
     }
   }
   __device__ __forceinline__ void get(float (&v)[8], int dt) const {
@@ -104,14 +143,53 @@ struct Eight {
       }
       return;
     }
-#pragma unroll
-    for (int i = 0; i < 7; ++i) {
-      if (c + i >= width) break;
-      if constexpr (F32) odp_gstore((uint32_t*)row + c + i, w[i / 4][i % 4]);
-      else odp_gstore((uint16_t*)row + c + i, (uint16_t)(w[0][i / 2] >> 16 * (i % 2)));
+    // The 4, 2 and 1 values that make up what is left.
+    int n = width - c;
+    if (n <= 0) return;
+    Eight rest = *this;
+    if constexpr (F32) {
+      uint32_t* to = (uint32_t*)row + c;
+      if (n & 4) {
+        *(ODP_GMEM u32x4_w*)(ODP_GMEM void*)to = rest.w[0];
+        rest.w[0] = rest.w[1];
+        to += 4;
+      }
+      if (n & 2) {
+        odp_gstore(to, rest.w[0][0]);
+        odp_gstore(to + 1, rest.w[0][1]);
+        rest.w[0][0] = rest.w[0][2];
+        to += 2;
+      }
+      if (n & 1) odp_gstore(to, rest.w[0][0]);
+    } else {
+      uint16_t* to = (uint16_t*)row + c;
+      if (n & 4) {
+        *(ODP_GMEM u32x2_h*)(ODP_GMEM void*)to = u32x2_t{rest.w[0][0], rest.w[0][1]};
+        rest.w[0][0] = rest.w[0][2];
+        rest.w[0][1] = rest.w[0][3];
+        to += 4;
+      }
+      if (n & 2) {
+        *(ODP_GMEM uint32_h*)(ODP_GMEM void*)to = rest.w[0][0];
+        rest.w[0][0] = rest.w[0][1];
+        to += 2;
+      }
+      if (n & 1) odp_gstore(to, (uint16_t)rest.w[0][0]);
     }
   }
 };
+
+// A thread's vectors of a row; nt: by non-temporal loads (NORM_ONCE).
+template <int T, bool F32, int NV>
+__device__ __forceinline__ void load_rows(Eight<F32> (&x)[NV], const char* row, int width, int t, int nt) {
+  if (!F32 && nt) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) x[v].template load<true>(row, 8 * (v * T + t), width);
+  } else {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) x[v].load(row, 8 * (v * T + t), width);
+  }
+}
 
 // 8 gains of the run-time type dt, 1 where there are none.
 __device__ __forceinline__ void load_gain(float (&g)[8], const char* row, int dt, float offset, int c, int width) {
@@ -196,7 +274,7 @@ struct NormArgs {
   float *rstd, *scales;
   int64_t ldx, ldr, ldg, n;  // pitches in bytes
   int64_t rows_per_gain;
-  int width, dt, ht, gt;
+  int width, dt, ht, gt, nt;
   float eps, offset;
 };
 
@@ -219,12 +297,8 @@ __global__ __launch_bounds__(norm_threads<T>()) void k_rms_norm(const NormArgs a
   const int width = a.width;
   Eight<XF> x[NV];
   Eight<HF> r[NV];
-#pragma unroll
-  for (int v = 0; v < NV; ++v) x[v].load(a.x + row * a.ldx, 8 * (v * T + t), width);
-  if (a.r != nullptr) {
-#pragma unroll
-    for (int v = 0; v < NV; ++v) r[v].load(a.r + row * a.ldr, 8 * (v * T + t), width);
-  }
+  load_rows<T>(x, a.x + row * a.ldx, width, t, a.nt);
+  if (a.r != nullptr) load_rows<T>(r, a.r + row * a.ldr, width, t, a.nt);
   float f[NV][8], sum = 0.0f;
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
@@ -314,12 +388,14 @@ struct NormGradArgs {
   char *dx, *dr, *dw;
   float* part;
   int64_t ldh, ldy, ldgh, ldg;  // pitches in bytes
-  int64_t rows_per_gain, len, strips;
-  int width, dt, ht, gt;
+  int64_t rows_per_gain, strips;
+  int width, dt, ht, gt, nt;
   float offset;
 };
 
-// Workgroup (gain, strip): rows [strip len, ..) of that gain's rows.
+// Workgroup (gain, strip): every strips-th ROWS of that gain's rows, so that the
+// workgroups together walk the tensors from front to back (4.7 TB/s; each along
+// rows of its own, 128 KB apart: 4.4).
 template <bool XF, bool HF, int T, int NV>
 __global__ __launch_bounds__(norm_threads<T>()) void k_rms_norm_grad(const NormGradArgs a) {
   constexpr int ROWS = norm_threads<T>() / T;
@@ -328,8 +404,8 @@ __global__ __launch_bounds__(norm_threads<T>()) void k_rms_norm_grad(const NormG
   const int t = T < 256 ? (int)(threadIdx.x % T) : (int)threadIdx.x;
   const int slot = T < 256 ? (int)(threadIdx.x / T) : 0;
   const int64_t group = blockIdx.x / a.strips, strip = blockIdx.x - group * a.strips;
-  const int64_t first = group * a.rows_per_gain + strip * a.len;
-  const int64_t last = group * a.rows_per_gain + min((strip + 1) * a.len, a.rows_per_gain);
+  const int64_t first = group * a.rows_per_gain + strip * ROWS, last = (group + 1) * a.rows_per_gain;
+  const int64_t step = a.strips * ROWS;
   const int width = a.width;
   const char* gain = a.gain == nullptr ? nullptr : a.gain + group * a.ldg;
   float g[NV][8], acc[NV][8];
@@ -339,23 +415,25 @@ __global__ __launch_bounds__(norm_threads<T>()) void k_rms_norm_grad(const NormG
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[v][i] = 0.0f;
   }
+  // The next row's loads go out before a row's sum over its threads and its
+  // stores, where the registers hold both (AHEAD).
+  constexpr bool AHEAD = NV * (XF ? 2 : 1) <= 2;
+  Eight<HF> h[NV], gh[NV];
+  Eight<XF> gy[NV];
+  float inv = 0.0f;
+  const bool with_gh = a.gh != nullptr && a.dx != nullptr;
+  const auto load = [&](int64_t row) {
+    load_rows<T>(h, a.h + row * a.ldh, width, t, a.nt);
+    load_rows<T>(gy, a.gy + row * a.ldy, width, t, a.nt);
+    if (with_gh) load_rows<T>(gh, a.gh + row * a.ldgh, width, t, a.nt);
+    inv = a.rstd[row];
+  };
   int turn = 0;
-  for (int64_t base = first; base < last; base += ROWS, ++turn) {
-    int64_t row = base + slot;
-    const bool live = row < last;
-    row = live ? row : last - 1;
-    Eight<HF> h[NV], gh[NV];
-    Eight<XF> gy[NV];
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      h[v].load(a.h + row * a.ldh, 8 * (v * T + t), width);
-      gy[v].load(a.gy + row * a.ldy, 8 * (v * T + t), width);
-    }
-    if (a.gh != nullptr && a.dx != nullptr) {
-#pragma unroll
-      for (int v = 0; v < NV; ++v) gh[v].load(a.gh + row * a.ldgh, 8 * (v * T + t), width);
-    }
-    const float inv = a.rstd[row];
+  if (AHEAD) load(min(first + slot, last - 1));
+  for (int64_t base = first; base < last; base += step, ++turn) {
+    const bool live = base + slot < last;
+    const int64_t row = live ? base + slot : last - 1;
+    if (!AHEAD) load(row);
     float u[NV][8], dot = 0.0f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -370,6 +448,12 @@ __global__ __launch_bounds__(norm_threads<T>()) void k_rms_norm_grad(const NormG
         dot = fmaf(p, g[v][i], dot);
       }
     }
+    Eight<XF> gy0[NV];
+    Eight<HF> gh0[NV];
+    const float inv0 = inv;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) gy0[v] = gy[v], gh0[v] = gh[v];
+    if (AHEAD && base + step < last) load(min(base + step + slot, last - 1));
     if (a.dx == nullptr) continue;
     const float mean = sum_row<T>(dot, red[0], turn) / (float)width;
     if (!live) continue;
@@ -377,12 +461,12 @@ __global__ __launch_bounds__(norm_threads<T>()) void k_rms_norm_grad(const NormG
     for (int v = 0; v < NV; ++v) {
       const int c = 8 * (v * T + t);
       float d[8];
-      gy[v].get(d, a.dt);
+      gy0[v].get(d, a.dt);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) d[i] = inv * (d[i] * g[v][i] - u[v][i] * mean);
-      if (a.gh != nullptr) {
+      for (int i = 0; i < 8; ++i) d[i] = inv0 * (d[i] * g[v][i] - u[v][i] * mean);
+      if (with_gh) {
         float o[8];
-        gh[v].get(o, a.ht);
+        gh0[v].get(o, a.ht);
 #pragma unroll
         for (int i = 0; i < 8; ++i) d[i] += o[i];
       }
@@ -429,53 +513,63 @@ __global__ __launch_bounds__(norm_threads<T>()) void k_rms_norm_grad(const NormG
   }
 }
 
-// dw of 64 columns of one gain: 16 waves sum every 16th strip, then each other.
-__global__ __launch_bounds__(1024) void k_gain_sum(const float* __restrict__ part, int64_t strips, int width, int tiles,
-                                                   int gt, void* dw) {
-  __shared__ float red[16][64];
+// dw of COLS columns of one gain: the threads of a workgroup take a strip each per
+// column, 8 at a time, then add up over LDS.  64 columns a workgroup, but 16 where
+// that leaves fewer than 64 workgroups (1001 columns of 1024 strips: 7 and 4 us).
+constexpr int GS_THREADS = 1024;
+template <int COLS>
+__global__ __launch_bounds__(GS_THREADS) void k_gain_sum(const float* __restrict__ part, int64_t strips, int width,
+                                                         int tiles, int gt, void* dw) {
+  constexpr int AT = GS_THREADS / COLS;  // strips at a time
+  __shared__ float red[AT][COLS + 1];
   const int64_t group = blockIdx.x / tiles;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c = (int)(blockIdx.x - group * tiles) * 64 + lane;
+  const int lane = threadIdx.x % COLS, own = threadIdx.x / COLS;
+  const int c = (int)(blockIdx.x - group * tiles) * COLS + lane;
   const float* p = part + group * strips * width + c;
   float s = 0.0f;
   if (c < width) {
-    int64_t i = wave;
-    for (; i + 16 * 3 < strips; i += 16 * 4) {
-      float v[4];
+    int64_t i = own;
+    for (; i + AT * 7 < strips; i += AT * 8) {
+      float v[8];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = p[(i + 16 * k) * width];
+      for (int k = 0; k < 8; ++k) v[k] = p[(i + AT * k) * width];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) s += v[k];
+      for (int k = 0; k < 8; ++k) s += v[k];
     }
-    for (; i < strips; i += 16) s += p[i * width];
+    for (; i < strips; i += AT) s += p[i * width];
   }
-  red[wave][lane] = s;
+  red[own][lane] = s;
   __syncthreads();
-  if (wave != 0 || c >= width) return;
+  if (threadIdx.x >= 64) return;
+  // One wave: 64 / COLS shares of the strips' sums a column.
+  constexpr int EACH = AT * COLS / 64;
+  s = 0.0f;
 #pragma unroll
-  for (int i = 1; i < 16; ++i) s += red[i][lane];
-  odp_store_from_float(dw, group * width + c, gt, s);
+  for (int i = 0; i < EACH; ++i) s += red[own * EACH + i][lane];
+#pragma unroll
+  for (int x = COLS; x < 64; x <<= 1) s += __shfl_xor(s, x);
+  if (own == 0 && c < width) odp_store_from_float(dw, group * width + c, gt, s);
 }
 
-// Strips of a gain's rows: about four workgroups a compute unit in all.
-struct Strips {
-  int64_t len, count;
-};
-constexpr int64_t NORM_GROUPS = 1024;
+// Bytes that a launch reads from which on it loads 16-bit rows non-temporally, as
+// they cannot lie in the 256 MB cache: 16384 x 4096 bfloat16, gradient (403 MB read)
+// 88 us, 116 through the caches, forward pass behind it (268 MB) 96 and 104.  Below,
+// what was written just before may be there: 4096 x 4096 (67 MB), 26 us and 21.
+constexpr int64_t NORM_ONCE = (int64_t)192 << 20;
+// Workgroups of the gradient: two a compute unit, which leave 512 strips to add up
+// (16384 x 4096: 88 + 5 us; 1024 strips 104 + 6).
+constexpr int64_t NORM_GROUPS = 512;
 
 int norm_tile(int64_t width) {  // threads of a row
   const int64_t v = (width + 7) / 8;
   return v <= 8 ? 8 : v <= 16 ? 16 : v <= 32 ? 32 : v <= 256 ? 64 : v <= 1024 ? 256 : 1024;
 }
 
-Strips strips_of(int64_t n, int64_t width, int64_t gains) {
-  const int64_t rows = n / gains;
+// Strips of a gain's rows.
+int64_t strips_of(int64_t n, int64_t width, int64_t gains) {
   const int t = norm_tile(width), at = t < 256 ? 256 / t : 1;
-  int64_t count = (NORM_GROUPS + gains - 1) / gains;
-  int64_t len = (rows + count - 1) / count;
-  len = (len + at - 1) / at * at;
-  if (len < 1) len = 1;
-  return {len, rows > 0 ? (rows + len - 1) / len : 1};
+  const int64_t rows = (n / gains + at - 1) / at, count = (NORM_GROUPS + gains - 1) / gains;
+  return rows < count ? (rows > 0 ? rows : 1) : count;
 }
 
 bool norm_type(int dt) { return dt == ODP_DTYPE_F32 || dt == ODP_DTYPE_BF16 || dt == ODP_DTYPE_F16; }
@@ -582,6 +676,7 @@ extern "C" int odp_rms_norm(odp_stream_t stream, int dtype, int stream_dtype, in
   a.gt = gain_dtype;
   a.eps = eps;
   a.offset = offset;
+  a.nt = n * width * (odp_dtype_size(dtype) + (residual != nullptr ? odp_dtype_size(stream_dtype) : 0)) > NORM_ONCE;
   hipStream_t s = odp_hip_stream(stream);
   if (dtype == ODP_DTYPE_F32) norm_form<true, true>(s, a, quant);
   else if (stream_dtype == ODP_DTYPE_F32 && residual != nullptr) norm_form<false, true>(s, a, quant);
@@ -591,8 +686,8 @@ extern "C" int odp_rms_norm(odp_stream_t stream, int dtype, int stream_dtype, in
 
 extern "C" int64_t odp_rms_norm_grad_scratch(int64_t n, int64_t width, int64_t gains) {
   if (n <= 0 || width < 1 || width > ODP_NORM_WIDE || gains < 1 || n % gains != 0) return 0;
-  const Strips s = strips_of(n, width, gains);
-  return s.count > 1 ? 4 * gains * s.count * width : 0;
+  const int64_t strips = strips_of(n, width, gains);
+  return strips > 1 ? 4 * gains * strips * width : 0;
 }
 
 extern "C" int odp_rms_norm_grad(odp_stream_t stream, int dtype, int stream_dtype, int gain_dtype, const void* h,
@@ -612,8 +707,8 @@ extern "C" int odp_rms_norm_grad(odp_stream_t stream, int dtype, int stream_dtyp
     return ODP_ERR_INVALID_ARGUMENT;
   }
   if (dx == nullptr && dgain == nullptr) return ODP_OK;
-  const Strips st = strips_of(n, width, gains);
-  if (dgain != nullptr && st.count > 1 && scratch == nullptr) {
+  const int64_t strips = strips_of(n, width, gains);
+  if (dgain != nullptr && strips > 1 && scratch == nullptr) {
     odp_set_error("%s: null scratch where odp_rms_norm_grad_scratch is not 0", what);
     return ODP_ERR_INVALID_ARGUMENT;
   }
@@ -625,32 +720,34 @@ extern "C" int odp_rms_norm_grad(odp_stream_t stream, int dtype, int stream_dtyp
   a.rstd = rstd;
   a.dx = (char*)dx;
   a.dr = (char*)dres;
-  a.dw = dgain != nullptr && st.count == 1 ? (char*)dgain : nullptr;
-  a.part = dgain != nullptr && st.count > 1 ? (float*)scratch : nullptr;
+  a.dw = dgain != nullptr && strips == 1 ? (char*)dgain : nullptr;
+  a.part = dgain != nullptr && strips > 1 ? (float*)scratch : nullptr;
   a.ldh = ldh * odp_dtype_size(stream_dtype);
   a.ldy = ldy * odp_dtype_size(dtype);
   a.ldgh = ldgh * odp_dtype_size(stream_dtype);
   a.ldg = ldg * odp_dtype_size(gain_dtype);
   a.rows_per_gain = n / gains;
-  a.len = st.len;
-  a.strips = st.count;
+  a.strips = strips;
   a.width = (int)width;
   a.dt = dtype;
   a.ht = stream_dtype;
   a.gt = gain_dtype;
   a.offset = offset;
+  a.nt = n * width * (odp_dtype_size(dtype) + odp_dtype_size(stream_dtype) * (gh != nullptr ? 2 : 1)) > NORM_ONCE;
   hipStream_t s = odp_hip_stream(stream);
-  const int64_t blocks = gains * st.count;  // at most n
+  const int64_t blocks = gains * strips;  // at most n
   if (dtype == ODP_DTYPE_F32) grad_form<true, true>(s, a, blocks);
   else if (stream_dtype == ODP_DTYPE_F32) grad_form<false, true>(s, a, blocks);
   else grad_form<false, false>(s, a, blocks);
   if (a.part != nullptr) {
-    const int tiles = (int)((width + 63) / 64);
+    const int cols = gains * ((width + 63) / 64) < 64 ? 16 : 64;
+    const int64_t tiles = (width + cols - 1) / cols;
     if (gains * tiles >= (int64_t)1 << 31) {
       odp_set_error("%s: too many gains", what);
       return ODP_ERR_UNSUPPORTED;
     }
-    k_gain_sum<<<(uint32_t)(gains * tiles), 1024, 0, s>>>(a.part, st.count, (int)width, tiles, gain_dtype, dgain);
+    const auto sum = cols == 16 ? k_gain_sum<16> : k_gain_sum<64>;
+    sum<<<(uint32_t)(gains * tiles), GS_THREADS, 0, s>>>(a.part, strips, (int)width, (int)tiles, gain_dtype, dgain);
   }
   return odp_check_launch(what);
 }
