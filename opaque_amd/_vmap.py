@@ -14,6 +14,7 @@ from collections.abc import Callable
 import torch
 
 _F = torch._C._functorch
+_VMAP = _F.TransformType.Vmap
 
 
 def front(t: torch.Tensor, d: int | None, size: int) -> torch.Tensor:
@@ -24,10 +25,10 @@ def front(t: torch.Tensor, d: int | None, size: int) -> torch.Tensor:
 def merged(call: Callable, *operands: torch.Tensor | None):
     """``call(size, dims, *physical operands)`` below the one active vmap, its outputs batched in front; None where
     another transform is active or no operand is batched.  ``dims``: each operand's batch dimension or None."""
-    stack = _F.get_interpreter_stack()
-    if stack is None or len(stack) != 1 or stack[0].key() != _F.TransformType.Vmap:
+    top = _F.peek_interpreter_stack()
+    level = 0 if top is None else top.level()
+    if level != 1 or top.key() != _VMAP:  # levels count from 1
         return None
-    level = stack[0].level()
     values, dims, size = [], [], None
     for t in operands:
         if t is not None and _F.is_batchedtensor(t):

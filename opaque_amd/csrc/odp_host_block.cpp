@@ -14,6 +14,7 @@ namespace {
 using odp_host::bytes_on;
 using odp_host::code_of;
 using odp_host::pitched;
+using odp_host::Rows;
 using odp_host::stream_of;
 
 struct Abi {
@@ -85,24 +86,24 @@ struct Normed {
 Normed norm_forward(const at::Tensor& x, const Maybe& residual, const Maybe& weight, double eps, double offset,
                     bool keep, int64_t quant) {
   const c10::OptionalDeviceGuard guard(x.device());
-  const at::Tensor rows = pitched(x), r = residual.has_value() ? pitched(*residual) : at::Tensor();
-  const int dt = code_of(rows), ht = r.defined() ? code_of(r) : dt;
-  const int64_t n = rows.size(0), width = rows.size(1);
+  const Rows rows(x), r = residual.has_value() ? Rows(*residual) : Rows();
+  const int dt = code_of(x), ht = residual.has_value() ? code_of(*residual) : dt;
+  const int64_t n = rows.n, width = rows.width;
   const Gain g(weight, dt);
   Normed out;
-  out.y = at::empty(x.sizes(), quant ? rows.options().dtype(at::kFloat8_e4m3fn) : rows.options());
-  if (r.defined()) out.h = at::empty(x.sizes(), r.options());
-  const auto f32 = rows.options().dtype(at::kFloat);
-  std::vector<int64_t> shape(x.sizes().vec());
-  shape.pop_back();
-  if (keep) out.rstd = at::empty(shape, f32);
+  const bool with = residual.has_value();
+  out.y = at::empty(x.sizes(), quant ? x.options().dtype(at::kFloat8_e4m3fn) : x.options());
+  if (with) out.h = at::empty(x.sizes(), residual->options());
+  const auto f32 = x.options().dtype(at::kFloat);
+  if (keep) out.rstd = at::empty(x.sizes().slice(0, x.dim() - 1), f32);
   if (quant) {
+    std::vector<int64_t> shape(x.sizes().vec());
+    shape.pop_back();
     if (quant == 2) shape.push_back((width + 127) / 128);
     out.scales = at::empty(shape, f32);
   }
-  check(abi.rms_norm(stream_of(rows), dt, ht, g.dt, rows.data_ptr(), rows.stride(0), r.defined() ? r.data_ptr() : nullptr,
-                     r.defined() ? r.stride(0) : 0, n, width, g.at, g.pitch, g.count, (float)eps, (float)offset,
-                     (int)quant, out.y.data_ptr(), r.defined() ? out.h.data_ptr() : nullptr,
+  check(abi.rms_norm(stream_of(x), dt, ht, g.dt, rows.at, rows.pitch, r.at, r.pitch, n, width, g.at, g.pitch, g.count,
+                     (float)eps, (float)offset, (int)quant, out.y.data_ptr(), with ? out.h.data_ptr() : nullptr,
                      keep ? (float*)out.rstd.data_ptr() : nullptr, quant ? (float*)out.scales.data_ptr() : nullptr),
         "odp_rms_norm");
   return out;
@@ -140,24 +141,23 @@ struct NormNode final : torch::autograd::Node {
       const at::Tensor& like = gy0.defined() ? gy0 : gh0;
       const c10::OptionalDeviceGuard guard(like.device());
       odp_host::as_saved(h_, like, ht, shape, kNorms);
-      const at::Tensor rows = pitched(h_);
-      const int64_t n = rows.size(0), width = rows.size(1);
-      const at::Tensor stat = odp_host::whole(rstd_.reshape({-1}), like, at::kFloat, {n}, kNorms);
+      const Rows rows(h_);
+      const int64_t n = rows.n, width = rows.width;
+      odp_host::as_saved(rstd_, like, at::kFloat, at::IntArrayRef(shape).slice(0, shape.size() - 1), kNorms);
+      const at::Tensor stat = rstd_.contiguous();
       if (has_w) odp_host::as_saved(w_, like, wt, w_shape, kNorms);
-      const auto options = rows.options().dtype(xt);
-      const at::Tensor gy = gy0.defined() ? pitched(gy0) : at::zeros({n, width}, options);
-      const at::Tensor gh = gh0.defined() ? pitched(gh0) : at::Tensor();
-      const Gain g(has_w ? Maybe(w_) : Maybe(), code_of(gy));
+      const auto options = h_.options().dtype(xt);
+      const Rows gy(gy0.defined() ? gy0 : at::zeros(shape, options)), gh = gh0.defined() ? Rows(gh0) : Rows();
+      const Gain g(has_w ? Maybe(w_) : Maybe(), code_of(gy.held));
       const bool same = xt == ht;
       if (need_x || need_r) dx = at::empty(shape, options);
-      if (need_r && !same) dr = at::empty(shape, rows.options());
-      if (need_w) dw = n > 0 ? at::empty(w_shape, rows.options().dtype(wt)) : at::zeros(w_shape, rows.options().dtype(wt));
+      if (need_r && !same) dr = at::empty(shape, h_.options());
+      if (need_w) dw = n > 0 ? at::empty(w_shape, w_.options()) : at::zeros(w_shape, w_.options());
       const int64_t words = need_w ? abi.rms_norm_grad_scratch(n, width, g.count) : 0;
-      const at::Tensor work = words > 0 ? bytes_on(rows, words) : at::Tensor();
-      check(abi.rms_norm_grad(stream_of(rows), code_of(gy), code_of(rows), g.dt, rows.data_ptr(), rows.stride(0),
-                              (const float*)stat.data_ptr(), gy.data_ptr(), gy.stride(0),
-                              gh.defined() ? gh.data_ptr() : nullptr, gh.defined() ? gh.stride(0) : 0, n, width, g.at,
-                              g.pitch, g.count, (float)offset, work.defined() ? work.data_ptr() : nullptr,
+      const at::Tensor work = words > 0 ? bytes_on(h_, words) : at::Tensor();
+      check(abi.rms_norm_grad(stream_of(h_), code_of(gy.held), code_of(h_), g.dt, rows.at, rows.pitch,
+                              (const float*)stat.data_ptr(), gy.at, gy.pitch, gh.at, gh.pitch, n, width, g.at, g.pitch,
+                              g.count, (float)offset, work.defined() ? work.data_ptr() : nullptr,
                               dx.defined() ? dx.data_ptr() : nullptr, dr.defined() ? dr.data_ptr() : nullptr,
                               dw.defined() ? dw.data_ptr() : nullptr),
             "odp_rms_norm_grad");
@@ -248,15 +248,16 @@ struct Options {
 
 std::pair<at::Tensor, at::Tensor> route_forward(const at::Tensor& z, const Maybe& bias, const Options& o) {
   const c10::OptionalDeviceGuard guard(z.device());
-  const at::Tensor rows = pitched(z), b = bias.has_value() ? bias->contiguous() : at::Tensor();
+  const Rows rows(z);
+  const at::Tensor b = bias.has_value() ? bias->contiguous() : at::Tensor();
   std::vector<int64_t> shape(z.sizes().vec());
   shape.back() = o.top_k;
-  const at::Tensor index = at::empty(shape, rows.options().dtype(at::kLong));
-  const at::Tensor weights = at::empty(shape, rows.options().dtype(at::kFloat));
-  check(abi.route(stream_of(rows), code_of(rows), rows.data_ptr(), rows.stride(0), rows.size(0), rows.size(1),
-                  (int)o.sigmoid, b.defined() ? (const float*)b.data_ptr() : nullptr,
-                  b.defined() && b.dim() == 2 ? b.size(0) : 1, o.groups, o.top_groups, (int)o.best, o.top_k,
-                  (int)o.renorm, (float)o.scale, (int64_t*)index.data_ptr(), (float*)weights.data_ptr()),
+  const at::Tensor index = at::empty(shape, z.options().dtype(at::kLong));
+  const at::Tensor weights = at::empty(shape, z.options().dtype(at::kFloat));
+  check(abi.route(stream_of(z), code_of(z), rows.at, rows.pitch, rows.n, rows.width, (int)o.sigmoid,
+                  b.defined() ? (const float*)b.data_ptr() : nullptr, b.defined() && b.dim() == 2 ? b.size(0) : 1,
+                  o.groups, o.top_groups, (int)o.best, o.top_k, (int)o.renorm, (float)o.scale,
+                  (int64_t*)index.data_ptr(), (float*)weights.data_ptr()),
         "odp_route");
   return {index, weights};
 }
@@ -284,14 +285,14 @@ struct RouteNode final : torch::autograd::Node {
       at::NoGradGuard no_grad;
       const c10::OptionalDeviceGuard guard(gw.device());
       odp_host::as_saved(z_, gw, type, shape, kRoutes);
-      const at::Tensor rows = pitched(z_);
+      const Rows rows(z_);
       std::vector<int64_t> chosen(shape);
       chosen.back() = o.top_k;
       const at::Tensor at_ = odp_host::whole(index_, gw, at::kLong, chosen, kRoutes), g = gw.contiguous();
-      dz = at::empty(shape, rows.options());
-      check(abi.route_grad(stream_of(rows), code_of(rows), rows.data_ptr(), rows.stride(0), rows.size(0), rows.size(1),
-                           (int)o.sigmoid, o.top_k, (int)o.renorm, (float)o.scale, (const int64_t*)at_.data_ptr(),
-                           (const float*)g.data_ptr(), o.top_k, dz.data_ptr()),
+      dz = at::empty(shape, z_.options());
+      check(abi.route_grad(stream_of(z_), code_of(z_), rows.at, rows.pitch, rows.n, rows.width, (int)o.sigmoid, o.top_k,
+                           (int)o.renorm, (float)o.scale, (const int64_t*)at_.data_ptr(), (const float*)g.data_ptr(),
+                           o.top_k, dz.data_ptr()),
             "odp_route_grad");
     }
     return {odp_host::first_only(grads, dz, true, kRoutes)};

@@ -39,6 +39,21 @@ inline at::Tensor pitched(const at::Tensor& t) {
   return r;
 }
 
+// The same as the kernels take them; a contiguous tensor of any dimensions as it
+// is, without the 1.5 us of a view.
+struct Rows {
+  at::Tensor held;
+  const void* at = nullptr;
+  int64_t n = 0, width = 0, pitch = 0;
+  Rows() = default;
+  explicit Rows(const at::Tensor& t) : width(t.size(-1)) {
+    held = t.is_contiguous() ? t : pitched(t);
+    n = t.numel() / width;
+    pitch = t.is_contiguous() ? width : held.stride(0);
+    at = held.data_ptr();
+  }
+};
+
 // A tangent on an input would be dropped without a word: the kernels read values.
 inline void no_tangent(const at::Tensor& t, const char* who) {
   TORCH_CHECK(!t._fw_grad(0).defined(), who, " have no forward-mode derivative");
