@@ -34,6 +34,8 @@ HIPCC_FLAGS = [
     "-packed-fp32-ops",
     "-Wall",
     "-Wno-unused-function",
+    # The sources one beside the other: 40 s instead of 5 minutes.
+    f"-parallel-jobs={min(8, os.cpu_count() or 1)}",
 ]
 
 

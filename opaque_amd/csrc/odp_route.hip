@@ -18,10 +18,13 @@
 // choice is the largest word below the last: the largest of (word - last) in
 // wrapping arithmetic, with nothing to mark.  The leading bits decide as the
 // keys in 64 bits would unless two that the choice hangs on lie within the
-// error of their float32 computation (`units_apart`); of such a token the
-// candidates' float64 keys are formed and ranked (`rank_exactly`), which a wave
-// takes in 2-3 us.  Keys are the logits themselves where those order as the scores
-// do (no bias, and no sums over groups); those of 16-bit types always decide.
+// error of their float32 computation (`units_apart`); of such a token (one in
+// some hundreds) the candidates' float64 keys are formed and ranked.  Keys are the
+// logits themselves where those order as the scores do (no bias, and no sums over
+// groups); those of 16-bit types always decide.
+//
+// 32768 tokens, 8 choices: of 64 experts 6 us, 256 15 us (33 MB of float32; a copy
+// of it takes 7), 256 with sigmoid scores and a bias 18, of 4 of 8 groups 23.
 #include <cmath>
 
 #include "odp_internal.h"
@@ -143,9 +146,9 @@ __device__ __forceinline__ float logit(const char* row, int dt, int e) {
   return dt == ODP_DTYPE_BF16 ? odp_bf2f(h) : (float)__builtin_bit_cast(_Float16, h);
 }
 
-// Values first to first + V of a row of `experts` (-inf past it).
+// Values first to first + V of a row of `experts` (`none` past it).
 template <int V>
-__device__ __forceinline__ void load_row(float (&z)[V], const char* row, int dt, int first, int experts) {
+__device__ __forceinline__ void load_row(float (&z)[V], const char* row, int dt, int first, int experts, float none) {
   if (first + V <= experts) {
     if (dt == ODP_DTYPE_F32) {
       const ODP_GMEM u32x4_w* p = (const ODP_GMEM u32x4_w*)(const ODP_GMEM void*)(row + 4 * first);
@@ -175,7 +178,7 @@ __device__ __forceinline__ void load_row(float (&z)[V], const char* row, int dt,
     return;
   }
 #pragma unroll
-  for (int i = 0; i < V; ++i) z[i] = first + i < experts ? logit(row, dt, first + i) : -INFINITY;
+  for (int i = 0; i < V; ++i) z[i] = first + i < experts ? logit(row, dt, first + i) : none;
 }
 
 // sigmoid without a loss of bits on either side.
@@ -200,81 +203,91 @@ struct Shares {
 };
 
 // A row's float64 keys, as ordered words: a masked expert (a logit of -inf)
-// below all others, a NaN key below those.
+// below all others, a NaN key below those.  What follows is for few tokens: its
+// loops hold one value at a time, so that the registers go to the others.
 struct Keys64 {
   const RouteArgs& a;
   const char* row;
   const float* bias;
-  bool sums;  // the keys are more than the logits
-  double top = 0.0, total = 1.0;
+  bool sums;   // the keys are more than the logits
+  double top;  // the largest logit
+  double total = 1.0;
   template <int L>
   __device__ __forceinline__ void normalise(int t) {
     if (!sums || a.sigmoid) return;
-    top = -INFINITY;
     total = 0.0;
-#pragma unroll 4
-    for (int e = t; e < a.experts; e += L) top = fmax(top, (double)logit(row, a.dt, e));
-    top = fmax_of<L>(top);
-#pragma unroll 4
+    float next = t < a.experts ? logit(row, a.dt, t) : 0.0f;
+#pragma unroll 1
     for (int e = t; e < a.experts; e += L) {
-      const double z = logit(row, a.dt, e);
+      const double z = next;
+      if (e + L < a.experts) next = logit(row, a.dt, e + L);
       total += z == -INFINITY ? 0.0 : exp(z - top);
     }
     total = sum_of<L>(total);
   }
-  __device__ __forceinline__ uint64_t operator()(int e) const {
-    const double z = logit(row, a.dt, e);
+  __device__ __forceinline__ uint64_t operator()(float logit_, float bias_) const {
+    const double z = logit_;
     double k = z + 0.0;  // the logits order as the scores do (-0 as 0)
-    if (sums) {
-      k = a.sigmoid ? 1.0 / (1.0 + exp(-z)) : exp(z - top) / total;
-      k += bias != nullptr ? (double)bias[e] : 0.0;
-    }
+    if (sums) k = (a.sigmoid ? 1.0 / (1.0 + exp(-z)) : exp(z - top) / total) + (double)bias_;
     return ordered(z == -INFINITY ? -INFINITY : k);
+  }
+  __device__ __forceinline__ float bias_of(int e) const { return bias != nullptr ? bias[e] : 0.0f; }
+  // The keys of list[j] (null: j) for j < count, by L threads.
+  template <int L>
+  __device__ __forceinline__ void fill(uint64_t* key, const int* list, int count, int t) const {
+    int e = t < count ? (list != nullptr ? list[t] : t) : 0;
+    float z = logit(row, a.dt, e), b = bias_of(e);
+#pragma unroll 1
+    for (int j = t; j < count; j += L) {
+      const float z0 = z, b0 = b;
+      if (j + L < count) {
+        e = list != nullptr ? list[j + L] : j + L;
+        z = logit(row, a.dt, e);
+        b = bias_of(e);
+      }
+      key[j] = (*this)(z0, b0);
+    }
+    wave_sync();
   }
 };
 
-// All of them, in a token's words of LDS, and a mask of the open groups from
-// them.  Group g is thread g % L's; masked experts add nothing to its score.
+// LDS of a wave, in 64-bit words: the words (32 bits) of all its tokens or the
+// float64 keys of one of them, and 64 more (a token's groups' scores, or its
+// choices by rank).
+template <int L, int V>
+constexpr int route_words() { return (L > 32 ? L : 32) * V + 64; }
+
+// All keys of a token in LDS, and a mask of the open groups from them.  Masked
+// experts add nothing to a group's score.
 template <int L, int V>
 __device__ __forceinline__ uint64_t open_exactly(const RouteArgs& a, Keys64& of, int t, uint64_t* key) {
   of.normalise<L>(t);
-#pragma unroll 2
-  for (int e = t; e < a.experts; e += L) key[e] = of(e);
-  wave_sync();
+  of.fill<L>(key, nullptr, a.experts, t);
   if (a.groups == 1) return ~0ull;
-  constexpr int PER = ((L * V < RT_GROUPS ? L * V : RT_GROUPS) + L - 1) / L;
-  const uint64_t least = ordered(-(double)INFINITY);
+  uint64_t* scores = key + route_words<L, V>() - 64;
   const auto value = [](uint64_t w) {
     return __longlong_as_double((long long)((int64_t)w < 0 ? w & 0x7fffffffffffffffull : ~w));
   };
-  uint64_t mine[PER], open = 0;
-  int above[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int g = t + i * L;
-    mine[i] = 0;
-    above[i] = 0;
-    if (g >= a.groups) continue;
+#pragma unroll 1
+  for (int g = t; g < a.groups; g += L) {
     uint64_t one = 0, two = 0;
-#pragma unroll 4
+#pragma unroll 2
     for (int k = 0; k < a.size; ++k) {
       const uint64_t w = key[g * a.size + k];
       two = max(two, min(one, w));
       one = max(one, w);
     }
-    mine[i] = a.best == 0 && one > 1 && two > least ? ordered(value(one) + value(two)) : one;
+    scores[g] = a.best == 0 && one > 1 && two > ordered(-(double)INFINITY) ? ordered(value(one) + value(two)) : one;
   }
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    for (int l = 0; l < L && i * L + l < a.groups; ++l) {
-      const uint64_t w = (uint64_t)__shfl((long long)mine[i], l, L);
-#pragma unroll
-      for (int k = 0; k < PER; ++k) above[k] += w > mine[k] || (w == mine[k] && i * L + l < t + k * L);
-    }
+  wave_sync();
+  uint64_t open = 0;
+#pragma unroll 1
+  for (int g = t; g < a.groups; g += L) {
+    int above = 0;
+#pragma unroll 2
+    for (int o = 0; o < a.groups; ++o) above += scores[o] > scores[g] || (scores[o] == scores[g] && o < g);
+    if (above < a.top_groups) open |= 1ull << g;
   }
-#pragma unroll
-  for (int i = 0; i < PER; ++i)
-    if (t + i * L < a.groups && above[i] < a.top_groups) open |= 1ull << (t + i * L);
   const uint32_t lo = or_of<L>((uint32_t)open), hi = or_of<L>((uint32_t)(open >> 32));
   return (uint64_t)hi << 32 | lo;
 }
@@ -285,14 +298,16 @@ __device__ __forceinline__ void route_exactly(const RouteArgs& a, Keys64& of, in
   const uint64_t open = open_exactly<L, V>(a, of, t, key);
   wave_sync();
   if (a.groups > 1) {
+#pragma unroll 1
     for (int e = t; e < a.experts; e += L)
       if (!(open >> (e / a.size) & 1)) key[e] = 0;
     wave_sync();
   }
+#pragma unroll 1
   for (int j = 0; j < a.top_k; ++j) {
     uint64_t most = 0;
     int at = t;
-#pragma unroll 4
+#pragma unroll 2
     for (int e = t; e < a.experts; e += L) {
       const uint64_t w = key[e];
       if (w > most) most = w, at = e;
@@ -309,65 +324,92 @@ __device__ __forceinline__ void route_exactly(const RouteArgs& a, Keys64& of, in
 }
 
 // The best top_k of `count` candidates, in the order of their float64 keys.
-template <int L, int PER>
+template <int L, int V>
 __device__ __forceinline__ void rank_exactly(const RouteArgs& a, Keys64& of, int t, int count, uint64_t* key,
                                              int* picked) {
+  int* ranked = (int*)(key + route_words<L, V>() - 64);
   of.normalise<L>(t);
-  int e[PER], above[PER];
-  uint64_t mine[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int j = t + i * L;
-    if (j >= count) break;
-    e[i] = picked[j];
-    mine[i] = of(e[i]);
-    key[j] = mine[i];
+  of.fill<L>(key, picked, count, t);
+#pragma unroll 1
+  for (int j = t; j < count; j += L) {
+    const uint64_t mine = key[j];
+    const int e = picked[j];
+    int above = 0;
+#pragma unroll 2
+    for (int i = 0; i < count; ++i) above += key[i] > mine || (key[i] == mine && picked[i] < e);
+    if (above < a.top_k) ranked[above] = e;
   }
   wave_sync();
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    if (t + i * L >= count) break;
-    above[i] = 0;
-#pragma unroll 4
-    for (int j = 0; j < count; ++j) above[i] += key[j] > mine[i] || (key[j] == mine[i] && picked[j] < e[i]);
+#pragma unroll 1
+  for (int j = t; j < a.top_k; j += L) picked[j] = ranked[j];
+  wave_sync();
+}
+
+// A token whose words do not decide, from the words of its choices and the one
+// below them: the candidates are the choices and, where `on`, all that lie within
+// `tol` of each other from the last choice on.
+template <int L, int V, int PICKS, typename F>
+__device__ __forceinline__ void choose_exactly(const RouteArgs& a, Keys64& of, const F& below, int t, uint32_t tol,
+                                               bool weird, bool on, uint64_t* key, uint32_t* chain) {
+  const uint32_t mask = (1u << a.bits) - 1;
+  int count = a.top_k;
+  bool full = weird;
+  if (on && !full) {
+    uint32_t last = chain[count];
+    for (++count;; ++count) {
+      const uint32_t m = below(last);
+      if (m == 0 || (last >> a.bits) - (m >> a.bits) > tol) break;
+      if (count == PICKS) {
+        full = true;
+        break;
+      }
+      if (t == 0) chain[count] = m;
+      last = m;
+    }
+    full |= count > PICKS;
   }
   wave_sync();
-#pragma unroll
-  for (int i = 0; i < PER; ++i)
-    if (t + i * L < count && above[i] < a.top_k) picked[above[i]] = e[i];
-  wave_sync();
+  if (!full) {
+    for (int j = t; j < count; j += L) chain[j] = mask - (chain[j] & mask);
+    wave_sync();
+    rank_exactly<L, V>(a, of, t, count, key, (int*)chain);
+  } else {
+    route_exactly<L, V>(a, of, t, key, (int*)chain);
+  }
 }
 
 // How far apart the leading parts of two words may lie with their keys the
 // wrong way round, in units of 2^-24 of the keys' range R (a score's 1 and the
-// bias's; a sigmoid's share is within 4 steps of 2^-24: its exponential 4 s (1 -
-// s), its sum 1, its reciprocal 2; a softmax's score s within 33 s: its
-// exponential 4, the sum of up to 1024 of them 22 + 4, the reciprocal 2, the
-// product 1).  The bias over its least, the sum, the product by 2^24 / R and its
-// whole part are a unit each.  Twice all that, for two words.
+// bias's).  A sigmoid's score s is within 4: its exponential's argument and the
+// exponential itself are off by s (1 - s) (|z| + 2), at most 1, its sum by 1, its
+// reciprocal by 2.  A softmax's by 42 s and one more: s |z - top| and 2 s of the
+// exponential, 34 s of the sum of up to 1024 of them (22 additions, and the terms'
+// own), 2 s of its reciprocal, s of the product.  The bias over its least, its share
+// of the range, their sum and the whole part of it are a unit each.  Twice all
+// that, for two words.
 __device__ __forceinline__ uint32_t units_apart(bool sigmoid, float largest) {
-  return sigmoid ? 16 : 9 + (uint32_t)(66.0f * fminf(largest, 1.0f));
+  return sigmoid ? 16 : 10 + (uint32_t)(84.0f * fminf(largest, 1.0f));
 }
 
 template <int L, int V>
 __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
   constexpr int TOKENS = RT_THREADS / L;
-  // A token's words: keys of the groups' search (32 bits), or of route_exactly.
-  __shared__ uint64_t lds[TOKENS * L * V];
   constexpr int PICKS = L * V < ODP_ROUTE_CHOICES ? L * V : ODP_ROUTE_CHOICES;
-  __shared__ int picks[TOKENS * PICKS];
-  const int slot = threadIdx.x / L, t = threadIdx.x % L;
+  __shared__ uint64_t lds[RT_THREADS / 64][route_words<L, V>()];
+  __shared__ uint32_t chains[TOKENS * (PICKS + 1)];
+  const int slot = threadIdx.x / L, t = threadIdx.x % L, mine = slot % (64 / L);
   int64_t token = (int64_t)blockIdx.x * TOKENS + slot;
   const bool live = token < a.n;
   token = live ? token : a.n - 1;
   const char* row = a.z + token * a.ldz;
   const float* bias = a.bias;
   if (bias != nullptr && a.rows_per_bias > 0) bias += token / a.rows_per_bias * a.experts;
-  int* picked = picks + slot * PICKS;
+  uint32_t* chain = chains + slot * (PICKS + 1);
+  uint64_t* words = lds[threadIdx.x / 64];
   const int first = t * V;
 
   float z[V];
-  load_row<V>(z, row, a.dt, first, a.experts);
+  load_row<V>(z, row, a.dt, first, a.experts, -INFINITY);
   const uint32_t mask = (1u << a.bits) - 1;
   // Keys that are sums (of a score and its bias, or of a group's two) are held
   // as their share of their range, logits of float32 as theirs of the row's
@@ -376,82 +418,95 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
   const bool fits = !sums && a.dt != ODP_DTYPE_F32;
   const uint32_t steps = 1u << min(24, 32 - a.bits);
   float top = -INFINITY, low = INFINITY, total = 0.0f;
-  bool odd = false, weird = false;  // odd: a NaN or +inf; weird: a row for route_exactly
+  uint32_t size = 0;  // the largest magnitude, by its bits: NaN above infinity
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     top = fmaxf(top, z[i]);
     low = fminf(low, z[i]);
-    odd |= !(z[i] < INFINITY);
+    size = max(size, __float_as_uint(z[i]) & 0x7fffffffu);
   }
+  const bool odd0 = size > 0x7f800000u || top == INFINITY;
+  const bool bounded = low > -INFINITY;  // no expert of this thread masked, none missing
   top = fmax_of<L>(top);
   const bool whole = !a.sigmoid && (sums || !a.renorm);
   float p[V];
   if (whole) {
+    if (a.renorm) {  // for keys alone (units_apart)
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      p[i] = z[i] == -INFINITY ? 0.0f : exp_near(z[i] - top);
-      total += p[i];
+      for (int i = 0; i < V; ++i) {
+        p[i] = __builtin_amdgcn_exp2f((z[i] - top) * 1.44269502f);
+        total += p[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        p[i] = z[i] == -INFINITY ? 0.0f : exp_near(z[i] - top);
+        total += p[i];
+      }
     }
     total = sum_of<L>(total);
   }
   uint32_t key[V];  // 0: no expert, or closed; leading parts: 1 masked, 2 and more the others
   uint32_t tol = 0;
+  bool weird = false;  // a row for route_exactly
+  const uint32_t place = mask - (uint32_t)first;
   if (sums) {
-    float lo = INFINITY, hi = -INFINITY, b[V];
+    float lo = 0.0f, hi = 0.0f, b[V];
     if (bias != nullptr) {
-      load_row<V>(b, (const char*)bias, ODP_DTYPE_F32, first, a.experts);
+      load_row<V>(b, (const char*)bias, ODP_DTYPE_F32, first, a.experts, bias[0]);
+      lo = hi = b[0];
+      uint32_t most = 0;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        if (first + i < a.experts) {
-          lo = fminf(lo, b[i]);
-          hi = fmaxf(hi, b[i]);
-          weird |= b[i] != b[i];
-        }
+        lo = fminf(lo, b[i]);
+        hi = fmaxf(hi, b[i]);
+        most = max(most, __float_as_uint(b[i]) & 0x7fffffffu);
       }
+      weird = most >= 0x7f800000u;
       lo = -fmax_of<L>(-lo);
       hi = fmax_of<L>(hi);
     } else {
-      lo = hi = 0.0f;
 #pragma unroll
       for (int i = 0; i < V; ++i) b[i] = 0.0f;
     }
     const float range = 1.0f + (hi - lo);
-    weird |= !(range < 1e30f);  // infinities among them, too
-    const float by = (float)(steps - 16) / range;
+    weird |= !(range < 1e30f);
+    const float by = (float)(steps - 16) * __builtin_amdgcn_rcpf(range);
     const float over = a.sigmoid ? 0.0f : __builtin_amdgcn_rcpf(total);
     tol = (units_apart(a.sigmoid, over) >> (24 - min(24, 32 - a.bits))) + 1;  // the largest score is e^0 over the sum
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int e = first + i;
-      const float s = a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + exp_near(-z[i])) : p[i] * over;
-      const uint32_t q = 2 + (uint32_t)fminf(((b[i] - lo) + s) * by, (float)(steps - 8));
-      key[i] = e < a.experts ? (z[i] == -INFINITY ? 1u : q) << a.bits | (mask - (uint32_t)e) : 0;
-      weird |= a.groups > 1 && e < a.experts && z[i] == -INFINITY;
+      const float s = a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z[i] * -1.44269502f)) : p[i] * over;
+      key[i] = (uint32_t)fmaf(s, by, fmaf(b[i] - lo, by, 2.0f)) << a.bits | (place - i);
     }
   } else if (fits) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int e = first + i;
-      key[i] = e < a.experts ? (ordered(z[i] + 0.0f) & ~mask) | (mask - (uint32_t)e) : 0;
-    }
+    for (int i = 0; i < V; ++i) key[i] = (ordered(z[i] + 0.0f) & ~mask) | (place - i);
   } else {
     low = fmaxf(-fmax_of<L>(-low), top - 128.0f);
     const float by = (float)(steps - 16) * __builtin_amdgcn_rcpf(fmaxf(top - low, 1e-30f));
 #pragma unroll
+    for (int i = 0; i < V; ++i)
+      key[i] = (uint32_t)fmaf(fmaxf(z[i] - low, 0.0f), by, 2.0f) << a.bits | (place - i);
+  }
+  if (__builtin_amdgcn_ballot_w64(!bounded) != 0) {
+#pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int e = first + i;
-      const uint32_t q = 2 + (uint32_t)fminf(fmaxf(z[i] - low, 0.0f) * by, (float)(steps - 8));
-      key[i] = e < a.experts ? (z[i] == -INFINITY ? 1u : q) << a.bits | (mask - (uint32_t)e) : 0;
+      if (first + i >= a.experts) {
+        key[i] = 0;
+      } else if (!fits && z[i] == -INFINITY) {
+        key[i] = 1u << a.bits | (place - i);
+        weird |= sums && a.groups > 1;
+      }
     }
   }
-  const uint32_t both = or_of<L>((odd ? 1u : 0u) | (weird ? 2u : 0u));
-  odd = (both & 1) != 0;
+  const uint32_t both = or_of<L>((odd0 ? 1u : 0u) | (weird ? 2u : 0u));
+  const bool odd = (both & 1) != 0;  // a NaN or +inf
   weird = both != 0;
-  uint64_t* words = lds + slot * L * V;
-  Keys64 exact{a, row, bias, sums};
+  Keys64 exact{a, row, bias, sums, top};
 
   if (a.groups > 1) {
-    uint32_t* scores = (uint32_t*)picked;  // [groups], before the choices
+    uint32_t* scores = chain;  // [groups], before the choices
     const auto second = [](uint32_t& one, uint32_t& two, uint32_t o1, uint32_t o2) {  // the two largest of four
       two = max(min(one, o1), max(two, o2));
       one = max(one, o1);
@@ -477,7 +532,7 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
       const int g = t / span;
       if (t == g * span && g < a.groups) scores[g] = score(one, two, g);
     } else {
-      uint32_t* all = (uint32_t*)words;
+      uint32_t* all = (uint32_t*)words + mine * L * V;
 #pragma unroll
       for (int i = 0; i < V; ++i)
         if (first + i < a.experts) all[first + i] = key[i];
@@ -499,13 +554,13 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
     uint64_t open = 0;
     uint32_t last = 0, next = 0;
     for (int g = t; g < a.groups; g += L) {
-      const uint32_t mine = scores[g];
+      const uint32_t own = scores[g];
       int above = 0;
 #pragma unroll 4
-      for (int o = 0; o < a.groups; ++o) above += scores[o] > mine;
+      for (int o = 0; o < a.groups; ++o) above += scores[o] > own;
       if (above < a.top_groups) open |= 1ull << g;
-      if (above == a.top_groups - 1) last = mine;
-      if (above == a.top_groups) next = mine;
+      if (above == a.top_groups - 1) last = own;
+      if (above == a.top_groups) next = own;
     }
     last = max_of<L>(last);
     next = max_of<L>(next);
@@ -513,9 +568,15 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
     open = (uint64_t)hi << 32 | lo;
     const int shift = a.best == 0 ? 6 : a.bits;
     const uint32_t apart = (last >> shift) - (next >> shift);
+    const bool unsure = !fits && !weird && apart <= (a.best == 0 ? 2 * tol : tol);
     wave_sync();
-    if (!fits && !weird && apart <= (a.best == 0 ? 2 * tol : tol)) open = open_exactly<L, V>(a, exact, t, words);
-    wave_sync();
+    if (__builtin_amdgcn_ballot_w64(unsure) != 0) {
+#pragma unroll 1
+      for (int k = 0; k < 64 / L; ++k) {
+        if (unsure && mine == k) open = open_exactly<L, V>(a, exact, t, words);
+        wave_sync();
+      }
+    }
     if (span > 0) {
       if (!(open >> ((t / span) & 63) & 1)) {
 #pragma unroll
@@ -530,45 +591,47 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
     }
   }
 
-  // The choices, best first, and beyond them all that lie within `tol` of each
-  // other from the last one on: the exact choice is among these candidates.
-  uint32_t last = 0;
-  int count = 0;
-  bool unsure = false, more = true, full = false;
-  for (int j = 0;; ++j) {
+  // The largest word below `last` (0: any), 0 where there is none: the largest
+  // difference then belongs to one above it, or to itself.
+  const auto below = [&](uint32_t last) {
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < V; ++i) m = max(m, key[i] - last);
     m = max_of<L>(m) + last;
-    // Nothing below the last one: the largest difference belongs to one above it (or to it).
-    const bool none = m == 0 || (j > 0 && m >= last);
-    bool near = false;
-    if (!fits && !none && j > 0 && (last >> a.bits) - (m >> a.bits) <= tol) {
-      near = true;
-      // Equal logits and biases are equal keys, which the words order already, and so are two masked ones.
-      const int e0 = (int)(mask - (last & mask)), e1 = (int)(mask - (m & mask));
-      const float z0 = logit(row, a.dt, e0), z1 = logit(row, a.dt, e1);
-      if (more) unsure |= z0 != z1 || (z0 != -INFINITY && bias != nullptr && bias[e0] != bias[e1]);
-    }
-    if (j >= a.top_k) {
-      more &= near;
-      full |= more && j >= PICKS;
-      more &= j < PICKS;
-      if (__builtin_amdgcn_ballot_w64(more) == 0) break;
-    }
-    if (more) {
-      if (t == 0) picked[j] = (int)(mask - (m & mask));
-      count = j + 1;
-    }
-    last = m;
+    return last != 0 && m >= last ? 0u : m;
+  };
+  uint32_t last = 0;
+  for (int j = 0; j <= a.top_k; ++j) {  // one more, for how near it lies
+    last = below(last);
+    if (t == 0) chain[j] = last;
   }
   wave_sync();
-  constexpr int PER = (PICKS + L - 1) / L;
-  if (weird || full) route_exactly<L, V>(a, exact, t, words, picked);
-  else if (unsure) rank_exactly<L, PER>(a, exact, t, count, words, picked);
-  wave_sync();
+  // The pairs that lie near each other: those of equal logits and biases are equal
+  // keys, which the words order already, and so are two masked experts.
+  bool near = false, last_near = false;
+  if (!fits) {
+    for (int j = t; j < a.top_k; j += L) {
+      const uint32_t w = chain[j], n = chain[j + 1];
+      if (n == 0 || (w >> a.bits) - (n >> a.bits) > tol || weird) continue;
+      const int e0 = (int)(mask - (w & mask)), e1 = (int)(mask - (n & mask));
+      const float z0 = logit(row, a.dt, e0), z1 = logit(row, a.dt, e1);
+      near |= z0 != z1 || (z0 != -INFINITY && bias != nullptr && bias[e0] != bias[e1]);
+      last_near |= j == a.top_k - 1;
+    }
+  }
+  const uint32_t flags = or_of<L>((near || weird ? 1u : 0u) | (last_near ? 2u : 0u));
+  // A choice that equals the next word is one of a run, which may end near others.
+  const bool on = (flags & 2) != 0, slow = weird || (!fits && flags != 0);
+  if (__builtin_amdgcn_ballot_w64(slow) != 0) {
+#pragma unroll 1
+    for (int k = 0; k < 64 / L; ++k) {
+      if (slow && mine == k) choose_exactly<L, V, PICKS>(a, exact, below, t, tol, weird, on, words, chain);
+      wave_sync();
+    }
+  }
 
   // The weights of the chosen, PER a thread.
+  constexpr int PER = (PICKS + L - 1) / L;
   const bool off = odd && !a.sigmoid;
   int e[PER];
   float x[PER], most = -INFINITY, sum = 0.0f;
@@ -576,7 +639,7 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
   for (int i = 0; i < PER; ++i) {
     const int j = t + i * L;
     if (j >= a.top_k) break;
-    e[i] = picked[j];
+    e[i] = slow ? (int)chain[j] : (int)(mask - (chain[j] & mask));
     x[i] = logit(row, a.dt, e[i]);
     most = fmaxf(most, x[i]);
   }
@@ -620,7 +683,7 @@ __global__ __launch_bounds__(RT_THREADS) void k_route_grad(const RouteArgs a) {
   float z[V], top = -INFINITY, total = 0.0f;
   bool odd = false;
   if (!a.sigmoid) {
-    load_row<V>(z, row, a.dt, first, a.experts);
+    load_row<V>(z, row, a.dt, first, a.experts, -INFINITY);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       top = fmaxf(top, z[i]);
