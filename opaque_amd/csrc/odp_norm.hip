@@ -273,6 +273,7 @@ struct NormArgs {
   char *y, *h;
   float *rstd, *scales;
   int64_t ldx, ldr, ldg, n;  // pitches in bytes
+  int64_t row0;              // the launch's first row
   int64_t rows_per_gain;
   int width, dt, ht, gt, nt;
   float eps, offset;
@@ -291,7 +292,7 @@ __global__ __launch_bounds__(norm_threads<T>()) void k_rms_norm(const NormArgs a
   constexpr int ROWS = norm_threads<T>() / T;
   __shared__ float red[2][T > 64 ? T / 64 : 1];
   const int t = T < 256 ? (int)(threadIdx.x % T) : (int)threadIdx.x;
-  int64_t row = (int64_t)blockIdx.x * ROWS + (T < 256 ? (int)(threadIdx.x / T) : 0);
+  int64_t row = a.row0 + (int64_t)blockIdx.x * ROWS + (T < 256 ? (int)(threadIdx.x / T) : 0);
   const bool live = row < a.n;
   row = live ? row : a.n - 1;
   const int width = a.width;
@@ -575,13 +576,18 @@ int64_t strips_of(int64_t n, int64_t width, int64_t gains) {
 
 bool norm_type(int dt) { return dt == ODP_DTYPE_F32 || dt == ODP_DTYPE_BF16 || dt == ODP_DTYPE_F16; }
 
+constexpr int64_t NORM_THREADS = (int64_t)1 << 31;  // of a launch: its threads are counted in 32 bits
+
 template <bool XF, bool HF, int T, int NV>
-void launch_norm(hipStream_t s, const NormArgs& a, int q) {
-  constexpr int TH = norm_threads<T>();
-  const uint32_t blocks = (uint32_t)((a.n + TH / T - 1) / (TH / T));
-  if (q == NQ_NONE) k_rms_norm<XF, HF, T, NV, NQ_NONE><<<blocks, TH, 0, s>>>(a);
-  else if (q == NQ_ROW) k_rms_norm<XF, HF, T, NV, NQ_ROW><<<blocks, TH, 0, s>>>(a);
-  else k_rms_norm<XF, HF, T, NV, NQ_BLOCK><<<blocks, TH, 0, s>>>(a);
+void launch_norm(hipStream_t s, NormArgs a, int q) {
+  constexpr int TH = norm_threads<T>(), ROWS = TH / T;
+  for (a.row0 = 0; a.row0 < a.n; a.row0 += NORM_THREADS / TH * ROWS) {
+    const int64_t left = (a.n - a.row0 + ROWS - 1) / ROWS;
+    const uint32_t blocks = (uint32_t)(left < NORM_THREADS / TH ? left : NORM_THREADS / TH);
+    if (q == NQ_NONE) k_rms_norm<XF, HF, T, NV, NQ_NONE><<<blocks, TH, 0, s>>>(a);
+    else if (q == NQ_ROW) k_rms_norm<XF, HF, T, NV, NQ_ROW><<<blocks, TH, 0, s>>>(a);
+    else k_rms_norm<XF, HF, T, NV, NQ_BLOCK><<<blocks, TH, 0, s>>>(a);
+  }
 }
 template <bool XF, bool HF, int T, int NV>
 void launch_grad(hipStream_t s, const NormGradArgs& a, int64_t blocks) {
@@ -737,16 +743,16 @@ extern "C" int odp_rms_norm_grad(odp_stream_t stream, int dtype, int stream_dtyp
   a.nt = n * width * (odp_dtype_size(dtype) + odp_dtype_size(stream_dtype) * (gh != nullptr ? 2 : 1)) > NORM_ONCE;
   hipStream_t s = odp_hip_stream(stream);
   const int64_t blocks = gains * strips;  // at most n
+  if (blocks * (width > 8192 ? 1024 : 256) > NORM_THREADS) {
+    odp_set_error("%s: %lld gains are more than one launch takes", what, (long long)gains);
+    return ODP_ERR_UNSUPPORTED;
+  }
   if (dtype == ODP_DTYPE_F32) grad_form<true, true>(s, a, blocks);
   else if (stream_dtype == ODP_DTYPE_F32) grad_form<false, true>(s, a, blocks);
   else grad_form<false, false>(s, a, blocks);
   if (a.part != nullptr) {
     const int cols = gains * ((width + 63) / 64) < 64 ? 16 : 64;
-    const int64_t tiles = (width + cols - 1) / cols;
-    if (gains * tiles >= (int64_t)1 << 31) {
-      odp_set_error("%s: too many gains", what);
-      return ODP_ERR_UNSUPPORTED;
-    }
+    const int64_t tiles = (width + cols - 1) / cols;  // of fewer than 512 gains
     const auto sum = cols == 16 ? k_gain_sum<16> : k_gain_sum<64>;
     sum<<<(uint32_t)(gains * tiles), GS_THREADS, 0, s>>>(a.part, strips, (int)width, (int)tiles, gain_dtype, dgain);
   }

@@ -131,6 +131,7 @@ struct RouteArgs {
   const int64_t* chosen;
   char* dz;
   int64_t ldz, n;         // pitch in bytes
+  int64_t token0;         // the launch's first token
   int64_t rows_per_bias;  // 0: one bias for all
   int64_t ldw;            // pitch of gw
   int experts, top_k, groups, top_groups, size;  // size: of a group
@@ -398,7 +399,7 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
   __shared__ uint64_t lds[RT_THREADS / 64][route_words<L, V>()];
   __shared__ uint32_t chains[TOKENS * (PICKS + 1)];
   const int slot = threadIdx.x / L, t = threadIdx.x % L, mine = slot % (64 / L);
-  int64_t token = (int64_t)blockIdx.x * TOKENS + slot;
+  int64_t token = a.token0 + (int64_t)blockIdx.x * TOKENS + slot;
   const bool live = token < a.n;
   token = live ? token : a.n - 1;
   const char* row = a.z + token * a.ldz;
@@ -669,7 +670,7 @@ __global__ __launch_bounds__(RT_THREADS) void k_route_grad(const RouteArgs a) {
   constexpr int TOKENS = RT_THREADS / L;
   __shared__ float lds[TOKENS * L * V];
   const int slot = threadIdx.x / L, t = threadIdx.x % L;
-  int64_t token = (int64_t)blockIdx.x * TOKENS + slot;
+  int64_t token = a.token0 + (int64_t)blockIdx.x * TOKENS + slot;
   const bool live = token < a.n;
   token = live ? token : a.n - 1;
   const char* row = a.z + token * a.ldz;
@@ -798,9 +799,14 @@ void launch_route(hipStream_t s, RouteArgs a, bool grad) {
   constexpr int TOKENS = RT_THREADS / L;
   const int span = a.size / V;
   a.span = a.size % V == 0 && (span & (span - 1)) == 0 ? span : 0;
-  const uint32_t blocks = (uint32_t)((a.n + TOKENS - 1) / TOKENS);
-  if (grad) k_route_grad<L, V><<<blocks, RT_THREADS, 0, s>>>(a);
-  else k_route<L, V><<<blocks, RT_THREADS, 0, s>>>(a);
+  // A launch's threads are counted in 32 bits.
+  constexpr int64_t MOST = ((int64_t)1 << 31) / RT_THREADS;
+  for (a.token0 = 0; a.token0 < a.n; a.token0 += MOST * TOKENS) {
+    const int64_t left = (a.n - a.token0 + TOKENS - 1) / TOKENS;
+    const uint32_t blocks = (uint32_t)(left < MOST ? left : MOST);
+    if (grad) k_route_grad<L, V><<<blocks, RT_THREADS, 0, s>>>(a);
+    else k_route<L, V><<<blocks, RT_THREADS, 0, s>>>(a);
+  }
 }
 
 void route_form(hipStream_t s, const RouteArgs& a, bool grad) {

@@ -61,6 +61,7 @@ def test_norm_gradient_checks(lib):
     for kw in ({"ldh": 4}, {"ldy": 4}, {"gh": BAD, "ldgh": 4}, {"ldg": 4}):
         refused(grad(**kw), N.ERR_INVALID_ARGUMENT, "pitch")
     refused(grad(scr=None), N.ERR_INVALID_ARGUMENT, "scratch")
+    refused(grad(n=1 << 24, gains=1 << 24), N.ERR_UNSUPPORTED, "more than one launch")
     assert grad(n=0, gains=1, h=None, rs=None, gy=None) == N.ODP_OK
     assert grad(dx=None, dg=None) == N.ODP_OK
     scratch = lib.odp_rms_norm_grad_scratch

@@ -333,6 +333,43 @@ def test_quantized_is_the_norm(path):
         assert ((q.to(F32) * s - y).abs() <= y.abs() * 2.0**-4 * (1 + 1e-5) + s * 2.0**-10 * (1 + 1e-5)).all()
 
 
+def test_under_the_other_transforms(path):
+    """grad alone, and what there is no derivative for: jvp, grad of grad."""
+    x, res, w, gy, gh = make(4, 40, F32, F32, F32)
+
+    def loss(x, r, w):
+        y, h = rms_norm(x, w, residual=r)
+        return (y * gy).sum() + (h * gh).sum()
+
+    got = torch.func.grad(loss, argnums=(0, 1, 2))(x, res, w)
+    ts = [t.clone().requires_grad_() for t in (x, res, w)]
+    y, h = rms_norm(ts[0], ts[2], residual=ts[1])
+    for a, b in zip(got, torch.autograd.grad([y, h], ts, [gy, gh])):
+        assert torch.equal(a, b)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda w: torch.func.grad(loss, argnums=2)(x, res, w).square().sum())(w)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda a: rms_norm(a, w), (x,), (torch.ones_like(x),))
+    with pytest.raises(NotImplementedError):
+        torch.func.vmap(lambda a: rms_norm_quantized(a, w)[0])(x)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        rms_norm_quantized(x, ts[2])
+    with torch.no_grad():
+        assert rms_norm_quantized(x, ts[2])[0].shape == x.shape
+
+
+def test_the_same_tensor_twice(path):
+    """x as its own residual: its gradient is both parts."""
+    x, _, w, gy, _ = make(5, 72, F32, None, F32)
+    leaf = x.clone().requires_grad_()
+    y, h = rms_norm(leaf, w, residual=leaf)
+    (both,) = torch.autograd.grad([y, h], [leaf], [gy, gy])
+    ts = [x.clone().requires_grad_(), x.clone().requires_grad_()]
+    y, h = rms_norm(ts[0], w, residual=ts[1])
+    a, b = torch.autograd.grad([y, h], ts, [gy, gy])
+    assert torch.equal(both, a + b)
+
+
 def test_module():
     m = RMSNorm(200, eps=1e-5, device=DEV, dtype=BF16)
     x, res, _, _, _ = make(4, 200, BF16, BF16)
@@ -341,6 +378,25 @@ def test_module():
     assert torch.equal(y, rms_norm(x, m.weight, residual=res, eps=1e-5)[0]) and m.weight.requires_grad
     plus = RMSNorm(200, unit_offset=True, device=DEV, dtype=BF16)
     assert not plus.weight.any() and torch.equal(plus(x), rms_norm(x, torch.ones(200, dtype=BF16, device=DEV)))
+
+
+def test_offsets_past_32_bits():
+    """More than 2^32 bytes and 2^31 elements: the last rows have the bits that they have alone."""
+    n, width = (1 << 19) + 3, 4104
+    x = torch.zeros(n, width, dtype=BF16, device=DEV)
+    last, res, w, gy, _ = make(5, width, BF16, BF16, BF16)
+    x[-5:] = last
+    leaf, gain = last.clone().requires_grad_(), w.clone().requires_grad_()
+    want = rms_norm(leaf, gain)
+    grads = torch.autograd.grad(want, [leaf, gain], gy)
+    x.requires_grad_()
+    y = rms_norm(x, gain)
+    assert torch.equal(y[-5:], want) and not y[-9:-5].any()
+    g = torch.zeros_like(y)
+    g[-5:] = gy
+    dx, dw = torch.autograd.grad(y, [x, gain], g)
+    assert torch.equal(dx[-5:], grads[0]) and not dx[-9:-5].any()
+    assert ((dw.double() - grads[1].double()).abs() <= grads[1].double().abs() * 2.0**-7 + 1e-6).all()
 
 
 def test_on_another_stream():

@@ -349,6 +349,37 @@ def test_differences():
             assert abs(diff - dz.flatten()[i].double()) < 1e-6
 
 
+def test_under_the_other_transforms(path):
+    z = logits(5, 12)
+    gw = torch.randn(5, 3, generator=torch.Generator().manual_seed(1)).to(DEV)
+    loss = lambda z: (route(z, 3)[1] * gw).sum()
+    leaf = z.clone().requires_grad_()
+    (want,) = torch.autograd.grad(loss(leaf), [leaf])
+    assert torch.equal(torch.func.grad(loss)(z), want)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda a: torch.func.grad(loss)(a).square().sum())(z)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(loss, (z,), (torch.ones_like(z),))
+
+
+def test_offsets_past_32_bits():
+    """More than 2^32 bytes and 2^31 logits."""
+    n, e = (1 << 21) + 5, 1024
+    z = torch.zeros(n, e, dtype=BF16, device=DEV)
+    last = logits(5, e, BF16)
+    z[-5:] = last
+    index, w = route(z.requires_grad_(), 4)
+    want = route(last, 4)
+    assert torch.equal(index[-5:], want[0]) and torch.equal(w[-5:], want[1])
+    assert (index[:-5] == torch.arange(4, device=DEV)).all()
+    gw = torch.zeros_like(w)
+    gw[-5:] = torch.randn(5, 4, generator=torch.Generator().manual_seed(1)).to(DEV)
+    (dz,) = torch.autograd.grad(w, [z], gw)
+    leaf = last.clone().requires_grad_()
+    (dw,) = torch.autograd.grad(route(leaf, 4)[1], [leaf], gw[-5:])
+    assert torch.equal(dz[-5:], dw) and not dz[-9:-5].any()
+
+
 def test_router_module():
     torch.manual_seed(0)
     r = Router(48, 16, 3, scores="sigmoid", balance=True, groups=4, top_groups=2, scale=2.0, device=DEV, dtype=BF16)
