@@ -570,8 +570,8 @@ int norm_tile(int64_t width) {  // threads of a row
 int64_t strips_of(int64_t n, int64_t width, int64_t gains) {
   const int t = norm_tile(width), at = t < 256 ? 256 / t : 1;
   const int64_t rows = (n / gains + at - 1) / at, count = (NORM_GROUPS + gains - 1) / gains;
-  // A few rows one after the other (1 us each) cost less than the launch that adds strips up.
-  return rows <= 4 ? 1 : rows < count ? rows : count;
+  // A few rows one after the other (below 1 us each) cost no more than the launch that adds strips up.
+  return rows <= 8 ? 1 : rows < count ? rows : count;
 }
 
 bool norm_type(int dt) { return dt == ODP_DTYPE_F32 || dt == ODP_DTYPE_BF16 || dt == ODP_DTYPE_F16; }

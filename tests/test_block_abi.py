@@ -11,7 +11,7 @@ import torch
 from opaque_amd import _native as N
 from opaque_amd.experts import Router, route
 from opaque_amd.global_norm import clip_by_global_norm, global_norm
-from opaque_amd.normalization import RMSNorm, rms_norm, rms_norm_quantized
+from opaque_amd.normalization import RMSNorm, rms_norm, rms_norm_quantized, route_norms
 from opaque_amd.types import clipped
 
 F32, BF16, F16, F64 = N.DTYPE_F32, N.DTYPE_BF16, N.DTYPE_F16, N.DTYPE_F64
@@ -206,3 +206,19 @@ def test_modules_on_the_host():
     assert r.weight.shape == (8, 12) and r.balance.dtype == torch.float32
     assert set(r.state_dict()) == {"weight", "balance"} and Router(12, 8, 2).balance is None
     Router(12, 8, 2, balance=True).load_state_dict({k: v.float() for k, v in r.state_dict().items()})
+
+
+def test_norms_are_replaced_on_their_own_gains():
+    class Other(torch.nn.Module):  # the layout of Hugging Face's
+        def __init__(self):
+            super().__init__()
+            self.weight, self.variance_epsilon = torch.nn.Parameter(torch.ones(6)), 1e-5
+
+    inner = torch.nn.Sequential(torch.nn.RMSNorm(6, eps=1e-4), torch.nn.Linear(6, 6), Other())
+    net = torch.nn.ModuleDict({"a": torch.nn.RMSNorm(6), "b": inner, "c": torch.nn.RMSNorm((2, 6)),
+                               "d": torch.nn.RMSNorm(6, elementwise_affine=False)})
+    kept = {k: v for k, v in net.named_parameters()}
+    assert route_norms(net, (torch.nn.RMSNorm, Other)) == ["a", "b.0", "b.2"]
+    assert {k: id(v) for k, v in net.named_parameters()} == {k: id(v) for k, v in kept.items()}
+    assert [net["a"].eps, net["b"][0].eps, net["b"][2].eps] == [torch.finfo(torch.float32).eps, 1e-4, 1e-5]
+    assert type(net["c"]) is type(net["d"]) is torch.nn.RMSNorm and type(net["b"][2]) is RMSNorm

@@ -152,3 +152,40 @@ def test_a_block_without_dp():
         assert abs(float(norm) / float(wnorm) - 1) < 1e-5
         for key_ in leaves:
             assert rel(out[key_], want[key_]) < 1e-5
+
+
+@pytest.mark.parametrize("dtype,tol", [(torch.float32, 1e-5), (torch.bfloat16, 2e-2)])
+def test_a_model_on_its_own_norms(dtype, tol):
+    """A Hugging Face Llama whose norm gains train under clipped_grad, with its norms replaced and without."""
+    transformers = pytest.importorskip("transformers")
+    from opaque_amd.normalization import RMSNorm, route_norms
+
+    torch.manual_seed(0)
+    cfg = transformers.LlamaConfig(vocab_size=128, hidden_size=64, intermediate_size=96, num_hidden_layers=2,
+                                   num_attention_heads=4, num_key_value_heads=2, max_position_embeddings=128,
+                                   attn_implementation="eager")
+    m = transformers.LlamaForCausalLM(cfg).eval().to(dtype).to(DEV)
+    for p in m.parameters():
+        p.requires_grad_(False)
+    gains = {k: p.requires_grad_() for k, p in m.named_parameters() if "norm" in k}
+    assert len(gains) == 5
+    g = torch.Generator().manual_seed(1)
+    ids, labels = (torch.randint(0, 128, (6, 24), generator=g).to(DEV) for _ in range(2))
+
+    def loss_fn(params, ids, labels):
+        fixed = {k: v for k, v in m.named_parameters() if k not in params}
+        return torch.func.functional_call(m, {**fixed, **params}, (ids.unsqueeze(0),),
+                                          {"labels": labels.unsqueeze(0)}).loss
+
+    def step():
+        fn, st = auto_clipped_grad(loss_fn, R=1.0, normalize_by=6, batch_argnums=(1, 2), return_aux=True)
+        (grads, aux), _ = fn(gains, ids, labels, state=st)
+        return grads.pytree, aux
+
+    want, waux = step()
+    kind = type(m.model.norm)
+    assert len(route_norms(m, (kind,))) == 5 and type(m.model.norm) is RMSNorm
+    got, aux = step()
+    assert rel(aux.grad_norms, waux.grad_norms) < tol and rel(aux.loss_values, waux.loss_values) < tol
+    for k in gains:
+        assert rel(got[k], want[k]) < tol, k
