@@ -18,8 +18,8 @@
 // choice is the largest word below the last: the largest of (word - last) in
 // wrapping arithmetic, with nothing to mark.  The leading bits decide as the
 // keys in 64 bits would unless two that the choice hangs on lie within the
-// error of their float32 computation (`units_apart`); of such a token (one in
-// some hundreds) the candidates' float64 keys are formed and ranked.  Keys are the
+// error of their float32 computation (`units_apart`); of such a token (one in a
+// thousand of 256 experts) the candidates' float64 keys are formed and ranked.  Keys are the
 // logits themselves where those order as the scores do (no bias, and no sums over
 // groups); those of 16-bit types always decide.
 //
@@ -427,7 +427,7 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
     size = max(size, __float_as_uint(z[i]) & 0x7fffffffu);
   }
   const bool odd0 = size > 0x7f800000u || top == INFINITY;
-  const bool bounded = low > -INFINITY;  // no expert of this thread masked, none missing
+  bool bounded = low > -INFINITY;  // no expert of this thread masked, none missing
   top = fmax_of<L>(top);
   const bool whole = !a.sigmoid && (sums || !a.renorm);
   float p[V];
@@ -454,18 +454,23 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
   if (sums) {
     float lo = 0.0f, hi = 0.0f, b[V];
     if (bias != nullptr) {
-      load_row<V>(b, (const char*)bias, ODP_DTYPE_F32, first, a.experts, bias[0]);
-      lo = hi = b[0];
+      load_row<V>(b, (const char*)bias, ODP_DTYPE_F32, first, a.experts, -INFINITY);
+      lo = INFINITY;
+      hi = -INFINITY;
       uint32_t most = 0;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        lo = fminf(lo, b[i]);
+        const bool shut = b[i] == -INFINITY;  // a key of -inf, as a masked expert's
+        z[i] = shut ? -INFINITY : z[i];
+        bounded &= !shut;
+        lo = fminf(lo, shut ? INFINITY : b[i]);
         hi = fmaxf(hi, b[i]);
-        most = max(most, __float_as_uint(b[i]) & 0x7fffffffu);
+        most = max(most, shut ? 0u : __float_as_uint(b[i]) & 0x7fffffffu);
       }
       weird = most >= 0x7f800000u;
       lo = -fmax_of<L>(-lo);
       hi = fmax_of<L>(hi);
+      if (!(lo <= hi)) lo = hi = 0.0f;  // all shut
     } else {
 #pragma unroll
       for (int i = 0; i < V; ++i) b[i] = 0.0f;
@@ -497,7 +502,7 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
         key[i] = 0;
       } else if (!fits && z[i] == -INFINITY) {
         key[i] = 1u << a.bits | (place - i);
-        weird |= sums && a.groups > 1;
+        weird |= sums && a.groups > 1 && a.best == 0;  // it adds nothing to its group's sum
       }
     }
   }

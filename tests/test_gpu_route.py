@@ -216,6 +216,28 @@ def test_masked_experts(path, e, scores):
 
 
 @pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("e", [8, 60, 256, 700])
+def test_experts_shut_by_their_bias(scores, e):
+    """A bias of -inf orders as a masked expert does, but such a one that is chosen all the same keeps its weight."""
+    for shut in (slice(1, 2), slice(0, e // 2), slice(2, None), slice(None)):
+        b = 0.1 * logits(1, e, seed=2)[0]
+        b[shut] = -torch.inf
+        check(logits(300, e), min(e, 5), scores=scores, bias=b)
+        check(logits(300, e, BF16), min(e, 5), scores=scores, bias=b, renormalize=False)
+        for best in ("top2", "max"):
+            check(logits(300, e), 3, scores=scores, bias=b, groups=4, top_groups=2, group_best=best)
+    z = logits(50, e)
+    z[:, ::3] = -torch.inf
+    b[:] = 0.1
+    b[1::3] = -torch.inf
+    for kw in ({}, {"groups": 4, "top_groups": 2, "group_best": "max"}, {"groups": 4, "top_groups": 2}):
+        index, w = route(z, 4, scores=scores, bias=b, **kw)
+        assert torch.equal(index, choice(z, 4, scores, b, kw.get("groups", 1), kw.get("top_groups", 1),
+                                         kw.get("group_best", "top2")))
+        assert w.isfinite().all()
+
+
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
 def test_nan_and_infinity(path, scores):
     """The index stays a set of experts, the other rows keep their bits."""
     for e, k in ((8, 3), (64, 6), (256, 8)):
