@@ -356,18 +356,15 @@ __device__ __forceinline__ void choose_exactly(const RouteArgs& a, Keys64& of, c
   int count = a.top_k;
   bool full = weird;
   if (on && !full) {
-    uint32_t last = chain[count];
-    for (++count;; ++count) {
+    uint32_t last = chain[count++];  // the first word below the choices is a candidate
+    for (; count < PICKS; ++count) {
       const uint32_t m = below(last);
       if (m == 0 || (last >> a.bits) - (m >> a.bits) > tol) break;
-      if (count == PICKS) {
-        full = true;
-        break;
-      }
       if (t == 0) chain[count] = m;
       last = m;
     }
-    full |= count > PICKS;
+    // No room to see whether the run ends here.
+    full = count >= PICKS;
   }
   wave_sync();
   if (!full) {

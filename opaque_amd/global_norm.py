@@ -70,6 +70,8 @@ def _run(name: str, grads, max_norm: float | None):
         tensors, td = list(grads.values()), None
     else:
         leaves, td = tree_flatten(grads)
+        if any(isinstance(t, ClippedPytree) for t in leaves):
+            raise TypeError(f"{name} takes one tree of tensors: pass each clipped or noised pytree by itself")
         places = [i for i, t in enumerate(leaves) if isinstance(t, torch.Tensor)]
         tensors = [leaves[i] for i in places]
     if not tensors:

@@ -12,7 +12,7 @@ from opaque_amd import _native as N
 from opaque_amd.experts import Router, route
 from opaque_amd.global_norm import clip_by_global_norm, global_norm
 from opaque_amd.normalization import RMSNorm, rms_norm, rms_norm_quantized, route_norms
-from opaque_amd.types import clipped
+from opaque_amd.types import SecondMomentNoiseOutput, clipped, noised
 
 F32, BF16, F16, F64 = N.DTYPE_F32, N.DTYPE_BF16, N.DTYPE_F16, N.DTYPE_F64
 BAD = 64  # a non-null, aligned address; never read
@@ -194,6 +194,10 @@ def test_tree_refusals():
             clip_by_global_norm({}, bad)
     with pytest.raises(TypeError, match="add the noise"):
         clip_by_global_norm(clipped({}, max_norm=1.0), 1.0)
+    pair = SecondMomentNoiseOutput(*(noised({}, max_norm=1.0, noise_stddev=1.0) for _ in range(2)))
+    for call in (global_norm, lambda t: clip_by_global_norm(t, 1.0)):
+        with pytest.raises(TypeError, match="by itself"):
+            call(pair)
     got, norm = clip_by_global_norm({"a": None, "b": [3]}, 1.0)
     assert got == {"a": None, "b": [3]} and float(norm) == 0
 

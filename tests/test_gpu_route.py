@@ -151,6 +151,20 @@ def test_equal_keys_go_to_the_lower_expert():
                 assert index[0].tolist() == list(range(min(e // 2, 9)))
 
 
+@pytest.mark.parametrize("e", [8, 16, 40, 64, 65, 200, 256, 1024])
+def test_long_runs_of_equal_keys(e):
+    """Runs that end before, at and after the last choice and the last place for a candidate."""
+    most = min(e, 64)
+    for k in {1, most // 2, most - 1, most} - {0}:
+        for run in {1, k, k + 1, most - 1, most, most + 1, e - 1, e}:
+            z = logits(9, e)
+            z[:, : min(run, e)] = 9.0
+            z[4:] = z[4:].flip(1)
+            check(z, k)
+            check(z, k, scores="sigmoid", bias=torch.full((e,), 0.25, device=DEV))
+            check(z, k, bias=torch.zeros(e, device=DEV))
+
+
 @pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("e", [16, 256, 1024])
 def test_keys_closer_than_float32(scores, e):
@@ -160,6 +174,7 @@ def test_keys_closer_than_float32(scores, e):
         p = torch.softmax(z[r].double(), 0) if scores == "softmax" else torch.sigmoid(z[r].double())
         bias = (0.5 - p).to(F32)  # key = 0.5 but for the rounding of the bias
         check(z[r: r + 1], 8, scores=scores, bias=bias)
+        check(z[r: r + 1], min(e, 64), scores=scores, bias=bias)
         check(z[r: r + 1], 8, scores=scores, bias=bias, groups=8, top_groups=4)
         check(z[r: r + 1], 8, scores=scores, bias=bias, groups=8, top_groups=4, group_best="max")
     # Logits a step apart.
