@@ -312,9 +312,9 @@ extern "C" int odp_tree_norm(odp_stream_t stream, const int64_t* leaves, int64_t
     k_tree_squares<<<blocks, TN_THREADS, 0, s>>>(l, part + parts);
     parts += blocks;
   }
-  if (!clip) {
+  if (!clip || parts == 0) {
     l.chunks = l.count = 0;
-    k_tree_scale<<<1, TN_THREADS, 0, s>>>(l, part, (int)parts, 0.0, wide, norm);
+    k_tree_scale<<<1, TN_THREADS, 0, s>>>(l, part, (int)parts, 0.0, wide, norm);  // the norm alone
     return odp_check_launch(what);
   }
   bool told = false;

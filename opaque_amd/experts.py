@@ -193,7 +193,8 @@ class Router(Linear):
         self.register_buffer("balance", torch.zeros(experts, device=device) if balance else None)
 
     def forward(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-        return route(super().forward(x), self.top_k, bias=self.balance, **self.options)
+        bias = None if self.balance is None else self.balance.float()  # the module may have been cast as a whole
+        return route(super().forward(x), self.top_k, bias=bias, **self.options)
 
 
 __all__ = ["Router", "route"]

@@ -149,6 +149,12 @@ def test_empty_trees(path):
     assert clip_by_global_norm({}, 1.0)[0] == {} and float(global_norm([None, 3])) == 0
     got, norm = clip_by_global_norm({"a": torch.empty(0, device=DEV)}, 1.0)
     assert got["a"].shape == (0,) and float(norm) == 0 and norm.device.type == "cuda"
+    for count in (8, 128, 129, 300):
+        none = {f"k{i}": torch.empty(0, 3, device=DEV) for i in range(count)}
+        got, norm = clip_by_global_norm(none, 1.0)
+        assert float(norm) == 0 == float(global_norm(none)) and all(t.shape == (0, 3) for t in got.values())
+        none["k7"] = torch.full((5,), 2.0, device=DEV)
+        assert abs(float(clip_by_global_norm(none, 1.0)[1]) - 20**0.5) < 1e-6
 
 
 def test_noised_trees(path):

@@ -427,6 +427,8 @@ def test_router_module():
     assert torch.equal(index, want[0]) and torch.equal(w, want[1]) and r.balance.dtype == F32
     w.sum().backward()
     assert r.weight.grad.isfinite().all() and "balance" in r.state_dict()
+    r.float().to(BF16)  # casts the buffer too
+    assert torch.equal(r(x)[0], index)
     plain = Router(48, 16, 3, device=DEV)
     assert plain.balance is None and plain(x.float())[0].shape == (2, 5, 3)
 
