@@ -14,11 +14,16 @@
 // workgroup) through one wave to a workgroup of 1024 (32768 values).  A gain of
 // its own for every group of rows (an example's) costs no launch more.  The
 // gains' gradient is summed in registers along a strip of rows, then over the
-// strips: no atomics, so results do not depend on the order of execution.
+// strips: no atomics, so results do not depend on the order of execution, and a
+// row's not on its place in the batch.
+//
+// 16384 x 4096 bfloat16 with a residual: forward 95 us for 537 MB (5.6 TB/s),
+// gradients 89 + 4 us for as much (6.1); a copy runs at 5.1.
 //
 // Vectors of 16 bytes are loaded at any address (this target's global loads
-// need no more than the type's own alignment), so odd widths run as even ones
-// do, but for the last vector of a row.
+// need no more than the type's own alignment).  Rows of odd widths start at odd
+// addresses, where each vector spans two lines: 8192 x 8191 119 + 145 us.  Cutting
+// such rows at aligned addresses would have a row's sum depend on its place.
 #include <cmath>
 
 #include "odp_internal.h"
@@ -594,7 +599,8 @@ void launch_grad(hipStream_t s, const NormGradArgs& a, int64_t blocks) {
   k_rms_norm_grad<XF, HF, T, NV><<<(uint32_t)blocks, norm_threads<T>(), 0, s>>>(a);
 }
 
-// The narrowest form whose registers hold a row.
+// The narrowest form whose registers hold a row.  (The gradient of rows above
+// 16384 values spills: 2048 x 32768 bfloat16 417 us, 1.3 TB/s.)
 #define ODP_NORM_FORM(CALL)                                 \
   do {                                                      \
     const int64_t v = (a.width + 7) / 8;                    \

@@ -98,13 +98,6 @@ __device__ __forceinline__ double sum_of(double v) {
   for (int s = 1; s < L; s <<= 1) v += __shfl_xor(v, s);
   return v;
 }
-template <int L>
-__device__ __forceinline__ double fmax_of(double v) {
-#pragma unroll
-  for (int s = 1; s < L; s <<= 1) v = fmax(v, __shfl_xor(v, s));
-  return v;
-}
-
 // LDS written by some threads of a wave and read by others of it.
 __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
