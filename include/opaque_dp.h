@@ -752,7 +752,8 @@ int odp_rms_norm_grad(odp_stream_t stream, int dtype, int stream_dtype, int gain
 int odp_route(odp_stream_t stream, int dtype, const void* logits, int64_t ldz, int64_t n, int64_t experts, int sigmoid,
               const float* bias, int64_t biases, int64_t groups, int64_t top_groups, int best, int64_t top_k,
               int renormalize, float scale, int64_t* index, float* weights);
-/* dlogits [n][experts] from gw (of the weights; pitch ldw) and the index.     */
+/* dlogits [n][experts] from gw (of the weights; pitch ldw) and the index.  A
+ * softmax's NaN or +inf makes a row's chosen entries NaN, without renormalize all. */
 int odp_route_grad(odp_stream_t stream, int dtype, const void* logits, int64_t ldz, int64_t n, int64_t experts,
                    int sigmoid, int64_t top_k, int renormalize, float scale, const int64_t* index, const float* gw,
                    int64_t ldw, void* dlogits);

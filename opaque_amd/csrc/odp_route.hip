@@ -659,11 +659,88 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
   }
 }
 
-// dz of a token's L threads: the chosen entries through LDS.
+// Values c to c + 8 of a 16-bit row, or to c + 4 of a float32 one (fewer at its end).
+__device__ __forceinline__ void store_some(char* row, int dt, int c, int experts, const float* v) {
+  const int n = dt == ODP_DTYPE_F32 ? 4 : 8;
+  if (c + n > experts) {
+    for (int i = 0; c + i < experts; ++i) odp_store_from_float(row, c + i, dt, v[i]);
+    return;
+  }
+  u32x4_t w;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (dt == ODP_DTYPE_F32) w[j] = __float_as_uint(v[j]);
+    else if (dt == ODP_DTYPE_BF16) w[j] = odp_f2bf2(v[2 * j], v[2 * j + 1]);
+    else
+      w[j] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2 * j]) |
+             (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2 * j + 1]) << 16;
+  }
+  if (dt == ODP_DTYPE_F32) *(ODP_GMEM u32x4_w*)(ODP_GMEM void*)(row + 4 * c) = w;
+  else *(ODP_GMEM u32x4_h*)(ODP_GMEM void*)(row + 2 * c) = w;
+}
+
+// Whether one of a row's values is NaN or +inf, for this thread's pieces of N.
+template <int L, int V, int N>
+__device__ __forceinline__ bool odd_pieces(const RouteArgs& a, const char* row, int t) {
+  bool odd = false;
+  float z[V / N][N];
+#pragma unroll
+  for (int j = 0; j < V / N; ++j) load_row<N>(z[j], row, a.dt, N * (t + j * L), a.experts, -INFINITY);
+#pragma unroll
+  for (int i = 0; i < V; ++i) odd |= !(z[i / N][i % N] < INFINITY);
+  return odd;
+}
+
+// A token's dz out of its chosen entries d (0 elsewhere): its L threads hold
+// pieces of N values side by side, 16 bytes each.  For a softmax that is not
+// renormalised every logit has a part.
+template <int L, int V, int N>
+__device__ __forceinline__ void store_dz(const RouteArgs& a, const char* row, char* to, const float* d, int t,
+                                         bool live) {
+  if (a.sigmoid || a.renorm) {
+    if (!live) return;
+    for (int c = N * t; c < a.experts; c += N * L) store_some(to, a.dt, c, a.experts, d + c);
+    return;
+  }
+  float z[V / N][N], top = -INFINITY, total = 0.0f, with = 0.0f;
+  bool odd = false;
+#pragma unroll
+  for (int j = 0; j < V / N; ++j) load_row<N>(z[j], row, a.dt, N * (t + j * L), a.experts, -INFINITY);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    top = fmaxf(top, z[i / N][i % N]);
+    odd |= !(z[i / N][i % N] < INFINITY);
+  }
+  odd = or_of<L>(odd ? 1u : 0u) != 0;
+  top = fmax_of<L>(top);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float& p = z[i / N][i % N];
+    p = p == -INFINITY ? 0.0f : exp_near(p - top);
+    total += p;
+    with += p == 0.0f ? 0.0f : p * d[N * (t + i / N * L) + i % N];
+  }
+  total = sum_of<L>(total);
+  const float over = total > 0.0f ? 1.0f / total : 0.0f;
+  with = sum_of<L>(with) * over;
+  if (!live) return;
+#pragma unroll
+  for (int j = 0; j < V / N; ++j) {
+    const int c = N * (t + j * L);
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[j][i] = odd ? NAN : z[j][i] == 0.0f ? 0.0f : z[j][i] * over * (d[c + i] - with);
+    if (c < a.experts) store_some(to, a.dt, c, a.experts, z[j]);
+  }
+}
+
+// dz of a token's L threads: the chosen entries through LDS, from which the row
+// leaves.  Every store of a wave writes whole lines; with the 8 or 16 values of
+// a thread side by side 32768 x 256 of float32 took 16 us, so 9 (33 MB written;
+// 12 for a softmax, whose rows are read too, 15 without renormalize, before 33).
 template <int L, int V>
 __global__ __launch_bounds__(RT_THREADS) void k_route_grad(const RouteArgs a) {
   constexpr int TOKENS = RT_THREADS / L;
-  __shared__ float lds[TOKENS * L * V];
+  __shared__ __align__(16) float lds[TOKENS * L * V];
   const int slot = threadIdx.x / L, t = threadIdx.x % L;
   int64_t token = a.token0 + (int64_t)blockIdx.x * TOKENS + slot;
   const bool live = token < a.n;
@@ -672,33 +749,14 @@ __global__ __launch_bounds__(RT_THREADS) void k_route_grad(const RouteArgs a) {
   const int64_t* chosen = a.chosen + token * a.top_k;
   const float* gw = a.gw + token * a.ldw;
   float* d = lds + slot * L * V;
-  const int first = t * V;
-  const bool dense = !a.sigmoid && !a.renorm;  // every expert's score depends on every logit
 #pragma unroll
-  for (int i = 0; i < V; ++i) d[first + i] = 0.0f;
-  float z[V], top = -INFINITY, total = 0.0f;
-  bool odd = false;
-  if (!a.sigmoid) {
-    load_row<V>(z, row, a.dt, first, a.experts, -INFINITY);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      top = fmaxf(top, z[i]);
-      odd |= !(z[i] < INFINITY);
-    }
-    odd = or_of<L>(odd ? 1u : 0u) != 0;
-  }
-  if (dense) {
-    top = fmax_of<L>(top);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      z[i] = z[i] == -INFINITY ? 0.0f : exp_near(z[i] - top);
-      total += z[i];
-    }
-    total = sum_of<L>(total);
-  }
+  for (int i = 0; i < V; ++i) d[4 * (t + i / 4 * L) + i % 4] = 0.0f;
   constexpr int PICKS = L * V < ODP_ROUTE_CHOICES ? L * V : ODP_ROUTE_CHOICES, PER = (PICKS + L - 1) / L;
   int e[PER];
   float x[PER], g[PER], most = -INFINITY, sum = 0.0f, dot = 0.0f;
+  bool odd = false;  // a softmax with a NaN or +inf
+  if (a.renorm && !a.sigmoid)
+    odd = a.dt == ODP_DTYPE_F32 ? odd_pieces<L, V, 4>(a, row, t) : odd_pieces<L, V, 8>(a, row, t);
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int j = t + i * L;
@@ -714,6 +772,7 @@ __global__ __launch_bounds__(RT_THREADS) void k_route_grad(const RouteArgs a) {
   }
   if (a.renorm) {
     most = fmax_of<L>(most);
+    odd = or_of<L>(odd ? 1u : 0u) != 0;
     const Shares share(a, most, 0.0f);
     float s[PER];
 #pragma unroll
@@ -746,47 +805,8 @@ __global__ __launch_bounds__(RT_THREADS) void k_route_grad(const RouteArgs a) {
     d[e[i]] = odd ? NAN : g[i] * a.scale;
   }
   wave_sync();
-  float out[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) out[i] = d[first + i];
-  if (dense) {
-    const float over = total > 0.0f ? 1.0f / total : 0.0f;
-    float with = 0.0f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) with += z[i] == 0.0f ? 0.0f : z[i] * out[i];
-    with = sum_of<L>(with) * over;
-#pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = odd ? NAN : z[i] == 0.0f ? 0.0f : z[i] * over * (out[i] - with);
-  }
-  if (!live) return;
-  char* to = a.dz + token * a.experts * (a.dt == ODP_DTYPE_F32 ? 4 : 2);
-  if (first + V <= a.experts) {
-    if (a.dt == ODP_DTYPE_F32) {
-      ODP_GMEM u32x4_w* w = (ODP_GMEM u32x4_w*)(ODP_GMEM void*)(to + 4 * first);
-#pragma unroll
-      for (int i = 0; i < V / 4; ++i)
-        w[i] = u32x4_t{__float_as_uint(out[4 * i]), __float_as_uint(out[4 * i + 1]), __float_as_uint(out[4 * i + 2]),
-                       __float_as_uint(out[4 * i + 3])};
-    } else {
-      ODP_GMEM u32x4_h* w = (ODP_GMEM u32x4_h*)(ODP_GMEM void*)(to + 2 * first);
-#pragma unroll
-      for (int i = 0; i < V / 8; ++i) {
-        u32x4_t v;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float x = out[8 * i + 2 * j], y = out[8 * i + 2 * j + 1];
-          v[j] = a.dt == ODP_DTYPE_BF16 ? odp_f2bf2(x, y)
-                                        : (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)x) |
-                                              (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)y) << 16;
-        }
-        w[i] = v;
-      }
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < V; ++i)
-    if (first + i < a.experts) odp_store_from_float(to, first + i, a.dt, out[i]);
+  if (a.dt == ODP_DTYPE_F32) store_dz<L, V, 4>(a, row, a.dz + token * a.experts * 4, d, t, live);
+  else store_dz<L, V, 8>(a, row, a.dz + token * a.experts * 2, d, t, live);
 }
 
 template <int L, int V>

@@ -280,6 +280,30 @@ def test_nan_and_infinity(path, scores):
     assert (index[:, 0] == 5).all() and not ((index == 9) | (index == 11)).any() and w.isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, BF16, torch.float16])
+def test_gradient_of_nan_and_infinity(path, dtype):
+    """It reaches its own token's entries, of chosen experts alone with renormalize."""
+    for e, k in ((7, 3), (60, 6), (130, 8), (256, 8)):
+        for renormalize in (True, False):
+            z = logits(12, e, dtype)
+            z[2, 4], z[6, 1], z[9, 5] = float("nan"), float("inf"), float("nan")
+            shut = torch.zeros(e, device=DEV)
+            shut[5] = -float("inf")
+            leaf = z.clone().requires_grad_()
+            index, w = route(leaf, k, bias=shut, renormalize=renormalize)
+            (dz,) = torch.autograd.grad(w, [leaf], torch.ones_like(w))
+            rest = [i for i in range(12) if i not in (2, 6, 9)]
+            assert not (index[rest] == 5).any()  # a NaN's token has no order
+            assert dz[rest].isfinite().all()
+            if not renormalize:
+                assert dz[[2, 6, 9]].isnan().all()
+                continue
+            for i in (2, 6, 9):
+                hit = torch.zeros(e, dtype=torch.bool, device=DEV)
+                hit[index[i]] = True
+                assert dz[i][hit].isnan().all() and (dz[i][~hit] == 0).all()
+
+
 def test_shapes_and_strides(path):
     z = logits(24, 40, BF16)
     b = 0.1 * logits(1, 40, seed=2)[0]
