@@ -780,15 +780,19 @@ __global__ __launch_bounds__(RT_THREADS) void k_route_grad(const RouteArgs a) {
       if (t + i * L >= a.top_k) break;
       s[i] = share(x[i]);
       sum += s[i];
-      dot += s[i] == 0.0f ? 0.0f : s[i] * g[i];
     }
     sum = sum_of<L>(sum);
-    dot = sum_of<L>(dot);
-    dot = sum > 0.0f ? dot / sum : 0.0f;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       if (t + i * L >= a.top_k) break;
-      g[i] = s[i] == 0.0f ? 0.0f : s[i] / sum * (g[i] - dot);
+      s[i] = s[i] == 0.0f ? 0.0f : s[i] / sum;  // 1 where it is the only one, whose gradient is then 0
+      dot += s[i] == 0.0f ? 0.0f : s[i] * g[i];
+    }
+    dot = sum_of<L>(dot);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (t + i * L >= a.top_k) break;
+      g[i] = s[i] == 0.0f ? 0.0f : s[i] * (g[i] - dot);
       if (a.sigmoid) g[i] *= sigmoid(-x[i]);
     }
   } else if (a.sigmoid) {

@@ -280,6 +280,16 @@ def test_nan_and_infinity(path, scores):
     assert (index[:, 0] == 5).all() and not ((index == 9) | (index == 11)).any() and w.isfinite().all()
 
 
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_one_choice_renormalized(path, scores):
+    """Its weight is the scale whatever the logits are, its gradient 0 to the bit."""
+    for e, groups in ((5, 1), (40, 4), (130, 1), (512, 8)):
+        leaf = logits(300, e, seed=e).requires_grad_()
+        index, w = route(leaf, 1, scores=scores, groups=groups, top_groups=1, renormalize=True, scale=2.5)
+        (dz,) = torch.autograd.grad(w, [leaf], logits(300, 1, seed=1))
+        assert (w == 2.5).all() and (dz == 0).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, BF16, torch.float16])
 def test_gradient_of_nan_and_infinity(path, dtype):
     """It reaches its own token's entries, of chosen experts alone with renormalize."""
