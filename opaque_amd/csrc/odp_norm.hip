@@ -17,8 +17,8 @@
 // strips: no atomics, so results do not depend on the order of execution, and a
 // row's not on its place in the batch.
 //
-// 16384 x 4096 bfloat16 with a residual: forward 92 us for 537 MB (5.8 TB/s),
-// gradients 89 + 4 us for as much (6.1); a copy runs at 5.1.
+// 16384 x 4096 bfloat16 with a residual: forward 92-95 us for 537 MB (5.7 TB/s),
+// gradients 83-89 + 4 us for as much (6.1); a copy runs at 5.1.
 //
 // Vectors of 16 bytes are loaded at any address (this target's global loads
 // need no more than the type's own alignment).  Rows of odd widths start at odd
@@ -302,6 +302,19 @@ constexpr int NQ_COLS = 128;          // columns of a block
 constexpr float NQ_MOST = 448.0f;     // the largest e4m3 value
 constexpr float NQ_LEAST = 1.17549435e-38f;
 
+// y / s for a scale s, 0 for an infinite one: the product with 1 / s rounds
+// twice; what it leaves of y puts that right, two instructions a value that the
+// memory's time hides.  0.8 codes in a million differ from those of 64 bits then
+// (float32 rows of 4096), as many as by a true division.
+struct Quotient {
+  float by, s;
+  __device__ __forceinline__ explicit Quotient(float scale) : by(1.0f / scale), s(scale == INFINITY ? 0.0f : scale) {}
+  __device__ __forceinline__ float operator()(float y) const {
+    const float q = y * by;
+    return fmaf(fmaf(-q, s, y), by, q);
+  }
+};
+
 template <int T>
 constexpr int norm_threads() { return T < 256 ? 256 : T; }
 
@@ -319,7 +332,7 @@ __global__ __launch_bounds__(norm_threads<T>()) void k_rms_norm(const NormArgs a
   load_rows<T>(x, a.x + row * a.ldx, width, t, a.nt);
   if (a.r != nullptr) load_rows<T>(r, a.r + row * a.ldr, width, t, a.nt);
   // The gains' loads go out with the row's; after its sum they were a second
-  // wait (95 us for 92 at 16384 x 4096, 4.1 for 4.0 at one row).
+  // wait (4.1 us for 4.0 at one row of 4096, 95 for 92 at 16384 on one card).
   const char* gain = a.gain == nullptr ? nullptr : a.gain + (a.ldg ? row / a.rows_per_gain * a.ldg : 0);
   Gains gains[NV];
 #pragma unroll
@@ -368,20 +381,24 @@ __global__ __launch_bounds__(norm_threads<T>()) void k_rms_norm(const NormArgs a
         const float s = m > 0x7f800000u ? __uint_as_float(m) : scale;
         if (live && (t & 15) == 0 && c < width)
           odp_gstore(a.scales + row * ((width + NQ_COLS - 1) / NQ_COLS) + c / NQ_COLS, s);
-        const float by = 1.0f / s;
+        const Quotient over(s);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[v][i] *= by;
+        for (int i = 0; i < 8; ++i) f[v][i] = over(f[v][i]);
       }
     }
   }
   if constexpr (Q == NQ_NONE) return;
-  float by = 1.0f;
   if constexpr (Q == NQ_ROW) {
     most = max_row<T>(most, red[0], 1);
     const float scale = fmaxf(__uint_as_float(most) / NQ_MOST, NQ_LEAST);
     const float s = most > 0x7f800000u ? __uint_as_float(most) : scale;
     if (live && t == 0) odp_gstore(a.scales + row, s);
-    by = 1.0f / s;
+    const Quotient over(s);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[v][i] = over(f[v][i]);
+    }
   }
   if (!live) return;
   char* q = a.y + row * width;
@@ -392,8 +409,8 @@ __global__ __launch_bounds__(norm_threads<T>()) void k_rms_norm(const NormArgs a
     u32x2_t w;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      int p = __builtin_amdgcn_cvt_pk_fp8_f32(f[v][4 * i] * by, f[v][4 * i + 1] * by, 0, false);
-      p = __builtin_amdgcn_cvt_pk_fp8_f32(f[v][4 * i + 2] * by, f[v][4 * i + 3] * by, p, true);
+      int p = __builtin_amdgcn_cvt_pk_fp8_f32(f[v][4 * i], f[v][4 * i + 1], 0, false);
+      p = __builtin_amdgcn_cvt_pk_fp8_f32(f[v][4 * i + 2], f[v][4 * i + 3], p, true);
       w[i] = (uint32_t)p;
     }
     if (c + 8 <= width) {

@@ -318,6 +318,15 @@ def test_quantized_values_that_are_none(path):
     assert s[1].isnan() and q[1].to(F32).isnan().all() and s[3].isnan()
     for i in (0, 2, 4):
         assert torch.equal(q[i].view(torch.uint8), clean[0][i].view(torch.uint8)) and s[i] == clean[1][i]
+    big = torch.zeros(2, 300, device=DEV)
+    big[:, :3] = torch.tensor([4.0, -1.0, 1e-4], device=DEV)  # of a root mean square of 0.24
+    for block in (None, 128):
+        q, s = rms_norm_quantized(big, torch.full((300,), 1e38, device=DEV), block=block)
+        first = s if block is None else s[:, 0]
+        q = q.to(F32)
+        assert first.isinf().all() and q[:, 0].isnan().all() and (q[:, 2:128] == 0).all()
+        q, s = rms_norm_quantized(big, torch.full((300,), 2e37, device=DEV), block=block)  # the largest y: 3.36e38
+        assert s.isfinite().all() and (q.to(F32)[:, 0] == 448).all() and (q.to(F32)[:, 1] == -112).all()
     q, s = rms_norm_quantized(x[:0], w, block=128)
     assert q.shape == (0, 300) and s.shape == (0, 3)
 
