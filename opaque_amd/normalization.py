@@ -297,7 +297,7 @@ def route_norms(model: torch.nn.Module, types=(torch.nn.RMSNorm,)) -> list[str]:
             if type(child) not in tuple(types) or weight is None or weight.dim() != 1:
                 continue
             eps = getattr(child, "eps", None) if hasattr(child, "eps") else child.variance_epsilon
-            eps = torch.finfo(weight.dtype).eps if eps is None else float(eps)  # torch's default
+            eps = _F32.eps if eps is None else float(eps)  # torch's default, of the type that it computes in
             setattr(mod, child_name, RMSNorm.sharing(weight, eps))
             names.append(f"{name}.{child_name}" if name else child_name)
     return names

@@ -212,6 +212,18 @@ def test_modules_on_the_host():
     Router(12, 8, 2, balance=True).load_state_dict({k: v.float() for k, v in r.state_dict().items()})
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_the_default_eps_is_torchs(dtype):
+    """By what torch gives for rows whose mean square lies between the types' eps."""
+    net = torch.nn.Sequential(torch.nn.RMSNorm(64, dtype=dtype))
+    x = (1e-3 * torch.randn(8, 64, generator=torch.Generator().manual_seed(0))).to(dtype)
+    y = net(x).detach().double()
+    route_norms(net)
+    want = x.double() / torch.sqrt(x.double().square().mean(1, keepdim=True) + net[0].eps)
+    # Half a step of the type for each of x's norm and the gain's product, and float32's sum.
+    assert ((y - want).abs() <= (torch.finfo(dtype).eps + 80 * 2.0**-24) * want.abs()).all()
+
+
 def test_norms_are_replaced_on_their_own_gains():
     class Other(torch.nn.Module):  # the layout of Hugging Face's
         def __init__(self):
