@@ -184,6 +184,23 @@ def test_keys_closer_than_float32(scores, e):
     check(z, 8, scores=scores, groups=4, top_groups=2, group_best="max")
 
 
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("e", [16, 60, 256, 1024])
+def test_rows_of_little_spread(scores, e):
+    """Rows of one value among others (an empty token's), logits that hardly differ, biases that swallow them."""
+    z = logits(64, e)
+    z[::3] = 0.0
+    z[1::6] = 0.25
+    small = torch.cat([1e-3 * logits(40, e, seed=1), 1e-5 * logits(40, e, seed=2)])
+    drift = 1e-3 * logits(1, e, seed=3)[0]
+    for rows in (z, small):
+        for bias in (None, torch.zeros(e, device=DEV), torch.full((e,), -0.7, device=DEV), drift, drift + 4096.0,
+                     torch.full((e,), 2.0**26, device=DEV), torch.full((e,), 2.0**50, device=DEV)):
+            check(rows, 8, scores=scores, bias=bias)
+            check(rows, 6, scores=scores, bias=bias, groups=4, top_groups=2)
+            check(rows, 6, scores=scores, bias=bias, groups=4, top_groups=2, group_best="max")
+
+
 def test_large_and_small_logits():
     z = logits(200, 64, spread=30.0)
     z[:50] -= 200.0
