@@ -302,16 +302,25 @@ constexpr int NQ_COLS = 128;          // columns of a block
 constexpr float NQ_MOST = 448.0f;     // the largest e4m3 value
 constexpr float NQ_LEAST = 1.17549435e-38f;
 
-// y / s for a scale s, 0 for an infinite one: the product with 1 / s rounds
-// twice; what it leaves of y puts that right, two instructions a value that the
-// memory's time hides.  0.8 codes in a million differ from those of 64 bits then
-// (float32 rows of 4096), as many as by a true division.
-struct Quotient {
-  float by, s;
-  __device__ __forceinline__ explicit Quotient(float scale) : by(1.0f / scale), s(scale == INFINITY ? 0.0f : scale) {}
-  __device__ __forceinline__ float operator()(float y) const {
-    const float q = y * by;
-    return fmaf(fmaf(-q, s, y), by, q);
+// The scale of a row or block, and its codes' values y / scale.  With 1 / rms = c
+// 2^k, 1 <= c < 2, and t = 2^k h w (of 16-bit values the exact product) these are
+// 448 t / max |t|: what a first quotient q leaves of 448 t puts q right, so that a
+// border between two codes is met where it is (of 4096 bfloat16 one value in 5000
+// lies on one, and goes to the even code).  At the ends of float32's range, t c /
+// scale (0 for finite y over an infinite scale).
+struct Codes {
+  float scale, times, den, over;
+  __device__ __forceinline__ Codes(uint32_t most, float c) {  // most: max |t|, its bits
+    const float m = __uint_as_float(most), y = m * c;
+    scale = y != y ? y : fmaxf(y / NQ_MOST, NQ_LEAST);
+    const bool middle = m >= 0x1p-100f && m <= 0x1p100f && scale > NQ_LEAST;
+    times = middle ? NQ_MOST : c;
+    over = 1.0f / (middle ? m : scale);
+    den = middle ? m : scale == INFINITY ? 0.0f : scale;
+  }
+  __device__ __forceinline__ float operator()(float t) const {
+    const float x = t * times, q = x * over;
+    return fmaf(fmaf(-q, den, x), over, q);
   }
 };
 
@@ -357,6 +366,10 @@ __global__ __launch_bounds__(norm_threads<T>()) void k_rms_norm(const NormArgs a
   sum = sum_row<T>(sum, red[0], 0);
   const float inv = 1.0f / sqrtf(sum / (float)width + a.eps);
   if (a.rstd != nullptr && t == 0 && live) odp_gstore(a.rstd + row, inv);
+  // For codes by its power of two alone (Codes); a NaN stays with what is left.
+  const uint32_t bits = __float_as_uint(inv);
+  const float by = Q == NQ_NONE ? inv : __uint_as_float(bits & 0x7f800000u);
+  const float rest = inv != inv ? inv : __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
   uint32_t most = 0;
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
@@ -364,40 +377,34 @@ __global__ __launch_bounds__(norm_threads<T>()) void k_rms_norm(const NormArgs a
     float g[8];
     gains[v].get(g, gain, a.gt, a.offset);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[v][i] = f[v][i] * inv * g[i];
+    for (int i = 0; i < 8; ++i) f[v][i] = f[v][i] * by * g[i];
     if constexpr (Q == NQ_NONE) {
       Eight<XF> y;
       y.set(f[v], a.dt);
       if (live) y.store(a.y + row * width * (XF ? 4 : 2), c, width);
     } else {
-      uint32_t m = 0;  // by the bits of |y|, above which those of infinities and NaN lie
+      uint32_t m = 0;  // by the bits, above which those of infinities and NaN lie
 #pragma unroll
       for (int i = 0; i < 8; ++i) m = max(m, c + i < width ? __float_as_uint(f[v][i]) & 0x7fffffffu : 0u);
       if constexpr (Q == NQ_ROW) {
         most = max(most, m);
       } else {
-        m = max_lanes<(T < 16 ? T : 16)>(m);  // 16 threads of 8 values
-        const float scale = fmaxf(__uint_as_float(m) / NQ_MOST, NQ_LEAST);
-        const float s = m > 0x7f800000u ? __uint_as_float(m) : scale;
+        const Codes code(max_lanes<(T < 16 ? T : 16)>(m), rest);  // 16 threads of 8 values
         if (live && (t & 15) == 0 && c < width)
-          odp_gstore(a.scales + row * ((width + NQ_COLS - 1) / NQ_COLS) + c / NQ_COLS, s);
-        const Quotient over(s);
+          odp_gstore(a.scales + row * ((width + NQ_COLS - 1) / NQ_COLS) + c / NQ_COLS, code.scale);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[v][i] = over(f[v][i]);
+        for (int i = 0; i < 8; ++i) f[v][i] = code(f[v][i]);
       }
     }
   }
   if constexpr (Q == NQ_NONE) return;
   if constexpr (Q == NQ_ROW) {
-    most = max_row<T>(most, red[0], 1);
-    const float scale = fmaxf(__uint_as_float(most) / NQ_MOST, NQ_LEAST);
-    const float s = most > 0x7f800000u ? __uint_as_float(most) : scale;
-    if (live && t == 0) odp_gstore(a.scales + row, s);
-    const Quotient over(s);
+    const Codes code(max_row<T>(most, red[0], 1), rest);
+    if (live && t == 0) odp_gstore(a.scales + row, code.scale);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[v][i] = over(f[v][i]);
+      for (int i = 0; i < 8; ++i) f[v][i] = code(f[v][i]);
     }
   }
   if (!live) return;

@@ -310,6 +310,23 @@ def test_quantized(dtype, block, width):
     assert q.to(F32).abs().max() <= 448 and not q[2].to(F32).any() and (scales[2] == torch.finfo(F32).tiny).all()
 
 
+@pytest.mark.parametrize("block", [None, 128])
+@pytest.mark.parametrize("width", [40, 128, 510, 2048])
+def test_quantized_borders(path, block, width):
+    """Every code of bfloat16 rows: 448 t / max |t| with t = h w is a quotient of 19 bits by 16, a border between two
+    codes or 2^-21 away from it, and float32's correct quotient tells which; borders go to the even code."""
+    x, res, w, _, _ = make(200, width, BF16, BF16, BF16)
+    q, _, h = rms_norm_quantized(x, w, residual=res, block=block)
+    t = h.double() * w.double()
+    size = width if block is None else block
+    parts = torch.nn.functional.pad(t, (0, -width % size)).view(200, -1, size)
+    v = (448 * parts / parts.abs().amax(2, keepdim=True)).view(200, -1)[:, :width]
+    step = torch.exp2(torch.floor(torch.log2(v.abs().clamp_min(2.0**-6))) - 3)
+    want = torch.round(v / step) * step
+    assert (v / step - torch.floor(v / step) == 0.5).any() or width < 510
+    assert torch.equal(q.double(), want)
+
+
 def test_quantized_values_that_are_none(path):
     x, res, w, _, _ = make(5, 300, F32, F32, F32)
     clean = rms_norm_quantized(x, w, residual=res)
