@@ -760,8 +760,8 @@ int odp_route_grad(odp_stream_t stream, int dtype, const void* logits, int64_t l
 
 /* ---- norm of a tree of gradients --------------------------------------------
  * leaves: a table in HOST memory, read during the call, ODP_TN_FIELDS words a
- * row.  norm = sqrt of the sum of all squares (float64 sums; stored as float64
- * where wide != 0, else float32); with clip != 0 every leaf's dst = src factor,
+ * row.  norm = sqrt of the sum of all squares (float64 sums, for float64 leaves also
+ * of squares beyond it; stored as float64 where wide != 0, else float32); with clip != 0 every leaf's dst = src factor,
  * factor = max_norm / norm where norm > max_norm, else 1 (an exact copy), NaN for
  * a NaN norm; dst may be src.  The factor and product are float32 (float64 for
  * float64 leaves).  scratch: odp_tree_norm_scratch() bytes on the 8-byte grid.

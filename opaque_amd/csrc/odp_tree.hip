@@ -8,10 +8,12 @@
 // bound by HBM.  Leaves travel in the kernels' arguments (TN_LEAVES a launch),
 // so a call copies no table and may be captured.  Squares are exact in float64
 // and added there: no overflow, and sums that do not depend on how a tree is cut
-// into leaves by more than 2^-53 of their size a step.  The second pass walks the
-// chunks backwards, the last read first, which the 256 MB cache still holds.
-// Every workgroup adds the first pass's partials for itself, in one order, so
-// neither a third launch nor an atomic is needed.
+// into leaves by more than 2^-53 of their size a step.  Float64 leaves may have
+// entries whose squares leave float64: those are added up beside, over 2^1200 or
+// times it (Far), so that the norm is infinite only where float64 cannot hold it.
+// The second pass walks the chunks backwards, the last read first, which the
+// 256 MB cache still holds.  Every workgroup adds the first pass's partials for
+// itself, in one order, so neither a third launch nor an atomic is needed.
 //
 // Four Llama-3-8B-shaped layers in bfloat16 (36 leaves, 1.74 GB): 261 us at 6.7 TB/s
 // and 650 at 5.4; 50 leaves of 64 to 4 million float32 (65 MB): 14 and 21 us.
@@ -62,8 +64,35 @@ __device__ __forceinline__ void put(char* p, u32x4_t w) {
   else *g = w;
 }
 
+// Sums of squares of float64 entries above 2^480, over 2^1200, and below 2^-480,
+// times it: the other squares, 2^45 of them, and these lie well within float64.
+struct Far {
+  double big = 0.0, small = 0.0;
+};
+constexpr double TN_FAR = 0x1p480, TN_BY = 0x1p600;
+
+__device__ __forceinline__ double square_wide(double v, double s, Far& far) {
+  const double m = fabs(v);
+  if (m > TN_FAR) {
+    const double t = v * (1.0 / TN_BY);
+    far.big = fma(t, t, far.big);
+  } else if (m < 1.0 / TN_FAR) {
+    const double t = v * TN_BY;
+    far.small = fma(t, t, far.small);
+  } else {
+    s = fma(v, v, s);
+  }
+  return s;
+}
+
+__device__ __forceinline__ double norm_of(double s, Far far) {
+  if (far.big > 0.0) return TN_BY * sqrt(far.big + s / TN_BY / TN_BY);
+  if (s != 0.0) return sqrt(s + far.small / TN_BY / TN_BY);
+  return sqrt(far.small) / TN_BY;
+}
+
 template <int DT>
-__device__ __forceinline__ double squares(u32x4_t w, double s) {
+__device__ __forceinline__ double squares(u32x4_t w, double s, Far& far) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if constexpr (DT == ODP_DTYPE_F32) {
@@ -71,8 +100,7 @@ __device__ __forceinline__ double squares(u32x4_t w, double s) {
       s = fma(v, v, s);
     } else if constexpr (DT == ODP_DTYPE_F64) {
       if (i & 1) continue;
-      const double v = __longlong_as_double((long long)((uint64_t)w[i + 1] << 32 | w[i]));
-      s = fma(v, v, s);
+      s = square_wide(__longlong_as_double((long long)((uint64_t)w[i + 1] << 32 | w[i])), s, far);
     } else {
       double a, b;
       if constexpr (DT == ODP_DTYPE_BF16) {
@@ -117,7 +145,8 @@ constexpr int TN_FLIGHT = 4;  // 16-byte pieces of a thread in flight
 
 // One chunk's squares, or its scaled copy.  NT: by non-temporal loads and stores.
 template <int DT, bool SCALE, bool NT>
-__device__ __forceinline__ double chunk_pass(const char* src, char* dst, int64_t n, float f, double d, double s) {
+__device__ __forceinline__ double chunk_pass(const char* src, char* dst, int64_t n, float f, double d, double s,
+                                             Far& far) {
   constexpr int E = DT == ODP_DTYPE_F64 ? 8 : DT == ODP_DTYPE_F32 ? 4 : 2, V = 16 / E;
   const int pieces = (int)(n / V);
   double part[TN_FLIGHT] = {};
@@ -133,7 +162,7 @@ __device__ __forceinline__ double chunk_pass(const char* src, char* dst, int64_t
       if constexpr (SCALE) {
         if (i + k * TN_THREADS < pieces) put<NT>(dst + 16 * (int64_t)(i + k * TN_THREADS), scaled<DT>(w[k], f, d));
       } else {
-        part[k] = squares<DT>(w[k], part[k]);
+        part[k] = squares<DT>(w[k], part[k], far);
       }
     }
   }
@@ -145,6 +174,8 @@ __device__ __forceinline__ double chunk_pass(const char* src, char* dst, int64_t
     if constexpr (SCALE) {
       if constexpr (DT == ODP_DTYPE_F64) odp_gstore((double*)dst + at, v * d);
       else odp_store_from_float(dst, at, DT, (float)v * f);
+    } else if constexpr (DT == ODP_DTYPE_F64) {
+      s = square_wide(v, s, far);
     } else {
       s = fma(v, v, s);
     }
@@ -152,8 +183,9 @@ __device__ __forceinline__ double chunk_pass(const char* src, char* dst, int64_t
   return s;
 }
 
-template <bool SCALE>
-__device__ __forceinline__ double one_chunk(const Leaves& l, int c, float f, double d, double s) {
+// WIDE: the tree has float64 leaves.
+template <bool SCALE, bool WIDE>
+__device__ __forceinline__ double one_chunk(const Leaves& l, int c, float f, double d, double s, Far& far) {
   const int leaf = leaf_of(l, c), dt = l.dt[leaf];
   const int64_t first = (int64_t)(c - l.start[leaf]) * l.chunk, n = min((int64_t)l.chunk, l.n[leaf] - first);
   const int64_t at = first * odp_dtype_size(dt);
@@ -161,10 +193,10 @@ __device__ __forceinline__ double one_chunk(const Leaves& l, int c, float f, dou
   char* dst = SCALE ? l.dst[leaf] + at : nullptr;
   const auto pass = [&](auto nt) {
     constexpr bool NT = decltype(nt)::value;
-    if (dt == ODP_DTYPE_BF16) return chunk_pass<ODP_DTYPE_BF16, SCALE, NT>(src, dst, n, f, d, s);
-    if (dt == ODP_DTYPE_F32) return chunk_pass<ODP_DTYPE_F32, SCALE, NT>(src, dst, n, f, d, s);
-    if (dt == ODP_DTYPE_F16) return chunk_pass<ODP_DTYPE_F16, SCALE, NT>(src, dst, n, f, d, s);
-    return chunk_pass<ODP_DTYPE_F64, SCALE, NT>(src, dst, n, f, d, s);
+    if (dt == ODP_DTYPE_BF16) return chunk_pass<ODP_DTYPE_BF16, SCALE, NT>(src, dst, n, f, d, s, far);
+    if (dt == ODP_DTYPE_F32) return chunk_pass<ODP_DTYPE_F32, SCALE, NT>(src, dst, n, f, d, s, far);
+    if (!WIDE || dt == ODP_DTYPE_F16) return chunk_pass<ODP_DTYPE_F16, SCALE, NT>(src, dst, n, f, d, s, far);
+    return chunk_pass<ODP_DTYPE_F64, SCALE, NT>(src, dst, n, f, d, s, far);
   };
   return l.once ? pass(std::true_type{}) : pass(std::false_type{});
 }
@@ -180,12 +212,21 @@ __device__ __forceinline__ double sum_block(double s, double* red) {
   return t;
 }
 
-__global__ __launch_bounds__(TN_THREADS) void k_tree_squares(const Leaves l, double* part) {
-  __shared__ double red[TN_THREADS / 64];
+// part: of the squares, and `apart` further on each of what Far holds.
+template <bool WIDE>
+__global__ __launch_bounds__(TN_THREADS) void k_tree_squares(const Leaves l, double* part, int64_t apart) {
+  __shared__ double red[WIDE ? 3 : 1][TN_THREADS / 64];
   double s = 0.0;
-  for (int c = blockIdx.x; c < l.chunks; c += gridDim.x) s = one_chunk<false>(l, c, 0.0f, 0.0, s);
-  s = sum_block(s, red);
+  Far far;
+  for (int c = blockIdx.x; c < l.chunks; c += gridDim.x) s = one_chunk<false, WIDE>(l, c, 0.0f, 0.0, s, far);
+  s = sum_block(s, red[0]);
   if (threadIdx.x == 0) odp_gstore(part + blockIdx.x, s);
+  if constexpr (WIDE) {
+    const double big = sum_block(far.big, red[1]), small = sum_block(far.small, red[2]);
+    if (threadIdx.x != 0) return;
+    odp_gstore(part + apart + blockIdx.x, big);
+    odp_gstore(part + 2 * apart + blockIdx.x, small);
+  }
 }
 
 __device__ __forceinline__ double factor_of(double norm, double most) {
@@ -199,29 +240,40 @@ __device__ __forceinline__ void store_norm(void* out, int wide, double norm) {
 }
 
 // out: where the norm goes (null but in the first launch).
-__global__ __launch_bounds__(TN_THREADS) void k_tree_scale(const Leaves l, const double* __restrict__ part, int parts,
-                                                           double most, int wide, void* out) {
-  __shared__ double red[TN_THREADS / 64];
+template <bool WIDE>
+__global__ __launch_bounds__(TN_THREADS) void k_tree_scale(const Leaves l, const double* __restrict__ part, int64_t apart,
+                                                           int parts, double most, int wide, void* out) {
+  __shared__ double red[WIDE ? 3 : 1][TN_THREADS / 64];
   double s = 0.0;
-  for (int i = threadIdx.x; i < parts; i += TN_THREADS) s += part[i];
-  const double norm = sqrt(sum_block(s, red));
+  Far far;
+  for (int i = threadIdx.x; i < parts; i += TN_THREADS) {
+    s += part[i];
+    if constexpr (WIDE) far.big += part[apart + i], far.small += part[2 * apart + i];
+  }
+  s = sum_block(s, red[0]);
+  if constexpr (WIDE) far.big = sum_block(far.big, red[1]), far.small = sum_block(far.small, red[2]);
+  const double norm = norm_of(s, far);
   if (out != nullptr && blockIdx.x == 0) store_norm(out, wide, norm);
   const double d = factor_of(norm, most);
   const float f = (float)d;
-  for (int c = l.chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) one_chunk<true>(l, c, f, d, 0.0);
+  for (int c = l.chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) one_chunk<true, WIDE>(l, c, f, d, 0.0, far);
 }
 
 // A small tree in one launch of one workgroup.
+template <bool WIDE>
 __global__ __launch_bounds__(TN_THREADS) void k_tree_small(const Leaves l, int clip, double most, int wide, void* out) {
-  __shared__ double red[TN_THREADS / 64];
+  __shared__ double red[WIDE ? 3 : 1][TN_THREADS / 64];
   double s = 0.0;
-  for (int c = 0; c < l.chunks; ++c) s = one_chunk<false>(l, c, 0.0f, 0.0, s);
-  const double norm = sqrt(sum_block(s, red));
+  Far far;
+  for (int c = 0; c < l.chunks; ++c) s = one_chunk<false, WIDE>(l, c, 0.0f, 0.0, s, far);
+  s = sum_block(s, red[0]);
+  if constexpr (WIDE) far.big = sum_block(far.big, red[1]), far.small = sum_block(far.small, red[2]);
+  const double norm = norm_of(s, far);
   store_norm(out, wide, norm);
   if (!clip) return;
   const double d = factor_of(norm, most);
   const float f = (float)d;
-  for (int c = l.chunks - 1; c >= 0; --c) one_chunk<true>(l, c, f, d, 0.0);
+  for (int c = l.chunks - 1; c >= 0; --c) one_chunk<true, WIDE>(l, c, f, d, 0.0, far);
 }
 
 // A tree of few and small leaves is one workgroup's.
@@ -256,7 +308,7 @@ void fill(Leaves& l, const int64_t* rows, int64_t n_leaves, int64_t k, int64_t c
 }  // namespace
 
 extern "C" int64_t odp_tree_norm_scratch(int64_t n_leaves) {
-  return n_leaves <= 0 ? 8 : 8 * TN_BLOCKS * ((n_leaves + TN_LEAVES - 1) / TN_LEAVES);
+  return n_leaves <= 0 ? 8 : 8 * 3 * TN_BLOCKS * ((n_leaves + TN_LEAVES - 1) / TN_LEAVES);
 }
 
 extern "C" int odp_tree_norm(odp_stream_t stream, const int64_t* leaves, int64_t n_leaves, int clip, double max_norm,
@@ -271,6 +323,7 @@ extern "C" int odp_tree_norm(odp_stream_t stream, const int64_t* leaves, int64_t
     return ODP_ERR_INVALID_ARGUMENT;
   }
   int64_t total = 0, used = 0, bytes = 0;
+  bool doubles = false;
   for (int64_t i = 0; i < n_leaves; ++i) {
     const int64_t* r = leaves + i * ODP_TN_FIELDS;
     const int64_t n = r[ODP_TN_N], dt = r[ODP_TN_DTYPE];
@@ -289,13 +342,15 @@ extern "C" int odp_tree_norm(odp_stream_t stream, const int64_t* leaves, int64_t
     total += n;
     bytes += n * odp_dtype_size((int)dt);
     used += n > 0;
+    doubles = doubles || dt == ODP_DTYPE_F64;
   }
   hipStream_t s = odp_hip_stream(stream);
   Leaves l;
   const int64_t launches = (n_leaves + TN_LEAVES - 1) / TN_LEAVES;
   if (total <= TN_SMALL && used <= TN_FEW && launches <= 1) {
     fill(l, leaves, n_leaves, 0, TN_SMALL, bytes);
-    k_tree_small<<<1, TN_THREADS, 0, s>>>(l, clip, max_norm, wide, norm);
+    const auto small = doubles ? k_tree_small<true> : k_tree_small<false>;
+    small<<<1, TN_THREADS, 0, s>>>(l, clip, max_norm, wide, norm);
     return odp_check_launch(what);
   }
   // Chunks of 32768 elements (of bfloat16 what the threads have in flight at once),
@@ -304,17 +359,20 @@ extern "C" int odp_tree_norm(odp_stream_t stream, const int64_t* leaves, int64_t
   while (chunk > 2048 && total / chunk < 2 * TN_BLOCKS) chunk >>= 1;
   while (total / chunk > (int64_t)1 << 28) chunk <<= 1;
   double* part = (double*)scratch;
+  const int64_t apart = TN_BLOCKS * launches;
+  const auto squares = doubles ? k_tree_squares<true> : k_tree_squares<false>;
+  const auto scale = doubles ? k_tree_scale<true> : k_tree_scale<false>;
   int64_t parts = 0;
   for (int64_t k = 0; k < launches; ++k) {
     fill(l, leaves, n_leaves, k, chunk, bytes);
     if (l.chunks == 0) continue;
     const int blocks = l.chunks < TN_BLOCKS ? l.chunks : TN_BLOCKS;
-    k_tree_squares<<<blocks, TN_THREADS, 0, s>>>(l, part + parts);
+    squares<<<blocks, TN_THREADS, 0, s>>>(l, part + parts, apart);
     parts += blocks;
   }
   if (!clip || parts == 0) {
     l.chunks = l.count = 0;
-    k_tree_scale<<<1, TN_THREADS, 0, s>>>(l, part, (int)parts, 0.0, wide, norm);  // the norm alone
+    scale<<<1, TN_THREADS, 0, s>>>(l, part, apart, (int)parts, 0.0, wide, norm);  // the norm alone
     return odp_check_launch(what);
   }
   bool told = false;
@@ -322,7 +380,7 @@ extern "C" int odp_tree_norm(odp_stream_t stream, const int64_t* leaves, int64_t
     fill(l, leaves, n_leaves, k, chunk, bytes);
     if (l.chunks == 0) continue;
     const int blocks = l.chunks < TN_BLOCKS ? l.chunks : TN_BLOCKS;
-    k_tree_scale<<<blocks, TN_THREADS, 0, s>>>(l, part, (int)parts, max_norm, wide, told ? nullptr : norm);
+    scale<<<blocks, TN_THREADS, 0, s>>>(l, part, apart, (int)parts, max_norm, wide, told ? nullptr : norm);
     told = true;
   }
   return odp_check_launch(what);

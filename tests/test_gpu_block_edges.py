@@ -1,0 +1,79 @@
+"""The ends of the norm, routing and tree-norm operators' ranges, on both host paths.
+
+Tolerances count roundings of half a step, 2^-24 of a value in float32 and 2^-53 in float64, as the operators' own tests
+do; each is derived beside its use.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from opaque_amd import vocabulary
+from opaque_amd.global_norm import clip_by_global_norm, global_norm
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+F32, BF16, F16, F64 = torch.float32, torch.bfloat16, torch.float16, torch.float64
+U = 2.0**-24
+
+
+@pytest.fixture(params=[True, False], ids=["helper", "functions"])
+def path(request, monkeypatch):
+    if not request.param:
+        monkeypatch.setattr(vocabulary, "_host_ready", [None])
+
+
+# ---------------------------------------------------------------------------
+# The norm of a tree
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("size", [5, 100, 40000])
+@pytest.mark.parametrize("power", [1019, 600, 481, 479, 0, -479, -481, -600, -1000])
+def test_float64_leaves_whose_squares_leave_float64(path, size, power):
+    """Finite trees have finite norms, of one workgroup and of many, one launch and several: entries near 2^power.
+
+    The norm is that of the entries over 2^power times 2^power, both exact: n additions of float64, 2^-53 n at most, n
+    below 2^18, so 2^-35; the factor and the product one step of 2^-53 each beside it.
+    """
+    g = torch.Generator(device=DEV).manual_seed(size)
+    # 2^1019 times 40000 values below 0.05 and 140 empty leaves (two launches): a norm below 2^1024.
+    base = [0.02 + 0.03 * torch.rand(size, generator=g, device=DEV, dtype=F64) for _ in range(3)]
+    unit = math.sqrt(sum(float(t.square().sum()) for t in base))
+    for empty in (0, 140):
+        grads = {f"k{i}": t * 2.0**power for i, t in enumerate(base)}
+        grads |= {f"e{i}": torch.empty(0, device=DEV) for i in range(empty)}
+        assert all(bool(t.isfinite().all()) for t in grads.values())
+        norm = global_norm(grads)
+        assert norm.dtype == F64 and abs(math.ldexp(float(norm), -power) / unit - 1) < 2.0**-35
+        for over in (0.5, 4.0):
+            got, same = clip_by_global_norm(grads, float(norm) / over)
+            assert torch.equal(same, norm)
+            for i, t in enumerate(base):
+                back = got[f"k{i}"] * 2.0**-power
+                # (entries of 2^-1000 / 32 and above keep their 53 bits)
+                assert ((back - t / max(over, 1.0)).abs() <= 2.0**-50 * t).all()
+
+
+def test_float64_leaves_of_all_sizes_together(path):
+    """Entries on both sides of float64's squares in one tree, beside leaves of other types; a true infinity stays one."""
+    tiny = torch.full((30000,), 1e-170, device=DEV, dtype=F64)
+    for big, want in ((1e200, 1e200 * 2**0.5), (2.0**480, 2.0**480 * 2**0.5), (1e3, math.hypot(1e3 * 2**0.5, 30.0))):
+        t = {"t": tiny, "b": torch.tensor([big, -big], device=DEV, dtype=F64), "f": torch.full((9,), 10.0, device=DEV),
+             "h": torch.zeros(5, device=DEV, dtype=BF16)}
+        got, norm = clip_by_global_norm(t, want / 2)
+        assert abs(float(norm) / want - 1) < 1e-14
+        assert abs(float(got["b"][0]) / (big / 2) - 1) < 1e-14 and float(got["b"][1]) < 0
+        assert torch.allclose(got["f"], torch.full_like(got["f"], 5.0), rtol=1e-6, atol=0)
+    only = {"t": tiny, "z": torch.zeros(40000, device=DEV)}
+    assert abs(float(global_norm(only)) / (1e-170 * 30000**0.5) - 1) < 1e-12
+    for bad, seen in ((float("inf"), math.isinf), (float("nan"), math.isnan)):
+        t = {"b": torch.tensor([1e200, bad, 1e-200], device=DEV, dtype=F64)}
+        assert seen(float(global_norm(t)))
+    # Beyond float64 itself: an infinite norm, which makes finite entries 0.
+    got, norm = clip_by_global_norm({"b": torch.full((4,), 1.5e308, device=DEV, dtype=F64)}, 1.0)
+    assert norm.isinf() and not got["b"].any()
