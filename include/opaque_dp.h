@@ -728,7 +728,10 @@ int odp_rms_norm(odp_stream_t stream, int dtype, int stream_dtype, int gain_dtyp
  * of `dtype` (null: not wanted) and dres of stream_dtype (null: not wanted, or the
  * same as dx where the types are), dgain [gains][width] of gain_dtype (null: not
  * wanted), summed over each gain's rows in float32.  h has stream_dtype (x's
- * where there was no residual).  scratch: odp_rms_norm_grad_scratch() bytes.   */
+ * where there was no residual).  scratch: odp_rms_norm_grad_scratch() bytes.  Gains
+ * are workgroups of one launch: any ODP_NORM_GRAD_GAINS of them are taken (four
+ * times as many up to 8192 columns), more are the caller's to cut.              */
+#define ODP_NORM_GRAD_GAINS ((int64_t)1 << 21)
 int64_t odp_rms_norm_grad_scratch(int64_t n, int64_t width, int64_t gains);
 int odp_rms_norm_grad(odp_stream_t stream, int dtype, int stream_dtype, int gain_dtype, const void* h, int64_t ldh,
                       const float* rstd, const void* gy, int64_t ldy, const void* gh, int64_t ldgh, int64_t n,

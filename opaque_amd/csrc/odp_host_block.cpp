@@ -2,6 +2,7 @@
 // norm, routing) and of the tree norm outside torch.func, on the host:
 // arguments to addresses, workspaces, and the autograd nodes.  No device code;
 // the work is the C entry points of libopaque_dp.so, bound by address.
+#include <algorithm>
 #include <map>
 #include <unordered_map>
 
@@ -155,12 +156,23 @@ struct NormNode final : torch::autograd::Node {
       if (need_w) dw = n > 0 ? at::empty(w_shape, w_.options()) : at::zeros(w_shape, w_.options());
       const int64_t words = need_w ? abi.rms_norm_grad_scratch(n, width, g.count) : 0;
       const at::Tensor work = words > 0 ? bytes_on(h_, words) : at::Tensor();
-      check(abi.rms_norm_grad(stream_of(h_), code_of(gy.held), code_of(h_), g.dt, rows.at, rows.pitch,
-                              (const float*)stat.data_ptr(), gy.at, gy.pitch, gh.at, gh.pitch, n, width, g.at, g.pitch,
-                              g.count, (float)offset, work.defined() ? work.data_ptr() : nullptr,
-                              dx.defined() ? dx.data_ptr() : nullptr, dr.defined() ? dr.data_ptr() : nullptr,
-                              dw.defined() ? dw.data_ptr() : nullptr),
-            "odp_rms_norm_grad");
+      const auto at = [](const at::Tensor& t, const void* p, int64_t items) {
+        return p == nullptr ? nullptr : (char*)const_cast<void*>(p) + items * (int64_t)t.element_size();
+      };
+      const auto out = [&](const at::Tensor& t, int64_t items) { return t.defined() ? at(t, t.data_ptr(), items) : nullptr; };
+      // More gains than a call takes go in parts of about one size, each with enough of them to need no scratch.
+      const int64_t parts = (g.count + ODP_NORM_GRAD_GAINS - 1) / ODP_NORM_GRAD_GAINS;
+      const int64_t most = (g.count + parts - 1) / parts, each = n / g.count;
+      for (int64_t i = 0; i < g.count; i += most) {
+        const int64_t gains = std::min(most, g.count - i), row = i * each;
+        check(abi.rms_norm_grad(stream_of(h_), code_of(gy.held), code_of(h_), g.dt, at(h_, rows.at, row * rows.pitch),
+                                rows.pitch, (const float*)stat.data_ptr() + row, at(gy.held, gy.at, row * gy.pitch),
+                                gy.pitch, at(h_, gh.at, row * gh.pitch), gh.pitch, gains * each, width,
+                                at(g.t, g.at, i * g.pitch), g.pitch, gains, (float)offset,
+                                work.defined() ? work.data_ptr() : nullptr, out(dx, row * width), out(dr, row * width),
+                                out(dw, i * width)),
+              "odp_rms_norm_grad");
+      }
       if (need_r && same) dr = dx;
       if (!need_x) dx = at::Tensor();
     }

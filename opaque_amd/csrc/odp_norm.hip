@@ -794,6 +794,7 @@ extern "C" int odp_rms_norm_grad(odp_stream_t stream, int dtype, int stream_dtyp
   hipStream_t s = odp_hip_stream(stream);
   const int64_t blocks = gains * strips;  // at most n
   if (blocks * (width > 8192 ? 1024 : 256) > NORM_THREADS) {
+    static_assert(ODP_NORM_GRAD_GAINS * 1024 <= NORM_THREADS, "what the header promises");
     odp_set_error("%s: %lld gains are more than one launch takes", what, (long long)gains);
     return ODP_ERR_UNSUPPORTED;
   }

@@ -24,6 +24,7 @@ from opaque_amd.vocabulary import _F32, _bound, _call, _OnDevice, _stream, pitch
 
 _ROW_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _WIDE = 32768  # the widest row (ODP_NORM_WIDE)
+_GRAD_GAINS = 1 << 21  # gains of a call (ODP_NORM_GRAD_GAINS)
 BLOCK = 128  # columns of a scale of ``rms_norm_quantized(block=128)``
 
 
@@ -31,7 +32,7 @@ class _Gain:
     """Gains as the kernels take them: [width], one for all rows, or [groups, width], one for each group of rows."""
 
     def __init__(self, weight: torch.Tensor | None, groups: int, like: torch.Tensor) -> None:
-        self.count, self.pitch, self.at, self.dt = max(groups, 1), 0, None, dtype_code(like.dtype)
+        self.count, self.pitch, self.held, self.dt = max(groups, 1), 0, None, dtype_code(like.dtype)
         if weight is None:
             return
         w = weight.detach()
@@ -42,7 +43,7 @@ class _Gain:
             if w.stride(0) != 0 or (w.stride(1) != 1 and w.shape[1] > 1):
                 w = pitched_rows(w)
                 self.pitch = w.stride(0)
-        self.held, self.at, self.dt = w, w.data_ptr(), dtype_code(w.dtype)
+        self.held, self.dt = w, dtype_code(w.dtype)
 
 
 def _forward(x, residual, weight, eps, offset, keep, quant=0):
@@ -59,7 +60,7 @@ def _forward(x, residual, weight, eps, offset, keep, quant=0):
     at = lambda t: None if t is None else t.data_ptr()
     with _OnDevice(x):
         _call("odp_rms_norm", _stream(x), dtype_code(x.dtype), dtype_code(x.dtype if r is None else r.dtype), g.dt,
-              rows.data_ptr(), rows.stride(0), at(r), 0 if r is None else r.stride(0), n, width, g.at, g.pitch, g.count,
+              rows.data_ptr(), rows.stride(0), at(r), 0 if r is None else r.stride(0), n, width, at(g.held), g.pitch, g.count,
               eps, offset, quant, y.data_ptr(), at(h), at(rstd), at(scales))
     return y, h, rstd, scales
 
@@ -86,12 +87,18 @@ def _gradients(gy, gh, h, rstd, weight, dtype, offset, groups, need_x, need_r, n
         dw = make((groups, width) if groups else (width,), dtype=weight.dtype, device=dev)
         words = int(N.load().odp_rms_norm_grad_scratch(n, width, g.count))
     scratch = torch.empty(words // 4, dtype=torch.float32, device=dev) if words else None
-    at = lambda t: None if t is None else t.data_ptr()
+    at = lambda t, items: None if t is None else t.data_ptr() + items * t.element_size()
     stat = rstd.contiguous()
+    # More gains than a call takes go in parts of about one size, each with enough of them to need no scratch.
+    most, each = -(-g.count // -(-g.count // _GRAD_GAINS)), n // g.count
     with _OnDevice(h):
-        _call("odp_rms_norm_grad", _stream(h), dtype_code(dtype), dtype_code(h.dtype), g.dt, rows.data_ptr(),
-              rows.stride(0), stat.data_ptr(), y2.data_ptr(), y2.stride(0), at(h2), 0 if h2 is None else h2.stride(0),
-              n, width, g.at, g.pitch, g.count, offset, at(scratch), at(dx), at(dr), at(dw))
+        for i in range(0, g.count, most):
+            gains, row = min(most, g.count - i), i * each
+            _call("odp_rms_norm_grad", _stream(h), dtype_code(dtype), dtype_code(h.dtype), g.dt,
+                  at(rows, row * rows.stride(0)), rows.stride(0), at(stat, row), at(y2, row * y2.stride(0)), y2.stride(0),
+                  at(h2, 0 if h2 is None else row * h2.stride(0)), 0 if h2 is None else h2.stride(0), gains * each, width,
+                  at(g.held, i * g.pitch), g.pitch, gains, offset, at(scratch, 0), at(dx, row * width),
+                  at(dr, row * width), at(dw, i * width))
     return dx if need_x else None, (dx if same else dr) if need_r else None, dw
 
 

@@ -13,6 +13,7 @@ import torch
 
 from opaque_amd import vocabulary
 from opaque_amd.global_norm import clip_by_global_norm, global_norm
+from opaque_amd.normalization import rms_norm
 
 pytestmark = pytest.mark.gpu
 
@@ -25,6 +26,38 @@ U = 2.0**-24
 def path(request, monkeypatch):
     if not request.param:
         monkeypatch.setattr(vocabulary, "_host_ready", [None])
+
+
+# ---------------------------------------------------------------------------
+# The root-mean-square norm
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("gains,rows,stream", [((1 << 23) + 5, 1, BF16), ((1 << 22) + 1, 2, F32)], ids=str)
+def test_more_gains_than_a_launch_takes(path, gains, rows, stream):
+    """What the forward pass takes the backward pass takes: pieces of the batch have the bits that they have alone."""
+    g = torch.Generator(device=DEV).manual_seed(7)
+    normal = lambda *s: torch.randn(*s, generator=g, device=DEV)
+    x, gy = normal(gains, rows, 8).to(BF16), normal(gains, rows, 8).to(BF16)
+    r, gh = normal(gains, rows, 8).to(stream), normal(gains, rows, 8).to(stream)
+    w = (1 + 0.3 * normal(gains, 8)).to(BF16)
+    one = lambda x, r, w: rms_norm(x, w, residual=r)
+
+    def step(at):
+        ts = [t[at].detach().requires_grad_() for t in (x, r, w)]
+        outs = torch.func.vmap(one)(*ts)
+        return [*outs, *torch.autograd.grad(outs, ts, [gy[at], gh[at]])]
+
+    whole = step(slice(None))
+    for first in (0, gains - 1000, *(k * gains // parts - 500 for parts in (2, 3, 5) for k in range(1, parts))):
+        for a, b in zip(whole, step(slice(first, first + 1000))):
+            assert torch.equal(a[first:first + 1000], b)
+    # Half a step of bfloat16 and the float32 roundings (48 steps of the terms' size) for the last piece.
+    h = (x[-1000:].float() + r[-1000:].float()).to(stream).double()
+    inv = 1 / torch.sqrt(h.square().mean(-1, keepdim=True) + 1e-6)
+    terms = gy[-1000:].double() * h * inv
+    want = terms.sum(1)
+    assert ((whole[4][-1000:].double() - want).abs() <= want.abs() * 2.0**-8 + 48 * U * terms.abs().sum(1)).all()
 
 
 # ---------------------------------------------------------------------------
