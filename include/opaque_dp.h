@@ -711,7 +711,7 @@ int odp_xent_dw(odp_stream_t stream, int dtype, const void* xc, int64_t n, int64
  * (pitch ldx) of `dtype` (float32, bfloat16 or float16), the stream (pitch ldr) of
  * stream_dtype, gains [gains][width] (pitch ldg, 0: one for all; null: 1) of
  * gain_dtype, both `dtype` or float32.  Gain i covers rows [i n / gains, ..): n is
- * a multiple of gains.  Sums of squares are float32, and y is rounded once.
+ * a multiple of gains (which may be 0 where n is).  Sums of squares are float32, and y is rounded once.
  * sum [n][width] receives h where there is a residual, rstd [n] (may be null)
  * 1 / sqrt(..).  quant 1 or 2: y [n][width] in e4m3 instead, with scales [n] or
  * [n][ceil(width / 128)] float32, the largest |y| of the row or of its 128 columns
@@ -741,7 +741,7 @@ int odp_rms_norm_grad(odp_stream_t stream, int dtype, int stream_dtype, int gain
 /* ---- routing to experts ----------------------------------------------------
  * For logits z [n][experts] (pitch ldz; float32, bfloat16 or float16): scores p =
  * softmax(z), or sigmoid(z) where sigmoid != 0; keys p + bias [biases][experts]
- * (null: none; bias i for the tokens [i n / biases, ..)); with `groups` > 1 the
+ * (null: none; bias i for the tokens [i n / biases, ..), 0 biases where n is 0); with `groups` > 1 the
  * best top_groups of the equal consecutive groups stay, by the sum of their two
  * best keys (best 0) or by their best (1); index [n][top_k] the best keys left,
  * best first, and weights [n][top_k] = scale p, over the sum of the chosen p with

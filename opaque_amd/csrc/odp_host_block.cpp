@@ -160,10 +160,11 @@ struct NormNode final : torch::autograd::Node {
         return p == nullptr ? nullptr : (char*)const_cast<void*>(p) + items * (int64_t)t.element_size();
       };
       const auto out = [&](const at::Tensor& t, int64_t items) { return t.defined() ? at(t, t.data_ptr(), items) : nullptr; };
-      // More gains than a call takes go in parts of about one size, each with enough of them to need no scratch.
+      // More gains than a call takes go in parts of about one size, each with enough of them to need no scratch;
+      // an empty batch may have none.
       const int64_t parts = (g.count + ODP_NORM_GRAD_GAINS - 1) / ODP_NORM_GRAD_GAINS;
-      const int64_t most = (g.count + parts - 1) / parts, each = n / g.count;
-      for (int64_t i = 0; i < g.count; i += most) {
+      const int64_t most = n > 0 ? (g.count + parts - 1) / parts : 0, each = n > 0 ? n / g.count : 0;
+      for (int64_t i = 0; n > 0 && i < g.count; i += most) {
         const int64_t gains = std::min(most, g.count - i), row = i * each;
         check(abi.rms_norm_grad(stream_of(h_), code_of(gy.held), code_of(h_), g.dt, at(h_, rows.at, row * rows.pitch),
                                 rows.pitch, (const float*)stat.data_ptr() + row, at(gy.held, gy.at, row * gy.pitch),

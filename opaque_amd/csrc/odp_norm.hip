@@ -684,7 +684,7 @@ int norm_check(const char* what, int dt, int ht, int gt, int64_t n, int64_t widt
                   (long long)ODP_NORM_WIDE);
     return ODP_ERR_INVALID_ARGUMENT;
   }
-  if (gains < 1 || n % gains != 0) {
+  if (gains < 1 ? n != 0 || gains < 0 : n % gains != 0) {  // an empty batch has no gains
     odp_set_error("%s: %lld rows do not divide into %lld gains", what, (long long)n, (long long)gains);
     return ODP_ERR_INVALID_ARGUMENT;
   }

@@ -915,7 +915,7 @@ extern "C" int odp_route(odp_stream_t stream, int dtype, const void* logits, int
                   (long long)experts, (long long)groups, RT_GROUPS, (long long)top_groups, (long long)top_k);
     return ODP_ERR_INVALID_ARGUMENT;
   }
-  if (bias != nullptr && (biases < 1 || n % biases != 0)) {
+  if (bias != nullptr && (biases < 1 ? n != 0 || biases < 0 : n % biases != 0)) {  // an empty batch has no biases
     odp_set_error("%s: %lld tokens do not divide into %lld biases", what, (long long)n, (long long)biases);
     return ODP_ERR_INVALID_ARGUMENT;
   }

@@ -31,8 +31,8 @@ BLOCK = 128  # columns of a scale of ``rms_norm_quantized(block=128)``
 class _Gain:
     """Gains as the kernels take them: [width], one for all rows, or [groups, width], one for each group of rows."""
 
-    def __init__(self, weight: torch.Tensor | None, groups: int, like: torch.Tensor) -> None:
-        self.count, self.pitch, self.held, self.dt = max(groups, 1), 0, None, dtype_code(like.dtype)
+    def __init__(self, weight: torch.Tensor | None, groups: int | None, like: torch.Tensor) -> None:
+        self.count, self.pitch, self.held, self.dt = 1 if groups is None else groups, 0, None, dtype_code(like.dtype)
         if weight is None:
             return
         w = weight.detach()
@@ -51,7 +51,7 @@ def _forward(x, residual, weight, eps, offset, keep, quant=0):
     rows = pitched_rows(x.detach())
     r = None if residual is None else pitched_rows(residual.detach())
     n, width = rows.shape
-    g, dev = _Gain(weight, 0, x), x.device
+    g, dev = _Gain(weight, None, x), x.device
     y = torch.empty(x.shape, dtype=torch.float8_e4m3fn if quant else x.dtype, device=dev)
     h = None if r is None else torch.empty(x.shape, dtype=r.dtype, device=dev)
     rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev) if keep else None
@@ -66,7 +66,7 @@ def _forward(x, residual, weight, eps, offset, keep, quant=0):
 
 
 def _gradients(gy, gh, h, rstd, weight, dtype, offset, groups, need_x, need_r, need_w):
-    """(dx, dres, dgain); dgain [width], or one for each of ``groups`` groups of rows."""
+    """(dx, dres, dgain); dgain [width], or one for each of ``groups`` groups of rows (none in an empty batch)."""
     like = gy if gy is not None else gh
     for t in (h, rstd, *(() if weight is None else (weight,))):
         if t.device != like.device:
@@ -84,15 +84,16 @@ def _gradients(gy, gh, h, rstd, weight, dtype, offset, groups, need_x, need_r, n
     dw = words = None
     if need_w:
         make = torch.empty if n else torch.zeros
-        dw = make((groups, width) if groups else (width,), dtype=weight.dtype, device=dev)
+        dw = make((width,) if groups is None else (groups, width), dtype=weight.dtype, device=dev)
         words = int(N.load().odp_rms_norm_grad_scratch(n, width, g.count))
     scratch = torch.empty(words // 4, dtype=torch.float32, device=dev) if words else None
     at = lambda t, items: None if t is None else t.data_ptr() + items * t.element_size()
     stat = rstd.contiguous()
     # More gains than a call takes go in parts of about one size, each with enough of them to need no scratch.
-    most, each = -(-g.count // -(-g.count // _GRAD_GAINS)), n // g.count
+    most = -(-g.count // -(-g.count // _GRAD_GAINS)) if n else 1
     with _OnDevice(h):
-        for i in range(0, g.count, most):
+        for i in range(0, g.count if n else 0, most):
+            each = n // g.count
             gains, row = min(most, g.count - i), i * each
             _call("odp_rms_norm_grad", _stream(h), dtype_code(dtype), dtype_code(h.dtype), g.dt,
                   at(rows, row * rows.stride(0)), rows.stride(0), at(stat, row), at(y2, row * y2.stride(0)), y2.stride(0),
@@ -123,11 +124,11 @@ class _NormGrad(torch.autograd.Function):
     def vmap(info, in_dims, gy, gh, h, rstd, weight, dtype, offset, groups, need_x, need_r, need_w):
         n = info.batch_size
         gy, gh, h, rstd = (None if t is None else front(t, d, n) for t, d in zip((gy, gh, h, rstd), in_dims))
-        each = max(groups, 1)
+        each = 1 if groups is None else groups
         if weight is not None:
             weight = _batched_gain(weight, in_dims[4], n, groups)
         dx, dr, dw = _NormGrad.apply(gy, gh, h, rstd, weight, dtype, offset, n * each, need_x, need_r, need_w)
-        if need_w and groups:
+        if need_w and groups is not None:
             dw = dw.unflatten(0, (n, groups))
         return (dx, dr, dw), (0 if need_x else None, 0 if need_r else None, 0 if need_w else None)
 
@@ -137,7 +138,7 @@ def _batched_gain(weight, d, n, groups):
     if d is not None:
         weight = weight.movedim(d, 0)
         return weight.flatten(0, 1) if weight.dim() == 3 else weight
-    if weight.dim() == 1 and not groups:
+    if weight.dim() == 1 and groups is None:
         return weight.unsqueeze(0).expand(n, -1)
     return (weight.unsqueeze(0).expand(n, *weight.shape).flatten(0, 1) if weight.dim() == 2
             else weight.unsqueeze(0).expand(n * groups, -1))
@@ -148,7 +149,7 @@ def _merge(n, dims, x, residual, weight):
     x = front(x, dims[0], n)
     residual = None if residual is None else front(residual, dims[1], n)
     if weight is not None and (dims[2] is not None or weight.dim() == 2):
-        weight = _batched_gain(weight, dims[2], n, weight.shape[0] if dims[2] is None else 0)
+        weight = _batched_gain(weight, dims[2], n, weight.shape[0] if dims[2] is None else None)
     return x, residual, weight
 
 
@@ -175,7 +176,7 @@ class _Norm(torch.autograd.Function):
             return None, None, None, None, None
         h, rstd, weight = ctx.saved_tensors
         need_x, need_r, need_w = ctx.needs_input_grad[:3]
-        groups = weight.shape[0] if weight is not None and weight.dim() == 2 else 0
+        groups = weight.shape[0] if weight is not None and weight.dim() == 2 else None
         dx, dr, dw = _NormGrad.apply(gy, gh, h, rstd, weight, ctx.dtype, ctx.offset, groups, need_x, need_r, need_w)
         return dx, dr, dw, None, None
 

@@ -12,6 +12,7 @@ import pytest
 import torch
 
 from opaque_amd import vocabulary
+from opaque_amd.experts import route
 from opaque_amd.global_norm import clip_by_global_norm, global_norm
 from opaque_amd.normalization import rms_norm
 
@@ -58,6 +59,32 @@ def test_more_gains_than_a_launch_takes(path, gains, rows, stream):
     terms = gy[-1000:].double() * h * inv
     want = terms.sum(1)
     assert ((whole[4][-1000:].double() - want).abs() <= want.abs() * 2.0**-8 + 48 * U * terms.abs().sum(1)).all()
+
+
+@pytest.mark.parametrize("shape", [(0, 24), (0, 3, 24), (4, 0, 24), (0, 0, 24)], ids=str)
+def test_an_empty_batch_of_examples(path, shape):
+    """vmap over no examples, or over examples without rows, with a gain or bias of each: empty results, zero gradients."""
+    b = shape[0]
+    x, r = (torch.ones(shape, device=DEV, requires_grad=True) for _ in range(2))
+    w = torch.ones(b, 24, device=DEV, requires_grad=True)
+    y, h = torch.func.vmap(lambda x, r, w: rms_norm(x, w, residual=r))(x, r, w)
+    assert y.shape == h.shape == shape
+    for t, d in zip((x, r, w), torch.autograd.grad([y, h], [x, r, w], [torch.ones_like(y), torch.ones_like(h)])):
+        assert d.shape == t.shape and not d.any()
+    total = lambda w, x: rms_norm(x, w).sum()
+    for each in (w.detach(), torch.ones(24, device=DEV)):
+        d = torch.func.vmap(torch.func.grad(total), in_dims=(0 if each.dim() == 2 else None, 0))(each, x.detach())
+        assert d.shape == (b, 24) and not d.any()
+    if len(shape) == 3:
+        rows = torch.func.vmap(torch.func.vmap(torch.func.grad(total), in_dims=(None, 0)))(w.detach(), x.detach())
+        assert rows.shape == shape
+        flat = torch.func.vmap(torch.func.vmap(rms_norm, in_dims=(0, None)))(x, w)
+        assert flat.shape == shape
+    bias = torch.zeros(b, 24, device=DEV)
+    index, weights = torch.func.vmap(lambda z, b: route(z, 2, bias=b))(x, bias)
+    assert index.shape == weights.shape == (*shape[:-1], 2)
+    dz = torch.func.vmap(torch.func.grad(lambda z, b: route(z, 2, bias=b)[1].sum()))(x.detach(), bias)
+    assert dz.shape == shape
 
 
 # ---------------------------------------------------------------------------
