@@ -280,35 +280,31 @@ class RMSNorm(torch.nn.Module):
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None):
         return rms_norm(x, self.weight, residual=residual, eps=self.eps, unit_offset=self.unit_offset)
 
-    @classmethod
-    def sharing(cls, weight: torch.nn.Parameter, eps: float) -> RMSNorm:
-        """A module on a given gain (shared, not copied)."""
-        m = cls(weight.shape[0], eps, device="meta", dtype=weight.dtype)
-        m.weight = weight
-        return m
-
     def extra_repr(self) -> str:
         return f"{self.weight.shape[0]}, eps={self.eps}" + (", unit_offset=True" if self.unit_offset else "")
 
 
 def route_norms(model: torch.nn.Module, types=(torch.nn.RMSNorm,)) -> list[str]:
-    """Replace the model's norms of the given classes by ``RMSNorm`` on the same gains; returns their names.
+    """Make the model's norms of the given classes ``RMSNorm``; returns their names, of a shared one each.
 
     Any class does whose forward is ``x / sqrt(mean(x^2) + eps) * weight`` over the last dimension, with a 1-D
     ``weight`` and ``eps`` or ``variance_epsilon`` (Hugging Face's): the product is rounded once here, where some round
-    before the gain too.  Norms without a gain or over several dimensions stay.
+    before the gain too.  The modules change their class in place, so gains, hooks, modes and sharing stay as they are.
+    Norms without a gain, over several dimensions or with a ``forward`` of the instance's own stay.
     """
-    names = []
-    for name, mod in list(model.named_modules()):
-        for child_name, child in list(mod.named_children()):
-            weight = getattr(child, "weight", None)
-            if type(child) not in tuple(types) or weight is None or weight.dim() != 1:
-                continue
-            eps = getattr(child, "eps", None) if hasattr(child, "eps") else child.variance_epsilon
-            eps = _F32.eps if eps is None else float(eps)  # torch's default, of the type that it computes in
-            setattr(mod, child_name, RMSNorm.sharing(weight, eps))
-            names.append(f"{name}.{child_name}" if name else child_name)
-    return names
+    found = []
+    for name, mod in model.named_modules(remove_duplicate=False):
+        weight = getattr(mod, "weight", None)
+        if type(mod) not in tuple(types) or weight is None or weight.dim() != 1:
+            continue
+        if type(mod) is RMSNorm or "forward" in vars(mod):
+            continue
+        eps = getattr(mod, "eps", None) if hasattr(mod, "eps") else mod.variance_epsilon
+        found.append((name, mod, _F32.eps if eps is None else float(eps)))  # torch's, of the type that it computes in
+    for _, mod, eps in found:
+        mod.__class__ = RMSNorm
+        mod.eps, mod.unit_offset = eps, False
+    return [name for name, _, _ in found]
 
 
 __all__ = ["BLOCK", "RMSNorm", "rms_norm", "rms_norm_quantized", "route_norms"]

@@ -3,9 +3,11 @@
 from __future__ import annotations
 
 import pytest
+import torch
 
 from opaque_amd import _native as N
 from opaque_amd import normalization
+from opaque_amd.normalization import RMSNorm, route_norms
 
 F32, BF16 = N.DTYPE_F32, N.DTYPE_BF16
 BAD = 64  # a non-null, aligned address; never read
@@ -35,3 +37,43 @@ def test_an_empty_batch_has_no_gains_and_no_biases(lib):
 def test_gains_of_a_gradient_call_match_the_header():
     text = (N.LIB_PATH.parents[1] / "include" / "opaque_dp.h").read_text()
     assert "ODP_NORM_GRAD_GAINS ((int64_t)1 << 21)" in text and normalization._GRAD_GAINS == 1 << 21
+
+
+def test_shared_norms_hooks_and_modes_stay():
+    """A norm under two names, of one parent and of two, is one norm afterwards too; its hooks run and its mode is kept."""
+    net = torch.nn.ModuleDict({"a": torch.nn.RMSNorm(6, eps=1e-3), "c": torch.nn.Sequential(torch.nn.RMSNorm(6))})
+    net["b"] = net["a"]
+    net["d"] = torch.nn.Sequential(net["a"], net["c"][0])
+    net["c"].eval()
+    calls, loads = [], []
+    handle = net["a"].register_forward_pre_hook(lambda mod, args: calls.append(type(mod)))
+    net["a"].register_load_state_dict_pre_hook(lambda mod, *rest: loads.append(type(mod)))
+    first, second = net["a"], net["c"][0]
+    assert sorted(route_norms(net)) == ["a", "b", "c.0", "d.0", "d.1"]
+    assert net["a"] is net["b"] is net["d"][0] is first and net["c"][0] is net["d"][1] is second
+    assert all(type(m) is RMSNorm for m in (first, second)) and first.eps == 1e-3 and "eps=0.001" in repr(first)
+    assert first.training and not second.training and sum(1 for _ in net.parameters()) == 2
+    with pytest.raises(RuntimeError, match="runs on the GPU"):
+        net["b"](torch.ones(2, 6))
+    net.load_state_dict(net.state_dict())
+    assert calls == [RMSNorm] and set(loads) == {RMSNorm}
+    handle.remove()
+    with pytest.raises(RuntimeError, match="runs on the GPU"):
+        net["b"](torch.ones(2, 6))
+    assert calls == [RMSNorm] and route_norms(net) == []
+
+
+def test_norms_that_stay_and_the_model_itself():
+    """A module with a forward of its own is not the class's norm; the package's own norms keep their unit offset."""
+    net = torch.nn.ModuleDict({"p": torch.nn.RMSNorm(6), "own": RMSNorm(6, unit_offset=True)})
+    net["p"].forward = lambda x: x
+    assert route_norms(net, (torch.nn.RMSNorm, RMSNorm)) == [] and net["own"].unit_offset
+    assert type(net["p"]) is torch.nn.RMSNorm
+    alone = torch.nn.RMSNorm(6)
+    assert route_norms(alone) == [""] and type(alone) is RMSNorm
+    without = torch.nn.Linear(6, 1)  # no eps: an error before anything changes
+    without.weight = torch.nn.Parameter(torch.ones(6))
+    both = torch.nn.Sequential(torch.nn.RMSNorm(6), without)
+    with pytest.raises(AttributeError):
+        route_norms(both, (torch.nn.RMSNorm, torch.nn.Linear))
+    assert type(both[0]) is torch.nn.RMSNorm
