@@ -179,8 +179,8 @@ class Router(Linear):
     """A router: logits from its weight [experts, width], through the full-weight seam, then ``route``.
 
     ``balance=True`` registers a float32 buffer ``balance`` [experts] of zeros that a training
-    loop may move against the experts' load.  ``forward`` returns
-    (index, weights) for ``capture.moe``.
+    loop may move against the experts' load; it stays float32 where the module is cast, as its
+    steps are small.  ``forward`` returns (index, weights) for ``capture.moe``.
     """
 
     def __init__(self, width: int, experts: int, top_k: int, *, scores: str = "softmax", balance: bool = False,
@@ -190,10 +190,17 @@ class Router(Linear):
         self.top_k = top_k
         self.options = {"scores": scores, "groups": groups, "top_groups": top_groups, "group_best": group_best,
                         "renormalize": renormalize, "scale": scale}
-        self.register_buffer("balance", torch.zeros(experts, device=device) if balance else None)
+        self.register_buffer("balance", torch.zeros(experts, dtype=torch.float32, device=device) if balance else None)
+
+    def _apply(self, fn, recurse=True):
+        kept = self.balance
+        super()._apply(fn, recurse)
+        if kept is not None and self.balance.dtype != torch.float32:
+            self.balance = kept.to(self.balance.device, torch.float32)
+        return self
 
     def forward(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-        bias = None if self.balance is None else self.balance.float()  # the module may have been cast as a whole
+        bias = None if self.balance is None else self.balance.float()  # a caller may bring another buffer
         return route(super().forward(x), self.top_k, bias=bias, **self.options)
 
 

@@ -2,11 +2,14 @@
 
 from __future__ import annotations
 
+import copy
+
 import pytest
 import torch
 
 from opaque_amd import _native as N
 from opaque_amd import normalization
+from opaque_amd.experts import Router
 from opaque_amd.normalization import RMSNorm, route_norms
 
 F32, BF16 = N.DTYPE_F32, N.DTYPE_BF16
@@ -77,3 +80,30 @@ def test_norms_that_stay_and_the_model_itself():
     with pytest.raises(AttributeError):
         route_norms(both, (torch.nn.RMSNorm, torch.nn.Linear))
     assert type(both[0]) is torch.nn.RMSNorm
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.double(),
+                                  lambda m: m.to(torch.bfloat16).float(), lambda m: m.to("cpu", torch.bfloat16),
+                                  lambda m: copy.deepcopy(m).bfloat16()],
+                         ids=["bfloat16", "half", "double", "back", "device", "copy"])
+def test_a_routers_bias_stays_float32(cast):
+    """Steps below a narrow type's resolution survive a cast of the model, and of the router itself."""
+    net = torch.nn.Sequential(torch.nn.Linear(8, 8), Router(8, 4, 2, balance=True))
+    step = torch.tensor([1.0, -1.0, 0.5, 0.0]) + 1e-5
+    net[1].balance += step
+    got = cast(net)
+    assert got[1].balance.dtype == torch.float32 and torch.equal(got[1].balance, step)
+    assert got[1].weight.dtype == got[0].weight.dtype and set(dict(got.named_buffers())) == {"1.balance"}
+    assert torch.equal(cast(Router(8, 4, 2, balance=True)).balance, torch.zeros(4))
+    assert cast(Router(8, 4, 2)).balance is None
+
+
+def test_a_routers_bias_is_float32_from_the_start():
+    before = torch.get_default_dtype()
+    try:
+        torch.set_default_dtype(torch.bfloat16)
+        assert Router(8, 4, 2, balance=True).balance.dtype == torch.float32
+    finally:
+        torch.set_default_dtype(before)
+    meta = Router(8, 4, 2, balance=True, device="meta", dtype=torch.bfloat16).to_empty(device="cpu")
+    assert meta.balance.dtype == torch.float32 and meta.weight.dtype == torch.bfloat16

@@ -11,10 +11,11 @@ import math
 import pytest
 import torch
 
-from opaque_amd import vocabulary
-from opaque_amd.experts import route
+from opaque_amd import capture, vocabulary
+from opaque_amd.clipping import clipped_grad
+from opaque_amd.experts import Router, route
 from opaque_amd.global_norm import clip_by_global_norm, global_norm
-from opaque_amd.normalization import rms_norm
+from opaque_amd.normalization import RMSNorm, rms_norm
 
 pytestmark = pytest.mark.gpu
 
@@ -85,6 +86,68 @@ def test_an_empty_batch_of_examples(path, shape):
     assert index.shape == weights.shape == (*shape[:-1], 2)
     dz = torch.func.vmap(torch.func.grad(lambda z, b: route(z, 2, bias=b)[1].sum()))(x.detach(), bias)
     assert dz.shape == shape
+
+
+# ---------------------------------------------------------------------------
+# The router
+# ---------------------------------------------------------------------------
+
+
+class Block(torch.nn.Module):
+    """Norm, router and experts; with ``plain`` the norm and the router in elementary operations."""
+
+    def __init__(self, dtype, plain=False):
+        super().__init__()
+        self.plain = plain
+        self.norm = RMSNorm(32, dtype=dtype)
+        self.router = Router(32, 8, 2, scores="sigmoid", balance=True, scale=1.5, dtype=dtype)
+        self.up, self.down = (torch.nn.Parameter(torch.empty(s, dtype=dtype)) for s in ((8, 48, 32), (8, 32, 24)))
+
+    def forward(self, x):
+        if not self.plain:
+            n = self.norm(x)
+            index, w = self.router(n)
+        else:
+            f = x.float()
+            n = (f / torch.sqrt(f.square().mean(-1, keepdim=True) + 1e-6) * self.norm.weight.float()).to(x.dtype)
+            p = torch.sigmoid(capture.linear(n, self.router.weight).float())
+            index = (p + self.router.balance).topk(2, -1).indices
+            w = p.gather(-1, index)
+            w = 1.5 * w / w.sum(-1, keepdim=True)
+        return x + capture.moe(n, self.up, self.down, index, w.to(n.dtype))
+
+
+@pytest.mark.parametrize("dtype,tol", [(F32, 1e-5), (BF16, 2e-2)], ids=str)
+def test_a_router_under_clipped_grad(path, dtype, tol):
+    """The module in a DP step, its weight a full-weight seam, its bias moved between steps: as with elementary operations
+    (1e-5 and 2e-2, the tolerances of the engine's own tests; the choices are the same, as the norms' roundings are)."""
+    g = torch.Generator().manual_seed(5)
+    own, plain = Block(F32), Block(F32, plain=True)
+    for p in own.parameters():
+        p.data = torch.randn(p.shape, generator=g) / p.shape[-1] ** 0.5 + (1 if p.dim() == 1 else 0)
+    plain.load_state_dict(own.state_dict())
+    own, plain = own.to(DEV, dtype), plain.to(DEV, dtype)
+    x = torch.randn(5, 12, 32, generator=g).to(dtype).to(DEV)
+    y = torch.randn(5, 12, 32, generator=g).to(DEV)
+    steps = {}
+    for m in (own, plain):
+        def loss(params, x, y):
+            return ((torch.func.functional_call(m, params, (x,)).float() - y) ** 2).mean()
+
+        fn, st = clipped_grad(loss, clipping_norm=0.05, normalize_by=5, batch_argnums=(1, 2), return_aux=True)
+        steps[m] = []
+        for k in range(2):
+            m.router.balance.copy_(0.2 * k * torch.linspace(-1, 1, 8, device=DEV))
+            (got, aux), st = fn(dict(m.named_parameters()), x, y, state=st)
+            steps[m].append({**got.pytree, "norms": aux.grad_norms, "losses": aux.loss_values})
+    for a, b in zip(steps[own], steps[plain]):
+        assert a["router.weight"].any() and a["norm.weight"].any()
+        for k, t in a.items():
+            assert (t.double() - b[k].double()).norm() <= tol * b[k].double().norm(), k
+    assert own.router.balance.dtype == F32
+    chosen = [own.router(own.norm(x))[0]]
+    own.router.balance.zero_()
+    assert not torch.equal(chosen[0], own.router(own.norm(x))[0])  # the bias is what moves the choice
 
 
 # ---------------------------------------------------------------------------
