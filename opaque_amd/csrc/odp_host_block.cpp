@@ -83,6 +83,12 @@ struct Normed {
   at::Tensor y, h, rstd, scales;
 };
 
+void no_tangents(const at::Tensor& x, const Maybe& residual, const Maybe& weight) {
+  odp_host::no_tangent(x, kNorms);
+  if (residual.has_value()) odp_host::no_tangent(*residual, kNorms);
+  if (weight.has_value()) odp_host::no_tangent(*weight, kNorms);
+}
+
 // quant: 0 none, 1 a scale per row, 2 per 128 columns.
 Normed norm_forward(const at::Tensor& x, const Maybe& residual, const Maybe& weight, double eps, double offset,
                     bool keep, int64_t quant) {
@@ -188,9 +194,7 @@ struct NormNode final : torch::autograd::Node {
 // (y, 1 / sqrt(..)) or, with a residual, (y, 1 / sqrt(..), the sum); without `keep` the second may be undefined.
 variable_list normed(const at::Tensor& x, const Maybe& residual, const Maybe& weight, double eps, double offset,
                      bool keep) {
-  odp_host::no_tangent(x, kNorms);
-  if (residual.has_value()) odp_host::no_tangent(*residual, kNorms);
-  if (weight.has_value()) odp_host::no_tangent(*weight, kNorms);
+  no_tangents(x, residual, weight);
   bool grad = true;
   if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(residual) || wants_grad(weight)))
     keep = true;
@@ -242,6 +246,7 @@ variable_list rms_norm_quantized(const at::Tensor& x, const Maybe& residual, con
                                  double offset, int64_t quant) {
   py::gil_scoped_release nogil;
   at::NoGradGuard no_grad;
+  no_tangents(x, residual, weight);
   const Normed o = norm_forward(x, residual, weight, eps, offset, false, quant);
   return residual.has_value() ? variable_list{o.y, o.scales, o.h} : variable_list{o.y, o.scales};
 }
@@ -355,6 +360,7 @@ std::pair<std::vector<at::Tensor>, at::Tensor> tree_norm(const std::vector<at::T
                      " supports float32, bfloat16, float16 and float64 leaves, got ", type);
     TORCH_CHECK(t.is_cuda() && t.device() == leaves[0].device(), who,
                 " runs on the GPU: its leaves must be CUDA tensors of one device");
+    odp_host::no_tangent(t, "the tree norm's operators");
     wide = wide || type == at::kDouble;
   }
   const c10::OptionalDeviceGuard guard(leaves.at(0).device());

@@ -18,7 +18,7 @@ from opaque_amd.capture import transformed
 from opaque_amd.engine import dtype_code
 from opaque_amd.pytree import tree_flatten, tree_unflatten
 from opaque_amd.types import ClippedPytree, NoisedPytree
-from opaque_amd.vocabulary import _bound, _call, _OnDevice, _stream
+from opaque_amd.vocabulary import _bound, _call, _OnDevice, _stream, no_tangent
 
 _LEAF_DTYPES = (torch.float32, torch.bfloat16, torch.float16, torch.float64)
 
@@ -80,6 +80,7 @@ def _run(name: str, grads, max_norm: float | None):
         out, norm = host.tree_norm(tensors, clip, max_norm or 0.0, name)
     else:
         wide = _checked(name, tensors)
+        no_tangent("the tree norm's operators", *tensors)
         with torch.no_grad():
             out, norm = _tree_norm([t.detach() for t in tensors], clip, max_norm or 0.0, wide)
     if not clip:
@@ -97,7 +98,7 @@ def global_norm(tree) -> torch.Tensor:
     Leaves are float32, bfloat16, float16 or float64 CUDA tensors (others of the
     tree are passed over); squares and sums are float64 (those of float64 leaves
     also where their squares leave it) and the result float32, with a float64 leaf float64.  Nothing is copied to the host, and the result
-    has no gradient.  An empty tree's norm is 0, on the CPU.
+    has no gradient (a forward-mode tangent is an error).  An empty tree's norm is 0, on the CPU.
     """
     return _run("global_norm", tree.pytree if isinstance(tree, ClippedPytree) else tree, None)[1]
 

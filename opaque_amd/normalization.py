@@ -20,7 +20,7 @@ from opaque_amd import _native as N
 from opaque_amd._vmap import front, merged
 from opaque_amd.capture import transformed
 from opaque_amd.engine import dtype_code
-from opaque_amd.vocabulary import _F32, _bound, _call, _OnDevice, _stream, pitched_rows
+from opaque_amd.vocabulary import _F32, _bound, _call, _OnDevice, _stream, no_tangent, pitched_rows
 
 _ROW_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _WIDE = 32768  # the widest row (ODP_NORM_WIDE)
@@ -250,7 +250,8 @@ def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor | None = None, *, r
     of the row over 448, or with ``block=128`` [..., ceil(width / 128)], that of
     every 128 columns; at least the least normal float32, so a row of zeros has
     a finite one.  A row (or block) that holds a NaN is NaN.  Not
-    differentiable: no input may require a gradient, unless gradients are off.
+    differentiable: no input may require a gradient, unless gradients are off, or
+    have a forward-mode tangent.
     """
     _check("rms_norm_quantized", x, weight, residual, eps)
     if block not in (None, BLOCK):
@@ -264,6 +265,7 @@ def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor | None = None, *, r
     quant, host = 2 if block else 1, _bound()
     if host is not None:
         return tuple(host.rms_norm_quantized(x, residual, weight, eps, offset, quant))
+    no_tangent("the norm operators", x, residual, weight)
     q, h, _, scales = _forward(x, residual, weight, float(eps), offset, False, quant)
     return (q, scales) if residual is None else (q, scales, h)
 

@@ -84,6 +84,12 @@ def _on_one_device(t: torch.Tensor, *saved: torch.Tensor) -> None:
             raise RuntimeError(f"vocabulary operators: a saved tensor came back on {s.device}, not {t.device}")
 
 
+def no_tangent(who: str, *tensors: torch.Tensor | None) -> None:
+    """A forward-mode tangent would be dropped without a word where no autograd.Function takes the call."""
+    if any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{who} have no forward-mode derivative")
+
+
 def pitched_rows(t: torch.Tensor) -> torch.Tensor:
     """2-D view [rows, d] with unit column stride and a pitch of at least d;
     rows laid out otherwise (transposed, expanded) are copied."""

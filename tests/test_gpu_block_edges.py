@@ -15,7 +15,7 @@ from opaque_amd import capture, vocabulary
 from opaque_amd.clipping import clipped_grad
 from opaque_amd.experts import Router, route
 from opaque_amd.global_norm import clip_by_global_norm, global_norm
-from opaque_amd.normalization import RMSNorm, rms_norm
+from opaque_amd.normalization import RMSNorm, rms_norm, rms_norm_quantized
 
 pytestmark = pytest.mark.gpu
 
@@ -200,3 +200,19 @@ def test_float64_leaves_of_all_sizes_together(path):
     # Beyond float64 itself: an infinite norm, which makes finite entries 0.
     got, norm = clip_by_global_norm({"b": torch.full((4,), 1.5e308, device=DEV, dtype=F64)}, 1.0)
     assert norm.isinf() and not got["b"].any()
+
+
+def test_tangents_are_refused_where_there_is_no_derivative(path):
+    """A dual tensor in is an error, not a result without its tangent; plain tensors beside the level are none."""
+    x, r = torch.randn(4, 32, device=DEV), torch.randn(4, 32, device=DEV)
+    w = torch.ones(32, device=DEV)
+    want = rms_norm_quantized(x, w, residual=r)[2], global_norm({"a": x})
+    with torch.autograd.forward_ad.dual_level():
+        dual = lambda t: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+        for args in ((dual(x), r, w), (x, dual(r), w), (x, r, dual(w))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                rms_norm_quantized(args[0], args[2], residual=args[1])
+        for call in (global_norm, lambda t: clip_by_global_norm(t, 1.0)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call({"a": x, "b": dual(r)})
+        assert torch.equal(rms_norm_quantized(x, w, residual=r)[2], want[0]) and global_norm({"a": x}) == want[1]
