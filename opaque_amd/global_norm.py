@@ -97,8 +97,9 @@ def global_norm(tree) -> torch.Tensor:
 
     Leaves are float32, bfloat16, float16 or float64 CUDA tensors (others of the
     tree are passed over); squares and sums are float64 (those of float64 leaves
-    also where their squares leave it) and the result float32, with a float64 leaf float64.  Nothing is copied to the host, and the result
-    has no gradient (a forward-mode tangent is an error).  An empty tree's norm is 0, on the CPU.
+    also where their squares leave it) and the result float32, with a float64
+    leaf float64.  Nothing is copied to the host, and the result has no gradient
+    (a forward-mode tangent is an error).  An empty tree's norm is 0, on the CPU.
     """
     return _run("global_norm", tree.pytree if isinstance(tree, ClippedPytree) else tree, None)[1]
 

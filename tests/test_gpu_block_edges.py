@@ -11,6 +11,7 @@ import math
 import pytest
 import torch
 
+from opaque_amd import _native as N
 from opaque_amd import capture, vocabulary
 from opaque_amd.clipping import clipped_grad
 from opaque_amd.experts import Router, route
@@ -60,6 +61,41 @@ def test_more_gains_than_a_launch_takes(path, gains, rows, stream):
     terms = gy[-1000:].double() * h * inv
     want = terms.sum(1)
     assert ((whole[4][-1000:].double() - want).abs() <= want.abs() * 2.0**-8 + 48 * U * terms.abs().sum(1)).all()
+
+
+@pytest.mark.parametrize("gains,rows,width", [(6, 300, 24), (6, 300, 1001), (6, 300, 4096), (100, 300, 40), (511, 260, 8),
+                                              (2, 2050, 200), (3, 40, 8200), (2, 40, 16400), (1, 40, 32768),
+                                              (2, 40, 32768)])
+@pytest.mark.parametrize("dtype,stream", [(BF16, BF16), (F32, F32), (F16, F32)], ids=str)
+def test_several_strips_of_several_gains(gains, rows, width, dtype, stream):
+    """Gains whose rows go to more than one workgroup: each sum against float64, dx with the bits of its example alone.
+
+    A gain's sum takes rows + 64 float32 additions at most, each half a step of 2^-24 of the terms' sizes (with the terms'
+    own products and 1 / sqrt), then half a step of its type.
+    """
+    words = N.load().odp_rms_norm_grad_scratch(gains * rows, width, gains)
+    assert words > 4 * gains * width and words % (4 * gains * width) == 0  # two strips a gain at least
+    g = torch.Generator(device=DEV).manual_seed(width + gains)
+    normal = lambda *s: torch.randn(*s, generator=g, device=DEV)
+    size = torch.exp(normal(gains, rows, 1))
+    ts = [(size * normal(gains, rows, width)).to(dtype), (size * normal(gains, rows, width)).to(stream),
+          (1 + 0.3 * normal(gains, width)).to(dtype)]
+    ts = [t.requires_grad_() for t in ts]
+    gy, gh = normal(gains, rows, width).to(dtype), normal(gains, rows, width).to(stream)
+    one = lambda x, r, w: rms_norm(x, w, residual=r)
+    outs = torch.func.vmap(one)(*ts)
+    dx, dr, dw = torch.autograd.grad(outs, ts, [gy, gh])
+    h = outs[1].detach().double()
+    terms = gy.double() * h / torch.sqrt(h.square().mean(-1, keepdim=True) + 1e-6)
+    want = terms.sum(1)
+    slack = (rows + 64) * U * terms.abs().sum(1) + want.abs() * torch.finfo(dtype).eps / 2 + 1e-30
+    worst = ((dw.double() - want).abs() - slack).max().item()
+    assert worst <= 0, worst
+    for i in {0, gains // 2, gains - 1}:
+        alone = [t[i].detach().requires_grad_() for t in ts]
+        a, b, c = torch.autograd.grad(one(*alone), alone, [gy[i], gh[i]])
+        assert torch.equal(a, dx[i]) and torch.equal(b, dr[i])
+        assert ((c.double() - want[i]).abs() <= slack[i]).all()
 
 
 @pytest.mark.parametrize("shape", [(0, 24), (0, 3, 24), (4, 0, 24), (0, 0, 24)], ids=str)
