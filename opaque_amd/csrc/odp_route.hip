@@ -38,6 +38,7 @@ typedef u32x4_t u32x4_w __attribute__((aligned(4)));
 
 constexpr int RT_THREADS = 256;
 constexpr int RT_GROUPS = 64;  // groups, at most (a mask of 64 bits)
+constexpr float ROUTE_DEEP = 32.0f;  // spread of the biases, in largest scores, from which on low ones are cut
 
 // e^x: 2^t from the hardware, t = x log2(e) rounded, and what the rounding took
 // off as a first-order factor; 2 units in the last place.
@@ -457,6 +458,7 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
   uint32_t key[V];  // 0: no expert, or closed; leading parts: 1 masked, 2 and more the others
   uint32_t tol = 0;
   bool weird = false;  // a row for route_exactly
+  bool cut = false;    // keys far below the largest bias share a leading part of 2
   const uint32_t place = mask - (uint32_t)first;
   if (sums) {
     float lo = 0.0f, hi = 0.0f, b[V];
@@ -464,7 +466,6 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
       load_row<V>(b, (const char*)bias, ODP_DTYPE_F32, first, a.experts, -INFINITY);
       lo = INFINITY;
       hi = -INFINITY;
-      uint32_t most = 0;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const bool shut = b[i] == -INFINITY;  // a key of -inf, as a masked expert's
@@ -472,9 +473,8 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
         bounded &= !shut;
         lo = fminf(lo, shut ? INFINITY : b[i]);
         hi = fmaxf(hi, b[i]);
-        most = max(most, shut ? 0u : __float_as_uint(b[i]) & 0x7fffffffu);
+        weird |= b[i] != b[i];
       }
-      weird = most >= 0x49800000u;  // from 2^20 on keys in 64 bits lose what the words still tell apart
       lo = -fmax_of<L>(-lo);
       hi = fmax_of<L>(hi);
       if (!(lo <= hi)) lo = hi = 0.0f;  // all shut
@@ -484,14 +484,37 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
     }
     const float over = a.sigmoid ? 0.0f : __builtin_amdgcn_rcpf(total);
     // The largest softmax is e^0 over the sum; a row that is all masked has none.
-    const float range = (total > 0.0f && !a.sigmoid ? over : 1.0f) + (hi - lo);
+    const float one = total > 0.0f && !a.sigmoid ? over : 1.0f;
+    // One bias far below the rest (an expert switched off by -1e4) would coarsen all
+    // keys.  Where `enough` experts lie within d of the largest, what is below that
+    // shares the least leading part: in order still, and near each other where the
+    // choice should come to hang on them after all.  Biases spread out evenly fail at
+    // the first d.  32768 tokens of 256 experts, one of them at -1e4: 24 us by sigmoids
+    // (20 without it; uncut 234), 27 in groups (23; 149).
+    const bool deep = hi - lo > ROUTE_DEEP * one;
+    if (__builtin_amdgcn_ballot_w64(deep) != 0 && deep) {
+      const float enough = (float)(a.groups > 1 ? 2 * a.top_k * a.groups / a.top_groups : a.top_k);
+#pragma unroll 1
+      for (float d = fminf((hi - lo) * 0.0625f, 0x1p15f * one);; d *= 0.125f) {
+        float within = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) within += z[i] > -INFINITY && b[i] >= hi - d ? 1.0f : 0.0f;
+        if (!(sum_of<L>(within) >= enough)) break;
+        cut = true;
+        lo = hi - d;
+        if (!(d > 8.0f * one)) break;
+      }
+    }
+    const float range = one + (hi - lo);
     weird |= !(range < 1e30f);
+    // From 2^20 on keys in 64 bits lose what the words still tell apart.
+    weird |= fmaxf(fabsf(lo), fabsf(hi)) >= 0x1p20f;
     const float by = (float)(steps - 16) * __builtin_amdgcn_rcpf(range);
     tol = (units_apart(a.sigmoid, over * __builtin_amdgcn_rcpf(range)) >> (24 - min(24, 32 - a.bits))) + 1;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const float s = a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z[i] * -1.44269502f)) : p[i] * over;
-      key[i] = (uint32_t)fmaf(s, by, fmaf(b[i] - lo, by, 2.0f)) << a.bits | (place - i);
+      key[i] = (uint32_t)fmaxf(fmaf(s, by, fmaf(b[i] - lo, by, 2.0f)), 2.0f) << a.bits | (place - i);
     }
   } else if (fits) {
 #pragma unroll
@@ -530,6 +553,11 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
     const auto score = [&](uint32_t one, uint32_t two, int g) {
       return a.best == 0 ? ((one >> a.bits) + (two >> a.bits)) << 6 | (uint32_t)(63 - g) : one;
     };
+    // A group's sum with a second key that is cut is more than the keys'.
+    bool mixed = false;
+    const auto cut_in = [&](uint32_t one, uint32_t two) {
+      mixed |= cut && a.best == 0 && two >> a.bits == 2 && one >> a.bits > 2;
+    };
     const int span = a.span;  // threads of a group; 0: its bounds lie between them
     if (span > 0) {
       uint32_t one = 0, two = 0;
@@ -544,7 +572,10 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
       if (L > 8 && span > 8) second(one, two, across<8>(one), across<8>(two));
       if (L > 16 && span > 16) second(one, two, across<16>(one), across<16>(two));
       const int g = t / span;
-      if (t == g * span && g < a.groups) scores[g] = score(one, two, g);
+      if (t == g * span && g < a.groups) {
+        scores[g] = score(one, two, g);
+        cut_in(one, two);
+      }
     } else {
       uint32_t* all = (uint32_t*)words + mine * L * V;
 #pragma unroll
@@ -562,6 +593,7 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
           i = i + 1 == a.size ? 0 : i + 1;
         }
         scores[g] = score(one, two, g);
+        cut_in(one, two);
       }
     }
     wave_sync();
@@ -583,6 +615,7 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
     const int shift = a.best == 0 ? 6 : a.bits;
     const uint32_t apart = (last >> shift) - (next >> shift);
     bool unsure = !fits && !weird && apart <= (a.best == 0 ? 2 * tol : tol);
+    if (__builtin_amdgcn_ballot_w64(mixed) != 0) unsure |= !weird && or_of<L>(mixed ? 1u : 0u) != 0;
     wave_sync();
     if (__builtin_amdgcn_ballot_w64(unsure && apart == 0) != 0) unsure &= apart != 0 || !all_equal<L>(a, row, bias, t);
     if (__builtin_amdgcn_ballot_w64(unsure) != 0) {

@@ -17,6 +17,7 @@ from opaque_amd.clipping import clipped_grad
 from opaque_amd.experts import Router, route
 from opaque_amd.global_norm import clip_by_global_norm, global_norm
 from opaque_amd.normalization import RMSNorm, rms_norm, rms_norm_quantized
+from test_gpu_route import check, logits
 
 pytestmark = pytest.mark.gpu
 
@@ -122,6 +123,55 @@ def test_an_empty_batch_of_examples(path, shape):
     assert index.shape == weights.shape == (*shape[:-1], 2)
     dz = torch.func.vmap(torch.func.grad(lambda z, b: route(z, 2, bias=b)[1].sum()))(x.detach(), bias)
     assert dz.shape == shape
+
+
+# ---------------------------------------------------------------------------
+# Routing
+# ---------------------------------------------------------------------------
+
+LOW = [-1e2, -1e3, -1e4, -1e5, -1e9, torch.finfo(F32).min]
+
+
+def biases(e, which, low):
+    """Biases of some steps, and the experts of ``which`` switched off by a low finite one."""
+    b = (torch.randn(e, generator=torch.Generator().manual_seed(e)) * 3).round() / 20
+    at = {"one": [e // 3], "some": list(range(1, e, 5)), "first": list(range(e // 4)), "few stay": list(range(3, e)),
+          "all": list(range(e)), "one of four stays": [i for i in range(e // 2) if i % (e // 4)],
+          "mixed": list(range(e // 2))}[which]
+    b[at] = low
+    if which == "mixed":  # by several amounts, some equal
+        b[at] = torch.tensor([low, 2 * low if low > -1e30 else low, -100.0, -40.0])[torch.arange(len(at)) % 4]
+    return b.to(DEV)
+
+
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("e", [8, 16, 60, 256, 300, 1024])
+@pytest.mark.parametrize("which", ["one", "some", "first", "few stay", "all", "one of four stays", "mixed"])
+def test_experts_switched_off_by_a_low_bias(scores, e, which):
+    """The float64 keys' choice whatever is below it, also where it reaches among the low ones or a group has one of them
+    in its sum."""
+    for low in LOW:
+        b = biases(e, which, low)
+        for dtype, spread in ((F32, 2.0), (BF16, 0.02)):
+            z = logits(200, e, dtype, spread=spread)
+            check(z, min(e, 6), scores=scores, bias=b)
+            for best in ("top2", "max"):
+                for groups, top_groups in ((4, 2), (4, 1), (2, 1)):
+                    check(z, min(6, e // groups * top_groups), scores=scores, bias=b, groups=groups, top_groups=top_groups,
+                          group_best=best, renormalize=False)
+
+
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("spread", [0.3, 3.0, 30.0, 3000.0])
+def test_biases_far_apart(scores, spread):
+    """Biases over many times the scores' range, equal ones among them, deep choices too."""
+    for e, k in ((8, 7), (64, 40), (256, 8), (256, 64), (1000, 16)):
+        b = (torch.randn(e, generator=torch.Generator().manual_seed(e + 1)) * 8).round() / 8 * spread
+        for s in (0.01, 2.0):
+            z = logits(150, e, spread=s)
+            check(z, k, scores=scores, bias=b.to(DEV))
+            for best in ("top2", "max"):
+                check(z, min(k, e // 2), scores=scores, bias=b.to(DEV), groups=8, top_groups=4, group_best=best)
 
 
 # ---------------------------------------------------------------------------
