@@ -67,7 +67,7 @@ struct Gain {
   int dt;
   Gain(const Maybe& w, int rows_dt) : dt(rows_dt) {
     if (!w.has_value()) return;
-    t = *w;
+    t = odp_host::plain(*w);
     dt = code_of(t);
     if (t.dim() == 1) {
       t = t.contiguous();
@@ -267,7 +267,7 @@ struct Options {
 std::pair<at::Tensor, at::Tensor> route_forward(const at::Tensor& z, const Maybe& bias, const Options& o) {
   const c10::OptionalDeviceGuard guard(z.device());
   const Rows rows(z);
-  const at::Tensor b = bias.has_value() ? bias->contiguous() : at::Tensor();
+  const at::Tensor b = bias.has_value() ? odp_host::plain(*bias).contiguous() : at::Tensor();
   std::vector<int64_t> shape(z.sizes().vec());
   shape.back() = o.top_k;
   const at::Tensor index = at::empty(shape, z.options().dtype(at::kLong));
@@ -306,7 +306,8 @@ struct RouteNode final : torch::autograd::Node {
       const Rows rows(z_);
       std::vector<int64_t> chosen(shape);
       chosen.back() = o.top_k;
-      const at::Tensor at_ = odp_host::whole(index_, gw, at::kLong, chosen, kRoutes), g = gw.contiguous();
+      const at::Tensor at_ = odp_host::whole(index_, gw, at::kLong, chosen, kRoutes);
+      const at::Tensor g = odp_host::plain(gw).contiguous();
       dz = at::empty(shape, z_.options());
       check(abi.route_grad(stream_of(z_), code_of(z_), rows.at, rows.pitch, rows.n, rows.width, (int)o.sigmoid, o.top_k,
                            (int)o.renorm, (float)o.scale, (const int64_t*)at_.data_ptr(), (const float*)g.data_ptr(),
@@ -369,7 +370,7 @@ std::pair<std::vector<at::Tensor>, at::Tensor> tree_norm(const std::vector<at::T
   std::map<at::ScalarType, std::pair<int64_t, at::Tensor>> buffers;
   std::vector<int64_t> at_(leaves.size()), table(leaves.size() * ODP_TN_FIELDS);
   for (size_t i = 0; i < leaves.size(); ++i) {
-    const at::Tensor& t = leaves[i];
+    const at::Tensor t = odp_host::plain(leaves[i]);
     src[i] = t.is_non_overlapping_and_dense() ? t : t.contiguous();
     auto& b = buffers[t.scalar_type()];
     at_[i] = b.first;

@@ -32,8 +32,12 @@ inline odp_stream_t stream_of(const at::Tensor& t) {
 inline at::Tensor bytes_on(const at::Tensor& t, int64_t n) { return at::empty({n}, t.options().dtype(at::kByte)); }
 inline int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 
+// What the memory holds is the tensor's values (a view of a conjugate's imaginary part has theirs negated).
+inline at::Tensor plain(const at::Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // Rows with unit column stride and a pitch of at least the width, copied if laid out otherwise.
-inline at::Tensor pitched(const at::Tensor& t) {
+inline at::Tensor pitched(const at::Tensor& given) {
+  const at::Tensor t = plain(given);
   at::Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
   if ((r.stride(1) != 1 && r.size(1) > 1) || r.stride(0) < r.size(1)) r = r.clone(at::MemoryFormat::Contiguous);
   return r;
@@ -47,9 +51,10 @@ struct Rows {
   int64_t n = 0, width = 0, pitch = 0;
   Rows() = default;
   explicit Rows(const at::Tensor& t) : width(t.size(-1)) {
-    held = t.is_contiguous() ? t : pitched(t);
+    const bool whole = t.is_contiguous() && !t.is_neg();
+    held = whole ? t : pitched(t);
     n = t.numel() / width;
-    pitch = t.is_contiguous() ? width : held.stride(0);
+    pitch = whole ? width : held.stride(0);
     at = held.data_ptr();
   }
 };

@@ -27,7 +27,7 @@ _BEST = ("top2", "max")
 
 def _choose(z, bias, sigmoid, groups, top_groups, best, top_k, renorm, scale):
     rows = pitched_rows(z.detach())
-    b = None if bias is None else bias.detach().contiguous()
+    b = None if bias is None else bias.detach().resolve_neg().contiguous()
     shape = (*z.shape[:-1], top_k)
     index = torch.empty(shape, dtype=torch.int64, device=z.device)
     weights = torch.empty(shape, dtype=torch.float32, device=z.device)
@@ -45,7 +45,7 @@ def _gradient(gw, z, index, sigmoid, top_k, renorm, scale):
             raise RuntimeError(f"routing operator: a saved tensor came back on {t.device}, not {gw.device}")
     if index.dtype != torch.int64 or index.shape != gw.shape or z.shape[:-1] != gw.shape[:-1]:
         raise RuntimeError("routing operator: a saved tensor came back otherwise than it was saved")
-    rows, g, idx = pitched_rows(z.detach()), gw.detach().contiguous(), index.contiguous()
+    rows, g, idx = pitched_rows(z.detach()), gw.detach().resolve_neg().contiguous(), index.contiguous()
     dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
     with _OnDevice(z):
         _call("odp_route_grad", _stream(z), dtype_code(z.dtype), rows.data_ptr(), rows.stride(0), rows.shape[0],

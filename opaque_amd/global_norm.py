@@ -35,7 +35,7 @@ def _dense(t: torch.Tensor) -> bool:
 
 def _tree_norm(leaves: list[torch.Tensor], clip: bool, max_norm: float, wide: bool):
     dev = leaves[0].device
-    src = [t if _dense(t) else t.contiguous() for t in leaves]
+    src = [t if _dense(t) else t.contiguous() for t in (t.resolve_neg() for t in leaves)]
     out = [torch.empty_like(t) for t in src] if clip else []
     table = torch.zeros(len(src), N.TN_FIELDS, dtype=torch.int64)
     for i, t in enumerate(src):

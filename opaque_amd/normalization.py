@@ -35,7 +35,7 @@ class _Gain:
         self.count, self.pitch, self.held, self.dt = 1 if groups is None else groups, 0, None, dtype_code(like.dtype)
         if weight is None:
             return
-        w = weight.detach()
+        w = weight.detach().resolve_neg()
         if w.dim() == 1:
             w = w.contiguous()
         else:

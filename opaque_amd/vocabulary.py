@@ -93,6 +93,7 @@ def no_tangent(who: str, *tensors: torch.Tensor | None) -> None:
 def pitched_rows(t: torch.Tensor) -> torch.Tensor:
     """2-D view [rows, d] with unit column stride and a pitch of at least d;
     rows laid out otherwise (transposed, expanded) are copied."""
+    t = t.resolve_neg()
     t2 = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
     if (t2.stride(1) != 1 and t2.shape[1] > 1) or t2.stride(0) < t2.shape[1]:
         t2 = t2.clone(memory_format=torch.contiguous_format)

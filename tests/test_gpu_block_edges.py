@@ -302,3 +302,32 @@ def test_tangents_are_refused_where_there_is_no_derivative(path):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 call({"a": x, "b": dual(r)})
         assert torch.equal(rms_norm_quantized(x, w, residual=r)[2], want[0]) and global_norm({"a": x}) == want[1]
+
+
+def test_views_whose_memory_holds_the_negative(path):
+    """The imaginary part of a conjugate is a view with a negative bit, dense where it is one element; torch._neg_view
+    makes one of any shape."""
+    x, r, gy = (torch.randn(6, 64, device=DEV) for _ in range(3))
+    w, b = torch.randn(64, device=DEV), 0.1 * torch.randn(64, device=DEV)
+    neg = lambda t: torch._neg_view(-t)
+    assert neg(x).is_neg() and torch.equal(neg(x), x)
+
+    def step(x, r, w, gy):
+        ts = [t.detach().requires_grad_() for t in (x, r, w)]
+        outs = rms_norm(ts[0], ts[2], residual=ts[1])
+        return [*outs, *torch.autograd.grad(outs, ts, [gy, gy])]
+
+    for a, c in zip(step(x, r, w, gy), step(neg(x), neg(r), neg(w), neg(gy))):
+        assert torch.equal(a, c)
+    for a, c in zip(rms_norm_quantized(x, w, residual=r), rms_norm_quantized(neg(x), neg(w), residual=neg(r))):
+        assert torch.equal(a.float(), c.float())
+    z, zn = x.clone().requires_grad_(), neg(x).requires_grad_()
+    (i, u), (j, v) = route(z, 4, bias=b), route(zn, 4, bias=neg(b))
+    assert torch.equal(i, j) and torch.equal(u, v)
+    g = torch.randn_like(u)
+    assert torch.equal(torch.autograd.grad(u, z, g)[0], torch.autograd.grad(v, zn, neg(g))[0])
+    one = torch.tensor(1.0 - 3.0j, device=DEV).conj().imag
+    assert one.is_neg() and float(one) == 3.0
+    tree, same = {"a": x, "b": one.clone().resolve_neg()}, {"a": neg(x), "b": one}
+    (p, m), (q, n) = clip_by_global_norm(tree, 1.0), clip_by_global_norm(same, 1.0)
+    assert torch.equal(m, n) and all(torch.equal(p[k], q[k]) for k in p) and float(q["b"]) > 0
