@@ -138,6 +138,7 @@ struct NormNode final : torch::autograd::Node {
     const at::Tensor& gy0 = grads[0];
     const at::Tensor gh0 = has_r ? grads[1] : at::Tensor();
     if (!gy0.defined() && !gh0.defined()) return variable_list(3);
+    odp_host::no_batch(grads, kNorms);
     const at::Tensor h_ = h.unpack(has_r ? shared_from_this() : nullptr), rstd_ = rstd.unpack();
     const at::Tensor w_ = has_w ? w.unpack() : at::Tensor();
     const bool need_x = task_should_compute_output(0), need_r = task_should_compute_output(1);
@@ -255,7 +256,7 @@ variable_list rms_norm_quantized(const at::Tensor& x, const Maybe& residual, con
 // Routing
 // ---------------------------------------------------------------------------
 
-constexpr const char* kRoutes = "the routing operator";
+constexpr const char* kRoutes = "the routing operators";
 
 struct Options {
   bool sigmoid;
@@ -297,6 +298,7 @@ struct RouteNode final : torch::autograd::Node {
     std::lock_guard<std::mutex> lock(mutex_);
     const at::Tensor& gw = grads[0];
     if (!gw.defined() || !task_should_compute_output(0)) return variable_list(1);
+    odp_host::no_batch(grads, kRoutes);
     const at::Tensor z_ = z.unpack(), index_ = index.unpack();
     at::Tensor dz;
     {

@@ -64,6 +64,14 @@ inline void no_tangent(const at::Tensor& t, const char* who) {
   TORCH_CHECK(!t._fw_grad(0).defined(), who, " have no forward-mode derivative");
 }
 
+// Gradients that is_grads_batched brings are a batch without an address.
+inline constexpr c10::DispatchKeySet kBatched{c10::DispatchKey::Batched, c10::DispatchKey::FuncTorchBatched};
+inline void no_batch(at::TensorList gs, const char* who) {
+  for (const at::Tensor& g : gs)
+    TORCH_CHECK(!g.defined() || !g.key_set().has_any(kBatched), who,
+                " take no gradients batched by is_grads_batched (or vectorize=True): torch.func's transforms run");
+}
+
 // Ties a first derivative to what it depends on, so that asking for a second
 // one is an error instead of zero: to the gradients gs it came from and, with
 // `inputs`, to the inputs of the node whose backward pass calls this (by

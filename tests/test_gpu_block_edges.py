@@ -331,3 +331,17 @@ def test_views_whose_memory_holds_the_negative(path):
     tree, same = {"a": x, "b": one.clone().resolve_neg()}, {"a": neg(x), "b": one}
     (p, m), (q, n) = clip_by_global_norm(tree, 1.0), clip_by_global_norm(same, 1.0)
     assert torch.equal(m, n) and all(torch.equal(p[k], q[k]) for k in p) and float(q["b"]) > 0
+
+
+def test_batched_gradients():
+    """is_grads_batched is refused by name; torch.func's jacrev gives the same rows."""
+    x, w = torch.randn(3, 16, device=DEV), torch.randn(16, device=DEV)
+    leaf = x.clone().requires_grad_()
+    y, (_, p) = rms_norm(leaf, w), route(leaf, 4)
+    for out in (y, p):
+        with pytest.raises(RuntimeError, match="is_grads_batched"):
+            torch.autograd.grad(out, leaf, torch.ones(2, *out.shape, device=DEV), is_grads_batched=True, retain_graph=True)
+    rows = torch.func.jacrev(lambda t: rms_norm(t, w))(x[0])
+    for k in range(16):
+        one = x[:1].clone().requires_grad_()
+        assert torch.equal(rows[k], torch.autograd.grad(rms_norm(one, w)[0, k], one)[0][0])
