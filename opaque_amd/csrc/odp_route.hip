@@ -473,8 +473,9 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
         bounded &= !shut;
         lo = fminf(lo, shut ? INFINITY : b[i]);
         hi = fmaxf(hi, b[i]);
-        weird |= b[i] != b[i];
       }
+#pragma unroll
+      for (int i = 0; i < V; i += 2) weird |= __builtin_isunordered(b[i], b[i + 1]);  // a NaN
       lo = -fmax_of<L>(-lo);
       hi = fmax_of<L>(hi);
       if (!(lo <= hi)) lo = hi = 0.0f;  // all shut
@@ -492,7 +493,7 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
     // the first d.  32768 tokens of 256 experts, one of them at -1e4: 24 us by sigmoids
     // (20 without it; uncut 234), 27 in groups (23; 149).
     const bool deep = hi - lo > ROUTE_DEEP * one;
-    if (__builtin_amdgcn_ballot_w64(deep) != 0 && deep) {
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(deep) != 0, 0) && deep) {
       const float enough = (float)(a.groups > 1 ? 2 * a.top_k * a.groups / a.top_groups : a.top_k);
 #pragma unroll 1
       for (float d = fminf((hi - lo) * 0.0625f, 0x1p15f * one);; d *= 0.125f) {
@@ -514,8 +515,14 @@ __global__ __launch_bounds__(RT_THREADS) void k_route(const RouteArgs a) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const float s = a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z[i] * -1.44269502f)) : p[i] * over;
-      key[i] = (uint32_t)fmaxf(fmaf(s, by, fmaf(b[i] - lo, by, 2.0f)), 2.0f) << a.bits | (place - i);
+      b[i] = fmaf(s, by, fmaf(b[i] - lo, by, 2.0f));
     }
+    if (__builtin_amdgcn_ballot_w64(cut) != 0) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) b[i] = fmaxf(b[i], 2.0f);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) key[i] = (uint32_t)b[i] << a.bits | (place - i);
   } else if (fits) {
 #pragma unroll
     for (int i = 0; i < V; ++i) key[i] = (ordered(z[i] + 0.0f) & ~mask) | (place - i);
