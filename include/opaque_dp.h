@@ -745,7 +745,8 @@ int odp_rms_norm_grad(odp_stream_t stream, int dtype, int stream_dtype, int gain
  * best top_groups of the equal consecutive groups stay, by the sum of their two
  * best keys (best 0) or by their best (1); index [n][top_k] the best keys left,
  * best first, and weights [n][top_k] = scale p, over the sum of the chosen p with
- * renormalize.  Equal keys (in 64 bits) give the lower expert.  An expert whose
+ * renormalize.  Without a bias, and without sums of groups where not all are open,
+ * the logits are the keys.  Equal keys (in 64 bits) give the lower expert.  An expert whose
  * logit is -inf comes after all others and weighs 0; a NaN (in a softmax also
  * +inf) makes the row's weights (sigmoid: those it touches) NaN.  index always
  * holds top_k different experts.  n < 2^31; the reference's models bring their

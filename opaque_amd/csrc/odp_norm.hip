@@ -22,8 +22,9 @@
 //
 // Vectors of 16 bytes are loaded at any address (this target's global loads
 // need no more than the type's own alignment).  Rows of odd widths start at odd
-// addresses, where each vector spans two lines: 8192 x 8191 119 + 145 us.  Cutting
-// such rows at aligned addresses would have a row's sum depend on its place.
+// addresses, where each vector spans two lines: 8192 x 8191 118 + 145 us, 8192 x
+// 8192 93 + 88.  Aligned vectors shifted into place in registers would give every
+// thread the same values; that has not been tried.
 #include <cmath>
 
 #include "odp_internal.h"
@@ -643,8 +644,13 @@ void launch_grad(hipStream_t s, const NormGradArgs& a, int64_t blocks) {
   k_rms_norm_grad<XF, HF, T, NV><<<(uint32_t)blocks, norm_threads<T>(), 0, s>>>(a);
 }
 
-// The narrowest form whose registers hold a row.  (The gradient of rows above
-// 16384 values spills: 2048 x 32768 bfloat16 417 us, 1.3 TB/s.)
+// The narrowest form of at most 32 values a thread.  The gradient holds a row's
+// h, gy and gh, the gains and their sums beside: with 4 vectors a thread it takes
+// 205-241 registers, two waves a SIMD without the next row's loads (16384 x 2048
+// bfloat16 81 us, 3.3 TB/s, for 49 forward; 8192 x 8192 88 for 93).  1024 threads
+// have 128 registers each, so rows above 8192 values spill: 12 bytes a thread with
+// 16-bit streams (4096 x 16384 90 us), 132 with float32 ones (305 us, 3.5 TB/s), and
+// 296-428 above 16384 values (2048 x 32768 373 us, 1.4 TB/s).
 #define ODP_NORM_FORM(CALL)                                 \
   do {                                                      \
     const int64_t v = (a.width + 7) / 8;                    \

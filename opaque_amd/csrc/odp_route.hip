@@ -21,10 +21,11 @@
 // error of their float32 computation (`units_apart`); of such a token (one in a
 // thousand of 256 experts) the candidates' float64 keys are formed and ranked.  Keys are the
 // logits themselves where those order as the scores do (no bias, and no sums over
-// groups); those of 16-bit types always decide.
+// groups that shut some), also where scores run together in 64 bits; those of 16-bit
+// types always decide.
 //
-// 32768 tokens, 8 choices: of 64 experts 6 us, 256 15 us (33 MB of float32; a copy
-// of it takes 7), 256 with sigmoid scores and a bias 18, of 4 of 8 groups 23.
+// 32768 tokens, 8 choices: of 64 experts 7 us, 256 15 us (33 MB of float32; a copy
+// of it takes 7), 256 with sigmoid scores and a bias 20-21, of 4 of 8 groups 24-26.
 #include <cmath>
 
 #include "odp_internal.h"
@@ -936,7 +937,7 @@ RouteArgs route_args(int dt, const void* z, int64_t ldz, int64_t n, int64_t expe
   a.groups = a.top_groups = 1;
   a.size = a.experts;
   a.per_size = 1.0f / (float)a.size;
-  a.bits = 8;  // words of 24 bits and more hold float32's error
+  a.bits = 8;  // leaves a leading part of 24 bits; of 23 above 256 experts, of 22 above 512
   while (1 << a.bits < a.experts) ++a.bits;
   return a;
 }

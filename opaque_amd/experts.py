@@ -132,7 +132,9 @@ def route(logits: torch.Tensor, top_k: int, *, scores: str = "softmax", bias: to
     (equal runs of experts, up to 64) only those of the ``top_groups`` best
     groups are open, by the sum of a group's two best or its best
     (``group_best`` "top2", "max").  Keys are compared as in 64 bits; equal ones
-    go to the lower expert or group.  The weights are ``scale`` times the chosen scores,
+    go to the lower expert or group.  Without a bias, and without sums of groups
+    where some stay shut, the logits themselves are compared, which order as the
+    scores do and further apart.  The weights are ``scale`` times the chosen scores,
     over their sum with ``renormalize``; their gradient reaches the logits.
 
     An expert whose logit is -inf is masked: chosen after all others, with
