@@ -249,7 +249,7 @@ def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor | None = None, *, r
     nearest-even from float32.  ``scales`` float32 [...], the largest magnitude
     of the row over 448, or with ``block=128`` [..., ceil(width / 128)], that of
     every 128 columns; at least the least normal float32, so a row of zeros has
-    a finite one.  A row (or block) that holds a NaN is NaN.  Not
+    a finite one (where ``eps`` is above 0).  A row (or block) that holds a NaN is NaN.  Not
     differentiable: no input may require a gradient, unless gradients are off, or
     have a forward-mode tangent.
     """
