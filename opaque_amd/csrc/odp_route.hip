@@ -41,7 +41,7 @@ constexpr int RT_THREADS = 256;
 constexpr int RT_GROUPS = 64;  // groups, at most (a mask of 64 bits)
 // Spread of the biases, in largest scores, from which on low ones are cut: 32768 x 256
 // by sigmoids with one at -100 take 23 us so and 27 in groups, uncut 28 and 40.  Below it
-// the keys keep 19 bits and more of the scores, and the search for the cut is not paid.
+// the scores keep 19 of a word's 24 bits, and the search for the cut is not paid.
 constexpr float ROUTE_DEEP = 32.0f;
 
 // e^x: 2^t from the hardware, t = x log2(e) rounded, and what the rounding took
